@@ -145,6 +145,14 @@ SIGNATURES = {
     "gncx_hip_decode_step": (C.c_int, [_vp, _vp, _i32, _i32, _i32]),
     "gncx_hip_decode_step_noalloc": (C.c_int, [_vp, _vp, _i32, _i32, _i32]),
     "gncx_hip_argmax": (None, [_fp, _i32, _vp]),
+    "gncx_hip_attention_tree": (
+        None,
+        [_fp, _fp, _fp, _fp, _fp, _i32, _i32, _vp, _i32, _i32, _i32, _f32, _i32, _vp, _sz, _sz, _i32, _f32, _sz, _i32,
+         _f32, _fp],
+    ),
+    "gncx_hip_kv_keep_rows": (None, [_vp, _vp, _i32, _i32, _i32, _vp, _i32]),
+    "gncx_hip_beam_select": (None, [_fp, _i32, _i32, _fp, _vp, _i32, _i32, _vp, _vp, _fp]),
+    "gncx_hip_kv_reorder": (None, [_vp, _vp, _i32, _i32, _sz, _i32, _i32, _i32, _vp]),
     "gncx_hip_set_host_coherence": (C.c_int, [C.c_int]),
     "gncx_hip_host_flush": (None, [_vp]),
 }

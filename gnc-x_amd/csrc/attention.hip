@@ -1515,4 +1515,217 @@ hipError_t launch_attention(const AttnArgs& a, void* workspace, size_t workspace
     }
 }
 
+// ---------------------------------------------------------------------------
+// Attention for a tree of drafted tokens over the KV cache.
+//
+// Several continuations of one sequence, drafted as a tree (speculative
+// decoding), are verified in one pass: node i of the tree stands at position
+// pos0 + depth(i), and sees the cached rows before pos0 (within its sliding
+// window), its ancestors and itself:
+//   s_j = scale q_i . k_j,  out_i = sum_j e^(s_j - m) v_j / (sum_j e^(s_j - m) + 1e-12)
+// with the decode step's prologue (per-head RMSNorm, NEOX RoPE at the node's
+// position) on q and k, and the node's K/V row stored at cache row pos0 + i.
+//
+// The tree's mask is an interval test.  With the nodes numbered in preorder,
+// the subtree of a is the interval [pre_a, end_a), so a is i or an ancestor of
+// i exactly when pre_a <= pre_i < end_a: two compares instead of a T x T mask,
+// and 6 bytes a node, which travel in the kernel arguments.
+namespace {
+
+struct TreeParams {
+    float* q;
+    float* k;
+    const float* v;
+    float* k_cache;
+    float* v_cache;
+    float* out;
+    const float* q_gamma;
+    const float* k_gamma;
+    const float* rope;  // [max depth + 1][HD]: cos then sin, or null
+    int32_t pos0, n, n_heads, n_kv, sw, norm_qk;
+    float scale, eps;
+    TreeTable tree;
+};
+
+// The decode step's prologue of every node's heads, a wave per head: the
+// per-head RMSNorm, then RoPE with the row of the node's depth; KV heads also
+// store their cache rows.  The arithmetic is prologue_head_r's of the decode
+// step (head_inv_rms, no contraction), so an accepted node's cache row is the
+// one that decoding its token would have stored.
+template <int HD>
+__global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p) {
+#pragma clang fp contract(off)
+    constexpr int H = HD / 2, NR = (H + 63) / 64;
+    __shared__ __align__(16) float xs[kWaves][HD];
+    const int t = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int head = static_cast<int>(blockIdx.y) * kWaves + wv;
+    if (head >= p.n_heads + p.n_kv) return;  // whole waves; no barrier below
+    const bool is_q = head < p.n_heads;
+    const size_t kn = static_cast<size_t>(p.n_kv) * HD;
+    const size_t at = static_cast<size_t>(is_q ? 0 : head - p.n_heads) * HD;
+    float* src = is_q ? p.q + (static_cast<size_t>(t) * p.n_heads + head) * HD : p.k + t * kn + at;
+    const float* gamma = is_q ? p.q_gamma : p.k_gamma;
+    float* x = xs[wv];
+    for (int i = lane; i < HD; i += 64) x[i] = src[i];
+    const float inv = p.norm_qk ? head_inv_rms(x, HD, p.eps, lane) : 1.0f;
+    const float* rc = p.rope ? p.rope + static_cast<size_t>(p.tree.depth[t]) * HD : nullptr;
+    const size_t row = (static_cast<size_t>(p.pos0) + t) * kn + at;
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        const int i = lane + 64 * r;
+        if (i < H) {
+            float a = x[i], b = x[i + H];
+            if (p.norm_qk) {
+                a = a * inv;
+                b = b * inv;
+                if (gamma) {
+                    a = a * gamma[i];
+                    b = b * gamma[i + H];
+                }
+            }
+            if (rc) {
+                const float c = rc[i], s = rc[i + H], u = a, w = b;
+                a = u * c - w * s;
+                b = w * c + u * s;
+            }
+            if (p.norm_qk || rc) {
+                src[i] = a;
+                src[i + H] = b;
+            }
+            if (!is_q) {
+                const float* vr = p.v + t * kn + at;
+                p.k_cache[row + i] = a;
+                p.k_cache[row + i + H] = b;
+                p.v_cache[row + i] = vr[i];
+                p.v_cache[row + i + H] = vr[i + H];
+            }
+        }
+    }
+}
+
+// One work-group per (head, node): a wave takes every fourth visible key, its
+// lanes the dims of the dot and of the sum, with a running maximum and sum;
+// the waves' results meet in LDS.
+template <int HD>
+__global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeParams p) {
+    constexpr int E = HD / 64;
+    __shared__ float os[kWaves][HD];
+    __shared__ float ms[kWaves], ls[kWaves];
+    const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    const int hk = h / (p.n_heads / p.n_kv);
+    const size_t kn = static_cast<size_t>(p.n_kv) * HD;
+    float q[E], o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        q[e] = p.q[(static_cast<size_t>(t) * p.n_heads + h) * HD + 64 * e + lane];
+        o[e] = 0.0f;
+    }
+    float m = -1e30f, l = 0.0f;
+    auto visit = [&](int row) {
+        const size_t at = static_cast<size_t>(row) * kn + static_cast<size_t>(hk) * HD + lane;
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s += q[e] * p.k_cache[at + 64 * e];
+        s = wave_sum(s) * p.scale;
+        const float m2 = fmaxf(m, s), a = expf(m - m2), w = expf(s - m2);
+        l = l * a + w;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * p.v_cache[at + 64 * e];
+        m = m2;
+    };
+    const int here = p.pos0 + p.tree.depth[t], pre = p.tree.pre[t];
+    const int lo = p.sw > 0 ? max(0, here - p.sw + 1) : 0;
+    for (int j = lo + wv; j < p.pos0; j += kWaves) visit(j);
+    for (int a = wv; a <= t; a += kWaves)
+        if (p.tree.pre[a] <= pre && pre < p.tree.end[a] && p.pos0 + p.tree.depth[a] >= lo) visit(p.pos0 + a);
+#pragma unroll
+    for (int e = 0; e < E; ++e) os[wv][64 * e + lane] = o[e];
+    if (lane == 0) {
+        ms[wv] = m;
+        ls[wv] = l;
+    }
+    __syncthreads();
+    float M = ms[0];
+    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, ms[w]);
+    for (int d = threadIdx.x; d < HD; d += kThreads) {
+        float sum = 0.0f, acc = 0.0f;
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = expf(ms[w] - M);
+            sum += ls[w] * f;
+            acc += os[w][d] * f;
+        }
+        p.out[(static_cast<size_t>(t) * p.n_heads + h) * HD + d] = acc / (sum + 1e-12f);
+    }
+}
+
+template <int HD>
+hipError_t launch_tree_hd(const TreeParams& p, hipStream_t stream) {
+    const int heads = p.n_heads + p.n_kv;
+    hipLaunchKernelGGL(tree_prologue_kernel<HD>, dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(tree_attention_kernel<HD>, dim3(p.n_heads, p.n), dim3(kThreads), 0, stream, p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+bool make_tree_table(const int32_t* parents, int32_t n, TreeTable& t) {
+    if (n < 1 || n > kMaxTreeNodes) return false;
+    int32_t size[kMaxTreeNodes], next[kMaxTreeNodes];  // subtree sizes; the next child's preorder number
+    for (int32_t i = 0; i < n; ++i) {
+        if (parents[i] < -1 || parents[i] >= i) return false;
+        size[i] = 1;
+    }
+    // a node's number is above its parent's: sizes from the last node up,
+    // preorder numbers from the first node down
+    for (int32_t i = n - 1; i >= 0; --i)
+        if (parents[i] >= 0) size[parents[i]] += size[i];
+    int32_t root = 0;
+    t.max_depth = 0;
+    for (int32_t i = 0; i < n; ++i) {
+        const int32_t a = parents[i];
+        int32_t& at = a >= 0 ? next[a] : root;
+        const int32_t depth = a >= 0 ? t.depth[a] + 1 : 0;
+        t.pre[i] = static_cast<uint16_t>(at);
+        t.end[i] = static_cast<uint16_t>(at + size[i]);
+        t.depth[i] = static_cast<uint16_t>(depth);
+        t.max_depth = depth > t.max_depth ? depth : t.max_depth;
+        next[i] = at + 1;
+        at += size[i];
+    }
+    return true;
+}
+
+hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, hipStream_t stream) {
+    if (a.n < 1 || a.n > kMaxTreeNodes || a.pos0 < 0 || a.n_heads < 1 || a.n_kv_heads < 1 ||
+        a.n_heads % a.n_kv_heads != 0)
+        return hipErrorInvalidValue;
+    TreeParams p{};
+    p.q = a.q;
+    p.k = a.k;
+    p.v = a.v;
+    p.k_cache = a.k_cache;
+    p.v_cache = a.v_cache;
+    p.out = a.out;
+    p.q_gamma = a.q_gamma;
+    p.k_gamma = a.k_gamma;
+    p.rope = a.rope;
+    p.pos0 = a.pos0;
+    p.n = a.n;
+    p.n_heads = a.n_heads;
+    p.n_kv = a.n_kv_heads;
+    p.sw = a.sliding_window;
+    p.norm_qk = a.norm_qk;
+    p.scale = a.scale;
+    p.eps = a.eps;
+    p.tree = tree;
+    switch (a.head_dim) {
+    case 64: return launch_tree_hd<64>(p, stream);
+    case 128: return launch_tree_hd<128>(p, stream);
+    case 256: return launch_tree_hd<256>(p, stream);
+    default: return hipErrorInvalidValue;
+    }
+}
+
 }  // namespace gncx

@@ -677,4 +677,328 @@ hipError_t launch_argmax(const float* x, int32_t n, int32_t* out, int32_t* log, 
     return hipGetLastError();
 }
 
+// ---------------------------------------------------------------------------
+// Choosing between continuations of one sequence and rearranging the KV caches
+// after the choice: the rows of an accepted draft path, beam search's
+// selection over beams and vocabulary, and the reordering of the beams' caches.
+namespace {
+
+constexpr int kCandThreads = 256;
+constexpr int kLayerGroup = 64;  // layers of a launch: their cache addresses travel in the kernel arguments
+
+struct LayerCaches {
+    float* c[2 * kLayerGroup];  // layer l: its k cache at 2 l, its v cache at 2 l + 1
+};
+
+// ---- rows of an accepted path ----------------------------------------------
+// Row row0 + i of every cache becomes the old row row0 + rows[i], rows
+// ascending.  A thread owns one float4 column of one cache and moves its rows
+// in order: as rows[i] >= i, no row is overwritten before it is read, and no
+// thread touches another's column, so the move is in place without a barrier.
+struct KeepParams {
+    LayerCaches caches;
+    int32_t kv_dim, n;
+    size_t row0;
+    uint16_t rows[kMaxKeepRows];
+};
+
+__global__ __launch_bounds__(kCandThreads) void keep_rows_kernel(KeepParams p) {
+    const int d4 = static_cast<int>(blockIdx.x * kCandThreads + threadIdx.x);
+    if (4 * d4 >= p.kv_dim) return;
+    float* c = p.caches.c[blockIdx.y] + p.row0 * p.kv_dim + 4 * d4;
+    for (int i = 0; i < p.n; ++i) {
+        const int r = p.rows[i];
+        if (r != i)
+            *reinterpret_cast<float4*>(c + static_cast<size_t>(i) * p.kv_dim) =
+                *reinterpret_cast<const float4*>(c + static_cast<size_t>(r) * p.kv_dim);
+    }
+}
+
+// ---- reordering of beams ------------------------------------------------------
+// Rows [row0, row0 + n_rows) of beam b become those of beam parents[b].  A
+// thread owns one float4 of one row in all beams: it loads every moving beam's
+// new value before it stores any, so the exchange is in place with no second
+// copy of the caches.  A parent outside [0, n_beams) leaves its beam as it is.
+struct ReorderParams {
+    LayerCaches caches;
+    size_t beam_stride, count;  // floats; float4 of a beam's rows
+    size_t start;               // floats of the rows before row0
+    int32_t n_beams;
+    const int32_t* parents;
+};
+
+template <int NB>
+__global__ __launch_bounds__(kCandThreads) void reorder_kernel(ReorderParams p) {
+    const size_t i = static_cast<size_t>(blockIdx.x) * kCandThreads + threadIdx.x;
+    if (i >= p.count) return;
+    float* c = p.caches.c[blockIdx.y] + p.start + 4 * i;
+    float4 v[NB];
+    bool moves[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        const int from = b < p.n_beams ? p.parents[b] : b;
+        moves[b] = from != b && from >= 0 && from < p.n_beams;
+        if (moves[b]) v[b] = *reinterpret_cast<const float4*>(c + static_cast<size_t>(from) * p.beam_stride);
+    }
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+        if (moves[b]) *reinterpret_cast<float4*>(c + static_cast<size_t>(b) * p.beam_stride) = v[b];
+}
+
+// ---- beam search's selection ------------------------------------------------------
+// score(b, v) = scores[b] + logits[b][v] - log sum_u e^logits[b][u]; the n_out
+// best, ties to the lowest b vocab + v.  Within a beam the order is the
+// logits', so one pass over them leaves, per (beam, part of the vocabulary),
+// the part's maximum, its sum of exponentials and its n_out best; a second
+// kernel joins the parts in double, where candidates of different beams meet.
+struct SelectParams {
+    const float* logits;
+    const float* scores;
+    const int32_t* finished;
+    int32_t finished_token, n_beams, vocab, n_out, chunk, n_chunks;
+    float2* ml;   // [beam][chunk] maximum, sum of e^(x - maximum)
+    float2* best;  // [beam][chunk][n_out] logit, word (as bits); -inf behind the last
+    int32_t* out_parents;
+    int32_t* out_tokens;
+    float* out_scores;
+};
+
+// Larger for the better candidate: the logit's bits in an order-preserving
+// form (NaN and -0 as -inf and +0), then the lower word.
+__device__ __forceinline__ float clean(float x) { return x != x ? -__builtin_inff() : x + 0.0f; }
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t word) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const uint32_t ordered = u & 0x80000000u ? ~u : u | 0x80000000u;
+    return static_cast<uint64_t>(ordered) << 32 | ~word;
+}
+__device__ __forceinline__ float logit_of(uint64_t key) {
+    const uint32_t o = static_cast<uint32_t>(key >> 32);
+    return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+#pragma unroll
+    for (int s = 32; s; s >>= 1) {
+        const uint64_t o = __shfl_xor(v, s, 64);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+__global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams p) {
+    __shared__ float red[kCandThreads / 64];
+    __shared__ uint64_t redk[kCandThreads / 64];
+    const int b = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    if (p.finished && p.finished[b]) return;
+    const int v0 = c * p.chunk, v1 = min(p.vocab, v0 + p.chunk);
+    const float* row = p.logits + static_cast<size_t>(b) * p.vocab;
+    float m = -__builtin_inff();
+    for (int v = v0 + tid; v < v1; v += kCandThreads) m = fmaxf(m, clean(row[v]));
+    m = wave_max(m);
+    if (lane == 0) red[wv] = m;
+    __syncthreads();
+    m = red[0];
+    for (int w = 1; w < kCandThreads / 64; ++w) m = fmaxf(m, red[w]);
+    float l = 0.0f;
+    for (int v = v0 + tid; v < v1; v += kCandThreads) {
+        const float x = clean(row[v]);
+        l += x == m ? 1.0f : expf(x - m);  // (x == m: an infinite maximum)
+    }
+    l = wave_sum(l);
+    __syncthreads();
+    if (lane == 0) red[wv] = l;
+    __syncthreads();
+    const size_t at = static_cast<size_t>(b) * p.n_chunks + c;
+    if (tid == 0) {
+        l = 0.0f;
+        for (int w = 0; w < kCandThreads / 64; ++w) l += red[w];
+        p.ml[at] = make_float2(m, l);
+    }
+    uint64_t last = ~uint64_t{0};
+    for (int i = 0; i < p.n_out; ++i) {
+        uint64_t k = 0;
+        for (int v = v0 + tid; v < v1; v += kCandThreads) {
+            const uint64_t kv = key_of(clean(row[v]), static_cast<uint32_t>(v));
+            if (kv < last && kv > k) k = kv;
+        }
+        k = wave_max_u64(k);
+        __syncthreads();
+        if (lane == 0) redk[wv] = k;
+        __syncthreads();
+        k = redk[0];
+        for (int w = 1; w < kCandThreads / 64; ++w) k = redk[w] > k ? redk[w] : k;
+        if (tid == 0)
+            p.best[at * p.n_out + i] = k ? make_float2(logit_of(k), __builtin_bit_cast(float, ~static_cast<uint32_t>(k)))
+                                         : make_float2(-__builtin_inff(), 0.0f);
+        last = k;
+    }
+}
+
+struct Candidate {
+    double score;
+    int64_t at;  // beam vocab + word
+    __device__ bool before(const Candidate& o) const { return score > o.score || (score == o.score && at < o.at); }
+};
+
+__global__ __launch_bounds__(kCandThreads) void select_join_kernel(SelectParams p) {
+    __shared__ double base[kMaxBeams];  // scores[b] - log sum: -inf for a beam with nothing left
+    __shared__ float top[kMaxBeams];
+    __shared__ bool ended[kMaxBeams];  // (finished may be one of the outputs)
+    __shared__ double reds[kCandThreads / 64];
+    __shared__ int64_t reda[kCandThreads / 64];
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const double inf = __builtin_inf();
+    if (tid < p.n_beams) {
+        const float s = clean(p.scores[tid]);
+        const bool done = p.finished && p.finished[tid];
+        float m = -__builtin_inff();
+        double sum = 0.0;
+        if (!done) {
+            for (int c = 0; c < p.n_chunks; ++c) m = fmaxf(m, p.ml[static_cast<size_t>(tid) * p.n_chunks + c].x);
+            for (int c = 0; c < p.n_chunks; ++c) {
+                const float2 v = p.ml[static_cast<size_t>(tid) * p.n_chunks + c];
+                if (v.x > -__builtin_inff())
+                    sum += static_cast<double>(v.y) *
+                           (v.x == m ? 1.0 : exp(static_cast<double>(v.x) - static_cast<double>(m)));
+            }
+        }
+        top[tid] = m;
+        ended[tid] = done;
+        base[tid] = done ? s : m > -__builtin_inff() ? static_cast<double>(s) - log(sum) : -inf;
+    }
+    __syncthreads();
+    const int per = p.n_chunks * p.n_out, total = p.n_beams * per;
+    Candidate last{inf, -1};
+    for (int i = 0; i < p.n_out; ++i) {
+        Candidate mine{-inf, INT64_MAX};
+        for (int j = tid; j < total; j += kCandThreads) {
+            const int b = j / per;
+            Candidate c{-inf, INT64_MAX};
+            if (ended[b]) {
+                if (j % per == 0) c = {base[b], static_cast<int64_t>(b) * p.vocab + p.finished_token};
+            } else {
+                const float2 e = p.best[j];
+                if (e.x > -__builtin_inff())
+                    c = {base[b] + (e.x == top[b] ? 0.0 : static_cast<double>(e.x) - static_cast<double>(top[b])),
+                         static_cast<int64_t>(b) * p.vocab + __builtin_bit_cast(int32_t, e.y)};
+            }
+            if (c.score > -inf && last.before(c) && c.before(mine)) mine = c;
+        }
+#pragma unroll
+        for (int s = 32; s; s >>= 1) {
+            const Candidate o{__shfl_xor(mine.score, s, 64), __shfl_xor(mine.at, s, 64)};
+            if (o.before(mine)) mine = o;
+        }
+        __syncthreads();
+        if (lane == 0) {
+            reds[wv] = mine.score;
+            reda[wv] = mine.at;
+        }
+        __syncthreads();
+        last = {reds[0], reda[0]};
+        for (int w = 1; w < kCandThreads / 64; ++w) {
+            const Candidate o{reds[w], reda[w]};
+            if (o.before(last)) last = o;
+        }
+        if (tid == 0) {
+            const bool some = last.score > -inf;
+            p.out_parents[i] = some ? static_cast<int32_t>(last.at / p.vocab) : -1;
+            p.out_tokens[i] = some ? static_cast<int32_t>(last.at % p.vocab) : -1;
+            p.out_scores[i] = some ? static_cast<float>(last.score) : -__builtin_inff();
+        }
+    }
+}
+
+int32_t select_chunk(int32_t vocab) { return vocab < 4096 ? vocab : 4096; }
+
+template <class F>
+hipError_t by_layers(float* const* k, float* const* v, int32_t n_layers, F&& launch) {
+    for (int32_t l0 = 0; l0 < n_layers; l0 += kLayerGroup) {
+        const int32_t n = n_layers - l0 < kLayerGroup ? n_layers - l0 : kLayerGroup;
+        LayerCaches c{};
+        for (int32_t l = 0; l < n; ++l) {
+            c.c[2 * l] = k[l0 + l];
+            c.c[2 * l + 1] = v[l0 + l];
+        }
+        launch(c, 2 * n);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+hipError_t launch_kv_keep_rows(float* const* k, float* const* v, int32_t n_layers, int32_t kv_dim, int32_t row0,
+                               const int32_t* rows, int32_t n, hipStream_t stream) {
+    if (n < 0 || n > kMaxKeepRows || kv_dim < 4 || kv_dim % 4 || row0 < 0) return hipErrorInvalidValue;
+    KeepParams p{};
+    p.kv_dim = kv_dim;
+    p.n = n;
+    p.row0 = static_cast<size_t>(row0);
+    for (int32_t i = 0; i < n; ++i) p.rows[i] = static_cast<uint16_t>(rows[i]);
+    return by_layers(k, v, n_layers, [&](const LayerCaches& c, int32_t caches) {
+        p.caches = c;
+        hipLaunchKernelGGL(keep_rows_kernel, dim3((kv_dim / 4 + kCandThreads - 1) / kCandThreads, caches), dim3(kCandThreads), 0,
+                           stream, p);
+    });
+}
+
+hipError_t launch_kv_reorder(float* const* k, float* const* v, int32_t n_layers, int32_t n_beams, size_t beam_stride,
+                             int32_t kv_dim, int32_t row0, int32_t n_rows, const int32_t* parents,
+                             hipStream_t stream) {
+    if (n_beams < 1 || n_beams > kMaxBeams || kv_dim < 4 || kv_dim % 4 || beam_stride % 4 || row0 < 0 || n_rows < 0)
+        return hipErrorInvalidValue;
+    ReorderParams p{};
+    p.beam_stride = beam_stride;
+    p.count = static_cast<size_t>(n_rows) * kv_dim / 4;
+    p.start = static_cast<size_t>(row0) * kv_dim;
+    p.n_beams = n_beams;
+    p.parents = parents;
+    const size_t groups = (p.count + kCandThreads - 1) / kCandThreads;
+    if (groups > 0x7fffffffu) return hipErrorInvalidValue;
+    return by_layers(k, v, n_layers, [&](const LayerCaches& c, int32_t caches) {
+        p.caches = c;
+        const dim3 grid(static_cast<uint32_t>(groups), caches);
+        if (n_beams <= 4) hipLaunchKernelGGL(reorder_kernel<4>, grid, dim3(kCandThreads), 0, stream, p);
+        else if (n_beams <= 8) hipLaunchKernelGGL(reorder_kernel<8>, grid, dim3(kCandThreads), 0, stream, p);
+        else if (n_beams <= 16) hipLaunchKernelGGL(reorder_kernel<16>, grid, dim3(kCandThreads), 0, stream, p);
+        else hipLaunchKernelGGL(reorder_kernel<32>, grid, dim3(kCandThreads), 0, stream, p);
+    });
+}
+
+size_t beam_select_workspace_bytes(int32_t n_beams, int32_t vocab, int32_t n_out) {
+    const size_t chunk = select_chunk(vocab), parts = static_cast<size_t>(n_beams) * ((vocab + chunk - 1) / chunk);
+    return parts * sizeof(float2) * (1 + static_cast<size_t>(n_out));
+}
+
+hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,
+                              const int32_t* finished, int32_t finished_token, int32_t n_out, int32_t* out_parents,
+                              int32_t* out_tokens, float* out_scores, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream) {
+    if (n_beams < 1 || n_beams > kMaxBeams || vocab < 1 || vocab > kMaxBeamVocab || n_out < 1 || n_out > kMaxBeamOut ||
+        workspace_bytes < beam_select_workspace_bytes(n_beams, vocab, n_out))
+        return hipErrorInvalidValue;
+    SelectParams p{};
+    p.logits = logits;
+    p.scores = scores;
+    p.finished = finished;
+    p.finished_token = finished_token;
+    p.n_beams = n_beams;
+    p.vocab = vocab;
+    p.n_out = n_out;
+    p.chunk = select_chunk(vocab);
+    p.n_chunks = (vocab + p.chunk - 1) / p.chunk;
+    p.ml = static_cast<float2*>(workspace);
+    p.best = p.ml + static_cast<size_t>(n_beams) * p.n_chunks;
+    p.out_parents = out_parents;
+    p.out_tokens = out_tokens;
+    p.out_scores = out_scores;
+    hipLaunchKernelGGL(select_parts_kernel, dim3(p.n_chunks, n_beams), dim3(kCandThreads), 0, stream, p);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(select_join_kernel, dim3(1), dim3(kCandThreads), 0, stream, p);
+    return hipGetLastError();
+}
+
 }  // namespace gncx

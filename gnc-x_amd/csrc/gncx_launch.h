@@ -157,6 +157,58 @@ hipError_t launch_attention_prefill(const PrefillArgs& a, hipStream_t stream);
 hipError_t launch_attention(const AttnArgs& a, void* workspace, size_t workspace_bytes,
                             hipStream_t stream);
 
+// Attention of a tree of n drafted tokens over the cache: node i at position
+// pos0 + depth[i], with the decode step's prologue (q and k in place) and its
+// K/V row stored at cache row pos0 + i, sees the cached rows of its window,
+// its ancestors and itself.
+constexpr int32_t kMaxTreeNodes = 512;
+struct TreeTable {
+    uint16_t pre[kMaxTreeNodes], end[kMaxTreeNodes];  // preorder interval of the node's subtree
+    uint16_t depth[kMaxTreeNodes];                    // 0 for a root
+    int32_t max_depth;
+};
+// host: false unless 1 <= n <= kMaxTreeNodes and every parent is -1 or an
+// earlier node
+bool make_tree_table(const int32_t* parents, int32_t n, TreeTable& t);
+struct TreeArgs {
+    float* q;        // [n][n_heads * head_dim]
+    float* k;        // [n][n_kv_heads * head_dim]
+    const float* v;  // [n][n_kv_heads * head_dim]
+    float* k_cache;  // rows [0, pos0) already filled
+    float* v_cache;
+    float* out;      // [n][n_heads * head_dim]
+    int32_t pos0, n, n_heads, n_kv_heads, head_dim;
+    float scale;
+    int32_t sliding_window;
+    int32_t norm_qk;
+    const float* q_gamma;
+    const float* k_gamma;
+    float eps;
+    const float* rope;  // device [max_depth + 1][head_dim]: cos[head_dim / 2] then sin, or null
+};
+hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, hipStream_t stream);
+
+// Rows of every layer's caches: row0 + i <- row0 + rows[i] for i < n, rows
+// (host) strictly ascending and below kMaxKeepOffset.
+constexpr int32_t kMaxKeepRows = 512;
+constexpr int32_t kMaxKeepOffset = 65536;
+hipError_t launch_kv_keep_rows(float* const* k, float* const* v, int32_t n_layers, int32_t kv_dim, int32_t row0,
+                               const int32_t* rows, int32_t n, hipStream_t stream);
+// Rows [row0, row0 + n_rows) of beam b's caches (beam_stride floats apart) <-
+// those of beam parents[b] (device), for every layer; in place.
+constexpr int32_t kMaxBeams = 32;
+hipError_t launch_kv_reorder(float* const* k, float* const* v, int32_t n_layers, int32_t n_beams, size_t beam_stride,
+                             int32_t kv_dim, int32_t row0, int32_t n_rows, const int32_t* parents, hipStream_t stream);
+// The n_out best of scores[b] + log softmax(logits[b])[v] over beams and
+// vocabulary, all device pointers; finished may be null.
+constexpr int32_t kMaxBeamOut = 64;
+constexpr int32_t kMaxBeamVocab = 1 << 22;
+size_t beam_select_workspace_bytes(int32_t n_beams, int32_t vocab, int32_t n_out);
+hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,
+                              const int32_t* finished, int32_t finished_token, int32_t n_out, int32_t* out_parents,
+                              int32_t* out_tokens, float* out_scores, void* workspace, size_t workspace_bytes,
+                              hipStream_t stream);
+
 // Per-head RMSNorm in place (reference cpp:895-953); gamma may be null.
 hipError_t launch_rmsnorm_heads(float* v, const float* gamma, int32_t n_heads, int32_t head_dim,
                                 float eps, hipStream_t stream);

@@ -2910,6 +2910,309 @@ GNCX_API void gncx_hip_argmax(const float* values, int32_t n, int32_t* out_index
     check(launch_argmax(values, n, out_index, nullptr, g_rt.aux.p, g_rt.aux.cap, g_rt.stream), where);
 }
 
+// ---- several continuations of one sequence --------------------------------
+// Tree attention, kept rows, beam selection and reordering: device pointers
+// only, like the other entries of callers whose state lives in HBM.
+
+namespace {
+
+// The library's GPU made current for a call, the caller's restored after it:
+// its streams and buffers belong to that GPU.
+struct DeviceGuard {
+    int before = -1;
+    bool ok = true;
+    explicit DeviceGuard(const char* where) {
+        int now = 0;
+        ok = check(hipGetDevice(&now), where);
+        if (!ok || now == g_rt.device) return;
+        before = now;
+        ok = check(hipSetDevice(g_rt.device), where);
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// p is memory of the library's GPU, 4-byte (or `align`-byte) aligned
+bool on_device(const void* p, const char* name, const char* where, uintptr_t align = 4) {
+    hipPointerAttribute_t a;
+    const hipError_t e = p ? hipPointerGetAttributes(&a, p) : hipErrorInvalidValue;
+    if (e != hipSuccess) (void)hipGetLastError();
+    if (e != hipSuccess || !(a.type == hipMemoryTypeManaged ||
+                             (a.type == hipMemoryTypeDevice && a.device == g_rt.device))) {
+        set_error(where, (std::string(name) + " must be memory of the library's GPU").c_str(), -1);
+        return false;
+    }
+    if (reinterpret_cast<uintptr_t>(p) % align) {
+        set_error(where, (std::string(name) + " must be " + std::to_string(align) + "-byte aligned").c_str(), -1);
+        return false;
+    }
+    return true;
+}
+
+// p is ordinary host memory, which the call reads before it returns
+bool on_host(const void* p, const char* name, const char* where) {
+    if (p && !is_device_ptr(p)) return true;
+    set_error(where, (std::string(name) + " must be host memory").c_str(), -1);
+    return false;
+}
+
+bool capturing() {
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (!g_rt.stream || hipStreamIsCapturing(g_rt.stream, &st) != hipSuccess) {
+        (void)hipGetLastError();
+        return false;
+    }
+    return st != hipStreamCaptureStatusNone;
+}
+
+// A workspace that calls on one stream share in stream order.  A call on
+// another stream than the last one's waits for the device first.  A graph
+// captured with the workspace keeps its address: from then on it is never
+// freed (a larger one is allocated beside it), and a capture that would need
+// a larger one is refused, as nothing can be allocated there.
+struct SharedWorkspace {
+    DevBuf buf;
+    hipStream_t last = nullptr;
+    bool used = false, in_graph = false;
+    void* take(size_t bytes, const char* where) {
+        if (capturing()) {
+            if (bytes > buf.cap) {
+                set_error(where, "the workspace must grow, which a stream capture does not allow: make the call once "
+                                 "before the capture", -1);
+                return nullptr;
+            }
+            in_graph = true;
+            return buf.p;
+        }
+        if (used && last != g_rt.stream && !check(hipDeviceSynchronize(), where)) return nullptr;
+        if (in_graph && bytes > buf.cap) {
+            buf = DevBuf{};  // the captured graphs keep the old one
+            in_graph = false;
+        }
+        if (!buf.ensure(bytes, where)) return nullptr;
+        used = true;
+        last = g_rt.stream;
+        return buf.p;
+    }
+};
+SharedWorkspace g_select_ws;
+
+// Every cache is memory of the library's GPU, holds `floats` floats, and no two
+// share a touched float: cache c's are [lo, floats) + beam * stride for beams
+// below n_beams.  The pointer query (0.2 us) is made once per allocation.
+bool layer_caches(float* const* k, float* const* v, int32_t n_layers, size_t lo, size_t floats, int32_t n_beams,
+                  size_t stride, const char* where) {
+    if (!k || !v || n_layers < 1) {
+        set_error(where, "k_caches and v_caches must name at least one layer", -1);
+        return false;
+    }
+    const size_t span = sizeof(float) * (stride * (n_beams - 1) + floats);
+    const size_t step = sizeof(float) * stride, own = sizeof(float) * (floats - lo);
+    static std::vector<std::pair<uintptr_t, uintptr_t>> at;  // (place within a stride, address); the call lock is held
+    at.clear();
+    uintptr_t base = 0, end = 0;  // the last pointer's allocation
+    for (int32_t i = 0; i < 2 * n_layers; ++i) {
+        const float* p = i % 2 ? v[i / 2] : k[i / 2];
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+        if (a < base || a >= end || a % 16) {
+            if (!on_device(p, i % 2 ? "every v cache" : "every k cache", where, 16)) return false;
+            hipDeviceptr_t b = nullptr;
+            size_t n = 0;
+            if (hipMemGetAddressRange(&b, &n, const_cast<float*>(p)) != hipSuccess) {
+                (void)hipGetLastError();
+                n = 0;
+            }
+            base = reinterpret_cast<uintptr_t>(b);
+            end = base + n;
+        }
+        if (a >= base && a < end && span > end - a) {
+            set_error(where, "the rows lie past the end of a cache's memory", -1);
+            return false;
+        }
+        at.emplace_back(n_beams > 1 ? a % step : a, a);
+    }
+    // two caches can meet only where their places within a stride are less
+    // than `own` apart (around its end, too)
+    std::sort(at.begin(), at.end());
+    const size_t n = at.size();
+    for (size_t i = 0; i < n; ++i)
+        for (size_t j = i + 1; j < (n_beams > 1 ? i + n : n); ++j) {
+            const auto &x = at[i], &y = at[j % n];
+            const uintptr_t apart = j < n ? y.first - x.first : y.first + step - x.first;
+            if (apart >= own) break;
+            const uintptr_t l = std::min(x.second, y.second), h = std::max(x.second, y.second);
+            // beams h sits behind l, at least and at most
+            const size_t b0 = n_beams > 1 ? (h - l) / step : 0, rest = h - l - b0 * (n_beams > 1 ? step : 0);
+            const size_t beams = static_cast<size_t>(n_beams);
+            if ((rest < own && b0 < beams) || (n_beams > 1 && step - rest < own && b0 + 1 < beams)) {
+                set_error(where, "two of the caches share memory", -1);
+                return false;
+            }
+        }
+    return true;
+}
+
+}  // namespace
+
+GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const float* v_nodes, float* k_cache_layer,
+                                      float* v_cache_layer, int32_t pos0, int32_t n_nodes, const int32_t* parents,
+                                      int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, float attn_scale,
+                                      int32_t sliding_window, const uint8_t* mmap_base, size_t q_norm_offset,
+                                      size_t k_norm_offset, int32_t has_norm_weight, float norm_eps,
+                                      size_t rope_freqs_offset, int32_t has_rope_freqs, float rope_base,
+                                      float* out_nodes) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_attention_tree";
+    if (n_nodes == 0) return;
+    if (n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || n_heads > 65535 || pos0 < 0 ||
+        pos0 > INT32_MAX - kMaxTreeNodes || (head_dim != 64 && head_dim != 128 && head_dim != 256)) {
+        set_error(where, "invalid head geometry or position (head_dim is 64, 128 or 256)", -1);
+        return;
+    }
+    TreeTable tree;
+    if (!on_host(parents, "parents", where)) return;
+    if (!make_tree_table(parents, n_nodes, tree)) {
+        set_error(where, "a tree has 1 to 512 nodes, and every parent is -1 or an earlier node", -1);
+        return;
+    }
+    if (has_norm_weight > 0 && !mmap_base) {
+        set_error(where, "no norm weights", -1);
+        return;
+    }
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    if (!on_device(q_nodes, "q_nodes", where, 16) || !on_device(k_nodes, "k_nodes", where, 16) ||
+        !on_device(v_nodes, "v_nodes", where, 16) || !on_device(k_cache_layer, "k_cache_layer", where, 16) ||
+        !on_device(v_cache_layer, "v_cache_layer", where, 16) || !on_device(out_nodes, "out_nodes", where, 16))
+        return;
+    // no two arguments share memory, but for k_nodes / v_nodes that are the
+    // cache rows they are stored to
+    const size_t qb = sizeof(float) * n_nodes * n_heads * head_dim, kvrow = sizeof(float) * n_kv_heads * head_dim;
+    const size_t kb = kvrow * n_nodes, cb = kvrow * (static_cast<size_t>(pos0) + n_nodes), at = kvrow * pos0;
+    const char* ps[] = {reinterpret_cast<char*>(q_nodes), reinterpret_cast<char*>(k_nodes),
+                        reinterpret_cast<const char*>(v_nodes), reinterpret_cast<char*>(k_cache_layer),
+                        reinterpret_cast<char*>(v_cache_layer), reinterpret_cast<char*>(out_nodes)};
+    const size_t bytes[] = {qb, kb, kb, cb, cb, qb};
+    for (int i = 0; i < 6; ++i)
+        for (int j = i + 1; j < 6; ++j)
+            if (overlaps(ps[i], bytes[i], ps[j], bytes[j]) &&
+                !((i == 1 && j == 3 && ps[1] == ps[3] + at) || (i == 2 && j == 4 && ps[2] == ps[4] + at))) {
+                set_error(where, "two of the vectors, caches and outputs overlap", -1);
+                return;
+            }
+    if (capturing()) {
+        set_error(where, "the positions' rotations are uploaded by the call, which a stream capture does not allow", -1);
+        return;
+    }
+    TreeArgs a{};
+    if (has_norm_weight > 0) {
+        a.q_gamma = reinterpret_cast<const float*>(
+            device_weights(mmap_base + q_norm_offset, sizeof(float) * static_cast<size_t>(head_dim), where));
+        a.k_gamma = reinterpret_cast<const float*>(
+            device_weights(mmap_base + k_norm_offset, sizeof(float) * static_cast<size_t>(head_dim), where));
+        if (!a.q_gamma || !a.k_gamma) return;
+    }
+    if (rope_base > 0.0f) {
+        std::array<float, kMaxRopeHalf> fac{};
+        if (has_rope_freqs && !read_factors(mmap_base, rope_freqs_offset, head_dim / 2, fac, where)) return;
+        a.rope = rope_rows(pos0, tree.max_depth + 1, head_dim, rope_base, has_rope_freqs ? fac.data() : nullptr, where);
+        if (!a.rope) return;
+    }
+    a.q = q_nodes;
+    a.k = k_nodes;
+    a.v = v_nodes;
+    a.k_cache = k_cache_layer;
+    a.v_cache = v_cache_layer;
+    a.out = out_nodes;
+    a.pos0 = pos0;
+    a.n = n_nodes;
+    a.n_heads = n_heads;
+    a.n_kv_heads = n_kv_heads;
+    a.head_dim = head_dim;
+    a.scale = attn_scale;
+    a.sliding_window = sliding_window;
+    a.norm_qk = has_norm_weight >= 0;
+    a.eps = norm_eps;
+    check(launch_attention_tree(a, tree, g_rt.stream), where);
+}
+
+GNCX_API void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t kv_dim,
+                                    int32_t row0, const int32_t* rows, int32_t n_rows) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_kv_keep_rows";
+    if (n_rows == 0) return;
+    if (kv_dim < 4 || kv_dim % 4 || row0 < 0 || n_rows < 0 || n_rows > kMaxKeepRows) {
+        set_error(where, "kv_dim must be a multiple of 4, row0 not negative, and at most 512 rows kept", -1);
+        return;
+    }
+    if (!on_host(rows, "rows", where)) return;
+    for (int32_t i = 0; i < n_rows; ++i)
+        if (rows[i] < 0 || rows[i] >= kMaxKeepOffset || (i > 0 && rows[i] <= rows[i - 1])) {
+            set_error(where, "rows must ascend strictly from 0 on, below 65536", -1);
+            return;
+        }
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    const size_t floats = (static_cast<size_t>(row0) + rows[n_rows - 1] + 1) * kv_dim;
+    if (!layer_caches(k_caches, v_caches, n_layers, static_cast<size_t>(row0) * kv_dim, floats, 1, 0, where)) return;
+    check(launch_kv_keep_rows(k_caches, v_caches, n_layers, kv_dim, row0, rows, n_rows, g_rt.stream), where);
+}
+
+GNCX_API void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,
+                                   const int32_t* finished, int32_t finished_token, int32_t n_out,
+                                   int32_t* out_parents, int32_t* out_tokens, float* out_scores) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_beam_select";
+    if (n_beams < 1 || n_beams > kMaxBeams || vocab < 1 || vocab > kMaxBeamVocab || n_out < 1 || n_out > kMaxBeamOut) {
+        set_error(where, "1 to 32 beams, 1 to 4194304 words and 1 to 64 outputs", -1);
+        return;
+    }
+    if (finished && (finished_token < 0 || finished_token >= vocab)) {
+        set_error(where, "finished_token is outside the vocabulary", -1);
+        return;
+    }
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    if (!on_device(logits, "logits", where) || !on_device(scores, "scores", where) ||
+        (finished && !on_device(finished, "finished", where)) || !on_device(out_parents, "out_parents", where) ||
+        !on_device(out_tokens, "out_tokens", where) || !on_device(out_scores, "out_scores", where))
+        return;
+    const size_t need = beam_select_workspace_bytes(n_beams, vocab, n_out);
+    void* ws = g_select_ws.take(need, where);
+    if (!ws) return;
+    check(launch_beam_select(logits, n_beams, vocab, scores, finished, finished_token, n_out, out_parents, out_tokens,
+                             out_scores, ws, g_select_ws.buf.cap, g_rt.stream),
+          where);
+}
+
+GNCX_API void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t n_beams,
+                                  size_t beam_stride, int32_t kv_dim, int32_t row0, int32_t n_rows,
+                                  const int32_t* parents) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_kv_reorder";
+    if (n_rows == 0) return;
+    if (n_beams < 1 || n_beams > kMaxBeams || kv_dim < 4 || kv_dim % 4 || row0 < 0 || n_rows < 0 ||
+        n_rows > INT32_MAX - row0 || beam_stride % 4 ||
+        (n_beams > 1 && beam_stride < (static_cast<size_t>(row0) + n_rows) * kv_dim)) {
+        set_error(where, "1 to 32 beams, kv_dim and beam_stride multiples of 4, and the rows within a beam's stride", -1);
+        return;
+    }
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    if (!on_device(parents, "parents", where) ||
+        !layer_caches(k_caches, v_caches, n_layers, static_cast<size_t>(row0) * kv_dim,
+                      (static_cast<size_t>(row0) + n_rows) * kv_dim, n_beams, beam_stride, where))
+        return;
+    check(launch_kv_reorder(k_caches, v_caches, n_layers, n_beams, beam_stride, kv_dim, row0, n_rows, parents,
+                            g_rt.stream),
+          where);
+}
+
 // ---- weight files and host buffers ------------------------------------
 // The reference's loader maps the GGUF read-only (cpp:327-404) and copies the
 // per-layer tensors, scratch vectors and KV caches into 2 MB-aligned,

@@ -437,6 +437,67 @@ int gncx_hip_decode_step_noalloc(const GNCXDecodeModel* model, const GNCXDecodeS
  * 16-byte aligned; n up to 4194304. */
 void gncx_hip_argmax(const float* values, int32_t n, int32_t* out_index);
 
+/* Several candidate continuations of one sequence: a drafted tree verified in
+ * one pass (speculative decoding), and beam search.  No counterpart in the
+ * reference, whose streamer decodes one continuation.  Caches, vectors and
+ * outputs are memory of the library's GPU, used in place and in the order of
+ * the library stream, and nothing synchronises with the host (but for the
+ * upload of a position's rotations, below).  Refused calls leave every output
+ * as it was.
+ *
+ * Attention of a drafted tree of n_nodes (1..512) tokens over the cache of the
+ * first pos0 positions.  parents (host memory, read before the call returns):
+ * parents[i] is -1 for a first token, else an earlier node; a node's depth is
+ * 0 without a parent, else its parent's plus 1, and its position pos0 + depth.
+ * As in gncx_hip_attention_prefill, q_nodes [n_nodes][n_heads*head_dim] and
+ * k_nodes [n_nodes][n_kv_heads*head_dim] receive the per-head RMSNorm (with
+ * weights for has_norm_weight > 0, without for 0, no norm at all below 0) and
+ * the rotation of their position, and cache rows pos0 + i those of node i (so
+ * the caches hold pos0 + n_nodes rows; k_nodes and v_nodes may be those rows
+ * themselves).  out_nodes[i] is the attention of node i over the cached rows,
+ * its ancestors and itself; with sliding_window > 0 over those of them within
+ * that many positions up to its own.  What a node does not see has no part in
+ * its output, whatever it holds.  head_dim is 64, 128 or 256; 16-byte aligned
+ * pointers; out_nodes overlaps no other argument.  The first call of a (pos0,
+ * depth) waits for the stream to upload the rotations, so the call cannot be
+ * captured into a graph (refused). */
+void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const float* v_nodes, float* k_cache_layer,
+                             float* v_cache_layer, int32_t pos0, int32_t n_nodes, const int32_t* parents,
+                             int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, float attn_scale,
+                             int32_t sliding_window, const uint8_t* mmap_base, size_t q_norm_offset,
+                             size_t k_norm_offset, int32_t has_norm_weight, float norm_eps, size_t rope_freqs_offset,
+                             int32_t has_rope_freqs, float rope_base, float* out_nodes);
+/* Row row0 + i of every layer's two caches <- the old row row0 + rows[i], for
+ * i < n_rows (at most 512): the accepted path of a tree whose nodes stand from
+ * row0 on.  rows (host memory, read before the call returns) ascend strictly
+ * from 0 on, below 65536.  Rows behind the n_rows kept ones stay as they are.
+ * k_caches / v_caches: host arrays of n_layers device addresses, 16-byte
+ * aligned; kv_dim (n_kv_heads*head_dim) a multiple of 4. */
+void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t kv_dim,
+                           int32_t row0, const int32_t* rows, int32_t n_rows);
+/* Beam search's selection.  The candidates are (b, v) for beams b < n_beams
+ * (1..32) and words v < vocab (up to 4194304) with the score
+ *   scores[b] + logits[b][v] - log(sum over u of e^logits[b][u]);
+ * a beam with finished[b] != 0 (finished may be NULL) has the one candidate
+ * (b, finished_token) with the score scores[b], and its logits are not read.
+ * The n_out (1..64) best come in falling order, equal scores by the lowest
+ * b * vocab + v.  A NaN logit or score counts as -inf, and a score of -inf is
+ * no candidate: outputs left over have parent -1, word -1, score -inf.  Sums
+ * and scores are formed in 64 bits.  out_scores may be scores, out_parents or
+ * out_tokens finished.  Can be captured into a graph after a call of the same
+ * sizes; graphs that hold it share one workspace and are not run at once. */
+void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,
+                          const int32_t* finished, int32_t finished_token, int32_t n_out, int32_t* out_parents,
+                          int32_t* out_tokens, float* out_scores);
+/* The beams' caches after a selection: rows [row0, row0 + n_rows) of beam b <-
+ * the old ones of beam parents[b] (device memory, as gncx_hip_beam_select
+ * writes them), in place, for every layer.  Beam b's cache of layer l starts
+ * beam_stride * b floats behind k_caches[l] / v_caches[l]; a parent outside
+ * [0, n_beams) leaves its beam as it is.  n_beams 1..32; kv_dim and
+ * beam_stride multiples of 4; addresses as in gncx_hip_kv_keep_rows. */
+void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t n_beams,
+                         size_t beam_stride, int32_t kv_dim, int32_t row0, int32_t n_rows, const int32_t* parents);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,97 @@
+"""Refusals of the entries for several continuations that need no device: they
+come before any HIP call, with the outputs untouched (CPU)."""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+import pytest
+
+from conftest import gncx
+
+
+@pytest.fixture(scope="module")
+def plib():
+    return gncx.load()
+
+
+def refused(lib, text):
+    assert lib.gncx_hip_last_status() != 0
+    assert text in lib.gncx_hip_last_error().decode()
+
+
+def tree(lib, parents, n=None, pos0=0, H=4, KV=2, hd=64, weight=-1):
+    p = None if parents is None else np.asarray(parents, np.int32)
+    out = np.full(8, 7.0, np.float32)
+    lib.gncx_hip_last_status()
+    lib.gncx_hip_attention_tree(None, None, None, None, None, pos0, len(parents) if n is None else n,
+                                None if p is None else p.ctypes.data, H, KV, hd, 1.0, 0, None, 0, 0, weight, 1e-6, 0,
+                                0, 0.0, out.ctypes.data)
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("parents", [[0], [1, -1], [-1, 1], [-1, 0, 2], [-2], [-1, -3], [-1, 2, 1], [-1] * 513])
+def test_tree_refuses_what_is_no_tree(plib, parents):
+    tree(plib, parents)
+    refused(plib, "every parent is -1 or an earlier node")
+
+
+def test_tree_refuses_negative_and_missing(plib):
+    tree(plib, [-1], n=-1)
+    refused(plib, "1 to 512 nodes")
+    tree(plib, None, n=1)
+    refused(plib, "parents must be host memory")
+    tree(plib, [-1], weight=1)
+    refused(plib, "no norm weights")
+
+
+@pytest.mark.parametrize("geo", [dict(H=3), dict(H=0), dict(KV=0), dict(hd=96), dict(hd=0), dict(pos0=-1),
+                                 dict(pos0=2 ** 31 - 512)])
+def test_tree_refuses_geometry(plib, geo):
+    tree(plib, [-1], **geo)
+    refused(plib, "invalid head geometry")
+
+
+def test_no_nodes_and_no_rows_are_no_error(plib):
+    plib.gncx_hip_last_status()
+    tree(plib, [])
+    plib.gncx_hip_kv_keep_rows(None, None, 1, 64, 0, None, 0)
+    plib.gncx_hip_kv_reorder(None, None, 1, 2, 64, 64, 0, 0, None)
+    assert plib.gncx_hip_last_status() == 0
+
+
+@pytest.mark.parametrize("rows", [[1, 1], [2, 1], [-1], [0, 65536]])
+def test_keep_refuses_rows_out_of_order(plib, rows):
+    r, none = np.asarray(rows, np.int32), (C.c_void_p * 1)()
+    plib.gncx_hip_kv_keep_rows(none, none, 1, 64, 0, r.ctypes.data, len(rows))
+    refused(plib, "ascend strictly")
+
+
+@pytest.mark.parametrize("kv_dim,row0,n", [(6, 0, 1), (0, 0, 1), (64, -1, 1), (64, 0, 513), (64, 0, -1)])
+def test_keep_refuses_sizes(plib, kv_dim, row0, n):
+    r, none = np.arange(max(n, 1), dtype=np.int32), (C.c_void_p * 1)()
+    plib.gncx_hip_kv_keep_rows(none, none, 1, kv_dim, row0, r.ctypes.data, n)
+    refused(plib, "multiple of 4")
+
+
+@pytest.mark.parametrize("beams,vocab,n_out", [(0, 10, 1), (33, 10, 1), (1, 0, 1), (1, 2 ** 22 + 1, 1), (1, 10, 0),
+                                               (1, 10, 65)])
+def test_select_refuses_sizes(plib, beams, vocab, n_out):
+    plib.gncx_hip_beam_select(None, beams, vocab, None, None, 0, n_out, None, None, None)
+    refused(plib, "beams")
+
+
+@pytest.mark.parametrize("token", [-1, 10])
+def test_select_refuses_a_finished_token_outside_the_vocabulary(plib, token):
+    done = np.zeros(2, np.int32)
+    plib.gncx_hip_beam_select(None, 2, 10, None, done.ctypes.data, token, 1, None, None, None)
+    refused(plib, "finished_token")
+
+
+@pytest.mark.parametrize("beams,stride,kv_dim,row0,n", [(0, 64, 64, 0, 1), (33, 64, 64, 0, 1), (2, 63, 64, 0, 1),
+                                                        (2, 66, 64, 0, 1), (2, 128, 6, 0, 1), (2, 128, 64, 1, 2),
+                                                        (2, 128, 64, -1, 1), (2, 128, 64, 0, -1)])
+def test_reorder_refuses_sizes(plib, beams, stride, kv_dim, row0, n):
+    none = (C.c_void_p * 1)()
+    plib.gncx_hip_kv_reorder(none, none, 1, beams, stride, kv_dim, row0, n, None)
+    refused(plib, "1 to 32 beams")
