@@ -1544,6 +1544,10 @@ struct TreeParams {
     const float* rope;  // [max depth + 1][HD]: cos then sin, or null
     int32_t pos0, n, n_heads, n_kv, sw, norm_qk;
     float scale, eps;
+    // the key ranges: first key, keys of one; their parts [range][n_kv][rows_pad]
+    int32_t first, chunk, rows_pad;
+    float* part_o;    // [..][HD]
+    float2* part_ml;  // (max, sum)
     TreeTable tree;
 };
 
@@ -1603,68 +1607,496 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p) {
     }
 }
 
-// One work-group per (head, node): a wave takes every fourth visible key, its
-// lanes the dims of the dot and of the sum, with a running maximum and sum;
-// the waves' results meet in LDS.
-template <int HD>
-__global__ __launch_bounds__(kThreads) void tree_attention_kernel(TreeParams p) {
-    constexpr int E = HD / 64;
-    __shared__ float os[kWaves][HD];
-    __shared__ float ms[kWaves], ls[kWaves];
-    const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    const int hk = h / (p.n_heads / p.n_kv);
-    const size_t kn = static_cast<size_t>(p.n_kv) * HD;
-    float q[E], o[E];
+// The products on the fp16 matrix cores, keys over waves.  A work-group owns 32
+// RT query rows (node, head) of one KV head and a range of keys; each of its
+// waves walks every fourth 32-key tile of the range by itself, with the tile's
+// K and V straight from memory into the registers that the products take, so
+// the loop has no barrier and every K/V byte is read once per 32 RT rows.
+//   S^T = K Q^T   v_mfma_f32_32x32x16_f16, operands as fp16 pairs, three
+//                 products a slice (hi hi, hi lo, lo hi: 2^-22 of the product);
+//                 lane (i, g) ends up with query row i's scores of the 16 keys
+//                 8 a + 4 g + b
+//   O^T += V^T P^T  with P from those registers, and O of row i in lane (i, .):
+//                 the softmax factors of a row never cross lanes
+// Pairs hold values of any size: every key, value and query row is scaled by a
+// power of two of its own.  A key's and a query's come back as factors of the
+// scores.  A value row's 2^e_j goes into its weight: with t_j = s_j + e_j the
+// weights of O are 2^(t_j - max t + 14), those of the sum l 2^(s_j - max s), two
+// running maxima a row, so a row's precision hangs on its largest term alone
+// and not on rows it does not see.  A value row that is not finite takes no part
+// in the products (0 times it would be NaN for the nodes that do not see it) and
+// is added lane by lane; so are the scores of an infinite key.
+// Parts are left normalised, o_part = sum w v / sum w, with (m, l) beside them:
+// no sum of large values can overflow between the kernels.  The reference's
+// 1e-12 beside a sum l >= 1 is below fp32's rounding and left out.
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+// 2^k as the exponent field of a float; k in [-126, 127]
+__device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_cast(float, field << 23); }
+// the exponent field of |x|'s power of two, kept where 2^(+-(14 + e)) are normal
+__device__ __forceinline__ int scale_field(float amax) {
+    const int f = static_cast<int>(__builtin_bit_cast(uint32_t, amax) >> 23) & 0xff;
+    return min(max(f, 30), 254);
+}
+__device__ __forceinline__ float max3_abs(float m, float a, float b) { return fmaxf(fmaxf(m, fabsf(a)), fabsf(b)); }
+// |x|'s bits: above 0x7f7fffff for infinities and NaN, ordered like |x| below
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
+    const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xf, 0xf, false));
+    return o > v ? o : v;
+}
+
+__device__ __forceinline__ void pair8(const float (&v)[8], float scale, half8_t& hi, half8_t& lo) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        q[e] = p.q[(static_cast<size_t>(t) * p.n_heads + h) * HD + 64 * e + lane];
-        o[e] = 0.0f;
-    }
-    float m = -1e30f, l = 0.0f;
-    auto visit = [&](int row) {
-        const size_t at = static_cast<size_t>(row) * kn + static_cast<size_t>(hk) * HD + lane;
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s += q[e] * p.k_cache[at + 64 * e];
-        s = wave_sum(s) * p.scale;
-        const float m2 = fmaxf(m, s), a = expf(m - m2), w = expf(s - m2);
-        l = l * a + w;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = o[e] * a + w * p.v_cache[at + 64 * e];
-        m = m2;
-    };
-    const int here = p.pos0 + p.tree.depth[t], pre = p.tree.pre[t];
-    const int lo = p.sw > 0 ? max(0, here - p.sw + 1) : 0;
-    for (int j = lo + wv; j < p.pos0; j += kWaves) visit(j);
-    for (int a = wv; a <= t; a += kWaves)
-        if (p.tree.pre[a] <= pre && pre < p.tree.end[a] && p.pos0 + p.tree.depth[a] >= lo) visit(p.pos0 + a);
-#pragma unroll
-    for (int e = 0; e < E; ++e) os[wv][64 * e + lane] = o[e];
-    if (lane == 0) {
-        ms[wv] = m;
-        ls[wv] = l;
-    }
-    __syncthreads();
-    float M = ms[0];
-    for (int w = 1; w < kWaves; ++w) M = fmaxf(M, ms[w]);
-    for (int d = threadIdx.x; d < HD; d += kThreads) {
-        float sum = 0.0f, acc = 0.0f;
-        for (int w = 0; w < kWaves; ++w) {
-            const float f = expf(ms[w] - M);
-            sum += ls[w] * f;
-            acc += os[w][d] * f;
-        }
-        p.out[(static_cast<size_t>(t) * p.n_heads + h) * HD + d] = acc / (sum + 1e-12f);
+    for (int i = 0; i < 8; ++i) {
+        const float x = v[i] * scale;
+        const _Float16 h = static_cast<_Float16>(x);
+        hi[i] = h;
+        lo[i] = static_cast<_Float16>(x - static_cast<float>(h));
     }
 }
 
+constexpr int kTreeKeys = 32;                     // keys of a tile
+constexpr int kTreeStep = kTreeKeys * kWaves;     // keys of a work-group's step
+constexpr int kTreeMaxChunks = 64;                // key ranges of a call
+
+template <int HD, int RT, int OCC>
+__global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) {
+    constexpr int NC = HD / 16, NN = HD / 32, R = 32 * RT;
+    constexpr int kPart = NN * 8 * 33;  // float4 of a wave's 32 rows, padded per (n, a, g)
+    constexpr int kQ = RT * NC * 64;    // half8 of the query rows' hi (and lo) parts
+    constexpr int kShared = kQ * 2 > kPart * kWaves ? kQ * 2 : kPart * kWaves;
+    __shared__ __align__(16) float4 shared[kShared];
+    __shared__ float qfac[R];
+    __shared__ __align__(16) float kfac[kWaves][kTreeKeys];
+    __shared__ float2 mls[kWaves][32];
+    __shared__ uint32_t interval[kMaxTreeNodes];  // pre | end << 16
+    __shared__ uint16_t depth[kMaxTreeNodes];
+    __shared__ float vfac[kWaves][kTreeKeys];     // a tile's value factors, for rows that are not finite
+    half8_t* const qhi = reinterpret_cast<half8_t*>(shared);
+    half8_t* const qlo = qhi + kQ;
+    // a tile's weights, for value rows that are not finite, behind the query rows
+    float(*const pw)[kTreeKeys][33] = reinterpret_cast<float(*)[kTreeKeys][33]>(shared + 2 * kQ);
+    static_assert((kShared - 2 * kQ) * 4 >= kWaves * kTreeKeys * 33, "room for the weights");
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * R;
+    const int total = p.pos0 + p.n;
+    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(total, c0 + p.chunk);
+    const uint32_t kn = static_cast<uint32_t>(p.n_kv) * HD;
+    const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
+    const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
+
+    float kr[NC][8], vr[NN][2][8];
+    // rows past the range are read as its last one (their weights are 0)
+    auto load_k = [&](int t0) {
+        const float* b = kbase + static_cast<size_t>(t0) * kn;
+        const uint32_t at = static_cast<uint32_t>(min(li, c1 - 1 - t0)) * kn + 8 * g;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const floatx4 v = *reinterpret_cast<const floatx4*>(b + (at + 16 * c + 4 * h));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kr[c][4 * h + i] = v[i];
+            }
+    };
+    auto load_v = [&](int t0) {
+        const float* b = vbase + static_cast<size_t>(t0) * kn;
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = 16 * c + 4 * g + (i & 3) + 8 * (i >> 2);
+                const uint32_t at = static_cast<uint32_t>(min(key, c1 - 1 - t0)) * kn + li;
+#pragma unroll
+                for (int n = 0; n < NN; ++n) vr[n][c][i] = b[at + 32 * n];
+            }
+    };
+    const int first = c0 + kTreeKeys * wv;
+    if (first < c1) {
+        load_k(first);
+        load_v(first);
+    }
+
+    // the query rows, 8 threads each: scaled, split and laid out as operands
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int r = row0 + 32 * rt + tid / 8, j = tid % 8;
+        float x[HD / 64][8], amax = 0.0f;
+        const float* src = p.q + (static_cast<size_t>(r < rows ? r / G : 0) * p.n_heads + hk * G + r % G) * HD + j * (HD / 8);
+#pragma unroll
+        for (int u = 0; u < HD / 64; ++u)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[u][i] = r < rows ? src[8 * u + i] : 0.0f;
+                amax = fmaxf(amax, fabsf(x[u][i]));
+            }
+        amax = group8_max(amax);
+        const int f = scale_field(amax);
+#pragma unroll
+        for (int u = 0; u < HD / 64; ++u) {
+            half8_t h, l;
+            pair8(x[u], pow2_field(254 + 7 - f), h, l);
+            const int unit = j * (HD / 64) + u, at = (rt * NC + unit / 2) * 64 + 32 * (unit & 1) + tid / 8;
+            qhi[at] = h;
+            qlo[at] = l;
+        }
+        if (j == 0) qfac[32 * rt + tid / 8] = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
+    }
+    if (c1 > p.pos0)
+        for (int i = tid; i < p.n; i += kThreads) {
+            interval[i] = p.tree.pre[i] | static_cast<uint32_t>(p.tree.end[i]) << 16;
+            depth[i] = p.tree.depth[i];
+        }
+    // this lane's rows: their place in the tree and first visible position
+    uint32_t pre[RT];
+    int lo[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int t = min(row0 + 32 * rt + li, rows - 1) / G;
+        pre[rt] = p.tree.pre[t];
+        lo[rt] = p.sw > 0 ? max(0, p.pos0 + p.tree.depth[t] - p.sw + 1) : 0;
+    }
+    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.tree.max_depth - p.sw + 1) : 0;
+    __syncthreads();
+
+    float m[RT], mt[RT], l[RT], qf[RT];
+    floatx16 o[RT][NN];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        m[rt] = mt[rt] = -1e30f;
+        l[rt] = 0.0f;
+        qf[rt] = qfac[32 * rt + li];
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[rt][n][r] = 0.0f;
+    }
+
+    for (int t0 = first; t0 < c1; t0 += kTreeStep) {
+        // ---- scores
+        float amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) amax = max3_abs(amax, kr[c][i], kr[c][i + 1]);
+        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
+        const uint64_t infinite = __ballot(amax == __builtin_inff());  // (NaN gives NaN scores by itself)
+        const int kf = scale_field(amax);
+        if (g == 0) kfac[wv][li] = pow2_field(kf - 7);
+        const float ks = pow2_field(254 + 7 - kf);
+        floatx16 st[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[rt][r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            half8_t kh, kl;
+            pair8(kr[c], ks, kh, kl);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                const half8_t h = qhi[(rt * NC + c) * 64 + lane], lw = qlo[(rt * NC + c) * 64 + lane];
+                st[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, h, st[rt], 0, 0, 0);
+                st[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, lw, st[rt], 0, 0, 0);
+                st[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, h, st[rt], 0, 0, 0);
+            }
+        }
+        const int next = t0 + kTreeStep;
+        if (next < c1) load_k(next);
+
+        // ---- the value rows' powers of two, in the lanes that hold their scores
+        float ve[16], vs[16];
+        uint32_t odd = 0;  // this lane half's value rows that are not finite
+        auto value_factors = [&]() {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                uint32_t b = 0;
+#pragma unroll
+                for (int n = 0; n < NN; ++n) b = max(b, abs_bits(vr[n][r >> 3][r & 7]));
+                b = dpp_max_u32<0xb1>(b);
+                b = dpp_max_u32<0x4e>(b);
+                b = dpp_max_u32<0x141>(b);
+                b = dpp_max_u32<0x140>(b);
+                b = max(b, static_cast<uint32_t>(__shfl_xor(static_cast<int>(b), 16, 64)));
+                if (b >= 0x7f800000u) odd |= 1u << r;
+                const int f = scale_field(__builtin_bit_cast(float, b));
+                ve[r] = static_cast<float>(f - 127);
+                vs[r] = pow2_field(254 + 14 - f);
+            }
+        };
+        value_factors();
+        const bool any_odd = __ballot(odd != 0) != 0;
+        if (any_odd) {
+            // their factors from the elements that are finite, and zeros for the products
+            const uint32_t was = odd;
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (abs_bits(vr[n][r >> 3][r & 7]) >= 0x7f800000u) vr[n][r >> 3][r & 7] = 0.0f;
+            value_factors();
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (was >> r & 1) vr[n][r >> 3][r & 7] = 0.0f;
+            odd = was;
+        }
+
+        // ---- softmax
+        const bool plain = t0 + kTreeKeys <= min(p.pos0, c1) && t0 >= lo_most;
+        float e[RT][16];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const floatx4 f = *reinterpret_cast<const floatx4*>(&kfac[wv][8 * a + 4 * g]);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) st[rt][4 * a + b] = st[rt][4 * a + b] * f[b] * qf[rt];
+            }
+            if (infinite) {
+                // an infinite key's scores from the elements (inf - inf of its pair says nothing)
+                const int row = min(row0 + 32 * rt + li, rows - 1);
+                const float* q = p.q + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD;
+                for (int j = 0; j < kTreeKeys; ++j)
+                    if (infinite >> j & 1) {
+                        const float* k = kbase + static_cast<size_t>(min(t0 + j, c1 - 1)) * kn;
+                        float s = 0.0f;
+                        for (int d = 0; d < HD; ++d) s += q[d] * k[d];
+                        s *= p.scale * 1.4426950408889634f;
+#pragma unroll
+                        for (int r = 0; r < 16; ++r)
+                            if (8 * (r >> 2) + 4 * g + (r & 3) == j) st[rt][r] = s;
+                    }
+            }
+            if (!plain) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = t0 + 8 * (r >> 2) + 4 * g + (r & 3);
+                    bool see = key < p.pos0 && key >= lo[rt];
+                    if (key >= p.pos0 && key < c1) {
+                        const uint32_t iv = interval[key - p.pos0];
+                        see = (iv & 0xffffu) <= pre[rt] && pre[rt] < iv >> 16 &&
+                              p.pos0 + depth[key - p.pos0] >= lo[rt];
+                    }
+                    if (!(see && key < c1)) st[rt][r] = -__builtin_inff();
+                }
+            }
+            float mx = -1e30f, mxt = -1e30f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                mx = fmaxf(mx, st[rt][r]);
+                mxt = fmaxf(mxt, st[rt][r] + ve[r]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            mxt = fmaxf(mxt, __shfl_xor(mxt, 32, 64));
+            const float m2 = fmaxf(m[rt], mx), mt2 = fmaxf(mt[rt], mxt);
+            float sum = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                sum += __builtin_amdgcn_exp2f(st[rt][r] - m2);
+                e[rt][r] = __builtin_amdgcn_exp2f(st[rt][r] + ve[r] - mt2 + 14.0f);
+            }
+            sum += __shfl_xor(sum, 32, 64);
+            l[rt] = l[rt] * __builtin_amdgcn_exp2f(m[rt] - m2) + sum;
+            const float alpha = __builtin_amdgcn_exp2f(mt[rt] - mt2);
+            m[rt] = m2;
+            mt[rt] = mt2;
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[rt][n][r] *= alpha;
+        }
+
+        // ---- weighted values
+        half8_t ph[RT][2], pl[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float w[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) w[i] = e[rt][8 * c + i];
+                split8(w, ph[rt][c], pl[rt][c]);
+            }
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                half8_t vh, vl;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float x = vr[n][c][i] * vs[8 * c + i];
+                    const _Float16 h = static_cast<_Float16>(x);
+                    vh[i] = h;
+                    vl[i] = static_cast<_Float16>(x - static_cast<float>(h));
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    o[rt][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[rt][c], o[rt][n], 0, 0, 0);
+                    o[rt][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[rt][c], o[rt][n], 0, 0, 0);
+                    o[rt][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[rt][c], o[rt][n], 0, 0, 0);
+                }
+            }
+        if (any_odd) {
+            // value rows that are not finite, for the rows that see them.  Bit r
+            // of half g's mask is key 8 (r / 4) + 4 g + r % 4.
+            if (li == 0)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) vfac[wv][8 * (r >> 2) + 4 * g + (r & 3)] = vs[r];
+            const uint32_t odd0 = __builtin_amdgcn_readlane(odd, 0), odd1 = __builtin_amdgcn_readlane(odd, 32);
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) pw[wv][8 * (r >> 2) + 4 * g + (r & 3)][li] = e[rt][r];
+                __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes, read back below
+                asm volatile("" ::: "memory");
+                for (int j = 0; j < kTreeKeys; ++j) {
+                    const int r = 4 * (j >> 3) + (j & 3);
+                    if (!(((j >> 2 & 1) ? odd1 : odd0) >> r & 1)) continue;
+                    const float w = pw[wv][j][li], f = vfac[wv][j];
+                    if (w == 0.0f) continue;
+                    const float* v = vbase + static_cast<size_t>(min(t0 + j, c1 - 1)) * kn;
+#pragma unroll
+                    for (int n = 0; n < NN; ++n)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            o[rt][n][i] += w * (v[32 * n + 8 * (i >> 2) + 4 * g + (i & 3)] * f);
+                }
+                asm volatile("" ::: "memory");
+            }
+        }
+        if (next < c1) load_v(next);
+    }
+
+    // ---- the waves' parts meet in LDS
+    const bool whole = gridDim.z == 1;
+    const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        __syncthreads();  // the query rows, or the parts of the row tile before, are done with
+        const float f = l[rt] > 0.0f || l[rt] != l[rt] ? __builtin_amdgcn_exp2f(mt[rt] - m[rt] - 28.0f) / l[rt] : 0.0f;
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+#pragma unroll
+            for (int a = 0; a < 4; ++a)
+                shared[wv * kPart + ((n * 4 + a) * 2 + g) * 33 + li] =
+                    make_float4(o[rt][n][4 * a] * f, o[rt][n][4 * a + 1] * f, o[rt][n][4 * a + 2] * f,
+                                o[rt][n][4 * a + 3] * f);
+        if (g == 0) mls[wv][li] = make_float2(m[rt], l[rt]);
+        __syncthreads();
+        for (int i = tid; i < 32 * HD / 4; i += kThreads) {
+            const int r = i / (HD / 4), d4 = i % (HD / 4), row = row0 + 32 * rt + r;
+            if (row >= rows) continue;
+            float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) M = fmaxf(M, mls[w][r].x);
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const float2 ml = mls[w][r];
+                const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
+                const float4 v = shared[w * kPart + d4 * 33 + r];
+                L += wt;
+                if (wt != 0.0f) {  // (a part without a key has nothing to add)
+                    x[0] += wt * v.x;
+                    x[1] += wt * v.y;
+                    x[2] += wt * v.z;
+                    x[3] += wt * v.w;
+                }
+            }
+            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            float* dst = whole ? p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD
+                               : p.part_o + (prow + 32 * rt + r) * HD;
+            reinterpret_cast<float4*>(dst)[d4] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+            if (!whole && d4 == 0) p.part_ml[prow + 32 * rt + r] = make_float2(M, L);
+        }
+    }
+}
+
+// out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the key
+// ranges c, a thread per float4, sixteen ranges' loads issued at once.
+constexpr int kTreeMergeLoads = 16;
 template <int HD>
-hipError_t launch_tree_hd(const TreeParams& p, hipStream_t stream) {
+__global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams p, int32_t chunks) {
+    const int G = p.n_heads / p.n_kv, rows = p.n * G, hk = blockIdx.y;
+    const int i = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
+    const int row = i / (HD / 4), d4 = i % (HD / 4);
+    if (row >= rows) return;
+    float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = 0; c0 < chunks; c0 += kTreeMergeLoads) {
+        float2 ml[kTreeMergeLoads];
+        float4 v[kTreeMergeLoads];
+#pragma unroll
+        for (int u = 0; u < kTreeMergeLoads; ++u) {
+            const int c = min(c0 + u, chunks - 1);
+            const size_t at = (static_cast<size_t>(c) * p.n_kv + hk) * p.rows_pad + row;
+            ml[u] = p.part_ml[at];
+            v[u] = reinterpret_cast<const float4*>(p.part_o + at * HD)[d4];
+        }
+        float m2 = M;
+#pragma unroll
+        for (int u = 0; u < kTreeMergeLoads; ++u) m2 = fmaxf(m2, ml[u].x);
+        const float a = __builtin_amdgcn_exp2f(M - m2);
+        M = m2;
+        L *= a;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] *= a;
+#pragma unroll
+        for (int u = 0; u < kTreeMergeLoads; ++u) {
+            const float wt = c0 + u < chunks ? ml[u].y * __builtin_amdgcn_exp2f(ml[u].x - m2) : 0.0f;
+            L += wt;
+            if (wt != 0.0f) {
+                x[0] += wt * v[u].x;
+                x[1] += wt * v[u].y;
+                x[2] += wt * v[u].z;
+                x[3] += wt * v[u].w;
+            }
+        }
+    }
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    reinterpret_cast<float4*>(p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD)[d4] =
+        make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+}
+
+// The split of a call: row tiles a wave, keys a work-group, key ranges.
+struct TreePlan {
+    int32_t rt, first, chunk, chunks, rows_pad;
+};
+
+TreePlan tree_plan(const TreeArgs& a) {
+    TreePlan pl;
+    const int32_t rows = a.n * (a.n_heads / a.n_kv_heads);
+    pl.rt = rows > 32 && a.head_dim <= 128 ? 2 : 1;
+    const int32_t groups = (rows + 32 * pl.rt - 1) / (32 * pl.rt);
+    pl.rows_pad = groups * 32 * pl.rt;
+    pl.first = a.sliding_window > 0 ? std::max(0, a.pos0 - a.sliding_window + 1) : 0;
+    const int64_t keys = static_cast<int64_t>(a.pos0) + a.n - pl.first;
+    // one work-group a CU (two of one row tile at head_dim up to 128 share one)
+    const int64_t want = std::max<int64_t>(1, (pl.rt == 1 && a.head_dim <= 128 ? 512 : 256) / (groups * a.n_kv_heads));
+    const int64_t steps = (keys + kTreeStep - 1) / kTreeStep;
+    const int64_t per = (steps + std::min<int64_t>(want, kTreeMaxChunks) - 1) / std::min<int64_t>(want, kTreeMaxChunks);
+    pl.chunk = static_cast<int32_t>(per * kTreeStep);
+    pl.chunks = static_cast<int32_t>((steps + per - 1) / per);
+    return pl;
+}
+
+template <int HD, int RT, int OCC>
+hipError_t launch_tree_keys(const TreeParams& p, const TreePlan& pl, hipStream_t stream) {
     const int heads = p.n_heads + p.n_kv;
     hipLaunchKernelGGL(tree_prologue_kernel<HD>, dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(tree_attention_kernel<HD>, dim3(p.n_heads, p.n), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((tree_keys_kernel<HD, RT, OCC>), dim3(p.n_kv, pl.rows_pad / (32 * RT), pl.chunks), dim3(kThreads), 0,
+                       stream, p);
+    e = hipGetLastError();
+    if (e != hipSuccess || pl.chunks == 1) return e;
+    const int64_t n = static_cast<int64_t>(p.n) * (p.n_heads / p.n_kv) * HD / 4;
+    hipLaunchKernelGGL(tree_merge_kernel<HD>, dim3(static_cast<uint32_t>((n + kThreads - 1) / kThreads), p.n_kv),
+                       dim3(kThreads), 0, stream, p, pl.chunks);
     return hipGetLastError();
 }
 
@@ -1697,7 +2129,13 @@ bool make_tree_table(const int32_t* parents, int32_t n, TreeTable& t) {
     return true;
 }
 
-hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, hipStream_t stream) {
+size_t attention_tree_workspace_bytes(const TreeArgs& a) {
+    const TreePlan pl = tree_plan(a);
+    return pl.chunks == 1 ? 0 : sizeof(float) * pl.chunks * a.n_kv_heads * pl.rows_pad * (a.head_dim + 2);
+}
+
+hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, void* workspace, size_t workspace_bytes,
+                                 hipStream_t stream) {
     if (a.n < 1 || a.n > kMaxTreeNodes || a.pos0 < 0 || a.n_heads < 1 || a.n_kv_heads < 1 ||
         a.n_heads % a.n_kv_heads != 0)
         return hipErrorInvalidValue;
@@ -1720,10 +2158,19 @@ hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, hipSt
     p.scale = a.scale;
     p.eps = a.eps;
     p.tree = tree;
-    switch (a.head_dim) {
-    case 64: return launch_tree_hd<64>(p, stream);
-    case 128: return launch_tree_hd<128>(p, stream);
-    case 256: return launch_tree_hd<256>(p, stream);
+    const TreePlan pl = tree_plan(a);
+    if (workspace_bytes < attention_tree_workspace_bytes(a)) return hipErrorInvalidValue;
+    p.first = pl.first;
+    p.chunk = pl.chunk;
+    p.rows_pad = pl.rows_pad;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.chunks) * a.n_kv_heads * pl.rows_pad * a.head_dim);
+    switch (a.head_dim * 4 + pl.rt) {
+    case 64 * 4 + 1: return launch_tree_keys<64, 1, 2>(p, pl, stream);
+    case 64 * 4 + 2: return launch_tree_keys<64, 2, 2>(p, pl, stream);
+    case 128 * 4 + 1: return launch_tree_keys<128, 1, 2>(p, pl, stream);
+    case 128 * 4 + 2: return launch_tree_keys<128, 2, 1>(p, pl, stream);
+    case 256 * 4 + 1: return launch_tree_keys<256, 1, 1>(p, pl, stream);
     default: return hipErrorInvalidValue;
     }
 }

@@ -186,7 +186,9 @@ struct TreeArgs {
     float eps;
     const float* rope;  // device [max_depth + 1][head_dim]: cos[head_dim / 2] then sin, or null
 };
-hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, hipStream_t stream);
+size_t attention_tree_workspace_bytes(const TreeArgs& a);
+hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, void* workspace, size_t workspace_bytes,
+                                 hipStream_t stream);
 
 // Rows of every layer's caches: row0 + i <- row0 + rows[i] for i < n, rows
 // (host) strictly ascending and below kMaxKeepOffset.

@@ -2996,7 +2996,7 @@ struct SharedWorkspace {
         return buf.p;
     }
 };
-SharedWorkspace g_select_ws;
+SharedWorkspace g_select_ws, g_tree_ws;
 
 // Every cache is memory of the library's GPU, holds `floats` floats, and no two
 // share a touched float: cache c's are [lo, floats) + beam * stride for beams
@@ -3135,7 +3135,9 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
     a.sliding_window = sliding_window;
     a.norm_qk = has_norm_weight >= 0;
     a.eps = norm_eps;
-    check(launch_attention_tree(a, tree, g_rt.stream), where);
+    void* ws = g_tree_ws.take(std::max<size_t>(attention_tree_workspace_bytes(a), 1), where);
+    if (!ws) return;
+    check(launch_attention_tree(a, tree, ws, g_tree_ws.buf.cap, g_rt.stream), where);
 }
 
 GNCX_API void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t kv_dim,
