@@ -1631,6 +1631,8 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p) {
 // 1e-12 beside a sum l >= 1 is below fp32's rounding and left out.
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
+// (by value: a bit cast of a vector's element in place takes the first element)
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
 // 2^k as the exponent field of a float; k in [-126, 127]
 __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_cast(float, field << 23); }
 // the exponent field of |x|'s power of two, kept where 2^(+-(14 + e)) are normal
@@ -1638,23 +1640,49 @@ __device__ __forceinline__ int scale_field(float amax) {
     const int f = static_cast<int>(__builtin_bit_cast(uint32_t, amax) >> 23) & 0xff;
     return min(max(f, 30), 254);
 }
-__device__ __forceinline__ float max3_abs(float m, float a, float b) { return fmaxf(fmaxf(m, fabsf(a)), fabsf(b)); }
-// |x|'s bits: above 0x7f7fffff for infinities and NaN, ordered like |x| below
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __builtin_bit_cast(uint32_t, x) & 0x7fffffffu; }
-
+// max(m, |a|, |b|), NaN if one is
+__device__ __forceinline__ float max3_abs(float m, float a, float b) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, fabsf(a)), fabsf(b));
+}
 template <int CTRL>
-__device__ __forceinline__ uint32_t dpp_max_u32(uint32_t v) {
-    const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), CTRL, 0xf, 0xf, false));
-    return o > v ? o : v;
+__device__ __forceinline__ float dpp_maximum(float v, float of) {
+    const int o = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, of), CTRL, 0xf, 0xf, false);
+    return __builtin_elementwise_maximum(v, __builtin_bit_cast(float, o));
+}
+// x[r], r < 16, each reduced over the 32 lanes of a wave half: lane i returns
+// the maximum of x[i / 2].  Four exchanges halve the number of values (a lane
+// keeps the half that its bit names and receives the other's part of it), the
+// last one joins the pairs: 78 instructions instead of 160 for 16 reductions.
+__device__ __forceinline__ float scatter_max(const float (&x)[16], int lane) {
+    float a[8], b[4], c[2];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x[i]),
+                                                        __builtin_bit_cast(uint32_t, x[i + 8]), false, false);
+        a[i] = __builtin_elementwise_maximum(as_float(s[0]), as_float(s[1]));
+    }
+    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) b[i] = dpp_maximum<0x128>(b3 ? a[i + 4] : a[i], b3 ? a[i] : a[i + 4]);  // row_ror:8
+#pragma unroll
+    for (int i = 0; i < 2; ++i) c[i] = dpp_maximum<0x141>(b2 ? b[i + 2] : b[i], b2 ? b[i] : b[i + 2]);  // row_half_mirror
+    const float d = dpp_maximum<0x4e>(b1 ? c[1] : c[0], b1 ? c[0] : c[1]);  // quad_perm [2,3,0,1]
+    return dpp_maximum<0xb1>(d, d);                                         // quad_perm [1,0,3,2]
 }
 
+// v scaled by a power of two as an fp16 pair; x scale and the remainder are
+// exact, so each part is one mixed fma
+__device__ __forceinline__ void pair_of(float v, float scale, _Float16& hi, _Float16& lo) {
+    hi = static_cast<_Float16>(__builtin_fmaf(v, scale, 0.0f));
+    lo = static_cast<_Float16>(__builtin_fmaf(v, scale, -static_cast<float>(hi)));
+}
 __device__ __forceinline__ void pair8(const float (&v)[8], float scale, half8_t& hi, half8_t& lo) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float x = v[i] * scale;
-        const _Float16 h = static_cast<_Float16>(x);
+        _Float16 h, l;
+        pair_of(v[i], scale, h, l);
         hi[i] = h;
-        lo[i] = static_cast<_Float16>(x - static_cast<float>(h));
+        lo[i] = l;
     }
 }
 
@@ -1665,21 +1693,19 @@ constexpr int kTreeMaxChunks = 64;                // key ranges of a call
 template <int HD, int RT, int OCC>
 __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) {
     constexpr int NC = HD / 16, NN = HD / 32, R = 32 * RT;
-    constexpr int kPart = NN * 8 * 33;  // float4 of a wave's 32 rows, padded per (n, a, g)
-    constexpr int kQ = RT * NC * 64;    // half8 of the query rows' hi (and lo) parts
+    constexpr int VW = NN < 4 ? NN : 4;  // value columns a lane loads at once: column 32 VW (n / VW) + VW li + n % VW
+    constexpr int kPart = HD / 4 * 33;   // float4 of a wave's 32 rows, padded per float4 column
+    constexpr int kQ = RT * NC * 64;     // half8 of the query rows' hi (and lo) parts
     constexpr int kShared = kQ * 2 > kPart * kWaves ? kQ * 2 : kPart * kWaves;
     __shared__ __align__(16) float4 shared[kShared];
     __shared__ float qfac[R];
-    __shared__ __align__(16) float kfac[kWaves][kTreeKeys];
+    __shared__ __align__(16) float kfac[kWaves][kTreeKeys];     // key factors, by key
+    __shared__ __align__(16) float vfac[kWaves][2][kTreeKeys];  // value factors and exponents, by half and register
     __shared__ float2 mls[kWaves][32];
     __shared__ uint32_t interval[kMaxTreeNodes];  // pre | end << 16
     __shared__ uint16_t depth[kMaxTreeNodes];
-    __shared__ float vfac[kWaves][kTreeKeys];     // a tile's value factors, for rows that are not finite
     half8_t* const qhi = reinterpret_cast<half8_t*>(shared);
     half8_t* const qlo = qhi + kQ;
-    // a tile's weights, for value rows that are not finite, behind the query rows
-    float(*const pw)[kTreeKeys][33] = reinterpret_cast<float(*)[kTreeKeys][33]>(shared + 2 * kQ);
-    static_assert((kShared - 2 * kQ) * 4 >= kWaves * kTreeKeys * 33, "room for the weights");
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * R;
@@ -1689,36 +1715,54 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
     const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
     const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
 
-    float kr[NC][8], vr[NN][2][8];
-    // rows past the range are read as its last one (their weights are 0)
+    // Buffer loads bounded by the range's last row: rows past it read as zeros.
+    auto tile_of = [&](const float* base, int t0) {
+        const uint32_t n = static_cast<uint32_t>(min(c1 - t0, kTreeKeys) - 1) * kn + HD;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + static_cast<size_t>(t0) * kn),
+                                                 static_cast<short>(0), static_cast<int32_t>(n * 4), 0x00020000);
+    };
+    float kr[NC][8], vr[NN][16];
+    const uint32_t kat = (static_cast<uint32_t>(li) * kn + 8 * g) * 4, vat = (4 * g * kn + VW * li) * 4;
     auto load_k = [&](int t0) {
-        const float* b = kbase + static_cast<size_t>(t0) * kn;
-        const uint32_t at = static_cast<uint32_t>(min(li, c1 - 1 - t0)) * kn + 8 * g;
+        const auto rs = tile_of(kbase, t0);
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const floatx4 v = *reinterpret_cast<const floatx4*>(b + (at + 16 * c + 4 * h));
+                const auto v = __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<int>(kat + 64 * c + 16 * h), 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) kr[c][4 * h + i] = v[i];
+                for (int i = 0; i < 4; ++i) kr[c][4 * h + i] = as_float(v[i]);
             }
     };
     auto load_v = [&](int t0) {
-        const float* b = vbase + static_cast<size_t>(t0) * kn;
+        const auto rs = tile_of(vbase, t0);
+        uint32_t row = kn * 4;
+        asm volatile("" : "+s"(row));  // (sixteen addresses kept over the loop would cost registers)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int r = 0; r < 16; ++r) {
+            const int at = static_cast<int>(vat + static_cast<uint32_t>(8 * (r >> 2) + (r & 3)) * row);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int key = 16 * c + 4 * g + (i & 3) + 8 * (i >> 2);
-                const uint32_t at = static_cast<uint32_t>(min(key, c1 - 1 - t0)) * kn + li;
+            for (int n = 0; n < NN; n += VW) {
+                if constexpr (VW == 4) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(rs, at + 128 * n, 0, 0);
 #pragma unroll
-                for (int n = 0; n < NN; ++n) vr[n][c][i] = b[at + 32 * n];
+                    for (int i = 0; i < 4; ++i) vr[n + i][r] = as_float(v[i]);
+                } else {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(rs, at + 128 * n, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) vr[n + i][r] = as_float(v[i]);
+                }
             }
+        }
     };
     const int first = c0 + kTreeKeys * wv;
+    // Loads run a tile ahead, a tile's keys while the tile before is in its value
+    // products, its values behind those; at head_dim 256 there are no registers
+    // for that: keys behind the products, values behind the scores.
+    constexpr bool kAhead = HD <= 128;
     if (first < c1) {
         load_k(first);
-        load_v(first);
+        if (kAhead) load_v(first);
     }
 
     // the query rows, 8 threads each: scaled, split and laid out as operands
@@ -1776,15 +1820,29 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
             for (int r = 0; r < 16; ++r) o[rt][n][r] = 0.0f;
     }
 
+    // whether row li of row tile rt sees a key
+    auto sees = [&](int key, int rt) {
+        bool see = key < p.pos0 && key >= lo[rt];
+        if (key >= p.pos0 && key < c1) {
+            const uint32_t iv = interval[key - p.pos0];
+            see = (iv & 0xffffu) <= pre[rt] && pre[rt] < iv >> 16 && p.pos0 + depth[key - p.pos0] >= lo[rt];
+        }
+        return see && key < c1;
+    };
+    int odd_first = c1, odd_last = -1;  // tiles that hold an infinity or a NaN (add_odd_keys below)
     for (int t0 = first; t0 < c1; t0 += kTreeStep) {
+        const int next = t0 + kTreeStep;
         // ---- scores
         float amax = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
             for (int i = 0; i < 8; i += 2) amax = max3_abs(amax, kr[c][i], kr[c][i + 1]);
-        amax = fmaxf(amax, __shfl_xor(amax, 32, 64));
-        const uint64_t infinite = __ballot(amax == __builtin_inff());  // (NaN gives NaN scores by itself)
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, amax),
+                                                            __builtin_bit_cast(uint32_t, amax), false, false);
+            amax = __builtin_elementwise_maximum(as_float(x[0]), as_float(x[1]));
+        }
         const int kf = scale_field(amax);
         if (g == 0) kfac[wv][li] = pow2_field(kf - 7);
         const float ks = pow2_field(254 + 7 - kf);
@@ -1805,51 +1863,48 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
                 st[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, h, st[rt], 0, 0, 0);
             }
         }
-        const int next = t0 + kTreeStep;
-        if (next < c1) load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+        if (!kAhead) load_v(t0);
 
-        // ---- the value rows' powers of two, in the lanes that hold their scores
-        float ve[16], vs[16];
-        uint32_t odd = 0;  // this lane half's value rows that are not finite
-        auto value_factors = [&]() {
+        // ---- the value rows' powers of two: lane i of half g forms register
+        // i / 2's, every lane reads its half's sixteen
+        uint32_t kbad;  // keys that are not finite: none to the products
+        {
+            float b[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                uint32_t b = 0;
+                b[r] = max3_abs(0.0f, vr[0][r], vr[1][r]);
 #pragma unroll
-                for (int n = 0; n < NN; ++n) b = max(b, abs_bits(vr[n][r >> 3][r & 7]));
-                b = dpp_max_u32<0xb1>(b);
-                b = dpp_max_u32<0x4e>(b);
-                b = dpp_max_u32<0x141>(b);
-                b = dpp_max_u32<0x140>(b);
-                b = max(b, static_cast<uint32_t>(__shfl_xor(static_cast<int>(b), 16, 64)));
-                if (b >= 0x7f800000u) odd |= 1u << r;
-                const int f = scale_field(__builtin_bit_cast(float, b));
-                ve[r] = static_cast<float>(f - 127);
-                vs[r] = pow2_field(254 + 14 - f);
+                for (int n = 2; n < NN; n += 2) b[r] = max3_abs(b[r], vr[n][r], vr[n + 1][r]);
             }
-        };
-        value_factors();
-        const bool any_odd = __ballot(odd != 0) != 0;
-        if (any_odd) {
-            // their factors from the elements that are finite, and zeros for the products
-            const uint32_t was = odd;
+            float bm = scatter_max(b, lane);
+            kbad = static_cast<uint32_t>(__ballot(!(amax < __builtin_inff())));
+            const bool vbad = __ballot(!(bm < __builtin_inff())) != 0;
+            if (vbad) {
+                // zeros for the products; the factors from the other elements
 #pragma unroll
-            for (int n = 0; n < NN; ++n)
+                for (int r = 0; r < 16; ++r) {
+                    b[r] = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (abs_bits(vr[n][r >> 3][r & 7]) >= 0x7f800000u) vr[n][r >> 3][r & 7] = 0.0f;
-            value_factors();
-#pragma unroll
-            for (int n = 0; n < NN; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (was >> r & 1) vr[n][r >> 3][r & 7] = 0.0f;
-            odd = was;
+                    for (int n = 0; n < NN; ++n) {
+                        vr[n][r] = fabsf(vr[n][r]) < __builtin_inff() ? vr[n][r] : 0.0f;
+                        b[r] = fmaxf(b[r], fabsf(vr[n][r]));
+                    }
+                }
+                bm = scatter_max(b, lane);
+            }
+            if (vbad || kbad) {
+                odd_first = min(odd_first, t0);
+                odd_last = t0;
+            }
+            const int f = scale_field(bm);
+            vfac[wv][0][16 * g + (li >> 1)] = pow2_field(254 + 14 - f);
+            vfac[wv][1][16 * g + (li >> 1)] = static_cast<float>(f - 127);
         }
 
         // ---- softmax
-        const bool plain = t0 + kTreeKeys <= min(p.pos0, c1) && t0 >= lo_most;
-        float e[RT][16];
+        const bool plain = t0 + kTreeKeys <= min(p.pos0, c1) && t0 >= lo_most && !kbad;
+        half8_t ph[RT][2], pl[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
 #pragma unroll
@@ -1858,82 +1913,84 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
 #pragma unroll
                 for (int b = 0; b < 4; ++b) st[rt][4 * a + b] = st[rt][4 * a + b] * f[b] * qf[rt];
             }
-            if (infinite) {
-                // an infinite key's scores from the elements (inf - inf of its pair says nothing)
-                const int row = min(row0 + 32 * rt + li, rows - 1);
-                const float* q = p.q + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD;
-                for (int j = 0; j < kTreeKeys; ++j)
-                    if (infinite >> j & 1) {
-                        const float* k = kbase + static_cast<size_t>(min(t0 + j, c1 - 1)) * kn;
-                        float s = 0.0f;
-                        for (int d = 0; d < HD; ++d) s += q[d] * k[d];
-                        s *= p.scale * 1.4426950408889634f;
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (8 * (r >> 2) + 4 * g + (r & 3) == j) st[rt][r] = s;
-                    }
-            }
-            if (!plain) {
+            if (!plain)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int key = t0 + 8 * (r >> 2) + 4 * g + (r & 3);
-                    bool see = key < p.pos0 && key >= lo[rt];
-                    if (key >= p.pos0 && key < c1) {
-                        const uint32_t iv = interval[key - p.pos0];
-                        see = (iv & 0xffffu) <= pre[rt] && pre[rt] < iv >> 16 &&
-                              p.pos0 + depth[key - p.pos0] >= lo[rt];
-                    }
-                    if (!(see && key < c1)) st[rt][r] = -__builtin_inff();
+                    const int j = 8 * (r >> 2) + 4 * g + (r & 3);
+                    if (!sees(t0 + j, rt) || (kbad >> j & 1)) st[rt][r] = -__builtin_inff();
                 }
+            float tv[16];
+#pragma unroll
+            for (int a = 0; a < 4; ++a) {
+                const floatx4 f = *reinterpret_cast<const floatx4*>(&vfac[wv][1][16 * g + 4 * a]);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) tv[4 * a + b] = st[rt][4 * a + b] + f[b];
             }
             float mx = -1e30f, mxt = -1e30f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 mx = fmaxf(mx, st[rt][r]);
-                mxt = fmaxf(mxt, st[rt][r] + ve[r]);
+                mxt = fmaxf(mxt, tv[r]);
             }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            mxt = fmaxf(mxt, __shfl_xor(mxt, 32, 64));
+            {
+                const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
+                                                                __builtin_bit_cast(uint32_t, mx), false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mxt),
+                                                                __builtin_bit_cast(uint32_t, mxt), false, false);
+                mx = fmaxf(as_float(x[0]), as_float(x[1]));
+                mxt = fmaxf(as_float(y[0]), as_float(y[1]));
+            }
             const float m2 = fmaxf(m[rt], mx), mt2 = fmaxf(mt[rt], mxt);
-            float sum = 0.0f;
+            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                sum += __builtin_amdgcn_exp2f(st[rt][r] - m2);
-                e[rt][r] = __builtin_amdgcn_exp2f(st[rt][r] + ve[r] - mt2 + 14.0f);
-            }
-            sum += __shfl_xor(sum, 32, 64);
-            l[rt] = l[rt] * __builtin_amdgcn_exp2f(m[rt] - m2) + sum;
-            const float alpha = __builtin_amdgcn_exp2f(mt[rt] - mt2);
-            m[rt] = m2;
-            mt[rt] = mt2;
-#pragma unroll
-            for (int n = 0; n < NN; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[rt][n][r] *= alpha;
-        }
-
-        // ---- weighted values
-        half8_t ph[RT][2], pl[RT][2];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+            for (int r = 0; r < 16; ++r) sum[r & 3] += __builtin_amdgcn_exp2f(st[rt][r] - m2);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float w[8];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = e[rt][8 * c + i];
-                split8(w, ph[rt][c], pl[rt][c]);
+                for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(tv[8 * c + i] - mt2);
+                pair8(w, 16384.0f, ph[rt][c], pl[rt][c]);
+            }
+            float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            {
+                const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, all),
+                                                                __builtin_bit_cast(uint32_t, all), false, false);
+                all = as_float(x[0]) + as_float(x[1]);
+            }
+            l[rt] = l[rt] * __builtin_amdgcn_exp2f(m[rt] - m2) + all;
+            if (__ballot(mt2 > mt[rt])) {
+                const float alpha = __builtin_amdgcn_exp2f(mt[rt] - mt2);
+#pragma unroll
+                for (int n = 0; n < NN; ++n)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[rt][n][r] *= alpha;
+            }
+            m[rt] = m2;
+            mt[rt] = mt2;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (kAhead && next < c1) load_k(next);
+        __builtin_amdgcn_sched_barrier(0);
+
+        // ---- weighted values
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float vs[8];
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+                const floatx4 f = *reinterpret_cast<const floatx4*>(&vfac[wv][0][16 * g + 8 * c + 4 * a]);
+#pragma unroll
+                for (int b = 0; b < 4; ++b) vs[4 * a + b] = f[b];
             }
 #pragma unroll
-        for (int n = 0; n < NN; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
+            for (int n = 0; n < NN; ++n) {
                 half8_t vh, vl;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float x = vr[n][c][i] * vs[8 * c + i];
-                    const _Float16 h = static_cast<_Float16>(x);
+                    _Float16 h, lw;
+                    pair_of(vr[n][8 * c + i], vs[i], h, lw);
                     vh[i] = h;
-                    vl[i] = static_cast<_Float16>(x - static_cast<float>(h));
+                    vl[i] = lw;
                 }
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -1942,36 +1999,47 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
                     o[rt][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[rt][c], o[rt][n], 0, 0, 0);
                 }
             }
-        if (any_odd) {
-            // value rows that are not finite, for the rows that see them.  Bit r
-            // of half g's mask is key 8 (r / 4) + 4 g + r % 4.
-            if (li == 0)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) vfac[wv][8 * (r >> 2) + 4 * g + (r & 3)] = vs[r];
-            const uint32_t odd0 = __builtin_amdgcn_readlane(odd, 0), odd1 = __builtin_amdgcn_readlane(odd, 32);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) pw[wv][8 * (r >> 2) + 4 * g + (r & 3)][li] = e[rt][r];
-                __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes, read back below
-                asm volatile("" ::: "memory");
-                for (int j = 0; j < kTreeKeys; ++j) {
-                    const int r = 4 * (j >> 3) + (j & 3);
-                    if (!(((j >> 2 & 1) ? odd1 : odd0) >> r & 1)) continue;
-                    const float w = pw[wv][j][li], f = vfac[wv][j];
-                    if (w == 0.0f) continue;
-                    const float* v = vbase + static_cast<size_t>(min(t0 + j, c1 - 1)) * kn;
-#pragma unroll
-                    for (int n = 0; n < NN; ++n)
-#pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            o[rt][n][i] += w * (v[32 * n + 8 * (i >> 2) + 4 * g + (i & 3)] * f);
-                }
-                asm volatile("" ::: "memory");
-            }
         }
-        if (next < c1) load_v(next);
+        __builtin_amdgcn_sched_barrier(0);
+        if (next < c1) {
+            if (kAhead) load_v(next);
+            else load_k(next);
+        }
     }
+
+    // What keys and values that are not finite add to the rows that see them, to
+    // this wave's normalised part of row tile rt in LDS: a weight of 0 takes
+    // nothing of a value row, whatever it holds; a key's score is -inf (no
+    // weight), or it makes its row NaN.
+    auto add_odd_keys = [&](int rt) {
+        float* part = reinterpret_cast<float*>(shared + wv * kPart + li);
+        const int row = min(row0 + 32 * rt + li, rows - 1);
+        const float* q = p.q + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD;
+        for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeStep)
+            for (int key = t0; key < min(t0 + kTreeKeys, c1); ++key) {
+                const float* k = kbase + static_cast<size_t>(key) * kn;
+                const float* v = vbase + static_cast<size_t>(key) * kn;
+                bool kodd = false, vodd = false;
+                for (int d = lane; d < HD; d += 64) {
+                    kodd |= !(fabsf(k[d]) < __builtin_inff());
+                    vodd |= !(fabsf(v[d]) < __builtin_inff());
+                }
+                kodd = __ballot(kodd) != 0;
+                vodd = __ballot(vodd) != 0;
+                if (!kodd && !vodd) continue;
+                float s = 0.0f;
+                for (int d = 0; d < HD; ++d) s += q[d] * k[d];
+                s *= p.scale * 1.4426950408889634f;
+                if (!sees(key, rt)) continue;
+                if (kodd) {
+                    if (!(s == -__builtin_inff())) l[rt] = __builtin_nanf("");
+                    continue;
+                }
+                const float w = __builtin_amdgcn_exp2f(s - m[rt]) / l[rt];
+                for (int d = g * (HD / 2); d < (g + 1) * (HD / 2); ++d)
+                    if (w > 0.0f && !(fabsf(v[d]) < __builtin_inff())) part[d / 4 * 33 * 4 + d % 4] += w * v[d];
+            }
+    };
 
     // ---- the waves' parts meet in LDS
     const bool whole = gridDim.z == 1;
@@ -1979,14 +2047,27 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         __syncthreads();  // the query rows, or the parts of the row tile before, are done with
-        const float f = l[rt] > 0.0f || l[rt] != l[rt] ? __builtin_amdgcn_exp2f(mt[rt] - m[rt] - 28.0f) / l[rt] : 0.0f;
+        const float f = l[rt] != 0.0f ? __builtin_amdgcn_exp2f(mt[rt] - m[rt] - 28.0f) / l[rt] : 0.0f;
 #pragma unroll
-        for (int n = 0; n < NN; ++n)
+        for (int a = 0; a < 4; ++a)
 #pragma unroll
-            for (int a = 0; a < 4; ++a)
-                shared[wv * kPart + ((n * 4 + a) * 2 + g) * 33 + li] =
-                    make_float4(o[rt][n][4 * a] * f, o[rt][n][4 * a + 1] * f, o[rt][n][4 * a + 2] * f,
-                                o[rt][n][4 * a + 3] * f);
+            for (int b = 0; b < 4; ++b) {
+                const int at = 8 * a + 4 * g + b, r = 4 * a + b;  // the lane's value row of a column tile
+                if constexpr (VW == 4) {
+#pragma unroll
+                    for (int n = 0; n < NN; n += 4)
+                        shared[wv * kPart + (8 * n + at) * 33 + li] = make_float4(
+                            o[rt][n][r] * f, o[rt][n + 1][r] * f, o[rt][n + 2][r] * f, o[rt][n + 3][r] * f);
+                } else if (b % 2 == 0) {
+                    shared[wv * kPart + at / 2 * 33 + li] =
+                        make_float4(o[rt][0][r] * f, o[rt][1][r] * f, o[rt][0][r + 1] * f, o[rt][1][r + 1] * f);
+                }
+            }
+        if (odd_last >= 0) {
+            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
+            asm volatile("" ::: "memory");
+            add_odd_keys(rt);
+        }
         if (g == 0) mls[wv][li] = make_float2(m[rt], l[rt]);
         __syncthreads();
         for (int i = tid; i < 32 * HD / 4; i += kThreads) {
