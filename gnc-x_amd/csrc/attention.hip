@@ -1690,6 +1690,40 @@ constexpr int kTreeKeys = 32;                     // keys of a tile
 constexpr int kTreeStep = kTreeKeys * kWaves;     // keys of a work-group's step
 constexpr int kTreeMaxChunks = 64;                // key ranges of a call
 
+// What keys and values that are not finite, of keys [t0, t1), add to a query row
+// that sees them: to part, its normalised output in LDS (float4 d / 4 at 33 (d /
+// 4), as the kernels leave it; the halves of a wave take half the columns each),
+// and to its sum l.  A weight of 0 takes nothing of a value row, whatever it
+// holds; an infinite key's score is -inf, no weight, or it makes its row NaN.
+template <int HD, class Sees>
+__device__ __forceinline__ void tree_odd_keys(const TreeParams& p, float* part, const float* q, const float* kbase,
+                                              const float* vbase, uint32_t kn, int t0, int t1, int lane, float m, float& l,
+                                              const Sees& sees) {
+    for (int key = t0; key < t1; ++key) {
+        const float* k = kbase + static_cast<size_t>(key) * kn;
+        const float* v = vbase + static_cast<size_t>(key) * kn;
+        bool kodd = false, vodd = false;
+        for (int d = lane; d < HD; d += 64) {
+            kodd |= !(fabsf(k[d]) < __builtin_inff());
+            vodd |= !(fabsf(v[d]) < __builtin_inff());
+        }
+        kodd = __ballot(kodd) != 0;
+        vodd = __ballot(vodd) != 0;
+        if (!kodd && !vodd) continue;
+        float s = 0.0f;
+        for (int d = 0; d < HD; ++d) s += q[d] * k[d];
+        s *= p.scale * 1.4426950408889634f;
+        if (!sees(key)) continue;
+        if (kodd) {
+            if (!(s == -__builtin_inff())) l = __builtin_nanf("");
+            continue;
+        }
+        const float w = __builtin_amdgcn_exp2f(s - m) / l;
+        for (int d = lane / 32 * (HD / 2); d < (lane / 32 + 1) * (HD / 2); ++d)
+            if (w > 0.0f && !(fabsf(v[d]) < __builtin_inff())) part[d / 4 * 33 * 4 + d % 4] += w * v[d];
+    }
+}
+
 template <int HD, int RT, int OCC>
 __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) {
     constexpr int NC = HD / 16, NN = HD / 32, R = 32 * RT;
@@ -1829,7 +1863,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
         }
         return see && key < c1;
     };
-    int odd_first = c1, odd_last = -1;  // tiles that hold an infinity or a NaN (add_odd_keys below)
+    int odd_first = c1, odd_last = -1;  // tiles that hold an infinity or a NaN (tree_odd_keys)
     for (int t0 = first; t0 < c1; t0 += kTreeStep) {
         const int next = t0 + kTreeStep;
         // ---- scores
@@ -2007,40 +2041,6 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
         }
     }
 
-    // What keys and values that are not finite add to the rows that see them, to
-    // this wave's normalised part of row tile rt in LDS: a weight of 0 takes
-    // nothing of a value row, whatever it holds; a key's score is -inf (no
-    // weight), or it makes its row NaN.
-    auto add_odd_keys = [&](int rt) {
-        float* part = reinterpret_cast<float*>(shared + wv * kPart + li);
-        const int row = min(row0 + 32 * rt + li, rows - 1);
-        const float* q = p.q + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD;
-        for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeStep)
-            for (int key = t0; key < min(t0 + kTreeKeys, c1); ++key) {
-                const float* k = kbase + static_cast<size_t>(key) * kn;
-                const float* v = vbase + static_cast<size_t>(key) * kn;
-                bool kodd = false, vodd = false;
-                for (int d = lane; d < HD; d += 64) {
-                    kodd |= !(fabsf(k[d]) < __builtin_inff());
-                    vodd |= !(fabsf(v[d]) < __builtin_inff());
-                }
-                kodd = __ballot(kodd) != 0;
-                vodd = __ballot(vodd) != 0;
-                if (!kodd && !vodd) continue;
-                float s = 0.0f;
-                for (int d = 0; d < HD; ++d) s += q[d] * k[d];
-                s *= p.scale * 1.4426950408889634f;
-                if (!sees(key, rt)) continue;
-                if (kodd) {
-                    if (!(s == -__builtin_inff())) l[rt] = __builtin_nanf("");
-                    continue;
-                }
-                const float w = __builtin_amdgcn_exp2f(s - m[rt]) / l[rt];
-                for (int d = g * (HD / 2); d < (g + 1) * (HD / 2); ++d)
-                    if (w > 0.0f && !(fabsf(v[d]) < __builtin_inff())) part[d / 4 * 33 * 4 + d % 4] += w * v[d];
-            }
-    };
-
     // ---- the waves' parts meet in LDS
     const bool whole = gridDim.z == 1;
     const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
@@ -2066,7 +2066,11 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
         if (odd_last >= 0) {
             __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
             asm volatile("" ::: "memory");
-            add_odd_keys(rt);
+            const int row = min(row0 + 32 * rt + li, rows - 1);
+            for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeStep)
+                tree_odd_keys<HD>(p, reinterpret_cast<float*>(shared + wv * kPart + li),
+                                  p.q + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD, kbase, vbase, kn,
+                                  t0, min(t0 + kTreeKeys, c1), lane, m[rt], l[rt], [&](int key) { return sees(key, rt); });
         }
         if (g == 0) mls[wv][li] = make_float2(m[rt], l[rt]);
         __syncthreads();
@@ -2095,6 +2099,383 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
             reinterpret_cast<float4*>(dst)[d4] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
             if (!whole && d4 == 0) p.part_ml[prow + 32 * rt + r] = make_float2(M, L);
         }
+    }
+}
+
+// x[i], i < 8, each reduced over a wave half: lane i returns the maximum of
+// x[i / 4] (scatter_max for eight values)
+__device__ __forceinline__ float scatter_max8(const float (&x)[8], int lane) {
+    float a[4], b[2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x[i]),
+                                                        __builtin_bit_cast(uint32_t, x[i + 4]), false, false);
+        a[i] = __builtin_elementwise_maximum(as_float(s[0]), as_float(s[1]));
+    }
+    const bool b3 = lane & 8, b2 = lane & 4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) b[i] = dpp_maximum<0x128>(b3 ? a[i + 2] : a[i], b3 ? a[i] : a[i + 2]);  // row_ror:8
+    const float c = dpp_maximum<0x141>(b2 ? b[1] : b[0], b2 ? b[0] : b[1]);  // row_half_mirror
+    const float d = dpp_maximum<0x4e>(c, c);                                 // quad_perm [2,3,0,1]
+    return dpp_maximum<0xb1>(d, d);                                          // quad_perm [1,0,3,2]
+}
+
+// Rows over waves, for more than 32 query rows of a KV head: a work-group takes
+// 32 RW rows and two 32-key tiles a step, which its waves load, scale, split and
+// lay out in LDS as operands once for all of them (waves 2 s and 2 s + 1 stage
+// tile s).  RW = 4: each wave owns 32 rows and takes both tiles; RW = 2: waves w
+// and w + 2 own the same 32 rows, a tile each, and meet at the end.  The products,
+// weights and factors are those of tree_keys_kernel.  The next step's loads are
+// in flight during this one's products; two work-groups a CU fill each other's
+// waits.
+template <int HD, int RW, int OCC>
+__global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) {
+    constexpr int NC = HD / 16, NN = HD / 32, R = 32 * RW, KW = kWaves / RW;
+    constexpr int VW = NN < 4 ? NN : 4;
+    constexpr int kPart = HD / 4 * 33;
+    constexpr int kTile = NC * 64;  // half8 of a tile's keys' hi (or lo) parts, and of its values'
+    constexpr int kShared = kTile * 8 > kPart * kWaves ? kTile * 8 : kPart * kWaves;
+    __shared__ __align__(16) float4 shared[kShared];
+    __shared__ __align__(16) float kfac[2][kTreeKeys];     // key factors (infinite: a key that is not finite)
+    __shared__ __align__(16) float vfac[2][2][kTreeKeys];  // value factors and exponents, by half and register
+    __shared__ float2 mls[kWaves][32];
+    __shared__ int kodd[2], odd_first, odd_last;
+    __shared__ uint32_t interval[kMaxTreeNodes];
+    __shared__ uint16_t depth[kMaxTreeNodes];
+    half8_t* const khi = reinterpret_cast<half8_t*>(shared);  // [tile][slice][lane]
+    half8_t* const klo = khi + 2 * kTile;
+    half8_t* const vhi = khi + 4 * kTile;                     // [tile][column tile][slice][lane]
+    half8_t* const vlo = khi + 6 * kTile;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * R;
+    const int total = p.pos0 + p.n;
+    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(total, c0 + p.chunk);
+    const uint32_t kn = static_cast<uint32_t>(p.n_kv) * HD;
+    const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
+    const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
+
+    // ---- staging: wave 2 s + c loads keys 16 c .. + 16 of tile s (four lanes a
+    // key, 64 bytes a load) and values of slice c (a lane half a row)
+    const int ts = wv >> 1, tc = wv & 1;
+    auto tile_of = [&](const float* base, int t0) {
+        const int n = min(c1 - t0, kTreeKeys);  // none past the range: every load reads zeros
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + static_cast<size_t>(t0) * kn), static_cast<short>(0),
+                                                 n > 0 ? static_cast<int32_t>((static_cast<uint32_t>(n - 1) * kn + HD) * 4) : 0,
+                                                 0x00020000);
+    };
+    float kst[NC][4], vst[NN][8];
+    const int key4 = 16 * tc + lane / 4, quarter = lane % 4;
+    const uint32_t kat = (static_cast<uint32_t>(key4) * kn + 4 * quarter) * 4;
+    const uint32_t vat = ((16 * tc + 4 * g) * kn + VW * li) * 4;
+    auto prefetch = [&](int t0) {
+        const auto ks = tile_of(kbase, t0 + kTreeKeys * ts), vs = tile_of(vbase, t0 + kTreeKeys * ts);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(ks, static_cast<int>(kat + 64 * c), 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) kst[c][i] = as_float(v[i]);
+        }
+        uint32_t row = kn * 4;
+        asm volatile("" : "+s"(row));  // (eight addresses kept over the loop would cost registers)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int at = static_cast<int>(vat + static_cast<uint32_t>(8 * (r >> 2) + (r & 3)) * row);
+#pragma unroll
+            for (int n = 0; n < NN; n += VW) {
+                if constexpr (VW == 4) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(vs, at + 128 * n, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vst[n + i][r] = as_float(v[i]);
+                } else {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(vs, at + 128 * n, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) vst[n + i][r] = as_float(v[i]);
+                }
+            }
+        }
+    };
+    auto stage = [&](int t0) {
+        float amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) amax = max3_abs(max3_abs(amax, kst[c][0], kst[c][1]), kst[c][2], kst[c][3]);
+        amax = dpp_maximum<0xb1>(amax, amax);
+        amax = dpp_maximum<0x4e>(amax, amax);
+        const bool kbad = !(amax < __builtin_inff());
+        const int kf = scale_field(amax);
+        const float ks = pow2_field(254 + 7 - kf);
+        if (quarter == 0) kfac[ts][key4] = kbad ? __builtin_inff() : pow2_field(kf - 7);
+        // slice c, half quarter / 2, elements 4 (quarter % 2) ..
+        const int kslot = (ts * kTile + (quarter >> 1) * 32 + key4) * 2 + (quarter & 1);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+            half4_t hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                _Float16 h, l;
+                pair_of(kst[c][i], ks, h, l);
+                hi[i] = h;
+                lo[i] = l;
+            }
+            reinterpret_cast<half4_t*>(khi)[kslot + 128 * c] = hi;
+            reinterpret_cast<half4_t*>(klo)[kslot + 128 * c] = lo;
+        }
+        float b[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            b[r] = max3_abs(0.0f, vst[0][r], vst[1][r]);
+#pragma unroll
+            for (int n = 2; n < NN; n += 2) b[r] = max3_abs(b[r], vst[n][r], vst[n + 1][r]);
+        }
+        float bm = scatter_max8(b, lane);
+        const bool vbad = __ballot(!(bm < __builtin_inff())) != 0;
+        if (vbad) {
+            // zeros for the products; the factors from the other elements
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                b[r] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NN; ++n) {
+                    vst[n][r] = fabsf(vst[n][r]) < __builtin_inff() ? vst[n][r] : 0.0f;
+                    b[r] = fmaxf(b[r], fabsf(vst[n][r]));
+                }
+            }
+            bm = scatter_max8(b, lane);
+        }
+        const bool kany = __ballot(kbad) != 0;
+        if ((kany || vbad) && lane == 0) {
+            if (kany) kodd[ts] = t0 + kTreeKeys * ts + 1;  // this step's mark: no step has it again
+            atomicMin(&odd_first, t0 + kTreeKeys * ts);
+            atomicMax(&odd_last, t0 + kTreeKeys * ts);
+        }
+        const int f = scale_field(bm);
+        vfac[ts][0][16 * g + 8 * tc + (li >> 2)] = pow2_field(254 + 14 - f);
+        vfac[ts][1][16 * g + 8 * tc + (li >> 2)] = static_cast<float>(f - 127);
+        float vs[8];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            const floatx4 w = *reinterpret_cast<const floatx4*>(&vfac[ts][0][16 * g + 8 * tc + 4 * a]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) vs[4 * a + i] = w[i];
+        }
+#pragma unroll
+        for (int n = 0; n < NN; ++n) {
+            half8_t hi, lo;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                _Float16 h, l;
+                pair_of(vst[n][i], vs[i], h, l);
+                hi[i] = h;
+                lo[i] = l;
+            }
+            vhi[ts * kTile + (n * 2 + tc) * 64 + lane] = hi;
+            vlo[ts * kTile + (n * 2 + tc) * 64 + lane] = lo;
+        }
+    };
+
+    prefetch(c0);
+    if (tid < 2) kodd[tid] = 0;
+    if (tid == 0) {
+        odd_first = c1;
+        odd_last = -1;
+    }
+    if (c1 > p.pos0)
+        for (int i = tid; i < p.n; i += kThreads) {
+            interval[i] = p.tree.pre[i] | static_cast<uint32_t>(p.tree.end[i]) << 16;
+            depth[i] = p.tree.depth[i];
+        }
+    // this wave's query rows as operands, in registers
+    const int rt = wv % RW, myrow = row0 + 32 * rt + li, srow = min(myrow, rows - 1);
+    const float* const qrow = p.q + (static_cast<size_t>(srow / G) * p.n_heads + hk * G + srow % G) * HD;
+    half8_t qh[NC], ql[NC];
+    float qf;
+    {
+        float x[NC][8], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[c][i] = qrow[16 * c + 8 * g + i];
+                amax = fmaxf(amax, fabsf(x[c][i]));
+            }
+        const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, amax),
+                                                        __builtin_bit_cast(uint32_t, amax), false, false);
+        const int f = scale_field(fmaxf(as_float(y[0]), as_float(y[1])));
+#pragma unroll
+        for (int c = 0; c < NC; ++c) pair8(x[c], pow2_field(254 + 7 - f), qh[c], ql[c]);
+        qf = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
+    }
+    const uint32_t pre = p.tree.pre[srow / G];
+    const int lo = p.sw > 0 ? max(0, p.pos0 + p.tree.depth[srow / G] - p.sw + 1) : 0;
+    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.tree.max_depth - p.sw + 1) : 0;
+    auto sees = [&](int key) {
+        bool see = key < p.pos0 && key >= lo;
+        if (key >= p.pos0 && key < c1) {
+            const uint32_t iv = interval[key - p.pos0];
+            see = (iv & 0xffffu) <= pre && pre < iv >> 16 && p.pos0 + depth[key - p.pos0] >= lo;
+        }
+        return see && key < c1;
+    };
+
+    float m = -1e30f, mt = -1e30f, l = 0.0f;
+    floatx16 o[NN];
+#pragma unroll
+    for (int n = 0; n < NN; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
+
+    auto take_tile = [&](int s, int t0) {
+        floatx16 st;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[r] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const half8_t kh = khi[s * kTile + c * 64 + lane], kl = klo[s * kTile + c * 64 + lane];
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], st, 0, 0, 0);
+        }
+        const bool plain = t0 + kTreeKeys <= min(p.pos0, c1) && t0 >= lo_most && kodd[s] != t0 + 1;
+        float tv[16];
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const floatx4 f = *reinterpret_cast<const floatx4*>(&kfac[s][8 * a + 4 * g]);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) st[4 * a + b] = st[4 * a + b] * f[b] * qf;
+        }
+        if (!plain)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = 8 * (r >> 2) + 4 * g + (r & 3);
+                if (!sees(t0 + j) || kfac[s][j] == __builtin_inff()) st[r] = -__builtin_inff();
+            }
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const floatx4 f = *reinterpret_cast<const floatx4*>(&vfac[s][1][16 * g + 4 * a]);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) tv[4 * a + b] = st[4 * a + b] + f[b];
+        }
+        float mx = -1e30f, mxt = -1e30f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            mx = fmaxf(mx, st[r]);
+            mxt = fmaxf(mxt, tv[r]);
+        }
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
+                                                            __builtin_bit_cast(uint32_t, mx), false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mxt),
+                                                            __builtin_bit_cast(uint32_t, mxt), false, false);
+            mx = fmaxf(as_float(x[0]), as_float(x[1]));
+            mxt = fmaxf(as_float(y[0]), as_float(y[1]));
+        }
+        const float m2 = fmaxf(m, mx), mt2 = fmaxf(mt, mxt);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[r & 3] += __builtin_amdgcn_exp2f(st[r] - m2);
+        half8_t ph[2], pl[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(tv[8 * c + i] - mt2);
+            pair8(w, 16384.0f, ph[c], pl[c]);
+        }
+        float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        {
+            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, all),
+                                                            __builtin_bit_cast(uint32_t, all), false, false);
+            all = as_float(x[0]) + as_float(x[1]);
+        }
+        l = l * __builtin_amdgcn_exp2f(m - m2) + all;
+        if (__ballot(mt2 > mt)) {
+            const float alpha = __builtin_amdgcn_exp2f(mt - mt2);
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
+        }
+        m = m2;
+        mt = mt2;
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const half8_t vh = vhi[s * kTile + (n * 2 + c) * 64 + lane], vl = vlo[s * kTile + (n * 2 + c) * 64 + lane];
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[c], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[c], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[c], o[n], 0, 0, 0);
+            }
+    };
+
+    __syncthreads();  // the marks' first values, the tree
+    for (int t0 = c0; t0 < c1; t0 += 2 * kTreeKeys) {
+        stage(t0);
+        __syncthreads();
+        if (t0 + 2 * kTreeKeys < c1) prefetch(t0 + 2 * kTreeKeys);
+        if constexpr (KW == 2) {
+            if (t0 + kTreeKeys * (wv / RW) < c1) take_tile(wv / RW, t0 + kTreeKeys * (wv / RW));
+        } else {
+            take_tile(0, t0);
+            if (t0 + kTreeKeys < c1) take_tile(1, t0 + kTreeKeys);
+        }
+        __syncthreads();  // every wave is done with the operands
+    }
+
+    // ---- the parts, normalised, through LDS
+    const bool whole = gridDim.z == 1;
+    const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
+    const float f = l != 0.0f ? __builtin_amdgcn_exp2f(mt - m - 28.0f) / l : 0.0f;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int at = 8 * a + 4 * g + b, r = 4 * a + b;
+            if constexpr (VW == 4) {
+#pragma unroll
+                for (int n = 0; n < NN; n += 4)
+                    shared[wv * kPart + (8 * n + at) * 33 + li] =
+                        make_float4(o[n][r] * f, o[n + 1][r] * f, o[n + 2][r] * f, o[n + 3][r] * f);
+            } else if (b % 2 == 0) {
+                shared[wv * kPart + at / 2 * 33 + li] =
+                    make_float4(o[0][r] * f, o[1][r] * f, o[0][r + 1] * f, o[1][r + 1] * f);
+            }
+        }
+    if (odd_last >= 0) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
+        asm volatile("" ::: "memory");
+        float* part = reinterpret_cast<float*>(shared + wv * kPart + li);
+        for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeKeys)
+            if (KW == 1 || (t0 - c0) / kTreeKeys % 2 == wv / RW)
+                tree_odd_keys<HD>(p, part, qrow, kbase, vbase, kn, t0, min(t0 + kTreeKeys, c1), lane, m, l, sees);
+    }
+    if (g == 0) mls[wv][li] = make_float2(m, l);
+    __syncthreads();
+    for (int i = tid; i < R * HD / 4; i += kThreads) {
+        const int r = i / (HD / 4), d4 = i % (HD / 4), row = row0 + r;
+        if (row >= rows) break;
+        float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < KW; ++w) M = fmaxf(M, mls[r / 32 + RW * w][r % 32].x);
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+            const float2 ml = mls[r / 32 + RW * w][r % 32];
+            const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
+            const float4 v = shared[(r / 32 + RW * w) * kPart + d4 * 33 + r % 32];
+            L += wt;
+            if (wt != 0.0f) {
+                x[0] += wt * v.x;
+                x[1] += wt * v.y;
+                x[2] += wt * v.z;
+                x[3] += wt * v.w;
+            }
+        }
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        float* dst = whole ? p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD
+                           : p.part_o + (prow + r) * HD;
+        reinterpret_cast<float4*>(dst)[d4] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        if (!whole && d4 == 0) p.part_ml[prow + r] = make_float2(M, L);
     }
 }
 
@@ -2143,36 +2524,39 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams p, int3
         make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
 }
 
-// The split of a call: row tiles a wave, keys a work-group, key ranges.
+// The split of a call: 32 row tiles a work-group (1: keys over its waves),
+// keys a work-group, key ranges.
 struct TreePlan {
-    int32_t rt, first, chunk, chunks, rows_pad;
+    int32_t tiles, first, chunk, chunks, rows_pad;
 };
 
 TreePlan tree_plan(const TreeArgs& a) {
     TreePlan pl;
     const int32_t rows = a.n * (a.n_heads / a.n_kv_heads);
-    pl.rt = rows > 32 && a.head_dim <= 128 ? 2 : 1;
-    const int32_t groups = (rows + 32 * pl.rt - 1) / (32 * pl.rt);
-    pl.rows_pad = groups * 32 * pl.rt;
+    pl.tiles = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+    const int32_t groups = (rows + 32 * pl.tiles - 1) / (32 * pl.tiles);
+    pl.rows_pad = groups * 32 * pl.tiles;
     pl.first = a.sliding_window > 0 ? std::max(0, a.pos0 - a.sliding_window + 1) : 0;
-    const int64_t keys = static_cast<int64_t>(a.pos0) + a.n - pl.first;
-    // one work-group a CU (two of one row tile at head_dim up to 128 share one)
-    const int64_t want = std::max<int64_t>(1, (pl.rt == 1 && a.head_dim <= 128 ? 512 : 256) / (groups * a.n_kv_heads));
-    const int64_t steps = (keys + kTreeStep - 1) / kTreeStep;
-    const int64_t per = (steps + std::min<int64_t>(want, kTreeMaxChunks) - 1) / std::min<int64_t>(want, kTreeMaxChunks);
-    pl.chunk = static_cast<int32_t>(per * kTreeStep);
+    const int64_t keys = static_cast<int64_t>(a.pos0) + a.n - pl.first, step = pl.tiles == 1 ? kTreeStep : 2 * kTreeKeys;
+    // work-groups that share the CUs: two each, one at head_dim 256
+    const int64_t want = std::max<int64_t>(1, (a.head_dim <= 128 ? 512 : 256) / (static_cast<int64_t>(groups) * a.n_kv_heads));
+    const int64_t steps = (keys + step - 1) / step, ranges = std::min<int64_t>(want, kTreeMaxChunks);
+    const int64_t per = (steps + ranges - 1) / ranges;
+    pl.chunk = static_cast<int32_t>(per * step);
     pl.chunks = static_cast<int32_t>((steps + per - 1) / per);
     return pl;
 }
 
-template <int HD, int RT, int OCC>
-hipError_t launch_tree_keys(const TreeParams& p, const TreePlan& pl, hipStream_t stream) {
+template <int HD, int OCC>
+hipError_t launch_tree(const TreeParams& p, const TreePlan& pl, hipStream_t stream) {
     const int heads = p.n_heads + p.n_kv;
     hipLaunchKernelGGL(tree_prologue_kernel<HD>, dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((tree_keys_kernel<HD, RT, OCC>), dim3(p.n_kv, pl.rows_pad / (32 * RT), pl.chunks), dim3(kThreads), 0,
-                       stream, p);
+    const dim3 grid(p.n_kv, pl.rows_pad / (32 * pl.tiles), pl.chunks);
+    if (pl.tiles == 1) hipLaunchKernelGGL((tree_keys_kernel<HD, 1, OCC>), grid, dim3(kThreads), 0, stream, p);
+    else if (pl.tiles == 2) hipLaunchKernelGGL((tree_rows_kernel<HD, 2, OCC>), grid, dim3(kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((tree_rows_kernel<HD, 4, OCC>), grid, dim3(kThreads), 0, stream, p);
     e = hipGetLastError();
     if (e != hipSuccess || pl.chunks == 1) return e;
     const int64_t n = static_cast<int64_t>(p.n) * (p.n_heads / p.n_kv) * HD / 4;
@@ -2246,12 +2630,10 @@ hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, void*
     p.rows_pad = pl.rows_pad;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.chunks) * a.n_kv_heads * pl.rows_pad * a.head_dim);
-    switch (a.head_dim * 4 + pl.rt) {
-    case 64 * 4 + 1: return launch_tree_keys<64, 1, 2>(p, pl, stream);
-    case 64 * 4 + 2: return launch_tree_keys<64, 2, 2>(p, pl, stream);
-    case 128 * 4 + 1: return launch_tree_keys<128, 1, 2>(p, pl, stream);
-    case 128 * 4 + 2: return launch_tree_keys<128, 2, 1>(p, pl, stream);
-    case 256 * 4 + 1: return launch_tree_keys<256, 1, 1>(p, pl, stream);
+    switch (a.head_dim) {
+    case 64: return launch_tree<64, 2>(p, pl, stream);
+    case 128: return launch_tree<128, 2>(p, pl, stream);
+    case 256: return launch_tree<256, 1>(p, pl, stream);
     default: return hipErrorInvalidValue;
     }
 }
