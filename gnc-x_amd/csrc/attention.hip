@@ -1607,70 +1607,68 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p) {
     }
 }
 
-// The products on the fp16 matrix cores, keys over waves.  A work-group owns 32
-// RT query rows (node, head) of one KV head and a range of keys; each of its
-// waves walks every fourth 32-key tile of the range by itself, with the tile's
-// K and V straight from memory into the registers that the products take, so
-// the loop has no barrier and every K/V byte is read once per 32 RT rows.
-//   S^T = K Q^T   v_mfma_f32_32x32x16_f16, operands as fp16 pairs, three
-//                 products a slice (hi hi, hi lo, lo hi: 2^-22 of the product);
-//                 lane (i, g) ends up with query row i's scores of the 16 keys
-//                 8 a + 4 g + b
-//   O^T += V^T P^T  with P from those registers, and O of row i in lane (i, .):
-//                 the softmax factors of a row never cross lanes
-// Pairs hold values of any size: every key, value and query row is scaled by a
-// power of two of its own.  A key's and a query's come back as factors of the
-// scores.  A value row's 2^e_j goes into its weight: with t_j = s_j + e_j the
-// weights of O are 2^(t_j - max t + 14), those of the sum l 2^(s_j - max s), two
-// running maxima a row, so a row's precision hangs on its largest term alone
-// and not on rows it does not see.  A value row that is not finite takes no part
-// in the products (0 times it would be NaN for the nodes that do not see it) and
-// is added lane by lane; so are the scores of an infinite key.
+// The products on the fp16 matrix cores.  Both kernels below compute, per 32-key
+// tile and 32 query rows (node, head) of one KV head,
+//   S^T = K Q^T      v_mfma_f32_32x32x16_f16, operands as fp16 pairs, three
+//                    products a slice (hi hi, hi lo, lo hi: 2^-22 of the product);
+//                    lane (i, g) ends up with query row i's scores of the 16 keys
+//                    8 a + 4 g + b
+//   O^T += V^T P^T   with P from those registers, and O of row i in lane (i, .):
+//                    the softmax factors of a row never cross lanes
+// Pairs hold 22 bits of values down to 2^-17 of their group's largest, and
+// values of any size are brought there by powers of two: one for a query row,
+// one for the keys and one for the values of a group (a tile, or half of it).
+// The keys' and the row's come back as a factor of the scores.  The values' 2^e
+// goes into the weights: those of O are 2^(s + e - max (s + e)), those of the sum
+// l 2^(s - max s), two running maxima a row, so that what a row does not see has
+// no say in its precision.
+// "Odd" keys, whose key or value row is not finite or lies more than 2^-14 below
+// its group's largest, are kept out of the products (0 times an infinity would be
+// NaN for the rows that do not see it) and added element by element at the end:
+// in real caches there are none.
 // Parts are left normalised, o_part = sum w v / sum w, with (m, l) beside them:
 // no sum of large values can overflow between the kernels.  The reference's
-// 1e-12 beside a sum l >= 1 is below fp32's rounding and left out.
+// 1e-12 beside a sum l > 1/2 is below fp32's rounding and left out.
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 // (by value: a bit cast of a vector's element in place takes the first element)
 __device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
-// 2^k as the exponent field of a float; k in [-126, 127]
+__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+// the float of exponent field `field` (2^(field - 127))
 __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_cast(float, field << 23); }
-// the exponent field of |x|'s power of two, kept where 2^(+-(14 + e)) are normal
+// amax's exponent field, kept where 2^(+-(14 + e)) are normal floats
 __device__ __forceinline__ int scale_field(float amax) {
-    const int f = static_cast<int>(__builtin_bit_cast(uint32_t, amax) >> 23) & 0xff;
+    const int f = static_cast<int>(as_bits(amax) >> 23) & 0xff;
     return min(max(f, 30), 254);
 }
 // max(m, |a|, |b|), NaN if one is
 __device__ __forceinline__ float max3_abs(float m, float a, float b) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(m, fabsf(a)), fabsf(b));
 }
+// max of v and of another lane's `of`, NaN if one is
 template <int CTRL>
 __device__ __forceinline__ float dpp_maximum(float v, float of) {
     const int o = __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, of), CTRL, 0xf, 0xf, false);
     return __builtin_elementwise_maximum(v, __builtin_bit_cast(float, o));
 }
-// x[r], r < 16, each reduced over the 32 lanes of a wave half: lane i returns
-// the maximum of x[i / 2].  Four exchanges halve the number of values (a lane
-// keeps the half that its bit names and receives the other's part of it), the
-// last one joins the pairs: 78 instructions instead of 160 for 16 reductions.
-__device__ __forceinline__ float scatter_max(const float (&x)[16], int lane) {
-    float a[8], b[4], c[2];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x[i]),
-                                                        __builtin_bit_cast(uint32_t, x[i + 8]), false, false);
-        a[i] = __builtin_elementwise_maximum(as_float(s[0]), as_float(s[1]));
-    }
-    const bool b3 = lane & 8, b2 = lane & 4, b1 = lane & 2;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) b[i] = dpp_maximum<0x128>(b3 ? a[i + 4] : a[i], b3 ? a[i] : a[i + 4]);  // row_ror:8
-#pragma unroll
-    for (int i = 0; i < 2; ++i) c[i] = dpp_maximum<0x141>(b2 ? b[i + 2] : b[i], b2 ? b[i] : b[i + 2]);  // row_half_mirror
-    const float d = dpp_maximum<0x4e>(b1 ? c[1] : c[0], b1 ? c[0] : c[1]);  // quad_perm [2,3,0,1]
-    return dpp_maximum<0xb1>(d, d);                                         // quad_perm [1,0,3,2]
+// f of the two halves' values, in every lane
+template <class F>
+__device__ __forceinline__ float across_halves(float v, F&& f) {
+    const auto x = __builtin_amdgcn_permlane32_swap(as_bits(v), as_bits(v), false, false);
+    return f(as_float(x[0]), as_float(x[1]));
+}
+__device__ __forceinline__ float maximum_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// the maximum over the wave in every lane, NaN if one is
+__device__ __forceinline__ float wave_maximum(float v) {
+    v = dpp_maximum<0xb1>(v, v);
+    v = dpp_maximum<0x4e>(v, v);
+    v = dpp_maximum<0x141>(v, v);
+    v = dpp_maximum<0x140>(v, v);
+    const auto x = __builtin_amdgcn_permlane16_swap(as_bits(v), as_bits(v), false, false);
+    return across_halves(maximum_of(as_float(x[0]), as_float(x[1])), maximum_of);
 }
 
-// v scaled by a power of two as an fp16 pair; x scale and the remainder are
+// v scaled by a power of two as an fp16 pair; v scale and the remainder are
 // exact, so each part is one mixed fma
 __device__ __forceinline__ void pair_of(float v, float scale, _Float16& hi, _Float16& lo) {
     hi = static_cast<_Float16>(__builtin_fmaf(v, scale, 0.0f));
@@ -1686,70 +1684,207 @@ __device__ __forceinline__ void pair8(const float (&v)[8], float scale, half8_t&
     }
 }
 
-constexpr int kTreeKeys = 32;                     // keys of a tile
-constexpr int kTreeStep = kTreeKeys * kWaves;     // keys of a work-group's step
-constexpr int kTreeMaxChunks = 64;                // key ranges of a call
+constexpr int kTreeKeys = 32;                  // keys of a tile
+constexpr int kTreeStep = kTreeKeys * kWaves;  // keys of a work-group's step, keys over waves
+constexpr int kTreeMaxChunks = 64;             // key ranges of a call
+constexpr float kOddBelow = 1.0f / 16384.0f;
 
-// What keys and values that are not finite, of keys [t0, t1), add to a query row
-// that sees them: to part, its normalised output in LDS (float4 d / 4 at 33 (d /
-// 4), as the kernels leave it; the halves of a wave take half the columns each),
-// and to its sum l.  A weight of 0 takes nothing of a value row, whatever it
-// holds; an infinite key's score is -inf, no weight, or it makes its row NaN.
-template <int HD, class Sees>
-__device__ __forceinline__ void tree_odd_keys(const TreeParams& p, float* part, const float* q, const float* kbase,
-                                              const float* vbase, uint32_t kn, int t0, int t1, int lane, float m, float& l,
-                                              const Sees& sees) {
-    for (int key = t0; key < t1; ++key) {
-        const float* k = kbase + static_cast<size_t>(key) * kn;
-        const float* v = vbase + static_cast<size_t>(key) * kn;
-        bool kodd = false, vodd = false;
-        for (int d = lane; d < HD; d += 64) {
-            kodd |= !(fabsf(k[d]) < __builtin_inff());
-            vodd |= !(fabsf(v[d]) < __builtin_inff());
+// whether a row of the largest element `row` is odd in a group whose largest
+// finite row has `top`
+__device__ __forceinline__ bool is_odd(float row, float top) {
+    return !(row < __builtin_inff()) || (row > 0.0f && row < top * kOddBelow);
+}
+
+// The tree's part in a kernel's LDS and a query row's place in it.
+struct TreeShared {
+    uint32_t interval[kMaxTreeNodes];  // pre | end << 16
+    uint16_t depth[kMaxTreeNodes];
+};
+__device__ __forceinline__ void load_tree(const TreeParams& p, TreeShared& t) {
+    for (int i = threadIdx.x; i < p.n; i += kThreads) {
+        t.interval[i] = p.tree.pre[i] | static_cast<uint32_t>(p.tree.end[i]) << 16;
+        t.depth[i] = p.tree.depth[i];
+    }
+}
+struct RowPlace {
+    uint32_t pre;
+    int lo;  // first position of its window
+};
+__device__ __forceinline__ RowPlace place_of(const TreeParams& p, int node) {
+    return {p.tree.pre[node], p.sw > 0 ? max(0, p.pos0 + p.tree.depth[node] - p.sw + 1) : 0};
+}
+// whether a query row sees a key of a range that ends at c1
+__device__ __forceinline__ bool sees_key(const TreeParams& p, const TreeShared& t, const RowPlace& at, int key, int c1) {
+    bool see = key < p.pos0 && key >= at.lo;
+    if (key >= p.pos0 && key < c1) {
+        const uint32_t iv = t.interval[key - p.pos0];
+        see = (iv & 0xffffu) <= at.pre && at.pre < iv >> 16 && p.pos0 + t.depth[key - p.pos0] >= at.lo;
+    }
+    return see && key < c1;
+}
+
+// One query row a lane: its running maxima of s and of s + e, and its sum.  The
+// maxima are rounded up to whole numbers, so that every factor that brings parts
+// to another maximum is a power of two and rounds nothing.
+struct RowState {
+    float m, mt, l;
+};
+// The softmax of a tile's scores: st (raw products, key factors kf, query factor
+// qf) in two halves of eight, half h with the values' exponent ve[h].  Leaves the
+// weights as pairs and returns what O so far is to be multiplied with (1: nothing).
+__device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&ve)[2], RowState& s, half8_t (&ph)[2],
+                                              half8_t (&pl)[2]) {
+    float mx[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        mx[h] = -1e30f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mx[h] = fmaxf(mx[h], st[8 * h + i]);
+    }
+    const auto larger = [](float a, float b) { return fmaxf(a, b); };
+    const float m2 = fmaxf(s.m, ceilf(across_halves(fmaxf(mx[0], mx[1]), larger)));
+    // (a half without a visible key, mx -1e30, has no say)
+    const float mt2 = fmaxf(s.mt, ceilf(across_halves(fmaxf(mx[0] + ve[0], mx[1] + ve[1]), larger)));
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        float e[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(st[8 * h + i] - m2);
+            sum[i & 1] += e[i];
         }
-        kodd = __ballot(kodd) != 0;
-        vodd = __ballot(vodd) != 0;
-        if (!kodd && !vodd) continue;
-        float s = 0.0f;
-        for (int d = 0; d < HD; ++d) s += q[d] * k[d];
-        s *= p.scale * 1.4426950408889634f;
-        if (!sees(key)) continue;
-        if (kodd) {
-            if (!(s == -__builtin_inff())) l = __builtin_nanf("");
-            continue;
+        // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), the second capped: it
+        // passes 2^126 only where the first is 0
+        pair8(e, __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f)), ph[h], pl[h]);
+    }
+    s.l = s.l * __builtin_amdgcn_exp2f(s.m - m2) +
+          across_halves(sum[0] + sum[1], [](float a, float b) { return a + b; });
+    const float alpha = __builtin_amdgcn_exp2f(s.mt - mt2);
+    s.m = m2;
+    s.mt = mt2;
+    return alpha;
+}
+
+// Adds the odd keys of [t0, t0 + GROUP) (below c1) to a query row: to part, its
+// normalised output in LDS (float4 d / 4 at 33 (d / 4); the halves of a wave take
+// half of the columns each), and to its state.  The keys are found again by the
+// rule that kept them out of the products.  A weight of 0 takes nothing from a
+// row, whatever it holds.
+template <int HD, int GROUP>
+__device__ void add_odd_keys(const TreeParams& p, const TreeShared& tree, const RowPlace& at, float* part, const float* q,
+                             const float* kbase, const float* vbase, uint32_t kn, int t0, int c1, int lane, RowState& s) {
+    // lane = key (GROUP of them), over its row
+    const bool in = lane % GROUP + t0 < c1;
+    float kmax = 0.0f, vmax = 0.0f;
+    const size_t mine = static_cast<size_t>(min(t0 + lane % GROUP, c1 - 1)) * kn;
+    for (int d = 0; d < HD; ++d) {
+        kmax = maximum_of(kmax, fabsf(kbase[mine + d]));
+        vmax = maximum_of(vmax, fabsf(vbase[mine + d]));
+    }
+    const float ktop = wave_max(in && kmax < __builtin_inff() ? kmax : 0.0f);
+    const float vtop = wave_max(in && vmax < __builtin_inff() ? vmax : 0.0f);
+    const uint64_t odd = __ballot(in && lane < GROUP && (is_odd(kmax, ktop) || is_odd(vmax, vtop)));
+    for (int j = 0; j < GROUP; ++j) {
+        if (!(odd >> j & 1)) continue;
+        const float* k = kbase + static_cast<size_t>(t0 + j) * kn;
+        const float* v = vbase + static_cast<size_t>(t0 + j) * kn;
+        float x = 0.0f;
+        for (int d = 0; d < HD; ++d) x += q[d] * k[d];
+        x *= p.scale * 1.4426950408889634f;
+        if (!sees_key(p, tree, at, t0 + j, c1) || x == -__builtin_inff()) continue;
+        const float m2 = fmaxf(s.m, ceilf(x)), a = s.l * __builtin_amdgcn_exp2f(s.m - m2), w = __builtin_amdgcn_exp2f(x - m2);
+        s.m = m2;
+        s.l = a + w;
+        const float fa = a / s.l, fw = w / s.l;
+        for (int d = lane / 32 * (HD / 2); d < (lane / 32 + 1) * (HD / 2); ++d) {
+            float& o = part[d / 4 * 33 * 4 + d % 4];
+            o = (fa != 0.0f ? o * fa : 0.0f) + (fw != 0.0f ? fw * v[d] : 0.0f);
         }
-        const float w = __builtin_amdgcn_exp2f(s - m) / l;
-        for (int d = lane / 32 * (HD / 2); d < (lane / 32 + 1) * (HD / 2); ++d)
-            if (w > 0.0f && !(fabsf(v[d]) < __builtin_inff())) part[d / 4 * 33 * 4 + d % 4] += w * v[d];
     }
 }
 
-template <int HD, int RT, int OCC>
+// the wave's normalised part to LDS: float4 column d4 of row li at 33 d4 + li
+template <int NN>
+__device__ __forceinline__ void store_part(float4* part, const floatx16 (&o)[NN], const RowState& s, int li, int g) {
+    const float f = s.l != 0.0f ? __builtin_amdgcn_exp2f(s.mt - s.m - 28.0f) / s.l : 0.0f;
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int at = 8 * a + 4 * g + b, r = 4 * a + b;  // the lane's column of a column tile
+            if constexpr (NN >= 4) {
+#pragma unroll
+                for (int n = 0; n < NN; n += 4)
+                    part[(8 * n + at) * 33 + li] = make_float4(o[n][r] * f, o[n + 1][r] * f, o[n + 2][r] * f, o[n + 3][r] * f);
+            } else if (b % 2 == 0) {
+                part[at / 2 * 33 + li] = make_float4(o[0][r] * f, o[1][r] * f, o[0][r + 1] * f, o[1][r + 1] * f);
+            }
+        }
+}
+
+// Rows of 32 query rows' parts in LDS (parts of a row `stride` float4 and one
+// `per` waves apart, N of them) joined and written: to the output, or as this key
+// range's part.
+template <int HD, int N>
+__device__ __forceinline__ void join_parts(const TreeParams& p, const float4* shared, const float2 (*mls)[32], int per, int tiles,
+                                           int row0, int hk, int G, int rows) {
+    constexpr int kPart = HD / 4 * 33;
+    const bool whole = gridDim.z == 1;
+    const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
+    for (int i = threadIdx.x; i < 32 * tiles * HD / 4; i += kThreads) {
+        const int r = i / (HD / 4), d4 = i % (HD / 4), row = row0 + r;
+        if (row >= rows) break;
+        float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < N; ++w) M = fmaxf(M, mls[r / 32 + per * w][r % 32].x);
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+            const float2 ml = mls[r / 32 + per * w][r % 32];
+            const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
+            const float4 v = shared[(r / 32 + per * w) * kPart + d4 * 33 + r % 32];
+            L += wt;
+            if (wt != 0.0f) {  // (a part without a key has nothing to add)
+                x[0] += wt * v.x;
+                x[1] += wt * v.y;
+                x[2] += wt * v.z;
+                x[3] += wt * v.w;
+            }
+        }
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        float* dst = whole ? p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD
+                           : p.part_o + (prow + r) * HD;
+        reinterpret_cast<float4*>(dst)[d4] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        if (!whole && d4 == 0) p.part_ml[prow + r] = make_float2(M, L);
+    }
+}
+
+// Keys over waves, for up to 32 query rows of a KV head: each wave of a work-group
+// walks every fourth 32-key tile of its range by itself, with the tile's K and V
+// straight from memory into the registers that the products take, so the loop has
+// no barrier and every K/V byte is read once.  Buffer loads are bounded by the
+// range's last row: rows past it read as zeros.
+template <int HD, int OCC>
 __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) {
-    constexpr int NC = HD / 16, NN = HD / 32, R = 32 * RT;
+    constexpr int NC = HD / 16, NN = HD / 32;
     constexpr int VW = NN < 4 ? NN : 4;  // value columns a lane loads at once: column 32 VW (n / VW) + VW li + n % VW
     constexpr int kPart = HD / 4 * 33;   // float4 of a wave's 32 rows, padded per float4 column
-    constexpr int kQ = RT * NC * 64;     // half8 of the query rows' hi (and lo) parts
-    constexpr int kShared = kQ * 2 > kPart * kWaves ? kQ * 2 : kPart * kWaves;
-    __shared__ __align__(16) float4 shared[kShared];
-    __shared__ float qfac[R];
-    __shared__ __align__(16) float kfac[kWaves][kTreeKeys];     // key factors, by key
-    __shared__ __align__(16) float vfac[kWaves][2][kTreeKeys];  // value factors and exponents, by half and register
+    constexpr int kQ = NC * 64;          // half8 of the query rows' hi (and lo) parts
+    static_assert(kQ * 2 <= kPart * kWaves, "the query rows fit where the parts go");
+    __shared__ __align__(16) float4 shared[kPart * kWaves];
+    __shared__ float qfac[32];
     __shared__ float2 mls[kWaves][32];
-    __shared__ uint32_t interval[kMaxTreeNodes];  // pre | end << 16
-    __shared__ uint16_t depth[kMaxTreeNodes];
+    __shared__ TreeShared tree;
     half8_t* const qhi = reinterpret_cast<half8_t*>(shared);
     half8_t* const qlo = qhi + kQ;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * R;
-    const int total = p.pos0 + p.n;
-    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(total, c0 + p.chunk);
+    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * 32;
+    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(p.pos0 + p.n, c0 + p.chunk);
     const uint32_t kn = static_cast<uint32_t>(p.n_kv) * HD;
     const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
     const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
 
-    // Buffer loads bounded by the range's last row: rows past it read as zeros.
     auto tile_of = [&](const float* base, int t0) {
         const uint32_t n = static_cast<uint32_t>(min(c1 - t0, kTreeKeys) - 1) * kn + HD;
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + static_cast<size_t>(t0) * kn),
@@ -1800,9 +1935,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
     }
 
     // the query rows, 8 threads each: scaled, split and laid out as operands
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = row0 + 32 * rt + tid / 8, j = tid % 8;
+    {
+        const int r = row0 + tid / 8, j = tid % 8;
         float x[HD / 64][8], amax = 0.0f;
         const float* src = p.q + (static_cast<size_t>(r < rows ? r / G : 0) * p.n_heads + hk * G + r % G) * HD + j * (HD / 8);
 #pragma unroll
@@ -1812,228 +1946,154 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
                 x[u][i] = r < rows ? src[8 * u + i] : 0.0f;
                 amax = fmaxf(amax, fabsf(x[u][i]));
             }
-        amax = group8_max(amax);
-        const int f = scale_field(amax);
+        const int f = scale_field(group8_max(amax));
 #pragma unroll
         for (int u = 0; u < HD / 64; ++u) {
             half8_t h, l;
             pair8(x[u], pow2_field(254 + 7 - f), h, l);
-            const int unit = j * (HD / 64) + u, at = (rt * NC + unit / 2) * 64 + 32 * (unit & 1) + tid / 8;
+            const int unit = j * (HD / 64) + u, at = unit / 2 * 64 + 32 * (unit & 1) + tid / 8;
             qhi[at] = h;
             qlo[at] = l;
         }
-        if (j == 0) qfac[32 * rt + tid / 8] = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
+        if (j == 0) qfac[tid / 8] = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
     }
-    if (c1 > p.pos0)
-        for (int i = tid; i < p.n; i += kThreads) {
-            interval[i] = p.tree.pre[i] | static_cast<uint32_t>(p.tree.end[i]) << 16;
-            depth[i] = p.tree.depth[i];
-        }
-    // this lane's rows: their place in the tree and first visible position
-    uint32_t pre[RT];
-    int lo[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int t = min(row0 + 32 * rt + li, rows - 1) / G;
-        pre[rt] = p.tree.pre[t];
-        lo[rt] = p.sw > 0 ? max(0, p.pos0 + p.tree.depth[t] - p.sw + 1) : 0;
-    }
+    if (c1 > p.pos0) load_tree(p, tree);
+    const int myrow = min(row0 + li, rows - 1);
+    const RowPlace place = place_of(p, myrow / G);
     const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.tree.max_depth - p.sw + 1) : 0;
     __syncthreads();
 
-    float m[RT], mt[RT], l[RT], qf[RT];
-    floatx16 o[RT][NN];
+    RowState s{-1e30f, -1e30f, 0.0f};
+    const float qf = qfac[li];
+    floatx16 o[NN];
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = mt[rt] = -1e30f;
-        l[rt] = 0.0f;
-        qf[rt] = qfac[32 * rt + li];
+    for (int n = 0; n < NN; ++n)
 #pragma unroll
-        for (int n = 0; n < NN; ++n)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) o[rt][n][r] = 0.0f;
-    }
+        for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
+    int odd_first = c1, odd_last = -1;  // tiles that hold odd keys
 
-    // whether row li of row tile rt sees a key
-    auto sees = [&](int key, int rt) {
-        bool see = key < p.pos0 && key >= lo[rt];
-        if (key >= p.pos0 && key < c1) {
-            const uint32_t iv = interval[key - p.pos0];
-            see = (iv & 0xffffu) <= pre[rt] && pre[rt] < iv >> 16 && p.pos0 + depth[key - p.pos0] >= lo[rt];
-        }
-        return see && key < c1;
-    };
-    int odd_first = c1, odd_last = -1;  // tiles that hold an infinity or a NaN (tree_odd_keys)
     for (int t0 = first; t0 < c1; t0 += kTreeStep) {
         const int next = t0 + kTreeStep;
         // ---- scores
-        float amax = 0.0f;
+        float krow = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-            for (int i = 0; i < 8; i += 2) amax = max3_abs(amax, kr[c][i], kr[c][i + 1]);
-        {
-            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, amax),
-                                                            __builtin_bit_cast(uint32_t, amax), false, false);
-            amax = __builtin_elementwise_maximum(as_float(x[0]), as_float(x[1]));
+            for (int i = 0; i < 8; i += 2) krow = max3_abs(krow, kr[c][i], kr[c][i + 1]);
+        krow = across_halves(krow, maximum_of);
+        float ktop = wave_maximum(krow);
+        uint32_t odd = static_cast<uint32_t>(__ballot(is_odd(krow, ktop)));  // keys, and with its values' below
+        if (odd) {
+            ktop = wave_max(krow < __builtin_inff() ? krow : 0.0f);
+            odd = static_cast<uint32_t>(__ballot(is_odd(krow, ktop)));
         }
-        const int kf = scale_field(amax);
-        if (g == 0) kfac[wv][li] = pow2_field(kf - 7);
-        const float ks = pow2_field(254 + 7 - kf);
-        floatx16 st[RT];
+        const int kf = scale_field(ktop);
+        const float ks = pow2_field(254 + 14 - kf);
+        floatx16 st;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) st[rt][r] = 0.0f;
+        for (int r = 0; r < 16; ++r) st[r] = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             half8_t kh, kl;
             pair8(kr[c], ks, kh, kl);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const half8_t h = qhi[(rt * NC + c) * 64 + lane], lw = qlo[(rt * NC + c) * 64 + lane];
-                st[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, h, st[rt], 0, 0, 0);
-                st[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, lw, st[rt], 0, 0, 0);
-                st[rt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, h, st[rt], 0, 0, 0);
-            }
+            const half8_t h = qhi[c * 64 + lane], lw = qlo[c * 64 + lane];
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, h, st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, lw, st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, h, st, 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         if (!kAhead) load_v(t0);
 
-        // ---- the value rows' powers of two: lane i of half g forms register
-        // i / 2's, every lane reads its half's sixteen
-        uint32_t kbad;  // keys that are not finite: none to the products
-        {
-            float b[16];
+        // ---- the values' power of two, and whether every row is near it (a row
+        // of zeros is as good)
+        float vrow[16], vtop = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            vrow[r] = max3_abs(0.0f, vr[0][r], vr[1][r]);
+#pragma unroll
+            for (int n = 2; n < NN; n += 2) vrow[r] = max3_abs(vrow[r], vr[n][r], vr[n + 1][r]);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) vtop = maximum_of(maximum_of(vtop, vrow[r]), vrow[r + 1]);
+        vtop = wave_maximum(vtop);
+        bool near = vtop < __builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const uint64_t here = __ballot(vrow[r] >= vtop * kOddBelow);
+            near = near && static_cast<uint32_t>(here) && here >> 32;
+        }
+        if (!near) {
+            // each row's largest element over its 32 lanes, then the rule
+            uint32_t bad = 0;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                b[r] = max3_abs(0.0f, vr[0][r], vr[1][r]);
-#pragma unroll
-                for (int n = 2; n < NN; n += 2) b[r] = max3_abs(b[r], vr[n][r], vr[n + 1][r]);
+                float x = vrow[r];
+                x = dpp_maximum<0xb1>(x, x);
+                x = dpp_maximum<0x4e>(x, x);
+                x = dpp_maximum<0x141>(x, x);
+                x = dpp_maximum<0x140>(x, x);
+                const auto y = __builtin_amdgcn_permlane16_swap(as_bits(x), as_bits(x), false, false);
+                vrow[r] = maximum_of(as_float(y[0]), as_float(y[1]));
             }
-            float bm = scatter_max(b, lane);
-            kbad = static_cast<uint32_t>(__ballot(!(amax < __builtin_inff())));
-            const bool vbad = __ballot(!(bm < __builtin_inff())) != 0;
-            if (vbad) {
-                // zeros for the products; the factors from the other elements
+            vtop = 0.0f;
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    b[r] = 0.0f;
+            for (int r = 0; r < 16; ++r)
+                if (vrow[r] < __builtin_inff()) vtop = fmaxf(vtop, vrow[r]);
+            vtop = across_halves(vtop, maximum_of);
 #pragma unroll
-                    for (int n = 0; n < NN; ++n) {
-                        vr[n][r] = fabsf(vr[n][r]) < __builtin_inff() ? vr[n][r] : 0.0f;
-                        b[r] = fmaxf(b[r], fabsf(vr[n][r]));
-                    }
-                }
-                bm = scatter_max(b, lane);
+            for (int r = 0; r < 16; ++r) {
+                const bool b = is_odd(vrow[r], vtop);
+                const uint64_t w = __ballot(b);
+                const int key = 8 * (r >> 2) + (r & 3);
+                if (static_cast<uint32_t>(w)) bad |= 1u << key;
+                if (w >> 32) bad |= 1u << (key + 4);
+#pragma unroll
+                for (int n = 0; n < NN; ++n) vr[n][r] = b ? 0.0f : vr[n][r];
             }
-            if (vbad || kbad) {
-                odd_first = min(odd_first, t0);
-                odd_last = t0;
-            }
-            const int f = scale_field(bm);
-            vfac[wv][0][16 * g + (li >> 1)] = pow2_field(254 + 14 - f);
-            vfac[wv][1][16 * g + (li >> 1)] = static_cast<float>(f - 127);
+            odd |= bad;
         }
+        if (odd) {
+            odd_first = min(odd_first, t0);
+            odd_last = t0;
+        }
+        const int vf = scale_field(vtop);
+        const float vs = pow2_field(254 + 14 - vf), ve[2] = {static_cast<float>(vf - 127), static_cast<float>(vf - 127)};
 
         // ---- softmax
-        const bool plain = t0 + kTreeKeys <= min(p.pos0, c1) && t0 >= lo_most && !kbad;
-        half8_t ph[RT][2], pl[RT][2];
+        const float sf = pow2_field(kf - 14) * qf;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const floatx4 f = *reinterpret_cast<const floatx4*>(&kfac[wv][8 * a + 4 * g]);
-#pragma unroll
-                for (int b = 0; b < 4; ++b) st[rt][4 * a + b] = st[rt][4 * a + b] * f[b] * qf[rt];
-            }
-            if (!plain)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int j = 8 * (r >> 2) + 4 * g + (r & 3);
-                    if (!sees(t0 + j, rt) || (kbad >> j & 1)) st[rt][r] = -__builtin_inff();
-                }
-            float tv[16];
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                const floatx4 f = *reinterpret_cast<const floatx4*>(&vfac[wv][1][16 * g + 4 * a]);
-#pragma unroll
-                for (int b = 0; b < 4; ++b) tv[4 * a + b] = st[rt][4 * a + b] + f[b];
-            }
-            float mx = -1e30f, mxt = -1e30f;
+        for (int r = 0; r < 16; ++r) st[r] *= sf;
+        if (t0 + kTreeKeys > min(p.pos0, c1) || t0 < lo_most || odd)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                mx = fmaxf(mx, st[rt][r]);
-                mxt = fmaxf(mxt, tv[r]);
+                const int j = 8 * (r >> 2) + 4 * g + (r & 3);
+                if (!sees_key(p, tree, place, t0 + j, c1) || (odd >> j & 1)) st[r] = -__builtin_inff();
             }
-            {
-                const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
-                                                                __builtin_bit_cast(uint32_t, mx), false, false);
-                const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mxt),
-                                                                __builtin_bit_cast(uint32_t, mxt), false, false);
-                mx = fmaxf(as_float(x[0]), as_float(x[1]));
-                mxt = fmaxf(as_float(y[0]), as_float(y[1]));
-            }
-            const float m2 = fmaxf(m[rt], mx), mt2 = fmaxf(mt[rt], mxt);
-            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        half8_t ph[2], pl[2];
+        const float alpha = tile_softmax(st, ve, s, ph, pl);
+        if (__ballot(alpha != 1.0f))
 #pragma unroll
-            for (int r = 0; r < 16; ++r) sum[r & 3] += __builtin_amdgcn_exp2f(st[rt][r] - m2);
+            for (int n = 0; n < NN; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float w[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(tv[8 * c + i] - mt2);
-                pair8(w, 16384.0f, ph[rt][c], pl[rt][c]);
-            }
-            float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            {
-                const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, all),
-                                                                __builtin_bit_cast(uint32_t, all), false, false);
-                all = as_float(x[0]) + as_float(x[1]);
-            }
-            l[rt] = l[rt] * __builtin_amdgcn_exp2f(m[rt] - m2) + all;
-            if (__ballot(mt2 > mt[rt])) {
-                const float alpha = __builtin_amdgcn_exp2f(mt[rt] - mt2);
-#pragma unroll
-                for (int n = 0; n < NN; ++n)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[rt][n][r] *= alpha;
-            }
-            m[rt] = m2;
-            mt[rt] = mt2;
-        }
+                for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
         __builtin_amdgcn_sched_barrier(0);
         if (kAhead && next < c1) load_k(next);
         __builtin_amdgcn_sched_barrier(0);
 
         // ---- weighted values
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float vs[8];
+        for (int n = 0; n < NN; ++n)
 #pragma unroll
-            for (int a = 0; a < 2; ++a) {
-                const floatx4 f = *reinterpret_cast<const floatx4*>(&vfac[wv][0][16 * g + 8 * c + 4 * a]);
+            for (int c = 0; c < 2; ++c) {
+                float x[8];
 #pragma unroll
-                for (int b = 0; b < 4; ++b) vs[4 * a + b] = f[b];
-            }
-#pragma unroll
-            for (int n = 0; n < NN; ++n) {
+                for (int i = 0; i < 8; ++i) x[i] = vr[n][8 * c + i];
                 half8_t vh, vl;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    _Float16 h, lw;
-                    pair_of(vr[n][8 * c + i], vs[i], h, lw);
-                    vh[i] = h;
-                    vl[i] = lw;
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    o[rt][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[rt][c], o[rt][n], 0, 0, 0);
-                    o[rt][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[rt][c], o[rt][n], 0, 0, 0);
-                    o[rt][n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[rt][c], o[rt][n], 0, 0, 0);
-                }
+                pair8(x, vs, vh, vl);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[c], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[c], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[c], o[n], 0, 0, 0);
             }
-        }
         __builtin_amdgcn_sched_barrier(0);
         if (next < c1) {
             if (kAhead) load_v(next);
@@ -2042,121 +2102,58 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
     }
 
     // ---- the waves' parts meet in LDS
-    const bool whole = gridDim.z == 1;
-    const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        __syncthreads();  // the query rows, or the parts of the row tile before, are done with
-        const float f = l[rt] != 0.0f ? __builtin_amdgcn_exp2f(mt[rt] - m[rt] - 28.0f) / l[rt] : 0.0f;
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int at = 8 * a + 4 * g + b, r = 4 * a + b;  // the lane's value row of a column tile
-                if constexpr (VW == 4) {
-#pragma unroll
-                    for (int n = 0; n < NN; n += 4)
-                        shared[wv * kPart + (8 * n + at) * 33 + li] = make_float4(
-                            o[rt][n][r] * f, o[rt][n + 1][r] * f, o[rt][n + 2][r] * f, o[rt][n + 3][r] * f);
-                } else if (b % 2 == 0) {
-                    shared[wv * kPart + at / 2 * 33 + li] =
-                        make_float4(o[rt][0][r] * f, o[rt][1][r] * f, o[rt][0][r + 1] * f, o[rt][1][r + 1] * f);
-                }
-            }
-        if (odd_last >= 0) {
-            __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
-            asm volatile("" ::: "memory");
-            const int row = min(row0 + 32 * rt + li, rows - 1);
-            for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeStep)
-                tree_odd_keys<HD>(p, reinterpret_cast<float*>(shared + wv * kPart + li),
-                                  p.q + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD, kbase, vbase, kn,
-                                  t0, min(t0 + kTreeKeys, c1), lane, m[rt], l[rt], [&](int key) { return sees(key, rt); });
-        }
-        if (g == 0) mls[wv][li] = make_float2(m[rt], l[rt]);
-        __syncthreads();
-        for (int i = tid; i < 32 * HD / 4; i += kThreads) {
-            const int r = i / (HD / 4), d4 = i % (HD / 4), row = row0 + 32 * rt + r;
-            if (row >= rows) continue;
-            float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) M = fmaxf(M, mls[w][r].x);
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float2 ml = mls[w][r];
-                const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
-                const float4 v = shared[w * kPart + d4 * 33 + r];
-                L += wt;
-                if (wt != 0.0f) {  // (a part without a key has nothing to add)
-                    x[0] += wt * v.x;
-                    x[1] += wt * v.y;
-                    x[2] += wt * v.z;
-                    x[3] += wt * v.w;
-                }
-            }
-            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-            float* dst = whole ? p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD
-                               : p.part_o + (prow + 32 * rt + r) * HD;
-            reinterpret_cast<float4*>(dst)[d4] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-            if (!whole && d4 == 0) p.part_ml[prow + 32 * rt + r] = make_float2(M, L);
-        }
+    __syncthreads();  // the query rows are done with
+    float4* const part = shared + wv * kPart;
+    store_part<NN>(part, o, s, li, g);
+    if (odd_last >= 0) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
+        asm volatile("" ::: "memory");
+        for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeStep)
+            add_odd_keys<HD, kTreeKeys>(p, tree, place, reinterpret_cast<float*>(part + li),
+                                        p.q + (static_cast<size_t>(myrow / G) * p.n_heads + hk * G + myrow % G) * HD, kbase,
+                                        vbase, kn, t0, c1, lane, s);
     }
-}
-
-// x[i], i < 8, each reduced over a wave half: lane i returns the maximum of
-// x[i / 4] (scatter_max for eight values)
-__device__ __forceinline__ float scatter_max8(const float (&x)[8], int lane) {
-    float a[4], b[2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x[i]),
-                                                        __builtin_bit_cast(uint32_t, x[i + 4]), false, false);
-        a[i] = __builtin_elementwise_maximum(as_float(s[0]), as_float(s[1]));
-    }
-    const bool b3 = lane & 8, b2 = lane & 4;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) b[i] = dpp_maximum<0x128>(b3 ? a[i + 2] : a[i], b3 ? a[i] : a[i + 2]);  // row_ror:8
-    const float c = dpp_maximum<0x141>(b2 ? b[1] : b[0], b2 ? b[0] : b[1]);  // row_half_mirror
-    const float d = dpp_maximum<0x4e>(c, c);                                 // quad_perm [2,3,0,1]
-    return dpp_maximum<0xb1>(d, d);                                          // quad_perm [1,0,3,2]
+    if (g == 0) mls[wv][li] = make_float2(s.m, s.l);
+    __syncthreads();
+    join_parts<HD, kWaves>(p, shared, mls, 1, 1, row0, hk, G, rows);
 }
 
 // Rows over waves, for more than 32 query rows of a KV head: a work-group takes
 // 32 RW rows and two 32-key tiles a step, which its waves load, scale, split and
 // lay out in LDS as operands once for all of them (waves 2 s and 2 s + 1 stage
-// tile s).  RW = 4: each wave owns 32 rows and takes both tiles; RW = 2: waves w
-// and w + 2 own the same 32 rows, a tile each, and meet at the end.  The products,
-// weights and factors are those of tree_keys_kernel.  The next step's loads are
-// in flight during this one's products; two work-groups a CU fill each other's
-// waits.
+// tile s, 16 keys and 16 values each, a group with powers of two of its own).
+// RW = 4: each wave owns 32 rows and takes both tiles; RW = 2: waves w and w + 2
+// own the same 32 rows, a tile each, and meet at the end.  The next step's loads
+// are in flight during this one's products; two work-groups a CU fill each
+// other's waits.
 template <int HD, int RW, int OCC>
 __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) {
-    constexpr int NC = HD / 16, NN = HD / 32, R = 32 * RW, KW = kWaves / RW;
+    constexpr int NC = HD / 16, NN = HD / 32, KW = kWaves / RW;
     constexpr int VW = NN < 4 ? NN : 4;
     constexpr int kPart = HD / 4 * 33;
     constexpr int kTile = NC * 64;  // half8 of a tile's keys' hi (or lo) parts, and of its values'
     constexpr int kShared = kTile * 8 > kPart * kWaves ? kTile * 8 : kPart * kWaves;
     __shared__ __align__(16) float4 shared[kShared];
-    __shared__ __align__(16) float kfac[2][kTreeKeys];     // key factors (infinite: a key that is not finite)
-    __shared__ __align__(16) float vfac[2][2][kTreeKeys];  // value factors and exponents, by half and register
+    __shared__ float kfac[2][2], vexp[2][2];  // [tile][half]: the keys' factor, the values' exponent
+    __shared__ uint32_t oddmask[2][2];        // [tile][half]: odd keys, from bit 16 half on
     __shared__ float2 mls[kWaves][32];
-    __shared__ int kodd[2], odd_first, odd_last;
-    __shared__ uint32_t interval[kMaxTreeNodes];
-    __shared__ uint16_t depth[kMaxTreeNodes];
+    __shared__ int odd_first, odd_last;
+    __shared__ TreeShared tree;
     half8_t* const khi = reinterpret_cast<half8_t*>(shared);  // [tile][slice][lane]
     half8_t* const klo = khi + 2 * kTile;
     half8_t* const vhi = khi + 4 * kTile;                     // [tile][column tile][slice][lane]
     half8_t* const vlo = khi + 6 * kTile;
     const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
     const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * R;
-    const int total = p.pos0 + p.n;
-    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(total, c0 + p.chunk);
+    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * 32 * RW;
+    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(p.pos0 + p.n, c0 + p.chunk);
     const uint32_t kn = static_cast<uint32_t>(p.n_kv) * HD;
     const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
     const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
 
     // ---- staging: wave 2 s + c loads keys 16 c .. + 16 of tile s (four lanes a
-    // key, 64 bytes a load) and values of slice c (a lane half a row)
+    // key, 64 bytes a load) and values of slice c, keys 16 c .. + 16, too (a lane
+    // half a row; register i of half g is key 16 c + 4 g + i % 4 + 8 (i / 4))
     const int ts = wv >> 1, tc = wv & 1;
     auto tile_of = [&](const float* base, int t0) {
         const int n = min(c1 - t0, kTreeKeys);  // none past the range: every load reads zeros
@@ -2196,15 +2193,20 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         }
     };
     auto stage = [&](int t0) {
-        float amax = 0.0f;
+        uint32_t odd = 0;  // this group's odd keys
+        float krow = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) amax = max3_abs(max3_abs(amax, kst[c][0], kst[c][1]), kst[c][2], kst[c][3]);
-        amax = dpp_maximum<0xb1>(amax, amax);
-        amax = dpp_maximum<0x4e>(amax, amax);
-        const bool kbad = !(amax < __builtin_inff());
-        const int kf = scale_field(amax);
-        const float ks = pow2_field(254 + 7 - kf);
-        if (quarter == 0) kfac[ts][key4] = kbad ? __builtin_inff() : pow2_field(kf - 7);
+        for (int c = 0; c < NC; ++c) krow = max3_abs(max3_abs(krow, kst[c][0], kst[c][1]), kst[c][2], kst[c][3]);
+        krow = dpp_maximum<0xb1>(krow, krow);
+        krow = dpp_maximum<0x4e>(krow, krow);
+        float ktop = wave_maximum(krow);
+        if (__ballot(is_odd(krow, ktop))) {
+            ktop = wave_max(krow < __builtin_inff() ? krow : 0.0f);
+            const uint64_t w = __ballot(is_odd(krow, ktop));
+            for (int j = 0; j < 16; ++j) odd |= static_cast<uint32_t>(w >> (4 * j) & 1) << j;
+        }
+        const int kf = scale_field(ktop);
+        const float ks = pow2_field(254 + 14 - kf);
         // slice c, half quarter / 2, elements 4 (quarter % 2) ..
         const int kslot = (ts * kTile + (quarter >> 1) * 32 + key4) * 2 + (quarter & 1);
 #pragma unroll
@@ -2221,73 +2223,78 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             reinterpret_cast<half4_t*>(khi)[kslot + 128 * c] = hi;
             reinterpret_cast<half4_t*>(klo)[kslot + 128 * c] = lo;
         }
-        float b[8];
+        float vrow[8], vtop = 0.0f;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            b[r] = max3_abs(0.0f, vst[0][r], vst[1][r]);
+            vrow[r] = max3_abs(0.0f, vst[0][r], vst[1][r]);
 #pragma unroll
-            for (int n = 2; n < NN; n += 2) b[r] = max3_abs(b[r], vst[n][r], vst[n + 1][r]);
+            for (int n = 2; n < NN; n += 2) vrow[r] = max3_abs(vrow[r], vst[n][r], vst[n + 1][r]);
         }
-        float bm = scatter_max8(b, lane);
-        const bool vbad = __ballot(!(bm < __builtin_inff())) != 0;
-        if (vbad) {
-            // zeros for the products; the factors from the other elements
+#pragma unroll
+        for (int r = 0; r < 8; r += 2) vtop = maximum_of(maximum_of(vtop, vrow[r]), vrow[r + 1]);
+        vtop = wave_maximum(vtop);
+        bool near = vtop < __builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const uint64_t here = __ballot(vrow[r] >= vtop * kOddBelow);
+            near = near && static_cast<uint32_t>(here) && here >> 32;
+        }
+        if (!near) {
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
-                b[r] = 0.0f;
-#pragma unroll
-                for (int n = 0; n < NN; ++n) {
-                    vst[n][r] = fabsf(vst[n][r]) < __builtin_inff() ? vst[n][r] : 0.0f;
-                    b[r] = fmaxf(b[r], fabsf(vst[n][r]));
-                }
+                float x = vrow[r];
+                x = dpp_maximum<0xb1>(x, x);
+                x = dpp_maximum<0x4e>(x, x);
+                x = dpp_maximum<0x141>(x, x);
+                x = dpp_maximum<0x140>(x, x);
+                const auto y = __builtin_amdgcn_permlane16_swap(as_bits(x), as_bits(x), false, false);
+                vrow[r] = maximum_of(as_float(y[0]), as_float(y[1]));
             }
-            bm = scatter_max8(b, lane);
-        }
-        const bool kany = __ballot(kbad) != 0;
-        if ((kany || vbad) && lane == 0) {
-            if (kany) kodd[ts] = t0 + kTreeKeys * ts + 1;  // this step's mark: no step has it again
-            atomicMin(&odd_first, t0 + kTreeKeys * ts);
-            atomicMax(&odd_last, t0 + kTreeKeys * ts);
-        }
-        const int f = scale_field(bm);
-        vfac[ts][0][16 * g + 8 * tc + (li >> 2)] = pow2_field(254 + 14 - f);
-        vfac[ts][1][16 * g + 8 * tc + (li >> 2)] = static_cast<float>(f - 127);
-        float vs[8];
+            vtop = 0.0f;
 #pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            const floatx4 w = *reinterpret_cast<const floatx4*>(&vfac[ts][0][16 * g + 8 * tc + 4 * a]);
+            for (int r = 0; r < 8; ++r)
+                if (vrow[r] < __builtin_inff()) vtop = fmaxf(vtop, vrow[r]);
+            vtop = across_halves(vtop, maximum_of);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vs[4 * a + i] = w[i];
+            for (int r = 0; r < 8; ++r) {
+                const bool b = is_odd(vrow[r], vtop);
+                const uint64_t w = __ballot(b);
+                const int key = 8 * (r >> 2) + (r & 3);
+                if (static_cast<uint32_t>(w)) odd |= 1u << key;
+                if (w >> 32) odd |= 1u << (key + 4);
+#pragma unroll
+                for (int n = 0; n < NN; ++n) vst[n][r] = b ? 0.0f : vst[n][r];
+            }
         }
+        const int vf = scale_field(vtop);
+        if (lane == 0) {
+            kfac[ts][tc] = pow2_field(kf - 14);
+            vexp[ts][tc] = static_cast<float>(vf - 127);
+            oddmask[ts][tc] = odd << (16 * tc);
+            if (odd) {
+                atomicMin(&odd_first, t0 + kTreeKeys * ts + 16 * tc);
+                atomicMax(&odd_last, t0 + kTreeKeys * ts + 16 * tc);
+            }
+        }
+        const float vs = pow2_field(254 + 14 - vf);
 #pragma unroll
         for (int n = 0; n < NN; ++n) {
             half8_t hi, lo;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                _Float16 h, l;
-                pair_of(vst[n][i], vs[i], h, l);
-                hi[i] = h;
-                lo[i] = l;
-            }
+            pair8(vst[n], vs, hi, lo);
             vhi[ts * kTile + (n * 2 + tc) * 64 + lane] = hi;
             vlo[ts * kTile + (n * 2 + tc) * 64 + lane] = lo;
         }
     };
 
     prefetch(c0);
-    if (tid < 2) kodd[tid] = 0;
     if (tid == 0) {
         odd_first = c1;
         odd_last = -1;
     }
-    if (c1 > p.pos0)
-        for (int i = tid; i < p.n; i += kThreads) {
-            interval[i] = p.tree.pre[i] | static_cast<uint32_t>(p.tree.end[i]) << 16;
-            depth[i] = p.tree.depth[i];
-        }
+    if (c1 > p.pos0) load_tree(p, tree);
     // this wave's query rows as operands, in registers
-    const int rt = wv % RW, myrow = row0 + 32 * rt + li, srow = min(myrow, rows - 1);
-    const float* const qrow = p.q + (static_cast<size_t>(srow / G) * p.n_heads + hk * G + srow % G) * HD;
+    const int rt = wv % RW, myrow = min(row0 + 32 * rt + li, rows - 1);
+    const float* const qrow = p.q + (static_cast<size_t>(myrow / G) * p.n_heads + hk * G + myrow % G) * HD;
     half8_t qh[NC], ql[NC];
     float qf;
     {
@@ -2299,26 +2306,15 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
                 x[c][i] = qrow[16 * c + 8 * g + i];
                 amax = fmaxf(amax, fabsf(x[c][i]));
             }
-        const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, amax),
-                                                        __builtin_bit_cast(uint32_t, amax), false, false);
-        const int f = scale_field(fmaxf(as_float(y[0]), as_float(y[1])));
+        const int f = scale_field(across_halves(amax, maximum_of));
 #pragma unroll
         for (int c = 0; c < NC; ++c) pair8(x[c], pow2_field(254 + 7 - f), qh[c], ql[c]);
         qf = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
     }
-    const uint32_t pre = p.tree.pre[srow / G];
-    const int lo = p.sw > 0 ? max(0, p.pos0 + p.tree.depth[srow / G] - p.sw + 1) : 0;
+    const RowPlace place = place_of(p, myrow / G);
     const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.tree.max_depth - p.sw + 1) : 0;
-    auto sees = [&](int key) {
-        bool see = key < p.pos0 && key >= lo;
-        if (key >= p.pos0 && key < c1) {
-            const uint32_t iv = interval[key - p.pos0];
-            see = (iv & 0xffffu) <= pre && pre < iv >> 16 && p.pos0 + depth[key - p.pos0] >= lo;
-        }
-        return see && key < c1;
-    };
 
-    float m = -1e30f, mt = -1e30f, l = 0.0f;
+    RowState st_row{-1e30f, -1e30f, 0.0f};
     floatx16 o[NN];
 #pragma unroll
     for (int n = 0; n < NN; ++n)
@@ -2336,68 +2332,23 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], st, 0, 0, 0);
             st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], st, 0, 0, 0);
         }
-        const bool plain = t0 + kTreeKeys <= min(p.pos0, c1) && t0 >= lo_most && kodd[s] != t0 + 1;
-        float tv[16];
+        const float ve[2] = {vexp[s][0], vexp[s][1]}, sf[2] = {kfac[s][0] * qf, kfac[s][1] * qf};
+        const uint32_t odd = __builtin_amdgcn_readfirstlane(oddmask[s][0] | oddmask[s][1]);
 #pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const floatx4 f = *reinterpret_cast<const floatx4*>(&kfac[s][8 * a + 4 * g]);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) st[4 * a + b] = st[4 * a + b] * f[b] * qf;
-        }
-        if (!plain)
+        for (int r = 0; r < 16; ++r) st[r] *= sf[r >> 3];
+        if (t0 + kTreeKeys > min(p.pos0, c1) || t0 < lo_most || odd)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int j = 8 * (r >> 2) + 4 * g + (r & 3);
-                if (!sees(t0 + j) || kfac[s][j] == __builtin_inff()) st[r] = -__builtin_inff();
+                if (!sees_key(p, tree, place, t0 + j, c1) || (odd >> j & 1)) st[r] = -__builtin_inff();
             }
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            const floatx4 f = *reinterpret_cast<const floatx4*>(&vfac[s][1][16 * g + 4 * a]);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) tv[4 * a + b] = st[4 * a + b] + f[b];
-        }
-        float mx = -1e30f, mxt = -1e30f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            mx = fmaxf(mx, st[r]);
-            mxt = fmaxf(mxt, tv[r]);
-        }
-        {
-            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mx),
-                                                            __builtin_bit_cast(uint32_t, mx), false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, mxt),
-                                                            __builtin_bit_cast(uint32_t, mxt), false, false);
-            mx = fmaxf(as_float(x[0]), as_float(x[1]));
-            mxt = fmaxf(as_float(y[0]), as_float(y[1]));
-        }
-        const float m2 = fmaxf(m, mx), mt2 = fmaxf(mt, mxt);
-        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[r & 3] += __builtin_amdgcn_exp2f(st[r] - m2);
         half8_t ph[2], pl[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = __builtin_amdgcn_exp2f(tv[8 * c + i] - mt2);
-            pair8(w, 16384.0f, ph[c], pl[c]);
-        }
-        float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        {
-            const auto x = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, all),
-                                                            __builtin_bit_cast(uint32_t, all), false, false);
-            all = as_float(x[0]) + as_float(x[1]);
-        }
-        l = l * __builtin_amdgcn_exp2f(m - m2) + all;
-        if (__ballot(mt2 > mt)) {
-            const float alpha = __builtin_amdgcn_exp2f(mt - mt2);
+        const float alpha = tile_softmax(st, ve, st_row, ph, pl);
+        if (__ballot(alpha != 1.0f))
 #pragma unroll
             for (int n = 0; n < NN; ++n)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
-        }
-        m = m2;
-        mt = mt2;
 #pragma unroll
         for (int n = 0; n < NN; ++n)
 #pragma unroll
@@ -2409,7 +2360,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             }
     };
 
-    __syncthreads();  // the marks' first values, the tree
+    __syncthreads();  // odd_first / odd_last, the tree
     for (int t0 = c0; t0 < c1; t0 += 2 * kTreeKeys) {
         stage(t0);
         __syncthreads();
@@ -2423,60 +2374,19 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         __syncthreads();  // every wave is done with the operands
     }
 
-    // ---- the parts, normalised, through LDS
-    const bool whole = gridDim.z == 1;
-    const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
-    const float f = l != 0.0f ? __builtin_amdgcn_exp2f(mt - m - 28.0f) / l : 0.0f;
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int at = 8 * a + 4 * g + b, r = 4 * a + b;
-            if constexpr (VW == 4) {
-#pragma unroll
-                for (int n = 0; n < NN; n += 4)
-                    shared[wv * kPart + (8 * n + at) * 33 + li] =
-                        make_float4(o[n][r] * f, o[n + 1][r] * f, o[n + 2][r] * f, o[n + 3][r] * f);
-            } else if (b % 2 == 0) {
-                shared[wv * kPart + at / 2 * 33 + li] =
-                    make_float4(o[0][r] * f, o[1][r] * f, o[0][r + 1] * f, o[1][r + 1] * f);
-            }
-        }
+    float4* const part = shared + wv * kPart;
+    store_part<NN>(part, o, st_row, li, g);
     if (odd_last >= 0) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
         asm volatile("" ::: "memory");
-        float* part = reinterpret_cast<float*>(shared + wv * kPart + li);
-        for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeKeys)
+        for (int t0 = odd_first; t0 <= odd_last; t0 += 16)
             if (KW == 1 || (t0 - c0) / kTreeKeys % 2 == wv / RW)
-                tree_odd_keys<HD>(p, part, qrow, kbase, vbase, kn, t0, min(t0 + kTreeKeys, c1), lane, m, l, sees);
+                add_odd_keys<HD, 16>(p, tree, place, reinterpret_cast<float*>(part + li), qrow, kbase, vbase, kn, t0, c1, lane,
+                                     st_row);
     }
-    if (g == 0) mls[wv][li] = make_float2(m, l);
+    if (g == 0) mls[wv][li] = make_float2(st_row.m, st_row.l);
     __syncthreads();
-    for (int i = tid; i < R * HD / 4; i += kThreads) {
-        const int r = i / (HD / 4), d4 = i % (HD / 4), row = row0 + r;
-        if (row >= rows) break;
-        float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < KW; ++w) M = fmaxf(M, mls[r / 32 + RW * w][r % 32].x);
-#pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            const float2 ml = mls[r / 32 + RW * w][r % 32];
-            const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
-            const float4 v = shared[(r / 32 + RW * w) * kPart + d4 * 33 + r % 32];
-            L += wt;
-            if (wt != 0.0f) {
-                x[0] += wt * v.x;
-                x[1] += wt * v.y;
-                x[2] += wt * v.z;
-                x[3] += wt * v.w;
-            }
-        }
-        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        float* dst = whole ? p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD
-                           : p.part_o + (prow + r) * HD;
-        reinterpret_cast<float4*>(dst)[d4] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-        if (!whole && d4 == 0) p.part_ml[prow + r] = make_float2(M, L);
-    }
+    join_parts<HD, KW>(p, shared, mls, RW, RW, row0, hk, G, rows);
 }
 
 // out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the key
@@ -2554,7 +2464,7 @@ hipError_t launch_tree(const TreeParams& p, const TreePlan& pl, hipStream_t stre
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid(p.n_kv, pl.rows_pad / (32 * pl.tiles), pl.chunks);
-    if (pl.tiles == 1) hipLaunchKernelGGL((tree_keys_kernel<HD, 1, OCC>), grid, dim3(kThreads), 0, stream, p);
+    if (pl.tiles == 1) hipLaunchKernelGGL((tree_keys_kernel<HD, OCC>), grid, dim3(kThreads), 0, stream, p);
     else if (pl.tiles == 2) hipLaunchKernelGGL((tree_rows_kernel<HD, 2, OCC>), grid, dim3(kThreads), 0, stream, p);
     else hipLaunchKernelGGL((tree_rows_kernel<HD, 4, OCC>), grid, dim3(kThreads), 0, stream, p);
     e = hipGetLastError();
