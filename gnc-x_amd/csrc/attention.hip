@@ -1615,9 +1615,10 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p) {
 //                    8 a + 4 g + b
 //   O^T += V^T P^T   with P from those registers, and O of row i in lane (i, .):
 //                    the softmax factors of a row never cross lanes
-// Pairs hold 22 bits of values down to 2^-17 of their group's largest, and
-// values of any size are brought there by powers of two: one for a query row,
-// one for the keys and one for the values of a group (a tile, or half of it).
+// Pairs hold about 22 bits of values from 2^-3 to 2^15, and 2^-25 absolutely
+// below.  Every query row, and every group of values (a tile's, or half of it), is
+// brought there by a power of two; a group of keys as well unless its largest
+// element lies there (their scores are sums, in which its small ones do not show).
 // The keys' and the row's come back as a factor of the scores.  The values' 2^e
 // goes into the weights: those of O are 2^(s + e - max (s + e)), those of the sum
 // l 2^(s - max s), two running maxima a row, so that what a row does not see has
@@ -1640,6 +1641,12 @@ __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_ca
 __device__ __forceinline__ int scale_field(float amax) {
     const int f = static_cast<int>(as_bits(amax) >> 23) & 0xff;
     return min(max(f, 30), 254);
+}
+// The exponent field of the power of two that a group of keys of largest element
+// top is divided by: 127 (none) from 2^-2 to 2^14, else one that brings it to 2^14.
+__device__ __forceinline__ int key_field(float top) {
+    const int f = static_cast<int>(as_bits(top) >> 23) & 0xff;
+    return f >= 127 - 2 && f < 127 + 14 ? 127 : min(max(f, 30), 254) - 14;
 }
 // max(m, |a|, |b|), NaN if one is
 __device__ __forceinline__ float max3_abs(float m, float a, float b) {
@@ -1668,20 +1675,32 @@ __device__ __forceinline__ float wave_maximum(float v) {
     return across_halves(maximum_of(as_float(x[0]), as_float(x[1])), maximum_of);
 }
 
-// v scaled by a power of two as an fp16 pair; v scale and the remainder are
-// exact, so each part is one mixed fma
-__device__ __forceinline__ void pair_of(float v, float scale, _Float16& hi, _Float16& lo) {
-    hi = static_cast<_Float16>(__builtin_fmaf(v, scale, 0.0f));
-    lo = static_cast<_Float16>(__builtin_fmaf(v, scale, -static_cast<float>(hi)));
-}
-__device__ __forceinline__ void pair8(const float (&v)[8], float scale, half8_t& hi, half8_t& lo) {
+// N floats, times scale, as fp16 pairs: hi nearest, lo nearest to the rest, which
+// is exact.  Two values a conversion, and the rest as one mixed fma that reads
+// its half of hi in place (written out, as the compiler converts every value once
+// more, alone, to subtract it: 2.4 times the issue cycles).
+typedef float floatx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
+template <bool SCALED, int N, class V>
+__device__ __forceinline__ void pairs(const float (&v)[N], float scale, V& hi, V& lo) {
+    uint32_t h[N / 2], l[N / 2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        _Float16 h, l;
-        pair_of(v[i], scale, h, l);
-        hi[i] = h;
-        lo[i] = l;
+    for (int i = 0; i < N / 2; ++i) {
+        const float a = v[2 * i], b = v[2 * i + 1];
+        h[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(SCALED ? floatx2{a * scale, b * scale} : floatx2{a, b}, half2_t));
+        float x, y;
+        if constexpr (SCALED) {
+            asm("v_fma_mix_f32 %0, %1, %2, -%3 op_sel_hi:[0,0,1]" : "=v"(x) : "v"(a), "v"(scale), "v"(h[i]));
+            asm("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(y) : "v"(b), "v"(scale), "v"(h[i]));
+        } else {
+            asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(x) : "v"(a), "v"(h[i]));
+            asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(y) : "v"(b), "v"(h[i]));
+        }
+        l[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{x, y}, half2_t));
     }
+    hi = __builtin_bit_cast(V, h);
+    lo = __builtin_bit_cast(V, l);
 }
 
 constexpr int kTreeKeys = 32;                  // keys of a tile
@@ -1756,7 +1775,7 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
         }
         // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), the second capped: it
         // passes 2^126 only where the first is 0
-        pair8(e, __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f)), ph[h], pl[h]);
+        pairs<true>(e, __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f)), ph[h], pl[h]);
     }
     s.l = s.l * __builtin_amdgcn_exp2f(s.m - m2) +
           across_halves(sum[0] + sum[1], [](float a, float b) { return a + b; });
@@ -1807,7 +1826,7 @@ __device__ void add_odd_keys(const TreeParams& p, const TreeShared& tree, const 
 // the wave's normalised part to LDS: float4 column d4 of row li at 33 d4 + li
 template <int NN>
 __device__ __forceinline__ void store_part(float4* part, const floatx16 (&o)[NN], const RowState& s, int li, int g) {
-    const float f = s.l != 0.0f ? __builtin_amdgcn_exp2f(s.mt - s.m - 28.0f) / s.l : 0.0f;
+    const float f = s.l != 0.0f ? __builtin_amdgcn_exp2f(s.mt - s.m - 14.0f) / s.l : 0.0f;
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
@@ -1832,30 +1851,40 @@ __device__ __forceinline__ void join_parts(const TreeParams& p, const float4* sh
     constexpr int kPart = HD / 4 * 33;
     const bool whole = gridDim.z == 1;
     const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
-    for (int i = threadIdx.x; i < 32 * tiles * HD / 4; i += kThreads) {
-        const int r = i / (HD / 4), d4 = i % (HD / 4), row = row0 + r;
-        if (row >= rows) break;
-        float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int count = min(32 * tiles, rows - row0) * (HD / 4);
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+        const int r = i / (HD / 4), d4 = i % (HD / 4);
+        float M = mls[r / 32][r % 32].x, L = mls[r / 32][r % 32].y;
+        float4 x = shared[r / 32 * kPart + d4 * 33 + r % 32];
+        if constexpr (N > 1) {
 #pragma unroll
-        for (int w = 0; w < N; ++w) M = fmaxf(M, mls[r / 32 + per * w][r % 32].x);
+            for (int w = 1; w < N; ++w) M = fmaxf(M, mls[r / 32 + per * w][r % 32].x);
+            L = 0.0f;
+            x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < N; ++w) {
-            const float2 ml = mls[r / 32 + per * w][r % 32];
-            const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
-            const float4 v = shared[(r / 32 + per * w) * kPart + d4 * 33 + r % 32];
-            L += wt;
-            if (wt != 0.0f) {  // (a part without a key has nothing to add)
-                x[0] += wt * v.x;
-                x[1] += wt * v.y;
-                x[2] += wt * v.z;
-                x[3] += wt * v.w;
+            for (int w = 0; w < N; ++w) {
+                const float2 ml = mls[r / 32 + per * w][r % 32];
+                const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
+                const float4 v = shared[(r / 32 + per * w) * kPart + d4 * 33 + r % 32];
+                L += wt;
+                if (wt != 0.0f) {  // (a part without a key has nothing to add)
+                    x.x += wt * v.x;
+                    x.y += wt * v.y;
+                    x.z += wt * v.z;
+                    x.w += wt * v.w;
+                }
             }
+            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
         }
-        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        float* dst = whole ? p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD
-                           : p.part_o + (prow + r) * HD;
-        reinterpret_cast<float4*>(dst)[d4] = make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-        if (!whole && d4 == 0) p.part_ml[prow + r] = make_float2(M, L);
+        if (whole) {
+            const int row = row0 + r;
+            if (N == 1 && L != L) x = make_float4(L, L, L, L);  // (an odd key that makes its row NaN)
+            reinterpret_cast<float4*>(p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD)[d4] = x;
+        } else {
+            reinterpret_cast<float4*>(p.part_o + (prow + r) * HD)[d4] = x;
+            if (d4 == 0) p.part_ml[prow + r] = make_float2(M, L);
+        }
     }
 }
 
@@ -1950,7 +1979,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
 #pragma unroll
         for (int u = 0; u < HD / 64; ++u) {
             half8_t h, l;
-            pair8(x[u], pow2_field(254 + 7 - f), h, l);
+            pairs<true>(x[u], pow2_field(254 + 7 - f), h, l);
             const int unit = j * (HD / 64) + u, at = unit / 2 * 64 + 32 * (unit & 1) + tid / 8;
             qhi[at] = h;
             qlo[at] = l;
@@ -1987,15 +2016,19 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
             ktop = wave_max(krow < __builtin_inff() ? krow : 0.0f);
             odd = static_cast<uint32_t>(__ballot(is_odd(krow, ktop)));
         }
-        const int kf = scale_field(ktop);
-        const float ks = pow2_field(254 + 14 - kf);
+        const int kf = key_field(ktop);
+        if (kf != 127)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) kr[c][i] *= pow2_field(254 - kf);
         floatx16 st;
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[r] = 0.0f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             half8_t kh, kl;
-            pair8(kr[c], ks, kh, kl);
+            pairs<false>(kr[c], 1.0f, kh, kl);
             const half8_t h = qhi[c * 64 + lane], lw = qlo[c * 64 + lane];
             st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, h, st, 0, 0, 0);
             st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, lw, st, 0, 0, 0);
@@ -2056,11 +2089,11 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
             odd_first = min(odd_first, t0);
             odd_last = t0;
         }
-        const int vf = scale_field(vtop);
-        const float vs = pow2_field(254 + 14 - vf), ve[2] = {static_cast<float>(vf - 127), static_cast<float>(vf - 127)};
+        const int vf = scale_field(vtop) - 14;  // the field of the power of two that they are divided by
+        const float vs = pow2_field(254 - vf), ve[2] = {static_cast<float>(vf - 127), static_cast<float>(vf - 127)};
 
         // ---- softmax
-        const float sf = pow2_field(kf - 14) * qf;
+        const float sf = pow2_field(kf) * qf;
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[r] *= sf;
         if (t0 + kTreeKeys > min(p.pos0, c1) || t0 < lo_most || odd)
@@ -2089,7 +2122,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] = vr[n][8 * c + i];
                 half8_t vh, vl;
-                pair8(x, vs, vh, vl);
+                pairs<true>(x, vs, vh, vl);
                 o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[c], o[n], 0, 0, 0);
                 o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[c], o[n], 0, 0, 0);
                 o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[c], o[n], 0, 0, 0);
@@ -2205,21 +2238,18 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             const uint64_t w = __ballot(is_odd(krow, ktop));
             for (int j = 0; j < 16; ++j) odd |= static_cast<uint32_t>(w >> (4 * j) & 1) << j;
         }
-        const int kf = scale_field(ktop);
-        const float ks = pow2_field(254 + 14 - kf);
+        const int kf = key_field(ktop);
+        if (kf != 127)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kst[c][i] *= pow2_field(254 - kf);
         // slice c, half quarter / 2, elements 4 (quarter % 2) ..
         const int kslot = (ts * kTile + (quarter >> 1) * 32 + key4) * 2 + (quarter & 1);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            typedef _Float16 half4_t __attribute__((ext_vector_type(4)));
             half4_t hi, lo;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                _Float16 h, l;
-                pair_of(kst[c][i], ks, h, l);
-                hi[i] = h;
-                lo[i] = l;
-            }
+            pairs<false>(kst[c], 1.0f, hi, lo);
             reinterpret_cast<half4_t*>(khi)[kslot + 128 * c] = hi;
             reinterpret_cast<half4_t*>(klo)[kslot + 128 * c] = lo;
         }
@@ -2266,9 +2296,10 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
                 for (int n = 0; n < NN; ++n) vst[n][r] = b ? 0.0f : vst[n][r];
             }
         }
-        const int vf = scale_field(vtop);
+        const int vf = scale_field(vtop) - 14;
+        const float vs = pow2_field(254 - vf);
         if (lane == 0) {
-            kfac[ts][tc] = pow2_field(kf - 14);
+            kfac[ts][tc] = pow2_field(kf);
             vexp[ts][tc] = static_cast<float>(vf - 127);
             oddmask[ts][tc] = odd << (16 * tc);
             if (odd) {
@@ -2276,11 +2307,10 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
                 atomicMax(&odd_last, t0 + kTreeKeys * ts + 16 * tc);
             }
         }
-        const float vs = pow2_field(254 + 14 - vf);
 #pragma unroll
         for (int n = 0; n < NN; ++n) {
             half8_t hi, lo;
-            pair8(vst[n], vs, hi, lo);
+            pairs<true>(vst[n], vs, hi, lo);
             vhi[ts * kTile + (n * 2 + tc) * 64 + lane] = hi;
             vlo[ts * kTile + (n * 2 + tc) * 64 + lane] = lo;
         }
@@ -2308,7 +2338,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             }
         const int f = scale_field(across_halves(amax, maximum_of));
 #pragma unroll
-        for (int c = 0; c < NC; ++c) pair8(x[c], pow2_field(254 + 7 - f), qh[c], ql[c]);
+        for (int c = 0; c < NC; ++c) pairs<true>(x[c], pow2_field(254 + 7 - f), qh[c], ql[c]);
         qf = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
     }
     const RowPlace place = place_of(p, myrow / G);
