@@ -751,29 +751,56 @@ __global__ __launch_bounds__(kCandThreads) void reorder_kernel(ReorderParams p) 
 // logits', so one pass over them leaves, per (beam, part of the vocabulary),
 // the part's maximum, its sum of exponentials and its n_out best; a second
 // kernel joins the parts in double, where candidates of different beams meet.
+//
+// Both find the n_out best of what their threads hold the same way.  The
+// n_out-th largest of 256 maxima of disjoint groups is a threshold that at least
+// n_out values reach, and few more: those go to LDS, and each one's rank is the
+// number of better ones.  Where too many reach it (a vocabulary of equal
+// logits), the best are taken one after another instead.
 struct SelectParams {
     const float* logits;
     const float* scores;
     const int32_t* finished;
-    int32_t finished_token, n_beams, vocab, n_out, chunk, n_chunks;
+    int32_t finished_token, n_beams, vocab, n_out, n_chunks;
     float2* ml;   // [beam][chunk] maximum, sum of e^(x - maximum)
-    float2* best;  // [beam][chunk][n_out] logit, word (as bits); -inf behind the last
+    float2* best;  // [beam][chunk][n_out] logit, word (as bits), in falling order; -inf behind the last
     int32_t* out_parents;
     int32_t* out_tokens;
     float* out_scores;
 };
+constexpr int kGroups = 256;       // maxima that the threshold is taken from
+constexpr int kMostRanked = 1024;  // values that are ranked
 
-// Larger for the better candidate: the logit's bits in an order-preserving
-// form (NaN and -0 as -inf and +0), then the lower word.
+// NaN and -0 as -inf and +0
 __device__ __forceinline__ float clean(float x) { return x != x ? -__builtin_inff() : x + 0.0f; }
-__device__ __forceinline__ uint64_t key_of(float x, uint32_t word) {
+// a float's bits in the floats' order, and back
+__device__ __forceinline__ uint32_t ordered(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const uint32_t ordered = u & 0x80000000u ? ~u : u | 0x80000000u;
-    return static_cast<uint64_t>(ordered) << 32 | ~word;
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ float logit_of(uint64_t key) {
-    const uint32_t o = static_cast<uint32_t>(key >> 32);
+__device__ __forceinline__ float unordered(uint32_t o) {
     return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o);
+}
+// Larger for the better candidate: the logit, then the lower word.
+__device__ __forceinline__ uint64_t key_of(float x, uint32_t word) {
+    return static_cast<uint64_t>(ordered(x)) << 32 | ~word;
+}
+
+// A lower bound (its last 12 bits cleared) on the n-th largest of the 256 floats
+// at maxima, by a wave: bit after bit of the ordered form, kept while n of them
+// reach it.
+__device__ __forceinline__ float nth_largest(const float* maxima, int n, int lane) {
+    const float4 v = reinterpret_cast<const float4*>(maxima)[lane];
+    const uint32_t o[4] = {ordered(v.x), ordered(v.y), ordered(v.z), ordered(v.w)};
+    uint32_t least = 0;
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t t = least | 1u << bit;
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) count += __builtin_popcountll(__ballot(o[i] >= t));
+        if (count >= n) least = t;
+    }
+    return least > 0x007fffffu ? unordered(least) : -__builtin_inff();  // (0x007fffff: -inf itself)
 }
 
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
@@ -785,51 +812,119 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     return v;
 }
 
+// A work-group holds 1024 V words of one beam in registers.
+template <int V>
 __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams p) {
-    __shared__ float red[kCandThreads / 64];
-    __shared__ uint64_t redk[kCandThreads / 64];
+    typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int kWavesHere = kCandThreads / 64;
+    __shared__ __align__(16) float maxima[kGroups];
+    __shared__ double sums[kWavesHere];
+    __shared__ uint64_t keys[kMostRanked];
+    __shared__ uint64_t redk[kWavesHere];
+    __shared__ int held;
     const int b = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     if (p.finished && p.finished[b]) return;
-    const int v0 = c * p.chunk, v1 = min(p.vocab, v0 + p.chunk);
+    const int v0 = c * 1024 * V + 4 * tid;  // this thread's words: v0 + 1024 j + i
     const float* row = p.logits + static_cast<size_t>(b) * p.vocab;
-    float m = -__builtin_inff();
-    for (int v = v0 + tid; v < v1; v += kCandThreads) m = fmaxf(m, clean(row[v]));
-    m = wave_max(m);
-    if (lane == 0) red[wv] = m;
-    __syncthreads();
-    m = red[0];
-    for (int w = 1; w < kCandThreads / 64; ++w) m = fmaxf(m, red[w]);
-    float l = 0.0f;
-    for (int v = v0 + tid; v < v1; v += kCandThreads) {
-        const float x = clean(row[v]);
-        l += x == m ? 1.0f : expf(x - m);  // (x == m: an infinite maximum)
+    float x[V][4], most = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int at = v0 + 1024 * j;
+        if (at + 4 <= p.vocab) {
+            const float4a4 w = *reinterpret_cast<const float4a4*>(row + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] = w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] = at + i < p.vocab ? row[at + i] : -__builtin_inff();
+        }
     }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[j][i] = clean(x[j][i]);
+            most = fmaxf(most, x[j][i]);
+        }
+    maxima[tid] = most;
+    if (tid == 0) held = 0;
+    __syncthreads();
+    // (the first maximum of the search is the part's)
+    float m;
+    {
+        const float4 w = reinterpret_cast<const float4*>(maxima)[lane];
+        m = wave_max(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
+    }
+    float l = 0.0f;
+    if (m > -__builtin_inff())
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = x[j][i] == m ? 1.0f : expf(x[j][i] - m);  // (x == m: an infinite maximum)
+            l += (e[0] + e[1]) + (e[2] + e[3]);
+        }
     l = wave_sum(l);
+    if (lane == 0) sums[wv] = static_cast<double>(l);
+    const float least = nth_largest(maxima, p.n_out, lane);
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += x[j][i] >= least && x[j][i] > -__builtin_inff();
+    if (mine) {
+        int at = atomicAdd(&held, mine);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (x[j][i] >= least && x[j][i] > -__builtin_inff()) {
+                    if (at < kMostRanked) keys[at] = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
+                    ++at;
+                }
+    }
     __syncthreads();
-    if (lane == 0) red[wv] = l;
-    __syncthreads();
-    const size_t at = static_cast<size_t>(b) * p.n_chunks + c;
+    const size_t part = static_cast<size_t>(b) * p.n_chunks + c;
+    float2* best = p.best + part * p.n_out;
     if (tid == 0) {
-        l = 0.0f;
-        for (int w = 0; w < kCandThreads / 64; ++w) l += red[w];
-        p.ml[at] = make_float2(m, l);
+        double s = sums[0];
+#pragma unroll
+        for (int w = 1; w < kWavesHere; ++w) s += sums[w];
+        p.ml[part] = make_float2(m, static_cast<float>(s));
+    }
+    const int n = held;
+    if (n <= kMostRanked) {
+        for (int i = tid; i < n; i += kCandThreads) {
+            const uint64_t k = keys[i];
+            int rank = 0;
+            for (int o = 0; o < n; ++o) rank += keys[o] > k;
+            if (rank < p.n_out)
+                best[rank] = make_float2(unordered(static_cast<uint32_t>(k >> 32)),
+                                         __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
+        }
+        for (int i = n + tid; i < p.n_out; i += kCandThreads) best[i] = make_float2(-__builtin_inff(), 0.0f);
+        return;
     }
     uint64_t last = ~uint64_t{0};
-    for (int i = 0; i < p.n_out; ++i) {
+    for (int r = 0; r < p.n_out; ++r) {
         uint64_t k = 0;
-        for (int v = v0 + tid; v < v1; v += kCandThreads) {
-            const uint64_t kv = key_of(clean(row[v]), static_cast<uint32_t>(v));
-            if (kv < last && kv > k) k = kv;
-        }
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t o = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
+                if (x[j][i] > -__builtin_inff() && o < last && o > k) k = o;
+            }
         k = wave_max_u64(k);
         __syncthreads();
         if (lane == 0) redk[wv] = k;
         __syncthreads();
         k = redk[0];
-        for (int w = 1; w < kCandThreads / 64; ++w) k = redk[w] > k ? redk[w] : k;
+#pragma unroll
+        for (int w = 1; w < kWavesHere; ++w) k = redk[w] > k ? redk[w] : k;
         if (tid == 0)
-            p.best[at * p.n_out + i] = k ? make_float2(logit_of(k), __builtin_bit_cast(float, ~static_cast<uint32_t>(k)))
-                                         : make_float2(-__builtin_inff(), 0.0f);
+            best[r] = make_float2(k ? unordered(static_cast<uint32_t>(k >> 32)) : -__builtin_inff(),
+                                  __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
         last = k;
     }
 }
@@ -840,48 +935,94 @@ struct Candidate {
     __device__ bool before(const Candidate& o) const { return score > o.score || (score == o.score && at < o.at); }
 };
 
-__global__ __launch_bounds__(kCandThreads) void select_join_kernel(SelectParams p) {
-    __shared__ double base[kMaxBeams];  // scores[b] - log sum: -inf for a beam with nothing left
+constexpr int kJoinThreads = 1024;
+__global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams p) {
+    constexpr int kWavesHere = kJoinThreads / 64;
+    __shared__ double base[kMaxBeams];  // scores[b] - log sum; -inf for a beam with nothing left
     __shared__ float top[kMaxBeams];
-    __shared__ bool ended[kMaxBeams];  // (finished may be one of the outputs)
-    __shared__ double reds[kCandThreads / 64];
-    __shared__ int64_t reda[kCandThreads / 64];
+    __shared__ bool ended[kMaxBeams];   // (finished and scores may be among the outputs)
+    __shared__ __align__(16) float maxima[kGroups];
+    __shared__ Candidate ranked[kMostRanked];
+    __shared__ int held;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const double inf = __builtin_inf();
-    if (tid < p.n_beams) {
-        const float s = clean(p.scores[tid]);
-        const bool done = p.finished && p.finished[tid];
+    const int per = p.n_chunks * p.n_out, total = p.n_beams * per;
+    if (tid == 0) held = 0;
+    // a wave per beam: the parts' maxima and sums
+    for (int b = wv; b < p.n_beams; b += kWavesHere) {
+        const float s = clean(p.scores[b]);
+        const bool done = p.finished && p.finished[b];
         float m = -__builtin_inff();
         double sum = 0.0;
         if (!done) {
-            for (int c = 0; c < p.n_chunks; ++c) m = fmaxf(m, p.ml[static_cast<size_t>(tid) * p.n_chunks + c].x);
-            for (int c = 0; c < p.n_chunks; ++c) {
-                const float2 v = p.ml[static_cast<size_t>(tid) * p.n_chunks + c];
+            const float2* ml = p.ml + static_cast<size_t>(b) * p.n_chunks;
+            for (int c = lane; c < p.n_chunks; c += 64) m = fmaxf(m, ml[c].x);
+            m = wave_max(m);
+            for (int c = lane; c < p.n_chunks; c += 64) {
+                const float2 v = ml[c];
                 if (v.x > -__builtin_inff())
                     sum += static_cast<double>(v.y) *
                            (v.x == m ? 1.0 : exp(static_cast<double>(v.x) - static_cast<double>(m)));
             }
+#pragma unroll
+            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
         }
-        top[tid] = m;
-        ended[tid] = done;
-        base[tid] = done ? s : m > -__builtin_inff() ? static_cast<double>(s) - log(sum) : -inf;
+        if (lane == 0) {
+            top[b] = m;
+            ended[b] = done;
+            base[b] = done ? s : m > -__builtin_inff() ? static_cast<double>(s) - log(sum) : -inf;
+        }
     }
     __syncthreads();
-    const int per = p.n_chunks * p.n_out, total = p.n_beams * per;
-    Candidate last{inf, -1};
-    for (int i = 0; i < p.n_out; ++i) {
-        Candidate mine{-inf, INT64_MAX};
-        for (int j = tid; j < total; j += kCandThreads) {
-            const int b = j / per;
-            Candidate c{-inf, INT64_MAX};
-            if (ended[b]) {
-                if (j % per == 0) c = {base[b], static_cast<int64_t>(b) * p.vocab + p.finished_token};
-            } else {
-                const float2 e = p.best[j];
-                if (e.x > -__builtin_inff())
-                    c = {base[b] + (e.x == top[b] ? 0.0 : static_cast<double>(e.x) - static_cast<double>(top[b])),
+    auto candidate = [&](int j) {
+        const int b = j / per;
+        if (ended[b]) return j % per ? Candidate{-inf, 0} : Candidate{base[b], static_cast<int64_t>(b) * p.vocab + p.finished_token};
+        const float2 e = p.best[j];
+        if (!(e.x > -__builtin_inff())) return Candidate{-inf, 0};
+        return Candidate{base[b] + (e.x == top[b] ? 0.0 : static_cast<double>(e.x) - static_cast<double>(top[b])),
                          static_cast<int64_t>(b) * p.vocab + __builtin_bit_cast(int32_t, e.y)};
-            }
+    };
+    // (a score's float is in the scores' order, so the threshold holds for floats)
+    float most = -__builtin_inff();
+    for (int j = tid; j < total; j += kJoinThreads) most = fmaxf(most, static_cast<float>(candidate(j).score));
+    most = fmaxf(most, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, most), 0xb1, 0xf, 0xf, false)));
+    most = fmaxf(most, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, most), 0x4e, 0xf, 0xf, false)));
+    if (tid % 4 == 0) maxima[tid / 4] = most;
+    __syncthreads();
+    const float least = nth_largest(maxima, p.n_out, lane);
+    for (int j = tid; j < total; j += kJoinThreads) {
+        const Candidate c = candidate(j);
+        if (c.score > -inf && static_cast<float>(c.score) >= least) {
+            const int at = atomicAdd(&held, 1);
+            if (at < kMostRanked) ranked[at] = c;
+        }
+    }
+    __syncthreads();
+    auto write = [&](int i, const Candidate& c) {
+        p.out_parents[i] = static_cast<int32_t>(c.at / p.vocab);
+        p.out_tokens[i] = static_cast<int32_t>(c.at % p.vocab);
+        p.out_scores[i] = static_cast<float>(c.score);
+    };
+    auto write_none = [&](int i) {
+        p.out_parents[i] = p.out_tokens[i] = -1;
+        p.out_scores[i] = -__builtin_inff();
+    };
+    const int n = held;
+    if (n <= kMostRanked) {
+        for (int i = tid; i < n; i += kJoinThreads) {
+            const Candidate c = ranked[i];
+            int rank = 0;
+            for (int o = 0; o < n; ++o) rank += ranked[o].before(c);
+            if (rank < p.n_out) write(rank, c);
+        }
+        for (int i = n + tid; i < p.n_out; i += kJoinThreads) write_none(i);
+        return;
+    }
+    Candidate last{inf, -1};
+    for (int r = 0; r < p.n_out; ++r) {
+        Candidate mine{-inf, INT64_MAX};
+        for (int j = tid; j < total; j += kJoinThreads) {
+            const Candidate c = candidate(j);
             if (c.score > -inf && last.before(c) && c.before(mine)) mine = c;
         }
 #pragma unroll
@@ -890,26 +1031,22 @@ __global__ __launch_bounds__(kCandThreads) void select_join_kernel(SelectParams 
             if (o.before(mine)) mine = o;
         }
         __syncthreads();
-        if (lane == 0) {
-            reds[wv] = mine.score;
-            reda[wv] = mine.at;
-        }
+        if (lane == 0) ranked[wv] = mine;
         __syncthreads();
-        last = {reds[0], reda[0]};
-        for (int w = 1; w < kCandThreads / 64; ++w) {
-            const Candidate o{reds[w], reda[w]};
-            if (o.before(last)) last = o;
-        }
-        if (tid == 0) {
-            const bool some = last.score > -inf;
-            p.out_parents[i] = some ? static_cast<int32_t>(last.at / p.vocab) : -1;
-            p.out_tokens[i] = some ? static_cast<int32_t>(last.at % p.vocab) : -1;
-            p.out_scores[i] = some ? static_cast<float>(last.score) : -__builtin_inff();
-        }
+        last = ranked[0];
+        for (int w = 1; w < kWavesHere; ++w)
+            if (ranked[w].before(last)) last = ranked[w];
+        if (tid == 0) write(r, last);
     }
 }
 
-int32_t select_chunk(int32_t vocab) { return vocab < 4096 ? vocab : 4096; }
+// float4 of a thread (a work-group takes 1024 times as many words): the fewest
+// that leave 512 parts, so that the second kernel has little to read
+int32_t select_vectors(int32_t n_beams, int32_t vocab) {
+    int32_t v = 2;
+    while (v < 16 && static_cast<int64_t>(n_beams) * ((vocab + 1024 * v - 1) / (1024 * v)) > 512) v *= 2;
+    return v;
+}
 
 template <class F>
 hipError_t by_layers(float* const* k, float* const* v, int32_t n_layers, F&& launch) {
@@ -968,8 +1105,8 @@ hipError_t launch_kv_reorder(float* const* k, float* const* v, int32_t n_layers,
 }
 
 size_t beam_select_workspace_bytes(int32_t n_beams, int32_t vocab, int32_t n_out) {
-    const size_t chunk = select_chunk(vocab), parts = static_cast<size_t>(n_beams) * ((vocab + chunk - 1) / chunk);
-    return parts * sizeof(float2) * (1 + static_cast<size_t>(n_out));
+    const int32_t words = 1024 * select_vectors(n_beams, vocab);
+    return static_cast<size_t>(n_beams) * ((vocab + words - 1) / words) * sizeof(float2) * (1 + static_cast<size_t>(n_out));
 }
 
 hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,
@@ -987,17 +1124,21 @@ hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t voca
     p.n_beams = n_beams;
     p.vocab = vocab;
     p.n_out = n_out;
-    p.chunk = select_chunk(vocab);
-    p.n_chunks = (vocab + p.chunk - 1) / p.chunk;
+    const int32_t v = select_vectors(n_beams, vocab);
+    p.n_chunks = (vocab + 1024 * v - 1) / (1024 * v);
     p.ml = static_cast<float2*>(workspace);
     p.best = p.ml + static_cast<size_t>(n_beams) * p.n_chunks;
     p.out_parents = out_parents;
     p.out_tokens = out_tokens;
     p.out_scores = out_scores;
-    hipLaunchKernelGGL(select_parts_kernel, dim3(p.n_chunks, n_beams), dim3(kCandThreads), 0, stream, p);
+    const dim3 grid(p.n_chunks, n_beams);
+    if (v == 2) hipLaunchKernelGGL(select_parts_kernel<2>, grid, dim3(kCandThreads), 0, stream, p);
+    else if (v == 4) hipLaunchKernelGGL(select_parts_kernel<4>, grid, dim3(kCandThreads), 0, stream, p);
+    else if (v == 8) hipLaunchKernelGGL(select_parts_kernel<8>, grid, dim3(kCandThreads), 0, stream, p);
+    else hipLaunchKernelGGL(select_parts_kernel<16>, grid, dim3(kCandThreads), 0, stream, p);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(select_join_kernel, dim3(1), dim3(kCandThreads), 0, stream, p);
+    hipLaunchKernelGGL(select_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, p);
     return hipGetLastError();
 }
 
