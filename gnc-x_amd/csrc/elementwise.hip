@@ -692,9 +692,11 @@ struct LayerCaches {
 
 // ---- rows of an accepted path ----------------------------------------------
 // Row row0 + i of every cache becomes the old row row0 + rows[i], rows
-// ascending.  A thread owns one float4 column of one cache and moves its rows
-// in order: as rows[i] >= i, no row is overwritten before it is read, and no
-// thread touches another's column, so the move is in place without a barrier.
+// ascending.  A thread owns one column (W floats) of one cache and moves its rows
+// in order, sixteen loads before their sixteen stores: as rows[i] >= i and the
+// rows ascend, no row is overwritten before it is read, and no thread touches
+// another's column, so the move is in place without a barrier.  Rows that stay
+// (rows[i] == i, the first ones only) are left out by the caller.
 struct KeepParams {
     LayerCaches caches;
     int32_t kv_dim, n;
@@ -702,15 +704,21 @@ struct KeepParams {
     uint16_t rows[kMaxKeepRows];
 };
 
-__global__ __launch_bounds__(kCandThreads) void keep_rows_kernel(KeepParams p) {
-    const int d4 = static_cast<int>(blockIdx.x * kCandThreads + threadIdx.x);
-    if (4 * d4 >= p.kv_dim) return;
-    float* c = p.caches.c[blockIdx.y] + p.row0 * p.kv_dim + 4 * d4;
-    for (int i = 0; i < p.n; ++i) {
-        const int r = p.rows[i];
-        if (r != i)
-            *reinterpret_cast<float4*>(c + static_cast<size_t>(i) * p.kv_dim) =
-                *reinterpret_cast<const float4*>(c + static_cast<size_t>(r) * p.kv_dim);
+template <int W>
+__global__ __launch_bounds__(64) void keep_rows_kernel(KeepParams p) {
+    typedef float vec __attribute__((ext_vector_type(W)));
+    constexpr int kAtOnce = 16;
+    const int d = W * static_cast<int>(blockIdx.x * 64 + threadIdx.x);
+    if (d >= p.kv_dim) return;
+    float* c = p.caches.c[blockIdx.y] + p.row0 * p.kv_dim + d;
+    for (int i = 0; i < p.n; i += kAtOnce) {
+        vec v[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)  // (past the end: the last row again)
+            v[u] = *reinterpret_cast<const vec*>(c + static_cast<size_t>(p.rows[min(i + u, p.n - 1)]) * p.kv_dim);
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u)
+            if (i + u < p.n) *reinterpret_cast<vec*>(c + static_cast<size_t>(i + u) * p.kv_dim) = v[u];
     }
 }
 
@@ -786,14 +794,14 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t word) {
     return static_cast<uint64_t>(ordered(x)) << 32 | ~word;
 }
 
-// A lower bound (its last 12 bits cleared) on the n-th largest of the 256 floats
+// A lower bound (its last 14 bits cleared) on the n-th largest of the 256 floats
 // at maxima, by a wave: bit after bit of the ordered form, kept while n of them
 // reach it.
 __device__ __forceinline__ float nth_largest(const float* maxima, int n, int lane) {
     const float4 v = reinterpret_cast<const float4*>(maxima)[lane];
     const uint32_t o[4] = {ordered(v.x), ordered(v.y), ordered(v.z), ordered(v.w)};
     uint32_t least = 0;
-    for (int bit = 31; bit >= 12; --bit) {
+    for (int bit = 31; bit >= 14; --bit) {
         const uint32_t t = least | 1u << bit;
         int count = 0;
 #pragma unroll
@@ -897,6 +905,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
         for (int i = tid; i < n; i += kCandThreads) {
             const uint64_t k = keys[i];
             int rank = 0;
+#pragma unroll 8
             for (int o = 0; o < n; ++o) rank += keys[o] > k;
             if (rank < p.n_out)
                 best[rank] = make_float2(unordered(static_cast<uint32_t>(k >> 32)),
@@ -946,8 +955,16 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
     __shared__ int held;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const double inf = __builtin_inf();
-    const int per = p.n_chunks * p.n_out, total = p.n_beams * per;
+    // entries of a part that the threshold is taken from: 2^shift
+    const int parts = p.n_beams * p.n_chunks;
+    int shift = 0;
+    while (parts << shift < kGroups && 1 << shift < p.n_out) ++shift;
+    const int first = 1 << shift;
     if (tid == 0) held = 0;
+    // (read ahead of what needs the beams' sums)
+    float2 ahead = make_float2(-__builtin_inff(), 0.0f);
+    if (tid < kGroups && tid < parts << shift && (tid & first - 1) < p.n_out)
+        ahead = p.best[static_cast<size_t>(tid >> shift) * p.n_out + (tid & first - 1)];
     // a wave per beam: the parts' maxima and sums
     for (int b = wv; b < p.n_beams; b += kWavesHere) {
         const float s = clean(p.scores[b]);
@@ -974,29 +991,41 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
         }
     }
     __syncthreads();
-    auto candidate = [&](int j) {
-        const int b = j / per;
-        if (ended[b]) return j % per ? Candidate{-inf, 0} : Candidate{base[b], static_cast<int64_t>(b) * p.vocab + p.finished_token};
-        const float2 e = p.best[j];
+    // the r-th best candidate of a part; -inf behind the last
+    auto entry = [&](int part, int r, float2 e) {
+        const int b = part / p.n_chunks;
+        if (ended[b])
+            return r || part % p.n_chunks ? Candidate{-inf, 0}
+                                          : Candidate{base[b], static_cast<int64_t>(b) * p.vocab + p.finished_token};
         if (!(e.x > -__builtin_inff())) return Candidate{-inf, 0};
         return Candidate{base[b] + (e.x == top[b] ? 0.0 : static_cast<double>(e.x) - static_cast<double>(top[b])),
                          static_cast<int64_t>(b) * p.vocab + __builtin_bit_cast(int32_t, e.y)};
     };
-    // (a score's float is in the scores' order, so the threshold holds for floats)
-    float most = -__builtin_inff();
-    for (int j = tid; j < total; j += kJoinThreads) most = fmaxf(most, static_cast<float>(candidate(j).score));
-    most = fmaxf(most, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, most), 0xb1, 0xf, 0xf, false)));
-    most = fmaxf(most, __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, most), 0x4e, 0xf, 0xf, false)));
-    if (tid % 4 == 0) maxima[tid / 4] = most;
+    auto candidate = [&](int part, int r) { return entry(part, r, p.best[static_cast<size_t>(part) * p.n_out + r]); };
+    // The parts' lists fall, so the threshold comes from their first entries (as
+    // many of each as make kGroups), and a list is read on only while it stays
+    // above.  A score's float is in the scores' order, so floats serve.
+    if (tid < kGroups) {
+        float most = tid < parts << shift && (tid & first - 1) < p.n_out
+                         ? static_cast<float>(entry(tid >> shift, tid & first - 1, ahead).score)
+                         : -__builtin_inff();
+        for (int j = tid + kGroups; j < parts << shift; j += kGroups)
+            if ((j & first - 1) < p.n_out)
+                most = fmaxf(most, static_cast<float>(candidate(j >> shift, j & first - 1).score));
+        maxima[tid] = most;
+    }
     __syncthreads();
     const float least = nth_largest(maxima, p.n_out, lane);
-    for (int j = tid; j < total; j += kJoinThreads) {
-        const Candidate c = candidate(j);
-        if (c.score > -inf && static_cast<float>(c.score) >= least) {
+    // (eight entries of a list at once, and on from there one by one)
+    const int wide = max(shift, 3), batch = 1 << wide;
+    for (int j = tid; j < parts << wide; j += kJoinThreads)
+        for (int r = j & batch - 1; r < p.n_out; ++r) {
+            const Candidate c = candidate(j >> wide, r);
+            if (!(c.score > -inf && static_cast<float>(c.score) >= least)) break;
             const int at = atomicAdd(&held, 1);
             if (at < kMostRanked) ranked[at] = c;
+            if (r < batch - 1) break;
         }
-    }
     __syncthreads();
     auto write = [&](int i, const Candidate& c) {
         p.out_parents[i] = static_cast<int32_t>(c.at / p.vocab);
@@ -1012,6 +1041,7 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
         for (int i = tid; i < n; i += kJoinThreads) {
             const Candidate c = ranked[i];
             int rank = 0;
+#pragma unroll 4
             for (int o = 0; o < n; ++o) rank += ranked[o].before(c);
             if (rank < p.n_out) write(rank, c);
         }
@@ -1021,8 +1051,8 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
     Candidate last{inf, -1};
     for (int r = 0; r < p.n_out; ++r) {
         Candidate mine{-inf, INT64_MAX};
-        for (int j = tid; j < total; j += kJoinThreads) {
-            const Candidate c = candidate(j);
+        for (int j = tid; j < parts * p.n_out; j += kJoinThreads) {
+            const Candidate c = candidate(j / p.n_out, j % p.n_out);
             if (c.score > -inf && last.before(c) && c.before(mine)) mine = c;
         }
 #pragma unroll
@@ -1069,15 +1099,23 @@ hipError_t by_layers(float* const* k, float* const* v, int32_t n_layers, F&& lau
 hipError_t launch_kv_keep_rows(float* const* k, float* const* v, int32_t n_layers, int32_t kv_dim, int32_t row0,
                                const int32_t* rows, int32_t n, hipStream_t stream) {
     if (n < 0 || n > kMaxKeepRows || kv_dim < 4 || kv_dim % 4 || row0 < 0) return hipErrorInvalidValue;
+    int32_t stay = 0;
+    while (stay < n && rows[stay] == stay) ++stay;
+    if (stay == n) return hipSuccess;
     KeepParams p{};
     p.kv_dim = kv_dim;
-    p.n = n;
-    p.row0 = static_cast<size_t>(row0);
-    for (int32_t i = 0; i < n; ++i) p.rows[i] = static_cast<uint16_t>(rows[i]);
+    p.n = n - stay;
+    p.row0 = static_cast<size_t>(row0) + stay;
+    for (int32_t i = stay; i < n; ++i) p.rows[i - stay] = static_cast<uint16_t>(rows[i] - stay);
+    // one float a thread while that leaves fewer than 4096 waves (a wave's loads
+    // are then whole 256-byte lines of a row), else four
+    const bool narrow = static_cast<int64_t>(n_layers) * 2 * ((kv_dim + 63) / 64) < 4096;
+    const int32_t per = narrow ? 64 : 256;
     return by_layers(k, v, n_layers, [&](const LayerCaches& c, int32_t caches) {
         p.caches = c;
-        hipLaunchKernelGGL(keep_rows_kernel, dim3((kv_dim / 4 + kCandThreads - 1) / kCandThreads, caches), dim3(kCandThreads), 0,
-                           stream, p);
+        const dim3 grid((kv_dim + per - 1) / per, caches);
+        if (narrow) hipLaunchKernelGGL(keep_rows_kernel<1>, grid, dim3(64), 0, stream, p);
+        else hipLaunchKernelGGL(keep_rows_kernel<4>, grid, dim3(64), 0, stream, p);
     });
 }
 
