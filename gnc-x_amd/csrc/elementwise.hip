@@ -724,9 +724,13 @@ __global__ __launch_bounds__(64) void keep_rows_kernel(KeepParams p) {
 
 // ---- reordering of beams ------------------------------------------------------
 // Rows [row0, row0 + n_rows) of beam b become those of beam parents[b].  A
-// thread owns one float4 of one row in all beams: it loads every moving beam's
-// new value before it stores any, so the exchange is in place with no second
-// copy of the caches.  A parent outside [0, n_beams) leaves its beam as it is.
+// thread owns U float4 of a cache's rows in all beams: it loads every moving
+// beam's new values before it stores any, so the exchange is in place with no
+// second copy of the caches.  A parent outside [0, n_beams) leaves its beam as it
+// is.  Bound by memory: 8 beams x 1000 rows x 1024 x 24 caches, 1.08 GB with four
+// distinct parents, 316 us with one float4 a thread and beam (too few bytes in
+// flight for its waits), 217 with four, 168 (6.4 TB/s) with stores that the caches
+// do not keep as well.
 struct ReorderParams {
     LayerCaches caches;
     size_t beam_stride, count;  // floats; float4 of a beam's rows
@@ -735,22 +739,37 @@ struct ReorderParams {
     const int32_t* parents;
 };
 
-template <int NB>
+template <int NB, int U>
 __global__ __launch_bounds__(kCandThreads) void reorder_kernel(ReorderParams p) {
-    const size_t i = static_cast<size_t>(blockIdx.x) * kCandThreads + threadIdx.x;
-    if (i >= p.count) return;
-    float* c = p.caches.c[blockIdx.y] + p.start + 4 * i;
-    float4 v[NB];
-    bool moves[NB];
+    typedef float vec __attribute__((ext_vector_type(4)));
+    const size_t first = static_cast<size_t>(blockIdx.x) * U * kCandThreads + threadIdx.x;
+    float* c = p.caches.c[blockIdx.y] + p.start;
+    vec v[U][NB];
+    int from[NB];
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-        const int from = b < p.n_beams ? p.parents[b] : b;
-        moves[b] = from != b && from >= 0 && from < p.n_beams;
-        if (moves[b]) v[b] = *reinterpret_cast<const float4*>(c + static_cast<size_t>(from) * p.beam_stride);
+        const int f = b < p.n_beams ? p.parents[b] : b;
+        from[b] = f >= 0 && f < p.n_beams ? f : b;
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
-        if (moves[b]) *reinterpret_cast<float4*>(c + static_cast<size_t>(b) * p.beam_stride) = v[b];
+    for (int u = 0; u < U; ++u) {
+        const size_t i = first + u * kCandThreads;
+        if (i < p.count)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (from[b] != b)
+                    v[u][b] = *reinterpret_cast<const vec*>(c + 4 * i + static_cast<size_t>(from[b]) * p.beam_stride);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const size_t i = first + u * kCandThreads;
+        if (i < p.count)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+                if (from[b] != b)
+                    __builtin_nontemporal_store(v[u][b],
+                                                reinterpret_cast<vec*>(c + 4 * i + static_cast<size_t>(b) * p.beam_stride));
+    }
 }
 
 // ---- beam search's selection ------------------------------------------------------
@@ -1130,15 +1149,21 @@ hipError_t launch_kv_reorder(float* const* k, float* const* v, int32_t n_layers,
     p.start = static_cast<size_t>(row0) * kv_dim;
     p.n_beams = n_beams;
     p.parents = parents;
-    const size_t groups = (p.count + kCandThreads - 1) / kCandThreads;
+    // as many float4 a thread and beam as 128 registers hold where that leaves
+    // 2048 work-groups, else one
+    const int32_t most = n_beams <= 8 ? 4 : n_beams <= 16 ? 2 : 1;
+    const size_t tiles = (p.count + kCandThreads - 1) / kCandThreads;
+    const int32_t u = tiles * 2 * n_layers >= 2048 * static_cast<size_t>(most) ? most : 1;
+    const size_t groups = (tiles + u - 1) / u;
     if (groups > 0x7fffffffu) return hipErrorInvalidValue;
     return by_layers(k, v, n_layers, [&](const LayerCaches& c, int32_t caches) {
         p.caches = c;
         const dim3 grid(static_cast<uint32_t>(groups), caches);
-        if (n_beams <= 4) hipLaunchKernelGGL(reorder_kernel<4>, grid, dim3(kCandThreads), 0, stream, p);
-        else if (n_beams <= 8) hipLaunchKernelGGL(reorder_kernel<8>, grid, dim3(kCandThreads), 0, stream, p);
-        else if (n_beams <= 16) hipLaunchKernelGGL(reorder_kernel<16>, grid, dim3(kCandThreads), 0, stream, p);
-        else hipLaunchKernelGGL(reorder_kernel<32>, grid, dim3(kCandThreads), 0, stream, p);
+        if (n_beams <= 4 && u == 4) hipLaunchKernelGGL((reorder_kernel<4, 4>), grid, dim3(kCandThreads), 0, stream, p);
+        else if (n_beams <= 8 && u == 4) hipLaunchKernelGGL((reorder_kernel<8, 4>), grid, dim3(kCandThreads), 0, stream, p);
+        else if (n_beams <= 8) hipLaunchKernelGGL((reorder_kernel<8, 1>), grid, dim3(kCandThreads), 0, stream, p);
+        else if (n_beams <= 16 && u == 2) hipLaunchKernelGGL((reorder_kernel<16, 2>), grid, dim3(kCandThreads), 0, stream, p);
+        else hipLaunchKernelGGL((reorder_kernel<32, 1>), grid, dim3(kCandThreads), 0, stream, p);
     });
 }
 

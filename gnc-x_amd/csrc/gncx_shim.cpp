@@ -3011,10 +3011,11 @@ bool layer_caches(float* const* k, float* const* v, int32_t n_layers, size_t lo,
     const size_t step = sizeof(float) * stride, own = sizeof(float) * (floats - lo);
     static std::vector<std::pair<uintptr_t, uintptr_t>> at;  // (place within a stride, address); the call lock is held
     at.clear();
-    uintptr_t base = 0, end = 0;  // the last pointer's allocation
+    uintptr_t bases[2] = {0, 0}, ends[2] = {0, 0};  // the last k cache's and v cache's allocations
     for (int32_t i = 0; i < 2 * n_layers; ++i) {
         const float* p = i % 2 ? v[i / 2] : k[i / 2];
         const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+        uintptr_t &base = bases[i % 2], &end = ends[i % 2];
         if (a < base || a >= end || a % 16) {
             if (!on_device(p, i % 2 ? "every v cache" : "every k cache", where, 16)) return false;
             hipDeviceptr_t b = nullptr;
