@@ -729,8 +729,8 @@ __global__ __launch_bounds__(64) void keep_rows_kernel(KeepParams p) {
 // second copy of the caches.  A parent outside [0, n_beams) leaves its beam as it
 // is.  Bound by memory: 8 beams x 1000 rows x 1024 x 24 caches, 1.08 GB with four
 // distinct parents, 316 us with one float4 a thread and beam (too few bytes in
-// flight for its waits), 217 with four, 168 (6.4 TB/s) with stores that the caches
-// do not keep as well.
+// flight for its waits), 217 with four, 168 (6.4 TB/s) with stores that pass the
+// caches, too.
 struct ReorderParams {
     LayerCaches caches;
     size_t beam_stride, count;  // floats; float4 of a beam's rows
@@ -1149,18 +1149,19 @@ hipError_t launch_kv_reorder(float* const* k, float* const* v, int32_t n_layers,
     p.start = static_cast<size_t>(row0) * kv_dim;
     p.n_beams = n_beams;
     p.parents = parents;
-    // as many float4 a thread and beam as 128 registers hold where that leaves
-    // 2048 work-groups, else one
-    const int32_t most = n_beams <= 8 ? 4 : n_beams <= 16 ? 2 : 1;
-    const size_t tiles = (p.count + kCandThreads - 1) / kCandThreads;
-    const int32_t u = tiles * 2 * n_layers >= 2048 * static_cast<size_t>(most) ? most : 1;
+    // float4 a thread and beam (128 registers hold 32 of them): one, two, four,
+    // us: 8 beams x 1000 rows x 1024 x 24 caches 307, 187, 168; 8 x 100 x 72 caches
+    // 58, 47, 48; 4 x 5 x 72 4.2, 3.4, 4.6; 8 x 10 rows of 512 x 8 (40 tiles) 4.2,
+    // 8.0, 8.4
+    const size_t tiles = (p.count + kCandThreads - 1) / kCandThreads, all = tiles * 2 * n_layers;
+    const int32_t u = all < 256 || n_beams > 16 ? 1 : all < 16384 || n_beams > 8 ? 2 : 4;
     const size_t groups = (tiles + u - 1) / u;
     if (groups > 0x7fffffffu) return hipErrorInvalidValue;
     return by_layers(k, v, n_layers, [&](const LayerCaches& c, int32_t caches) {
         p.caches = c;
         const dim3 grid(static_cast<uint32_t>(groups), caches);
-        if (n_beams <= 4 && u == 4) hipLaunchKernelGGL((reorder_kernel<4, 4>), grid, dim3(kCandThreads), 0, stream, p);
-        else if (n_beams <= 8 && u == 4) hipLaunchKernelGGL((reorder_kernel<8, 4>), grid, dim3(kCandThreads), 0, stream, p);
+        if (n_beams <= 8 && u == 4) hipLaunchKernelGGL((reorder_kernel<8, 4>), grid, dim3(kCandThreads), 0, stream, p);
+        else if (n_beams <= 8 && u == 2) hipLaunchKernelGGL((reorder_kernel<8, 2>), grid, dim3(kCandThreads), 0, stream, p);
         else if (n_beams <= 8) hipLaunchKernelGGL((reorder_kernel<8, 1>), grid, dim3(kCandThreads), 0, stream, p);
         else if (n_beams <= 16 && u == 2) hipLaunchKernelGGL((reorder_kernel<16, 2>), grid, dim3(kCandThreads), 0, stream, p);
         else hipLaunchKernelGGL((reorder_kernel<32, 1>), grid, dim3(kCandThreads), 0, stream, p);
