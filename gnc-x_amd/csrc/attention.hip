@@ -21,6 +21,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 #include "gncx_device.h"
@@ -1852,6 +1853,7 @@ __device__ __forceinline__ void join_parts(const TreeParams& p, const float4* sh
     const bool whole = gridDim.z == 1;
     const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
     const int count = min(32 * tiles, rows - row0) * (HD / 4);
+#pragma unroll 4
     for (int i = threadIdx.x; i < count; i += kThreads) {
         const int r = i / (HD / 4), d4 = i % (HD / 4);
         float M = mls[r / 32][r % 32].x, L = mls[r / 32][r % 32].y;
@@ -1963,6 +1965,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
         if (kAhead) load_v(first);
     }
 
+    const int myrow = min(row0 + li, rows - 1);
+    const RowPlace place = place_of(p, myrow / G);
     // the query rows, 8 threads each: scaled, split and laid out as operands
     {
         const int r = row0 + tid / 8, j = tid % 8;
@@ -1987,8 +1991,6 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
         if (j == 0) qfac[tid / 8] = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
     }
     if (c1 > p.pos0) load_tree(p, tree);
-    const int myrow = min(row0 + li, rows - 1);
-    const RowPlace place = place_of(p, myrow / G);
     const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.tree.max_depth - p.sw + 1) : 0;
     __syncthreads();
 
@@ -2420,48 +2422,61 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
 }
 
 // out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the key
-// ranges c, a thread per float4, sixteen ranges' loads issued at once.
-constexpr int kTreeMergeLoads = 16;
-template <int HD>
+// ranges c.  CG threads share a float4 of the output, each with every CG-th
+// range, at most eight, whose loads go out at once; their sums meet in LDS.
+constexpr int kTreeMergeLoads = 8;
+template <int HD, int CG>
 __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams p, int32_t chunks) {
+    static_assert(kTreeMergeLoads * 8 >= kTreeMaxChunks, "eight threads take every range");
+    constexpr int kCols = kThreads / CG;  // float4 of a work-group
+    __shared__ float4 part[CG][kCols];
+    __shared__ float2 mls[CG][kCols];
     const int G = p.n_heads / p.n_kv, rows = p.n * G, hk = blockIdx.y;
-    const int i = static_cast<int>(blockIdx.x) * kThreads + static_cast<int>(threadIdx.x);
-    const int row = i / (HD / 4), d4 = i % (HD / 4);
-    if (row >= rows) return;
-    float M = -1e30f, L = 0.0f, x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 0; c0 < chunks; c0 += kTreeMergeLoads) {
-        float2 ml[kTreeMergeLoads];
-        float4 v[kTreeMergeLoads];
+    const int col = threadIdx.x % kCols, cg = threadIdx.x / kCols;
+    const int i = static_cast<int>(blockIdx.x) * kCols + col, row = min(i / (HD / 4), rows - 1), d4 = i % (HD / 4);
+    float2 ml[kTreeMergeLoads];
+    float4 v[kTreeMergeLoads];
 #pragma unroll
-        for (int u = 0; u < kTreeMergeLoads; ++u) {
-            const int c = min(c0 + u, chunks - 1);
-            const size_t at = (static_cast<size_t>(c) * p.n_kv + hk) * p.rows_pad + row;
-            ml[u] = p.part_ml[at];
-            v[u] = reinterpret_cast<const float4*>(p.part_o + at * HD)[d4];
-        }
-        float m2 = M;
-#pragma unroll
-        for (int u = 0; u < kTreeMergeLoads; ++u) m2 = fmaxf(m2, ml[u].x);
-        const float a = __builtin_amdgcn_exp2f(M - m2);
-        M = m2;
-        L *= a;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[k] *= a;
-#pragma unroll
-        for (int u = 0; u < kTreeMergeLoads; ++u) {
-            const float wt = c0 + u < chunks ? ml[u].y * __builtin_amdgcn_exp2f(ml[u].x - m2) : 0.0f;
-            L += wt;
-            if (wt != 0.0f) {
-                x[0] += wt * v[u].x;
-                x[1] += wt * v[u].y;
-                x[2] += wt * v[u].z;
-                x[3] += wt * v[u].w;
-            }
-        }
+    for (int u = 0; u < kTreeMergeLoads; ++u) {
+        const int c = min(cg + u * CG, chunks - 1);
+        const size_t at = (static_cast<size_t>(c) * p.n_kv + hk) * p.rows_pad + row;
+        ml[u] = p.part_ml[at];
+        v[u] = reinterpret_cast<const float4*>(p.part_o + at * HD)[d4];
     }
+    auto join = [](float m, float l, const float4& o, float M, float& L, float4& x) {
+        const float wt = l * __builtin_amdgcn_exp2f(m - M);
+        L += wt;
+        if (wt != 0.0f) {  // (a part without a key has nothing to add)
+            x.x += wt * o.x;
+            x.y += wt * o.y;
+            x.z += wt * o.z;
+            x.w += wt * o.w;
+        }
+    };
+    float M = -1e30f, L = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int u = 0; u < kTreeMergeLoads; ++u) M = fmaxf(M, ml[u].x);
+#pragma unroll
+    for (int u = 0; u < kTreeMergeLoads; ++u) join(ml[u].x, cg + u * CG < chunks ? ml[u].y : 0.0f, v[u], M, L, x);
+    if constexpr (CG > 1) {
+        // the threads' sums, normalised like the ranges' parts
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        part[cg][col] = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        mls[cg][col] = make_float2(M, L);
+        __syncthreads();
+        if (cg) return;
+        x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        L = 0.0f;
+#pragma unroll
+        for (int c = 1; c < CG; ++c) M = fmaxf(M, mls[c][col].x);
+#pragma unroll
+        for (int c = 0; c < CG; ++c) join(mls[c][col].x, mls[c][col].y, part[c][col], M, L, x);
+    }
+    if (i / (HD / 4) >= rows) return;
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
     reinterpret_cast<float4*>(p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD)[d4] =
-        make_float4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
 }
 
 // The split of a call: 32 row tiles a work-group (1: keys over its waves),
@@ -2477,13 +2492,18 @@ TreePlan tree_plan(const TreeArgs& a) {
     const int32_t groups = (rows + 32 * pl.tiles - 1) / (32 * pl.tiles);
     pl.rows_pad = groups * 32 * pl.tiles;
     pl.first = a.sliding_window > 0 ? std::max(0, a.pos0 - a.sliding_window + 1) : 0;
-    const int64_t keys = static_cast<int64_t>(a.pos0) + a.n - pl.first, step = pl.tiles == 1 ? kTreeStep : 2 * kTreeKeys;
-    // work-groups that share the CUs: two each, one at head_dim 256
-    const int64_t want = std::max<int64_t>(1, (a.head_dim <= 128 ? 512 : 256) / (static_cast<int64_t>(groups) * a.n_kv_heads));
-    const int64_t steps = (keys + step - 1) / step, ranges = std::min<int64_t>(want, kTreeMaxChunks);
-    const int64_t per = (steps + ranges - 1) / ranges;
-    pl.chunk = static_cast<int32_t>(per * step);
-    pl.chunks = static_cast<int32_t>((steps + per - 1) / per);
+    const int64_t keys = static_cast<int64_t>(a.pos0) + a.n - pl.first, tiles = (keys + kTreeKeys - 1) / kTreeKeys;
+    const int64_t heads = static_cast<int64_t>(groups) * a.n_kv_heads, unit = pl.tiles == 1 ? kWaves : 2;
+    // tiles a work-group for that many of them, whole steps from one step on
+    auto tiles_for = [&](int64_t work_groups) {
+        const int64_t ranges = std::min<int64_t>(std::max<int64_t>(1, work_groups / heads), kTreeMaxChunks);
+        const int64_t t = (tiles + ranges - 1) / ranges;
+        return t < unit ? t : (t + unit - 1) / unit * unit;
+    };
+    int64_t per = tiles_for(256);
+    if (pl.tiles == 4 && a.head_dim <= 128 && per > 6 * unit) per = tiles_for(512);
+    pl.chunk = static_cast<int32_t>(per * kTreeKeys);
+    pl.chunks = static_cast<int32_t>((tiles + per - 1) / per);
     return pl;
 }
 
@@ -2500,8 +2520,14 @@ hipError_t launch_tree(const TreeParams& p, const TreePlan& pl, hipStream_t stre
     e = hipGetLastError();
     if (e != hipSuccess || pl.chunks == 1) return e;
     const int64_t n = static_cast<int64_t>(p.n) * (p.n_heads / p.n_kv) * HD / 4;
-    hipLaunchKernelGGL(tree_merge_kernel<HD>, dim3(static_cast<uint32_t>((n + kThreads - 1) / kThreads), p.n_kv),
-                       dim3(kThreads), 0, stream, p, pl.chunks);
+    auto merge = [&](auto cg) {
+        constexpr int CG = decltype(cg)::value, kCols = kThreads / CG;
+        hipLaunchKernelGGL((tree_merge_kernel<HD, CG>), dim3(static_cast<uint32_t>((n + kCols - 1) / kCols), p.n_kv),
+                           dim3(kThreads), 0, stream, p, pl.chunks);
+    };
+    if (pl.chunks <= kTreeMergeLoads) merge(std::integral_constant<int, 1>{});
+    else if (pl.chunks <= 4 * kTreeMergeLoads) merge(std::integral_constant<int, 4>{});
+    else merge(std::integral_constant<int, 8>{});
     return hipGetLastError();
 }
 
