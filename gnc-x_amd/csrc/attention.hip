@@ -1530,7 +1530,7 @@ hipError_t launch_attention(const AttnArgs& a, void* workspace, size_t workspace
 // The tree's mask is an interval test.  With the nodes numbered in preorder,
 // the subtree of a is the interval [pre_a, end_a), so a is i or an ancestor of
 // i exactly when pre_a <= pre_i < end_a: two compares instead of a T x T mask,
-// and 6 bytes a node, which travel in the kernel arguments.
+// and 6 bytes a node, which travel in the first launch's arguments.
 namespace {
 
 struct TreeParams {
@@ -1549,7 +1549,10 @@ struct TreeParams {
     int32_t first, chunk, rows_pad;
     float* part_o;    // [..][HD]
     float2* part_ml;  // (max, sum)
-    TreeTable tree;
+    // the tree's table on the device, as the prologue kernel leaves it
+    uint32_t* interval;  // [n] pre | end << 16
+    uint16_t* depth;     // [n]
+    int32_t max_depth;
 };
 
 // The decode step's prologue of every node's heads, a wave per head: the
@@ -1558,11 +1561,18 @@ struct TreeParams {
 // step (head_inv_rms, no contraction), so an accepted node's cache row is the
 // one that decoding its token would have stored.
 template <int HD>
-__global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p) {
+__global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, TreeTable tree) {
 #pragma clang fp contract(off)
     constexpr int H = HD / 2, NR = (H + 63) / 64;
     __shared__ __align__(16) float xs[kWaves][HD];
     const int t = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    // the 3 KB of the table travel once, in this launch's arguments (a launch takes
+    // the host 1.3 us longer for them), and stay in memory for the next kernel
+    if (blockIdx.x == 0 && blockIdx.y == 0)
+        for (int i = threadIdx.x; i < p.n; i += kThreads) {
+            p.interval[i] = tree.pre[i] | static_cast<uint32_t>(tree.end[i]) << 16;
+            p.depth[i] = tree.depth[i];
+        }
     const int head = static_cast<int>(blockIdx.y) * kWaves + wv;
     if (head >= p.n_heads + p.n_kv) return;  // whole waves; no barrier below
     const bool is_q = head < p.n_heads;
@@ -1573,7 +1583,7 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p) {
     float* x = xs[wv];
     for (int i = lane; i < HD; i += 64) x[i] = src[i];
     const float inv = p.norm_qk ? head_inv_rms(x, HD, p.eps, lane) : 1.0f;
-    const float* rc = p.rope ? p.rope + static_cast<size_t>(p.tree.depth[t]) * HD : nullptr;
+    const float* rc = p.rope ? p.rope + static_cast<size_t>(tree.depth[t]) * HD : nullptr;
     const size_t row = (static_cast<size_t>(p.pos0) + t) * kn + at;
 #pragma unroll
     for (int r = 0; r < NR; ++r) {
@@ -1722,8 +1732,8 @@ struct TreeShared {
 };
 __device__ __forceinline__ void load_tree(const TreeParams& p, TreeShared& t) {
     for (int i = threadIdx.x; i < p.n; i += kThreads) {
-        t.interval[i] = p.tree.pre[i] | static_cast<uint32_t>(p.tree.end[i]) << 16;
-        t.depth[i] = p.tree.depth[i];
+        t.interval[i] = p.interval[i];
+        t.depth[i] = p.depth[i];
     }
 }
 struct RowPlace {
@@ -1731,7 +1741,7 @@ struct RowPlace {
     int lo;  // first position of its window
 };
 __device__ __forceinline__ RowPlace place_of(const TreeParams& p, int node) {
-    return {p.tree.pre[node], p.sw > 0 ? max(0, p.pos0 + p.tree.depth[node] - p.sw + 1) : 0};
+    return {p.interval[node] & 0xffffu, p.sw > 0 ? max(0, p.pos0 + p.depth[node] - p.sw + 1) : 0};
 }
 // whether a query row sees a key of a range that ends at c1
 __device__ __forceinline__ bool sees_key(const TreeParams& p, const TreeShared& t, const RowPlace& at, int key, int c1) {
@@ -1991,7 +2001,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
         if (j == 0) qfac[tid / 8] = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
     }
     if (c1 > p.pos0) load_tree(p, tree);
-    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.tree.max_depth - p.sw + 1) : 0;
+    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.max_depth - p.sw + 1) : 0;
     __syncthreads();
 
     RowState s{-1e30f, -1e30f, 0.0f};
@@ -2344,7 +2354,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         qf = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
     }
     const RowPlace place = place_of(p, myrow / G);
-    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.tree.max_depth - p.sw + 1) : 0;
+    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.max_depth - p.sw + 1) : 0;
 
     RowState st_row{-1e30f, -1e30f, 0.0f};
     floatx16 o[NN];
@@ -2508,9 +2518,9 @@ TreePlan tree_plan(const TreeArgs& a) {
 }
 
 template <int HD, int OCC>
-hipError_t launch_tree(const TreeParams& p, const TreePlan& pl, hipStream_t stream) {
+hipError_t launch_tree(const TreeParams& p, const TreeTable& tree, const TreePlan& pl, hipStream_t stream) {
     const int heads = p.n_heads + p.n_kv;
-    hipLaunchKernelGGL(tree_prologue_kernel<HD>, dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL(tree_prologue_kernel<HD>, dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p, tree);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const dim3 grid(p.n_kv, pl.rows_pad / (32 * pl.tiles), pl.chunks);
@@ -2560,9 +2570,14 @@ bool make_tree_table(const int32_t* parents, int32_t n, TreeTable& t) {
     return true;
 }
 
+namespace {
+constexpr size_t kTreeTableBytes = 4096;  // of a workspace: the table, then the parts
+static_assert(kMaxTreeNodes * 6 <= kTreeTableBytes);
+}  // namespace
+
 size_t attention_tree_workspace_bytes(const TreeArgs& a) {
     const TreePlan pl = tree_plan(a);
-    return pl.chunks == 1 ? 0 : sizeof(float) * pl.chunks * a.n_kv_heads * pl.rows_pad * (a.head_dim + 2);
+    return kTreeTableBytes + (pl.chunks == 1 ? 0 : sizeof(float) * pl.chunks * a.n_kv_heads * pl.rows_pad * (a.head_dim + 2));
 }
 
 hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, void* workspace, size_t workspace_bytes,
@@ -2588,18 +2603,20 @@ hipError_t launch_attention_tree(const TreeArgs& a, const TreeTable& tree, void*
     p.norm_qk = a.norm_qk;
     p.scale = a.scale;
     p.eps = a.eps;
-    p.tree = tree;
+    p.max_depth = tree.max_depth;
+    p.interval = static_cast<uint32_t*>(workspace);
+    p.depth = reinterpret_cast<uint16_t*>(p.interval + kMaxTreeNodes);
     const TreePlan pl = tree_plan(a);
     if (workspace_bytes < attention_tree_workspace_bytes(a)) return hipErrorInvalidValue;
     p.first = pl.first;
     p.chunk = pl.chunk;
     p.rows_pad = pl.rows_pad;
-    p.part_o = static_cast<float*>(workspace);
+    p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + kTreeTableBytes);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.chunks) * a.n_kv_heads * pl.rows_pad * a.head_dim);
     switch (a.head_dim) {
-    case 64: return launch_tree<64, 2>(p, pl, stream);
-    case 128: return launch_tree<128, 2>(p, pl, stream);
-    case 256: return launch_tree<256, 1>(p, pl, stream);
+    case 64: return launch_tree<64, 2>(p, tree, pl, stream);
+    case 128: return launch_tree<128, 2>(p, tree, pl, stream);
+    case 256: return launch_tree<256, 1>(p, tree, pl, stream);
     default: return hipErrorInvalidValue;
     }
 }

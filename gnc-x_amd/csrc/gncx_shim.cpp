@@ -3136,7 +3136,7 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
     a.sliding_window = sliding_window;
     a.norm_qk = has_norm_weight >= 0;
     a.eps = norm_eps;
-    void* ws = g_tree_ws.take(std::max<size_t>(attention_tree_workspace_bytes(a), 1), where);
+    void* ws = g_tree_ws.take(attention_tree_workspace_bytes(a), where);
     if (!ws) return;
     check(launch_attention_tree(a, tree, ws, g_tree_ws.buf.cap, g_rt.stream), where);
 }
