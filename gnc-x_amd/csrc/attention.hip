@@ -1759,37 +1759,48 @@ __device__ __forceinline__ bool sees_key(const TreeParams& p, const TreeShared& 
 struct RowState {
     float m, mt, l;
 };
-// The softmax of a tile's scores: st (raw products, key factors kf, query factor
-// qf) in two halves of eight, half h with the values' exponent ve[h].  Leaves the
-// weights as pairs and returns what O so far is to be multiplied with (1: nothing).
-__device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&ve)[2], RowState& s, half8_t (&ph)[2],
+// The softmax of a tile's scores st, in NG groups of 16 / NG registers, group h
+// with the values' exponent ve[h].  Leaves the weights as pairs and returns what O
+// so far is to be multiplied with (1: nothing).
+template <int NG>
+__device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&ve)[NG], RowState& s, half8_t (&ph)[2],
                                               half8_t (&pl)[2]) {
-    float mx[2];
+    constexpr int W = 16 / NG;
+    float mx = -1e30f, mxt = -1e30f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        mx[h] = -1e30f;
+    for (int h = 0; h < NG; ++h) {
+        float x = -1e30f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) mx[h] = fmaxf(mx[h], st[8 * h + i]);
+        for (int i = 0; i < W; ++i) x = fmaxf(x, st[W * h + i]);
+        mx = fmaxf(mx, x);
+        mxt = fmaxf(mxt, x + ve[h]);  // (a group without a visible key, x -1e30, has no say)
     }
     const auto larger = [](float a, float b) { return fmaxf(a, b); };
-    const float m2 = fmaxf(s.m, ceilf(across_halves(fmaxf(mx[0], mx[1]), larger)));
-    // (a half without a visible key, mx -1e30, has no say)
-    const float mt2 = fmaxf(s.mt, ceilf(across_halves(fmaxf(mx[0] + ve[0], mx[1] + ve[1]), larger)));
-    float sum[2] = {0.0f, 0.0f};
+    const float m2 = fmaxf(s.m, ceilf(across_halves(mx, larger)));
+    const float mt2 = fmaxf(s.mt, ceilf(across_halves(mxt, larger)));
+    // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), the second capped: it
+    // passes 2^126 only where the first is 0
+    float f[NG], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float e[8];
+    for (int h = 0; h < NG; ++h) f[h] = __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f));
+    half4_t hi[4], lo[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            e[i] = __builtin_amdgcn_exp2f(st[8 * h + i] - m2);
-            sum[i & 1] += e[i];
+    for (int a = 0; a < 4; ++a) {
+        float e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            e[i] = __builtin_amdgcn_exp2f(st[4 * a + i] - m2);
+            sum[i] += e[i];
         }
-        // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), the second capped: it
-        // passes 2^126 only where the first is 0
-        pairs<true>(e, __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f)), ph[h], pl[h]);
+        pairs<true>(e, f[a * NG / 4], hi[a], lo[a]);
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        ph[c] = __builtin_shufflevector(hi[2 * c], hi[2 * c + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+        pl[c] = __builtin_shufflevector(lo[2 * c], lo[2 * c + 1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
     s.l = s.l * __builtin_amdgcn_exp2f(s.m - m2) +
-          across_halves(sum[0] + sum[1], [](float a, float b) { return a + b; });
+          across_halves((sum[0] + sum[1]) + (sum[2] + sum[3]), [](float a, float b) { return a + b; });
     const float alpha = __builtin_amdgcn_exp2f(s.mt - mt2);
     s.m = m2;
     s.mt = mt2;
@@ -2102,7 +2113,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
             odd_last = t0;
         }
         const int vf = scale_field(vtop) - 14;  // the field of the power of two that they are divided by
-        const float vs = pow2_field(254 - vf), ve[2] = {static_cast<float>(vf - 127), static_cast<float>(vf - 127)};
+        const float vs = pow2_field(254 - vf), ve[1] = {static_cast<float>(vf - 127)};
 
         // ---- softmax
         const float sf = pow2_field(kf) * qf;
@@ -2163,17 +2174,16 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
     join_parts<HD, kWaves>(p, shared, mls, 1, 1, row0, hk, G, rows);
 }
 
-// Rows over waves, for more than 32 query rows of a KV head: a work-group takes
-// 32 RW rows and two 32-key tiles a step, which its waves load, scale, split and
-// lay out in LDS as operands once for all of them (waves 2 s and 2 s + 1 stage
+// Rows and keys over waves, for 33 to 64 query rows of a KV head: a work-group
+// takes 64 rows and two 32-key tiles a step, which its waves load, scale, split
+// and lay out in LDS as operands once for all of them (waves 2 s and 2 s + 1 stage
 // tile s, 16 keys and 16 values each, a group with powers of two of its own).
-// RW = 4: each wave owns 32 rows and takes both tiles; RW = 2: waves w and w + 2
-// own the same 32 rows, a tile each, and meet at the end.  The next step's loads
-// are in flight during this one's products; two work-groups a CU fill each
-// other's waits.
-template <int HD, int RW, int OCC>
-__global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) {
-    constexpr int NC = HD / 16, NN = HD / 32, KW = kWaves / RW;
+// Waves w and w + 2 own the same 32 rows, a tile each, and meet at the end.  The
+// next step's loads are in flight during this one's products; two work-groups a CU
+// fill each other's waits.
+template <int HD, int OCC>
+__global__ __launch_bounds__(kThreads, OCC) void tree_pair_kernel(TreeParams p) {
+    constexpr int NC = HD / 16, NN = HD / 32, RW = 2, KW = 2;
     constexpr int VW = NN < 4 ? NN : 4;
     constexpr int kPart = HD / 4 * 33;
     constexpr int kTile = NC * 64;  // half8 of a tile's keys' hi (or lo) parts, and of its values'
@@ -2407,12 +2417,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         stage(t0);
         __syncthreads();
         if (t0 + 2 * kTreeKeys < c1) prefetch(t0 + 2 * kTreeKeys);
-        if constexpr (KW == 2) {
-            if (t0 + kTreeKeys * (wv / RW) < c1) take_tile(wv / RW, t0 + kTreeKeys * (wv / RW));
-        } else {
-            take_tile(0, t0);
-            if (t0 + kTreeKeys < c1) take_tile(1, t0 + kTreeKeys);
-        }
+        if (t0 + kTreeKeys * (wv / RW) < c1) take_tile(wv / RW, t0 + kTreeKeys * (wv / RW));
         __syncthreads();  // every wave is done with the operands
     }
 
@@ -2422,13 +2427,294 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
         asm volatile("" ::: "memory");
         for (int t0 = odd_first; t0 <= odd_last; t0 += 16)
-            if (KW == 1 || (t0 - c0) / kTreeKeys % 2 == wv / RW)
+            if ((t0 - c0) / kTreeKeys % 2 == wv / RW)
                 add_odd_keys<HD, 16>(p, tree, place, reinterpret_cast<float*>(part + li), qrow, kbase, vbase, kn, t0, c1, lane,
                                      st_row);
     }
     if (g == 0) mls[wv][li] = make_float2(st_row.m, st_row.l);
     __syncthreads();
     join_parts<HD, KW>(p, shared, mls, RW, RW, row0, hk, G, rows);
+}
+
+// The order of N times (two operand reads from LDS, three products): the reads
+// two steps ahead.  Left alone each step's reads wait behind the products of the
+// step before, and then for LDS: 200 cycles a step instead of 100.
+template <int N>
+__device__ __forceinline__ void interleave_reads() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 3, 0);
+        if (i + 2 < N) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+    }
+}
+
+// Rows over waves, for more than 64 query rows of a KV head: a work-group takes
+// 128 rows, 32 a wave, and walks its range tile by tile.  Its waves load, scale,
+// split and lay out a tile in LDS as operands once for all of them, 8 keys and 8
+// values each (a group with powers of two of its own), two tiles in turn: the next
+// one is laid out, and the one after loaded, while this one is in the products, so
+// a tile takes one barrier.  Two work-groups a CU fill each other's waits.
+template <int HD, int OCC>
+__global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) {
+    constexpr int NC = HD / 16, NN = HD / 32;
+    constexpr int VW = NN < 4 ? NN : 4;
+    constexpr int kPart = HD / 4 * 33;
+    constexpr int kTile = NC * 64;  // half8 of a tile's keys' hi (or lo) parts, and of its values'
+    constexpr int kShared = kTile * 8 > kPart * kWaves ? kTile * 8 : kPart * kWaves;
+    __shared__ __align__(16) float4 shared[kShared];
+    __shared__ __align__(16) float kfac[2][kWaves], vexp[2][kWaves];  // [tile in turn][group]: the keys' factor, the values' exponent
+    __shared__ __align__(16) uint32_t oddmask[2][kWaves];             // [tile in turn][group]: odd keys, from bit 8 group on
+    __shared__ float2 mls[kWaves][32];
+    __shared__ int odd_first, odd_last;
+    __shared__ TreeShared tree;
+    half8_t* const khi = reinterpret_cast<half8_t*>(shared);  // [tile in turn][slice][lane]
+    half8_t* const klo = khi + 2 * kTile;
+    half8_t* const vhi = khi + 4 * kTile;                     // [tile in turn][column tile][slice][lane]
+    half8_t* const vlo = khi + 6 * kTile;
+    const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * 32 * kWaves;
+    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(p.pos0 + p.n, c0 + p.chunk);
+    const uint32_t kn = static_cast<uint32_t>(p.n_kv) * HD;
+    const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
+    const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
+
+    // ---- staging: wave w takes keys and values 8 w .. + 8 of a tile: keys eight
+    // lanes a row (128 bytes a load), values a lane half a row (register i of half
+    // g is row 8 w + 4 g + i)
+    auto tile_of = [&](const float* base, int t0) {
+        const int n = min(c1 - t0, kTreeKeys);  // none past the range: every load reads zeros
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + static_cast<size_t>(t0) * kn), static_cast<short>(0),
+                                                 n > 0 ? static_cast<int32_t>((static_cast<uint32_t>(n - 1) * kn + HD) * 4) : 0,
+                                                 0x00020000);
+    };
+    float kst[NN][4], vst[NN][4];
+    const int key8 = 8 * wv + lane / 8, part8 = lane % 8;
+    const uint32_t kat = (static_cast<uint32_t>(key8) * kn + 4 * part8) * 4;
+    const uint32_t vat = ((8 * wv + 4 * g) * kn + VW * li) * 4;
+    auto prefetch = [&](int t0) {
+        const auto ks = tile_of(kbase, t0), vs = tile_of(vbase, t0);
+#pragma unroll
+        for (int j = 0; j < NN; ++j) {
+            const auto v = __builtin_amdgcn_raw_buffer_load_b128(ks, static_cast<int>(kat + 128 * j), 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) kst[j][i] = as_float(v[i]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int at = static_cast<int>(vat + static_cast<uint32_t>(r) * kn * 4);
+#pragma unroll
+            for (int n = 0; n < NN; n += VW) {
+                if constexpr (VW == 4) {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(vs, at + 128 * n, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) vst[n + i][r] = as_float(v[i]);
+                } else {
+                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(vs, at + 128 * n, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) vst[n + i][r] = as_float(v[i]);
+                }
+            }
+        }
+    };
+    auto stage = [&](int b, int t0) {
+        uint32_t odd = 0;  // this group's odd keys
+        float krow = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NN; ++j) krow = max3_abs(max3_abs(krow, kst[j][0], kst[j][1]), kst[j][2], kst[j][3]);
+        krow = dpp_maximum<0xb1>(krow, krow);
+        krow = dpp_maximum<0x4e>(krow, krow);
+        krow = dpp_maximum<0x141>(krow, krow);
+        float ktop = wave_maximum(krow);
+        if (__ballot(is_odd(krow, ktop))) {
+            ktop = wave_max(krow < __builtin_inff() ? krow : 0.0f);
+            const uint64_t w = __ballot(is_odd(krow, ktop));
+            for (int j = 0; j < 8; ++j) odd |= static_cast<uint32_t>(w >> (8 * j) & 1) << j;
+        }
+        const int kf = key_field(ktop);
+        if (kf != 127)
+#pragma unroll
+            for (int j = 0; j < NN; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) kst[j][i] *= pow2_field(254 - kf);
+        // columns 32 j + 4 part8: slice 2 j + part8 / 4, half part8 / 2 % 2, elements 4 (part8 % 2) ..
+        const int kslot = (b * kTile + (part8 >> 2) * 64 + (part8 >> 1 & 1) * 32 + key8) * 2 + (part8 & 1);
+#pragma unroll
+        for (int j = 0; j < NN; ++j) {
+            half4_t hi, lo;
+            pairs<false>(kst[j], 1.0f, hi, lo);
+            reinterpret_cast<half4_t*>(khi)[kslot + 256 * j] = hi;
+            reinterpret_cast<half4_t*>(klo)[kslot + 256 * j] = lo;
+        }
+        float vrow[4], vtop = 0.0f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            vrow[r] = max3_abs(0.0f, vst[0][r], vst[1][r]);
+#pragma unroll
+            for (int n = 2; n < NN; n += 2) vrow[r] = max3_abs(vrow[r], vst[n][r], vst[n + 1][r]);
+        }
+        vtop = wave_maximum(maximum_of(maximum_of(vrow[0], vrow[1]), maximum_of(vrow[2], vrow[3])));
+        bool near = vtop < __builtin_inff();
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const uint64_t here = __ballot(vrow[r] >= vtop * kOddBelow);
+            near = near && static_cast<uint32_t>(here) && here >> 32;
+        }
+        if (!near) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float x = vrow[r];
+                x = dpp_maximum<0xb1>(x, x);
+                x = dpp_maximum<0x4e>(x, x);
+                x = dpp_maximum<0x141>(x, x);
+                x = dpp_maximum<0x140>(x, x);
+                const auto y = __builtin_amdgcn_permlane16_swap(as_bits(x), as_bits(x), false, false);
+                vrow[r] = maximum_of(as_float(y[0]), as_float(y[1]));
+            }
+            vtop = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (vrow[r] < __builtin_inff()) vtop = fmaxf(vtop, vrow[r]);
+            vtop = across_halves(vtop, maximum_of);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const bool bad = is_odd(vrow[r], vtop);
+                const uint64_t w = __ballot(bad);
+                if (static_cast<uint32_t>(w)) odd |= 1u << r;
+                if (w >> 32) odd |= 1u << (r + 4);
+#pragma unroll
+                for (int n = 0; n < NN; ++n) vst[n][r] = bad ? 0.0f : vst[n][r];
+            }
+        }
+        const int vf = scale_field(vtop) - 14;
+        const float vs = pow2_field(254 - vf);
+        if (lane == 0) {
+            kfac[b][wv] = pow2_field(kf);
+            vexp[b][wv] = static_cast<float>(vf - 127);
+            oddmask[b][wv] = odd << (8 * wv);
+            if (odd) {
+                atomicMin(&odd_first, t0 + 8 * wv);
+                atomicMax(&odd_last, t0 + 8 * wv);
+            }
+        }
+        // slice wv / 2, elements 4 (wv % 2) ..
+#pragma unroll
+        for (int n = 0; n < NN; ++n) {
+            half4_t hi, lo;
+            pairs<true>(vst[n], vs, hi, lo);
+            const int at = (b * kTile + (n * 2 + (wv >> 1)) * 64 + lane) * 2 + (wv & 1);
+            reinterpret_cast<half4_t*>(vhi)[at] = hi;
+            reinterpret_cast<half4_t*>(vlo)[at] = lo;
+        }
+    };
+
+    prefetch(c0);
+    if (tid == 0) {
+        odd_first = c1;
+        odd_last = -1;
+    }
+    if (c1 > p.pos0) load_tree(p, tree);
+    // this wave's query rows as operands, in registers
+    const int myrow = min(row0 + 32 * wv + li, rows - 1);
+    const float* const qrow = p.q + (static_cast<size_t>(myrow / G) * p.n_heads + hk * G + myrow % G) * HD;
+    const RowPlace place = place_of(p, myrow / G);
+    half8_t qh[NC], ql[NC];
+    float qf;
+    {
+        float x[NC][8], amax = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[c][i] = qrow[16 * c + 8 * g + i];
+                amax = fmaxf(amax, fabsf(x[c][i]));
+            }
+        const int f = scale_field(across_halves(amax, maximum_of));
+#pragma unroll
+        for (int c = 0; c < NC; ++c) pairs<true>(x[c], pow2_field(254 + 7 - f), qh[c], ql[c]);
+        qf = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
+    }
+    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.max_depth - p.sw + 1) : 0;
+
+    RowState s{-1e30f, -1e30f, 0.0f};
+    floatx16 o[NN];
+#pragma unroll
+    for (int n = 0; n < NN; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
+
+    auto take_tile = [&](int b, int t0) {
+        floatx16 st;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[r] = 0.0f;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const half8_t kh = khi[b * kTile + c * 64 + lane], kl = klo[b * kTile + c * 64 + lane];
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], st, 0, 0, 0);
+            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], st, 0, 0, 0);
+        }
+        interleave_reads<NC>();
+        __builtin_amdgcn_sched_barrier(0);
+        const floatx4 kf = *reinterpret_cast<const floatx4*>(kfac[b]), vx = *reinterpret_cast<const floatx4*>(vexp[b]);
+        typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
+        const uint32x4 om = *reinterpret_cast<const uint32x4*>(oddmask[b]);
+        const uint32_t odd = __builtin_amdgcn_readfirstlane(om[0] | om[1] | om[2] | om[3]);
+        const float ve[4] = {vx[0], vx[1], vx[2], vx[3]}, sf[4] = {kf[0] * qf, kf[1] * qf, kf[2] * qf, kf[3] * qf};
+#pragma unroll
+        for (int r = 0; r < 16; ++r) st[r] *= sf[r >> 2];
+        if (t0 + kTreeKeys > min(p.pos0, c1) || t0 < lo_most || odd)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int j = 8 * (r >> 2) + 4 * g + (r & 3);
+                if (!sees_key(p, tree, place, t0 + j, c1) || (odd >> j & 1)) st[r] = -__builtin_inff();
+            }
+        half8_t ph[2], pl[2];
+        const float alpha = tile_softmax(st, ve, s, ph, pl);
+        if (__ballot(alpha != 1.0f))
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const half8_t vh = vhi[b * kTile + (n * 2 + c) * 64 + lane], vl = vlo[b * kTile + (n * 2 + c) * 64 + lane];
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[c], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[c], o[n], 0, 0, 0);
+                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[c], o[n], 0, 0, 0);
+            }
+        interleave_reads<2 * NN>();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    __syncthreads();  // odd_first / odd_last, the tree
+    stage(0, c0);
+    if (c0 + kTreeKeys < c1) prefetch(c0 + kTreeKeys);
+    __syncthreads();
+    int b = 0;
+    for (int t0 = c0; t0 < c1; t0 += kTreeKeys, b ^= 1) {
+        if (t0 + kTreeKeys < c1) stage(b ^ 1, t0 + kTreeKeys);
+        if (t0 + 2 * kTreeKeys < c1) prefetch(t0 + 2 * kTreeKeys);
+        take_tile(b, t0);
+        __syncthreads();  // the next tile is laid out, and this one done with
+    }
+
+    float4* const part = shared + wv * kPart;
+    store_part<NN>(part, o, s, li, g);
+    if (odd_last >= 0) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
+        asm volatile("" ::: "memory");
+        for (int t0 = odd_first; t0 <= odd_last; t0 += 8)
+            add_odd_keys<HD, 8>(p, tree, place, reinterpret_cast<float*>(part + li), qrow, kbase, vbase, kn, t0, c1, lane, s);
+    }
+    if (g == 0) mls[wv][li] = make_float2(s.m, s.l);
+    __syncthreads();
+    join_parts<HD, 1>(p, shared, mls, kWaves, kWaves, row0, hk, G, rows);
 }
 
 // out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the key
@@ -2525,8 +2811,8 @@ hipError_t launch_tree(const TreeParams& p, const TreeTable& tree, const TreePla
     if (e != hipSuccess) return e;
     const dim3 grid(p.n_kv, pl.rows_pad / (32 * pl.tiles), pl.chunks);
     if (pl.tiles == 1) hipLaunchKernelGGL((tree_keys_kernel<HD, OCC>), grid, dim3(kThreads), 0, stream, p);
-    else if (pl.tiles == 2) hipLaunchKernelGGL((tree_rows_kernel<HD, 2, OCC>), grid, dim3(kThreads), 0, stream, p);
-    else hipLaunchKernelGGL((tree_rows_kernel<HD, 4, OCC>), grid, dim3(kThreads), 0, stream, p);
+    else if (pl.tiles == 2) hipLaunchKernelGGL((tree_pair_kernel<HD, OCC>), grid, dim3(kThreads), 0, stream, p);
+    else hipLaunchKernelGGL((tree_rows_kernel<HD, OCC>), grid, dim3(kThreads), 0, stream, p);
     e = hipGetLastError();
     if (e != hipSuccess || pl.chunks == 1) return e;
     const int64_t n = static_cast<int64_t>(p.n) * (p.n_heads / p.n_kv) * HD / 4;
