@@ -2789,7 +2789,7 @@ TreePlan tree_plan(const TreeArgs& a) {
     pl.rows_pad = groups * 32 * pl.tiles;
     pl.first = a.sliding_window > 0 ? std::max(0, a.pos0 - a.sliding_window + 1) : 0;
     const int64_t keys = static_cast<int64_t>(a.pos0) + a.n - pl.first, tiles = (keys + kTreeKeys - 1) / kTreeKeys;
-    const int64_t heads = static_cast<int64_t>(groups) * a.n_kv_heads, unit = pl.tiles == 1 ? kWaves : 2;
+    const int64_t heads = static_cast<int64_t>(groups) * a.n_kv_heads, unit = pl.tiles == 1 ? kWaves : pl.tiles == 2 ? 2 : 1;
     // tiles a work-group for that many of them, whole steps from one step on
     auto tiles_for = [&](int64_t work_groups) {
         const int64_t ranges = std::min<int64_t>(std::max<int64_t>(1, work_groups / heads), kTreeMaxChunks);
@@ -2797,7 +2797,13 @@ TreePlan tree_plan(const TreeArgs& a) {
         return t < unit ? t : (t + unit - 1) / unit * unit;
     };
     int64_t per = tiles_for(256);
-    if (pl.tiles == 4 && a.head_dim <= 128 && per > 6 * unit) per = tiles_for(512);
+    // Two work-groups of the 128-row kernel share a CU with heads up to 128.  Twice
+    // the ranges halve the tiles of each and double the parts that meet, which take
+    // about as long each: worth it where a range has more tiles than there are
+    // ranges.  32 heads over 8 of 128: 256 nodes at 300 (5 tiles, 4 ranges)
+    // 48.6 -> 44.0 us, at 4096 (17, 4) 112 -> 95; 64 nodes at 8192 (17, 16) 56 -> 52,
+    // but at 4096 (9, 16) 38.5 -> 41.8; 32 nodes at 2048 (3, 32) 27.2 -> 30.5.
+    if (pl.tiles == 4 && a.head_dim <= 128 && per > 256 / heads) per = tiles_for(512);
     pl.chunk = static_cast<int32_t>(per * kTreeKeys);
     pl.chunks = static_cast<int32_t>((tiles + per - 1) / per);
     return pl;
