@@ -2104,8 +2104,7 @@ struct RopeRows {
 } g_rope_rows;
 
 const float* rope_rows(int32_t pos0, int32_t batch, int32_t head_dim, float base, const float* factors,
-                       const char* where) {
-    RopeRows& r = g_rope_rows;
+                       const char* where, RopeRows& r = g_rope_rows) {
     const int32_t half = head_dim / 2;
     const bool same = r.pos0 == pos0 && r.batch == batch && r.head_dim == head_dim && r.base == base &&
                       r.has_fac == (factors != nullptr) &&
@@ -2957,39 +2956,42 @@ bool on_host(const void* p, const char* name, const char* where) {
     return false;
 }
 
-bool capturing() {
+// the capture that the library stream is in, 0 without one
+unsigned long long capture_id() {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (!g_rt.stream || hipStreamIsCapturing(g_rt.stream, &st) != hipSuccess) {
+    unsigned long long id = 0;
+    if (!g_rt.stream || hipStreamGetCaptureInfo(g_rt.stream, &st, &id) != hipSuccess) {
         (void)hipGetLastError();
-        return false;
+        return 0;
     }
-    return st != hipStreamCaptureStatusNone;
+    return st == hipStreamCaptureStatusNone ? 0 : id;
 }
 
 // A workspace that calls on one stream share in stream order.  A call on
-// another stream than the last one's waits for the device first.  A graph
-// captured with the workspace keeps its address: from then on it is never
-// freed (a larger one is allocated beside it), and a capture that would need
-// a larger one is refused, as nothing can be allocated there.
+// another stream than the last one's waits for the device first.  A captured
+// call takes memory that belongs to its graph (shared by the calls captured on
+// one stream, never freed, as the graph may be replayed at any time), so graphs
+// may be replayed beside one another and beside other calls.
 struct SharedWorkspace {
-    DevBuf buf;
-    hipStream_t last = nullptr;
-    bool used = false, in_graph = false;
+    DevBuf buf, graph;
+    hipStream_t last = nullptr, graph_stream = nullptr;
+    unsigned long long graph_id = 0;
+    bool used = false;
     void* take(size_t bytes, const char* where) {
-        if (capturing()) {
-            if (bytes > buf.cap) {
-                set_error(where, "the workspace must grow, which a stream capture does not allow: make the call once "
-                                 "before the capture", -1);
-                return nullptr;
-            }
-            in_graph = true;
-            return buf.p;
+        if (const unsigned long long id = capture_id()) {
+            if (id == graph_id && g_rt.stream == graph_stream && bytes <= graph.cap) return graph.p;
+            graph = DevBuf{};  // the earlier graph keeps its own
+            graph_id = 0;
+            // (an allocation is no work of the stream; this mode allows it in a capture)
+            hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+            if (!check(hipThreadExchangeStreamCaptureMode(&mode), where)) return nullptr;
+            const bool ok = graph.ensure(bytes, where);
+            if (!check(hipThreadExchangeStreamCaptureMode(&mode), where) || !ok) return nullptr;
+            graph_id = id;
+            graph_stream = g_rt.stream;
+            return graph.p;
         }
         if (used && last != g_rt.stream && !check(hipDeviceSynchronize(), where)) return nullptr;
-        if (in_graph && bytes > buf.cap) {
-            buf = DevBuf{};  // the captured graphs keep the old one
-            in_graph = false;
-        }
         if (!buf.ensure(bytes, where)) return nullptr;
         used = true;
         last = g_rt.stream;
@@ -2997,20 +2999,27 @@ struct SharedWorkspace {
     }
 };
 SharedWorkspace g_select_ws, g_tree_ws;
+RopeRows g_tree_rope;  // the trees' rotations, read in the order of g_tree_ws
+
+constexpr int32_t kMaxLayers = 4096;
+constexpr int32_t kMaxKvDim = 1 << 24;                      // (so that no product of sizes passes 64 bits)
+constexpr size_t kMaxBeamStride = static_cast<size_t>(1) << 55;
+
+bool layer_arrays(float* const* k, float* const* v, int32_t n_layers, const char* where) {
+    if (k && v && n_layers >= 1 && n_layers <= kMaxLayers) return true;
+    set_error(where, "k_caches and v_caches must name at least one layer, and at most 4096", -1);
+    return false;
+}
 
 // Every cache is memory of the library's GPU, holds `floats` floats, and no two
 // share a touched float: cache c's are [lo, floats) + beam * stride for beams
 // below n_beams.  The pointer query (0.2 us) is made once per allocation.
 bool layer_caches(float* const* k, float* const* v, int32_t n_layers, size_t lo, size_t floats, int32_t n_beams,
                   size_t stride, const char* where) {
-    if (!k || !v || n_layers < 1) {
-        set_error(where, "k_caches and v_caches must name at least one layer", -1);
-        return false;
-    }
     const size_t span = sizeof(float) * (stride * (n_beams - 1) + floats);
     const size_t step = sizeof(float) * stride, own = sizeof(float) * (floats - lo);
-    static std::vector<std::pair<uintptr_t, uintptr_t>> at;  // (place within a stride, address); the call lock is held
-    at.clear();
+    static std::array<std::pair<uintptr_t, uintptr_t>, 2 * kMaxLayers> at;  // (place within a stride, address); the call lock is held
+    const size_t n = 2 * static_cast<size_t>(n_layers);
     uintptr_t bases[2] = {0, 0}, ends[2] = {0, 0};  // the last k cache's and v cache's allocations
     for (int32_t i = 0; i < 2 * n_layers; ++i) {
         const float* p = i % 2 ? v[i / 2] : k[i / 2];
@@ -3031,12 +3040,11 @@ bool layer_caches(float* const* k, float* const* v, int32_t n_layers, size_t lo,
             set_error(where, "the rows lie past the end of a cache's memory", -1);
             return false;
         }
-        at.emplace_back(n_beams > 1 ? a % step : a, a);
+        at[i] = {n_beams > 1 ? a % step : a, a};
     }
     // two caches can meet only where their places within a stride are less
     // than `own` apart (around its end, too)
-    std::sort(at.begin(), at.end());
-    const size_t n = at.size();
+    std::sort(at.begin(), at.begin() + n);
     for (size_t i = 0; i < n; ++i)
         for (size_t j = i + 1; j < (n_beams > 1 ? i + n : n); ++j) {
             const auto &x = at[i], &y = at[j % n];
@@ -3103,11 +3111,23 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
                 set_error(where, "two of the vectors, caches and outputs overlap", -1);
                 return;
             }
-    if (capturing()) {
+    if (capture_id()) {
         set_error(where, "the positions' rotations are uploaded by the call, which a stream capture does not allow", -1);
         return;
     }
     TreeArgs a{};
+    a.pos0 = pos0;
+    a.n = n_nodes;
+    a.n_heads = n_heads;
+    a.n_kv_heads = n_kv_heads;
+    a.head_dim = head_dim;
+    a.scale = attn_scale;
+    a.sliding_window = sliding_window;
+    a.norm_qk = has_norm_weight >= 0;
+    a.eps = norm_eps;
+    // (before the rotations: a call on another stream that still reads them has ended)
+    void* ws = g_tree_ws.take(attention_tree_workspace_bytes(a), where);
+    if (!ws) return;
     if (has_norm_weight > 0) {
         a.q_gamma = reinterpret_cast<const float*>(
             device_weights(mmap_base + q_norm_offset, sizeof(float) * static_cast<size_t>(head_dim), where));
@@ -3118,7 +3138,8 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
     if (rope_base > 0.0f) {
         std::array<float, kMaxRopeHalf> fac{};
         if (has_rope_freqs && !read_factors(mmap_base, rope_freqs_offset, head_dim / 2, fac, where)) return;
-        a.rope = rope_rows(pos0, tree.max_depth + 1, head_dim, rope_base, has_rope_freqs ? fac.data() : nullptr, where);
+        a.rope = rope_rows(pos0, tree.max_depth + 1, head_dim, rope_base, has_rope_freqs ? fac.data() : nullptr, where,
+                           g_tree_rope);
         if (!a.rope) return;
     }
     a.q = q_nodes;
@@ -3127,17 +3148,6 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
     a.k_cache = k_cache_layer;
     a.v_cache = v_cache_layer;
     a.out = out_nodes;
-    a.pos0 = pos0;
-    a.n = n_nodes;
-    a.n_heads = n_heads;
-    a.n_kv_heads = n_kv_heads;
-    a.head_dim = head_dim;
-    a.scale = attn_scale;
-    a.sliding_window = sliding_window;
-    a.norm_qk = has_norm_weight >= 0;
-    a.eps = norm_eps;
-    void* ws = g_tree_ws.take(attention_tree_workspace_bytes(a), where);
-    if (!ws) return;
     check(launch_attention_tree(a, tree, ws, g_tree_ws.buf.cap, g_rt.stream), where);
 }
 
@@ -3146,10 +3156,11 @@ GNCX_API void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_cach
     std::lock_guard<CallLock> lk(g_mu);
     const char* where = "gncx_hip_kv_keep_rows";
     if (n_rows == 0) return;
-    if (kv_dim < 4 || kv_dim % 4 || row0 < 0 || n_rows < 0 || n_rows > kMaxKeepRows) {
-        set_error(where, "kv_dim must be a multiple of 4, row0 not negative, and at most 512 rows kept", -1);
+    if (kv_dim < 4 || kv_dim % 4 || kv_dim > kMaxKvDim || row0 < 0 || n_rows < 0 || n_rows > kMaxKeepRows) {
+        set_error(where, "kv_dim must be a multiple of 4 up to 2^24, row0 not negative, and at most 512 rows kept", -1);
         return;
     }
+    if (!layer_arrays(k_caches, v_caches, n_layers, where)) return;
     if (!on_host(rows, "rows", where)) return;
     for (int32_t i = 0; i < n_rows; ++i)
         if (rows[i] < 0 || rows[i] >= kMaxKeepOffset || (i > 0 && rows[i] <= rows[i - 1])) {
@@ -3184,11 +3195,17 @@ GNCX_API void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t
         (finished && !on_device(finished, "finished", where)) || !on_device(out_parents, "out_parents", where) ||
         !on_device(out_tokens, "out_tokens", where) || !on_device(out_scores, "out_scores", where))
         return;
+    const size_t ob = sizeof(int32_t) * n_out;
+    if (overlaps(out_parents, ob, out_tokens, ob) || overlaps(out_parents, ob, out_scores, ob) ||
+        overlaps(out_tokens, ob, out_scores, ob)) {
+        set_error(where, "two of the outputs overlap", -1);
+        return;
+    }
     const size_t need = beam_select_workspace_bytes(n_beams, vocab, n_out);
     void* ws = g_select_ws.take(need, where);
     if (!ws) return;
     check(launch_beam_select(logits, n_beams, vocab, scores, finished, finished_token, n_out, out_parents, out_tokens,
-                             out_scores, ws, g_select_ws.buf.cap, g_rt.stream),
+                             out_scores, ws, need, g_rt.stream),
           where);
 }
 
@@ -3198,12 +3215,13 @@ GNCX_API void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches
     std::lock_guard<CallLock> lk(g_mu);
     const char* where = "gncx_hip_kv_reorder";
     if (n_rows == 0) return;
-    if (n_beams < 1 || n_beams > kMaxBeams || kv_dim < 4 || kv_dim % 4 || row0 < 0 || n_rows < 0 ||
-        n_rows > INT32_MAX - row0 || beam_stride % 4 ||
+    if (n_beams < 1 || n_beams > kMaxBeams || kv_dim < 4 || kv_dim % 4 || kv_dim > kMaxKvDim || row0 < 0 || n_rows < 0 ||
+        n_rows > INT32_MAX - row0 || beam_stride % 4 || beam_stride > kMaxBeamStride ||
         (n_beams > 1 && beam_stride < (static_cast<size_t>(row0) + n_rows) * kv_dim)) {
         set_error(where, "1 to 32 beams, kv_dim and beam_stride multiples of 4, and the rows within a beam's stride", -1);
         return;
     }
+    if (!layer_arrays(k_caches, v_caches, n_layers, where)) return;
     if (!ensure_runtime(where)) return;
     DeviceGuard dev(where);
     if (!dev.ok) return;

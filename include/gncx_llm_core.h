@@ -471,8 +471,9 @@ void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const float* v_node
  * i < n_rows (at most 512): the accepted path of a tree whose nodes stand from
  * row0 on.  rows (host memory, read before the call returns) ascend strictly
  * from 0 on, below 65536.  Rows behind the n_rows kept ones stay as they are.
- * k_caches / v_caches: host arrays of n_layers device addresses, 16-byte
- * aligned; kv_dim (n_kv_heads*head_dim) a multiple of 4. */
+ * k_caches / v_caches: host arrays of n_layers (1..4096) device addresses,
+ * 16-byte aligned, of caches that do not overlap; kv_dim (n_kv_heads*head_dim)
+ * a multiple of 4 up to 2^24. */
 void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t kv_dim,
                            int32_t row0, const int32_t* rows, int32_t n_rows);
 /* Beam search's selection.  The candidates are (b, v) for beams b < n_beams
@@ -484,8 +485,8 @@ void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_caches, int32
  * b * vocab + v.  A NaN logit or score counts as -inf, and a score of -inf is
  * no candidate: outputs left over have parent -1, word -1, score -inf.  Sums
  * and scores are formed in 64 bits.  out_scores may be scores, out_parents or
- * out_tokens finished.  Can be captured into a graph after a call of the same
- * sizes; graphs that hold it share one workspace and are not run at once. */
+ * out_tokens finished; no two outputs overlap.  Captured into a graph, the
+ * call's workspace (at most 5 MiB) belongs to the graph for the process's life. */
 void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,
                           const int32_t* finished, int32_t finished_token, int32_t n_out, int32_t* out_parents,
                           int32_t* out_tokens, float* out_scores);

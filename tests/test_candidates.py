@@ -67,7 +67,8 @@ def test_keep_refuses_rows_out_of_order(plib, rows):
     refused(plib, "ascend strictly")
 
 
-@pytest.mark.parametrize("kv_dim,row0,n", [(6, 0, 1), (0, 0, 1), (64, -1, 1), (64, 0, 513), (64, 0, -1)])
+@pytest.mark.parametrize("kv_dim,row0,n", [(6, 0, 1), (0, 0, 1), (64, -1, 1), (64, 0, 513), (64, 0, -1),
+                                           (2 ** 24 + 4, 0, 1)])
 def test_keep_refuses_sizes(plib, kv_dim, row0, n):
     r, none = np.arange(max(n, 1), dtype=np.int32), (C.c_void_p * 1)()
     plib.gncx_hip_kv_keep_rows(none, none, 1, kv_dim, row0, r.ctypes.data, n)
@@ -90,8 +91,18 @@ def test_select_refuses_a_finished_token_outside_the_vocabulary(plib, token):
 
 @pytest.mark.parametrize("beams,stride,kv_dim,row0,n", [(0, 64, 64, 0, 1), (33, 64, 64, 0, 1), (2, 63, 64, 0, 1),
                                                         (2, 66, 64, 0, 1), (2, 128, 6, 0, 1), (2, 128, 64, 1, 2),
-                                                        (2, 128, 64, -1, 1), (2, 128, 64, 0, -1)])
+                                                        (2, 128, 64, -1, 1), (2, 128, 64, 0, -1),
+                                                        (2, 2 ** 62, 64, 0, 1), (2, 2 ** 25, 2 ** 24 + 4, 0, 1)])
 def test_reorder_refuses_sizes(plib, beams, stride, kv_dim, row0, n):
     none = (C.c_void_p * 1)()
     plib.gncx_hip_kv_reorder(none, none, 1, beams, stride, kv_dim, row0, n, None)
     refused(plib, "1 to 32 beams")
+
+
+@pytest.mark.parametrize("layers", [0, -1, 4097, 2 ** 31 - 1])
+def test_caches_refuse_numbers_of_layers(plib, layers):
+    r, none = np.zeros(1, np.int32), (C.c_void_p * 1)()
+    plib.gncx_hip_kv_keep_rows(none, none, layers, 64, 0, r.ctypes.data, 1)
+    refused(plib, "at least one layer")
+    plib.gncx_hip_kv_reorder(none, none, layers, 2, 64, 64, 0, 1, None)
+    refused(plib, "at least one layer")

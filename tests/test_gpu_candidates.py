@@ -334,6 +334,34 @@ def test_tree_on_other_streams(lib, torch_mod):
         assert bool(((t.out.double() - want).abs() <= tol).all())
 
 
+def test_tree_rotations_on_two_streams(lib, torch_mod):
+    """Calls at other positions, in turn on two streams with nothing between
+    them: none rewrites the rotations that another still reads."""
+    torch = torch_mod
+    calls = []
+    for i in range(6):
+        calls.append(Tree(torch, 8, 2, 128, 40 + 500 * i, make_parents("random", 60 + i), base=1e4, weight=1, seed=i))
+    want = []
+    for t in calls:
+        q, k, kc, vc = (x.clone() for x in (t.q, t.k, t.kc, t.vc))
+        t.call(lib)
+        want.append(t.out.clone())
+        for x, old in ((t.q, q), (t.k, k), (t.kc, kc), (t.vc, vc)):
+            x.copy_(old)
+        t.out.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    try:
+        for i, t in enumerate(calls):
+            lib.gncx_hip_set_stream(streams[i % 2].cuda_stream)
+            t.call(lib)
+    finally:
+        lib.gncx_hip_set_stream(None)
+    torch.cuda.synchronize()
+    for t, w in zip(calls, want):
+        assert torch.equal(t.out, w)
+
+
 def test_tree_refuses_host_overlap_alignment_and_capture(lib, torch_mod):
     torch = torch_mod
     lib.gncx_hip_last_status()
@@ -685,23 +713,60 @@ def test_selection_and_reordering_captured(lib, torch_mod):
                      torch.randn(4 * (i + 1), device="cuda"), 64)
 
 
-def test_select_capture_refuses_to_grow_its_workspace(lib, torch_mod):
+def test_select_outputs_that_overlap_are_refused(lib, torch_mod):
     torch = torch_mod
-    logits = torch.randn(1, 1 << 22, device="cuda")
-    scores, out = torch.zeros(1, device="cuda"), torch.zeros(64, device="cuda")
-    idx = torch.zeros(64, dtype=torch.int32, device="cuda")
-    # a call no other test makes: the largest vocabulary, with the most outputs
-    big = torch.randn(4, 1 << 22, device="cuda")
-    sc = torch.zeros(4, device="cuda")
-    s = torch.cuda.Stream()
-    g = torch.cuda.CUDAGraph()
+    x, sc = torch.randn(2, 50, device="cuda"), torch.zeros(2, device="cuda")
+    out = torch.zeros(12, dtype=torch.int32, device="cuda")
+    at = [out.data_ptr() + 16 * i for i in range(3)]
     lib.gncx_hip_last_status()
-    lib.gncx_hip_set_stream(s.cuda_stream)
-    try:
-        with torch.cuda.graph(g, stream=s):
-            lib.gncx_hip_beam_select(big.data_ptr(), 4, 1 << 22, sc.data_ptr(), None, 0, 64, idx.data_ptr(),
-                                     idx.data_ptr(), out.data_ptr())
-    finally:
-        lib.gncx_hip_set_stream(None)
-    refused(lib, "capture")
-    check_select(lib, torch, logits, scores, 64)
+    for a, b, c in ((0, 0, 1), (0, 1, 0), (0, 1, 1)):
+        lib.gncx_hip_beam_select(x.data_ptr(), 2, 50, sc.data_ptr(), None, 0, 4, at[a], at[b], at[c])
+        refused(lib, "outputs overlap")
+    lib.gncx_hip_beam_select(x.data_ptr(), 2, 50, sc.data_ptr(), None, 0, 5, *at)
+    refused(lib, "outputs overlap")
+    assert not out.any()
+    lib.gncx_hip_beam_select(x.data_ptr(), 2, 50, sc.data_ptr(), None, 0, 4, *at)
+    gncx.check(lib)
+
+
+def test_select_graphs_run_beside_one_another(lib, torch_mod):
+    """Two graphs captured with no call before them, replayed on two streams at
+    once and beside eager calls on a third: each has a workspace of its own."""
+    torch = torch_mod
+    B, V, n = 6, 151936, 64
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    sets = []
+    for s in streams:
+        t = dict(x=torch.randn(B, V, device="cuda"), sc=torch.randn(B, device="cuda"),
+                 par=torch.zeros(n, dtype=torch.int32, device="cuda"),
+                 tok=torch.zeros(n, dtype=torch.int32, device="cuda"), best=torch.zeros(n, device="cuda"))
+        g = torch.cuda.CUDAGraph()
+        lib.gncx_hip_set_stream(s.cuda_stream)
+        try:
+            with torch.cuda.graph(g, stream=s):
+                for _ in range(3):
+                    lib.gncx_hip_beam_select(t["x"].data_ptr(), B, V, t["sc"].data_ptr(), None, 0, n,
+                                             t["par"].data_ptr(), t["tok"].data_ptr(), t["best"].data_ptr())
+        finally:
+            lib.gncx_hip_set_stream(None)
+        gncx.check(lib)
+        sets.append((g, s, t))
+    x, sc = torch.randn(B, V, device="cuda"), torch.randn(B, device="cuda")
+    alone = select_reference(x, sc, n)
+    for _ in range(4):
+        for _, _, t in sets:
+            t["x"].normal_()
+            t["par"].fill_(-5)
+            t["tok"].fill_(-5)
+        torch.cuda.synchronize()
+        for g, s, _ in sets:
+            with torch.cuda.stream(s):
+                for _ in range(5):
+                    g.replay()
+        par, tok, _ = select(lib, torch, x, sc, n)
+        torch.cuda.synchronize()
+        assert np.array_equal(par, alone[0]) and np.array_equal(tok, alone[1])
+        for _, _, t in sets:
+            want = select_reference(t["x"], t["sc"], n)
+            assert np.array_equal(t["par"].cpu().numpy(), want[0])
+            assert np.array_equal(t["tok"].cpu().numpy(), want[1])
