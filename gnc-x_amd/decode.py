@@ -38,7 +38,14 @@ differences are where the streamer works on host memory:
   with the per-token residual add + RMSNorm loops before them folded in,
   gncx_hip_swiglu_matbatch for the down projection, and
   gncx_hip_attention_prefill for the per-token prologue + attention loop
-  (one causal batch).
+  (one causal batch);
+* with device buffers a sequence can have several continuations, which the
+  streamer has not: generate_drafted() checks a drafted tree of tokens in one
+  pass (verify_tree: the prefill's batched calls around
+  gncx_hip_attention_tree) and keeps the accepted path's cache rows
+  (gncx_hip_kv_keep_rows); beam_search() decodes beams side by side, chosen by
+  gncx_hip_beam_select and followed by the caches through
+  gncx_hip_kv_reorder.
 
 Weights are random-init with the block statistics of the synthetic
 benchmark inputs: fp16 scales |N(0, 0.02)|, uniform random code bytes,
@@ -49,7 +56,7 @@ from __future__ import annotations
 import ctypes as C
 from dataclasses import dataclass, field
 
-from . import Q4_K, Q6_K, DecodeLayer, DecodeModel, DecodeState, DecodeTensor, row_bytes
+from . import Q4_K, Q6_K, DecodeLayer, DecodeModel, DecodeState, DecodeTensor, check, row_bytes
 
 _ALIGN = 32  # GGUF default data alignment
 
@@ -241,6 +248,29 @@ def load_model_gguf(path) -> Model:
         rope_base=float(meta.get(f"{a}.rope.freq_base", 10000.0)),
         layer_type=tensors["blk.0.attn_q.weight"].ggml_type, embd_type=tensors["token_embd.weight"].ggml_type)
     return Model(shape, mm, {n: t.abs_file_offset for n, t in tensors.items()})
+
+
+def lookup_draft(ids, depth: int = 8, width: int = 4):
+    """(tokens, parents) of a tree drafted from the sequence itself: what came
+    behind the last `width` earlier places that the last two ids (or, without
+    one, the last id) stand at, up to `depth` ids of each, joined where they
+    begin alike."""
+    ids = list(ids)
+    for m in (2, 1):
+        tail = ids[-m:]
+        places = [i + m for i in range(len(ids) - m) if ids[i:i + m] == tail][-width:]
+        if places:
+            break
+    tokens, parents, at = [], [], {}
+    for i in reversed(places):
+        node = -1
+        for t in ids[i:i + depth]:
+            if (node, t) not in at:
+                at[node, t] = len(tokens)
+                tokens.append(t)
+                parents.append(node)
+            node = at[node, t]
+    return tokens, parents
 
 
 class Decoder:
@@ -581,24 +611,180 @@ class Decoder:
         the SwiGLU inside the down projection's matbatch."""
         s, L, m = self.s, self.lib, self.m
         self._norm_rows = bn
+
+        def attention(l):
+            p = f"blk.{l}"
+            L.gncx_hip_attention_prefill(bq.data_ptr(), bk.data_ptr(), bv.data_ptr(), self.kc[l].data_ptr(),
+                                         self.vc[l].data_ptr(), 0, B, s.n_heads, s.n_kv, s.head_dim, self.scale, 0,
+                                         m.base, m.off(f"{p}.attn_q_norm.weight"), m.off(f"{p}.attn_k_norm.weight"),
+                                         1, s.eps, 0, 0, s.rope_base, ba.data_ptr())
+
+        self._rows_layers(B, attention, bh, bq, bk, bv, ba, bp, bg, bu)
+        self._add(bh, bp)
+        self.hidden.copy_(bh[B - 1])
+        return self._lm_head()
+
+    def _rows_layers(self, B, attention, bh, bq, bk, bv, ba, bp, bg, bu):
+        """The layers over B rows with the extensions, attention(l) from bq, bk
+        and bv to ba; the last layer's output (bp) is not added yet."""
+        s, m = self.s, self.m
         for l in range(s.n_layers):
             p = f"blk.{l}"
             # the previous layer's residual add and this layer's first norm go
             # into the Q/K/V matbatch's activation pass
             self._matbatch_multi_addnorm(p, "qkv", "attn_norm", bh, None if l == 0 else bp, B,
                                          (s.q_dim, s.kv_dim, s.kv_dim), (bq, bk, bv))
-            L.gncx_hip_attention_prefill(bq.data_ptr(), bk.data_ptr(), bv.data_ptr(), self.kc[l].data_ptr(),
-                                         self.vc[l].data_ptr(), 0, B, s.n_heads, s.n_kv, s.head_dim, self.scale, 0,
-                                         m.base, m.off(f"{p}.attn_q_norm.weight"), m.off(f"{p}.attn_k_norm.weight"),
-                                         1, s.eps, 0, 0, s.rope_base, ba.data_ptr())
+            attention(l)
             self._matbatch(f"{p}.attn_output.weight", ba.data_ptr(), B, s.q_dim, s.embed, bp.data_ptr())
             self._matbatch_multi_addnorm(p, ("ffn_gate", "ffn_up"), "ffn_norm", bh, bp, B, (s.ffn, s.ffn), (bg, bu))
             # SwiGLU formed by the down projection's activation pass
-            L.gncx_hip_swiglu_matbatch(m.base, m.off(f"{p}.ffn_down.weight"), s.layer_type, bg.data_ptr(),
-                                       bu.data_ptr(), B, s.ffn, s.embed, bp.data_ptr())
-        self._add(bh, bp)
-        self.hidden.copy_(bh[B - 1])
-        return self._lm_head()
+            self.lib.gncx_hip_swiglu_matbatch(m.base, m.off(f"{p}.ffn_down.weight"), s.layer_type, bg.data_ptr(),
+                                              bu.data_ptr(), B, s.ffn, s.embed, bp.data_ptr())
+
+    # -- several continuations of one sequence --------------------------------------
+    def _device_only(self, what):
+        if not self.hidden.is_cuda:
+            raise ValueError(f"{what} keeps every buffer in device memory")
+
+    def _rows_logits(self, tokens, attention):
+        """Logits [len(tokens)][vocab] of one pass over the tokens, with
+        attention(l, q, k, v, out) over each layer's row tensors."""
+        torch, s, L, m = self.torch, self.s, self.lib, self.m
+        n = len(tokens)
+        row = lambda d: torch.empty(n, d, dtype=torch.float32, device=self.hidden.device)  # noqa: E731
+        bh, bn, bp = row(s.embed), row(s.embed), row(s.embed)
+        bq, bk, bv, ba = row(s.q_dim), row(s.kv_dim), row(s.kv_dim), row(s.q_dim)
+        bg, bu, logits = row(s.ffn), row(s.ffn), row(s.vocab)
+        ids = (C.c_int32 * n)(*(int(t) for t in tokens))
+        L.gncx_hip_fetch_token_embeddings(s.embd_type, m.base, m.off("token_embd.weight"), ids, n, s.vocab, s.embed,
+                                          1.0, bh.data_ptr())
+        self._rows_layers(n, lambda l: attention(l, bq, bk, bv, ba), bh, bq, bk, bv, ba, bp, bg, bu)
+        L.gncx_hip_add_rmsnorm_rows(bh.data_ptr(), bp.data_ptr(), n, m.base, m.off("output_norm.weight"), s.embed,
+                                    s.eps, bn.data_ptr())
+        L.gncx_xfold_universal_matbatch(m.base, m.off("token_embd.weight"), s.embd_type, bn.data_ptr(), n, s.embed,
+                                        s.vocab, logits.data_ptr(), None)
+        return logits
+
+    def verify_tree(self, tokens, parents, pos: int):
+        """Logits [n][vocab] behind every token of a drafted tree whose first
+        tokens (parent -1) continue the `pos` cached positions; the nodes' K and
+        V become cache rows pos .. pos + n - 1 (keep_path keeps a path's)."""
+        self._device_only("a drafted tree")
+        n, s, m = len(tokens), self.s, self.m
+        if n != len(parents) or not 1 <= n <= 512:
+            raise ValueError("a tree has 1 to 512 tokens, each with a parent")
+        if pos < 0 or pos + n > self.max_seq:
+            raise ValueError("the tree ends past the KV cache")
+        par = (C.c_int32 * n)(*(int(p) for p in parents))
+
+        def attention(l, q, k, v, out):
+            p = f"blk.{l}"
+            self.lib.gncx_hip_attention_tree(q.data_ptr(), k.data_ptr(), v.data_ptr(), self.kc[l].data_ptr(),
+                                             self.vc[l].data_ptr(), pos, n, C.addressof(par), s.n_heads, s.n_kv,
+                                             s.head_dim, self.scale, 0, m.base, m.off(f"{p}.attn_q_norm.weight"),
+                                             m.off(f"{p}.attn_k_norm.weight"), 1, s.eps, 0, 0, s.rope_base,
+                                             out.data_ptr())
+
+        logits = self._rows_logits(tokens, attention)
+        check(self.lib)
+        return logits
+
+    def keep_path(self, pos: int, path):
+        """Cache rows pos + path[i] (path ascending) of a verified tree become
+        rows pos + i."""
+        self._device_only("a drafted tree")
+        P, n = C.c_void_p, self.s.n_layers
+        rows = (C.c_int32 * len(path))(*(int(i) for i in path))
+        self.lib.gncx_hip_kv_keep_rows((P * n)(*(t.data_ptr() for t in self.kc)),
+                                       (P * n)(*(t.data_ptr() for t in self.vc)), n, self.s.kv_dim, pos,
+                                       C.addressof(rows), len(path))
+        check(self.lib)
+
+    def generate_drafted(self, prompt, n_new: int, draft=None):
+        """generate() with drafts: draft(ids so far) returns (tokens, parents) of
+        a tree that may continue them (by default lookup_draft), and each pass
+        accepts its longest greedy path.  Returns the new ids."""
+        draft = draft or lookup_draft
+        ids, new = list(prompt), []
+        if n_new < 1:
+            return new
+        token, pos = self.greedy(self.prefill(ids)), len(ids)
+        while True:
+            new.append(token)
+            if len(new) == n_new:
+                return new
+            # node 0 is the token just chosen, the draft hangs below it
+            tokens, parents = draft(ids + new)
+            room = min(511, self.max_seq - pos - 1)
+            tokens = [token] + [int(t) for t in tokens[:room]]
+            parents = [-1] + [int(p) + 1 for p in parents[:room]]
+            best = self.torch.argmax(self.verify_tree(tokens, parents, pos), dim=1).tolist()
+            path = [0]
+            for i in range(1, len(tokens)):
+                if len(new) + 1 < n_new and parents[i] == path[-1] and tokens[i] == best[path[-1]]:
+                    path.append(i)
+                    new.append(tokens[i])
+            self.keep_path(pos, path)
+            pos += len(path)
+            token = best[path[-1]]
+
+    def beam_search(self, prompt, n_beams: int, n_new: int, end: int = -1):
+        """The n_beams (at most 32) continuations of n_new tokens that beam
+        search finds, [(token ids, sum of log probabilities)] in falling order; a
+        continuation that reaches the token `end` (if not negative) stays as it
+        is.  Each beam has caches of its own."""
+        self._device_only("beam search")
+        torch, s, L, m = self.torch, self.s, self.lib, self.m
+        if not 1 <= n_beams <= 32 or n_new < 1:
+            raise ValueError("1 to 32 beams and at least one new token")
+        P, dev, pos = C.c_void_p, self.hidden.device, len(prompt)
+        if pos < 1 or pos + n_new - 1 > self.max_seq:
+            raise ValueError("the beams end past the KV cache")
+        first = self.prefill(list(prompt))
+        # beam b's rows of layer l, [layer][beam][row][kv_dim]; the prompt's are
+        # put into beam 0's and spread by the first reordering
+        rows = pos + n_new - 1
+        kc, vc = (torch.zeros(s.n_layers, n_beams, rows, s.kv_dim, dtype=torch.float32, device=dev) for _ in range(2))
+        for l in range(s.n_layers):
+            kc[l, 0, :pos].copy_(self.kc[l][:pos])
+            vc[l, 0, :pos].copy_(self.vc[l][:pos])
+        ks, vs = ((P * s.n_layers)(*(c[l].data_ptr() for l in range(s.n_layers))) for c in (kc, vc))
+        parents, tokens = (torch.zeros(n_beams, dtype=torch.int32, device=dev) for _ in range(2))
+        finished = torch.zeros(n_beams, dtype=torch.int32, device=dev)
+        scores = torch.zeros(n_beams, dtype=torch.float32, device=dev)
+        chosen = torch.zeros(n_beams, n_new, dtype=torch.int32, device=dev)
+
+        def attention(l, q, k, v, out):
+            at = (l * n_beams) * rows * s.kv_dim * 4
+            p = f"blk.{l}"
+            for b in range(n_beams):
+                L.gncx_hip_attention_step_fused(q[b].data_ptr(), k[b].data_ptr(), v[b].data_ptr(),
+                                                kc.data_ptr() + at + 4 * b * rows * s.kv_dim,
+                                                vc.data_ptr() + at + 4 * b * rows * s.kv_dim, pos, s.n_heads, s.n_kv,
+                                                s.head_dim, self.scale, 0, 1, m.base,
+                                                m.off(f"{p}.attn_q_norm.weight"), m.off(f"{p}.attn_k_norm.weight"), 1,
+                                                s.eps, 0, 0, s.rope_base, out[b].data_ptr())
+
+        logits = first
+        for i in range(n_new):
+            if i:
+                logits = self._rows_logits(tokens.clamp(min=0).tolist(), attention)
+                pos += 1
+            L.gncx_hip_beam_select(logits.data_ptr(), n_beams if i else 1, s.vocab, scores.data_ptr(),
+                                   finished.data_ptr() if end >= 0 else None, max(end, 0), n_beams,
+                                   parents.data_ptr(), tokens.data_ptr(), scores.data_ptr())
+            if i + 1 < n_new:
+                # the first choice spreads the prompt's rows, a later one the rows since
+                start = len(prompt) if i else 0
+                L.gncx_hip_kv_reorder(ks, vs, s.n_layers, n_beams, rows * s.kv_dim, s.kv_dim, start, pos - start,
+                                      parents.data_ptr())
+            check(L)
+            came = parents.clamp(min=0).long()  # (-1: no candidate left, score -inf)
+            chosen = chosen[came]
+            chosen[:, i] = tokens
+            if end >= 0:
+                finished = torch.where(parents < 0, 0, finished[came] | (tokens == end).int())
+        return [(t, c) for t, c in zip(chosen.tolist(), scores.tolist()) if c > float("-inf")]
 
     def _matbatch_multi_addnorm(self, p, names, norm, hidden, delta, b, out_dims, outs):
         """gncx_hip_matbatch_multi_addnorm: hidden += delta (None: no add), then

@@ -106,3 +106,22 @@ def test_caches_refuse_numbers_of_layers(plib, layers):
     refused(plib, "at least one layer")
     plib.gncx_hip_kv_reorder(none, none, layers, 2, 64, 64, 0, 1, None)
     refused(plib, "at least one layer")
+
+
+@pytest.mark.parametrize("ids,tokens,parents", [
+    ([], [], []), ([7], [], []), ([1, 2, 3], [], []),
+    ([4, 9, 8, 4], [9, 8, 4], [-1, 0, 1]),  # no earlier pair: behind the last id
+    ([1, 2, 3, 4, 1, 2, 5, 6, 1, 2], [5, 6, 1, 2, 3, 4, 1, 2, 5, 6, 1, 2],
+     [-1, 0, 1, 2, -1, 4, 5, 6, 7, 8, 9, 10]),
+    ([3, 3, 3, 3], [3, 3], [-1, 0]),  # branches that begin alike are one
+])
+def test_lookup_draft(ids, tokens, parents):
+    import gncx_amd.decode as dec
+    assert dec.lookup_draft(ids) == (tokens, parents)
+
+
+def test_lookup_draft_has_a_depth_and_a_width():
+    import gncx_amd.decode as dec
+    ids = [x for i in range(10) for x in (1, 2, 10 + i, 20 + i, 30 + i)] + [1, 2]
+    tokens, parents = dec.lookup_draft(ids, depth=2, width=3)
+    assert (tokens, parents) == ([19, 29, 18, 28, 17, 27], [-1, 0, -1, 2, -1, 4])

@@ -770,3 +770,173 @@ def test_select_graphs_run_beside_one_another(lib, torch_mod):
             want = select_reference(t["x"], t["sc"], n)
             assert np.array_equal(t["par"].cpu().numpy(), want[0])
             assert np.array_equal(t["tok"].cpu().numpy(), want[1])
+
+
+# ---- a run of them together: the decode driver --------------------------------------------
+LOGITS = 1e-3  # the bar of this driver's logits between its batched and its one-token calls (relative L2)
+
+
+def small_decoder(lib, torch, hd, max_seq=96, seed=7, **kw):
+    import gncx_amd.decode as dec
+    shape = dec.Qwen3Shape(n_layers=2, embed=256, n_heads=4, n_kv=2, head_dim=hd, ffn=512, vocab=600)
+    model = dec.build_model(torch, shape, seed=seed)
+    return dec, model, dec.Decoder(lib, torch, model, max_seq=max_seq, fused=True, **kw)
+
+
+def distance(got, want):
+    got, want = np.asarray(got, np.float64), np.asarray(want, np.float64)
+    return np.linalg.norm(got - want) / np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_a_tree_is_its_branches_decoded_one_by_one(lib, torch_mod, hd):
+    """Every node's logits, and after keep_path the next step's, against another
+    decoder that steps along the node's branch alone."""
+    torch = torch_mod
+    dec, model, d = small_decoder(lib, torch, hd)
+    prompt = [11, 22, 33, 44, 55, 66, 77]
+    tokens, parents = [5, 6, 7, 8, 5, 9, 10, 599, 0], [-1, 0, 0, 1, 2, 4, 5, 3, -1]
+    d.prefill(prompt)
+    got = d.verify_tree(tokens, parents, len(prompt)).cpu().numpy()
+    ref = dec.Decoder(lib, torch, model, max_seq=96, fused=True)
+    for i in range(len(tokens)):
+        branch, j = [], i
+        while j >= 0:
+            branch.insert(0, j)
+            j = parents[j]
+        ref.prefill(prompt)
+        for at, j in enumerate(branch):
+            want = ref.forward_token(tokens[j], len(prompt) + at).cpu().numpy()
+        assert distance(got[i], want) < LOGITS, i
+    path = [0, 2, 4, 5, 6]
+    d.keep_path(len(prompt), path)
+    ref.prefill(prompt)
+    for at, j in enumerate(path):
+        ref.forward_token(tokens[j], len(prompt) + at)
+    pos = len(prompt) + len(path)
+    assert distance(d.forward_token(17, pos).cpu(), ref.forward_token(17, pos).cpu()) < LOGITS
+    for a, b in zip(d.kc + d.vc, ref.kc + ref.vc):
+        assert distance(a[:pos].cpu(), b[:pos].cpu()) < LOGITS
+    gncx.check(lib)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("kind", ["none", "lookup", "right", "wide"])
+def test_drafted_generation_is_greedy(lib, torch_mod, hd, kind):
+    """Whatever the drafts, every new id is the largest logit (to the bar's
+    width) of a decoder that steps along the ids one by one; right drafts are
+    accepted, so they take few passes."""
+    torch = torch_mod
+    dec, model, d = small_decoder(lib, torch, hd)
+    prompt, n_new = [3, 599, 17, 3, 599, 250, 3, 599], 24
+    plain = d.generate(prompt, n_new)
+    rng = np.random.default_rng(1)
+    passes = []
+
+    def draft(ids):
+        at = len(ids) - len(prompt)
+        passes.append(at)
+        if kind == "none":
+            return [], []
+        rest = plain[at:at + 6]
+        if kind == "right":
+            return rest, list(range(-1, len(rest) - 1))
+        tokens, parents = [], []  # wrong branches before, beside and below the right one
+        last = -1
+        for t in rest:
+            for _ in range(20):
+                tokens.append(int(rng.integers(600)))
+                parents.append(int(rng.integers(-1, len(tokens) - 1)))
+            tokens.append(t)
+            parents.append(last)
+            last = len(tokens) - 1
+        return tokens[:60], parents[:60]
+
+    new = d.generate_drafted(prompt, n_new, None if kind == "lookup" else draft)
+    assert len(new) == n_new
+    ref = dec.Decoder(lib, torch, model, max_seq=96, fused=True)
+    logits, same = ref.prefill(prompt), 0
+    for i, t in enumerate(new):
+        x = logits.cpu().numpy().astype(np.float64)
+        assert x[t] >= x.max() - 2 * LOGITS * np.linalg.norm(x), i
+        logits = ref.forward_token(t, len(prompt) + i)
+    while same < n_new and new[same] == plain[same]:
+        same += 1
+    if kind == "right" and same == n_new:
+        assert passes == [1, 8, 15, 22]  # six accepted and one chosen a pass
+    if kind == "none":
+        assert passes == list(range(1, n_new))
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("beams,end", [(1, -1), (4, -1), (5, 123), (32, -1)])
+def test_beam_search(lib, torch_mod, hd, beams, end):
+    """Scores against the ids' log probabilities by a decoder that steps along
+    them one by one, and the ids against a beam search over that decoder
+    wherever its decisions are wider than the bar."""
+    torch = torch_mod
+    dec, model, d = small_decoder(lib, torch, hd)
+    prompt, n_new = [11, 22, 33, 44, 55], 5
+    got = d.beam_search(prompt, beams, n_new, end)
+    ref = dec.Decoder(lib, torch, model, max_seq=96, fused=True)
+    memo = {}
+
+    def log_probs(ids):  # and how far the bar lets each of them be off
+        if ids not in memo:
+            logits = ref.prefill(prompt)
+            for i, t in enumerate(ids):
+                logits = ref.forward_token(t, len(prompt) + i)
+            x = logits.cpu().numpy().astype(np.float64)
+            memo[ids] = (x - x.max() - np.log(np.exp(x - x.max()).sum()), 2 * LOGITS * np.linalg.norm(x))
+        return memo[ids]
+
+    def steps(ids):  # the tokens that count: up to the first end
+        ids = tuple(ids)
+        return ids[:ids.index(end) + 1] if end in ids else ids
+
+    assert 1 <= len(got) <= beams
+    assert [c for _, c in got] == sorted((c for _, c in got), reverse=True)
+    for ids, score in got:
+        want = bar = 0.0
+        for i, t in enumerate(steps(ids)):
+            lp, off = log_probs(tuple(ids[:i]))
+            want, bar = want + lp[t], bar + off
+        assert abs(score - want) <= bar + 1e-4
+        assert all(t == end for t in ids[len(steps(ids)):])
+    hyps, clear = [((), 0.0, 0.0)], True
+    for _ in range(n_new):
+        cand = []
+        for ids, c, bar in hyps:
+            if end in ids:
+                cand.append((ids + (end,), c, bar))
+                continue
+            lp, off = log_probs(ids)
+            cand += [(ids + (t,), c + lp[t], bar + off) for t in range(600)]
+        cand.sort(key=lambda h: -h[1])
+        for a, b in zip(cand[:beams], cand[1:beams + 1]):
+            clear &= a[1] - b[1] > a[2] + b[2]
+        hyps = cand[:beams]
+    if clear:
+        assert [tuple(i) for i, _ in got] == [h[0] for h in hyps]
+    assert got[0][1] >= hyps[0][1] - 2 * hyps[0][2] - 1e-4 or not clear
+    gncx.check(lib)
+
+
+def test_driver_refusals(lib, torch_mod):
+    _, _, d = small_decoder(lib, torch_mod, 64, max_seq=16)
+    d.prefill([1, 2, 3])
+    for tokens, parents, pos in (([], [], 3), ([1], [-1, 0], 3), ([1, 2], [-1, 0], 15), ([1], [-1], -1)):
+        with pytest.raises(ValueError):
+            d.verify_tree(tokens, parents, pos)
+    with pytest.raises(RuntimeError, match="earlier node"):
+        d.verify_tree([1, 2], [1, -1], 3)
+    with pytest.raises(RuntimeError, match="ascend"):
+        d.keep_path(3, [1, 0])
+    for beams, n in ((0, 4), (33, 4), (2, 0), (2, 15)):
+        with pytest.raises(ValueError):
+            d.beam_search([1, 2, 3], beams, n)
+    _, _, h = small_decoder(lib, torch_mod, 64, max_seq=16, device="cpu")
+    with pytest.raises(ValueError):
+        h.verify_tree([1], [-1], 0)
+    with pytest.raises(ValueError):
+        h.beam_search([1, 2, 3], 2, 2)
