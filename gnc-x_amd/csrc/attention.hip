@@ -1654,10 +1654,13 @@ __device__ __forceinline__ int scale_field(float amax) {
     return min(max(f, 30), 254);
 }
 // The exponent field of the power of two that a group of keys of largest element
-// top is divided by: 127 (none) from 2^-2 to 2^14, else one that brings it to 2^14.
-__device__ __forceinline__ int key_field(float top) {
+// top is divided by, `small` if one's largest is below kPlainAbove: 127 (none) for
+// larger ones up to 2^14, else one that brings top to 2^14.  A pair's last bit is
+// 2^-25 at the least, so either way a key is kept to 2^-22 of its largest element.
+constexpr float kPlainAbove = 0.125f;
+__device__ __forceinline__ int key_field(float top, bool small) {
     const int f = static_cast<int>(as_bits(top) >> 23) & 0xff;
-    return f >= 127 - 2 && f < 127 + 14 ? 127 : min(max(f, 30), 254) - 14;
+    return !small && f < 127 + 14 ? 127 : min(max(f, 30), 254) - 14;
 }
 // max(m, |a|, |b|), NaN if one is
 __device__ __forceinline__ float max3_abs(float m, float a, float b) {
@@ -2039,7 +2042,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) 
             ktop = wave_max(krow < __builtin_inff() ? krow : 0.0f);
             odd = static_cast<uint32_t>(__ballot(is_odd(krow, ktop)));
         }
-        const int kf = key_field(ktop);
+        const int kf = key_field(ktop, __ballot(krow < kPlainAbove) != 0);
         if (kf != 127)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
@@ -2260,7 +2263,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_pair_kernel(TreeParams p) 
             const uint64_t w = __ballot(is_odd(krow, ktop));
             for (int j = 0; j < 16; ++j) odd |= static_cast<uint32_t>(w >> (4 * j) & 1) << j;
         }
-        const int kf = key_field(ktop);
+        const int kf = key_field(ktop, __ballot(krow < kPlainAbove) != 0);
         if (kf != 127)
 #pragma unroll
             for (int c = 0; c < NC; ++c)
@@ -2532,7 +2535,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             const uint64_t w = __ballot(is_odd(krow, ktop));
             for (int j = 0; j < 8; ++j) odd |= static_cast<uint32_t>(w >> (8 * j) & 1) << j;
         }
-        const int kf = key_field(ktop);
+        const int kf = key_field(ktop, __ballot(krow < kPlainAbove) != 0);
         if (kf != 127)
 #pragma unroll
             for (int j = 0; j < NN; ++j)

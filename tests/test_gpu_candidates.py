@@ -91,7 +91,15 @@ class Tree:
         |ds| <= (2^-21 + 8 sqrt(hd) u) max_j scale sum_d |q_d k_jd| for a score
         (operands kept to 2^-22 each, rounding errors of hd additions taken as
         independent), and per output 2 ds + 2^-20 + 8 sqrt(N) u of
-        sum_j w_j |v_j| / l (the weights, their split, the sum over N keys)."""
+        sum_j w_j |v_j| / l (the weights, their split, the sum over N keys).
+        An element far below its row's largest is kept as a pair of halves whose
+        last bit is that of the row: to 2^-22 of a key row's largest element,
+        which adds 2^-22 scale max_j |k_j|_max sum_d |q_d| to ds, and to 2^-25 of
+        a value row's, which adds 2^-25 sum_j w_j |v_j|_max / l.
+        A weight is an fp32 number relative to its row's largest, 1, and an
+        output one by itself: below the smallest normal number, 2^-126, either
+        may count as zero, so an output may be off by 2^-126 sum_j |v_j| / l
+        and by 2^-126 besides."""
         torch, n, H, KV, hd = self.torch, self.n, self.H, self.KV, self.hd
         see = torch.from_numpy(self.visible()).cuda()
         keys = self.pos0 + n
@@ -110,7 +118,11 @@ class Tree:
             l = w.sum(1, keepdim=True) + 1e-12
             want[:, h] = w @ v / l
             ds = (2.0 ** -21 + 8 * math.sqrt(hd) * U) * size
+            largest = torch.where(see, k.abs().amax(1) * qh.abs().sum(1, keepdim=True), 0.0)
+            ds += 2.0 ** -22 * self.scale * largest.amax(1, keepdim=True)
             tol[:, h] = (2 * ds + 2.0 ** -20 + 8 * math.sqrt(keys) * U) * (w @ v.abs() / l)
+            tol[:, h] += 2.0 ** -25 * (w @ v.abs().amax(1, keepdim=True) / l)
+            tol[:, h] += 2.0 ** -126 * (see.double() @ v.abs() / l + 1)
         return want.view(n, H * hd), tol.view(n, H * hd)
 
     def verify(self, lib):
@@ -275,6 +287,41 @@ def test_tree_values_of_any_size(lib, torch_mod, hd, ks, vs):
         c *= vs
     t.q *= min(1.0 / ks, 1e4)
     t.vc[60:70] *= 1e3
+    t.verify(lib)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n", [5, 12, 40, 200])
+@pytest.mark.parametrize("pos0", [0, 37])
+def test_tree_neighbours_of_other_sizes(lib, torch_mod, hd, n, pos0):
+    """First tokens that see themselves (and, with pos0, a few cached rows no
+    larger than they are), of sizes from 0 to 1e30 side by side in a tile: each
+    keeps the precision of its own size."""
+    torch = torch_mod
+    t = Tree(torch, 8, 2, hd, pos0, [-1] * n, seed=n)
+    rng = np.random.default_rng(n)
+    for rows, lo, hi in ((t.k, -25, 3), (t.v, -30, 30)):
+        size = torch.from_numpy(10.0 ** rng.uniform(lo, hi, n)).float().cuda()
+        size[rng.integers(n)] = 0.0
+        rows *= size[:, None]
+    t.kc[:pos0] *= 1e-25
+    t.vc[:pos0] *= 1e-30
+    if pos0:  # a row whose weight is 1 among cached ones
+        t.k[:, ::7] = 0.0
+    t.verify(lib)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("n", [6, 12, 40])
+def test_tree_small_keys_beside_larger_ones(lib, torch_mod, hd, n):
+    """Keys of 1e-5 to 1 side by side under large queries, where a key that is
+    kept to the precision of a larger neighbour would change its score."""
+    torch = torch_mod
+    t = Tree(torch, 8, 2, hd, 2, [-1] * n, seed=n)
+    rng = np.random.default_rng(n)
+    t.k *= torch.from_numpy(10.0 ** rng.uniform(-5, 0, n)).float().cuda()[:, None]
+    t.kc[:2] *= torch.from_numpy(10.0 ** rng.uniform(-5, -4, 2)).float().cuda()[:, None]
+    t.q *= 1e4
     t.verify(lib)
 
 
@@ -711,6 +758,32 @@ def test_selection_and_reordering_captured(lib, torch_mod):
         # a call that needs a larger workspace leaves the graphs theirs
         check_select(lib, torch, torch.randn(4 * (i + 1), 151936, device="cuda"),
                      torch.randn(4 * (i + 1), device="cuda"), 64)
+
+
+def test_kept_rows_captured(lib, torch_mod):
+    torch = torch_mod
+    layers, kv_dim, row0, rows = 66, 72, 3, [0, 2, 3, 9]
+    k, v = (torch.empty(layers, 16, kv_dim, device="cuda") for _ in range(2))
+    ka, va, r = addresses(k), addresses(v), np.asarray(rows, np.int32)
+    g, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    lib.gncx_hip_set_stream(s.cuda_stream)
+    try:
+        with torch.cuda.graph(g, stream=s):
+            lib.gncx_hip_kv_keep_rows(ka, va, layers, kv_dim, row0, r.ctypes.data, len(rows))
+    finally:
+        lib.gncx_hip_set_stream(None)
+    gncx.check(lib)
+    r[:] = 0  # read before the call returned
+    for _ in range(4):
+        k.normal_()
+        v.normal_()
+        want = [c.clone() for c in (k, v)]
+        for w, c in zip(want, (k, v)):
+            w[:, row0:row0 + len(rows)] = c[:, [row0 + i for i in rows]]
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1])
 
 
 def test_select_outputs_that_overlap_are_refused(lib, torch_mod):
