@@ -1717,9 +1717,8 @@ __device__ __forceinline__ void pairs(const float (&v)[N], float scale, V& hi, V
     lo = __builtin_bit_cast(V, l);
 }
 
-constexpr int kTreeKeys = 32;                  // keys of a tile
-constexpr int kTreeStep = kTreeKeys * kWaves;  // keys of a work-group's step, keys over waves
-constexpr int kTreeMaxChunks = 64;             // key ranges of a call
+constexpr int kTreeKeys = 32;        // keys of a tile
+constexpr int kTreeMaxChunks = 256;  // key ranges of a call
 constexpr float kOddBelow = 1.0f / 16384.0f;
 
 // whether a row of the largest element `row` is odd in a group whose largest
@@ -1762,19 +1761,17 @@ __device__ __forceinline__ bool sees_key(const TreeParams& p, const TreeShared& 
 struct RowState {
     float m, mt, l;
 };
-// The softmax of a tile's scores st, in NG groups of 16 / NG registers, group h
-// with the values' exponent ve[h].  Leaves the weights as pairs and returns what O
+// The softmax of a tile's scores st, registers 4 h .. of group h with the values'
+// exponent ve[h].  Leaves the weights as pairs and returns what O
 // so far is to be multiplied with (1: nothing).
-template <int NG>
-__device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&ve)[NG], RowState& s, half8_t (&ph)[2],
+__device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&ve)[4], RowState& s, half8_t (&ph)[2],
                                               half8_t (&pl)[2]) {
-    constexpr int W = 16 / NG;
     float mx = -1e30f, mxt = -1e30f;
 #pragma unroll
-    for (int h = 0; h < NG; ++h) {
+    for (int h = 0; h < 4; ++h) {
         float x = -1e30f;
 #pragma unroll
-        for (int i = 0; i < W; ++i) x = fmaxf(x, st[W * h + i]);
+        for (int i = 0; i < 4; ++i) x = fmaxf(x, st[4 * h + i]);
         mx = fmaxf(mx, x);
         mxt = fmaxf(mxt, x + ve[h]);  // (a group without a visible key, x -1e30, has no say)
     }
@@ -1783,9 +1780,9 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
     const float mt2 = fmaxf(s.mt, ceilf(across_halves(mxt, larger)));
     // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), the second capped: it
     // passes 2^126 only where the first is 0
-    float f[NG], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    float f[4], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int h = 0; h < NG; ++h) f[h] = __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f));
+    for (int h = 0; h < 4; ++h) f[h] = __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f));
     half4_t hi[4], lo[4];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -1795,7 +1792,7 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
             e[i] = __builtin_amdgcn_exp2f(st[4 * a + i] - m2);
             sum[i] += e[i];
         }
-        pairs<true>(e, f[a * NG / 4], hi[a], lo[a]);
+        pairs<true>(e, f[a], hi[a], lo[a]);
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -1810,26 +1807,26 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
     return alpha;
 }
 
-// Adds the odd keys of [t0, t0 + GROUP) (below c1) to a query row: to part, its
+// Adds the odd keys of [t0, t0 + 8) (below c1) to a query row: to part, its
 // normalised output in LDS (float4 d / 4 at 33 (d / 4); the halves of a wave take
 // half of the columns each), and to its state.  The keys are found again by the
 // rule that kept them out of the products.  A weight of 0 takes nothing from a
 // row, whatever it holds.
-template <int HD, int GROUP>
+template <int HD>
 __device__ void add_odd_keys(const TreeParams& p, const TreeShared& tree, const RowPlace& at, float* part, const float* q,
                              const float* kbase, const float* vbase, uint32_t kn, int t0, int c1, int lane, RowState& s) {
-    // lane = key (GROUP of them), over its row
-    const bool in = lane % GROUP + t0 < c1;
+    // lane = key (eight of them), over its row
+    const bool in = lane % 8 + t0 < c1;
     float kmax = 0.0f, vmax = 0.0f;
-    const size_t mine = static_cast<size_t>(min(t0 + lane % GROUP, c1 - 1)) * kn;
+    const size_t mine = static_cast<size_t>(min(t0 + lane % 8, c1 - 1)) * kn;
     for (int d = 0; d < HD; ++d) {
         kmax = maximum_of(kmax, fabsf(kbase[mine + d]));
         vmax = maximum_of(vmax, fabsf(vbase[mine + d]));
     }
     const float ktop = wave_max(in && kmax < __builtin_inff() ? kmax : 0.0f);
     const float vtop = wave_max(in && vmax < __builtin_inff() ? vmax : 0.0f);
-    const uint64_t odd = __ballot(in && lane < GROUP && (is_odd(kmax, ktop) || is_odd(vmax, vtop)));
-    for (int j = 0; j < GROUP; ++j) {
+    const uint64_t odd = __ballot(in && lane < 8 && (is_odd(kmax, ktop) || is_odd(vmax, vtop)));
+    for (int j = 0; j < 8; ++j) {
         if (!(odd >> j & 1)) continue;
         const float* k = kbase + static_cast<size_t>(t0 + j) * kn;
         const float* v = vbase + static_cast<size_t>(t0 + j) * kn;
@@ -1867,576 +1864,28 @@ __device__ __forceinline__ void store_part(float4* part, const floatx16 (&o)[NN]
         }
 }
 
-// Rows of 32 query rows' parts in LDS (parts of a row `stride` float4 and one
-// `per` waves apart, N of them) joined and written: to the output, or as this key
-// range's part.
-template <int HD, int N>
-__device__ __forceinline__ void join_parts(const TreeParams& p, const float4* shared, const float2 (*mls)[32], int per, int tiles,
-                                           int row0, int hk, int G, int rows) {
-    constexpr int kPart = HD / 4 * 33;
+// A work-group's rows from the waves' parts in LDS, with (m, l) beside them: to the
+// output, or as this key range's part.
+template <int HD>
+__device__ __forceinline__ void store_rows(const TreeParams& p, const float4* shared, const float2 (*mls)[32], int row0, int hk,
+                                           int G, int rows) {
     const bool whole = gridDim.z == 1;
     const size_t prow = (static_cast<size_t>(blockIdx.z) * p.n_kv + hk) * p.rows_pad + row0;
-    const int count = min(32 * tiles, rows - row0) * (HD / 4);
+    const int count = min(32 * kWaves, rows - row0) * (HD / 4);
 #pragma unroll 4
     for (int i = threadIdx.x; i < count; i += kThreads) {
         const int r = i / (HD / 4), d4 = i % (HD / 4);
-        float M = mls[r / 32][r % 32].x, L = mls[r / 32][r % 32].y;
-        float4 x = shared[r / 32 * kPart + d4 * 33 + r % 32];
-        if constexpr (N > 1) {
-#pragma unroll
-            for (int w = 1; w < N; ++w) M = fmaxf(M, mls[r / 32 + per * w][r % 32].x);
-            L = 0.0f;
-            x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-            for (int w = 0; w < N; ++w) {
-                const float2 ml = mls[r / 32 + per * w][r % 32];
-                const float wt = ml.y * __builtin_amdgcn_exp2f(ml.x - M);
-                const float4 v = shared[(r / 32 + per * w) * kPart + d4 * 33 + r % 32];
-                L += wt;
-                if (wt != 0.0f) {  // (a part without a key has nothing to add)
-                    x.x += wt * v.x;
-                    x.y += wt * v.y;
-                    x.z += wt * v.z;
-                    x.w += wt * v.w;
-                }
-            }
-            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-            x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-        }
+        const float2 ml = mls[r / 32][r % 32];
+        float4 x = shared[r / 32 * (HD / 4 * 33) + d4 * 33 + r % 32];
         if (whole) {
             const int row = row0 + r;
-            if (N == 1 && L != L) x = make_float4(L, L, L, L);  // (an odd key that makes its row NaN)
+            if (ml.y != ml.y) x = make_float4(ml.y, ml.y, ml.y, ml.y);  // (an odd key that makes its row NaN)
             reinterpret_cast<float4*>(p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD)[d4] = x;
         } else {
             reinterpret_cast<float4*>(p.part_o + (prow + r) * HD)[d4] = x;
-            if (d4 == 0) p.part_ml[prow + r] = make_float2(M, L);
+            if (d4 == 0) p.part_ml[prow + r] = ml;
         }
     }
-}
-
-// Keys over waves, for up to 32 query rows of a KV head: each wave of a work-group
-// walks every fourth 32-key tile of its range by itself, with the tile's K and V
-// straight from memory into the registers that the products take, so the loop has
-// no barrier and every K/V byte is read once.  Buffer loads are bounded by the
-// range's last row: rows past it read as zeros.
-template <int HD, int OCC>
-__global__ __launch_bounds__(kThreads, OCC) void tree_keys_kernel(TreeParams p) {
-    constexpr int NC = HD / 16, NN = HD / 32;
-    constexpr int VW = NN < 4 ? NN : 4;  // value columns a lane loads at once: column 32 VW (n / VW) + VW li + n % VW
-    constexpr int kPart = HD / 4 * 33;   // float4 of a wave's 32 rows, padded per float4 column
-    constexpr int kQ = NC * 64;          // half8 of the query rows' hi (and lo) parts
-    static_assert(kQ * 2 <= kPart * kWaves, "the query rows fit where the parts go");
-    __shared__ __align__(16) float4 shared[kPart * kWaves];
-    __shared__ float qfac[32];
-    __shared__ float2 mls[kWaves][32];
-    __shared__ TreeShared tree;
-    half8_t* const qhi = reinterpret_cast<half8_t*>(shared);
-    half8_t* const qlo = qhi + kQ;
-    const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * 32;
-    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(p.pos0 + p.n, c0 + p.chunk);
-    const uint32_t kn = static_cast<uint32_t>(p.n_kv) * HD;
-    const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
-    const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
-
-    auto tile_of = [&](const float* base, int t0) {
-        const uint32_t n = static_cast<uint32_t>(min(c1 - t0, kTreeKeys) - 1) * kn + HD;
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + static_cast<size_t>(t0) * kn),
-                                                 static_cast<short>(0), static_cast<int32_t>(n * 4), 0x00020000);
-    };
-    float kr[NC][8], vr[NN][16];
-    const uint32_t kat = (static_cast<uint32_t>(li) * kn + 8 * g) * 4, vat = (4 * g * kn + VW * li) * 4;
-    auto load_k = [&](int t0) {
-        const auto rs = tile_of(kbase, t0);
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const auto v = __builtin_amdgcn_raw_buffer_load_b128(rs, static_cast<int>(kat + 64 * c + 16 * h), 0, 0);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) kr[c][4 * h + i] = as_float(v[i]);
-            }
-    };
-    auto load_v = [&](int t0) {
-        const auto rs = tile_of(vbase, t0);
-        uint32_t row = kn * 4;
-        asm volatile("" : "+s"(row));  // (sixteen addresses kept over the loop would cost registers)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int at = static_cast<int>(vat + static_cast<uint32_t>(8 * (r >> 2) + (r & 3)) * row);
-#pragma unroll
-            for (int n = 0; n < NN; n += VW) {
-                if constexpr (VW == 4) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(rs, at + 128 * n, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) vr[n + i][r] = as_float(v[i]);
-                } else {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(rs, at + 128 * n, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) vr[n + i][r] = as_float(v[i]);
-                }
-            }
-        }
-    };
-    const int first = c0 + kTreeKeys * wv;
-    // Loads run a tile ahead, a tile's keys while the tile before is in its value
-    // products, its values behind those; at head_dim 256 there are no registers
-    // for that: keys behind the products, values behind the scores.
-    constexpr bool kAhead = HD <= 128;
-    if (first < c1) {
-        load_k(first);
-        if (kAhead) load_v(first);
-    }
-
-    const int myrow = min(row0 + li, rows - 1);
-    const RowPlace place = place_of(p, myrow / G);
-    // the query rows, 8 threads each: scaled, split and laid out as operands
-    {
-        const int r = row0 + tid / 8, j = tid % 8;
-        float x[HD / 64][8], amax = 0.0f;
-        const float* src = p.q + (static_cast<size_t>(r < rows ? r / G : 0) * p.n_heads + hk * G + r % G) * HD + j * (HD / 8);
-#pragma unroll
-        for (int u = 0; u < HD / 64; ++u)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[u][i] = r < rows ? src[8 * u + i] : 0.0f;
-                amax = fmaxf(amax, fabsf(x[u][i]));
-            }
-        const int f = scale_field(group8_max(amax));
-#pragma unroll
-        for (int u = 0; u < HD / 64; ++u) {
-            half8_t h, l;
-            pairs<true>(x[u], pow2_field(254 + 7 - f), h, l);
-            const int unit = j * (HD / 64) + u, at = unit / 2 * 64 + 32 * (unit & 1) + tid / 8;
-            qhi[at] = h;
-            qlo[at] = l;
-        }
-        if (j == 0) qfac[tid / 8] = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
-    }
-    if (c1 > p.pos0) load_tree(p, tree);
-    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.max_depth - p.sw + 1) : 0;
-    __syncthreads();
-
-    RowState s{-1e30f, -1e30f, 0.0f};
-    const float qf = qfac[li];
-    floatx16 o[NN];
-#pragma unroll
-    for (int n = 0; n < NN; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
-    int odd_first = c1, odd_last = -1;  // tiles that hold odd keys
-
-    for (int t0 = first; t0 < c1; t0 += kTreeStep) {
-        const int next = t0 + kTreeStep;
-        // ---- scores
-        float krow = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; i += 2) krow = max3_abs(krow, kr[c][i], kr[c][i + 1]);
-        krow = across_halves(krow, maximum_of);
-        float ktop = wave_maximum(krow);
-        uint32_t odd = static_cast<uint32_t>(__ballot(is_odd(krow, ktop)));  // keys, and with its values' below
-        if (odd) {
-            ktop = wave_max(krow < __builtin_inff() ? krow : 0.0f);
-            odd = static_cast<uint32_t>(__ballot(is_odd(krow, ktop)));
-        }
-        const int kf = key_field(ktop, __ballot(krow < kPlainAbove) != 0);
-        if (kf != 127)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) kr[c][i] *= pow2_field(254 - kf);
-        floatx16 st;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            half8_t kh, kl;
-            pairs<false>(kr[c], 1.0f, kh, kl);
-            const half8_t h = qhi[c * 64 + lane], lw = qlo[c * 64 + lane];
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, h, st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, lw, st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, h, st, 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (!kAhead) load_v(t0);
-
-        // ---- the values' power of two, and whether every row is near it (a row
-        // of zeros is as good)
-        float vrow[16], vtop = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            vrow[r] = max3_abs(0.0f, vr[0][r], vr[1][r]);
-#pragma unroll
-            for (int n = 2; n < NN; n += 2) vrow[r] = max3_abs(vrow[r], vr[n][r], vr[n + 1][r]);
-        }
-#pragma unroll
-        for (int r = 0; r < 16; r += 2) vtop = maximum_of(maximum_of(vtop, vrow[r]), vrow[r + 1]);
-        vtop = wave_maximum(vtop);
-        bool near = vtop < __builtin_inff();
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const uint64_t here = __ballot(vrow[r] >= vtop * kOddBelow);
-            near = near && static_cast<uint32_t>(here) && here >> 32;
-        }
-        if (!near) {
-            // each row's largest element over its 32 lanes, then the rule
-            uint32_t bad = 0;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                float x = vrow[r];
-                x = dpp_maximum<0xb1>(x, x);
-                x = dpp_maximum<0x4e>(x, x);
-                x = dpp_maximum<0x141>(x, x);
-                x = dpp_maximum<0x140>(x, x);
-                const auto y = __builtin_amdgcn_permlane16_swap(as_bits(x), as_bits(x), false, false);
-                vrow[r] = maximum_of(as_float(y[0]), as_float(y[1]));
-            }
-            vtop = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (vrow[r] < __builtin_inff()) vtop = fmaxf(vtop, vrow[r]);
-            vtop = across_halves(vtop, maximum_of);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const bool b = is_odd(vrow[r], vtop);
-                const uint64_t w = __ballot(b);
-                const int key = 8 * (r >> 2) + (r & 3);
-                if (static_cast<uint32_t>(w)) bad |= 1u << key;
-                if (w >> 32) bad |= 1u << (key + 4);
-#pragma unroll
-                for (int n = 0; n < NN; ++n) vr[n][r] = b ? 0.0f : vr[n][r];
-            }
-            odd |= bad;
-        }
-        if (odd) {
-            odd_first = min(odd_first, t0);
-            odd_last = t0;
-        }
-        const int vf = scale_field(vtop) - 14;  // the field of the power of two that they are divided by
-        const float vs = pow2_field(254 - vf), ve[1] = {static_cast<float>(vf - 127)};
-
-        // ---- softmax
-        const float sf = pow2_field(kf) * qf;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] *= sf;
-        if (t0 + kTreeKeys > min(p.pos0, c1) || t0 < lo_most || odd)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = 8 * (r >> 2) + 4 * g + (r & 3);
-                if (!sees_key(p, tree, place, t0 + j, c1) || (odd >> j & 1)) st[r] = -__builtin_inff();
-            }
-        half8_t ph[2], pl[2];
-        const float alpha = tile_softmax(st, ve, s, ph, pl);
-        if (__ballot(alpha != 1.0f))
-#pragma unroll
-            for (int n = 0; n < NN; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
-        __builtin_amdgcn_sched_barrier(0);
-        if (kAhead && next < c1) load_k(next);
-        __builtin_amdgcn_sched_barrier(0);
-
-        // ---- weighted values
-#pragma unroll
-        for (int n = 0; n < NN; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float x[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = vr[n][8 * c + i];
-                half8_t vh, vl;
-                pairs<true>(x, vs, vh, vl);
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[c], o[n], 0, 0, 0);
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[c], o[n], 0, 0, 0);
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[c], o[n], 0, 0, 0);
-            }
-        __builtin_amdgcn_sched_barrier(0);
-        if (next < c1) {
-            if (kAhead) load_v(next);
-            else load_k(next);
-        }
-    }
-
-    // ---- the waves' parts meet in LDS
-    __syncthreads();  // the query rows are done with
-    float4* const part = shared + wv * kPart;
-    store_part<NN>(part, o, s, li, g);
-    if (odd_last >= 0) {
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
-        asm volatile("" ::: "memory");
-        for (int t0 = odd_first; t0 <= odd_last; t0 += kTreeStep)
-            add_odd_keys<HD, kTreeKeys>(p, tree, place, reinterpret_cast<float*>(part + li),
-                                        p.q + (static_cast<size_t>(myrow / G) * p.n_heads + hk * G + myrow % G) * HD, kbase,
-                                        vbase, kn, t0, c1, lane, s);
-    }
-    if (g == 0) mls[wv][li] = make_float2(s.m, s.l);
-    __syncthreads();
-    join_parts<HD, kWaves>(p, shared, mls, 1, 1, row0, hk, G, rows);
-}
-
-// Rows and keys over waves, for 33 to 64 query rows of a KV head: a work-group
-// takes 64 rows and two 32-key tiles a step, which its waves load, scale, split
-// and lay out in LDS as operands once for all of them (waves 2 s and 2 s + 1 stage
-// tile s, 16 keys and 16 values each, a group with powers of two of its own).
-// Waves w and w + 2 own the same 32 rows, a tile each, and meet at the end.  The
-// next step's loads are in flight during this one's products; two work-groups a CU
-// fill each other's waits.
-template <int HD, int OCC>
-__global__ __launch_bounds__(kThreads, OCC) void tree_pair_kernel(TreeParams p) {
-    constexpr int NC = HD / 16, NN = HD / 32, RW = 2, KW = 2;
-    constexpr int VW = NN < 4 ? NN : 4;
-    constexpr int kPart = HD / 4 * 33;
-    constexpr int kTile = NC * 64;  // half8 of a tile's keys' hi (or lo) parts, and of its values'
-    constexpr int kShared = kTile * 8 > kPart * kWaves ? kTile * 8 : kPart * kWaves;
-    __shared__ __align__(16) float4 shared[kShared];
-    __shared__ float kfac[2][2], vexp[2][2];  // [tile][half]: the keys' factor, the values' exponent
-    __shared__ uint32_t oddmask[2][2];        // [tile][half]: odd keys, from bit 16 half on
-    __shared__ float2 mls[kWaves][32];
-    __shared__ int odd_first, odd_last;
-    __shared__ TreeShared tree;
-    half8_t* const khi = reinterpret_cast<half8_t*>(shared);  // [tile][slice][lane]
-    half8_t* const klo = khi + 2 * kTile;
-    half8_t* const vhi = khi + 4 * kTile;                     // [tile][column tile][slice][lane]
-    half8_t* const vlo = khi + 6 * kTile;
-    const int tid = threadIdx.x, lane = tid & 63, li = lane & 31, g = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int hk = blockIdx.x, G = p.n_heads / p.n_kv, rows = p.n * G, row0 = static_cast<int>(blockIdx.y) * 32 * RW;
-    const int c0 = p.first + static_cast<int>(blockIdx.z) * p.chunk, c1 = min(p.pos0 + p.n, c0 + p.chunk);
-    const uint32_t kn = static_cast<uint32_t>(p.n_kv) * HD;
-    const float* const kbase = p.k_cache + static_cast<size_t>(hk) * HD;
-    const float* const vbase = p.v_cache + static_cast<size_t>(hk) * HD;
-
-    // ---- staging: wave 2 s + c loads keys 16 c .. + 16 of tile s (four lanes a
-    // key, 64 bytes a load) and values of slice c, keys 16 c .. + 16, too (a lane
-    // half a row; register i of half g is key 16 c + 4 g + i % 4 + 8 (i / 4))
-    const int ts = wv >> 1, tc = wv & 1;
-    auto tile_of = [&](const float* base, int t0) {
-        const int n = min(c1 - t0, kTreeKeys);  // none past the range: every load reads zeros
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(base + static_cast<size_t>(t0) * kn), static_cast<short>(0),
-                                                 n > 0 ? static_cast<int32_t>((static_cast<uint32_t>(n - 1) * kn + HD) * 4) : 0,
-                                                 0x00020000);
-    };
-    float kst[NC][4], vst[NN][8];
-    const int key4 = 16 * tc + lane / 4, quarter = lane % 4;
-    const uint32_t kat = (static_cast<uint32_t>(key4) * kn + 4 * quarter) * 4;
-    const uint32_t vat = ((16 * tc + 4 * g) * kn + VW * li) * 4;
-    auto prefetch = [&](int t0) {
-        const auto ks = tile_of(kbase, t0 + kTreeKeys * ts), vs = tile_of(vbase, t0 + kTreeKeys * ts);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const auto v = __builtin_amdgcn_raw_buffer_load_b128(ks, static_cast<int>(kat + 64 * c), 0, 0);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) kst[c][i] = as_float(v[i]);
-        }
-        uint32_t row = kn * 4;
-        asm volatile("" : "+s"(row));  // (eight addresses kept over the loop would cost registers)
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const int at = static_cast<int>(vat + static_cast<uint32_t>(8 * (r >> 2) + (r & 3)) * row);
-#pragma unroll
-            for (int n = 0; n < NN; n += VW) {
-                if constexpr (VW == 4) {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b128(vs, at + 128 * n, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) vst[n + i][r] = as_float(v[i]);
-                } else {
-                    const auto v = __builtin_amdgcn_raw_buffer_load_b64(vs, at + 128 * n, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) vst[n + i][r] = as_float(v[i]);
-                }
-            }
-        }
-    };
-    auto stage = [&](int t0) {
-        uint32_t odd = 0;  // this group's odd keys
-        float krow = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) krow = max3_abs(max3_abs(krow, kst[c][0], kst[c][1]), kst[c][2], kst[c][3]);
-        krow = dpp_maximum<0xb1>(krow, krow);
-        krow = dpp_maximum<0x4e>(krow, krow);
-        float ktop = wave_maximum(krow);
-        if (__ballot(is_odd(krow, ktop))) {
-            ktop = wave_max(krow < __builtin_inff() ? krow : 0.0f);
-            const uint64_t w = __ballot(is_odd(krow, ktop));
-            for (int j = 0; j < 16; ++j) odd |= static_cast<uint32_t>(w >> (4 * j) & 1) << j;
-        }
-        const int kf = key_field(ktop, __ballot(krow < kPlainAbove) != 0);
-        if (kf != 127)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) kst[c][i] *= pow2_field(254 - kf);
-        // slice c, half quarter / 2, elements 4 (quarter % 2) ..
-        const int kslot = (ts * kTile + (quarter >> 1) * 32 + key4) * 2 + (quarter & 1);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            half4_t hi, lo;
-            pairs<false>(kst[c], 1.0f, hi, lo);
-            reinterpret_cast<half4_t*>(khi)[kslot + 128 * c] = hi;
-            reinterpret_cast<half4_t*>(klo)[kslot + 128 * c] = lo;
-        }
-        float vrow[8], vtop = 0.0f;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            vrow[r] = max3_abs(0.0f, vst[0][r], vst[1][r]);
-#pragma unroll
-            for (int n = 2; n < NN; n += 2) vrow[r] = max3_abs(vrow[r], vst[n][r], vst[n + 1][r]);
-        }
-#pragma unroll
-        for (int r = 0; r < 8; r += 2) vtop = maximum_of(maximum_of(vtop, vrow[r]), vrow[r + 1]);
-        vtop = wave_maximum(vtop);
-        bool near = vtop < __builtin_inff();
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const uint64_t here = __ballot(vrow[r] >= vtop * kOddBelow);
-            near = near && static_cast<uint32_t>(here) && here >> 32;
-        }
-        if (!near) {
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                float x = vrow[r];
-                x = dpp_maximum<0xb1>(x, x);
-                x = dpp_maximum<0x4e>(x, x);
-                x = dpp_maximum<0x141>(x, x);
-                x = dpp_maximum<0x140>(x, x);
-                const auto y = __builtin_amdgcn_permlane16_swap(as_bits(x), as_bits(x), false, false);
-                vrow[r] = maximum_of(as_float(y[0]), as_float(y[1]));
-            }
-            vtop = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (vrow[r] < __builtin_inff()) vtop = fmaxf(vtop, vrow[r]);
-            vtop = across_halves(vtop, maximum_of);
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-                const bool b = is_odd(vrow[r], vtop);
-                const uint64_t w = __ballot(b);
-                const int key = 8 * (r >> 2) + (r & 3);
-                if (static_cast<uint32_t>(w)) odd |= 1u << key;
-                if (w >> 32) odd |= 1u << (key + 4);
-#pragma unroll
-                for (int n = 0; n < NN; ++n) vst[n][r] = b ? 0.0f : vst[n][r];
-            }
-        }
-        const int vf = scale_field(vtop) - 14;
-        const float vs = pow2_field(254 - vf);
-        if (lane == 0) {
-            kfac[ts][tc] = pow2_field(kf);
-            vexp[ts][tc] = static_cast<float>(vf - 127);
-            oddmask[ts][tc] = odd << (16 * tc);
-            if (odd) {
-                atomicMin(&odd_first, t0 + kTreeKeys * ts + 16 * tc);
-                atomicMax(&odd_last, t0 + kTreeKeys * ts + 16 * tc);
-            }
-        }
-#pragma unroll
-        for (int n = 0; n < NN; ++n) {
-            half8_t hi, lo;
-            pairs<true>(vst[n], vs, hi, lo);
-            vhi[ts * kTile + (n * 2 + tc) * 64 + lane] = hi;
-            vlo[ts * kTile + (n * 2 + tc) * 64 + lane] = lo;
-        }
-    };
-
-    prefetch(c0);
-    if (tid == 0) {
-        odd_first = c1;
-        odd_last = -1;
-    }
-    if (c1 > p.pos0) load_tree(p, tree);
-    // this wave's query rows as operands, in registers
-    const int rt = wv % RW, myrow = min(row0 + 32 * rt + li, rows - 1);
-    const float* const qrow = p.q + (static_cast<size_t>(myrow / G) * p.n_heads + hk * G + myrow % G) * HD;
-    half8_t qh[NC], ql[NC];
-    float qf;
-    {
-        float x[NC][8], amax = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[c][i] = qrow[16 * c + 8 * g + i];
-                amax = fmaxf(amax, fabsf(x[c][i]));
-            }
-        const int f = scale_field(across_halves(amax, maximum_of));
-#pragma unroll
-        for (int c = 0; c < NC; ++c) pairs<true>(x[c], pow2_field(254 + 7 - f), qh[c], ql[c]);
-        qf = pow2_field(f - 7) * (p.scale * 1.4426950408889634f);
-    }
-    const RowPlace place = place_of(p, myrow / G);
-    const int lo_most = p.sw > 0 ? max(0, p.pos0 + p.max_depth - p.sw + 1) : 0;
-
-    RowState st_row{-1e30f, -1e30f, 0.0f};
-    floatx16 o[NN];
-#pragma unroll
-    for (int n = 0; n < NN; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) o[n][r] = 0.0f;
-
-    auto take_tile = [&](int s, int t0) {
-        floatx16 st;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const half8_t kh = khi[s * kTile + c * 64 + lane], kl = klo[s * kTile + c * 64 + lane];
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, qh[c], st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kh, ql[c], st, 0, 0, 0);
-            st = __builtin_amdgcn_mfma_f32_32x32x16_f16(kl, qh[c], st, 0, 0, 0);
-        }
-        const float ve[2] = {vexp[s][0], vexp[s][1]}, sf[2] = {kfac[s][0] * qf, kfac[s][1] * qf};
-        const uint32_t odd = __builtin_amdgcn_readfirstlane(oddmask[s][0] | oddmask[s][1]);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) st[r] *= sf[r >> 3];
-        if (t0 + kTreeKeys > min(p.pos0, c1) || t0 < lo_most || odd)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = 8 * (r >> 2) + 4 * g + (r & 3);
-                if (!sees_key(p, tree, place, t0 + j, c1) || (odd >> j & 1)) st[r] = -__builtin_inff();
-            }
-        half8_t ph[2], pl[2];
-        const float alpha = tile_softmax(st, ve, st_row, ph, pl);
-        if (__ballot(alpha != 1.0f))
-#pragma unroll
-            for (int n = 0; n < NN; ++n)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) o[n][r] *= alpha;
-#pragma unroll
-        for (int n = 0; n < NN; ++n)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                const half8_t vh = vhi[s * kTile + (n * 2 + c) * 64 + lane], vl = vlo[s * kTile + (n * 2 + c) * 64 + lane];
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, ph[c], o[n], 0, 0, 0);
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vh, pl[c], o[n], 0, 0, 0);
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vl, ph[c], o[n], 0, 0, 0);
-            }
-    };
-
-    __syncthreads();  // odd_first / odd_last, the tree
-    for (int t0 = c0; t0 < c1; t0 += 2 * kTreeKeys) {
-        stage(t0);
-        __syncthreads();
-        if (t0 + 2 * kTreeKeys < c1) prefetch(t0 + 2 * kTreeKeys);
-        if (t0 + kTreeKeys * (wv / RW) < c1) take_tile(wv / RW, t0 + kTreeKeys * (wv / RW));
-        __syncthreads();  // every wave is done with the operands
-    }
-
-    float4* const part = shared + wv * kPart;
-    store_part<NN>(part, o, st_row, li, g);
-    if (odd_last >= 0) {
-        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
-        asm volatile("" ::: "memory");
-        for (int t0 = odd_first; t0 <= odd_last; t0 += 16)
-            if ((t0 - c0) / kTreeKeys % 2 == wv / RW)
-                add_odd_keys<HD, 16>(p, tree, place, reinterpret_cast<float*>(part + li), qrow, kbase, vbase, kn, t0, c1, lane,
-                                     st_row);
-    }
-    if (g == 0) mls[wv][li] = make_float2(st_row.m, st_row.l);
-    __syncthreads();
-    join_parts<HD, KW>(p, shared, mls, RW, RW, row0, hk, G, rows);
 }
 
 // The order of N times (two operand reads from LDS, three products): the reads
@@ -2705,25 +2154,27 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
     stage(0, c0);
     if (c0 + kTreeKeys < c1) prefetch(c0 + kTreeKeys);
     __syncthreads();
+    // (a wave whose 32 rows are none stages for the others)
+    const bool mine = row0 + 32 * wv < rows;
     int b = 0;
     for (int t0 = c0; t0 < c1; t0 += kTreeKeys, b ^= 1) {
         if (t0 + kTreeKeys < c1) stage(b ^ 1, t0 + kTreeKeys);
         if (t0 + 2 * kTreeKeys < c1) prefetch(t0 + 2 * kTreeKeys);
-        take_tile(b, t0);
+        if (mine) take_tile(b, t0);
         __syncthreads();  // the next tile is laid out, and this one done with
     }
 
     float4* const part = shared + wv * kPart;
     store_part<NN>(part, o, s, li, g);
-    if (odd_last >= 0) {
+    if (mine && odd_last >= 0) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
         asm volatile("" ::: "memory");
         for (int t0 = odd_first; t0 <= odd_last; t0 += 8)
-            add_odd_keys<HD, 8>(p, tree, place, reinterpret_cast<float*>(part + li), qrow, kbase, vbase, kn, t0, c1, lane, s);
+            add_odd_keys<HD>(p, tree, place, reinterpret_cast<float*>(part + li), qrow, kbase, vbase, kn, t0, c1, lane, s);
     }
     if (g == 0) mls[wv][li] = make_float2(s.m, s.l);
     __syncthreads();
-    join_parts<HD, 1>(p, shared, mls, kWaves, kWaves, row0, hk, G, rows);
+    store_rows<HD>(p, shared, mls, row0, hk, G, rows);
 }
 
 // out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the key
@@ -2732,7 +2183,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
 constexpr int kTreeMergeLoads = 8;
 template <int HD, int CG>
 __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams p, int32_t chunks) {
-    static_assert(kTreeMergeLoads * 8 >= kTreeMaxChunks, "eight threads take every range");
+    static_assert(kTreeMergeLoads * 32 >= kTreeMaxChunks, "32 threads take every range");
     constexpr int kCols = kThreads / CG;  // float4 of a work-group
     __shared__ float4 part[CG][kCols];
     __shared__ float2 mls[CG][kCols];
@@ -2784,35 +2235,37 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams p, int3
         make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
 }
 
-// The split of a call: 32 row tiles a work-group (1: keys over its waves),
-// keys a work-group, key ranges.
+// The split of a call: groups of rows, keys of a range, ranges.
 struct TreePlan {
-    int32_t tiles, first, chunk, chunks, rows_pad;
+    int32_t groups, first, chunk, chunks, rows_pad;
 };
 
 TreePlan tree_plan(const TreeArgs& a) {
     TreePlan pl;
+    constexpr int32_t kRows = 32 * kWaves;
     const int32_t rows = a.n * (a.n_heads / a.n_kv_heads);
-    pl.tiles = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-    const int32_t groups = (rows + 32 * pl.tiles - 1) / (32 * pl.tiles);
-    pl.rows_pad = groups * 32 * pl.tiles;
+    pl.groups = (rows + kRows - 1) / kRows;
+    pl.rows_pad = pl.groups * kRows;
     pl.first = a.sliding_window > 0 ? std::max(0, a.pos0 - a.sliding_window + 1) : 0;
     const int64_t keys = static_cast<int64_t>(a.pos0) + a.n - pl.first, tiles = (keys + kTreeKeys - 1) / kTreeKeys;
-    const int64_t heads = static_cast<int64_t>(groups) * a.n_kv_heads, unit = pl.tiles == 1 ? kWaves : pl.tiles == 2 ? 2 : 1;
-    // tiles a work-group for that many of them, whole steps from one step on
-    auto tiles_for = [&](int64_t work_groups) {
-        const int64_t ranges = std::min<int64_t>(std::max<int64_t>(1, work_groups / heads), kTreeMaxChunks);
-        const int64_t t = (tiles + ranges - 1) / ranges;
-        return t < unit ? t : (t + unit - 1) / unit * unit;
+    const int64_t heads = static_cast<int64_t>(pl.groups) * a.n_kv_heads;
+    auto ranges_of = [&](int64_t work_groups) {
+        return std::min<int64_t>(std::max<int64_t>(1, work_groups / heads), kTreeMaxChunks);
     };
-    int64_t per = tiles_for(256);
-    // Two work-groups of the 128-row kernel share a CU with heads up to 128.  Twice
-    // the ranges halve the tiles of each and double the parts that meet, which take
-    // about as long each: worth it where a range has more tiles than there are
-    // ranges.  32 heads over 8 of 128: 256 nodes at 300 (5 tiles, 4 ranges)
-    // 48.6 -> 44.0 us, at 4096 (17, 4) 112 -> 95; 64 nodes at 8192 (17, 16) 56 -> 52,
-    // but at 4096 (9, 16) 38.5 -> 41.8; 32 nodes at 2048 (3, 32) 27.2 -> 30.5.
-    if (pl.tiles == 4 && a.head_dim <= 128 && per > 256 / heads) per = tiles_for(512);
+    int64_t ranges = ranges_of(256), per = (tiles + ranges - 1) / ranges;
+    // Two work-groups share a CU with heads up to 128.  Twice the ranges halve the
+    // tiles of each, and double the parts that meet, the more the more rows there
+    // are: worth it from per = ranges on for a group of 128 rows, sooner for fewer.
+    // 32 heads over 8 of 128, 256 against 512 work-groups: 128 rows at 2048 (per 3,
+    // ranges 32) 27.2 and 30.5 us, at 32000 (32) 95.6 and 88.2; 256 rows at 4096 (9,
+    // 16) 38.5 and 41.8, at 8192 (17) 56 and 52; 1024 rows at 300 (5, 4) 48.6 and
+    // 44.0; 64 rows at 4096 (5, 32) 26.5 and 27.3, at 8192 (9) 36.0 and 34.3; 16 rows
+    // at 2048 (3, 32) 19.1 and 18.3, at 32749 (32) 87 and 60.
+    const int64_t used = std::min<int64_t>(kWaves, (rows + 31) / 32);
+    if (a.head_dim <= 128 && per * kWaves * kWaves >= ranges * used * used) {
+        ranges = ranges_of(512);
+        per = (tiles + ranges - 1) / ranges;
+    }
     pl.chunk = static_cast<int32_t>(per * kTreeKeys);
     pl.chunks = static_cast<int32_t>((tiles + per - 1) / per);
     return pl;
@@ -2824,10 +2277,7 @@ hipError_t launch_tree(const TreeParams& p, const TreeTable& tree, const TreePla
     hipLaunchKernelGGL(tree_prologue_kernel<HD>, dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p, tree);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const dim3 grid(p.n_kv, pl.rows_pad / (32 * pl.tiles), pl.chunks);
-    if (pl.tiles == 1) hipLaunchKernelGGL((tree_keys_kernel<HD, OCC>), grid, dim3(kThreads), 0, stream, p);
-    else if (pl.tiles == 2) hipLaunchKernelGGL((tree_pair_kernel<HD, OCC>), grid, dim3(kThreads), 0, stream, p);
-    else hipLaunchKernelGGL((tree_rows_kernel<HD, OCC>), grid, dim3(kThreads), 0, stream, p);
+    hipLaunchKernelGGL((tree_rows_kernel<HD, OCC>), dim3(p.n_kv, pl.groups, pl.chunks), dim3(kThreads), 0, stream, p);
     e = hipGetLastError();
     if (e != hipSuccess || pl.chunks == 1) return e;
     const int64_t n = static_cast<int64_t>(p.n) * (p.n_heads / p.n_kv) * HD / 4;
@@ -2838,7 +2288,8 @@ hipError_t launch_tree(const TreeParams& p, const TreeTable& tree, const TreePla
     };
     if (pl.chunks <= kTreeMergeLoads) merge(std::integral_constant<int, 1>{});
     else if (pl.chunks <= 4 * kTreeMergeLoads) merge(std::integral_constant<int, 4>{});
-    else merge(std::integral_constant<int, 8>{});
+    else if (pl.chunks <= 8 * kTreeMergeLoads) merge(std::integral_constant<int, 8>{});
+    else merge(std::integral_constant<int, 32>{});
     return hipGetLastError();
 }
 

@@ -3075,8 +3075,8 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
     const char* where = "gncx_hip_attention_tree";
     if (n_nodes == 0) return;
     if (n_heads < 1 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || n_heads > 65535 || pos0 < 0 ||
-        pos0 > INT32_MAX - kMaxTreeNodes || (head_dim != 64 && head_dim != 128 && head_dim != 256)) {
-        set_error(where, "invalid head geometry or position (head_dim is 64, 128 or 256)", -1);
+        pos0 > INT32_MAX - kMaxTreeNodes || n_heads / n_kv_heads > 8192 || (head_dim != 64 && head_dim != 128 && head_dim != 256)) {
+        set_error(where, "invalid head geometry or position (head_dim is 64, 128 or 256, at most 8192 heads to a KV head)", -1);
         return;
     }
     TreeTable tree;
