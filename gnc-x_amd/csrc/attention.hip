@@ -1560,6 +1560,9 @@ struct TreeParams {
 // store their cache rows.  The arithmetic is prologue_head_r's of the decode
 // step (head_inv_rms, no contraction), so an accepted node's cache row is the
 // one that decoding its token would have stored.
+// A launch of its own (4 nodes, 40 heads of 128: 3.7 us; 128 nodes, 36 heads: 4.9):
+// done by the next kernel's work-groups, its rotations and norms are on the way of
+// each of them, 3.7 + 8.3 us against 14.2 (4 nodes at 300).
 template <int HD>
 __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, TreeTable tree) {
 #pragma clang fp contract(off)
@@ -1618,7 +1621,7 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, T
     }
 }
 
-// The products on the fp16 matrix cores.  Both kernels below compute, per 32-key
+// The products on the fp16 matrix cores.  The kernel below computes, per 32-key
 // tile and 32 query rows (node, head) of one KV head,
 //   S^T = K Q^T      v_mfma_f32_32x32x16_f16, operands as fp16 pairs, three
 //                    products a slice (hi hi, hi lo, lo hi: 2^-22 of the product);
@@ -1627,9 +1630,9 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, T
 //   O^T += V^T P^T   with P from those registers, and O of row i in lane (i, .):
 //                    the softmax factors of a row never cross lanes
 // Pairs hold about 22 bits of values from 2^-3 to 2^15, and 2^-25 absolutely
-// below.  Every query row, and every group of values (a tile's, or half of it), is
-// brought there by a power of two; a group of keys as well unless its largest
-// element lies there (their scores are sums, in which its small ones do not show).
+// below.  Every query row, and every group of eight values, is brought there by a
+// power of two; a group of eight keys as well unless all of them lie there.  So an
+// element keeps 2^-22 of itself or of its row's largest, where that is more.
 // The keys' and the row's come back as a factor of the scores.  The values' 2^e
 // goes into the weights: those of O are 2^(s + e - max (s + e)), those of the sum
 // l 2^(s - max s), two running maxima a row, so that what a row does not see has
@@ -1890,7 +1893,7 @@ __device__ __forceinline__ void store_rows(const TreeParams& p, const float4* sh
 
 // The order of N times (two operand reads from LDS, three products): the reads
 // two steps ahead.  Left alone each step's reads wait behind the products of the
-// step before, and then for LDS: 200 cycles a step instead of 100.
+// step before, and then for LDS: about 200 cycles a step instead of 100.
 template <int N>
 __device__ __forceinline__ void interleave_reads() {
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
@@ -1901,12 +1904,19 @@ __device__ __forceinline__ void interleave_reads() {
     }
 }
 
-// Rows over waves, for more than 64 query rows of a KV head: a work-group takes
-// 128 rows, 32 a wave, and walks its range tile by tile.  Its waves load, scale,
-// split and lay out a tile in LDS as operands once for all of them, 8 keys and 8
-// values each (a group with powers of two of its own), two tiles in turn: the next
-// one is laid out, and the one after loaded, while this one is in the products, so
-// a tile takes one barrier.  Two work-groups a CU fill each other's waits.
+// A work-group takes 128 query rows of a KV head, 32 a wave, and walks its range
+// of keys tile by tile.  Its waves load, scale, split and lay out a tile in LDS as
+// operands once for all of them, 8 keys and 8 values each (a group with powers of
+// two of its own), two tiles in turn: the next one is laid out, and the one after
+// loaded, while this one is in the products, so a tile takes one barrier.  Waves
+// without rows (a call of fewer) stage for the others.  Two work-groups a CU fill
+// each other's waits.
+// Few rows: bound by the reads of the cache (1 node at 32749, 32 heads over 8 of
+// 128: 268 MB in a call of 60 us, 4.5 TB/s).  Many: by the matrix cores and the
+// work beside them (splitting the tile, the softmax), of which a SIMD has 50 and
+// 71 thousand cycles in 131 (128 nodes at 8192, 32 over 4 of 128: 75 us, 0.69
+// PFLOP/s of fp16 products; 512 nodes at 32000, 32 over 8: 0.88 to 0.93, a large
+// library product of the kind runs at 1.17).
 template <int HD, int OCC>
 __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) {
     constexpr int NC = HD / 16, NN = HD / 32;
@@ -2178,7 +2188,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
 }
 
 // out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the key
-// ranges c.  CG threads share a float4 of the output, each with every CG-th
+// ranges c.  Bound by the read of the parts: 128 nodes at 8192, 32 heads of 128 (15
+// ranges, 33 MB) 11.3 us, 2.9 TB/s; 4 nodes at 300 (10 ranges) 2.7 us.  CG threads share a float4 of the output, each with every CG-th
 // range, at most eight, whose loads go out at once; their sums meet in LDS.
 constexpr int kTreeMergeLoads = 8;
 template <int HD, int CG>
