@@ -3085,8 +3085,8 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
         set_error(where, "a tree has 1 to 512 nodes, and every parent is -1 or an earlier node", -1);
         return;
     }
-    if (has_norm_weight > 0 && !mmap_base) {
-        set_error(where, "no norm weights", -1);
+    if ((has_norm_weight > 0 || (has_rope_freqs && rope_base > 0.0f)) && !mmap_base) {
+        set_error(where, "no norm weights or rope factors", -1);
         return;
     }
     if (!ensure_runtime(where)) return;

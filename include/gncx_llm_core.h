@@ -457,8 +457,9 @@ void gncx_hip_argmax(const float* values, int32_t n, int32_t* out_index);
  * themselves).  out_nodes[i] is the attention of node i over the cached rows,
  * its ancestors and itself; with sliding_window > 0 over those of them within
  * that many positions up to its own.  What a node does not see has no part in
- * its output, whatever it holds.  head_dim is 64, 128 or 256; 16-byte aligned
- * pointers; out_nodes overlaps no other argument.  The first call of a (pos0,
+ * its output, whatever it holds.  head_dim is 64, 128 or 256, with at most 8192
+ * query heads to a KV head; pointers are 16-byte aligned, and no two of the
+ * vectors, caches and outputs overlap but as said.  The first call of a (pos0,
  * depth) waits for the stream to upload the rotations, so the call cannot be
  * captured into a graph (refused). */
 void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const float* v_nodes, float* k_cache_layer,

@@ -20,13 +20,13 @@ def refused(lib, text):
     assert text in lib.gncx_hip_last_error().decode()
 
 
-def tree(lib, parents, n=None, pos0=0, H=4, KV=2, hd=64, weight=-1):
+def tree(lib, parents, n=None, pos0=0, H=4, KV=2, hd=64, weight=-1, factors=0, base=0.0):
     p = None if parents is None else np.asarray(parents, np.int32)
     out = np.full(8, 7.0, np.float32)
     lib.gncx_hip_last_status()
     lib.gncx_hip_attention_tree(None, None, None, None, None, pos0, len(parents) if n is None else n,
                                 None if p is None else p.ctypes.data, H, KV, hd, 1.0, 0, None, 0, 0, weight, 1e-6, 0,
-                                0, 0.0, out.ctypes.data)
+                                factors, base, out.ctypes.data)
     assert (out == 7.0).all()
 
 
@@ -43,9 +43,12 @@ def test_tree_refuses_negative_and_missing(plib):
     refused(plib, "parents must be host memory")
     tree(plib, [-1], weight=1)
     refused(plib, "no norm weights")
+    tree(plib, [-1], factors=1, base=1e4)
+    refused(plib, "rope factors")
 
 
 @pytest.mark.parametrize("geo", [dict(H=3), dict(H=0), dict(KV=0), dict(hd=96), dict(hd=0), dict(pos0=-1),
+                                 dict(H=8193, KV=1),
                                  dict(pos0=2 ** 31 - 512)])
 def test_tree_refuses_geometry(plib, geo):
     tree(plib, [-1], **geo)

@@ -154,7 +154,8 @@ def test_tree_attention(lib, torch_mod, H, KV, hd, shape, n, pos0, sw):
     (32, 8, 128, "random", 512, 100, 0), (32, 8, 128, "chain", 512, 1000, 77), (16, 16, 64, "random", 400, 1001, 600),
     (32, 4, 128, "binary", 130, 4001, 0), (32, 8, 128, "random", 25, 20011, 0), (32, 8, 128, "chain", 4, 16383, 1000),
     (32, 1, 128, "random", 65, 9000, 0), (8, 2, 256, "random", 129, 3001, 0), (8, 8, 64, "roots", 511, 2, 1),
-    (2, 1, 64, "random", 100, 32000, 0), (12, 4, 128, "random", 300, 513, 0)])
+    (2, 1, 64, "random", 100, 32000, 0), (12, 4, 128, "random", 300, 513, 0), (8, 1, 128, "chain", 4, 30000, 0),
+    (4, 1, 64, "random", 40, 20000, 5000), (8, 2, 256, "random", 6, 12000, 0), (64, 1, 128, "binary", 3, 9001, 0)])
 def test_tree_attention_large(lib, torch_mod, H, KV, hd, shape, n, pos0, sw):
     Tree(torch_mod, H, KV, hd, pos0, make_parents(shape, n), sw, seed=n).verify(lib)
 
