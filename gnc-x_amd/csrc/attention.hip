@@ -1639,8 +1639,9 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, T
 // no say in its precision.
 // "Odd" keys, whose key or value row is not finite or lies more than 2^-14 below
 // its group's largest, are kept out of the products (0 times an infinity would be
-// NaN for the rows that do not see it) and added element by element at the end:
-// in real caches there are none.
+// NaN for the rows that do not see it) and added element by element at the end,
+// from lists that the staging leaves (128 nodes at 8192, 32 heads over 4 of 128: 92
+// us without odd keys, 128 with one in a hundred, 475 with one in eight).
 // Parts are left normalised, o_part = sum w v / sum w, with (m, l) beside them:
 // no sum of large values can overflow between the kernels.  The reference's
 // 1e-12 beside a sum l > 1/2 is below fp32's rounding and left out.
@@ -1810,41 +1811,50 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
     return alpha;
 }
 
-// Adds the odd keys of [t0, t0 + 8) (below c1) to a query row: to part, its
-// normalised output in LDS (float4 d / 4 at 33 (d / 4); the halves of a wave take
-// half of the columns each), and to its state.  The keys are found again by the
-// rule that kept them out of the products.  A weight of 0 takes nothing from a
-// row, whatever it holds.
+// The odd keys of [t0, t0 + 8) (below c1), by the rule that keeps them out of the
+// products, as a mask.
 template <int HD>
-__device__ void add_odd_keys(const TreeParams& p, const TreeShared& tree, const RowPlace& at, float* part, const float* q,
-                             const float* kbase, const float* vbase, uint32_t kn, int t0, int c1, int lane, RowState& s) {
+__device__ uint32_t odd_keys(const float* kbase, const float* vbase, uint32_t kn, int t0, int c1, int lane) {
     // lane = key (eight of them), over its row
     const bool in = lane % 8 + t0 < c1;
     float kmax = 0.0f, vmax = 0.0f;
     const size_t mine = static_cast<size_t>(min(t0 + lane % 8, c1 - 1)) * kn;
-    for (int d = 0; d < HD; ++d) {
-        kmax = maximum_of(kmax, fabsf(kbase[mine + d]));
-        vmax = maximum_of(vmax, fabsf(vbase[mine + d]));
+#pragma unroll 4
+    for (int d = 0; d < HD; d += 4) {
+        const floatx4 k = *reinterpret_cast<const floatx4*>(kbase + mine + d), v = *reinterpret_cast<const floatx4*>(vbase + mine + d);
+        kmax = max3_abs(max3_abs(kmax, k[0], k[1]), k[2], k[3]);
+        vmax = max3_abs(max3_abs(vmax, v[0], v[1]), v[2], v[3]);
     }
     const float ktop = wave_max(in && kmax < __builtin_inff() ? kmax : 0.0f);
     const float vtop = wave_max(in && vmax < __builtin_inff() ? vmax : 0.0f);
-    const uint64_t odd = __ballot(in && lane < 8 && (is_odd(kmax, ktop) || is_odd(vmax, vtop)));
-    for (int j = 0; j < 8; ++j) {
-        if (!(odd >> j & 1)) continue;
-        const float* k = kbase + static_cast<size_t>(t0 + j) * kn;
-        const float* v = vbase + static_cast<size_t>(t0 + j) * kn;
-        float x = 0.0f;
-        for (int d = 0; d < HD; ++d) x += q[d] * k[d];
-        x *= p.scale * 1.4426950408889634f;
-        if (!sees_key(p, tree, at, t0 + j, c1) || x == -__builtin_inff()) continue;
-        const float m2 = fmaxf(s.m, ceilf(x)), a = s.l * __builtin_amdgcn_exp2f(s.m - m2), w = __builtin_amdgcn_exp2f(x - m2);
-        s.m = m2;
-        s.l = a + w;
-        const float fa = a / s.l, fw = w / s.l;
-        for (int d = lane / 32 * (HD / 2); d < (lane / 32 + 1) * (HD / 2); ++d) {
-            float& o = part[d / 4 * 33 * 4 + d % 4];
-            o = (fa != 0.0f ? o * fa : 0.0f) + (fw != 0.0f ? fw * v[d] : 0.0f);
-        }
+    return static_cast<uint32_t>(__ballot(in && lane < 8 && (is_odd(kmax, ktop) || is_odd(vmax, vtop))));
+}
+
+// Adds a key to a query row, element by element: to part, its normalised output in
+// LDS (float4 d / 4 at 33 (d / 4); the halves of a wave, g, take half of the columns
+// each), and to its state.  A weight of 0 takes nothing from a row, whatever it holds.
+template <int HD>
+__device__ void add_odd_key(const TreeParams& p, const TreeShared& tree, const RowPlace& at, float4* part, const float* q,
+                            const float* k, const float* v, int key, int c1, int g, RowState& s) {
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int d = g * (HD / 2); d < (g + 1) * (HD / 2); d += 4) {
+        const floatx4 a = *reinterpret_cast<const floatx4*>(q + d), b = *reinterpret_cast<const floatx4*>(k + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[i] += a[i] * b[i];
+    }
+    const float x = across_halves((sum[0] + sum[1]) + (sum[2] + sum[3]), [](float a, float b) { return a + b; }) *
+                    (p.scale * 1.4426950408889634f);
+    if (!sees_key(p, tree, at, key, c1) || x == -__builtin_inff()) return;
+    const float m2 = fmaxf(s.m, ceilf(x)), a = s.l * __builtin_amdgcn_exp2f(s.m - m2), w = __builtin_amdgcn_exp2f(x - m2);
+    s.m = m2;
+    s.l = a + w;
+    const float fa = a / s.l, fw = w / s.l;
+    auto add = [&](float o, float e) { return (fa != 0.0f ? o * fa : 0.0f) + (fw != 0.0f ? fw * e : 0.0f); };
+#pragma unroll 4
+    for (int d = g * (HD / 8); d < (g + 1) * (HD / 8); ++d) {
+        const float4 o = part[33 * d], e = reinterpret_cast<const float4*>(v)[d];
+        part[33 * d] = make_float4(add(o.x, e.x), add(o.y, e.y), add(o.z, e.z), add(o.w, e.w));
     }
 }
 
@@ -1892,8 +1902,8 @@ __device__ __forceinline__ void store_rows(const TreeParams& p, const float4* sh
 }
 
 // The order of N times (two operand reads from LDS, three products): the reads
-// two steps ahead.  Left alone each step's reads wait behind the products of the
-// step before, and then for LDS: about 200 cycles a step instead of 100.
+// ahead of the products before.  Left alone they come behind those, and are then
+// waited for (512 nodes at 32000, 32 heads over 8 of 128: 886 us instead of 861).
 template <int N>
 __device__ __forceinline__ void interleave_reads() {
     __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
@@ -1928,7 +1938,11 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
     __shared__ __align__(16) float kfac[2][kWaves], vexp[2][kWaves];  // [tile in turn][group]: the keys' factor, the values' exponent
     __shared__ __align__(16) uint32_t oddmask[2][kWaves];             // [tile in turn][group]: odd keys, from bit 8 group on
     __shared__ float2 mls[kWaves][32];
-    __shared__ int odd_first, odd_last;
+    // groups with odd keys, by the wave that staged them: tile of the range << 8 |
+    // mask; the first tile whose group found no place
+    constexpr int kOddGroups = 64;
+    __shared__ uint32_t odd_group[kWaves][kOddGroups];
+    __shared__ int odd_count[kWaves], odd_more[kWaves];
     __shared__ TreeShared tree;
     half8_t* const khi = reinterpret_cast<half8_t*>(shared);  // [tile in turn][slice][lane]
     half8_t* const klo = khi + 2 * kTile;
@@ -2056,8 +2070,13 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             vexp[b][wv] = static_cast<float>(vf - 127);
             oddmask[b][wv] = odd << (8 * wv);
             if (odd) {
-                atomicMin(&odd_first, t0 + 8 * wv);
-                atomicMax(&odd_last, t0 + 8 * wv);
+                const int n = odd_count[wv];
+                if (n < kOddGroups) {
+                    odd_group[wv][n] = static_cast<uint32_t>(t0 - c0) / kTreeKeys << 8 | odd;
+                    odd_count[wv] = n + 1;
+                } else {
+                    odd_more[wv] = min(odd_more[wv], t0);
+                }
             }
         }
         // slice wv / 2, elements 4 (wv % 2) ..
@@ -2072,9 +2091,9 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
     };
 
     prefetch(c0);
-    if (tid == 0) {
-        odd_first = c1;
-        odd_last = -1;
+    if (tid < kWaves) {
+        odd_count[tid] = 0;
+        odd_more[tid] = c1;
     }
     if (c1 > p.pos0) load_tree(p, tree);
     // this wave's query rows as operands, in registers
@@ -2160,7 +2179,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         __builtin_amdgcn_sched_barrier(0);
     };
 
-    __syncthreads();  // odd_first / odd_last, the tree
+    __syncthreads();  // no odd keys yet, the tree
     stage(0, c0);
     if (c0 + kTreeKeys < c1) prefetch(c0 + kTreeKeys);
     __syncthreads();
@@ -2176,11 +2195,23 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
 
     float4* const part = shared + wv * kPart;
     store_part<NN>(part, o, s, li, g);
-    if (mine && odd_last >= 0) {
+    if (mine && (odd_count[0] | odd_count[1] | odd_count[2] | odd_count[3])) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own writes
         asm volatile("" ::: "memory");
-        for (int t0 = odd_first; t0 <= odd_last; t0 += 8)
-            add_odd_keys<HD>(p, tree, place, reinterpret_cast<float*>(part + li), qrow, kbase, vbase, kn, t0, c1, lane, s);
+        auto add = [&](int t0, uint32_t odd) {
+            for (odd = __builtin_amdgcn_readfirstlane(odd); odd; odd &= odd - 1) {
+                const int key = t0 + __builtin_ctz(odd);
+                const size_t row = static_cast<size_t>(key) * kn;
+                add_odd_key<HD>(p, tree, place, part + li, qrow, kbase + row, vbase + row, key, c1, g, s);
+            }
+        };
+        for (int w = 0; w < kWaves; ++w) {
+            for (int i = 0; i < odd_count[w]; ++i)
+                add(__builtin_amdgcn_readfirstlane(c0 + static_cast<int>(odd_group[w][i] >> 8) * kTreeKeys + 8 * w),
+                    odd_group[w][i] & 0xffu);
+            for (int t0 = __builtin_amdgcn_readfirstlane(odd_more[w]); t0 < c1; t0 += kTreeKeys)
+                if (t0 + 8 * w < c1) add(t0 + 8 * w, odd_keys<HD>(kbase, vbase, kn, t0 + 8 * w, c1, lane));
+        }
     }
     if (g == 0) mls[wv][li] = make_float2(s.m, s.l);
     __syncthreads();

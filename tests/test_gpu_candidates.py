@@ -312,6 +312,19 @@ def test_tree_neighbours_of_other_sizes(lib, torch_mod, hd, n, pos0):
     t.verify(lib)
 
 
+@pytest.mark.parametrize("H,KV,hd,n,pos0", [(16, 16, 64, 400, 20000), (8, 8, 128, 20, 5000), (4, 1, 256, 3, 3000)])
+def test_tree_many_rows_of_other_sizes(lib, torch_mod, H, KV, hd, n, pos0):
+    """One row in eight far below its neighbours, over ranges of many tiles, and a
+    few of them infinite where a window hides them."""
+    torch = torch_mod
+    t = Tree(torch, H, KV, hd, pos0, make_parents("random", n), sw=pos0 - 100, seed=n)
+    t.vc[3:pos0:8] *= 1e-9
+    t.kc[2:pos0:41] *= 1e-9
+    t.vc[0] = float("inf")
+    t.kc[1] = float("nan")
+    t.verify(lib)
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 @pytest.mark.parametrize("n", [6, 12, 40])
 def test_tree_small_keys_beside_larger_ones(lib, torch_mod, hd, n):
