@@ -1563,14 +1563,18 @@ struct TreeParams {
 // A launch of its own (4 nodes, 40 heads of 128: 3.7 us; 128 nodes, 36 heads: 4.9):
 // done by the next kernel's work-groups, its rotations and norms are on the way of
 // each of them, 3.7 + 8.3 us against 14.2 (4 nodes at 300).
-template <int HD>
-__global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, TreeTable tree) {
+template <int N>
+struct TreeRows {
+    uint16_t pre[N], end[N], depth[N];
+};
+template <int HD, int N>
+__global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, TreeRows<N> tree) {
 #pragma clang fp contract(off)
     constexpr int H = HD / 2, NR = (H + 63) / 64;
     __shared__ __align__(16) float xs[kWaves][HD];
     const int t = blockIdx.x, lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-    // the 3 KB of the table travel once, in this launch's arguments (a launch takes
-    // the host 1.3 us longer for them), and stay in memory for the next kernel
+    // the table travels once, in this launch's arguments, and stays in memory for the
+    // next kernel
     if (blockIdx.x == 0 && blockIdx.y == 0)
         for (int i = threadIdx.x; i < p.n; i += kThreads) {
             p.interval[i] = tree.pre[i] | static_cast<uint32_t>(tree.end[i]) << 16;
@@ -2316,7 +2320,19 @@ TreePlan tree_plan(const TreeArgs& a) {
 template <int HD, int OCC>
 hipError_t launch_tree(const TreeParams& p, const TreeTable& tree, const TreePlan& pl, hipStream_t stream) {
     const int heads = p.n_heads + p.n_kv;
-    hipLaunchKernelGGL(tree_prologue_kernel<HD>, dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p, tree);
+    auto prologue = [&](auto rows) {
+        constexpr int N = sizeof(rows) / 6;
+        for (int32_t i = 0; i < p.n; ++i) {
+            rows.pre[i] = tree.pre[i];
+            rows.end[i] = tree.end[i];
+            rows.depth[i] = tree.depth[i];
+        }
+        hipLaunchKernelGGL((tree_prologue_kernel<HD, N>), dim3(p.n, (heads + kWaves - 1) / kWaves), dim3(kThreads), 0, stream, p,
+                           rows);
+    };
+    // (a launch takes the host 1.3 us longer for 3 KB of arguments)
+    if (p.n <= 64) prologue(TreeRows<64>{});
+    else prologue(TreeRows<kMaxTreeNodes>{});
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((tree_rows_kernel<HD, OCC>), dim3(p.n_kv, pl.groups, pl.chunks), dim3(kThreads), 0, stream, p);
