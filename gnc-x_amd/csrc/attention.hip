@@ -1735,15 +1735,27 @@ __device__ __forceinline__ bool is_odd(float row, float top) {
     return !(row < __builtin_inff()) || (row > 0.0f && row < top * kOddBelow);
 }
 
-// The tree's part in a kernel's LDS and a query row's place in it.
+// The keys of a range from its first tile with a node on, to the end of its last
+// tile, in LDS: a row (pre, lo) sees key t0 + i when pre - first < count (in its
+// subtree's interval, first | count << 16; a cached row's is everything, a row's
+// behind the range nothing) and, with a window, place >= lo.
 struct TreeShared {
-    uint32_t interval[kMaxTreeNodes];  // pre | end << 16
-    uint16_t depth[kMaxTreeNodes];
+    static constexpr int kMost = kMaxTreeNodes + 2 * kTreeKeys;
+    __align__(16) uint32_t interval[kMost];
+    __align__(16) int32_t place[kMost];  // position
 };
-__device__ __forceinline__ void load_tree(const TreeParams& p, TreeShared& t) {
-    for (int i = threadIdx.x; i < p.n; i += kThreads) {
-        t.interval[i] = p.interval[i];
-        t.depth[i] = p.depth[i];
+__device__ __forceinline__ void load_tree(const TreeParams& p, TreeShared& t, int t0, int c1) {
+    for (int i = threadIdx.x; i < (c1 - t0 + kTreeKeys - 1) / kTreeKeys * kTreeKeys; i += kThreads) {
+        const int key = t0 + i, node = key - p.pos0;
+        uint32_t iv = node < 0 ? 0xffffu << 16 : 0;
+        int place = key;
+        if (node >= 0 && key < c1) {
+            iv = p.interval[node];
+            iv -= iv << 16;  // (the end less the first)
+            place = p.pos0 + p.depth[node];
+        }
+        t.interval[i] = iv;
+        t.place[i] = place;
     }
 }
 struct RowPlace {
@@ -1753,14 +1765,10 @@ struct RowPlace {
 __device__ __forceinline__ RowPlace place_of(const TreeParams& p, int node) {
     return {p.interval[node] & 0xffffu, p.sw > 0 ? max(0, p.pos0 + p.depth[node] - p.sw + 1) : 0};
 }
-// whether a query row sees a key of a range that ends at c1
-__device__ __forceinline__ bool sees_key(const TreeParams& p, const TreeShared& t, const RowPlace& at, int key, int c1) {
-    bool see = key < p.pos0 && key >= at.lo;
-    if (key >= p.pos0 && key < c1) {
-        const uint32_t iv = t.interval[key - p.pos0];
-        see = (iv & 0xffffu) <= at.pre && at.pre < iv >> 16 && p.pos0 + t.depth[key - p.pos0] >= at.lo;
-    }
-    return see && key < c1;
+__device__ __forceinline__ bool in_interval(uint32_t iv, uint32_t pre) { return pre - (iv & 0xffffu) < iv >> 16; }
+// whether a query row sees a key, of the tree's part from t0 on
+__device__ __forceinline__ bool sees_key(const TreeShared& t, int t0, const RowPlace& at, int key) {
+    return key < t0 ? key >= at.lo : in_interval(t.interval[key - t0], at.pre) && t.place[key - t0] >= at.lo;
 }
 
 // One query row a lane: its running maxima of s and of s + e, and its sum.  The
@@ -1838,8 +1846,8 @@ __device__ uint32_t odd_keys(const float* kbase, const float* vbase, uint32_t kn
 // LDS (float4 d / 4 at 33 (d / 4); the halves of a wave, g, take half of the columns
 // each), and to its state.  A weight of 0 takes nothing from a row, whatever it holds.
 template <int HD>
-__device__ void add_odd_key(const TreeParams& p, const TreeShared& tree, const RowPlace& at, float4* part, const float* q,
-                            const float* k, const float* v, int key, int c1, int g, RowState& s) {
+__device__ void add_odd_key(const TreeParams& p, const TreeShared& tree, int tree0, const RowPlace& at, float4* part,
+                            const float* q, const float* k, const float* v, int key, int g, RowState& s) {
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
     for (int d = g * (HD / 2); d < (g + 1) * (HD / 2); d += 4) {
@@ -1849,7 +1857,7 @@ __device__ void add_odd_key(const TreeParams& p, const TreeShared& tree, const R
     }
     const float x = across_halves((sum[0] + sum[1]) + (sum[2] + sum[3]), [](float a, float b) { return a + b; }) *
                     (p.scale * 1.4426950408889634f);
-    if (!sees_key(p, tree, at, key, c1) || x == -__builtin_inff()) return;
+    if (!sees_key(tree, tree0, at, key) || x == -__builtin_inff()) return;
     const float m2 = fmaxf(s.m, ceilf(x)), a = s.l * __builtin_amdgcn_exp2f(s.m - m2), w = __builtin_amdgcn_exp2f(x - m2);
     s.m = m2;
     s.l = a + w;
@@ -2099,7 +2107,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         odd_count[tid] = 0;
         odd_more[tid] = c1;
     }
-    if (c1 > p.pos0) load_tree(p, tree);
+    const int tree0 = c0 + max(p.pos0 - c0, 0) / kTreeKeys * kTreeKeys;  // (behind the range: no node in it)
+    if (c1 > p.pos0) load_tree(p, tree, tree0, c1);
     // this wave's query rows as operands, in registers
     const int myrow = min(row0 + 32 * wv + li, rows - 1);
     const float* const qrow = p.q + (static_cast<size_t>(myrow / G) * p.n_heads + hk * G + myrow % G) * HD;
@@ -2156,12 +2165,29 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         const float ve[4] = {vx[0], vx[1], vx[2], vx[3]}, sf[4] = {kf[0] * qf, kf[1] * qf, kf[2] * qf, kf[3] * qf};
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[r] *= sf[r >> 2];
-        if (t0 + kTreeKeys > min(p.pos0, c1) || t0 < lo_most || odd)
+        const float hidden = -__builtin_inff();
+        if (t0 + kTreeKeys > p.pos0) {
+            typedef int32_t int32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int j = 8 * (r >> 2) + 4 * g + (r & 3);
-                if (!sees_key(p, tree, place, t0 + j, c1) || (odd >> j & 1)) st[r] = -__builtin_inff();
+            for (int a = 0; a < 4; ++a) {
+                const int at = t0 - tree0 + 8 * a + 4 * g;
+                const uint32x4 iv = *reinterpret_cast<const uint32x4*>(tree.interval + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) st[4 * a + i] = in_interval(iv[i], place.pre) ? st[4 * a + i] : hidden;
+                if (p.sw > 0) {
+                    const int32x4 x = *reinterpret_cast<const int32x4*>(tree.place + at);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) st[4 * a + i] = x[i] >= place.lo ? st[4 * a + i] : hidden;
+                }
             }
+        } else if (t0 < lo_most) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) st[r] = t0 + 8 * (r >> 2) + 4 * g + (r & 3) >= place.lo ? st[r] : hidden;
+        }
+        if (odd)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (odd >> (8 * (r >> 2) + 4 * g + (r & 3)) & 1) st[r] = hidden;
         half8_t ph[2], pl[2];
         const float alpha = tile_softmax(st, ve, s, ph, pl);
         if (__ballot(alpha != 1.0f))
@@ -2187,13 +2213,14 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
     stage(0, c0);
     if (c0 + kTreeKeys < c1) prefetch(c0 + kTreeKeys);
     __syncthreads();
-    // (a wave whose 32 rows are none stages for the others)
+    // (a wave whose 32 rows are none, or see no later node, stages for the others)
     const bool mine = row0 + 32 * wv < rows;
+    const int last = mine ? p.pos0 + min(row0 + 32 * wv + 31, rows - 1) / G : -1;
     int b = 0;
     for (int t0 = c0; t0 < c1; t0 += kTreeKeys, b ^= 1) {
         if (t0 + kTreeKeys < c1) stage(b ^ 1, t0 + kTreeKeys);
         if (t0 + 2 * kTreeKeys < c1) prefetch(t0 + 2 * kTreeKeys);
-        if (mine) take_tile(b, t0);
+        if (t0 <= last) take_tile(b, t0);
         __syncthreads();  // the next tile is laid out, and this one done with
     }
 
@@ -2206,7 +2233,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
             for (odd = __builtin_amdgcn_readfirstlane(odd); odd; odd &= odd - 1) {
                 const int key = t0 + __builtin_ctz(odd);
                 const size_t row = static_cast<size_t>(key) * kn;
-                add_odd_key<HD>(p, tree, place, part + li, qrow, kbase + row, vbase + row, key, c1, g, s);
+                add_odd_key<HD>(p, tree, tree0, place, part + li, qrow, kbase + row, vbase + row, key, g, s);
             }
         };
         for (int w = 0; w < kWaves; ++w) {
