@@ -1529,8 +1529,9 @@ hipError_t launch_attention(const AttnArgs& a, void* workspace, size_t workspace
 //
 // The tree's mask is an interval test.  With the nodes numbered in preorder,
 // the subtree of a is the interval [pre_a, end_a), so a is i or an ancestor of
-// i exactly when pre_a <= pre_i < end_a: two compares instead of a T x T mask,
-// and 6 bytes a node, which travel in the first launch's arguments.
+// i exactly when pre_a <= pre_i < end_a, pre_i - pre_a < end_a - pre_a without a
+// sign: one compare instead of a T x T mask, and 6 bytes a node, which travel in
+// the first launch's arguments.
 namespace {
 
 struct TreeParams {
