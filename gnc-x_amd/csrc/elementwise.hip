@@ -1062,12 +1062,15 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
     };
     const int n = held;
     if (n <= kMostRanked) {
-        for (int i = tid; i < n; i += kJoinThreads) {
+        // eight threads a candidate
+        for (int i = tid / 8; i < n; i += kJoinThreads / 8) {
             const Candidate c = ranked[i];
             int rank = 0;
 #pragma unroll 4
-            for (int o = 0; o < n; ++o) rank += ranked[o].before(c);
-            if (rank < p.n_out) write(rank, c);
+            for (int o = tid % 8; o < n; o += 8) rank += ranked[o].before(c);
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) rank += __shfl_xor(rank, d, 8);
+            if (tid % 8 == 0 && rank < p.n_out) write(rank, c);
         }
         for (int i = n + tid; i < p.n_out; i += kJoinThreads) write_none(i);
         return;
