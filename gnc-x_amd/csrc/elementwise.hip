@@ -698,14 +698,14 @@ struct LayerCaches {
 // another's column, so the move is in place without a barrier.  Rows that stay
 // (rows[i] == i, the first ones only) are left out by the caller.
 // Bound by memory, a round of loads and stores after the other: 400 of 512 rows of
-// 1024 in 72 caches (118 MB read and written) 72 us with 16 at once, 53 (4.4 TB/s)
-// with 64; 4 of 16 rows 4.2.  The rows are read as one vector: each of sixteen
-// scalar loads from the arguments, in host memory, was waited for.
+// 1024 in 72 caches (118 MB read and written) 72 us with 16 at once, 50 (4.7 TB/s)
+// with 64; 4 of 16 rows 4.2.  The rows are read as one vector, a round ahead: each
+// of sixteen scalar loads from the arguments, in host memory, was waited for.
 struct KeepParams {
     LayerCaches caches;
     int32_t kv_dim, n;
     size_t row0;
-    uint16_t rows[kMaxKeepRows];
+    uint16_t rows[kMaxKeepRows];  // 0 past n
 };
 
 template <int W, int kAtOnce>
@@ -714,9 +714,11 @@ __global__ __launch_bounds__(64) void keep_rows_kernel(KeepParams p) {
     const int lane = threadIdx.x, d = W * static_cast<int>(blockIdx.x * 64 + lane);
     const bool in = d < p.kv_dim;
     float* c = p.caches.c[blockIdx.y] + p.row0 * p.kv_dim + (in ? d : 0);
+    // lane u: where row i + u comes from (past the end row 0, read for nothing)
+    int next = p.rows[lane % kAtOnce];
     for (int i = 0; i < p.n; i += kAtOnce) {
-        // lane u: where row i + u comes from (past the end: the last row again)
-        const int from = p.rows[min(i + lane % kAtOnce, p.n - 1)];
+        const int from = next;
+        next = p.rows[min(i + kAtOnce + lane % kAtOnce, kMaxKeepRows - 1)];
         vec v[kAtOnce];
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u)
@@ -1141,7 +1143,7 @@ hipError_t launch_kv_keep_rows(float* const* k, float* const* v, int32_t n_layer
     return by_layers(k, v, n_layers, [&](const LayerCaches& c, int32_t caches) {
         p.caches = c;
         const dim3 grid((kv_dim + per - 1) / per, caches);
-        // (a call of few rows would read the last one again 48 times)
+        // (a call of few rows would read 48 for nothing)
         if (p.n <= 16 && narrow) hipLaunchKernelGGL((keep_rows_kernel<1, 16>), grid, dim3(64), 0, stream, p);
         else if (narrow) hipLaunchKernelGGL((keep_rows_kernel<1, 64>), grid, dim3(64), 0, stream, p);
         else if (p.n <= 16) hipLaunchKernelGGL((keep_rows_kernel<4, 16>), grid, dim3(64), 0, stream, p);
