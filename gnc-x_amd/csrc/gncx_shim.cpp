@@ -1780,11 +1780,15 @@ void fetch_embedding(int32_t type, const uint8_t* base, size_t off, int32_t toke
     const size_t rb = row_bytes(type, dim);
     const uint8_t* row = base + off + static_cast<size_t>(token) * rb;
     const uint8_t* drow;
-    // a registered (or device-resident) table is read in place; otherwise only the row travels
+    // A device-resident table, or the copy of one in a read-only mapping, is read
+    // in place; otherwise only the row travels: a copy kept under the table's
+    // address may be of what stood there before (an array freed since, a table
+    // rewritten since), and without the table's size it cannot be compared.
     auto it = g_rt.weights.find(reinterpret_cast<uintptr_t>(base + off));
     if (is_device_ptr(row)) {
         drow = row;
-    } else if (it != g_rt.weights.end() && (static_cast<size_t>(token) + 1) * rb <= it->second.bytes) {
+    } else if (it != g_rt.weights.end() && it->second.trust == kMapped &&
+               (static_cast<size_t>(token) + 1) * rb <= it->second.bytes) {
         drow = it->second.d + static_cast<size_t>(token) * rb;
     } else {
         if (!g_rt.aux.ensure(round_up(rb, 16), where)) return;

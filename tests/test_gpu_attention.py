@@ -540,3 +540,77 @@ def test_argmax_first_of_equal_maxima(lib, n):
         gncx.check(lib)
         want = int(torch.argmax(torch.nan_to_num(c, nan=float("-inf"))).item())
         assert int(out.item()) == want, (n, int(out.item()), want)
+
+
+@pytest.mark.parametrize("kind", ["array", "ram"])
+@pytest.mark.parametrize("name,t", [("q8_0", 8), ("q6_k", 14), ("bf16", 30)])
+def test_embedding_rows_of_memory_that_was_copied_as_something_else(lib, golden, oracle, name, t, kind):
+    """A row is decoded from what its address holds now: norm weights copied to
+    the device from the same address, and a table rewritten in place since it
+    was copied, have no part in it."""
+    tab, dim = golden[f"emb_{name}_tab"], 512
+    rb = gncx.row_bytes(t, dim)
+    vocab = tab.nbytes // rb
+    fetch = {8: lib.gncx_fetch_token_embedding_q8_0, 14: lib.gncx_fetch_token_embedding_q6_k,
+             30: lib.gncx_fetch_token_embedding_bf16}[t]
+    size, h = 16384, None  # of 4096 norm weights: more than any of the tables
+    if kind == "ram":
+        h = lib.gncx_ram_alloc(size)
+        mem = np.ctypeslib.as_array((C.c_uint8 * size).from_address(lib.gncx_ram_get_ptr(h)))
+    else:
+        mem = np.zeros(size, np.uint8)
+    try:
+        gamma, x, y = synth.make_norm_gamma(4096, 7), np.ones(4096, np.float32), np.zeros(4096, np.float32)
+        mem[:] = gamma.view(np.uint8)
+        lib.gncx_rmsnorm_and_encode_4phase(ptr(x), ptr(mem), 0, 4096, 1e-6, 0, ptr(y), None, None)
+        gncx.check(lib)
+        mem[:tab.nbytes] = tab
+
+        def row(i):
+            e = np.zeros(dim, np.float32)
+            fetch(ptr(mem), 0, i, dim, 1.0, ptr(e))
+            gncx.check(lib)
+            return e
+
+        assert np.array_equal(row(5), golden[f"emb_{name}_y5"])
+        # the whole table copied as one, then a row rewritten
+        ids, out = np.arange(vocab, dtype=np.int32), np.zeros((vocab, dim), np.float32)
+        lib.gncx_hip_fetch_token_embeddings(t, ptr(mem), 0, ptr(ids), vocab, vocab, dim, 1.0, ptr(out))
+        gncx.check(lib)
+        for i in range(vocab):
+            assert np.array_equal(row(i), out[i]), i
+        mem[5 * rb:6 * rb] = tab[3 * rb:4 * rb]
+        assert np.array_equal(row(5), out[3])
+        assert np.array_equal(row(4), out[4]) and np.array_equal(row(6), out[6])
+    finally:
+        lib.gncx_hip_weight_forget(None)
+        if h:
+            lib.gncx_ram_free(h)
+
+
+@pytest.mark.parametrize("name,t", [("q8_0", 8), ("q6_k", 14), ("bf16", 30)])
+def test_embedding_rows_of_a_mapped_table(lib, golden, tmp_path, name, t):
+    """Rows of a table in a mapped file, before and after the library has copied
+    the table."""
+    tab, dim = golden[f"emb_{name}_tab"], 512
+    vocab = tab.nbytes // gncx.row_bytes(t, dim)
+    fetch = {8: lib.gncx_fetch_token_embedding_q8_0, 14: lib.gncx_fetch_token_embedding_q6_k,
+             30: lib.gncx_fetch_token_embedding_bf16}[t]
+    f = tmp_path / "table.bin"
+    f.write_bytes(bytes(64) + tab.tobytes())
+    n = C.c_size_t()
+    h = lib.gncx_gla_map_readonly(str(f).encode(), C.addressof(n))
+    try:
+        base = lib.gncx_gla_get_base_ptr(h)
+        e = np.zeros(dim, np.float32)
+        for _ in range(2):
+            fetch(base, 64, 5, dim, 1.0, ptr(e))
+            gncx.check(lib)
+            assert np.array_equal(e, golden[f"emb_{name}_y5"])
+            fetch(base, 64, 11, dim, 0.37, ptr(e))
+            assert np.array_equal(e, golden[f"emb_{name}_y11s"])
+            ids, out = np.arange(vocab, dtype=np.int32), np.zeros((vocab, dim), np.float32)
+            lib.gncx_hip_fetch_token_embeddings(t, base, 64, ptr(ids), vocab, vocab, dim, 1.0, ptr(out))
+            gncx.check(lib)
+    finally:
+        lib.gncx_gla_unmap(h)
