@@ -1795,11 +1795,13 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
     const auto larger = [](float a, float b) { return fmaxf(a, b); };
     const float m2 = fmaxf(s.m, ceilf(across_halves(mx, larger)));
     const float mt2 = fmaxf(s.mt, ceilf(across_halves(mxt, larger)));
-    // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), the second capped: it
-    // passes 2^126 only where the first is 0
-    float f[4], sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), at most 2^14; the second
+    // may pass the largest float where the first is small, so its exponent is added
+    // (the bounds are beyond any sum of two: a weight is 0 there either way)
+    int f[4];
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int h = 0; h < 4; ++h) f[h] = __builtin_amdgcn_exp2f(fminf(m2 - mt2 + ve[h] + 14.0f, 126.0f));
+    for (int h = 0; h < 4; ++h) f[h] = static_cast<int>(__builtin_amdgcn_fmed3f(m2 - mt2 + ve[h] + 14.0f, -512.0f, 512.0f));
     half4_t hi[4], lo[4];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -1808,8 +1810,9 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
         for (int i = 0; i < 4; ++i) {
             e[i] = __builtin_amdgcn_exp2f(st[4 * a + i] - m2);
             sum[i] += e[i];
+            e[i] = __builtin_ldexpf(e[i], f[a]);
         }
-        pairs<true>(e, f[a], hi[a], lo[a]);
+        pairs<false>(e, 1.0f, hi[a], lo[a]);
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c) {

@@ -339,6 +339,21 @@ def test_tree_small_keys_beside_larger_ones(lib, torch_mod, hd, n):
     t.verify(lib)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("below,value", [(100, 1e33), (115, 3e36), (120, 3e36), (124, 1e38)])
+def test_tree_large_value_of_a_small_weight(lib, torch_mod, hd, below, value):
+    """A value row far above the others, under a weight of 2^-below: together
+    they are most of the output."""
+    torch = torch_mod
+    t = Tree(torch, 8, 2, hd, 120, [-1, 0, 0], seed=hd)
+    for c in (t.q, t.k, t.kc):
+        c.zero_()
+    t.q[:, ::hd] = 16.0
+    t.kc[50, ::hd] = -below * math.log(2.0) / (16.0 * t.scale)
+    t.vc[50] *= value
+    t.verify(lib)
+
+
 def test_tree_is_a_prefill_for_a_chain(lib, torch_mod):
     torch = torch_mod
     H, KV, hd, pos0, n = 32, 8, 128, 300, 40
