@@ -1772,36 +1772,36 @@ __device__ __forceinline__ bool sees_key(const TreeShared& t, int t0, const RowP
     return key < t0 ? key >= at.lo : in_interval(t.interval[key - t0], at.pre) && t.place[key - t0] >= at.lo;
 }
 
-// One query row a lane: its running maxima of s and of s + e, and its sum.  The
-// maxima are rounded up to whole numbers, so that every factor that brings parts
-// to another maximum is a power of two and rounds nothing.
+// One query row a lane: its running maxima of s (m) and of s + e (m + d), and its
+// sum.  The maxima are rounded up to whole numbers, so that every factor that brings
+// parts to another maximum is a power of two and rounds nothing; the second is kept
+// by its distance, as scores of 2^24 and more hold no e.
 struct RowState {
-    float m, mt, l;
+    float m, d, l;
 };
 // The softmax of a tile's scores st, registers 4 h .. of group h with the values'
 // exponent ve[h].  Leaves the weights as pairs and returns what O
 // so far is to be multiplied with (1: nothing).
 __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&ve)[4], RowState& s, half8_t (&ph)[2],
                                               half8_t (&pl)[2]) {
-    float mx = -1e30f, mxt = -1e30f;
+    float x[4] = {-1e30f, -1e30f, -1e30f, -1e30f};  // (a group without a visible key has no say)
 #pragma unroll
-    for (int h = 0; h < 4; ++h) {
-        float x = -1e30f;
+    for (int h = 0; h < 4; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x = fmaxf(x, st[4 * h + i]);
-        mx = fmaxf(mx, x);
-        mxt = fmaxf(mxt, x + ve[h]);  // (a group without a visible key, x -1e30, has no say)
-    }
+        for (int i = 0; i < 4; ++i) x[h] = fmaxf(x[h], st[4 * h + i]);
     const auto larger = [](float a, float b) { return fmaxf(a, b); };
-    const float m2 = fmaxf(s.m, ceilf(across_halves(mx, larger)));
-    const float mt2 = fmaxf(s.mt, ceilf(across_halves(mxt, larger)));
-    // 2^(s + e - mt + 14) = 2^(s - m) 2^(m + e - mt + 14), at most 2^14; the second
-    // may pass the largest float where the first is small, so its exponent is added
-    // (the bounds are beyond any sum of two: a weight is 0 there either way)
+    const float m2 = fmaxf(s.m, ceilf(across_halves(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), larger)));
+    float mxt = -1e30f;
+#pragma unroll
+    for (int h = 0; h < 4; ++h) mxt = fmaxf(mxt, x[h] - m2 + ve[h]);
+    const float d1 = s.d + (s.m - m2), d2 = fmaxf(d1, ceilf(across_halves(mxt, larger)));
+    // 2^(s + e - m - d + 14) = 2^(s - m) 2^(e - d + 14), at most 2^14; the second may
+    // pass the largest float where the first is small, so its exponent is added (the
+    // bounds are beyond any sum of two: a weight is 0 there either way)
     int f[4];
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int h = 0; h < 4; ++h) f[h] = static_cast<int>(__builtin_amdgcn_fmed3f(m2 - mt2 + ve[h] + 14.0f, -512.0f, 512.0f));
+    for (int h = 0; h < 4; ++h) f[h] = static_cast<int>(__builtin_amdgcn_fmed3f(ve[h] - d2 + 14.0f, -512.0f, 512.0f));
     half4_t hi[4], lo[4];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -1821,9 +1821,9 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
     }
     s.l = s.l * __builtin_amdgcn_exp2f(s.m - m2) +
           across_halves((sum[0] + sum[1]) + (sum[2] + sum[3]), [](float a, float b) { return a + b; });
-    const float alpha = __builtin_amdgcn_exp2f(s.mt - mt2);
+    const float alpha = __builtin_amdgcn_exp2f(d1 - d2);
     s.m = m2;
-    s.mt = mt2;
+    s.d = d2;
     return alpha;
 }
 
@@ -1877,7 +1877,7 @@ __device__ void add_odd_key(const TreeParams& p, const TreeShared& tree, int tre
 // the wave's normalised part to LDS: float4 column d4 of row li at 33 d4 + li
 template <int NN>
 __device__ __forceinline__ void store_part(float4* part, const floatx16 (&o)[NN], const RowState& s, int li, int g) {
-    const float f = s.l != 0.0f ? __builtin_amdgcn_exp2f(s.mt - s.m - 14.0f) / s.l : 0.0f;
+    const float f = s.l != 0.0f ? __builtin_amdgcn_exp2f(s.d - 14.0f) / s.l : 0.0f;
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
@@ -2141,7 +2141,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
     // of 128, 256 nodes at 4096: 97 -> 89)
     if ((blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z)) / 256 & 1) __builtin_amdgcn_s_setprio(1);
 
-    RowState s{-1e30f, -1e30f, 0.0f};
+    RowState s{-1e30f, 0.0f, 0.0f};
     floatx16 o[NN];
 #pragma unroll
     for (int n = 0; n < NN; ++n)

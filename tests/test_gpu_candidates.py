@@ -354,6 +354,34 @@ def test_tree_large_value_of_a_small_weight(lib, torch_mod, hd, below, value):
     t.verify(lib)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("size", [1e-8, 1.0, 1e9])
+@pytest.mark.parametrize("exponent", [12, 14, 20])
+def test_tree_scores_of_any_size(lib, torch_mod, hd, size, exponent):
+    """Scores so far apart that one key has all the weight, and so large that
+    32 bits hold no fraction of them: the output is that key's value row.  (Its
+    elements are kept to 2^-22 of themselves or 2^-25 of the row's largest, and
+    the sum of weights is 1.)"""
+    torch = torch_mod
+    H, KV, n, pos0 = 8, 2, 5, 140
+    t = Tree(torch, H, KV, hd, pos0, [-1] * n, seed=hd)
+    for c in (t.q, t.k, t.kc):
+        c.zero_()
+    # scores j 2^(2 exponent - 7) scale, in a random order of j, the nodes' own 0
+    t.q[:, ::hd] = 2.0 ** exponent
+    order = torch.from_numpy(np.random.default_rng(exponent).permutation(pos0)).cuda()
+    for h in range(KV):
+        t.kc[:pos0, h * hd] = (order + 1 + h) % (pos0 + 1) * 2.0 ** (exponent - 7)
+    t.v *= size
+    t.vc *= size
+    t.call(lib)
+    for h in range(H):
+        kv = h // (H // KV)
+        want = t.vc[int(t.kc[:pos0, kv * hd].argmax()), kv * hd:(kv + 1) * hd].double()
+        off = (t.out[:, h * hd:(h + 1) * hd].double() - want).abs()
+        assert bool((off <= 2.0 ** -21 * want.abs() + 2.0 ** -24 * want.abs().max()).all()), h
+
+
 def test_tree_is_a_prefill_for_a_chain(lib, torch_mod):
     torch = torch_mod
     H, KV, hd, pos0, n = 32, 8, 128, 300, 40
