@@ -2276,26 +2276,32 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams p, int3
         ml[u] = p.part_ml[at];
         v[u] = reinterpret_cast<const float4*>(p.part_o + at * HD)[d4];
     }
-    auto join = [](float m, float l, const float4& o, float M, float& L, float4& x) {
-        const float wt = l * __builtin_amdgcn_exp2f(m - M);
-        L += wt;
-        if (wt != 0.0f) {  // (a part without a key has nothing to add)
-            x.x += wt * o.x;
-            x.y += wt * o.y;
-            x.z += wt * o.z;
-            x.w += wt * o.w;
+    // x += f o; a part without a key (f 0) has nothing to add
+    auto add = [](float4& x, float f, const float4& o) {
+        if (f != 0.0f) {
+            x.x += f * o.x;
+            x.y += f * o.y;
+            x.z += f * o.z;
+            x.w += f * o.w;
         }
     };
-    float M = -1e30f, L = 0.0f;
+    // (weights are divided by their sum before they meet the values, whose sum may be
+    // past the largest float where their mean is not)
+    auto share = [](float L) { return L != 0.0f ? 1.0f / L : 0.0f; };
+    float M = -1e30f, L = 0.0f, w[kTreeMergeLoads];
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int u = 0; u < kTreeMergeLoads; ++u) M = fmaxf(M, ml[u].x);
 #pragma unroll
-    for (int u = 0; u < kTreeMergeLoads; ++u) join(ml[u].x, cg + u * CG < chunks ? ml[u].y : 0.0f, v[u], M, L, x);
+    for (int u = 0; u < kTreeMergeLoads; ++u) {
+        w[u] = cg + u * CG < chunks ? ml[u].y * __builtin_amdgcn_exp2f(ml[u].x - M) : 0.0f;
+        L += w[u];
+    }
+    float inv = share(L);
+#pragma unroll
+    for (int u = 0; u < kTreeMergeLoads; ++u) add(x, w[u] * inv, v[u]);
     if constexpr (CG > 1) {
-        // the threads' sums, normalised like the ranges' parts
-        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        part[cg][col] = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        part[cg][col] = x;
         mls[cg][col] = make_float2(M, L);
         __syncthreads();
         if (cg) return;
@@ -2304,12 +2310,14 @@ __global__ __launch_bounds__(kThreads) void tree_merge_kernel(TreeParams p, int3
 #pragma unroll
         for (int c = 1; c < CG; ++c) M = fmaxf(M, mls[c][col].x);
 #pragma unroll
-        for (int c = 0; c < CG; ++c) join(mls[c][col].x, mls[c][col].y, part[c][col], M, L, x);
+        for (int c = 0; c < CG; ++c) L += mls[c][col].y * __builtin_amdgcn_exp2f(mls[c][col].x - M);
+        inv = share(L);
+#pragma unroll
+        for (int c = 0; c < CG; ++c)
+            add(x, mls[c][col].y * __builtin_amdgcn_exp2f(mls[c][col].x - M) * inv, part[c][col]);
     }
     if (i / (HD / 4) >= rows) return;
-    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-    reinterpret_cast<float4*>(p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD)[d4] =
-        make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+    reinterpret_cast<float4*>(p.out + (static_cast<size_t>(row / G) * p.n_heads + hk * G + row % G) * HD)[d4] = x;
 }
 
 // The split of a call: groups of rows, keys of a range, ranges.

@@ -382,6 +382,21 @@ def test_tree_scores_of_any_size(lib, torch_mod, hd, size, exponent):
         assert bool((off <= 2.0 ** -21 * want.abs() + 2.0 ** -24 * want.abs().max()).all()), h
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("pos0,rows", [(200, [3, 9]), (300, [3, 150, 290]), (5000, range(0, 5000, 100)),
+                                       (20000, [1, 19999])])
+def test_tree_means_of_the_largest_values(lib, torch_mod, hd, pos0, rows):
+    """Value rows near the largest float, whose sum is past it and whose mean is
+    not, in one part of the keys and over many."""
+    torch = torch_mod
+    t = Tree(torch, 8, 2, hd, pos0, [-1, -1, 0], seed=hd)
+    t.q.zero_()
+    t.vc[list(rows)] = 3e38
+    t.vc[rows[-1], ::3] = -3e38
+    t.v[0] = 3e38
+    t.verify(lib)
+
+
 def test_tree_is_a_prefill_for_a_chain(lib, torch_mod):
     torch = torch_mod
     H, KV, hd, pos0, n = 32, 8, 128, 300, 40
