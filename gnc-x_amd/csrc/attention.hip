@@ -1640,8 +1640,12 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, T
 // element keeps 2^-22 of itself or of its row's largest, where that is more.
 // The keys' and the row's come back as a factor of the scores.  The values' 2^e
 // goes into the weights: those of O are 2^(s + e - max (s + e)), those of the sum
-// l 2^(s - max s), two running maxima a row, so that what a row does not see has
-// no say in its precision.
+// l 2^(s - max s), two running maxima a row, so that other groups that a row does
+// not see have no say in its precision.  Within a group a hidden row may set e, by
+// 2^14 above a visible one at most ("odd" keys, below), which leaves the weight of
+// the largest term at 2^-2 or more, where a pair still holds it to 2^-22.  Value rows
+// of zeros, which any e suits and which bring nothing to O, take no part in the
+// second maximum: their weights are added to l alone.
 // "Odd" keys, whose key or value row is not finite or lies more than 2^-14 below
 // its group's largest, are kept out of the products (0 times an infinity would be
 // NaN for the rows that do not see it) and added element by element at the end,
@@ -1827,6 +1831,26 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
     return alpha;
 }
 
+// Adds the weights of a tile's keys whose value rows are zeros (bits 8 + 4 g .. of
+// group h's word) to the sum, and takes them out of the tile.
+typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void leave_zeros(floatx16& st, const uint32x4& words, int g, RowState& s) {
+    float most = -1e30f, sum = 0.0f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (words[r >> 2] >> (8 + 4 * g + (r & 3)) & 1) most = fmaxf(most, st[r]);
+    const float m2 = fmaxf(s.m, ceilf(across_halves(most, [](float a, float b) { return fmaxf(a, b); })));
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        if (words[r >> 2] >> (8 + 4 * g + (r & 3)) & 1) {
+            sum += __builtin_amdgcn_exp2f(st[r] - m2);
+            st[r] = -__builtin_inff();
+        }
+    s.l = s.l * __builtin_amdgcn_exp2f(s.m - m2) + across_halves(sum, [](float a, float b) { return a + b; });
+    s.d += s.m - m2;
+    s.m = m2;
+}
+
 // The odd keys of [t0, t0 + 8) (below c1), by the rule that keeps them out of the
 // products, as a mask.
 template <int HD>
@@ -1877,7 +1901,10 @@ __device__ void add_odd_key(const TreeParams& p, const TreeShared& tree, int tre
 // the wave's normalised part to LDS: float4 column d4 of row li at 33 d4 + li
 template <int NN>
 __device__ __forceinline__ void store_part(float4* part, const floatx16 (&o)[NN], const RowState& s, int li, int g) {
-    const float f = s.l != 0.0f ? __builtin_amdgcn_exp2f(s.d - 14.0f) / s.l : 0.0f;
+    const float f = s.l != 0.0f ? 1.0f / s.l : 0.0f;
+    // (2^(d - 14) alone may be below the smallest float)
+    const int e = static_cast<int>(__builtin_amdgcn_fmed3f(s.d - 14.0f, -512.0f, 512.0f));
+    auto out = [&](float x) { return __builtin_ldexpf(x * f, e); };
 #pragma unroll
     for (int a = 0; a < 4; ++a)
 #pragma unroll
@@ -1886,9 +1913,9 @@ __device__ __forceinline__ void store_part(float4* part, const floatx16 (&o)[NN]
             if constexpr (NN >= 4) {
 #pragma unroll
                 for (int n = 0; n < NN; n += 4)
-                    part[(8 * n + at) * 33 + li] = make_float4(o[n][r] * f, o[n + 1][r] * f, o[n + 2][r] * f, o[n + 3][r] * f);
+                    part[(8 * n + at) * 33 + li] = make_float4(out(o[n][r]), out(o[n + 1][r]), out(o[n + 2][r]), out(o[n + 3][r]));
             } else if (b % 2 == 0) {
-                part[at / 2 * 33 + li] = make_float4(o[0][r] * f, o[1][r] * f, o[0][r + 1] * f, o[1][r + 1] * f);
+                part[at / 2 * 33 + li] = make_float4(out(o[0][r]), out(o[1][r]), out(o[0][r + 1]), out(o[1][r + 1]));
             }
         }
 }
@@ -1952,7 +1979,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
     constexpr int kShared = kTile * 8 > kPart * kWaves ? kTile * 8 : kPart * kWaves;
     __shared__ __align__(16) float4 shared[kShared];
     __shared__ __align__(16) float kfac[2][kWaves], vexp[2][kWaves];  // [tile in turn][group]: the keys' factor, the values' exponent
-    __shared__ __align__(16) uint32_t oddmask[2][kWaves];             // [tile in turn][group]: odd keys, from bit 8 group on
+    __shared__ __align__(16) uint32_t oddmask[2][kWaves];             // [tile in turn][group]: odd keys | value rows of zeros << 8
     __shared__ float2 mls[kWaves][32];
     // groups with odd keys, by the wave that staged them: tile of the range << 8 |
     // mask; the first tile whose group found no place
@@ -2011,7 +2038,7 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         }
     };
     auto stage = [&](int b, int t0) {
-        uint32_t odd = 0;  // this group's odd keys
+        uint32_t odd = 0, zeros = 0;  // this group's odd keys, and value rows of zeros beside others
         float krow = 0.0f;
 #pragma unroll
         for (int j = 0; j < NN; ++j) krow = max3_abs(max3_abs(krow, kst[j][0], kst[j][1]), kst[j][2], kst[j][3]);
@@ -2075,6 +2102,9 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
                 const uint64_t w = __ballot(bad);
                 if (static_cast<uint32_t>(w)) odd |= 1u << r;
                 if (w >> 32) odd |= 1u << (r + 4);
+                const uint64_t z = __ballot(vrow[r] == 0.0f && vtop > 0.0f);
+                if (static_cast<uint32_t>(z)) zeros |= 1u << r;
+                if (z >> 32) zeros |= 1u << (r + 4);
 #pragma unroll
                 for (int n = 0; n < NN; ++n) vst[n][r] = bad ? 0.0f : vst[n][r];
             }
@@ -2083,8 +2113,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         const float vs = pow2_field(254 - vf);
         if (lane == 0) {
             kfac[b][wv] = pow2_field(kf);
-            vexp[b][wv] = static_cast<float>(vf - 127);
-            oddmask[b][wv] = odd << (8 * wv);
+            vexp[b][wv] = vtop > 0.0f ? static_cast<float>(vf - 127) : -1e30f;  // (zeros alone: below every other's)
+            oddmask[b][wv] = odd | zeros << 8;
             if (odd) {
                 const int n = odd_count[wv];
                 if (n < kOddGroups) {
@@ -2163,9 +2193,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         interleave_reads<NC>();
         __builtin_amdgcn_sched_barrier(0);
         const floatx4 kf = *reinterpret_cast<const floatx4*>(kfac[b]), vx = *reinterpret_cast<const floatx4*>(vexp[b]);
-        typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
         const uint32x4 om = *reinterpret_cast<const uint32x4*>(oddmask[b]);
-        const uint32_t odd = __builtin_amdgcn_readfirstlane(om[0] | om[1] | om[2] | om[3]);
+        const uint32_t apart = __builtin_amdgcn_readfirstlane(om[0] | om[1] | om[2] | om[3]);
         const float ve[4] = {vx[0], vx[1], vx[2], vx[3]}, sf[4] = {kf[0] * qf, kf[1] * qf, kf[2] * qf, kf[3] * qf};
 #pragma unroll
         for (int r = 0; r < 16; ++r) st[r] *= sf[r >> 2];
@@ -2188,10 +2217,13 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
 #pragma unroll
             for (int r = 0; r < 16; ++r) st[r] = t0 + 8 * (r >> 2) + 4 * g + (r & 3) >= place.lo ? st[r] : hidden;
         }
-        if (odd)
+        if (__builtin_expect(apart != 0, 0)) {
+            // by the lane's register: key 8 (r / 4) + 4 g + r % 4
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (odd >> (8 * (r >> 2) + 4 * g + (r & 3)) & 1) st[r] = hidden;
+                if (om[r >> 2] >> (4 * g + (r & 3)) & 1) st[r] = hidden;
+            if (apart >> 8) leave_zeros(st, om, g, s);
+        }
         half8_t ph[2], pl[2];
         const float alpha = tile_softmax(st, ve, s, ph, pl);
         if (__ballot(alpha != 1.0f))

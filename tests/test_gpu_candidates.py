@@ -397,6 +397,61 @@ def test_tree_means_of_the_largest_values(lib, torch_mod, hd, pos0, rows):
     t.verify(lib)
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("big", [1e6, 1e20, 3e38])
+@pytest.mark.parametrize("flat", [False, True])
+def test_tree_value_rows_of_zeros_beside_hidden_ones(lib, torch_mod, hd, big, flat):
+    """A value row of zeros takes nothing from the precision of the others,
+    whatever rows that its node does not see stand beside it: an earlier branch's
+    among the nodes, or one before the window at the start of a long range.  With
+    equal scores (flat) every weight is 1 of all."""
+    torch = torch_mod
+    for pos0, sw in ((100, 0), (9000, 8900)):
+        t = Tree(torch, 8, 2, hd, pos0, [-1] + list(range(-1, 6)) + [-1, 7, 7], sw=sw, seed=hd)
+        t.v[0] = big                        # node 0 stands alone; the others do not see it
+        t.v[1], t.v[3] = 0.0, 0.0
+        first = max(0, pos0 - sw + 1) if sw else 0
+        if sw:
+            t.vc[first] = big               # only nodes without a parent see it
+            t.vc[first + 5:first + 7] = 0.0
+        t.vc[first + 40] = 0.0
+        t.vc[first + 64:first + 72] = 0.0   # a whole group
+        if flat:
+            t.q.zero_()
+        t.verify(lib)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_tree_nodes_that_see_zeros_alone(lib, torch_mod, hd):
+    torch = torch_mod
+    t = Tree(torch, 8, 2, hd, 37, [-1] * 9, seed=hd)
+    t.vc.zero_()
+    t.v[:4] = 0.0
+    t.v[5] = 1e30
+    t.verify(lib)
+    assert not t.out[:4].any() and bool(t.out[5].all())
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("pos0", [60, 4000])
+@pytest.mark.parametrize("size,below", [(1.0, 110), (1e-20, 55), (1e-33, 10)])
+def test_tree_small_terms_under_rows_of_zeros(lib, torch_mod, hd, pos0, size, below):
+    """Value rows of zeros have almost all of the weight; what is left for the
+    others, 2^-below of small values, is the output."""
+    torch = torch_mod
+    t = Tree(torch, 8, 2, hd, pos0, [-1, 0, 0], seed=hd)
+    for c in (t.q, t.k, t.kc):
+        c.zero_()
+    t.q[:, ::hd] = 16.0
+    zeros = torch.arange(pos0, device="cuda")
+    zeros = zeros[(zeros % 3 == 0) | (zeros // 8 % 3 == 0)]
+    t.kc[zeros[:, None], torch.arange(0, 2 * hd, hd, device="cuda")] = below * math.log(2.0) / (16.0 * t.scale)
+    t.v *= size
+    t.vc *= size
+    t.vc[zeros] = 0.0
+    t.verify(lib)
+
+
 def test_tree_is_a_prefill_for_a_chain(lib, torch_mod):
     torch = torch_mod
     H, KV, hd, pos0, n = 32, 8, 128, 300, 40
