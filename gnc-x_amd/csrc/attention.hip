@@ -2114,7 +2114,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
         if (lane == 0) {
             kfac[b][wv] = pow2_field(kf);
             vexp[b][wv] = vtop > 0.0f ? static_cast<float>(vf - 127) : -1e30f;  // (zeros alone: below every other's)
-            oddmask[b][wv] = odd | zeros << 8;
+            // (rows past the range are zeros as well, and nobody's)
+            oddmask[b][wv] = odd | (zeros & ((1u << min(max(c1 - t0 - 8 * wv, 0), 8)) - 1)) << 8;
             if (odd) {
                 const int n = odd_count[wv];
                 if (n < kOddGroups) {
