@@ -2936,18 +2936,52 @@ struct DeviceGuard {
     }
 };
 
-// p is memory of the library's GPU, 4-byte (or `align`-byte) aligned
-bool on_device(const void* p, const char* name, const char* where, uintptr_t align = 4) {
-    hipPointerAttribute_t a;
-    const hipError_t e = p ? hipPointerGetAttributes(&a, p) : hipErrorInvalidValue;
-    if (e != hipSuccess) (void)hipGetLastError();
-    if (e != hipSuccess || !(a.type == hipMemoryTypeManaged ||
-                             (a.type == hipMemoryTypeDevice && a.device == g_rt.device))) {
-        set_error(where, (std::string(name) + " must be memory of the library's GPU").c_str(), -1);
+// The allocations that a call's pointers lie in, the last eight: each is asked for
+// once (two queries of 0.2 us).
+struct Allocations {
+    std::array<uintptr_t, 8> lo{}, hi{};
+    unsigned count = 0;
+    // the end of a's allocation, 0 if it is not known
+    uintptr_t end_of(uintptr_t a) const {
+        for (unsigned i = 0; i < lo.size(); ++i)
+            if (a >= lo[i] && a < hi[i]) return hi[i];
+        return 0;
+    }
+    void add(const void* p) {
+        hipDeviceptr_t base = nullptr;
+        size_t n = 0;
+        if (hipMemGetAddressRange(&base, &n, const_cast<void*>(p)) != hipSuccess) {
+            (void)hipGetLastError();
+            return;
+        }
+        const unsigned i = count++ % lo.size();
+        lo[i] = reinterpret_cast<uintptr_t>(base);
+        hi[i] = lo[i] + n;
+    }
+};
+
+// p is `align`-byte aligned memory of the library's GPU that holds `bytes` from p on
+bool on_device(const void* p, size_t bytes, const char* name, const char* where, Allocations& seen,
+               uintptr_t align = 4) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    if (!seen.end_of(a)) {
+        hipPointerAttribute_t at;
+        const hipError_t e = p ? hipPointerGetAttributes(&at, p) : hipErrorInvalidValue;
+        if (e != hipSuccess) (void)hipGetLastError();
+        if (e != hipSuccess || !(at.type == hipMemoryTypeManaged ||
+                                 (at.type == hipMemoryTypeDevice && at.device == g_rt.device))) {
+            set_error(where, (std::string(name) + " must be memory of the library's GPU").c_str(), -1);
+            return false;
+        }
+        seen.add(p);
+    }
+    if (a % align) {
+        set_error(where, (std::string(name) + " must be " + std::to_string(align) + "-byte aligned").c_str(), -1);
         return false;
     }
-    if (reinterpret_cast<uintptr_t>(p) % align) {
-        set_error(where, (std::string(name) + " must be " + std::to_string(align) + "-byte aligned").c_str(), -1);
+    const uintptr_t end = seen.end_of(a);
+    if (end && bytes > end - a) {
+        set_error(where, (std::string(name) + " reaches past the end of its memory").c_str(), -1);
         return false;
     }
     return true;
@@ -3017,33 +3051,18 @@ bool layer_arrays(float* const* k, float* const* v, int32_t n_layers, const char
 
 // Every cache is memory of the library's GPU, holds `floats` floats, and no two
 // share a touched float: cache c's are [lo, floats) + beam * stride for beams
-// below n_beams.  The pointer query (0.2 us) is made once per allocation.
+// below n_beams.
 bool layer_caches(float* const* k, float* const* v, int32_t n_layers, size_t lo, size_t floats, int32_t n_beams,
                   size_t stride, const char* where) {
     const size_t span = sizeof(float) * (stride * (n_beams - 1) + floats);
     const size_t step = sizeof(float) * stride, own = sizeof(float) * (floats - lo);
     static std::array<std::pair<uintptr_t, uintptr_t>, 2 * kMaxLayers> at;  // (place within a stride, address); the call lock is held
     const size_t n = 2 * static_cast<size_t>(n_layers);
-    uintptr_t bases[2] = {0, 0}, ends[2] = {0, 0};  // the last k cache's and v cache's allocations
+    Allocations seen;
     for (int32_t i = 0; i < 2 * n_layers; ++i) {
         const float* p = i % 2 ? v[i / 2] : k[i / 2];
         const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-        uintptr_t &base = bases[i % 2], &end = ends[i % 2];
-        if (a < base || a >= end || a % 16) {
-            if (!on_device(p, i % 2 ? "every v cache" : "every k cache", where, 16)) return false;
-            hipDeviceptr_t b = nullptr;
-            size_t n = 0;
-            if (hipMemGetAddressRange(&b, &n, const_cast<float*>(p)) != hipSuccess) {
-                (void)hipGetLastError();
-                n = 0;
-            }
-            base = reinterpret_cast<uintptr_t>(b);
-            end = base + n;
-        }
-        if (a >= base && a < end && span > end - a) {
-            set_error(where, "the rows lie past the end of a cache's memory", -1);
-            return false;
-        }
+        if (!on_device(p, span, i % 2 ? "every v cache" : "every k cache", where, seen, 16)) return false;
         at[i] = {n_beams > 1 ? a % step : a, a};
     }
     // two caches can meet only where their places within a stride are less
@@ -3096,18 +3115,18 @@ GNCX_API void gncx_hip_attention_tree(float* q_nodes, float* k_nodes, const floa
     if (!ensure_runtime(where)) return;
     DeviceGuard dev(where);
     if (!dev.ok) return;
-    if (!on_device(q_nodes, "q_nodes", where, 16) || !on_device(k_nodes, "k_nodes", where, 16) ||
-        !on_device(v_nodes, "v_nodes", where, 16) || !on_device(k_cache_layer, "k_cache_layer", where, 16) ||
-        !on_device(v_cache_layer, "v_cache_layer", where, 16) || !on_device(out_nodes, "out_nodes", where, 16))
-        return;
-    // no two arguments share memory, but for k_nodes / v_nodes that are the
-    // cache rows they are stored to
     const size_t qb = sizeof(float) * n_nodes * n_heads * head_dim, kvrow = sizeof(float) * n_kv_heads * head_dim;
     const size_t kb = kvrow * n_nodes, cb = kvrow * (static_cast<size_t>(pos0) + n_nodes), at = kvrow * pos0;
     const char* ps[] = {reinterpret_cast<char*>(q_nodes), reinterpret_cast<char*>(k_nodes),
                         reinterpret_cast<const char*>(v_nodes), reinterpret_cast<char*>(k_cache_layer),
                         reinterpret_cast<char*>(v_cache_layer), reinterpret_cast<char*>(out_nodes)};
     const size_t bytes[] = {qb, kb, kb, cb, cb, qb};
+    const char* names[] = {"q_nodes", "k_nodes", "v_nodes", "k_cache_layer", "v_cache_layer", "out_nodes"};
+    Allocations seen;
+    for (int i = 0; i < 6; ++i)
+        if (!on_device(ps[i], bytes[i], names[i], where, seen, 16)) return;
+    // no two arguments share memory, but for k_nodes / v_nodes that are the
+    // cache rows they are stored to
     for (int i = 0; i < 6; ++i)
         for (int j = i + 1; j < 6; ++j)
             if (overlaps(ps[i], bytes[i], ps[j], bytes[j]) &&
@@ -3195,11 +3214,15 @@ GNCX_API void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t
     if (!ensure_runtime(where)) return;
     DeviceGuard dev(where);
     if (!dev.ok) return;
-    if (!on_device(logits, "logits", where) || !on_device(scores, "scores", where) ||
-        (finished && !on_device(finished, "finished", where)) || !on_device(out_parents, "out_parents", where) ||
-        !on_device(out_tokens, "out_tokens", where) || !on_device(out_scores, "out_scores", where))
+    const size_t ob = sizeof(int32_t) * n_out, ib = sizeof(int32_t) * n_beams;
+    Allocations seen;
+    if (!on_device(logits, sizeof(float) * n_beams * vocab, "logits", where, seen) ||
+        !on_device(scores, ib, "scores", where, seen) ||
+        (finished && !on_device(finished, ib, "finished", where, seen)) ||
+        !on_device(out_parents, ob, "out_parents", where, seen) ||
+        !on_device(out_tokens, ob, "out_tokens", where, seen) ||
+        !on_device(out_scores, ob, "out_scores", where, seen))
         return;
-    const size_t ob = sizeof(int32_t) * n_out;
     if (overlaps(out_parents, ob, out_tokens, ob) || overlaps(out_parents, ob, out_scores, ob) ||
         overlaps(out_tokens, ob, out_scores, ob)) {
         set_error(where, "two of the outputs overlap", -1);
@@ -3229,7 +3252,8 @@ GNCX_API void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches
     if (!ensure_runtime(where)) return;
     DeviceGuard dev(where);
     if (!dev.ok) return;
-    if (!on_device(parents, "parents", where) ||
+    Allocations seen;
+    if (!on_device(parents, sizeof(int32_t) * n_beams, "parents", where, seen) ||
         !layer_caches(k_caches, v_caches, n_layers, static_cast<size_t>(row0) * kv_dim,
                       (static_cast<size_t>(row0) + n_rows) * kv_dim, n_beams, beam_stride, where))
         return;

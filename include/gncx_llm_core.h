@@ -443,7 +443,8 @@ void gncx_hip_argmax(const float* values, int32_t n, int32_t* out_index);
  * outputs are memory of the library's GPU, used in place and in the order of
  * the library stream, and nothing synchronises with the host (but for the
  * upload of a position's rotations, below).  Refused calls leave every output
- * as it was.
+ * as it was; refused is also what would reach past the end of the allocation
+ * that a pointer lies in.
  *
  * Attention of a drafted tree of n_nodes (1..512) tokens over the cache of the
  * first pos0 positions.  parents (host memory, read before the call returns):

@@ -837,6 +837,66 @@ def test_refusals_on_the_device(lib, torch_mod):
     assert not c.any() and not p.any()
 
 
+def past_the_end(torch, t):
+    """Bytes from t's first to the end of the allocation that it lies in."""
+    at = t.data_ptr()
+    for s in torch.cuda.memory_snapshot():
+        if s["address"] <= at < s["address"] + s["total_size"]:
+            return s["address"] + s["total_size"] - at
+    raise AssertionError("not the allocator's memory")
+
+
+@pytest.mark.parametrize("short", ["q", "k", "v", "kc", "vc", "out"])
+def test_tree_vectors_and_caches_that_end_early_are_refused(lib, torch_mod, short):
+    """Nothing is launched where a vector, cache or output would be read or
+    written past the end of its memory."""
+    torch = torch_mod
+    t = Tree(torch, 8, 2, 128, 16, make_parents("chain", 4))
+    before = {n: getattr(t, n).clone() for n in ("q", "k", "kc", "vc")}
+    lib.gncx_hip_last_status()
+    old, old_pos = getattr(t, short), t.pos0
+    if short in ("kc", "vc"):
+        t.pos0 = past_the_end(torch, old) // (4 * 256) - 3  # 3 of 4 rows fit
+    else:
+        # the last 16 bytes of its memory
+        end = past_the_end(torch, old)
+
+        class Last:
+            data_ptr = staticmethod(lambda: old.data_ptr() + end - 16)
+        setattr(t, short, Last)
+    t.call(lib, check=False)
+    refused(lib, "end")
+    setattr(t, short, old)
+    t.pos0 = old_pos
+    for n, v in before.items():
+        assert torch.equal(getattr(t, n), v)
+    t.call(lib)
+
+
+def test_select_and_reorder_refuse_what_ends_early(lib, torch_mod):
+    torch = torch_mod
+    B, V, n = 3, 100, 4
+    flat = torch.zeros(4096, device="cuda")
+    lib.gncx_hip_last_status()
+    last = flat.data_ptr() + past_the_end(torch, flat) - 4  # a float, where more are needed
+    x, sc, fin = torch.randn(B, V, device="cuda"), torch.zeros(B, device="cuda"), torch.zeros(B, dtype=torch.int32, device="cuda")
+    out = torch.zeros(3, n, dtype=torch.int32, device="cuda")
+    good = [x.data_ptr(), sc.data_ptr(), fin.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr()]
+    for i in range(6):
+        a = list(good)
+        a[i] = last
+        lib.gncx_hip_beam_select(a[0], B, V, a[1], a[2], 0, n, *a[3:])
+        refused(lib, "end")
+    assert not out.any()
+    lib.gncx_hip_beam_select(good[0], B, V, good[1], good[2], 0, n, *good[3:])
+    gncx.check(lib)
+    c = torch.randn(2, B, 8, 64, device="cuda")
+    before = c.clone()
+    lib.gncx_hip_kv_reorder(addresses(c[:1]), addresses(c[1:]), 1, B, 512, 64, 0, 8, last)
+    refused(lib, "end")
+    assert torch.equal(c, before)
+
+
 # ---- graphs ------------------------------------------------------------------------------
 def test_selection_and_reordering_captured(lib, torch_mod):
     """A beam step's selection and reordering in a graph, replayed between eager
