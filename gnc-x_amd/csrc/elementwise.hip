@@ -799,7 +799,7 @@ struct SelectParams {
     const float* scores;
     const int32_t* finished;
     int32_t finished_token, n_beams, vocab, n_out, n_chunks;
-    float2* ml;   // [beam][chunk] maximum, sum of e^(x - maximum)
+    double2* ml;   // [beam][chunk] maximum, sum of e^(x - maximum)
     float2* best;  // [beam][chunk][n_out] logit, word (as bits), in falling order; -inf behind the last
     int32_t* out_parents;
     int32_t* out_tokens;
@@ -838,6 +838,28 @@ __device__ __forceinline__ float nth_largest(const float* maxima, int n, int lan
         if (count >= n) least = t;
     }
     return least > 0x007fffffu ? unordered(least) : -__builtin_inff();  // (0x007fffff: -inf itself)
+}
+
+// v and another lane's, through DPP (no LDS round trip, unlike a shuffle)
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ double dpp_add_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROW_MASK, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROW_MASK, 0xf, false);
+    return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// Sum over the wave, returned in every lane: wave_sum's steps.
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v = dpp_add_f64<0xb1>(v);
+    v = dpp_add_f64<0x4e>(v);
+    v = dpp_add_f64<0x141>(v);
+    v = dpp_add_f64<0x140>(v);
+    v = dpp_add_f64<0x142, 0xa>(v);
+    v = dpp_add_f64<0x143, 0xc>(v);
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), 63);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), 63);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
@@ -892,17 +914,19 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
         const float4 w = reinterpret_cast<const float4*>(maxima)[lane];
         m = wave_max(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
     }
-    float l = 0.0f;
+    // exponentials of 32 bits, summed in 64 (a sum of 32 loses those of a large vocabulary
+    // one by one beside a word that has most of the weight)
+    double l = 0.0;
     if (m > -__builtin_inff())
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float e[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) e[i] = x[j][i] == m ? 1.0f : expf(x[j][i] - m);  // (x == m: an infinite maximum)
-            l += (e[0] + e[1]) + (e[2] + e[3]);
+            l += (static_cast<double>(e[0]) + e[1]) + (static_cast<double>(e[2]) + e[3]);
         }
-    l = wave_sum(l);
-    if (lane == 0) sums[wv] = static_cast<double>(l);
+    l = wave_sum_f64(l);
+    if (lane == 0) sums[wv] = l;
     const float least = nth_largest(maxima, p.n_out, lane);
     int mine = 0;
 #pragma unroll
@@ -927,7 +951,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
         double s = sums[0];
 #pragma unroll
         for (int w = 1; w < kWavesHere; ++w) s += sums[w];
-        p.ml[part] = make_float2(m, static_cast<float>(s));
+        p.ml[part] = make_double2(m, s);
     }
     const int n = held;
     if (n <= kMostRanked) {
@@ -1001,17 +1025,14 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
         float m = -__builtin_inff();
         double sum = 0.0;
         if (!done) {
-            const float2* ml = p.ml + static_cast<size_t>(b) * p.n_chunks;
-            for (int c = lane; c < p.n_chunks; c += 64) m = fmaxf(m, ml[c].x);
+            const double2* ml = p.ml + static_cast<size_t>(b) * p.n_chunks;
+            for (int c = lane; c < p.n_chunks; c += 64) m = fmaxf(m, static_cast<float>(ml[c].x));
             m = wave_max(m);
             for (int c = lane; c < p.n_chunks; c += 64) {
-                const float2 v = ml[c];
-                if (v.x > -__builtin_inff())
-                    sum += static_cast<double>(v.y) *
-                           (v.x == m ? 1.0 : exp(static_cast<double>(v.x) - static_cast<double>(m)));
+                const double2 v = ml[c];
+                if (v.x > -__builtin_inff()) sum += v.y * (v.x == m ? 1.0 : exp(v.x - m));
             }
-#pragma unroll
-            for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+            sum = wave_sum_f64(sum);
         }
         if (lane == 0) {
             top[b] = m;
@@ -1187,7 +1208,7 @@ hipError_t launch_kv_reorder(float* const* k, float* const* v, int32_t n_layers,
 
 size_t beam_select_workspace_bytes(int32_t n_beams, int32_t vocab, int32_t n_out) {
     const int32_t words = 1024 * select_vectors(n_beams, vocab);
-    return static_cast<size_t>(n_beams) * ((vocab + words - 1) / words) * sizeof(float2) * (1 + static_cast<size_t>(n_out));
+    return static_cast<size_t>(n_beams) * ((vocab + words - 1) / words) * (sizeof(double2) + sizeof(float2) * n_out);
 }
 
 hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,
@@ -1207,8 +1228,8 @@ hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t voca
     p.n_out = n_out;
     const int32_t v = select_vectors(n_beams, vocab);
     p.n_chunks = (vocab + 1024 * v - 1) / (1024 * v);
-    p.ml = static_cast<float2*>(workspace);
-    p.best = p.ml + static_cast<size_t>(n_beams) * p.n_chunks;
+    p.ml = static_cast<double2*>(workspace);
+    p.best = reinterpret_cast<float2*>(p.ml + static_cast<size_t>(n_beams) * p.n_chunks);
     p.out_parents = out_parents;
     p.out_tokens = out_tokens;
     p.out_scores = out_scores;

@@ -485,8 +485,9 @@ void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_caches, int32
  * (b, finished_token) with the score scores[b], and its logits are not read.
  * The n_out (1..64) best come in falling order, equal scores by the lowest
  * b * vocab + v.  A NaN logit or score counts as -inf, and a score of -inf is
- * no candidate: outputs left over have parent -1, word -1, score -inf.  Sums
- * and scores are formed in 64 bits.  out_scores may be scores, out_parents or
+ * no candidate: outputs left over have parent -1, word -1, score -inf.
+ * Exponentials are formed in 32 bits (so a score may be off by 2^-19), their
+ * sums and the scores in 64.  out_scores may be scores, out_parents or
  * out_tokens finished; no two outputs overlap.  Captured into a graph, the
  * call's workspace (at most 5 MiB) belongs to the graph for the process's life. */
 void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t vocab, const float* scores,

@@ -785,6 +785,24 @@ def test_select_unaligned_rows_and_outputs_over_inputs(lib, torch_mod):
     assert np.allclose(scores.cpu().numpy(), want[2], rtol=1e-6)
 
 
+@pytest.mark.parametrize("V", [16384, 151936])
+@pytest.mark.parametrize("gap", [12.0, 14.0, 15.5])
+def test_select_sums_of_many_small_exponentials(lib, torch_mod, V, gap):
+    """One large logit among equal small ones, whose exponentials are lost one by
+    one in a 32-bit sum that holds the large one's.  The exponentials are formed
+    in 32 bits (1 ulp of expf and the difference's half step, gap u, each of
+    itself), so the sum is off by at most (2 + gap) u of the small ones' part of
+    it, and the score by that and its own rounding."""
+    torch = torch_mod
+    logits = torch.full((1, V), -gap, device="cuda")
+    logits[0, V // 3] = 0.0
+    _, tok, got = select(lib, torch, logits, torch.zeros(1, device="cuda"), 1)
+    small = (V - 1) * math.exp(-gap)
+    want = -math.log1p(small)
+    assert tok[0] == V // 3
+    assert abs(float(got[0]) - want) <= (2 + gap) * U * small / (1 + small) + U * abs(want) + 2.0 ** -50
+
+
 # ---- reordering ------------------------------------------------------------------------
 @pytest.mark.parametrize("layers,beams,kv_dim,row0,rows,parents", [
     (1, 1, 4, 0, 1, [0]), (1, 1, 4, 0, 1, [-1]), (2, 2, 8, 1, 3, [1, 0]), (3, 4, 128, 5, 17, [0, 0, 0, 0]),
