@@ -781,7 +781,7 @@ __global__ __launch_bounds__(kCandThreads) void reorder_kernel(ReorderParams p) 
 
 // ---- beam search's selection ------------------------------------------------------
 // score(b, v) = scores[b] + logits[b][v] - log sum_u e^logits[b][u]; the n_out
-// best, ties to the lowest b vocab + v.  Within a beam the order is the
+// best, ties to the lowest b vocab + v (Candidate).  Within a beam the order is the
 // logits', so one pass over them leaves, per (beam, part of the vocabulary),
 // the part's maximum, its sum of exponentials and its n_out best; a second
 // kernel joins the parts in double, where candidates of different beams meet.
@@ -991,9 +991,17 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
     }
 }
 
+// The order of equal scores: the lower beam, then the larger logit (64 bits may not
+// part the scores of two logits, and the parts' lists are by logits), then the lower
+// word.  Words are below 2^22, beams below 2^5.
+constexpr int kWordBits = 22;
+static_assert(kMaxBeamVocab <= 1 << kWordBits && kMaxBeams <= 1 << (63 - 32 - kWordBits));
+__device__ __forceinline__ int64_t place_of(int beam, float logit, int word) {
+    return static_cast<int64_t>(beam) << (32 + kWordBits) | static_cast<int64_t>(~ordered(logit)) << kWordBits | word;
+}
 struct Candidate {
     double score;
-    int64_t at;  // beam vocab + word
+    int64_t at;  // place_of
     __device__ bool before(const Candidate& o) const { return score > o.score || (score == o.score && at < o.at); }
 };
 
@@ -1046,10 +1054,10 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
         const int b = part / p.n_chunks;
         if (ended[b])
             return r || part % p.n_chunks ? Candidate{-inf, 0}
-                                          : Candidate{base[b], static_cast<int64_t>(b) * p.vocab + p.finished_token};
+                                          : Candidate{base[b], place_of(b, 0.0f, p.finished_token)};
         if (!(e.x > -__builtin_inff())) return Candidate{-inf, 0};
         return Candidate{base[b] + (e.x == top[b] ? 0.0 : static_cast<double>(e.x) - static_cast<double>(top[b])),
-                         static_cast<int64_t>(b) * p.vocab + __builtin_bit_cast(int32_t, e.y)};
+                         place_of(b, e.x, __builtin_bit_cast(int32_t, e.y))};
     };
     auto candidate = [&](int part, int r) { return entry(part, r, p.best[static_cast<size_t>(part) * p.n_out + r]); };
     // The parts' lists fall, so the threshold comes from their first entries (as
@@ -1078,8 +1086,8 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
         }
     __syncthreads();
     auto write = [&](int i, const Candidate& c) {
-        p.out_parents[i] = static_cast<int32_t>(c.at / p.vocab);
-        p.out_tokens[i] = static_cast<int32_t>(c.at % p.vocab);
+        p.out_parents[i] = static_cast<int32_t>(c.at >> (32 + kWordBits));
+        p.out_tokens[i] = static_cast<int32_t>(c.at & ((1 << kWordBits) - 1));
         p.out_scores[i] = static_cast<float>(c.score);
     };
     auto write_none = [&](int i) {

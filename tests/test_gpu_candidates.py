@@ -803,6 +803,25 @@ def test_select_sums_of_many_small_exponentials(lib, torch_mod, V, gap):
     assert abs(float(got[0]) - want) <= (2 + gap) * U * small / (1 + small) + U * abs(want) + 2.0 ** -50
 
 
+@pytest.mark.parametrize("V", [7, 200, 5000, 151936])
+@pytest.mark.parametrize("score", [1e20, -1e20, float("inf"), 0.0])
+def test_select_scores_that_64_bits_do_not_part(lib, torch_mod, V, score):
+    """Words of a beam whose scores are equal in 64 bits although their logits are
+    not (a beam's score that swallows them, logits next to 0): the larger logit
+    first, equal ones by the lower word; beams with equal scores by the lower beam."""
+    torch = torch_mod
+    n_out = 20
+    g = torch.Generator(device="cuda").manual_seed(V)
+    logits = torch.randint(-40, 40, (3, V), generator=g, device="cuda").float() / 4
+    if score == 0.0:
+        logits *= 1e-30
+    scores = torch.tensor([-1e30, score, score], device="cuda")  # (the first beam comes last)
+    order = np.argsort(-logits.cpu().numpy(), axis=1, kind="stable")
+    par, tok, _ = select(lib, torch, logits, scores, n_out)
+    assert par.tolist() == np.repeat([1, 2, 0], V)[:n_out].tolist()
+    assert np.array_equal(tok, order[[1, 2, 0]].reshape(-1)[:n_out])
+
+
 # ---- reordering ------------------------------------------------------------------------
 @pytest.mark.parametrize("layers,beams,kv_dim,row0,rows,parents", [
     (1, 1, 4, 0, 1, [0]), (1, 1, 4, 0, 1, [-1]), (2, 2, 8, 1, 3, [1, 0]), (3, 4, 128, 5, 17, [0, 0, 0, 0]),
