@@ -1049,15 +1049,17 @@ __global__ __launch_bounds__(kJoinThreads) void select_join_kernel(SelectParams 
         }
     }
     __syncthreads();
-    // the r-th best candidate of a part; -inf behind the last
+    // the r-th best candidate of a part; -inf behind the last, and for a score that
+    // the output's 32 bits hold as -inf
     auto entry = [&](int part, int r, float2 e) {
         const int b = part / p.n_chunks;
         if (ended[b])
             return r || part % p.n_chunks ? Candidate{-inf, 0}
                                           : Candidate{base[b], place_of(b, 0.0f, p.finished_token)};
         if (!(e.x > -__builtin_inff())) return Candidate{-inf, 0};
-        return Candidate{base[b] + (e.x == top[b] ? 0.0 : static_cast<double>(e.x) - static_cast<double>(top[b])),
-                         place_of(b, e.x, __builtin_bit_cast(int32_t, e.y))};
+        const double score = base[b] + (e.x == top[b] ? 0.0 : static_cast<double>(e.x) - static_cast<double>(top[b]));
+        if (!(static_cast<float>(score) > -__builtin_inff())) return Candidate{-inf, 0};
+        return Candidate{score, place_of(b, e.x, __builtin_bit_cast(int32_t, e.y))};
     };
     auto candidate = [&](int part, int r) { return entry(part, r, p.best[static_cast<size_t>(part) * p.n_out + r]); };
     // The parts' lists fall, so the threshold comes from their first entries (as

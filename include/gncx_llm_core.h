@@ -486,8 +486,8 @@ void gncx_hip_kv_keep_rows(float* const* k_caches, float* const* v_caches, int32
  * The n_out (1..64) best come in falling order, equal scores by the lowest
  * b * vocab + v (but for a beam's words of different logits whose scores are
  * equal in 64 bits: those by falling logits).  A NaN logit or score counts as
- * -inf, and a score of -inf is no candidate: outputs left over have parent -1,
- * word -1, score -inf.
+ * -inf, and a score of -inf (also one below the least float) is no candidate:
+ * outputs left over have parent -1, word -1, score -inf.
  * Exponentials are formed in 32 bits (so a score may be off by 2^-19), their
  * sums and the scores in 64.  out_scores may be scores, out_parents or
  * out_tokens finished; no two outputs overlap.  Captured into a graph, the

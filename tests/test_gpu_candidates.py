@@ -822,6 +822,21 @@ def test_select_scores_that_64_bits_do_not_part(lib, torch_mod, V, score):
     assert np.array_equal(tok, order[[1, 2, 0]].reshape(-1)[:n_out])
 
 
+def test_select_scores_below_the_least_float(lib, torch_mod):
+    """A score that 32 bits hold as -inf is no candidate."""
+    torch = torch_mod
+    logits = torch.tensor([[0.0, -3e38, -1e38, 0.0], [-3e38, 5.0, 1.0, -3e38]], device="cuda")
+    scores = torch.tensor([-3e38, -1.0], device="cuda")
+    par, tok, out = select(lib, torch, logits, scores, 10)
+    # (beam 1's words 0 and 3 are at -3e38 - 6, equal in 64 bits to beam 0's -3e38 -
+    # log 2, and come behind them; beam 0's word 2 is at -4e38)
+    assert par.tolist() == [1, 1, 0, 0, 1, 1] + [-1] * 4
+    assert tok.tolist() == [1, 2, 0, 3, 0, 3] + [-1] * 4
+    assert np.isfinite(out[:6]).all() and (out[6:] == -np.inf).all()
+    par, tok, out = select(lib, torch, logits[:1].contiguous(), scores, 3)
+    assert par.tolist() == [0, 0, -1] and tok.tolist() == [0, 3, -1] and out[2] == -np.inf
+
+
 # ---- reordering ------------------------------------------------------------------------
 @pytest.mark.parametrize("layers,beams,kv_dim,row0,rows,parents", [
     (1, 1, 4, 0, 1, [0]), (1, 1, 4, 0, 1, [-1]), (2, 2, 8, 1, 3, [1, 0]), (3, 4, 128, 5, 17, [0, 0, 0, 0]),
