@@ -3257,6 +3257,18 @@ GNCX_API void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches
         !layer_caches(k_caches, v_caches, n_layers, static_cast<size_t>(row0) * kv_dim,
                       (static_cast<size_t>(row0) + n_rows) * kv_dim, n_beams, beam_stride, where))
         return;
+    // the parents are read while the rows are written
+    const size_t first = sizeof(float) * row0 * static_cast<size_t>(kv_dim);
+    const size_t rows = sizeof(float) * n_rows * static_cast<size_t>(kv_dim), step = sizeof(float) * beam_stride;
+    for (int32_t i = 0; i < 2 * n_layers; ++i) {
+        const char* c = reinterpret_cast<const char*>(i % 2 ? v_caches[i / 2] : k_caches[i / 2]) + first;
+        if (!overlaps(c, step * (n_beams - 1) + rows, parents, sizeof(int32_t) * n_beams)) continue;
+        for (int32_t b = 0; b < n_beams; ++b)
+            if (overlaps(c + b * step, rows, parents, sizeof(int32_t) * n_beams)) {
+                set_error(where, "the parents lie within the rows of a cache", -1);
+                return;
+            }
+    }
     check(launch_kv_reorder(k_caches, v_caches, n_layers, n_beams, beam_stride, kv_dim, row0, n_rows, parents,
                             g_rt.stream),
           where);

@@ -500,7 +500,8 @@ void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t vocab, c
  * writes them), in place, for every layer.  Beam b's cache of layer l starts
  * beam_stride * b floats behind k_caches[l] / v_caches[l]; a parent outside
  * [0, n_beams) leaves its beam as it is.  n_beams 1..32; kv_dim and
- * beam_stride multiples of 4; addresses as in gncx_hip_kv_keep_rows. */
+ * beam_stride multiples of 4; addresses as in gncx_hip_kv_keep_rows; parents
+ * lie outside the rows. */
 void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t n_beams,
                          size_t beam_stride, int32_t kv_dim, int32_t row0, int32_t n_rows, const int32_t* parents);
 

@@ -865,6 +865,21 @@ def test_reorder(lib, torch_mod, layers, beams, kv_dim, row0, rows, parents):
         assert torch.equal(got.view(torch.int32), w.view(torch.int32))
 
 
+def test_reorder_refuses_parents_within_the_caches(lib, torch_mod):
+    """The parents are read while the beams' rows are written."""
+    torch = torch_mod
+    c = torch.zeros(2, 3, 8, 64, device="cuda")  # (zeros: parents 0, wherever they are read)
+    ks, vs = addresses(c[:1]), addresses(c[1:])
+    lib.gncx_hip_last_status()
+    for at in (c[0, 0, 2], c[0, 2, 7, 60:], c[1, 1, 5]):
+        lib.gncx_hip_kv_reorder(ks, vs, 1, 3, 512, 64, 2, 6, at.data_ptr())
+        refused(lib, "parents lie")
+    before = c[:, 1].normal_().clone()
+    lib.gncx_hip_kv_reorder(ks, vs, 1, 3, 512, 64, 2, 6, c[0, 2, 1].data_ptr())  # (a row before row0)
+    gncx.check(lib)
+    assert not c[:, 1, 2:].any() and torch.equal(c[:, 1, :2], before[:, :2])
+
+
 def test_refusals_on_the_device(lib, torch_mod):
     torch = torch_mod
     lib.gncx_hip_last_status()
