@@ -719,11 +719,18 @@ class Decoder:
             tokens = [token] + [int(t) for t in tokens[:room]]
             parents = [-1] + [int(p) + 1 for p in parents[:room]]
             best = self.torch.argmax(self.verify_tree(tokens, parents, pos), dim=1).tolist()
-            path = [0]
+            # accepted: every node that is its accepted parent's greedy next token;
+            # kept: the way to the deepest (the first of them), up to n_new ids
+            depth = {0: 0}
             for i in range(1, len(tokens)):
-                if len(new) + 1 < n_new and parents[i] == path[-1] and tokens[i] == best[path[-1]]:
-                    path.append(i)
-                    new.append(tokens[i])
+                if parents[i] in depth and tokens[i] == best[parents[i]]:
+                    depth[i] = depth[parents[i]] + 1
+            node, path = max(depth, key=depth.get), []
+            while node >= 0:
+                path.insert(0, node)
+                node = parents[node]
+            path = path[:n_new - len(new)]
+            new += [tokens[i] for i in path[1:]]
             self.keep_path(pos, path)
             pos += len(path)
             token = best[path[-1]]
@@ -731,8 +738,9 @@ class Decoder:
     def beam_search(self, prompt, n_beams: int, n_new: int, end: int = -1):
         """The n_beams (at most 32) continuations of n_new tokens that beam
         search finds, [(token ids, sum of log probabilities)] in falling order; a
-        continuation that reaches the token `end` (if not negative) stays as it
-        is.  Each beam has caches of its own."""
+        continuation that reaches the token `end` (if not negative) keeps its
+        score, and its ids are filled up with `end`.  Each beam has caches of its
+        own."""
         self._device_only("beam search")
         torch, s, L, m = self.torch, self.s, self.lib, self.m
         if not 1 <= n_beams <= 32 or n_new < 1:

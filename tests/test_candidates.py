@@ -128,3 +128,42 @@ def test_lookup_draft_has_a_depth_and_a_width():
     ids = [x for i in range(10) for x in (1, 2, 10 + i, 20 + i, 30 + i)] + [1, 2]
     tokens, parents = dec.lookup_draft(ids, depth=2, width=3)
     assert (tokens, parents) == ([19, 29, 18, 28, 17, 27], [-1, 0, -1, 2, -1, 4])
+
+
+def drafted(dec, next_of, prompt, n_new, draft, max_seq=64):
+    """generate_drafted over a stand-in model whose greedy next id is next_of[id];
+    the ids, and the paths it kept."""
+    import types
+    import torch
+    logits = lambda t: torch.nn.functional.one_hot(torch.tensor(next_of[t]), len(next_of)).float()  # noqa: E731
+    kept = []
+    d = types.SimpleNamespace(torch=torch, max_seq=max_seq, prefill=lambda ids: logits(ids[-1]),
+                              greedy=lambda x: int(x.argmax()),
+                              verify_tree=lambda tokens, parents, pos: torch.stack([logits(t) for t in tokens]),
+                              keep_path=lambda pos, path: kept.append((pos, list(path))))
+    return dec.Decoder.generate_drafted(d, prompt, n_new, draft), kept
+
+
+def test_drafted_generation_takes_the_longest_of_equal_branches():
+    """Two drafted nodes of one token below the same node: the branch that is
+    accepted further is kept, whichever comes first."""
+    import gncx_amd.decode as dec
+    next_of = [1, 2, 3, 4, 5, 6, 7, 0]
+    # below the chosen token 1: the token 2 twice; below the second, 3 and 4
+    draft = lambda ids: ([2, 7, 2, 3, 4, 5], [-1, 0, -1, 2, 3, 0])  # noqa: E731
+    new, kept = drafted(dec, next_of, [0], 5, draft)
+    assert new == [1, 2, 3, 4, 5] and kept[0] == (1, [0, 3, 4, 5])
+    # equally long ones: the first
+    draft = lambda ids: ([2, 2, 3, 3], [-1, -1, 1, 0])  # noqa: E731
+    new, kept = drafted(dec, next_of, [0], 4, draft)
+    assert new == [1, 2, 3, 4] and kept[0] == (1, [0, 2, 3])
+
+
+@pytest.mark.parametrize("n_new", range(1, 9))
+def test_drafted_generation_stops_at_the_number_of_ids(n_new):
+    import gncx_amd.decode as dec
+    next_of = [1, 2, 3, 4, 5, 6, 7, 0]
+    draft = lambda ids: ([next_of[ids[-1]], 0, next_of[next_of[ids[-1]]]], [-1, 0, 0])  # noqa: E731
+    new, kept = drafted(dec, next_of, [5, 6], n_new, draft)
+    assert new == [7, 0, 1, 2, 3, 4, 5, 6][:n_new]
+    assert sum(len(p) for _, p in kept) <= n_new
