@@ -468,6 +468,41 @@ def test_tree_is_a_prefill_for_a_chain(lib, torch_mod):
     assert bool(((t.out - out).abs() <= 2 * tol).all())
 
 
+def test_tree_past_4_gib(lib, torch_mod):
+    """Cache rows past 2^32 bytes, read and written."""
+    torch = torch_mod
+    Tree(torch, 8, 8, 128, 1060000, [-1, 0, 0, 1], seed=1).verify(lib)
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("H,KV,hd", [(32, 8, 128), (4, 4, 64), (8, 2, 256)])
+@pytest.mark.parametrize("shape,sw", [("chain", 5), ("random", 40), ("random", 90), ("roots", 1)])
+def test_tree_with_a_window_is_its_branches_decoded(lib, torch_mod, H, KV, hd, shape, sw):
+    """Every node's output against a fused decode step with the same window, over
+    a cache that holds the node's branch alone."""
+    torch = torch_mod
+    pos0, n = 83, 23
+    t = Tree(torch, H, KV, hd, pos0, make_parents(shape, n), sw=sw, weight=1, base=1e6, seed=sw)
+    q, k = t.q.clone(), t.k.clone()
+    t.call(lib)
+    _, tol = t.reference()
+    d, out = depths(t.parents), torch.empty(H * hd, device="cuda")
+    for i in range(n):
+        branch, a = [], i
+        while a >= 0:
+            branch.insert(0, pos0 + a)
+            a = t.parents[a]
+        rows = list(range(pos0)) + branch
+        kc, vc = t.kc[rows].clone(), t.vc[rows].clone()
+        qi, ki = q[i].clone(), k[i].clone()
+        lib.gncx_hip_attention_step_fused(qi.data_ptr(), ki.data_ptr(), t.v[i].data_ptr(), kc.data_ptr(),
+                                          vc.data_ptr(), pos0 + d[i], H, KV, hd, t.scale, sw, 1, t.gamma.data_ptr(),
+                                          0, 4 * hd, 1, EPS, 0, 0, t.base, out.data_ptr())
+        gncx.check(lib)
+        # (both are within the bound of the 64-bit formula)
+        assert bool(((t.out[i].double() - out.double()).abs() <= 2 * tol[i]).all()), i
+
+
 def test_tree_rows_in_the_cache_itself(lib, torch_mod):
     """k_nodes and v_nodes may be the cache rows that they are stored to."""
     torch = torch_mod
