@@ -441,10 +441,13 @@ void gncx_hip_argmax(const float* values, int32_t n, int32_t* out_index);
  * one pass (speculative decoding), and beam search.  No counterpart in the
  * reference, whose streamer decodes one continuation.  Caches, vectors and
  * outputs are memory of the library's GPU, used in place and in the order of
- * the library stream, and nothing synchronises with the host (but for the
- * upload of a position's rotations, below).  Refused calls leave every output
- * as it was; refused is also what would reach past the end of the allocation
- * that a pointer lies in.
+ * the library stream.  The host waits for the GPU in three places: for the
+ * upload of a position's rotations (below), where a tree or a selection needs a
+ * larger workspace than any before it (its memory is allocated anew), and
+ * where it is issued on another library stream than the last one of its kind
+ * (the two share a workspace; captured calls have their graph's).  Refused
+ * calls leave every output as it was; refused is also what would reach past the
+ * end of the allocation that a pointer lies in.
  *
  * Attention of a drafted tree of n_nodes (1..512) tokens over the cache of the
  * first pos0 positions.  parents (host memory, read before the call returns):
