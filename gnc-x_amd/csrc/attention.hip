@@ -1649,8 +1649,8 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, T
 // "Odd" keys, whose key or value row is not finite or lies more than 2^-14 below
 // its group's largest, are kept out of the products (0 times an infinity would be
 // NaN for the rows that do not see it) and added element by element at the end,
-// from lists that the staging leaves (128 nodes at 8192, 32 heads over 4 of 128: 92
-// us without odd keys, 128 with one in a hundred, 475 with one in eight).
+// from lists that the staging leaves (128 nodes at 8192, 32 heads over 4 of 128: 79
+// us without odd keys, 109 with one value row in a hundred, 444 with one in eight).
 // Parts are left normalised, o_part = sum w v / sum w, with (m, l) beside them:
 // no sum of large values can overflow between the kernels.  The reference's
 // 1e-12 beside a sum l > 1/2 is below fp32's rounding and left out.
@@ -1832,7 +1832,8 @@ __device__ __forceinline__ float tile_softmax(const floatx16& st, const float (&
 }
 
 // Adds the weights of a tile's keys whose value rows are zeros (bits 8 + 4 g .. of
-// group h's word) to the sum, and takes them out of the tile.
+// group h's word) to the sum, and takes them out of the tile (128 nodes at 8192: 79
+// us without such rows, 84 with one in a hundred, 100 with one in eight).
 typedef uint32_t uint32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void leave_zeros(floatx16& st, const uint32x4& words, int g, RowState& s) {
     float most = -1e30f, sum = 0.0f;
@@ -1967,7 +1968,7 @@ __device__ __forceinline__ void interleave_reads() {
 // Few rows: bound by the reads of the cache (1 node at 32749, 32 heads over 8 of
 // 128: 268 MB in a call of 60 us, 4.5 TB/s).  Many: by the matrix cores and the
 // work beside them (splitting the tile, the softmax), of which a SIMD has 50 and
-// 71 thousand cycles in 131 (128 nodes at 8192, 32 over 4 of 128: 75 us, 0.69
+// 71 thousand cycles in 136 (128 nodes at 8192, 32 over 4 of 128: 75 us, 0.69
 // PFLOP/s of fp16 products; 512 nodes at 32000, 32 over 8: 0.88 to 0.93, a large
 // library product of the kind runs at 1.17).
 template <int HD, int OCC>
@@ -2287,8 +2288,8 @@ __global__ __launch_bounds__(kThreads, OCC) void tree_rows_kernel(TreeParams p) 
 }
 
 // out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the key
-// ranges c.  Bound by the read of the parts: 128 nodes at 8192, 32 heads of 128 (15
-// ranges, 33 MB) 11.3 us, 2.9 TB/s; 4 nodes at 300 (10 ranges) 2.7 us.  CG threads share a float4 of the output, each with every CG-th
+// ranges c.  Bound by the read of the parts: 128 nodes at 8192, 32 heads of 128 (16
+// ranges, 34 MB) 11.5 us, 2.9 TB/s; 4 nodes at 300 (10 ranges) 2.7 us.  CG threads share a float4 of the output, each with every CG-th
 // range, at most eight, whose loads go out at once; their sums meet in LDS.
 constexpr int kTreeMergeLoads = 8;
 template <int HD, int CG>

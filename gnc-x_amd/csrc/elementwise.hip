@@ -737,7 +737,7 @@ __global__ __launch_bounds__(64) void keep_rows_kernel(KeepParams p) {
 // is.  Bound by memory: 8 beams x 1000 rows x 1024 x 24 caches, 1.08 GB with four
 // distinct parents, 316 us with one float4 a thread and beam (too few bytes in
 // flight for its waits), 217 with four, 168 (6.4 TB/s) with stores that pass the
-// caches, too.
+// caches, too (one set of caches again and again; two in turn 210 to 229).
 struct ReorderParams {
     LayerCaches caches;
     size_t beam_stride, count;  // floats; float4 of a beam's rows
@@ -792,8 +792,8 @@ __global__ __launch_bounds__(kCandThreads) void reorder_kernel(ReorderParams p) 
 // number of better ones.  Where too many reach it (a vocabulary of equal
 // logits), the best are taken one after another instead.
 // Bound by the waits from step to step, not by bytes: 16 beams x 151936 words, 32
-// out (9.7 MB), parts 9.2 us, 1.1 TB/s, and join 8.2 (11.4 with one thread, not
-// eight, to rank a candidate); 4 x 32000, 8 out, 4.9 and 5.2.
+// out (9.7 MB), parts 9.6 us, 1.0 TB/s, and join 8.3 (11.4 with one thread, not
+// eight, to rank a candidate); 4 x 32000, 8 out, 4.8 and 4.9.
 struct SelectParams {
     const float* logits;
     const float* scores;
