@@ -1643,9 +1643,9 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, T
 // l 2^(s - max s), two running maxima a row, so that other groups that a row does
 // not see have no say in its precision.  Within a group a hidden row may set e, by
 // 2^14 above a visible one at most ("odd" keys, below), which leaves the weight of
-// the largest term at 2^-2 or more, where a pair still holds it to 2^-22.  Value rows
-// of zeros, which any e suits and which bring nothing to O, take no part in the
-// second maximum: their weights are added to l alone.
+// the largest term at 2^-2 or more: a pair still holds it to 2^-22, and every smaller
+// one to 2^-23 of it.  Value rows of zeros, which any e suits and which bring nothing
+// to O, take no part in the second maximum: their weights are added to l alone.
 // "Odd" keys, whose key or value row is not finite or lies more than 2^-14 below
 // its group's largest, are kept out of the products (0 times an infinity would be
 // NaN for the rows that do not see it) and added element by element at the end,
