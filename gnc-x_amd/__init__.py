@@ -153,6 +153,13 @@ SIGNATURES = {
     "gncx_hip_kv_keep_rows": (None, [_vp, _vp, _i32, _i32, _i32, _vp, _i32]),
     "gncx_hip_beam_select": (None, [_fp, _i32, _i32, _fp, _vp, _i32, _i32, _vp, _vp, _fp]),
     "gncx_hip_kv_reorder": (None, [_vp, _vp, _i32, _i32, _sz, _i32, _i32, _i32, _vp]),
+    "gncx_hip_rope_frequencies": (
+        C.c_int, [_i32, C.c_double, _i32, C.c_double, _i32, C.c_double, C.c_double, _fp, _vp, _vp]),
+    "gncx_hip_rope_rows": (None, [_fp, _i32, _i32, _i32, _i32, _vp, _vp, _i32, _fp]),
+    "gncx_hip_kv_append_paged": (
+        None, [_vp, _vp, _fp, _fp, _fp, _i32, _vp, _sz, _sz, _i32, _f32, _vp, _fp]),
+    "gncx_hip_attention_paged": (None, [_vp, _vp, _fp, _i32, _f32, _i32, _fp]),
+    "gncx_hip_token_logprobs": (None, [_fp, _i32, _i32, _vp, _i32, _fp, _fp, _vp, _fp]),
     "gncx_hip_set_host_coherence": (C.c_int, [C.c_int]),
     "gncx_hip_host_flush": (None, [_vp]),
 }
@@ -181,6 +188,25 @@ class DecodeState(C.Structure):
                [(n, C.c_void_p) for n in ("q", "k", "v", "attn", "proj", "normed", "gate", "up", "act", "logits")] + \
                [("k_cache", C.POINTER(C.c_void_p)), ("v_cache", C.POINTER(C.c_void_p)), ("max_seq", C.c_int32),
                 ("token", C.c_void_p), ("token_log", C.c_void_p)]
+
+
+# ctypes mirrors of the paged cache's structs
+class PagedCache(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("k_pages", "v_pages", "scales")] + \
+               [(n, C.c_int32) for n in ("n_pages", "page_tokens", "n_kv_heads", "head_dim")]
+
+
+class PagedBatch(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_seqs", "n_rows", "max_pages")] + \
+               [(n, C.c_void_p) for n in ("row_start", "lengths", "pages")]
+
+
+class Rotation(C.Structure):
+    _fields_ = [("freqs", C.c_void_p), ("n_rot", C.c_int32), ("interleaved", C.c_int32), ("magnitude", C.c_float)]
+
+
+# scalings of gncx_hip_rope_frequencies
+ROPE_PLAIN, ROPE_LINEAR, ROPE_BASE, ROPE_YARN = range(4)
 
 
 class GncxLibraryMissing(RuntimeError):

@@ -871,6 +871,76 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     return v;
 }
 
+// The n_out best of the words that a work-group holds (thread tid's words: v0 + 1024 j +
+// i), in two steps with a barrier between them: those that reach `least`
+// (nth_largest's of the threads' maxima) go to LDS, held being 0 before a barrier, then
+// the best go to `best` in falling order, -inf behind the last.
+struct PartWords {
+    uint64_t keys[kMostRanked];
+    uint64_t redk[kCandThreads / 64];
+    int held;
+};
+template <int V>
+__device__ __forceinline__ void gather_words(const float (&x)[V][4], int v0, float least, PartWords& sh) {
+    int mine = 0;
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mine += x[j][i] >= least && x[j][i] > -__builtin_inff();
+    if (mine) {
+        int at = atomicAdd(&sh.held, mine);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (x[j][i] >= least && x[j][i] > -__builtin_inff()) {
+                    if (at < kMostRanked) sh.keys[at] = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
+                    ++at;
+                }
+    }
+}
+template <int V>
+__device__ __forceinline__ void rank_words(const float (&x)[V][4], int v0, int n_out, float2* best, PartWords& sh) {
+    constexpr int kWavesHere = kCandThreads / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int n = sh.held;
+    if (n <= kMostRanked) {
+        for (int i = tid; i < n; i += kCandThreads) {
+            const uint64_t k = sh.keys[i];
+            int rank = 0;
+#pragma unroll 8
+            for (int o = 0; o < n; ++o) rank += sh.keys[o] > k;
+            if (rank < n_out)
+                best[rank] = make_float2(unordered(static_cast<uint32_t>(k >> 32)),
+                                         __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
+        }
+        for (int i = n + tid; i < n_out; i += kCandThreads) best[i] = make_float2(-__builtin_inff(), 0.0f);
+        return;
+    }
+    uint64_t last = ~uint64_t{0};
+    for (int r = 0; r < n_out; ++r) {
+        uint64_t k = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint64_t o = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
+                if (x[j][i] > -__builtin_inff() && o < last && o > k) k = o;
+            }
+        k = wave_max_u64(k);
+        __syncthreads();
+        if (lane == 0) sh.redk[wv] = k;
+        __syncthreads();
+        k = sh.redk[0];
+#pragma unroll
+        for (int w = 1; w < kWavesHere; ++w) k = sh.redk[w] > k ? sh.redk[w] : k;
+        if (tid == 0)
+            best[r] = make_float2(k ? unordered(static_cast<uint32_t>(k >> 32)) : -__builtin_inff(),
+                                  __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
+        last = k;
+    }
+}
+
 // A work-group holds 1024 V words of one beam in registers.
 template <int V>
 __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams p) {
@@ -878,9 +948,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
     constexpr int kWavesHere = kCandThreads / 64;
     __shared__ __align__(16) float maxima[kGroups];
     __shared__ double sums[kWavesHere];
-    __shared__ uint64_t keys[kMostRanked];
-    __shared__ uint64_t redk[kWavesHere];
-    __shared__ int held;
+    __shared__ PartWords sh;
     const int b = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     if (p.finished && p.finished[b]) return;
     const int v0 = c * 1024 * V + 4 * tid;  // this thread's words: v0 + 1024 j + i
@@ -906,7 +974,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
             most = fmaxf(most, x[j][i]);
         }
     maxima[tid] = most;
-    if (tid == 0) held = 0;
+    if (tid == 0) sh.held = 0;
     __syncthreads();
     // (the first maximum of the search is the part's)
     float m;
@@ -928,22 +996,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
     l = wave_sum_f64(l);
     if (lane == 0) sums[wv] = l;
     const float least = nth_largest(maxima, p.n_out, lane);
-    int mine = 0;
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mine += x[j][i] >= least && x[j][i] > -__builtin_inff();
-    if (mine) {
-        int at = atomicAdd(&held, mine);
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (x[j][i] >= least && x[j][i] > -__builtin_inff()) {
-                    if (at < kMostRanked) keys[at] = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
-                    ++at;
-                }
-    }
+    gather_words(x, v0, least, sh);
     __syncthreads();
     const size_t part = static_cast<size_t>(b) * p.n_chunks + c;
     float2* best = p.best + part * p.n_out;
@@ -953,42 +1006,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
         for (int w = 1; w < kWavesHere; ++w) s += sums[w];
         p.ml[part] = make_double2(m, s);
     }
-    const int n = held;
-    if (n <= kMostRanked) {
-        for (int i = tid; i < n; i += kCandThreads) {
-            const uint64_t k = keys[i];
-            int rank = 0;
-#pragma unroll 8
-            for (int o = 0; o < n; ++o) rank += keys[o] > k;
-            if (rank < p.n_out)
-                best[rank] = make_float2(unordered(static_cast<uint32_t>(k >> 32)),
-                                         __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
-        }
-        for (int i = n + tid; i < p.n_out; i += kCandThreads) best[i] = make_float2(-__builtin_inff(), 0.0f);
-        return;
-    }
-    uint64_t last = ~uint64_t{0};
-    for (int r = 0; r < p.n_out; ++r) {
-        uint64_t k = 0;
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint64_t o = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
-                if (x[j][i] > -__builtin_inff() && o < last && o > k) k = o;
-            }
-        k = wave_max_u64(k);
-        __syncthreads();
-        if (lane == 0) redk[wv] = k;
-        __syncthreads();
-        k = redk[0];
-#pragma unroll
-        for (int w = 1; w < kWavesHere; ++w) k = redk[w] > k ? redk[w] : k;
-        if (tid == 0)
-            best[r] = make_float2(k ? unordered(static_cast<uint32_t>(k >> 32)) : -__builtin_inff(),
-                                  __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
-        last = k;
-    }
+    rank_words(x, v0, p.n_out, best, sh);
 }
 
 // The order of equal scores: the lower beam, then the larger logit (64 bits may not
@@ -1142,6 +1160,230 @@ int32_t select_vectors(int32_t n_beams, int32_t vocab) {
     return v;
 }
 
+// ---- log probabilities ----------------------------------------------------------------
+// log p(v) = x_v - m - log S and H = log S - T / S, with S the sum of e^(x - m) and T that
+// of e^(x - m) (x - m).  As in beam search's selection, a work-group holds a part of
+// a row in registers and leaves its maximum, its two sums and its n_top best; a second
+// kernel joins the parts of a row.  A row of one part is finished by the first.
+struct LogprobParams {
+    const float* logits;
+    const int32_t* tokens;  // null: no out_logprobs
+    int32_t vocab, n_top, n_chunks;
+    double* sums;  // [row][chunk][3] maximum, S, T
+    float2* best;  // [row][chunk][n_top] logit, word (as bits), in falling order; -inf behind the last
+    float* out_logprobs;
+    float* out_entropy;
+    int32_t* out_top_tokens;
+    float* out_top_logprobs;
+};
+
+// A row's log probabilities from its maximum and sums
+struct RowSums {
+    float m;
+    double log_s;
+    __device__ float logprob(float x) const {
+        if (!(x > -__builtin_inff())) return -__builtin_inff();
+        return static_cast<float>((x == m ? 0.0 : static_cast<double>(x) - static_cast<double>(m)) - log_s);
+    }
+};
+__device__ __forceinline__ void finish_row(const LogprobParams& p, size_t row, const RowSums& r, double s, double t) {
+    if (p.tokens) {
+        const int32_t w = p.tokens[row];
+        const bool in = w >= 0 && w < p.vocab;
+        const float x = in ? clean(p.logits[row * p.vocab + w]) : -__builtin_inff();
+        p.out_logprobs[row] = r.logprob(x);
+    }
+    if (p.out_entropy) p.out_entropy[row] = s > 0.0 ? static_cast<float>(r.log_s - t / s) : 0.0f;
+}
+__device__ __forceinline__ void finish_top(const LogprobParams& p, size_t row, const RowSums& r, int i, float2 e) {
+    const bool in = e.x > -__builtin_inff();
+    p.out_top_tokens[row * p.n_top + i] = in ? __builtin_bit_cast(int32_t, e.y) : -1;
+    p.out_top_logprobs[row * p.n_top + i] = r.logprob(e.x);
+}
+
+template <int V>
+__global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobParams p) {
+    typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int kWavesHere = kCandThreads / 64;
+    __shared__ __align__(16) float maxima[kGroups];
+    __shared__ double sums[kWavesHere][2];
+    __shared__ PartWords sh;
+    __shared__ float2 tops[kMaxTopWords];
+    const size_t b = blockIdx.x / p.n_chunks;
+    const int c = blockIdx.x % p.n_chunks, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int v0 = c * 1024 * V + 4 * tid;  // this thread's words: v0 + 1024 j + i
+    const float* row = p.logits + b * p.vocab;
+    float x[V][4], most = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const int at = v0 + 1024 * j;
+        if (at + 4 <= p.vocab) {
+            const float4a4 w = *reinterpret_cast<const float4a4*>(row + at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] = w[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[j][i] = at + i < p.vocab ? row[at + i] : -__builtin_inff();
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[j][i] = clean(x[j][i]);
+            most = fmaxf(most, x[j][i]);
+        }
+    maxima[tid] = most;
+    if (tid == 0) sh.held = 0;
+    __syncthreads();
+    float m;
+    {
+        const float4 w = reinterpret_cast<const float4*>(maxima)[lane];
+        m = wave_max(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
+    }
+    double s = 0.0, t = 0.0;
+    if (m > -__builtin_inff())
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float e[4], f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // (x == m: an infinite maximum; below -104 the exponential is 0)
+                const float d = x[j][i] == m ? 0.0f : fmaxf(x[j][i] - m, -200.0f);
+                e[i] = expf(d);
+                f[i] = e[i] * d;
+            }
+            s += (static_cast<double>(e[0]) + e[1]) + (static_cast<double>(e[2]) + e[3]);
+            t += (static_cast<double>(f[0]) + f[1]) + (static_cast<double>(f[2]) + f[3]);
+        }
+    s = wave_sum_f64(s);
+    t = wave_sum_f64(t);
+    if (lane == 0) {
+        sums[wv][0] = s;
+        sums[wv][1] = t;
+    }
+    if (p.n_top) gather_words(x, v0, nth_largest(maxima, p.n_top, lane), sh);
+    __syncthreads();
+    const size_t part = blockIdx.x;
+    const bool whole = p.n_chunks == 1;
+    s = sums[0][0];
+    t = sums[0][1];
+#pragma unroll
+    for (int w = 1; w < kWavesHere; ++w) {
+        s += sums[w][0];
+        t += sums[w][1];
+    }
+    const RowSums r{m, log(s)};
+    if (tid == 0) {
+        if (whole) {
+            finish_row(p, b, r, s, t);
+        } else {
+            p.sums[3 * part] = m;
+            p.sums[3 * part + 1] = s;
+            p.sums[3 * part + 2] = t;
+        }
+    }
+    if (p.n_top == 0) return;
+    rank_words(x, v0, p.n_top, whole ? tops : p.best + part * p.n_top, sh);
+    if (!whole) return;
+    __syncthreads();
+    if (tid < p.n_top) finish_top(p, b, r, tid, tops[tid]);
+}
+
+__global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParams p) {
+    __shared__ __align__(16) float maxima[kGroups];
+    __shared__ PartWords sh;
+    const size_t row = blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, parts = p.n_chunks;
+    const double* sums = p.sums + 3 * row * parts;
+    const float2* best = p.best + row * parts * p.n_top;
+    // every wave: the parts' maxima and sums
+    float m = -__builtin_inff();
+    for (int c = lane; c < parts; c += 64) m = fmaxf(m, static_cast<float>(sums[3 * c]));
+    m = wave_max(m);
+    double s = 0.0, t = 0.0;
+    for (int c = lane; c < parts; c += 64) {
+        const double mc = sums[3 * c];
+        if (mc > -__builtin_inff()) {
+            const double d = mc == m ? 0.0 : mc - m, f = exp(d);
+            s += f * sums[3 * c + 1];
+            t += f * (sums[3 * c + 2] + (f > 0.0 ? d * sums[3 * c + 1] : 0.0));
+        }
+    }
+    s = wave_sum_f64(s);
+    t = wave_sum_f64(t);
+    const RowSums r{m, log(s)};
+    if (tid == 0) {
+        finish_row(p, row, r, s, t);
+        sh.held = 0;
+    }
+    if (p.n_top == 0) return;
+    // The parts' lists fall: a threshold from their first 2^shift entries, and a list
+    // is read on only while it stays above.
+    int shift = 0;
+    while (parts << shift < kGroups && 1 << shift < p.n_top) ++shift;
+    const int first = 1 << shift;
+    float most = -__builtin_inff();
+    for (int j = tid; j < parts << shift; j += kGroups)
+        if ((j & (first - 1)) < p.n_top) most = fmaxf(most, best[static_cast<size_t>(j >> shift) * p.n_top + (j & (first - 1))].x);
+    maxima[tid] = most;
+    __syncthreads();
+    const float least = nth_largest(maxima, p.n_top, lane);
+    const int wide = max(shift, 3), batch = 1 << wide;
+    for (int j = tid; j < parts << wide; j += kCandThreads)
+        for (int i = j & (batch - 1); i < p.n_top; ++i) {
+            const float2 e = best[static_cast<size_t>(j >> wide) * p.n_top + i];
+            if (!(e.x > -__builtin_inff() && e.x >= least)) break;
+            const int at = atomicAdd(&sh.held, 1);
+            if (at < kMostRanked) sh.keys[at] = key_of(e.x, __builtin_bit_cast(uint32_t, e.y));
+            if (i < batch - 1) break;
+        }
+    __syncthreads();
+    auto word_of = [](uint64_t k) {
+        return make_float2(unordered(static_cast<uint32_t>(k >> 32)), __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
+    };
+    const int n = sh.held;
+    if (n <= kMostRanked) {
+        // eight threads a candidate
+        for (int i = tid / 8; i < n; i += kCandThreads / 8) {
+            const uint64_t k = sh.keys[i];
+            int rank = 0;
+#pragma unroll 4
+            for (int o = tid % 8; o < n; o += 8) rank += sh.keys[o] > k;
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) rank += __shfl_xor(rank, d, 8);
+            if (tid % 8 == 0 && rank < p.n_top) finish_top(p, row, r, rank, word_of(k));
+        }
+        for (int i = n + tid; i < p.n_top; i += kCandThreads) finish_top(p, row, r, i, make_float2(-__builtin_inff(), 0.0f));
+        return;
+    }
+    uint64_t last = ~uint64_t{0};
+    for (int i = 0; i < p.n_top; ++i) {
+        uint64_t k = 0;
+        for (int j = tid; j < parts * p.n_top; j += kCandThreads) {
+            const float2 e = best[j];
+            const uint64_t o = key_of(e.x, __builtin_bit_cast(uint32_t, e.y));
+            if (e.x > -__builtin_inff() && o < last && o > k) k = o;
+        }
+        k = wave_max_u64(k);
+        __syncthreads();
+        if (lane == 0) sh.redk[wv] = k;
+        __syncthreads();
+        k = sh.redk[0];
+#pragma unroll
+        for (int w = 1; w < kCandThreads / 64; ++w) k = sh.redk[w] > k ? sh.redk[w] : k;
+        if (tid == 0) finish_top(p, row, r, i, k ? word_of(k) : make_float2(-__builtin_inff(), 0.0f));
+        last = k;
+    }
+}
+
+// float4 of a thread: the fewest that leave 512 parts over all rows
+int32_t logprob_vectors(int32_t n_rows, int32_t vocab) {
+    int32_t v = 2;
+    while (v < 16 && static_cast<int64_t>(n_rows) * ((vocab + 1024 * v - 1) / (1024 * v)) > 512) v *= 2;
+    return v;
+}
+
 template <class F>
 hipError_t by_layers(float* const* k, float* const* v, int32_t n_layers, F&& launch) {
     for (int32_t l0 = 0; l0 < n_layers; l0 += kLayerGroup) {
@@ -1251,6 +1493,43 @@ hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t voca
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL(select_join_kernel, dim3(1), dim3(kJoinThreads), 0, stream, p);
+    return hipGetLastError();
+}
+
+size_t token_logprobs_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t n_top) {
+    const int32_t words = 1024 * logprob_vectors(n_rows, vocab), chunks = (vocab + words - 1) / words;
+    return chunks == 1 ? 0 : static_cast<size_t>(n_rows) * chunks * (3 * sizeof(double) + sizeof(float2) * n_top);
+}
+
+hipError_t launch_token_logprobs(const float* logits, int32_t n_rows, int32_t vocab, const int32_t* tokens,
+                                 int32_t n_top, float* out_logprobs, float* out_entropy, int32_t* out_top_tokens,
+                                 float* out_top_logprobs, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (n_rows < 1 || vocab < 1 || vocab > kMaxBeamVocab || n_top < 0 || n_top > kMaxTopWords ||
+        workspace_bytes < token_logprobs_workspace_bytes(n_rows, vocab, n_top))
+        return hipErrorInvalidValue;
+    const int32_t v = logprob_vectors(n_rows, vocab);
+    LogprobParams p{};
+    p.logits = logits;
+    p.tokens = tokens;
+    p.vocab = vocab;
+    p.n_top = n_top;
+    p.n_chunks = (vocab + 1024 * v - 1) / (1024 * v);
+    const int64_t parts = static_cast<int64_t>(n_rows) * p.n_chunks;
+    if (parts > 0x7fffffff) return hipErrorInvalidValue;
+    p.sums = static_cast<double*>(workspace);
+    p.best = reinterpret_cast<float2*>(p.sums + 3 * parts);
+    p.out_logprobs = out_logprobs;
+    p.out_entropy = out_entropy;
+    p.out_top_tokens = out_top_tokens;
+    p.out_top_logprobs = out_top_logprobs;
+    const dim3 grid(static_cast<uint32_t>(parts));
+    if (v == 2) hipLaunchKernelGGL(logprob_parts_kernel<2>, grid, dim3(kCandThreads), 0, stream, p);
+    else if (v == 4) hipLaunchKernelGGL(logprob_parts_kernel<4>, grid, dim3(kCandThreads), 0, stream, p);
+    else if (v == 8) hipLaunchKernelGGL(logprob_parts_kernel<8>, grid, dim3(kCandThreads), 0, stream, p);
+    else hipLaunchKernelGGL(logprob_parts_kernel<16>, grid, dim3(kCandThreads), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.n_chunks == 1) return e;
+    hipLaunchKernelGGL(logprob_join_kernel, dim3(n_rows), dim3(kCandThreads), 0, stream, p);
     return hipGetLastError();
 }
 

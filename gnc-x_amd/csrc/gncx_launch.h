@@ -211,6 +211,61 @@ hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t voca
                               int32_t* out_tokens, float* out_scores, void* workspace, size_t workspace_bytes,
                               hipStream_t stream);
 
+// Rotary positions of rows (n_rot even, up to head_dim): see GNCXRotation.
+struct RotationArgs {
+    const double* freqs;  // device [n_rot / 2]
+    int32_t n_rot, interleaved;
+    float magnitude;
+};
+hipError_t launch_rope_rows(const float* rows, int32_t n_rows, int32_t row_stride, int32_t n_heads, int32_t head_dim,
+                            const int32_t* positions, const RotationArgs& rot, int32_t out_stride, float* out,
+                            hipStream_t stream);
+
+// A layer's paged cache of 16-token blocks in e4m3 and the sequences of a call:
+// see GNCXPagedCache and GNCXPagedBatch.
+constexpr int32_t kKvBlock = 16;
+constexpr int32_t kMaxSeqs = 65536;
+struct PagedArgs {
+    uint8_t* k_pages;
+    uint8_t* v_pages;
+    float* scales;
+    int32_t n_pages, page_tokens, n_kv, head_dim;
+    int32_t n_seqs, n_rows, max_pages;
+    const int32_t* row_start;
+    const int32_t* lengths;
+    const int32_t* pages;
+};
+struct AppendArgs {
+    PagedArgs c;
+    const float* q;  // null: no queries
+    const float* k;
+    const float* v;
+    float* out_q;
+    int32_t n_heads, norm;  // norm: 1 per-head RMSNorm of q and k
+    const float* q_gamma;   // may be null (no weight)
+    const float* k_gamma;
+    float eps;
+    RotationArgs rot;
+};
+hipError_t launch_kv_append_paged(const AppendArgs& a, hipStream_t stream);
+struct PagedAttnArgs {
+    PagedArgs c;
+    const float* q;
+    float* out;
+    int32_t n_heads, sliding_window;
+    float scale;
+};
+size_t attention_paged_workspace_bytes(const PagedAttnArgs& a);
+hipError_t launch_attention_paged(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+// Log probabilities of tokens, entropies and the n_top best words of rows of
+// logits; tokens / out_logprobs, out_entropy and the top outputs may be null.
+constexpr int32_t kMaxTopWords = 64;
+size_t token_logprobs_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t n_top);
+hipError_t launch_token_logprobs(const float* logits, int32_t n_rows, int32_t vocab, const int32_t* tokens,
+                                 int32_t n_top, float* out_logprobs, float* out_entropy, int32_t* out_top_tokens,
+                                 float* out_top_logprobs, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 // Per-head RMSNorm in place (reference cpp:895-953); gamma may be null.
 hipError_t launch_rmsnorm_heads(float* v, const float* gamma, int32_t n_heads, int32_t head_dim,
                                 float eps, hipStream_t stream);

@@ -3274,6 +3274,302 @@ GNCX_API void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches
           where);
 }
 
+// ---- many sequences at once ---------------------------------------------------
+// Rotary positions, the paged cache of 8-bit blocks and the attention over it, and
+// log probabilities: device pointers only, nothing read back to the host.
+
+namespace {
+
+SharedWorkspace g_paged_ws, g_logprob_ws;
+
+constexpr int64_t kMaxPositions = int64_t{1} << 30;
+
+// A rotation of heads of head_dim floats; null is none.
+bool rotation_args(const GNCXRotation* rot, int32_t head_dim, int32_t multiple, RotationArgs& a, const char* where,
+                   Allocations& seen) {
+    a = RotationArgs{nullptr, 0, 0, 1.0f};
+    if (!rot || rot->n_rot == 0) return true;
+    if (rot->n_rot < 0 || rot->n_rot % multiple || rot->n_rot > head_dim) {
+        set_error(where, ("n_rot must be a multiple of " + std::to_string(multiple) + " up to head_dim").c_str(), -1);
+        return false;
+    }
+    if (!on_device(rot->freqs, sizeof(double) * (rot->n_rot / 2), "the rotation's freqs", where, seen, 8)) return false;
+    a = RotationArgs{rot->freqs, rot->n_rot, rot->interleaved != 0, rot->magnitude};
+    return true;
+}
+
+// an array of a call, for the checks that no two overlap
+struct Span {
+    const void* p;
+    size_t bytes;
+};
+bool apart(std::initializer_list<Span> written, std::initializer_list<Span> others, const char* where) {
+    for (auto w = written.begin(); w != written.end(); ++w) {
+        for (auto o = w + 1; o != written.end(); ++o)
+            if (w->p && o->p && overlaps(w->p, w->bytes, o->p, o->bytes)) {
+                set_error(where, "two of the outputs overlap", -1);
+                return false;
+            }
+        for (const Span& o : others)
+            if (w->p && o.p && overlaps(w->p, w->bytes, o.p, o.bytes)) {
+                set_error(where, "an output overlaps an input", -1);
+                return false;
+            }
+    }
+    return true;
+}
+
+struct PagedSizes {
+    size_t codes, scales, row_start, lengths, pages;
+};
+// What needs no device: the geometry of the cache and of the batch.
+bool paged_geometry(const GNCXPagedCache* c, const GNCXPagedBatch* b, int32_t n_heads, PagedArgs& a, PagedSizes& z,
+                    const char* where) {
+    if (!c || !b) {
+        set_error(where, "no cache or batch", -1);
+        return false;
+    }
+    const int32_t pt = c->page_tokens;
+    if ((c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) || c->n_kv_heads < 1 || c->n_kv_heads > 65535 ||
+        n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv_heads || c->n_pages < 1 ||
+        (pt != 16 && pt != 32 && pt != 64 && pt != 128 && pt != 256)) {
+        set_error(where, "invalid cache geometry (head_dim is 64, 128 or 256, page_tokens 16, 32, 64, 128 or 256)", -1);
+        return false;
+    }
+    if (b->n_seqs < 1 || b->n_seqs > kMaxSeqs || b->n_rows < 0 || b->max_pages < 1 ||
+        static_cast<int64_t>(b->max_pages) * pt > kMaxPositions ||
+        static_cast<int64_t>(b->n_rows) * n_heads > INT32_MAX) {
+        set_error(where, "invalid batch (1 to 65536 sequences, up to 2^30 positions, n_rows * n_heads below 2^31)", -1);
+        return false;
+    }
+    a = PagedArgs{c->k_pages, c->v_pages, c->scales, c->n_pages, pt,        c->n_kv_heads, c->head_dim,
+                  b->n_seqs,  b->n_rows,  b->max_pages, b->row_start, b->lengths, b->pages};
+    const size_t blocks = static_cast<size_t>(c->n_pages) * c->n_kv_heads * (pt / kKvBlock);
+    z.codes = blocks * kKvBlock * c->head_dim;
+    z.scales = blocks * 2 * sizeof(float);
+    z.row_start = sizeof(int32_t) * (static_cast<size_t>(b->n_seqs) + 1);
+    z.lengths = sizeof(int32_t) * static_cast<size_t>(b->n_seqs);
+    z.pages = sizeof(int32_t) * static_cast<size_t>(b->n_seqs) * b->max_pages;
+    return true;
+}
+bool paged_pointers(const PagedArgs& a, const PagedSizes& z, const char* where, Allocations& seen) {
+    return on_device(a.k_pages, z.codes, "k_pages", where, seen, 16) &&
+           on_device(a.v_pages, z.codes, "v_pages", where, seen, 16) &&
+           on_device(a.scales, z.scales, "scales", where, seen, 8) &&
+           on_device(a.row_start, z.row_start, "row_start", where, seen) &&
+           on_device(a.lengths, z.lengths, "lengths", where, seen) &&
+           on_device(a.pages, z.pages, "pages", where, seen);
+}
+
+}  // namespace
+
+GNCX_API int gncx_hip_rope_frequencies(int32_t n_rot, double base, int32_t scaling, double factor,
+                                       int32_t trained_context, double beta_fast, double beta_slow,
+                                       const float* factors, double* out_freqs, float* out_magnitude) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_rope_frequencies";
+    const bool yarn = scaling == GNCX_ROPE_YARN;
+    const auto positive = [](double v) { return v > 0.0 && std::isfinite(v); };
+    if (n_rot < 2 || n_rot % 2 || n_rot > 1024 || !positive(base) || scaling < GNCX_ROPE_PLAIN ||
+        scaling > GNCX_ROPE_YARN || (scaling != GNCX_ROPE_PLAIN && !positive(factor)) ||
+        (scaling == GNCX_ROPE_BASE && n_rot == 2) ||
+        (yarn && (trained_context < 1 || base <= 1.0 || !positive(beta_fast) || !positive(beta_slow)))) {
+        set_error(where, "n_rot is even, 2 to 1024; base, factor and betas are positive; the scaling is one of four", -1);
+        return -1;
+    }
+    if (!out_freqs || (yarn && !out_magnitude)) {
+        set_error(where, "no output", -1);
+        return -1;
+    }
+    const int32_t half = n_rot / 2;
+    std::array<float, 512> fac{};
+    if (factors) {
+        if (is_device_ptr(factors)) {
+            if (!check(hipMemcpy(fac.data(), factors, sizeof(float) * half, hipMemcpyDeviceToHost), where)) return -1;
+        } else {
+            std::memcpy(fac.data(), factors, sizeof(float) * half);
+        }
+    }
+    if (scaling == GNCX_ROPE_BASE) base *= std::pow(factor, static_cast<double>(n_rot) / (n_rot - 2));
+    // the pair that turns `turns` times within the trained context
+    const auto pair_of = [&](double turns) {
+        return n_rot * std::log(trained_context / (turns * 2.0 * M_PI)) / (2.0 * std::log(base));
+    };
+    double low = 0.0, high = 0.0;
+    if (yarn) {
+        low = std::max(std::floor(pair_of(beta_fast)), 0.0);
+        high = std::min(std::ceil(pair_of(beta_slow)), static_cast<double>(n_rot - 1));
+    }
+    std::array<double, 512> f{};
+    for (int32_t i = 0; i < half; ++i) {
+        f[i] = std::pow(base, -2.0 * i / n_rot);
+        if (scaling == GNCX_ROPE_LINEAR) f[i] /= factor;
+        if (yarn) {
+            const double ramp = std::min(std::max((i - low) / std::max(0.001, high - low), 0.0), 1.0);
+            f[i] = f[i] / factor * ramp + f[i] * (1.0 - ramp);
+        }
+        if (factors && fac[i] != 0.0f) f[i] /= fac[i];
+    }
+    if (is_device_ptr(out_freqs)) {
+        if (!check(hipMemcpy(out_freqs, f.data(), sizeof(double) * half, hipMemcpyHostToDevice), where)) return -1;
+    } else {
+        std::memcpy(out_freqs, f.data(), sizeof(double) * half);
+    }
+    if (out_magnitude) *out_magnitude = yarn ? static_cast<float>(0.1 * std::log(factor) + 1.0) : 1.0f;
+    return 0;
+}
+
+GNCX_API void gncx_hip_rope_rows(const float* rows, int32_t n_rows, int32_t row_stride, int32_t n_heads,
+                                 int32_t head_dim, const int32_t* positions, const GNCXRotation* rotation,
+                                 int32_t out_stride, float* out_rows) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_rope_rows";
+    if (n_rows == 0) return;
+    if (n_rows < 0 || n_heads < 1 || head_dim < 2 || head_dim % 2 || head_dim > 1024 || n_heads > 65535 ||
+        static_cast<int64_t>(n_heads) * head_dim > std::min(row_stride, out_stride)) {
+        set_error(where, "head_dim is even, 2 to 1024, and a row's heads fit its strides", -1);
+        return;
+    }
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    Allocations seen;
+    RotationArgs rot;
+    const auto bytes = [&](int32_t stride) {
+        return sizeof(float) * (static_cast<size_t>(n_rows - 1) * stride + static_cast<size_t>(n_heads) * head_dim);
+    };
+    const size_t in = bytes(row_stride), out = bytes(out_stride), at = sizeof(int32_t) * static_cast<size_t>(n_rows);
+    if (!rotation_args(rotation, head_dim, 2, rot, where, seen) || !on_device(rows, in, "rows", where, seen) ||
+        !on_device(positions, at, "positions", where, seen) || !on_device(out_rows, out, "out_rows", where, seen) ||
+        !apart({{out_rows, out}}, {{positions, at}, {rot.freqs, sizeof(double) * (rot.n_rot / 2)}}, where))
+        return;
+    if (!(rows == out_rows && row_stride == out_stride) && !apart({{out_rows, out}}, {{rows, in}}, where)) return;
+    check(launch_rope_rows(rows, n_rows, row_stride, n_heads, head_dim, positions, rot, out_stride, out_rows,
+                           g_rt.stream),
+          where);
+}
+
+GNCX_API void gncx_hip_kv_append_paged(const GNCXPagedCache* cache, const GNCXPagedBatch* batch, const float* q_rows,
+                                       const float* k_rows, const float* v_rows, int32_t n_heads,
+                                       const uint8_t* mmap_base, size_t q_norm_offset, size_t k_norm_offset,
+                                       int32_t has_norm_weight, float norm_eps, const GNCXRotation* rotation,
+                                       float* out_q) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_kv_append_paged";
+    AppendArgs a{};
+    PagedSizes z;
+    if (!paged_geometry(cache, batch, n_heads, a.c, z, where)) return;
+    if (has_norm_weight > 0 && !mmap_base) {
+        set_error(where, "no norm weights", -1);
+        return;
+    }
+    if (a.c.n_rows == 0) return;
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    const int32_t hd = a.c.head_dim;
+    const size_t row = sizeof(float) * static_cast<size_t>(a.c.n_rows) * hd, qb = row * n_heads, kb = row * a.c.n_kv;
+    Allocations seen;
+    if (!paged_pointers(a.c, z, where, seen) || !rotation_args(rotation, hd, 8, a.rot, where, seen) ||
+        !on_device(k_rows, kb, "k_rows", where, seen, 16) || !on_device(v_rows, kb, "v_rows", where, seen, 16) ||
+        (q_rows && (!on_device(q_rows, qb, "q_rows", where, seen, 16) || !on_device(out_q, qb, "out_q", where, seen, 16))))
+        return;
+    const Span q{q_rows == out_q ? nullptr : q_rows, qb}, out{q_rows ? out_q : nullptr, qb};
+    if (!apart({{a.c.k_pages, z.codes}, {a.c.v_pages, z.codes}, {a.c.scales, z.scales}, out},
+               {q, {k_rows, kb}, {v_rows, kb}, {a.c.row_start, z.row_start}, {a.c.lengths, z.lengths},
+                {a.c.pages, z.pages}, {a.rot.freqs, sizeof(double) * (a.rot.n_rot / 2)}},
+               where))
+        return;
+    a.q = q_rows;
+    a.k = k_rows;
+    a.v = v_rows;
+    a.out_q = out_q;
+    a.n_heads = n_heads;
+    a.norm = has_norm_weight >= 0;
+    a.eps = norm_eps;
+    if (has_norm_weight > 0) {
+        const size_t bytes = sizeof(float) * static_cast<size_t>(hd);
+        a.k_gamma = reinterpret_cast<const float*>(device_weights(mmap_base + k_norm_offset, bytes, where));
+        if (!a.k_gamma) return;
+        if (q_rows) {
+            a.q_gamma = reinterpret_cast<const float*>(device_weights(mmap_base + q_norm_offset, bytes, where));
+            if (!a.q_gamma) return;
+        }
+        if ((reinterpret_cast<uintptr_t>(a.k_gamma) | reinterpret_cast<uintptr_t>(a.q_gamma)) % 16) {
+            set_error(where, "norm weights must be 16-byte aligned", -1);
+            return;
+        }
+    }
+    check(launch_kv_append_paged(a, g_rt.stream), where);
+}
+
+GNCX_API void gncx_hip_attention_paged(const GNCXPagedCache* cache, const GNCXPagedBatch* batch, const float* q_rows,
+                                       int32_t n_heads, float attn_scale, int32_t sliding_window, float* out_rows) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_attention_paged";
+    PagedAttnArgs a{};
+    PagedSizes z;
+    if (!paged_geometry(cache, batch, n_heads, a.c, z, where)) return;
+    if (a.c.n_rows == 0) return;
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    const size_t qb = sizeof(float) * static_cast<size_t>(a.c.n_rows) * n_heads * a.c.head_dim;
+    Allocations seen;
+    if (!paged_pointers(a.c, z, where, seen) || !on_device(q_rows, qb, "q_rows", where, seen, 16) ||
+        !on_device(out_rows, qb, "out_rows", where, seen, 16) ||
+        !apart({{out_rows, qb}},
+               {{q_rows, qb}, {a.c.k_pages, z.codes}, {a.c.v_pages, z.codes}, {a.c.scales, z.scales},
+                {a.c.row_start, z.row_start}, {a.c.lengths, z.lengths}, {a.c.pages, z.pages}},
+               where))
+        return;
+    a.q = q_rows;
+    a.out = out_rows;
+    a.n_heads = n_heads;
+    a.sliding_window = sliding_window;
+    a.scale = attn_scale;
+    const size_t need = attention_paged_workspace_bytes(a);
+    void* ws = need ? g_paged_ws.take(need, where) : nullptr;
+    if (need && !ws) return;
+    check(launch_attention_paged(a, ws, need, g_rt.stream), where);
+}
+
+GNCX_API void gncx_hip_token_logprobs(const float* logits, int32_t n_rows, int32_t vocab, const int32_t* tokens,
+                                      int32_t n_top, float* out_logprobs, float* out_entropy, int32_t* out_top_tokens,
+                                      float* out_top_logprobs) {
+    std::lock_guard<CallLock> lk(g_mu);
+    const char* where = "gncx_hip_token_logprobs";
+    if (n_rows == 0) return;
+    if (n_rows < 0 || vocab < 1 || vocab > kMaxBeamVocab || n_top < 0 || n_top > kMaxTopWords) {
+        set_error(where, "1 to 4194304 words and 0 to 64 alternatives", -1);
+        return;
+    }
+    if (!tokens != !out_logprobs || (n_top > 0 && (!out_top_tokens || !out_top_logprobs))) {
+        set_error(where, "tokens come with out_logprobs, alternatives with their two outputs", -1);
+        return;
+    }
+    if (!ensure_runtime(where)) return;
+    DeviceGuard dev(where);
+    if (!dev.ok) return;
+    const size_t rb = sizeof(float) * static_cast<size_t>(n_rows), lb = rb * vocab, tb = rb * n_top;
+    Allocations seen;
+    if (!on_device(logits, lb, "logits", where, seen) || (tokens && !on_device(tokens, rb, "tokens", where, seen)) ||
+        (out_logprobs && !on_device(out_logprobs, rb, "out_logprobs", where, seen)) ||
+        (out_entropy && !on_device(out_entropy, rb, "out_entropy", where, seen)) ||
+        (n_top && (!on_device(out_top_tokens, tb, "out_top_tokens", where, seen) ||
+                   !on_device(out_top_logprobs, tb, "out_top_logprobs", where, seen))) ||
+        !apart({{out_logprobs, rb}, {out_entropy, rb}, {n_top ? out_top_tokens : nullptr, tb},
+                {n_top ? out_top_logprobs : nullptr, tb}},
+               {{logits, lb}, {tokens, rb}}, where))
+        return;
+    const size_t need = token_logprobs_workspace_bytes(n_rows, vocab, n_top);
+    void* ws = need ? g_logprob_ws.take(need, where) : nullptr;
+    if (need && !ws) return;
+    check(launch_token_logprobs(logits, n_rows, vocab, tokens, n_top, out_logprobs, out_entropy, out_top_tokens,
+                                out_top_logprobs, ws, need, g_rt.stream),
+          where);
+}
+
 // ---- weight files and host buffers ------------------------------------
 // The reference's loader maps the GGUF read-only (cpp:327-404) and copies the
 // per-layer tensors, scratch vectors and KV caches into 2 MB-aligned,

@@ -1,0 +1,887 @@
+// paged.hip -- many sequences at once over a paged cache of 8-bit blocks: rotary
+// positions of rows, appending keys and values (with the per-head RMSNorm and the
+// rotation on the way), and attention over the cache.
+//
+// A block is 16 positions of one KV head, K as [16][HD] and V as [HD][16] e4m3
+// codes, each with a power of two as scale.  A power of two costs up to a bit of
+// range that e4m3 has to spare, and buys that a value's code is the same digits in
+// any scale: a block whose scale grows while tokens are appended keeps its codes
+// exactly (but for those that become subnormal), and bfloat16, which the matrix
+// instructions take, holds code times scale exactly.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "gncx_device.h"
+#include "gncx_launch.h"
+
+namespace gncx {
+namespace {
+
+using namespace dev;
+
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+// ---- rotation ------------------------------------------------------------------
+// cos and sin of position * freq: the angle's turns in 64 bits, as 32 keep a far
+// position's only to 2^-24 of it, then one turn at most in 32.
+__device__ __forceinline__ void turn_of(int32_t pos, double freq, float magnitude, float& c, float& s) {
+    double t = static_cast<double>(pos) * freq * 0.15915494309189535;  // 1 / (2 pi)
+    t -= rint(t);
+    sincospif(2.0f * static_cast<float>(t), &s, &c);
+    c *= magnitude;
+    s *= magnitude;
+}
+
+// Floats of pair p of a head: the rotated part's pairs, then the rest's, paired alike.
+__device__ __forceinline__ void pair_floats(int p, int n_rot, int head_dim, bool inter, int& a, int& b) {
+    const int half = n_rot / 2;
+    if (inter) {
+        a = 2 * p;
+        b = a + 1;
+    } else if (p < half) {
+        a = p;
+        b = p + half;
+    } else {
+        a = n_rot + p - half;
+        b = a + (head_dim - n_rot) / 2;
+    }
+}
+
+// Four pairs from 4 u on as two float4 each, where n_rot and head_dim are multiples of 8.
+struct FourPairs {
+    int off_a, off_b;  // where the two float4 stand
+    bool inter;
+    __device__ FourPairs(int u, int n_rot, int head_dim, bool interleaved) : inter(interleaved) {
+        if (inter) {
+            off_a = 8 * u;
+            off_b = off_a + 4;
+        } else {
+            pair_floats(4 * u, n_rot, head_dim, false, off_a, off_b);
+        }
+    }
+    __device__ void load(const float* head, float (&a)[4], float (&b)[4]) const {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(head + off_a), y = *reinterpret_cast<const f32x4*>(head + off_b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = inter ? (j < 2 ? x[2 * j & 3] : y[2 * j & 3]) : x[j];
+            b[j] = inter ? (j < 2 ? x[(2 * j + 1) & 3] : y[(2 * j + 1) & 3]) : y[j];
+        }
+    }
+    __device__ void store(float* head, const float (&a)[4], const float (&b)[4]) const {
+        f32x4 x, y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = inter ? (j & 1 ? b[j / 2] : a[j / 2]) : a[j];
+            y[j] = inter ? (j & 1 ? b[2 + j / 2] : a[2 + j / 2]) : b[j];
+        }
+        *reinterpret_cast<f32x4*>(head + off_a) = x;
+        *reinterpret_cast<f32x4*>(head + off_b) = y;
+    }
+};
+
+__device__ __forceinline__ void turn_pairs(float (&a)[4], float (&b)[4], const float (&c)[4], const float (&s)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float x = a[j] * c[j] - b[j] * s[j];
+        b[j] = b[j] * c[j] + a[j] * s[j];
+        a[j] = x;
+    }
+}
+
+// A work-group takes a row and some of its heads; its first threads form the
+// row's cosines and sines, one pair each, for all of them.
+constexpr int kRopeThreads = 256;
+constexpr int kMaxRopeDim = 1024;
+struct RopeRowsParams {
+    const float* rows;
+    float* out;
+    const int32_t* positions;
+    RotationArgs rot;
+    int32_t n_heads, head_dim, stride, out_stride, heads_per_group;
+};
+
+template <bool VEC>
+__global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeRowsParams p) {
+    __shared__ __align__(16) float cs[kMaxRopeDim / 2], sn[kMaxRopeDim / 2];
+    const int row = blockIdx.x, tid = threadIdx.x, half = p.rot.n_rot / 2, pairs = p.head_dim / 2;
+    const int h0 = blockIdx.y * p.heads_per_group, h1 = min(h0 + p.heads_per_group, p.n_heads);
+    const int32_t pos = p.positions[row];
+    for (int i = tid; i < pairs; i += kRopeThreads) {
+        float c = 1.0f, s = 0.0f;
+        if (i < half) turn_of(pos, p.rot.freqs[i], p.rot.magnitude, c, s);
+        cs[i] = c;
+        sn[i] = s;
+    }
+    __syncthreads();
+    const float* in = p.rows + static_cast<size_t>(row) * p.stride;
+    float* out = p.out + static_cast<size_t>(row) * p.out_stride;
+    const bool inter = p.rot.interleaved != 0;
+    const int units = VEC ? pairs / 4 : pairs, each = kRopeThreads / units;  // heads at once
+    if constexpr (VEC) {
+        const int u = tid % units;
+        const FourPairs at(u, p.rot.n_rot, p.head_dim, inter);
+        float c[4], s[4];
+        *reinterpret_cast<f32x4*>(c) = reinterpret_cast<const f32x4*>(cs)[u];
+        *reinterpret_cast<f32x4*>(s) = reinterpret_cast<const f32x4*>(sn)[u];
+        const bool turns = 4 * u < half;
+        if (tid < units * each)
+            for (int h = h0 + tid / units; h < h1; h += each) {
+                float a[4], b[4];
+                at.load(in + h * p.head_dim, a, b);
+                if (turns) turn_pairs(a, b, c, s);
+                at.store(out + h * p.head_dim, a, b);
+            }
+    } else {
+        for (int i = tid; i < (h1 - h0) * pairs; i += kRopeThreads) {
+            const int h = h0 + i / pairs, q = i % pairs;
+            int a, b;
+            pair_floats(q, p.rot.n_rot, p.head_dim, inter, a, b);
+            const float x = in[h * p.head_dim + a], y = in[h * p.head_dim + b];
+            out[h * p.head_dim + a] = q < half ? x * cs[q] - y * sn[q] : x;
+            out[h * p.head_dim + b] = q < half ? y * cs[q] + x * sn[q] : y;
+        }
+    }
+}
+
+// ---- the sequences of a call ------------------------------------------------------
+// The rows of a sequence that have a place: [row0, row0 + count) at positions len ..
+struct SeqRows {
+    int32_t row0, count, len;
+};
+__device__ __forceinline__ int clamp_row(const PagedArgs& c, int32_t r) { return min(max(r, 0), c.n_rows); }
+__device__ __forceinline__ SeqRows seq_rows(const PagedArgs& c, int s) {
+    SeqRows r;
+    r.row0 = clamp_row(c, c.row_start[s]);
+    r.len = c.lengths[s];
+    const int32_t room = c.max_pages * c.page_tokens;
+    r.count = r.len < 0 || r.len > room ? 0 : min(max(clamp_row(c, c.row_start[s + 1]) - r.row0, 0), room - r.len);
+    return r;
+}
+// The last sequence s with first(s) <= at, by a wave; -1 before the first.  first
+// ascends (where row_start does; otherwise some sequence or none is found).
+template <class F>
+__device__ __forceinline__ int find_seq(int n_seqs, int64_t at, F&& first) {
+    const int lane = threadIdx.x & 63;
+    int found = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
+        const int s = s0 + lane;
+        const uint64_t in = __ballot(s < n_seqs && first(min(s, n_seqs - 1)) <= at);
+        found += __builtin_popcountll(in);
+        if (~in) break;
+    }
+    return found - 1;
+}
+// The block of a position below max_pages * page_tokens: its number in the pool's
+// [page][head] order, -1 if its page is not there.
+__device__ __forceinline__ int64_t block_of(const PagedArgs& c, int s, int head, int32_t pos) {
+    const int32_t page = c.pages[static_cast<size_t>(s) * c.max_pages + pos / c.page_tokens];
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.n_pages)) return -1;
+    return (static_cast<int64_t>(page) * c.n_kv + head) * (c.page_tokens / kKvBlock) + pos % c.page_tokens / kKvBlock;
+}
+
+// ---- appending ----------------------------------------------------------------------
+// Powers of two of the scales
+constexpr int kLeastExp = -100, kMostExp = 120;
+// The least e with amax <= 448 2^e (448 = 0.875 2^9, e4m3's largest)
+__device__ __forceinline__ int scale_exp(float amax) {
+    int k;
+    const float f = frexpf(amax, &k);
+    const int e = amax == 0.0f ? kLeastExp : f <= 0.875f ? k - 9 : k - 8;
+    return min(max(e, kLeastExp), kMostExp);
+}
+__device__ __forceinline__ float pow2(int e) { return __builtin_bit_cast(float, (e + 127) << 23); }
+__device__ __forceinline__ float finite_size(float x) {
+    const float a = fabsf(x);
+    return a < __builtin_inff() ? a : 0.0f;  // (NaN compares false)
+}
+__device__ __forceinline__ float to_code_range(float x, float inv) {
+    return fabsf(x) < __builtin_inff() ? x * inv : __builtin_nanf("");
+}
+__device__ __forceinline__ uint32_t four_codes(float a, float b, float c, float d) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+    return static_cast<uint32_t>(r);
+}
+// Codes to a scale 1 / f as large
+__device__ __forceinline__ uint32_t moved_codes(uint32_t w, float f) {
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), false);
+    const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(w), true);
+    return four_codes(lo.x * f, lo.y * f, hi.x * f, hi.y * f);
+}
+
+template <int N>
+__device__ __forceinline__ float lanes_sum(float v) {
+    if constexpr (N == 32) {
+        v = group_sum<16>(v);
+        return v + __shfl_xor(v, 16, 64);
+    } else {
+        return group_sum<N>(v);
+    }
+}
+
+struct AppendParams {
+    AppendArgs a;
+    int64_t kv_groups;    // work-groups of the cache's blocks
+    int32_t head_groups;  // of a row's queries
+};
+
+// Blocks and queries in one launch.  A work-group takes the new tokens of one block
+// of K or of V: 16 tokens, HD / 8 threads each.  Nobody else touches the block, so
+// its old tokens are moved to a larger scale on the way, without atomics.  Sequence
+// s has the blocks from slot row_start[s] / 16 + 2 s on: as many as it can touch.
+// The other work-groups take 16 heads of a query row each.
+template <int HD>
+__global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
+    constexpr int kPer = HD / 8, kThreadsHere = 2 * HD;  // threads of a token or head
+    __shared__ float red[kThreadsHere / 64];
+    __shared__ __align__(16) uint8_t vt[HD * kKvBlock];
+    __shared__ __align__(16) float cs[HD / 2], sn[HD / 2];
+    const AppendArgs& a = p.a;
+    const PagedArgs& c = a.c;
+    const int tid = threadIdx.x, u = tid % kPer, wv = tid >> 6, lane = tid & 63;
+    const bool inter = a.rot.interleaved != 0;
+    const int half = a.rot.n_rot / 2;
+    const FourPairs at(u, a.rot.n_rot, HD, inter);
+    auto normed = [&](float(&x)[4], float(&y)[4], const float* gamma) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ss += x[j] * x[j] + y[j] * y[j];
+        ss = lanes_sum<kPer>(ss);
+        const float inv = 1.0f / sqrtf(ss / HD + a.eps);
+        float gx[4], gy[4];
+        if (gamma) at.load(gamma, gx, gy);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = gamma ? x[j] * inv * gx[j] : x[j] * inv;
+            y[j] = gamma ? y[j] * inv * gy[j] : y[j] * inv;
+        }
+    };
+    if (blockIdx.x >= p.kv_groups) {
+        const int64_t b = blockIdx.x - p.kv_groups;
+        const int row = static_cast<int>(b / p.head_groups), h = static_cast<int>(b % p.head_groups) * 16 + tid / kPer;
+        const int s = find_seq(c.n_seqs, row, [&](int i) { return clamp_row(c, c.row_start[i]); });
+        if (s < 0) return;
+        const SeqRows r = seq_rows(c, s);
+        if (row - r.row0 >= r.count) return;
+        if (tid < half) turn_of(r.len + row - r.row0, a.rot.freqs[tid], a.rot.magnitude, cs[tid], sn[tid]);
+        __syncthreads();
+        if (h >= a.n_heads) return;
+        const size_t head = (static_cast<size_t>(row) * a.n_heads + h) * HD;
+        float x[4], y[4];
+        at.load(a.q + head, x, y);
+        if (a.norm) normed(x, y, a.q_gamma);
+        if (4 * u < half) {
+            float cc[4], ss[4];
+            *reinterpret_cast<f32x4*>(cc) = reinterpret_cast<const f32x4*>(cs)[u];
+            *reinterpret_cast<f32x4*>(ss) = reinterpret_cast<const f32x4*>(sn)[u];
+            turn_pairs(x, y, cc, ss);
+        }
+        at.store(a.out_q + head, x, y);
+        return;
+    }
+    const int which = blockIdx.x & 1, hk = (blockIdx.x >> 1) % c.n_kv;
+    const int64_t slot = (blockIdx.x >> 1) / c.n_kv;
+    auto first_slot = [&](int i) { return static_cast<int64_t>(clamp_row(c, c.row_start[i]) >> 4) + 2 * i; };
+    const int s = find_seq(c.n_seqs, slot, first_slot);
+    if (s < 0) return;
+    const SeqRows r = seq_rows(c, s);
+    const int64_t nth = slot - first_slot(s);
+    if (r.count == 0 || nth > (r.len + r.count - 1) / kKvBlock - r.len / kKvBlock) return;
+    const int32_t base = (r.len / kKvBlock + static_cast<int32_t>(nth)) * kKvBlock;  // the block's first position
+    const int64_t block = block_of(c, s, hk, base);
+    if (block < 0) return;
+    // the block's tokens [held, end) are new, those before are kept
+    const int held = max(r.len - base, 0), end = min(r.len + r.count - base, kKvBlock), tok = tid / kPer;
+    const bool is_new = tok >= held && tok < end;
+    float* scale_at = c.scales + 2 * block + which;
+    const float was = held ? *scale_at : 0.0f;
+    const int row = r.row0 + base - r.len + tok;
+    const size_t head = (static_cast<size_t>(row) * c.n_kv + hk) * HD;
+    uint8_t* codes = (which ? c.v_pages : c.k_pages) + static_cast<size_t>(block) * (kKvBlock * HD);
+    // old codes: of K the thread's own eight, of V eight tokens of a float
+    uint32_t old0 = 0, old1 = 0;
+    if (which) {
+        const uint2 w = reinterpret_cast<const uint2*>(codes)[tid];
+        old0 = w.x;
+        old1 = w.y;
+    } else if (tok < held) {
+        old0 = *reinterpret_cast<const uint32_t*>(codes + tok * HD + at.off_a);
+        old1 = *reinterpret_cast<const uint32_t*>(codes + tok * HD + at.off_b);
+    }
+    float x[4] = {}, y[4] = {};
+    if (is_new) {
+        if (which) {
+            *reinterpret_cast<f32x4*>(x) = reinterpret_cast<const f32x4*>(a.v + head)[2 * u];
+            *reinterpret_cast<f32x4*>(y) = reinterpret_cast<const f32x4*>(a.v + head)[2 * u + 1];
+        } else {
+            at.load(a.k + head, x, y);
+        }
+    }
+    if (!which) {
+        if (a.norm) normed(x, y, a.k_gamma);
+        if (is_new && 4 * u < half) {
+            float cc[4], ss[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) turn_of(base + tok, a.rot.freqs[4 * u + j], a.rot.magnitude, cc[j], ss[j]);
+            turn_pairs(x, y, cc, ss);
+        }
+    }
+    float amax = 0.0f;
+    if (is_new)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fmaxf(finite_size(x[j]), finite_size(y[j])));
+    amax = wave_max(amax);
+    if (lane == 0) red[wv] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreadsHere / 64; ++i) amax = fmaxf(amax, red[i]);
+    int e = scale_exp(amax);
+    const int e_was = min(max(static_cast<int>(__builtin_bit_cast(uint32_t, was) >> 23 & 0xff) - 127, kLeastExp), kMostExp);
+    if (held) e = max(e, e_was);
+    const float inv = pow2(-e);
+    // (a factor below 2^-126 leaves nothing of any code)
+    const bool moves = held && e > e_was;
+    const float f = moves ? (e - e_was < 126 ? pow2(e_was - e) : 0.0f) : 1.0f;
+    if (tid == 0) *scale_at = pow2(e);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        x[j] = to_code_range(x[j], inv);
+        y[j] = to_code_range(y[j], inv);
+    }
+    if (!which) {
+        uint32_t w0, w1;
+        if (is_new) {
+            // in the order of the thread's two float4
+            w0 = inter ? four_codes(x[0], y[0], x[1], y[1]) : four_codes(x[0], x[1], x[2], x[3]);
+            w1 = inter ? four_codes(x[2], y[2], x[3], y[3]) : four_codes(y[0], y[1], y[2], y[3]);
+        } else {
+            if (!moves || tok >= held) return;
+            w0 = moved_codes(old0, f);
+            w1 = moved_codes(old1, f);
+        }
+        *reinterpret_cast<uint32_t*>(codes + tok * HD + at.off_a) = w0;
+        *reinterpret_cast<uint32_t*>(codes + tok * HD + at.off_b) = w1;
+        return;
+    }
+    if (is_new) {
+        const uint32_t w0 = four_codes(x[0], x[1], x[2], x[3]), w1 = four_codes(y[0], y[1], y[2], y[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            vt[(8 * u + j) * kKvBlock + tok] = static_cast<uint8_t>(byte_of(w0, j));
+            vt[(8 * u + 4 + j) * kKvBlock + tok] = static_cast<uint8_t>(byte_of(w1, j));
+        }
+    }
+    __syncthreads();
+    const uint2 fresh = reinterpret_cast<const uint2*>(vt)[tid];
+    // of bytes t0 .. t0 + 3: those below `held` moved, those in [held, end) new, the others as they are
+    auto mixed = [&](uint32_t old, uint32_t now, int t0) {
+        auto below = [&](int n) {  // bytes of tokens below n
+            const int k = min(max(n - t0, 0), 4);
+            return k == 4 ? 0xffffffffu : (1u << 8 * k) - 1u;
+        };
+        const uint32_t kept = below(held), all = below(end);
+        const uint32_t m = moves ? moved_codes(old, f) : old;
+        return (m & kept) | (now & all & ~kept) | (old & ~all);
+    };
+    const int t0 = tid % 2 * 8;
+    if (t0 < end && (moves || t0 + 8 > held))
+        reinterpret_cast<uint2*>(codes)[tid] = make_uint2(mixed(old0, fresh.x, t0), mixed(old1, fresh.y, t0 + 4));
+}
+
+// ---- attention ----------------------------------------------------------------------
+// S^T = K Q^T and O^T = V^T P^T on the matrix instructions, 64 keys a step: a query row
+// stays in a lane column (lane % 16) from its scores to its output.  A step is four
+// blocks; a 16-key product takes four tokens of each, so that the lanes of group
+// lane / 16 hold the scores of all 16 tokens of one block, and read those tokens of
+// V as 16 bytes of one float's row.
+// Precision: codes are exact in fp16 and code times scale in bfloat16.  Queries go in
+// as pairs of fp16 (22 bits, behind a power of two that takes the row's largest to
+// 2^14), weights as three bfloat16 (24 bits, and the range of a float, so that the
+// values' scales need no care).  Scores, sums and outputs are held in 32 bits.
+constexpr int kAttnThreads = 256, kAttnWaves = 4;
+constexpr int kMaxParts = 128;
+
+struct PagedParams {
+    PagedArgs c;
+    const float* q;
+    float* out;
+    float2* part_ml;  // [slot][KV head][part][row] maximum, sum
+    float* part_o;    // [slot][KV head][part][row][HD], divided by the sum
+    int32_t n_heads, group, sw, parts, least;  // least: steps of a part at least
+    float scale;      // attn_scale log2(e)
+    int64_t slots;
+};
+
+// The rows, keys and parts of a work-group.  Rows of a sequence and KV head are
+// numbered token by token, `group` heads each; tile t takes rows [R t, R t + R), and
+// sequence s has the slots from row_start[s] group / R + s on.
+struct Tile {
+    int seq, row_lo, rows, n_parts, step0, step1, per;  // steps of 64 keys; per: of a part
+    int32_t lo, hi;                                     // keys that some row may see
+    SeqRows r;
+};
+template <int R>
+__device__ __forceinline__ bool find_tile(const PagedParams& p, int64_t slot, Tile& t) {
+    const PagedArgs& c = p.c;
+    auto first = [&](int i) { return static_cast<int64_t>(clamp_row(c, c.row_start[i])) * p.group / R + i; };
+    t.seq = find_seq(c.n_seqs, slot, first);
+    if (t.seq < 0) return false;
+    t.r = seq_rows(c, t.seq);
+    const int64_t nth = slot - first(t.seq);
+    t.rows = t.r.count * p.group;
+    if (nth * R >= t.rows) return false;
+    t.row_lo = static_cast<int>(nth) * R;
+    const int32_t t0 = t.row_lo / p.group, t1 = (min(t.row_lo + R, t.rows) - 1) / p.group;
+    t.hi = t.r.len + t1 + 1;
+    t.lo = p.sw > 0 ? max(t.r.len + t0 - p.sw + 1, 0) : 0;
+    t.step0 = t.lo / 64;
+    t.step1 = (t.hi + 63) / 64;
+    const int n = t.step1 - t.step0;
+    t.per = max((n + p.parts - 1) / p.parts, p.least);
+    t.n_parts = (n + t.per - 1) / t.per;
+    return true;
+}
+
+__device__ __forceinline__ float xor_max(float v) {
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float xor_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {  // of a, then b
+    return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+__device__ __forceinline__ f16x8 codes_f16(uint32_t w0, uint32_t w1) {
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
+    const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
+    const f16x2 c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, false);
+    const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
+    return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+__device__ __forceinline__ bf16x8 codes_bf16(uint32_t w0, uint32_t w1, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
+    return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+// 0x80 in every byte of w that is a NaN
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// KEYS: the four waves share 16 RT rows and take every fourth step each (few rows: a
+// decode step); otherwise each has 16 RT rows of its own.
+template <int HD, int RT, bool KEYS>
+__global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(PagedParams p) {
+    constexpr int R = KEYS ? 16 * RT : 16 * RT * kAttnWaves;
+    constexpr int kSlices = HD / 64, kDims = HD / 16;
+    constexpr float kInf = __builtin_inff();
+    const PagedArgs& c = p.c;
+    const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x % c.n_kv;
+    const int part = static_cast<int>(blockIdx.x / c.n_kv) % p.parts;
+    const int64_t slot = blockIdx.x / c.n_kv / p.parts;
+    Tile t;
+    if (!find_tile<R>(p, slot, t) || part >= t.n_parts) return;
+    // this wave's rows, and the steps that they see
+    const int row_w = t.row_lo + (KEYS ? 0 : 16 * RT * wv);
+    if (!KEYS && row_w >= t.rows) return;
+    const int last_w = min(row_w + 16 * RT, t.rows) - 1;
+    const int32_t pos_first = t.r.len + row_w / p.group, pos_last = t.r.len + last_w / p.group;
+    const int32_t lo_w = p.sw > 0 ? max(pos_first - p.sw + 1, 0) : 0;
+    const int32_t low_most = p.sw > 0 ? max(pos_last - p.sw + 1, 0) : 0;
+    int step = t.step0 + part * t.per, step_end = min(step + t.per, t.step1);
+    if (!KEYS) {
+        step = max(step, lo_w / 64);
+        step_end = min(step_end, (pos_last + 64) / 64);
+    }
+    // queries: lane (n, g) has floats 64 i + 16 g + 0 .. 15 of row n, as the keys' lanes do
+    f16x8 qh[RT][2 * kSlices], ql[RT][2 * kSlices];
+    float fac[RT], m[RT], l[RT];
+    int32_t pos[RT];
+    f32x4 o[RT][kDims];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = min(row_w + 16 * rt + n, t.rows - 1);
+        pos[rt] = t.r.len + row / p.group;
+        const float* q = p.q + ((static_cast<size_t>(t.r.row0) + row / p.group) * p.n_heads + hk * p.group + row % p.group) * HD;
+        f32x4 v[kSlices][4];
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[i][j] = *reinterpret_cast<const f32x4*>(q + 64 * i + 16 * g + 4 * j);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(v[i][j][k]));
+            }
+        most = xor_max(most);
+        int e = 0;
+        (void)frexpf(most, &e);
+        e = most > 0.0f && most < kInf ? e - 14 : 0;
+        fac[rt] = ldexpf(p.scale, e);
+#pragma unroll
+        for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float x = ldexpf(v[i][j / 4][j % 4], -e);
+                const _Float16 h = static_cast<_Float16>(x);
+                qh[rt][2 * i + j / 8][j % 8] = h;
+                ql[rt][2 * i + j / 8][j % 8] = static_cast<_Float16>(x - static_cast<float>(h));
+            }
+        m[rt] = -kInf;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[rt][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    const int32_t room = c.max_pages * c.page_tokens;
+    for (step += KEYS ? wv : 0; step < step_end; step += KEYS ? kAttnWaves : 1) {
+        const int32_t k0 = 64 * step;
+        // the lane's block of K (rows of the product), and of V, scores and scales
+        const int32_t at_k = k0 + 16 * (n >> 2), at_v = k0 + 16 * g;
+        const int64_t bk = at_k < room ? block_of(c, t.seq, hk, at_k) : -1;
+        const int64_t bv = at_v < room ? block_of(c, t.seq, hk, at_v) : -1;
+        // (a block that is not there: the first one is read, and hidden)
+        const uint8_t* kp = c.k_pages + (bk < 0 ? 0 : bk) * (kKvBlock * HD) + (n & 3) * HD + 16 * g;
+        const uint8_t* vp = c.v_pages + (bv < 0 ? 0 : bv) * (kKvBlock * HD) + 16 * n;
+        float2 scale = *reinterpret_cast<const float2*>(c.scales + 2 * (bv < 0 ? 0 : bv));
+        const bool there = bv >= 0 && at_v < t.hi && at_v + 16 > t.lo;
+        if (!there) scale = make_float2(1.0f, 1.0f);
+        const bool full = k0 + 63 <= pos_first && k0 >= low_most && __ballot(there) == ~uint64_t{0};
+        uint4 kw[4][kSlices], vw[kDims];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i) kw[j][i] = *reinterpret_cast<const uint4*>(kp + 4 * j * HD + 64 * i);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) vw[d] = *reinterpret_cast<const uint4*>(vp + 256 * d);
+        f32x4 s[RT][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) s[rt][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i) {
+                const f16x8 a = codes_f16(kw[j][i].x, kw[j][i].y), b = codes_f16(kw[j][i].z, kw[j][i].w);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[rt][2 * i], s[rt][j], 0, 0, 0);
+                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[rt][2 * i + 1], s[rt][j], 0, 0, 0);
+                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[rt][2 * i], s[rt][j], 0, 0, 0);
+                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[rt][2 * i + 1], s[rt][j], 0, 0, 0);
+                }
+            }
+        }
+        // NaN codes of V, which rows that do not see them must not meet (0 NaN is NaN), are
+        // taken out of a step that is not seen whole, and met by a product of their own
+        uint32_t bad = 0;
+        if (!full)
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+                bad |= nan_bytes(vw[d].x) | nan_bytes(vw[d].y) | nan_bytes(vw[d].z) | nan_bytes(vw[d].w);
+        const bool clean = !__any(bad != 0);
+        bf16x8 w[RT][2][3], sees[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const float f = fac[rt] * scale.x;
+            float x[16], most = -kInf;
+            uint32_t seen = 0xffffu;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = s[rt][j / 4][j % 4] * f;
+            if (!full) {
+                const int32_t low = p.sw > 0 ? pos[rt] - p.sw + 1 : 0;
+                seen = 0;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const bool in = there && at_v + j <= pos[rt] && at_v + j >= low;
+                    x[j] = in ? x[j] : -kInf;
+                    seen |= in ? 1u << j : 0u;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
+            const float mx = fmaxf(m[rt], xor_max(most)), use = mx == -kInf ? 0.0f : mx;
+            const float alpha = __builtin_amdgcn_exp2f(m[rt] - use);
+            m[rt] = mx;
+            float sum = 0.0f;
+            uint32_t h[16], md[16], lw[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float e = __builtin_amdgcn_exp2f(x[j] - use);
+                sum += e;
+                // e = three numbers of 8 bits, cut off one after the other: nothing is lost
+                h[j] = __builtin_bit_cast(uint32_t, e) & 0xffff0000u;
+                const float r1 = e - __builtin_bit_cast(float, h[j]);
+                md[j] = __builtin_bit_cast(uint32_t, r1) & 0xffff0000u;
+                lw[j] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, md[j]));
+            }
+            l[rt] = l[rt] * alpha + sum;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint4 a, b, cc, dd;
+                a = make_uint4(high_halves(h[8 * k], h[8 * k + 1]), high_halves(h[8 * k + 2], h[8 * k + 3]),
+                               high_halves(h[8 * k + 4], h[8 * k + 5]), high_halves(h[8 * k + 6], h[8 * k + 7]));
+                b = make_uint4(high_halves(md[8 * k], md[8 * k + 1]), high_halves(md[8 * k + 2], md[8 * k + 3]),
+                               high_halves(md[8 * k + 4], md[8 * k + 5]), high_halves(md[8 * k + 6], md[8 * k + 7]));
+                cc = make_uint4(high_halves(lw[8 * k], lw[8 * k + 1]), high_halves(lw[8 * k + 2], lw[8 * k + 3]),
+                                high_halves(lw[8 * k + 4], lw[8 * k + 5]), high_halves(lw[8 * k + 6], lw[8 * k + 7]));
+                w[rt][k][0] = __builtin_bit_cast(bf16x8, a);
+                w[rt][k][1] = __builtin_bit_cast(bf16x8, b);
+                w[rt][k][2] = __builtin_bit_cast(bf16x8, cc);
+                auto one = [&](int j) {
+                    return ((seen >> j & 1u) ? 0x3f80u : 0u) | ((seen >> (j + 1) & 1u) ? 0x3f800000u : 0u);
+                };
+                dd = make_uint4(one(8 * k), one(8 * k + 2), one(8 * k + 4), one(8 * k + 6));
+                sees[rt][k] = __builtin_bit_cast(bf16x8, dd);
+            }
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) o[rt][d] *= alpha;
+        }
+        if (clean) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                const bf16x8 a = codes_bf16(vw[d].x, vw[d].y, scale.y), b = codes_bf16(vw[d].z, vw[d].w, scale.y);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                    for (int k = 2; k >= 0; --k) {
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[rt][0][k], o[rt][d], 0, 0, 0);
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, w[rt][1][k], o[rt][d], 0, 0, 0);
+                    }
+            }
+        } else {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                const uint32_t z[4] = {nan_bytes(vw[d].x) >> 7, nan_bytes(vw[d].y) >> 7, nan_bytes(vw[d].z) >> 7,
+                                       nan_bytes(vw[d].w) >> 7};
+                const bf16x8 a = codes_bf16(vw[d].x & ~(z[0] * 0xffu), vw[d].y & ~(z[1] * 0xffu), scale.y);
+                const bf16x8 b = codes_bf16(vw[d].z & ~(z[2] * 0xffu), vw[d].w & ~(z[3] * 0xffu), scale.y);
+                const bf16x8 na = codes_bf16(z[0] * 0x38u, z[1] * 0x38u, 1.0f);  // (0x38: one)
+                const bf16x8 nb = codes_bf16(z[2] * 0x38u, z[3] * 0x38u, 1.0f);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+                    for (int k = 2; k >= 0; --k) {
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[rt][0][k], o[rt][d], 0, 0, 0);
+                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, w[rt][1][k], o[rt][d], 0, 0, 0);
+                    }
+                    f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
+                    count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(na, sees[rt][0], count, 0, 0, 0);
+                    count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(nb, sees[rt][1], count, 0, 0, 0);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (count[r] > 0.0f) o[rt][d][r] = __builtin_nanf("");
+                }
+            }
+        }
+    }
+    // out: floats 16 d + 4 g .. + 3 of row n
+    const size_t part_row = ((static_cast<size_t>(slot) * c.n_kv + hk) * p.parts + part) * R;
+    auto out_of = [&](int row) {  // row of the sequence
+        return p.out + ((static_cast<size_t>(t.r.row0) + row / p.group) * p.n_heads + hk * p.group + row % p.group) * HD;
+    };
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        l[rt] = xor_sum(l[rt]);
+        // divided by the sum here, before the parts' weights meet the values
+        const float inv = l[rt] != 0.0f ? 1.0f / l[rt] : 0.0f;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) o[rt][d] *= inv;
+    }
+    if constexpr (!KEYS) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int row = row_w + 16 * rt + n;
+            if (row >= t.rows) continue;
+            float* to = out_of(row);
+            if (t.n_parts > 1) {
+                const size_t i = part_row + row - t.row_lo;
+                if (g == 0) p.part_ml[i] = make_float2(m[rt], l[rt]);
+                to = p.part_o + i * HD;
+            }
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(to + 16 * d + 4 * g) = o[rt][d];
+        }
+    } else {
+        // the waves' parts of a row meet in LDS (a row of HD + 4 floats: no two rows on the same banks)
+        __shared__ __align__(16) float os[kAttnWaves][R][HD + 4];
+        __shared__ float2 mls[kAttnWaves][R];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            if (g == 0) mls[wv][16 * rt + n] = make_float2(m[rt], l[rt]);
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(&os[wv][16 * rt + n][16 * d + 4 * g]) = o[rt][d];
+        }
+        __syncthreads();
+        const int rows = min(R, t.rows - t.row_lo);
+        for (int i = tid; i < rows * (HD / 4); i += kAttnThreads) {
+            const int row = i / (HD / 4), d = i % (HD / 4);
+            float M = -kInf, L = 0.0f, wt[kAttnWaves];
+#pragma unroll
+            for (int k = 0; k < kAttnWaves; ++k) M = fmaxf(M, mls[k][row].x);
+            const float use = M == -kInf ? 0.0f : M;
+#pragma unroll
+            for (int k = 0; k < kAttnWaves; ++k) {
+                wt[k] = mls[k][row].y * __builtin_amdgcn_exp2f(mls[k][row].x - use);
+                L += wt[k];
+            }
+            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < kAttnWaves; ++k)
+                if (wt[k] != 0.0f) x += (wt[k] * inv) * *reinterpret_cast<const f32x4*>(&os[k][row][4 * d]);
+            float* to = out_of(t.row_lo + row);
+            if (t.n_parts > 1) {
+                if (d == 0) p.part_ml[part_row + row] = make_float2(M, L);
+                to = p.part_o + (part_row + row) * HD;
+            }
+            *reinterpret_cast<f32x4*>(to + 4 * d) = x;
+        }
+    }
+}
+
+// out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the parts c.
+template <int HD, int R>
+__global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedParams p) {
+    const PagedArgs& c = p.c;
+    const int hk = blockIdx.x % c.n_kv;
+    const int64_t slot = blockIdx.x / c.n_kv;
+    Tile t;
+    if (!find_tile<R>(p, slot, t) || t.n_parts == 1) return;
+    const size_t base = (static_cast<size_t>(slot) * c.n_kv + hk) * p.parts * R;
+    const int rows = min(R, t.rows - t.row_lo);
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += kAttnThreads) {
+        const int row = i / (HD / 4), d = i % (HD / 4);
+        float M = -__builtin_inff(), L = 0.0f;
+        for (int k = 0; k < t.n_parts; ++k) M = fmaxf(M, p.part_ml[base + static_cast<size_t>(k) * R + row].x);
+        const float use = M == -__builtin_inff() ? 0.0f : M;
+        for (int k = 0; k < t.n_parts; ++k) {
+            const float2 ml = p.part_ml[base + static_cast<size_t>(k) * R + row];
+            L += ml.y * __builtin_amdgcn_exp2f(ml.x - use);
+        }
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < t.n_parts; ++k) {
+            const size_t at = base + static_cast<size_t>(k) * R + row;
+            const float2 ml = p.part_ml[at];
+            const float w = ml.y * __builtin_amdgcn_exp2f(ml.x - use);
+            if (w != 0.0f) x += (w * inv) * *reinterpret_cast<const f32x4*>(p.part_o + at * HD + 4 * d);
+        }
+        const int r = t.row_lo + row;
+        *reinterpret_cast<f32x4*>(p.out + ((static_cast<size_t>(t.r.row0) + r / p.group) * p.n_heads + hk * p.group +
+                                           r % p.group) * HD + 4 * d) = x;
+    }
+}
+
+// The split of a call, from what the host knows of it: few rows a sequence share
+// their keys over the waves, many have waves of their own; keys are cut into parts
+// until there are work-groups for the chip.
+struct PagedPlan {
+    bool keys;
+    int32_t rows, parts, least;
+    int64_t slots;
+};
+PagedPlan paged_plan(const PagedAttnArgs& a) {
+    PagedPlan pl;
+    const int64_t group = a.n_heads / a.c.n_kv, rows = group * a.c.n_rows;
+    pl.keys = rows <= 32 * static_cast<int64_t>(a.c.n_seqs);
+    pl.rows = pl.keys ? 16 : a.c.head_dim == 256 ? 64 : 128;
+    pl.least = pl.keys ? 4 : 8;
+    pl.slots = rows / pl.rows + a.c.n_seqs;
+    const int64_t groups = (pl.keys ? std::max<int64_t>(rows / pl.rows, a.c.n_seqs) : pl.slots) * a.c.n_kv;
+    const int64_t steps = (static_cast<int64_t>(a.c.max_pages) * a.c.page_tokens + 63) / 64;
+    const int64_t want = (512 + groups - 1) / groups, most = (steps + pl.least - 1) / pl.least;
+    pl.parts = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxParts})));
+    return pl;
+}
+
+template <int HD>
+hipError_t paged_attention(PagedParams& p, const PagedPlan& pl, hipStream_t stream) {
+    const int64_t groups = pl.slots * p.c.n_kv;
+    if (groups * pl.parts > 0x7fffffff) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<uint32_t>(groups * pl.parts));
+    constexpr int kOwn = HD == 256 ? 1 : 2;
+    if (pl.keys) hipLaunchKernelGGL((paged_attn_kernel<HD, 1, true>), grid, dim3(kAttnThreads), 0, stream, p);
+    else hipLaunchKernelGGL((paged_attn_kernel<HD, kOwn, false>), grid, dim3(kAttnThreads), 0, stream, p);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || pl.parts == 1) return e;
+    const dim3 merge(static_cast<uint32_t>(groups));
+    if (pl.keys) hipLaunchKernelGGL((paged_merge_kernel<HD, 16>), merge, dim3(kAttnThreads), 0, stream, p);
+    else hipLaunchKernelGGL((paged_merge_kernel<HD, 64 * kOwn>), merge, dim3(kAttnThreads), 0, stream, p);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_rope_rows(const float* rows, int32_t n_rows, int32_t row_stride, int32_t n_heads, int32_t head_dim,
+                            const int32_t* positions, const RotationArgs& rot, int32_t out_stride, float* out,
+                            hipStream_t stream) {
+    if (n_rows < 1 || n_heads < 1 || head_dim < 2 || head_dim % 2 || head_dim > kMaxRopeDim || rot.n_rot < 0 ||
+        rot.n_rot % 2 || rot.n_rot > head_dim)
+        return hipErrorInvalidValue;
+    RopeRowsParams p{rows, out, positions, rot, n_heads, head_dim, row_stride, out_stride, n_heads};
+    const auto aligned = [](const float* x) { return reinterpret_cast<uintptr_t>(x) % 16 == 0; };
+    const bool vec = head_dim % 8 == 0 && rot.n_rot % 8 == 0 && row_stride % 4 == 0 && out_stride % 4 == 0 &&
+                     aligned(rows) && aligned(out);
+    // a row's heads in as many work-groups as make 1024 of them, at least as many
+    // heads each as it takes at once
+    const int32_t at_once = std::max(1, kRopeThreads / (vec ? head_dim / 8 : head_dim / 2));
+    const int32_t most = (n_heads + at_once - 1) / at_once;
+    const int32_t groups = std::min(most, std::max(1, (1024 + n_rows - 1) / n_rows));
+    p.heads_per_group = (n_heads + groups - 1) / groups;
+    const dim3 grid(n_rows, (n_heads + p.heads_per_group - 1) / p.heads_per_group);
+    if (grid.y > 65535) return hipErrorInvalidValue;
+    if (vec) hipLaunchKernelGGL(rope_rows_kernel<true>, grid, dim3(kRopeThreads), 0, stream, p);
+    else hipLaunchKernelGGL(rope_rows_kernel<false>, grid, dim3(kRopeThreads), 0, stream, p);
+    return hipGetLastError();
+}
+
+hipError_t launch_kv_append_paged(const AppendArgs& a, hipStream_t stream) {
+    AppendParams p{a, 0, (a.n_heads + 15) / 16};
+    p.kv_groups = (static_cast<int64_t>(a.c.n_rows / kKvBlock) + 2 * a.c.n_seqs) * a.c.n_kv * 2;
+    const int64_t groups = p.kv_groups + (a.q ? static_cast<int64_t>(a.c.n_rows) * p.head_groups : 0);
+    if (groups > 0x7fffffff) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<uint32_t>(groups));
+    if (a.c.head_dim == 64) hipLaunchKernelGGL(append_kernel<64>, grid, dim3(128), 0, stream, p);
+    else if (a.c.head_dim == 128) hipLaunchKernelGGL(append_kernel<128>, grid, dim3(256), 0, stream, p);
+    else if (a.c.head_dim == 256) hipLaunchKernelGGL(append_kernel<256>, grid, dim3(512), 0, stream, p);
+    else return hipErrorInvalidValue;
+    return hipGetLastError();
+}
+
+size_t attention_paged_workspace_bytes(const PagedAttnArgs& a) {
+    const PagedPlan pl = paged_plan(a);
+    if (pl.parts == 1) return 0;
+    return static_cast<size_t>(pl.slots) * a.c.n_kv * pl.parts * pl.rows * (sizeof(float2) + sizeof(float) * a.c.head_dim);
+}
+
+hipError_t launch_attention_paged(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+    if (workspace_bytes < attention_paged_workspace_bytes(a)) return hipErrorInvalidValue;
+    const PagedPlan pl = paged_plan(a);
+    PagedParams p{};
+    p.c = a.c;
+    p.q = a.q;
+    p.out = a.out;
+    p.n_heads = a.n_heads;
+    p.group = a.n_heads / a.c.n_kv;
+    p.sw = a.sliding_window;
+    p.parts = pl.parts;
+    p.least = pl.least;
+    p.scale = a.scale * 1.44269504088896341f;
+    p.slots = pl.slots;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.slots) * a.c.n_kv * pl.parts * pl.rows * a.c.head_dim);
+    if (a.c.head_dim == 64) return paged_attention<64>(p, pl, stream);
+    if (a.c.head_dim == 128) return paged_attention<128>(p, pl, stream);
+    if (a.c.head_dim == 256) return paged_attention<256>(p, pl, stream);
+    return hipErrorInvalidValue;
+}
+
+}  // namespace gncx

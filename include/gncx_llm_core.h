@@ -508,6 +508,118 @@ void gncx_hip_beam_select(const float* logits, int32_t n_beams, int32_t vocab, c
 void gncx_hip_kv_reorder(float* const* k_caches, float* const* v_caches, int32_t n_layers, int32_t n_beams,
                          size_t beam_stride, int32_t kv_dim, int32_t row0, int32_t n_rows, const int32_t* parents);
 
+/* Many sequences at once, over a paged cache of 8-bit blocks.  No counterpart
+ * in the reference, whose streamer decodes one sequence over an fp32 cache.
+ * Rows, caches, tables and outputs are memory of the library's GPU, used in
+ * place and in the order of the library stream; the structs are host memory,
+ * read before the call returns.  Nothing is read back to the host, so a decode
+ * step can be captured into a graph and replayed with lengths that a kernel
+ * moves on.  The host waits for the GPU only where attention or log
+ * probabilities need a larger workspace than before or are issued on another
+ * library stream than the last ones (captured calls have their graph's).
+ * Refused calls leave every output as it was; refused is also what would reach
+ * past the end of the allocation that a pointer lies in.
+ *
+ * A layer's cache: pages of page_tokens (16, 32, 64, 128 or 256) positions.  A
+ * block is 16 positions of one KV head: K as [16][head_dim], V as
+ * [head_dim][16], e4m3 codes (OCP), each of the two with a scale, a power of two
+ * between 2^-100 and 2^120; a value is its code times its block's scale.
+ * head_dim is 64, 128 or 256. */
+typedef struct GNCXPagedCache {
+    uint8_t* k_pages; /* [n_pages][n_kv_heads][page_tokens / 16][16 * head_dim], 16-byte aligned */
+    uint8_t* v_pages;
+    float* scales;    /* [n_pages][n_kv_heads][page_tokens / 16][2]: K's, V's; 8-byte aligned */
+    int32_t n_pages, page_tokens, n_kv_heads, head_dim;
+} GNCXPagedCache;
+/* The sequences of a call (device arrays).  Rows row_start[s] ..
+ * row_start[s + 1] - 1 (ascending, up to n_rows) are the next tokens of
+ * sequence s, whose pages hold lengths[s] tokens before them: row
+ * row_start[s] + i is at position lengths[s] + i, which lies in the page
+ * pages[s * max_pages + position / page_tokens].  A sequence may have no rows.
+ * Rows behind the last sequence's, rows past max_pages * page_tokens positions
+ * and rows of a sequence whose length is negative or past that are no rows: what
+ * belongs to them stays as it is.  A page outside [0, n_pages) is not there:
+ * nothing is stored to it, and nothing in it is seen.  Sequences may share pages
+ * that none of them appends to. */
+typedef struct GNCXPagedBatch {
+    int32_t n_seqs, n_rows, max_pages; /* 1..65536 sequences, max_pages * page_tokens up to 2^30 */
+    const int32_t* row_start;          /* [n_seqs + 1] */
+    const int32_t* lengths;            /* [n_seqs] */
+    const int32_t* pages;              /* [n_seqs][max_pages] */
+} GNCXPagedBatch;
+/* A rotation of the first n_rot (even) floats of a head: pair i < n_rot / 2 is
+ * floats (i, i + n_rot / 2), with interleaved != 0 (2 i, 2 i + 1), and is turned by
+ * position * freqs[i] radians, formed in 64 bits, and multiplied by magnitude.
+ * n_rot = 0: none. */
+typedef struct GNCXRotation {
+    const double* freqs; /* device [n_rot / 2], of gncx_hip_rope_frequencies; 8-byte aligned */
+    int32_t n_rot, interleaved;
+    float magnitude;
+} GNCXRotation;
+/* out_freqs[i] (host or device memory, n_rot / 2 doubles) = the radians a position
+ * turns pair i by: base^(-2 i / n_rot), scaled for contexts `factor` times the
+ * trained one:
+ *   GNCX_ROPE_PLAIN   as it is
+ *   GNCX_ROPE_LINEAR  divided by factor
+ *   GNCX_ROPE_BASE    of the base times factor^(n_rot / (n_rot - 2))
+ *   GNCX_ROPE_YARN    divided by factor where a pair turns less than beta_slow
+ *                     times within trained_context positions, as it is where it
+ *                     turns more than beta_fast times, mixed in between;
+ *                     *out_magnitude (host) is 0.1 ln(factor) + 1, otherwise 1
+ * and divided by factors[i] (host or device, n_rot / 2 floats, as a GGUF's
+ * rope_freqs tensor holds; NULL for none, 0 leaves a pair as it is).  Waits for
+ * the device where out_freqs is device memory.  0, or -1 with
+ * gncx_hip_last_error set. */
+enum { GNCX_ROPE_PLAIN = 0, GNCX_ROPE_LINEAR = 1, GNCX_ROPE_BASE = 2, GNCX_ROPE_YARN = 3 };
+int gncx_hip_rope_frequencies(int32_t n_rot, double base, int32_t scaling, double factor, int32_t trained_context,
+                              double beta_fast, double beta_slow, const float* factors, double* out_freqs,
+                              float* out_magnitude);
+/* out_rows[r] = rows[r] (n_heads heads of head_dim floats, even, up to 1024) with
+ * every head rotated to positions[r] (device); rows are row_stride and
+ * out_stride floats apart, and what lies between them stays as it is.  A negative
+ * position turns back.  out_rows may be rows (with one stride), and does not
+ * overlap it otherwise. */
+void gncx_hip_rope_rows(const float* rows, int32_t n_rows, int32_t row_stride, int32_t n_heads, int32_t head_dim,
+                        const int32_t* positions, const GNCXRotation* rotation, int32_t out_stride, float* out_rows);
+/* The batch's k_rows and v_rows [n_rows][n_kv_heads*head_dim] into the cache, K
+ * behind the per-head RMSNorm (as in gncx_hip_attention_prefill: with weights for
+ * has_norm_weight > 0, without for 0, none below 0) and the rotation of its position
+ * (rotation may be NULL: none; n_rot a multiple of 8); with q_rows
+ * [n_rows][n_heads*head_dim] (may be NULL), out_q (may be q_rows) receives the
+ * same of the queries.  k_rows and v_rows stay as they are.
+ * A block's scale is the least power of two that 448 times reaches every finite
+ * value stored to it; where it holds earlier tokens and their scale is smaller,
+ * their codes are rounded to the new one (exact but for codes that become
+ * subnormal).  Infinities and NaN are stored as NaN.  Rows of one call go to
+ * places of their own: no page that is appended to may stand twice in the tables.
+ * No two of the arguments' arrays overlap but as said. */
+void gncx_hip_kv_append_paged(const GNCXPagedCache* cache, const GNCXPagedBatch* batch, const float* q_rows,
+                              const float* k_rows, const float* v_rows, int32_t n_heads, const uint8_t* mmap_base,
+                              size_t q_norm_offset, size_t k_norm_offset, int32_t has_norm_weight, float norm_eps,
+                              const GNCXRotation* rotation, float* out_q);
+/* out_rows [n_rows][n_heads*head_dim] = the attention of q_rows (rotated) over the
+ * cache: a row sees its sequence's positions up to its own, which the cache holds
+ * already (gncx_hip_kv_append_paged), with sliding_window > 0 the last so many of
+ * them; what it does not see has no part in its output, whatever it holds.  A row
+ * that sees nothing (its pages are not there) gives zeros.  16-byte aligned;
+ * out_rows overlaps nothing. */
+void gncx_hip_attention_paged(const GNCXPagedCache* cache, const GNCXPagedBatch* batch, const float* q_rows,
+                              int32_t n_heads, float attn_scale, int32_t sliding_window, float* out_rows);
+/* For each of n_rows rows of logits [vocab] (1 to 4194304 words):
+ *   out_logprobs[r] = log softmax(row)[tokens[r]], -inf for a token outside the vocabulary
+ *   out_entropy[r]  = -sum over v of p(v) log p(v), in nats
+ *   out_top_tokens, out_top_logprobs [n_rows][n_top]: the n_top (0..64) most
+ *     probable words, equal ones by the lowest, behind the last one above -inf
+ *     filled with -1 and -inf.
+ * tokens and out_logprobs may both be NULL, as may out_entropy, and for n_top = 0
+ * out_top_tokens and out_top_logprobs.  A NaN logit counts as -inf; a row without a
+ * word above -inf has log probabilities -inf and entropy 0.  Exponentials are formed
+ * in 32 bits, their sums and the logarithms in 64.  No two outputs overlap, nor an
+ * output and an input. */
+void gncx_hip_token_logprobs(const float* logits, int32_t n_rows, int32_t vocab, const int32_t* tokens, int32_t n_top,
+                             float* out_logprobs, float* out_entropy, int32_t* out_top_tokens,
+                             float* out_top_logprobs);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,945 @@
+"""GPU: many sequences at once through the C-ABI with device pointers, against
+64-bit formulas: rotary positions of rows, appending to the paged cache of 8-bit
+blocks, attention over it, and log probabilities."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+from conftest import gncx
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24  # half a step of fp32
+EPS = 1e-6
+BLOCK = 16
+
+
+def refused(lib, text):
+    assert lib.gncx_hip_last_status() != 0
+    assert text in lib.gncx_hip_last_error().decode()
+
+
+def randn(torch, seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def whole(torch, values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+# ---- rotary positions ---------------------------------------------------------------
+class Turn:
+    """A rotation, and what it does in 64 bits."""
+
+    def __init__(self, torch, n_rot, inter=0, magnitude=1.0, base=1e4):
+        self.torch, self.n, self.inter, self.magnitude = torch, n_rot, inter, magnitude
+        self.freqs = torch.from_numpy(base ** (-2.0 * np.arange(max(n_rot // 2, 1)) / max(n_rot, 1))).cuda()
+        self.c = gncx.Rotation(self.freqs.data_ptr(), n_rot, inter, magnitude)
+        self.magnitude = self.c.magnitude  # as a float
+
+    def ref(self):
+        return C.addressof(self.c)
+
+    def __call__(self, x, at):
+        """x [rows][heads][head_dim] (64 bits): the result, and how far 32 bits may be off
+        from it.  A turn is off by half a step below 1/2, 2^-26 or 2 pi 2^-26 radians; the
+        cosine and sine by four steps, the products and their sum by three roundings:
+        under 2^-23.4 + 8 u + 3 u < 13 u of |a| + |b|."""
+        torch, n = self.torch, self.n
+        if n == 0:
+            return x.clone(), torch.zeros_like(x)
+        angle = at.double()[:, None, None] * self.freqs
+        a, b = (x[..., 0:n:2], x[..., 1:n:2]) if self.inter else (x[..., :n // 2], x[..., n // 2:n])
+        y, tol = x.clone(), torch.zeros_like(x)
+        p = self.magnitude * (a * angle.cos() - b * angle.sin())
+        q = self.magnitude * (b * angle.cos() + a * angle.sin())
+        t = 13 * U * abs(self.magnitude) * (a.abs() + b.abs())
+        if self.inter:
+            y[..., 0:n:2], y[..., 1:n:2], tol[..., 0:n:2], tol[..., 1:n:2] = p, q, t, t
+        else:
+            y[..., :n // 2], y[..., n // 2:n], tol[..., :n // 2], tol[..., n // 2:n] = p, q, t, t
+        return y, tol
+
+
+@pytest.mark.parametrize("rows,heads,hd,n_rot,inter,mag,pad,shift", [
+    (1, 40, 128, 128, 0, 1.0, 0, 0), (3, 5, 64, 64, 1, 1.0, 0, 0), (7, 3, 128, 32, 0, 1.25, 8, 4),
+    (7, 3, 128, 32, 1, 1.25, 8, 4), (5, 2, 80, 80, 0, 1.0, 0, 0), (5, 2, 80, 20, 1, 0.5, 0, 0),
+    (4, 3, 96, 70, 0, 1.0, 0, 0), (4, 3, 6, 2, 1, 1.0, 1, 0), (2, 70, 256, 256, 0, 1.0, 0, 0),
+    (2, 1, 1024, 1024, 1, 1.0, 0, 0), (2, 3, 1024, 8, 0, 1.0, 0, 0), (300, 9, 128, 128, 0, 1.0, 3, 1),
+    (6, 4, 64, 0, 0, 3.0, 0, 0), (6, 2, 2, 2, 0, 1.0, 0, 0), (1100, 2, 64, 48, 1, 1.0, 0, 0)])
+def test_rope_rows(lib, torch_mod, rows, heads, hd, n_rot, inter, mag, pad, shift):
+    torch = torch_mod
+    width, t = heads * hd, Turn(torch, n_rot, inter, mag)
+    held = randn(torch, rows, rows * (width + pad) + shift)
+    x = held[shift:].view(rows, width + pad)
+    at = torch.randint(-5000, 1000000, (rows,), generator=torch.Generator(device="cuda").manual_seed(1), device="cuda",
+                       dtype=torch.int32)
+    at[0] = 0
+    want, tol = t(x[:, :width].double().view(rows, heads, hd), at)
+    out = torch.full((rows, width + pad + 4), 7.0, device="cuda")
+    before = held.clone()
+    lib.gncx_hip_rope_rows(x.data_ptr(), rows, width + pad, heads, hd, at.data_ptr(), t.ref(), width + pad + 4,
+                           out.data_ptr())
+    gncx.check(lib)
+    assert torch.equal(held, before) and (out[:, width:] == 7.0).all()
+    got = out[:, :width].reshape(rows, heads, hd)
+    assert ((got.double() - want).abs() <= tol).all()
+    assert torch.equal(got[..., n_rot:], x[:, :width].view(rows, heads, hd)[..., n_rot:])
+    # in place: the same, and what lies between the rows stays
+    lib.gncx_hip_rope_rows(x.data_ptr(), rows, width + pad, heads, hd, at.data_ptr(), t.ref(), width + pad, x.data_ptr())
+    gncx.check(lib)
+    assert torch.equal(x[:, :width].reshape(rows, heads, hd), got)
+    assert torch.equal(x[:, width:], before[shift:].view(rows, width + pad)[:, width:])
+
+
+def test_rope_turns_back_and_differentiates(lib, torch_mod):
+    """Negative positions are the rotation's transpose, <R x, y> = <x, R' y>: its gradient."""
+    torch, t = torch_mod, Turn(torch_mod, 64, 0, 1.2)
+    x, y = randn(torch, 1, 9, 4 * 64), randn(torch, 2, 9, 4 * 64)
+    at = whole(torch, [0, 1, 2, 77, 500, 4095, 4096, 100000, 7])
+    back, rx, ry = -at, torch.empty_like(x), torch.empty_like(y)
+    lib.gncx_hip_rope_rows(x.data_ptr(), 9, 256, 4, 64, at.data_ptr(), t.ref(), 256, rx.data_ptr())
+    lib.gncx_hip_rope_rows(y.data_ptr(), 9, 256, 4, 64, back.data_ptr(), t.ref(), 256, ry.data_ptr())
+    gncx.check(lib)
+    _, tx = t(x.double().view(9, 4, 64), at)
+    _, ty = t(y.double().view(9, 4, 64), back)
+    off = (tx.view(9, -1) * y.double().abs() + ty.view(9, -1) * x.double().abs()).sum(1)
+    assert (((rx.double() * y.double()).sum(1) - (x.double() * ry.double()).sum(1)).abs() <= off).all()
+
+
+def test_rope_frequencies_on_the_device(lib, torch_mod):
+    torch = torch_mod
+    fac = np.linspace(1, 4, 32, dtype=np.float32)
+    d_fac, mag = torch.from_numpy(fac).cuda(), C.c_float()
+    out, host = torch.zeros(32, dtype=torch.float64, device="cuda"), np.zeros(32)
+    for f, o in ((d_fac.data_ptr(), out.data_ptr()), (fac.ctypes.data, host.ctypes.data)):
+        assert lib.gncx_hip_rope_frequencies(64, 1e4, gncx.ROPE_YARN, 4.0, 4096, 32.0, 1.0, f, o, C.addressof(mag)) == 0
+    assert (out.cpu().numpy() == host).all() and host[0] == 1.0
+
+
+def test_rope_refusals(lib, torch_mod):
+    torch, t = torch_mod, Turn(torch_mod, 64)
+    x, at = randn(torch, 1, 4, 128), whole(torch, [1, 2, 3, 4])
+    before = x.clone()
+
+    def call(rows=x.data_ptr(), n=4, stride=128, heads=2, hd=64, pos=at.data_ptr(), rot=t.ref(), ostride=128,
+             out=x.data_ptr()):
+        lib.gncx_hip_last_status()
+        lib.gncx_hip_rope_rows(rows, n, stride, heads, hd, pos, rot, ostride, out)
+
+    host = np.zeros(1000, np.float32)  # (kept: its address is passed)
+    for kw, text in ((dict(rows=host.ctypes.data), "memory of the library's GPU"), (dict(out=host.ctypes.data), "GPU"),
+                     (dict(pos=host.ctypes.data), "GPU"), (dict(rows=x.data_ptr() + 2), "4-byte aligned"),
+                     (dict(n=2 ** 24), "past the end"), (dict(out=x.data_ptr() + 512), "overlaps"),
+                     (dict(ostride=129), "overlap"), (dict(pos=x.data_ptr()), "overlaps"),
+                     (dict(heads=4, hd=32), "multiple of 2 up to head_dim"),
+                     (dict(rot=C.byref(gncx.Rotation(t.freqs.data_ptr(), 63, 0, 1.0))), "multiple of 2"),
+                     (dict(rot=C.byref(gncx.Rotation(t.freqs.data_ptr(), -2, 0, 1.0))), "multiple of 2"),
+                     (dict(rot=C.byref(gncx.Rotation(host.ctypes.data, 64, 0, 1.0))), "GPU"),
+                     (dict(rot=C.byref(gncx.Rotation(t.freqs.data_ptr() + 4, 64, 0, 1.0))), "8-byte aligned")):
+        call(**kw)
+        refused(lib, text)
+    assert torch.equal(x, before)
+    call(rot=None)  # no rotation: a copy onto itself
+    gncx.check(lib)
+    assert torch.equal(x, before)
+
+
+# ---- the paged cache ------------------------------------------------------------------
+class Paged:
+    """A layer's cache whose blocks hold values already (codes of N(0, 1) with scales to
+    them, what lies behind the sequences' ends and in pages of nobody NaN codes and NaN
+    scales), and the tables of some sequences.  held: tokens before the call, new: rows."""
+
+    def __init__(self, torch, held, new, H=4, KV=2, hd=64, page=32, seed=0, spare=3, room=0, size=1.0):
+        self.torch, self.held, self.new = torch, list(held), list(new)
+        self.H, self.KV, self.hd, self.page = H, KV, hd, page
+        need = [-(-(max(a, 0) + b) // page) for a, b in zip(held, new)]
+        self.max_pages = max(max(need), 1) + room
+        self.n_pages = sum(need) + spare
+        rng = np.random.default_rng(seed)
+        names = rng.permutation(self.n_pages)
+        self.table = np.full((len(held), self.max_pages), -1, np.int32)
+        at = 0
+        for s, n in enumerate(need):
+            self.table[s, :n] = names[at:at + n]
+            at += n
+        self.rows = sum(new)
+        blocks = page // BLOCK
+        self.k = torch.full((self.n_pages, KV, blocks, BLOCK, hd), 0x7f, dtype=torch.uint8, device="cuda")
+        self.v = torch.full((self.n_pages, KV, blocks, hd, BLOCK), 0xff, dtype=torch.uint8, device="cuda")
+        self.scales = torch.full((self.n_pages, KV, blocks, 2), float("nan"), device="cuda")
+        for s, a in enumerate(held):
+            if a <= 0:
+                continue
+            kk, vv = (size * randn(torch, 7 * s + i + seed, -(-a // BLOCK) * BLOCK, KV, hd) for i in (1, 2))
+            for b in range(-(-a // BLOCK)):
+                name, blk, n = int(self.table[s, b * BLOCK // page]), b * BLOCK % page // BLOCK, min(BLOCK, a - b * BLOCK)
+                for x, codes, i in ((kk, self.k, 0), (vv, self.v, 1)):
+                    y = x[b * BLOCK:b * BLOCK + n].transpose(0, 1)  # [KV][n][hd]
+                    scale = torch.exp2(torch.ceil(torch.log2(y.abs().amax((1, 2)).double() / 448))).float()
+                    q = (y / scale[:, None, None]).to(torch.float8_e4m3fn).view(torch.uint8)
+                    if i:
+                        codes[name, :, blk, :, :n] = q.transpose(1, 2)
+                    else:
+                        codes[name, :, blk, :n] = q
+                    self.scales[name, :, blk, i] = scale
+        self.starts = np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+        self.q, self.kr, self.vr = (size * randn(torch, 90 + i + seed, max(self.rows, 1), n * hd)
+                                    for i, n in enumerate((H, KV, KV)))
+        self.gamma = 1 + 0.1 * randn(torch, 5 + seed, 2, hd)
+        self.out = torch.full_like(self.q, float("nan"))
+        self.scale = 1 / math.sqrt(hd)
+        self.upload()
+
+    def upload(self):
+        torch = self.torch
+        self.d_table, self.d_len, self.d_start = (torch.from_numpy(np.array(a, np.int32)).cuda()
+                                                  for a in (self.table, self.held, self.starts))
+        self.cache = gncx.PagedCache(self.k.data_ptr(), self.v.data_ptr(), self.scales.data_ptr(), self.n_pages,
+                                     self.page, self.KV, self.hd)
+        self.batch = gncx.PagedBatch(len(self.held), self.q.shape[0], self.max_pages, self.d_start.data_ptr(),
+                                     self.d_len.data_ptr(), self.d_table.data_ptr())
+
+    def append(self, lib, turn=None, norm=-1, q=True, check=True, out=None):
+        out = self.out if out is None else out
+        lib.gncx_hip_kv_append_paged(C.byref(self.cache), C.byref(self.batch), self.q.data_ptr() if q else None,
+                                     self.kr.data_ptr(), self.vr.data_ptr(), self.H, self.gamma.data_ptr(), 0,
+                                     4 * self.hd, norm, EPS, turn.ref() if turn else None, out.data_ptr() if q else None)
+        if check:
+            gncx.check(lib)
+
+    def attend(self, lib, sw=0, check=True, q=None, out=None):
+        q, out = self.q if q is None else q, self.out if out is None else out
+        lib.gncx_hip_attention_paged(C.byref(self.cache), C.byref(self.batch), q.data_ptr(), self.H, self.scale, sw,
+                                     out.data_ptr())
+        if check:
+            gncx.check(lib)
+
+    def tokens(self, s, end):
+        """Keys and values [end][KV][hd] (64 bits) of sequence s, and which of them are there."""
+        torch = self.torch
+        names = self.table[s, [t // self.page for t in range(end)]]
+        there = torch.from_numpy((names >= 0) & (names < self.n_pages)).cuda()
+        names = torch.from_numpy(np.where((names >= 0) & (names < self.n_pages), names, 0)).cuda().long()
+        t = torch.arange(end, device="cuda")
+        blk, tok = t % self.page // BLOCK, t % BLOCK
+        f8 = torch.float8_e4m3fn
+        k = self.k.view(f8).float().double()[names, :, blk, tok] * self.scales.double()[names, :, blk, 0, None]
+        v = self.v.view(f8).float().double()[names, :, blk, :, tok] * self.scales.double()[names, :, blk, 1, None]
+        return k, v, there
+
+    def check_attention(self, q=None, out=None, sw=0):
+        """out against 64 bits.  A score is off by ds <= (2^-21 + 8 sqrt(hd) u) max_j scale
+        sum_d |q_d k_jd| (queries kept to 2^-22 each, roundings of the sum taken as
+        independent), and by 2^-23 of the row's largest |q| for elements far below it; the
+        weights are exact pieces of fp32 exponentials of 2 steps, so an output is off by
+        (2 ds + 2^-20 + 8 sqrt(N) u) sum_j w_j |v_j| / l."""
+        torch = self.torch
+        q, out = self.q if q is None else q, self.out if out is None else out
+        G = self.H // self.KV
+        for s, (a, n) in enumerate(zip(self.held, self.new)):
+            r0 = int(self.starts[s])
+            n = min(n, self.max_pages * self.page - a)
+            if n <= 0 or a < 0:
+                continue
+            k, v, there = self.tokens(s, a + n)
+            at = torch.arange(a, a + n, device="cuda")
+            key = torch.arange(a + n, device="cuda")
+            see = there[None, :] & (key[None, :] <= at[:, None])
+            if sw:
+                see &= key[None, :] > at[:, None] - sw
+            for h in range(self.H):
+                qh = q[r0:r0 + n].view(n, self.H, self.hd)[:, h].double().contiguous()
+                kh, vh = k[:, h // G].contiguous(), v[:, h // G].contiguous()
+                # a key or value may be NaN where nobody of these rows sees it, and only there
+                seen = see.any(0)[:, None]
+                kh, vh = torch.where(seen, kh, 0.0), torch.where(seen, vh, 0.0)
+                sc = torch.where(see, qh @ kh.t().contiguous() * self.scale, -math.inf)
+                size = torch.where(see, qh.abs() @ kh.abs().t().contiguous(), 0.0).amax(1, keepdim=True) * self.scale
+                far = torch.where(see, kh.abs().sum(1)[None, :], 0.0).amax(1, keepdim=True) * self.scale
+                w = torch.exp(sc - sc.amax(1, keepdim=True).clamp(min=-1e300))
+                l = w.sum(1, keepdim=True).clamp(min=1e-300)
+                want = w @ vh / l
+                ds = (2.0 ** -21 + 8 * math.sqrt(self.hd) * U) * size + 2.0 ** -36 * qh.abs().amax(1, keepdim=True) * far
+                tol = (2 * ds + 2.0 ** -20 + 8 * math.sqrt(a + n) * U) * (w @ vh.abs() / l) + 1e-37
+                got = out[r0:r0 + n].view(n, self.H, self.hd)[:, h].double()
+                assert ((got - want).abs() <= tol).all(), (s, h, float(((got - want).abs() / tol).max()))
+
+
+def nearest_e4m3(x):
+    """How far a stored value may be from x / scale: half a step, 2^-4 of it, 2^-10 below the normal ones."""
+    return (2.0 ** -4 * x.abs()).clamp(min=2.0 ** -10)
+
+
+def check_append(p, before, turn=None, norm=-1, q=True):
+    """The cache after p.append(): scales, kept and new codes, and everything else as it was;
+    out_q against the formula."""
+    torch, f8 = p.torch, p.torch.float8_e4m3fn
+    k0, v0, s0 = before
+    k, v, scales = k0.clone(), v0.clone(), s0.clone()
+    turn = turn or Turn(torch, 0)
+
+    def head(x, n, gamma, at):
+        """64-bit result and how far 32 bits may be off.  A norm's sum (positive terms) is off
+        by at most 14 of its roundings, its root by half of that; with the root, the
+        division and the products, 12 u of an element, and 12 u mag (|a| + |b|) turned."""
+        x = x.double().view(-1, n, p.hd)
+        if norm < 0:
+            return turn(x, at)
+        x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS)
+        x = x * gamma.double() if norm > 0 else x
+        y, tol = turn(x, at)
+        return y, tol * (25 / 13) + 12 * U * x.abs()
+
+    for s, (a, n) in enumerate(zip(p.held, p.new)):
+        room = p.max_pages * p.page
+        n = min(n, room - a) if 0 <= a <= room else 0
+        r0 = int(p.starts[s])
+        if n <= 0:
+            continue
+        at = torch.arange(a, a + n, device="cuda", dtype=torch.int32)
+        rows = slice(r0, r0 + n)
+        if q:
+            want, tol = head(p.q[rows], p.H, p.gamma[0], at)
+            assert ((p.out[rows].double().view(n, p.H, p.hd) - want).abs() <= tol).all()
+        wk, tk = head(p.kr[rows], p.KV, p.gamma[1], at)
+        wv = p.vr[rows].double().view(n, p.KV, p.hd)
+        pos = a
+        while pos < a + n:
+            end = min(a + n, pos // BLOCK * BLOCK + BLOCK)
+            name, blk = int(p.table[s, pos // p.page]), pos % p.page // BLOCK
+            lo, hi = pos % BLOCK, pos % BLOCK + end - pos
+            if 0 <= name < p.n_pages:
+                for i, (x, tol, codes, got) in enumerate(((wk, tk, k, p.k), (wv, 0 * wv, v, p.v))):
+                    y, t = (z[pos - a:end - a].transpose(0, 1) for z in (x, tol))  # [KV][tokens][hd]
+                    fin = torch.where(y.isfinite(), y.abs(), 0.0)
+                    most = fin.amax((1, 2))
+                    scale = torch.exp2(torch.ceil(torch.log2(most / 448)).clamp(min=-100, max=120))
+                    old = s0[name, :, blk, i].double()
+                    if lo:
+                        scale = torch.maximum(scale, old)
+                    new_scale = p.scales[name, :, blk, i].double()
+                    # (a rotated maximum within its error of the border may take either)
+                    slack = torch.where(y.isfinite(), t, 0.0).amax((1, 2))
+                    assert ((new_scale == scale) | ((most + slack > 448 * scale) & (new_scale == 2 * scale)) |
+                            ((most - slack <= 224 * scale) & (2 * new_scale == scale))).all()
+                    scales[name, :, blk, i] = p.scales[name, :, blk, i]
+                    g = got[name, :, blk].view(f8).float()
+                    c = codes[name, :, blk].view(f8).float()
+                    if i:
+                        g, c = g.transpose(1, 2), c.transpose(1, 2)
+                    if lo:
+                        kept = (c[:, :lo] * (old / new_scale).float()[:, None, None]).to(f8).float()
+                        assert torch.equal(kept.nan_to_num(nan=1e9), g[:, :lo].nan_to_num(nan=1e9))
+                    z = y / new_scale[:, None, None]
+                    off = (g[:, lo:hi].double() - z).abs()
+                    ok = torch.where(y.isfinite(), off <= nearest_e4m3(z) + t / new_scale[:, None, None], g[:, lo:hi].isnan())
+                    assert ok.all()
+                    full = got[name, :, blk].clone()
+                    if i:
+                        codes[name, :, blk, :, :hi] = full[:, :, :hi]
+                    else:
+                        codes[name, :, blk, :hi] = full[:, :hi]
+            pos = end
+    # nothing else has changed
+    assert torch.equal(k, p.k) and torch.equal(v, p.v)
+    assert torch.equal(scales.nan_to_num(nan=-1.0), p.scales.nan_to_num(nan=-1.0))
+
+
+def state(p):
+    return p.k.clone(), p.v.clone(), p.scales.clone()
+
+
+@pytest.mark.parametrize("held,new", [
+    ([0], [1]), ([5], [1]), ([15], [1]), ([16], [1]), ([31], [2]), ([0], [100]), ([7, 0, 33], [40, 0, 3]),
+    ([0, 16, 1, 47, 100, 3], [16, 16, 15, 1, 33, 0]), ([300] * 70, [1] * 70), (list(range(67)), [1 + i % 3 for i in range(67)])])
+@pytest.mark.parametrize("H,KV,hd,page,n_rot,inter,norm", [(4, 2, 64, 16, 64, 0, 1), (33, 3, 128, 32, 64, 1, 0),
+                                                            (2, 1, 256, 64, 256, 0, -1), (8, 8, 128, 128, 0, 0, 1)])
+def test_append(lib, torch_mod, held, new, H, KV, hd, page, n_rot, inter, norm):
+    p = Paged(torch_mod, held, new, H=H, KV=KV, hd=hd, page=page)
+    turn = Turn(torch_mod, n_rot, inter, 1.1) if n_rot else None
+    before = state(p)
+    p.append(lib, turn, norm)
+    check_append(p, before, turn, norm)
+    # without queries the cache is the same
+    after = state(p)
+    p.k, p.v, p.scales = (x.clone() for x in before)
+    p.upload()
+    p.append(lib, turn, norm, q=False)
+    for x, y in zip(state(p), after):
+        assert torch_mod.equal(x.nan_to_num(nan=-1.0) if x.is_floating_point() else x,
+                               y.nan_to_num(nan=-1.0) if y.is_floating_point() else y)
+
+
+def test_append_grows_a_blocks_scale_and_keeps_what_is_held(lib, torch_mod):
+    """Tokens of growing size one by one: each is there to half a step of the last scale,
+    as if all had come at once (codes above the subnormal ones move exactly)."""
+    torch = torch_mod
+    p = Paged(torch, [0], [16], H=2, KV=2, hd=64)
+    rows = (p.kr.clone(), p.vr.clone())
+    for x in rows:
+        x.mul_(2.0 ** torch.arange(16, device="cuda")[:, None] / 64)
+    p.kr, p.vr = rows
+    p.append(lib)
+    at_once = state(p)
+    p.scales.fill_(float("nan"))
+    p.starts = np.array([0, 1], np.int32)
+    for t in range(16):
+        p.held, p.new = [t], [1]
+        p.kr, p.vr = (x[t:t + 1].clone() for x in rows)
+        p.q = p.q[:1].clone()
+        p.upload()
+        p.append(lib)
+    assert torch.equal(p.scales.nan_to_num(nan=-1), at_once[2].nan_to_num(nan=-1))
+    f8 = torch.float8_e4m3fn
+    for got, want in ((p.k, at_once[0]), (p.v, at_once[1])):
+        a, b = got.view(f8).float(), want.view(f8).float()
+        same = (a == b) | (a.isnan() & b.isnan())
+        # (subnormal codes: a second rounding moves them by a step of 2^-9 at most)
+        assert (same | ((b.abs() < 2.0 ** -6) & ((a - b).abs() <= 2.0 ** -9))).all()
+
+
+def test_append_zeros_tiny_huge_and_non_finite_values(lib, torch_mod):
+    torch = torch_mod
+    p = Paged(torch, [0, 3, 0, 0, 20], [5, 4, 6, 18, 1], H=2, KV=2, hd=64)
+    r = p.starts
+    for x in (p.kr, p.vr):
+        x[r[0]:r[1]] = 0.0                       # zeros only: the least scale
+        x[r[1]:r[2]] *= 2.0 ** -120              # below the least scale's codes
+        x[r[2]:r[3]] = torch.sign(x[r[2]:r[3]]) * 3.4e38
+        x[r[3] + 2, 7] = float("inf")
+        x[r[3] + 2, 8] = float("-inf")
+        x[r[3] + 3] = float("nan")
+        x[r[3] + 17, 70] = float("nan")
+        x[r[4]] *= 1e-30                         # beside larger ones that are held
+    before = state(p)
+    p.append(lib)
+    check_append(p, before)
+    assert (p.scales[int(p.table[0, 0]), :, 0] == 2.0 ** -100).all()
+    assert (p.scales[int(p.table[2, 0]), :, 0] == 2.0 ** 120).all()
+
+
+def test_append_at_the_border_of_a_scale(lib, torch_mod):
+    """448 times a power of two is reached, the next float is not; the third row's largest
+    is 1, from the clamp, and 448 2^-8 is the first to reach it."""
+    torch = torch_mod
+    up = float(np.nextafter(np.float32(448), np.float32(1000)))
+    p = Paged(torch, [0, 0, 0], [1, 1, 1], H=2, KV=1, hd=64)
+    for x in (p.kr, p.vr):
+        x.clamp_(-1, 1)
+        x[0, 3], x[1, 3], x[2, 3] = 448.0, -up, 224.0 * 2.0 ** -10
+    p.append(lib)
+    for s, want in enumerate((1.0, 2.0, 2.0 ** -8)):
+        assert (p.scales[int(p.table[s, 0]), :, 0] == want).all()
+
+
+def test_append_leaves_rows_and_pages_that_are_not_there(lib, torch_mod):
+    """Lengths outside the table, rows past its end, pages outside the pool, rows behind the
+    last sequence: nothing of them is touched."""
+    torch = torch_mod
+    p = Paged(torch, [10, 20, 30, 76], [3, 4, 5, 8], H=4, KV=2, hd=64, page=16)
+    p.max_pages, p.table = 5, p.table[:, :5].copy()  # 80 positions: room for four of the last sequence's rows
+    p.q = randn(torch, 3, p.rows + 6, 4 * 64)
+    p.kr, p.vr = (randn(torch, 4 + i, p.rows + 6, 2 * 64) for i in range(2))
+    p.out = torch.full_like(p.q, 7.0)
+    p.held[0] = -1
+    p.table[1, 1] = p.n_pages
+    p.table[2, 2] = -2 ** 31
+    p.upload()
+    before = state(p)
+    p.append(lib)
+    keep = p.out.clone()
+    check_append(p, before)
+    assert (keep[:3] == 7).all() and (keep[12 + 4:] == 7).all() and (keep[3:16] != 7).any(1).all()
+
+
+def test_append_out_q_in_place_and_refusals(lib, torch_mod):
+    torch = torch_mod
+    p = Paged(torch, [5, 0], [2, 30], H=8, KV=2, hd=64)
+    turn = Turn(torch, 64)
+    before = state(p)
+    p.append(lib, turn, 1)
+    q, after = p.out.clone(), state(p)
+    keep = p.q.clone()
+    p.append(lib, turn, 1, out=p.q)
+    assert torch.equal(p.q, q)
+    p.q.copy_(keep)
+    base = dict(cache=p.cache, batch=p.batch, q=p.q.data_ptr(), k=p.kr.data_ptr(), v=p.vr.data_ptr(),
+                g=p.gamma.data_ptr(), rot=turn.ref(), out=p.out.data_ptr())
+
+    def call(**kw):
+        a = {**base, **kw}
+        lib.gncx_hip_last_status()
+        lib.gncx_hip_kv_append_paged(C.byref(a["cache"]), C.byref(a["batch"]), a["q"], a["k"], a["v"], 8, a["g"], 0,
+                                     256, 1, EPS, a["rot"], a["out"])
+
+    def with_(struct, **kw):
+        c = type(struct)()
+        C.pointer(c)[0] = struct
+        for n, v in kw.items():
+            setattr(c, n, v)
+        return c
+
+    memory = np.zeros(100000, np.float32)
+    host = memory.ctypes.data
+    for kw, text in ((dict(q=host), "GPU"), (dict(k=host), "GPU"), (dict(v=None), "GPU"), (dict(out=None), "GPU"),
+                     (dict(out=p.q.data_ptr() + 16), "overlaps"), (dict(k=p.kr.data_ptr() + 4), "16-byte"),
+                     (dict(out=p.kr.data_ptr()), "overlaps"),
+                     (dict(cache=with_(p.cache, scales=host)), "GPU"),
+                     (dict(cache=with_(p.cache, scales=p.scales.data_ptr() + 4)), "8-byte"),
+                     (dict(cache=with_(p.cache, n_pages=p.n_pages + 10000)), "past the end"),
+                     (dict(cache=with_(p.cache, v_pages=p.k.data_ptr())), "overlap"),
+                     (dict(cache=with_(p.cache, k_pages=p.k.data_ptr() + 8)), "16-byte"),
+                     (dict(batch=with_(p.batch, lengths=None)), "GPU"),
+                     (dict(batch=with_(p.batch, n_rows=10 ** 6)), "past the end"),
+                     (dict(batch=with_(p.batch, max_pages=10 ** 6)), "past the end"),
+                     (dict(batch=with_(p.batch, pages=p.scales.data_ptr())), "overlaps an input"),
+                     (dict(g=p.gamma.data_ptr() + 4), "16-byte"),
+                     (dict(rot=C.byref(gncx.Rotation(turn.freqs.data_ptr(), 60, 0, 1.0))), "multiple of 8"),
+                     (dict(rot=C.byref(gncx.Rotation(turn.freqs.data_ptr(), 72, 0, 1.0))), "multiple of 8")):
+        call(**kw)
+        refused(lib, text)
+    assert torch.equal(p.k, after[0]) and torch.equal(p.v, after[1])
+    assert not torch.equal(before[0], after[0])
+
+
+@pytest.mark.parametrize("H,KV,hd,page", [(4, 2, 64, 16), (32, 8, 128, 64), (8, 2, 256, 32), (5, 1, 128, 256),
+                                           (12, 4, 128, 128), (16, 16, 64, 32), (64, 1, 64, 16)])
+@pytest.mark.parametrize("held,new", [([0], [1]), ([63], [1]), ([64], [1]), ([1, 500, 17, 0], [1, 1, 1, 1]),
+                                       ([1000], [1]), ([130, 0, 700], [1, 0, 3]), ([0], [200]), ([77, 0, 300], [64, 90, 0]),
+                                       ([3000, 5], [2, 1])])
+@pytest.mark.parametrize("sw", [0, 100])
+def test_attention(lib, torch_mod, H, KV, hd, page, held, new, sw):
+    p = Paged(torch_mod, held, new, H=H, KV=KV, hd=hd, page=page, seed=3)
+    p.append(lib)
+    p.out.fill_(float("nan"))
+    p.attend(lib, sw)
+    p.check_attention(sw=sw)
+
+
+@pytest.mark.parametrize("sw", [1, 16, 17, 64, 65, 10000])
+@pytest.mark.parametrize("held,new", [([200, 40], [1, 1]), ([200, 40], [70, 33])])
+def test_attention_windows(lib, torch_mod, sw, held, new):
+    p = Paged(torch_mod, held, new, H=4, KV=2, hd=64, seed=4)
+    p.append(lib)
+    p.attend(lib, sw)
+    p.check_attention(sw=sw)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_sees_nothing_of_hidden_places(lib, torch_mod, rows):
+    """NaN and infinity-like keys and values behind a row's position, before its window, and
+    in pages that are not there; a row that sees them gets NaN."""
+    torch = torch_mod
+    p = Paged(torch, [90, 10], [rows, rows], H=4, KV=2, hd=64, page=16, seed=5)
+    p.append(lib)
+    p.attend(lib, 64)
+    clean = p.out.clone()
+    # before every window of sequence 0
+    for t in range(90 - 64 - 11, 90 - 64 + 1):
+        name, blk, tok = int(p.table[0, t // 16]), 0, t % 16
+        p.k[name, :, blk, tok] = 0x7f
+        p.v[name, :, blk, :, tok] = 0xff
+    p.attend(lib, 64)
+    assert torch.equal(p.out, clean)
+    # the last row's own key and value: NaN for that row alone, value: those floats alone
+    last = 90 + rows - 1
+    name, tok = int(p.table[0, last // 16]), last % 16
+    p.v[name, 1, 0, 5, tok] = 0x7f
+    p.k[name, 0, 0, tok, 9] = 0xff
+    p.attend(lib, 64)
+    got, want = p.out.view(2 * rows, 4, 64), clean.view(2 * rows, 4, 64)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[rows - 1, :2] = True
+    bad[rows - 1, 2:, 5] = True
+    assert torch.equal(got.isnan(), bad)
+    assert torch.equal(got[~bad], want[~bad])
+
+
+def test_attention_rows_without_anything_and_rows_that_are_none(lib, torch_mod):
+    torch = torch_mod
+    p = Paged(torch, [40, 50, 60, 70], [1, 3, 2, 2], H=4, KV=2, hd=64, page=16, seed=6)
+    p.append(lib)
+    p.q = randn(torch, 3, p.rows + 4, 4 * 64)
+    p.out = torch.full_like(p.q, 7.0)
+    p.table[0] = -1                         # nothing is there: zeros
+    p.table[1, 1] = p.n_pages               # a hole
+    p.held[2] = -5                          # no sequence
+    p.held[3] = p.max_pages * 16 - 1        # the second row is past the table
+    p.upload()
+    p.attend(lib)
+    assert (p.out[0] == 0).all()
+    assert (p.out[4:6] == 7).all() and (p.out[7:] == 7).all()
+    p.new = [0, 3, 0, 0]
+    p.check_attention()
+
+
+def test_attention_of_large_and_small_numbers(lib, torch_mod):
+    """Scores of 2^24 and more, values near the largest and the least scale, queries of very
+    different sizes, a row of zeros."""
+    torch = torch_mod
+    p = Paged(torch, [100, 100, 100, 100, 100], [1, 1, 1, 1, 2], H=4, KV=2, hd=64, seed=8)
+    p.append(lib)
+    p.q[0] *= 1e7
+    p.q[1] *= 1e-20
+    p.q[2] = 0.0
+    p.q[3, ::2] *= 1e-6
+    for s, e in ((2, 110), (3, -90)):
+        for b in range(7):
+            p.scales[int(p.table[s, b * 16 // 32]), :, b * 16 % 32 // 16, 1] *= 2.0 ** e
+    p.attend(lib)
+    p.check_attention()
+    # a block of large values that is hidden beside small ones that are seen
+    p.attend(lib, 10)
+    p.check_attention(sw=10)
+
+
+@pytest.mark.parametrize("bad", ["inf", "nan"])
+def test_attention_of_a_query_that_is_not_finite(lib, torch_mod, bad):
+    torch = torch_mod
+    p = Paged(torch, [100, 20], [1, 30], H=8, KV=2, hd=64, seed=9)
+    p.append(lib)
+    p.attend(lib)
+    want = p.out.clone()
+    p.q.view(31, 8, 64)[3, 2, 7] = float(bad)
+    p.attend(lib)
+    hit = torch.zeros(31, 8, dtype=torch.bool, device="cuda")
+    hit[3, 2] = True
+    assert p.out.view(31, 8, 64)[hit].isnan().all()
+    assert torch.equal(p.out.view(31, 8, 64)[~hit], want.view(31, 8, 64)[~hit])
+
+
+def test_shared_pages_and_reordered_sequences(lib, torch_mod):
+    """Sequences with a common beginning in the same pages, in another order: the same rows."""
+    torch = torch_mod
+    p = Paged(torch, [64, 64], [5, 5], H=4, KV=2, hd=64, seed=10)
+    p.table[1, :2] = p.table[0, :2]
+    p.upload()
+    p.append(lib)
+    p.attend(lib)
+    p.check_attention()
+    first = p.out.clone()
+    p.table = p.table[::-1].copy()
+    p.q, p.kr, p.vr = (torch.cat([x[5:], x[:5]]) for x in (p.q, p.kr, p.vr))
+    p.upload()
+    p.attend(lib)
+    assert torch.equal(torch.cat([p.out[5:], p.out[:5]]), first)
+
+
+def test_one_call_is_the_rows_of_many(lib, torch_mod):
+    """A prompt in one call, and token by token: the same cache but for a second rounding of
+    subnormal codes, outputs that agree with the cache they saw."""
+    torch = torch_mod
+    p = Paged(torch, [0, 0], [37, 20], H=4, KV=2, hd=64, seed=11)
+    turn = Turn(torch, 64)
+    p.append(lib, turn, 1)
+    rq, out, at_once = p.out.clone(), torch.empty_like(p.out), state(p)
+    p.attend(lib, q=rq, out=out)
+    p.check_attention(q=rq, out=out)
+    rows, starts, f8 = (p.kr.clone(), p.vr.clone(), p.q.clone()), p.starts, torch.float8_e4m3fn
+    p.k.fill_(0x7f)
+    p.v.fill_(0x7f)
+    for t in range(37):
+        now = [s for s in range(2) if starts[s] + t < starts[s + 1]]
+        pick = [int(starts[s]) + t for s in now]
+        p.held, p.new = [t if s in now else int(starts[s + 1] - starts[s]) for s in range(2)], [int(s in now) for s in range(2)]
+        p.starts = np.concatenate([[0], np.cumsum(p.new)]).astype(np.int32)
+        p.kr, p.vr, p.q = (x[pick].clone() for x in rows)
+        p.out = torch.empty_like(p.q)
+        p.upload()
+        p.append(lib, turn, 1)
+        assert torch.equal(p.out, rq[pick])
+        p.attend(lib, q=rq[pick].clone(), out=p.q)
+        p.check_attention(q=rq[pick], out=p.q)
+    assert torch.equal(p.scales.nan_to_num(nan=-1), at_once[2].nan_to_num(nan=-1))
+    for got, was in ((p.k, at_once[0]), (p.v, at_once[1])):
+        a, b = got.view(f8).float(), was.view(f8).float()
+        assert ((a == b) | (a.isnan() & b.isnan()) | ((b.abs() < 2.0 ** -6) & ((a - b).abs() <= 2.0 ** -9)) | b.isnan()).all()
+
+
+def test_offsets_past_4_gib(lib, torch_mod):
+    """A pool of 4.5 GiB for K and as much for V; the sequence's pages are its last ones."""
+    torch = torch_mod
+    n_pages = 9 * 2 ** 29 // (2 * 128 * 128) + 1
+    p = Paged(torch, [300], [2], H=4, KV=2, hd=128, page=128, seed=12)
+    k, v = (torch.zeros(n_pages, 2, 8, 16 * 128, dtype=torch.uint8, device="cuda") for _ in range(2))
+    scales = torch.ones(n_pages, 2, 8, 2, device="cuda")
+    assert k.numel() > 2 ** 32
+    used = [int(x) for x in p.table[0]]
+    for i, name in enumerate(used):
+        k[n_pages - 1 - i] = p.k[name].view(2, 8, -1)
+        v[n_pages - 1 - i] = p.v[name].view(2, 8, -1)
+        scales[n_pages - 1 - i] = p.scales[name]
+    want = Paged.__new__(Paged)
+    want.__dict__.update(p.__dict__)
+    want.append(lib)
+    want.out = torch.empty_like(p.q)
+    want.attend(lib)
+    p.k, p.v, p.scales, p.n_pages = k, v, scales, n_pages
+    p.table = np.array([[n_pages - 1 - i for i in range(len(used))]], np.int32)
+    p.upload()
+    p.append(lib)
+    p.attend(lib)
+    assert torch.equal(p.out, want.out)
+    for i, name in enumerate(used):
+        assert torch.equal(k[n_pages - 1 - i].view(-1), want.k[name].reshape(-1))
+    assert int(k[:n_pages - len(used)].count_nonzero()) == 0
+
+
+def test_attention_refusals(lib, torch_mod):
+    torch = torch_mod
+    p = Paged(torch, [40], [2], H=4, KV=2, hd=64)
+    p.append(lib)
+    p.out.fill_(7.0)
+    memory = np.zeros(10000, np.float32)
+    host = memory.ctypes.data
+
+    def call(q=p.q.data_ptr(), out=p.out.data_ptr(), **kw):
+        b = gncx.PagedBatch()
+        C.pointer(b)[0] = p.batch
+        for n, v in kw.items():
+            setattr(b, n, v)
+        lib.gncx_hip_last_status()
+        lib.gncx_hip_attention_paged(C.byref(p.cache), C.byref(b), q, 4, p.scale, 0, out)
+
+    for kw, text in ((dict(q=host), "GPU"), (dict(out=host), "GPU"), (dict(out=p.q.data_ptr()), "overlaps"),
+                     (dict(q=p.q.data_ptr() + 4), "16-byte"), (dict(n_rows=10 ** 6), "past the end"),
+                     (dict(out=p.scales.data_ptr()), "overlaps"), (dict(pages=host), "GPU"),
+                     (dict(row_start=None), "GPU"), (dict(max_pages=10 ** 7), "past the end")):
+        call(**kw)
+        refused(lib, text)
+    assert (p.out == 7.0).all()
+
+
+def test_captured_decode_steps(lib, torch_mod):
+    """A decode step captured once and replayed, its lengths moved on by a kernel in the
+    graph, against the same steps eagerly, with other work between the replays."""
+    torch = torch_mod
+    turn = Turn(torch, 64)
+    p = Paged(torch, [5, 40, 700], [1, 1, 1], H=4, KV=2, hd=64, page=16, room=3, seed=13)
+    names = sorted(set(range(p.n_pages)) - set(p.table[p.table >= 0].tolist()))
+    p.table[2, 44] = names[0] if p.table[2, 44] < 0 else p.table[2, 44]
+    p.upload()
+    steps = [tuple(randn(torch, 50 + 3 * i + j, 3, n * 64) for j, n in enumerate((4, 2, 2))) for i in range(4)]
+    start = state(p)
+
+    def step(i):
+        for x, y in zip((p.q, p.kr, p.vr), steps[i]):
+            x.copy_(y)
+
+    rq, out = torch.empty_like(p.q), torch.empty_like(p.q)
+    want = []
+    for i in range(4):
+        step(i)
+        p.append(lib, turn, 1, out=rq)
+        p.attend(lib, q=rq, out=out)
+        p.d_len.add_(1)
+        want.append(out.clone())
+    cache = state(p)
+    for x, y in zip((p.k, p.v, p.scales), start):
+        x.copy_(y)
+    p.d_len.copy_(whole(torch, p.held))
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    lib.gncx_hip_set_stream(stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            p.append(lib, turn, 1, out=rq)
+            p.attend(lib, q=rq, out=out)
+            p.d_len.add_(1)
+        lib.gncx_hip_set_stream(None)
+        other = Paged(torch, [900, 30], [1, 1], H=32, KV=8, hd=128, seed=14)
+        for i in range(4):
+            step(i)
+            torch.cuda.synchronize()
+            graph.replay()
+            other.append(lib)  # eager calls beside the replay
+            other.attend(lib)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[i])
+            other.check_attention()
+        for x, y in zip(state(p), cache):
+            assert torch.equal(x.float().nan_to_num(nan=-1), y.float().nan_to_num(nan=-1))
+    finally:
+        lib.gncx_hip_set_stream(None)
+
+
+def test_calls_on_another_stream(lib, torch_mod):
+    torch = torch_mod
+    p = Paged(torch, [2000, 3], [1, 1], H=32, KV=8, hd=128, seed=15)
+    p.append(lib)
+    p.attend(lib)
+    want = p.out.clone()
+    stream = torch.cuda.Stream()
+    try:
+        for i in range(4):
+            lib.gncx_hip_set_stream(stream.cuda_stream if i % 2 == 0 else None)
+            p.out.fill_(0.0)
+            torch.cuda.synchronize()
+            p.attend(lib)
+            torch.cuda.synchronize()
+            assert torch.equal(p.out, want)
+    finally:
+        lib.gncx_hip_set_stream(None)
+
+
+# ---- log probabilities ------------------------------------------------------------------
+def logprobs(lib, torch, x, tokens, n_top, entropy=True):
+    rows, vocab = x.shape
+    lp, en = (torch.full((rows,), 7.0, device="cuda") for _ in range(2))
+    words = torch.full((rows, n_top), 7, dtype=torch.int32, device="cuda")
+    best = torch.full((rows, n_top), 7.0, device="cuda")
+    lib.gncx_hip_token_logprobs(x.data_ptr(), rows, vocab, None if tokens is None else tokens.data_ptr(), n_top,
+                                None if tokens is None else lp.data_ptr(), en.data_ptr() if entropy else None,
+                                words.data_ptr() if n_top else None, best.data_ptr() if n_top else None)
+    gncx.check(lib)
+    return lp, en, words, best
+
+
+def check_logprobs(torch, x, tokens, n_top, got):
+    """Against 64 bits.  An exponential is off by 2 steps and by u |d| of its argument's
+    rounding, so log S by 4 u + u sum p |d|, a result besides by its own rounding, and the
+    entropy's sum by sum p |d| (5 u + u |d|)."""
+    lp, en, words, best = got
+    rows, vocab = x.shape
+    y = torch.where(x.isnan(), -math.inf, x.double())
+    m = y.amax(1, keepdim=True)
+    d = torch.where(y == m, 0.0, y - m).clamp(min=-1000)
+    none = (m == -math.inf)[:, 0]
+    e = torch.where(y == -math.inf, 0.0, d.exp())
+    s = e.sum(1, keepdim=True).clamp(min=1e-300)
+    p = e / s
+    lpr = torch.where(y == -math.inf, -math.inf, torch.where(y == m, 0.0, y - m) - s.log())
+    h = torch.where(none, 0.0, -(p * torch.where(p > 0, d, 0.0)).sum(1) + s.log()[:, 0])
+    spread = (p * d.abs()).sum(1)
+    t1 = 4 * U + U * spread
+    assert ((en.double() - h).abs() <= t1 + 5 * U * spread + U * (p * d * d).sum(1) + 2 * U * h.abs()).all()
+    if tokens is not None:
+        inside = (tokens >= 0) & (tokens < vocab)
+        want = lpr.gather(1, tokens.long().clamp(0, vocab - 1)[:, None])[:, 0]
+        want = torch.where(inside, want, -math.inf)
+        fin = want.isfinite()
+        assert torch.equal(lp[~fin].double(), want[~fin])
+        assert ((lp.double() - want).abs() <= t1 + 2 * U * want.abs())[fin].all()
+    if n_top:
+        z = torch.where(x.isnan(), -math.inf, x) + 0.0
+        order = torch.sort(z, dim=1, descending=True, stable=True)
+        k = min(n_top, vocab)
+        v, i = order.values[:, :k], order.indices[:, :k]
+        miss = v == -math.inf
+        assert torch.equal(words[:, :k].long(), torch.where(miss, -1, i))
+        w = torch.where(miss, -math.inf, lpr.gather(1, i))
+        fin = w.isfinite()
+        assert torch.equal(best[:, :k].double()[~fin], w[~fin])
+        assert ((best[:, :k].double() - w).abs() <= t1[:, None] + 2 * U * w.abs())[fin].all()
+        assert (words[:, k:] == -1).all() and (best[:, k:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 5), (2, 300), (1, 2047), (1, 2048), (1, 2049), (5, 4097),
+                                         (1, 50257), (64, 32000), (300, 1000), (700, 16385), (1, 151936), (9, 151936),
+                                         (1, 2 ** 22)])
+@pytest.mark.parametrize("n_top", [0, 1, 20, 64])
+def test_logprobs(lib, torch_mod, rows, vocab, n_top):
+    torch = torch_mod
+    x = 3 * randn(torch, rows + vocab, rows, vocab)
+    tokens = torch.randint(0, vocab, (rows,), device="cuda", dtype=torch.int32,
+                           generator=torch.Generator(device="cuda").manual_seed(1))
+    check_logprobs(torch, x, tokens, n_top, logprobs(lib, torch, x, tokens, n_top))
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 7), (4, 3000), (2, 60000), (700, 20000)])
+@pytest.mark.parametrize("kind", ["equal", "masked", "none", "nan", "inf", "steep", "flat", "ties", "lowest"])
+def test_logprobs_of_odd_rows(lib, torch_mod, rows, vocab, kind):
+    torch = torch_mod
+    x = 3 * randn(torch, rows + vocab, rows, vocab)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    if kind == "equal":
+        x.fill_(1.5)
+    elif kind == "masked":
+        x.masked_fill_(torch.rand(rows, vocab, generator=g, device="cuda") < 0.999, -math.inf)
+        x[:, 3] = 1.0
+    elif kind == "none":
+        x.fill_(-math.inf)
+        x[0, vocab - 1] = -3.0 if rows > 1 else -math.inf
+    elif kind == "nan":
+        x[:, 1::3] = math.nan
+    elif kind == "inf":
+        x[:, vocab // 2] = math.inf
+        x[0, vocab - 1] = math.inf
+    elif kind == "steep":
+        x *= 1e4
+    elif kind == "flat":
+        x *= 1e-6
+    elif kind == "ties":
+        x = (x * 2).round() / 2 * torch.where(x > 0, 1.0, -0.0)
+    else:
+        x[:, ::2] = torch.finfo(torch.float32).min
+    tokens = torch.randint(-2, vocab + 2, (rows,), device="cuda", dtype=torch.int32, generator=g)
+    tokens[0] = 3
+    for n_top in (0, 5, 64):
+        check_logprobs(torch, x, tokens, n_top, logprobs(lib, torch, x, tokens, n_top))
+
+
+def test_logprobs_without_some_outputs_and_refusals(lib, torch_mod):
+    torch = torch_mod
+    x = randn(torch, 1, 3, 5000)
+    tokens = whole(torch, [4, 4999, 0])
+    full = logprobs(lib, torch, x, tokens, 4)
+    lp, en, words, best = logprobs(lib, torch, x, None, 4)
+    assert (lp == 7).all() and torch.equal(en, full[1]) and torch.equal(words, full[2]) and torch.equal(best, full[3])
+    lp, en, _, _ = logprobs(lib, torch, x, tokens, 0, entropy=False)
+    assert torch.equal(lp, full[0]) and (en == 7).all()
+    memory = np.zeros(20000, np.float32)
+    out, host = torch.full((64,), 7.0, device="cuda"), memory.ctypes.data
+    o = out.data_ptr()
+
+    def call(logits=x.data_ptr(), rows=3, vocab=5000, toks=tokens.data_ptr(), top=4, lp=o, en=o + 12, w=o + 24, b=o + 72):
+        lib.gncx_hip_last_status()
+        lib.gncx_hip_token_logprobs(logits, rows, vocab, toks, top, lp, en, w, b)
+
+    for kw, text in ((dict(logits=host), "GPU"), (dict(toks=host), "GPU"), (dict(lp=host), "GPU"),
+                     (dict(rows=10 ** 5), "past the end"), (dict(en=o + 4), "two of the outputs"),
+                     (dict(w=o + 20), "two of the outputs"), (dict(b=x.data_ptr()), "overlaps an input"),
+                     (dict(lp=tokens.data_ptr()), "overlaps an input"), (dict(logits=x.data_ptr() + 2), "4-byte")):
+        call(**kw)
+        refused(lib, text)
+    assert (out == 7.0).all()
+    call()
+    gncx.check(lib)
+    assert torch.equal(out[:3], full[0]) and torch.equal(out[18:30].view(3, 4), full[3])
+
+
+def test_logprobs_captured(lib, torch_mod):
+    torch = torch_mod
+    x = torch.empty(3, 70001, device="cuda")
+    tokens = whole(torch, [0, 70000, 5])
+    outs = (torch.zeros(3, device="cuda"), torch.zeros(3, device="cuda"),
+            torch.zeros(3, 8, dtype=torch.int32, device="cuda"), torch.zeros(3, 8, device="cuda"))
+
+    def call():
+        lib.gncx_hip_token_logprobs(x.data_ptr(), 3, 70001, tokens.data_ptr(), 8, *(o.data_ptr() for o in outs))
+        gncx.check(lib)
+
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    lib.gncx_hip_set_stream(stream.cuda_stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            call()
+        lib.gncx_hip_set_stream(None)
+        for i in range(4):
+            x.copy_(3 * randn(torch, i, 3, 70001))
+            torch.cuda.synchronize()
+            graph.replay()
+            eager = logprobs(lib, torch, 3 * randn(torch, 100 + i, 40, 30000), None, 4)
+            torch.cuda.synchronize()
+            check_logprobs(torch, x, tokens, 8, outs)
+            assert eager[1].isfinite().all()
+    finally:
+        lib.gncx_hip_set_stream(None)

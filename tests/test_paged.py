@@ -1,0 +1,205 @@
+"""Many sequences at once: the rotations' frequencies, and the refusals that need
+no device: they come before any HIP call, with the outputs untouched (CPU)."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import pathlib
+import subprocess
+
+import numpy as np
+import pytest
+
+from conftest import gncx
+
+ROOT = pathlib.Path(__file__).resolve().parents[1]
+
+
+@pytest.fixture(scope="module")
+def plib():
+    return gncx.load()
+
+
+def refused(lib, text):
+    assert lib.gncx_hip_last_status() != 0
+    assert text in lib.gncx_hip_last_error().decode()
+
+
+# ---- frequencies ----------------------------------------------------------------------
+def frequencies(lib, n_rot, base=1e6, scaling=0, factor=1.0, trained=32768, fast=32.0, slow=1.0, factors=None):
+    out, mag = np.full(max(n_rot // 2, 1), -7.0), C.c_float(-7.0)
+    lib.gncx_hip_last_status()
+    rc = lib.gncx_hip_rope_frequencies(n_rot, base, scaling, factor, trained, fast, slow,
+                                       None if factors is None else factors.ctypes.data, out.ctypes.data,
+                                       C.addressof(mag))
+    return rc, out, mag.value
+
+
+@pytest.mark.parametrize("n_rot", [2, 24, 64, 128, 256])
+@pytest.mark.parametrize("base", [1e4, 1e6])
+def test_plain_and_linear_frequencies(plib, n_rot, base):
+    want = base ** (-2.0 * np.arange(n_rot // 2) / n_rot)
+    rc, got, mag = frequencies(plib, n_rot, base)
+    assert rc == 0 and mag == 1.0
+    np.testing.assert_allclose(got, want, rtol=1e-14)
+    rc, got, mag = frequencies(plib, n_rot, base, gncx.ROPE_LINEAR, 4.0)
+    assert rc == 0 and mag == 1.0
+    np.testing.assert_allclose(got, want / 4.0, rtol=1e-14)
+
+
+def test_base_scaling_stretches_the_slowest_pair_by_the_factor(plib):
+    # the last pair's exponent is (n - 2) / n, so factor^(n / (n - 2)) of the base is the factor
+    for n in (64, 128):
+        plain = frequencies(plib, n, 1e4)[1]
+        rc, got, mag = frequencies(plib, n, 1e4, gncx.ROPE_BASE, 8.0)
+        assert rc == 0 and mag == 1.0 and got[0] == 1.0
+        assert math.isclose(got[-1], plain[-1] / 8.0, rel_tol=1e-13)
+        assert (np.diff(got / plain) < 0).all()
+
+
+@pytest.mark.parametrize("n_rot,base,trained", [(128, 1e6, 32768), (64, 1e4, 4096), (128, 1e4, 2048)])
+def test_yarn_keeps_fast_pairs_and_stretches_slow_ones(plib, n_rot, base, trained):
+    plain = frequencies(plib, n_rot, base)[1]
+    rc, got, mag = frequencies(plib, n_rot, base, gncx.ROPE_YARN, 4.0, trained)
+    assert rc == 0 and math.isclose(mag, 0.1 * math.log(4.0) + 1.0, rel_tol=2e-7)
+    turns = trained * plain / (2 * math.pi)  # within the trained context
+    share = (got / plain - 0.25) / 0.75      # 1: as it is, 0: divided by the factor
+    # pairs well on either side (the borders are rounded outwards to whole pairs)
+    step = plain[0] / plain[1]
+    assert np.allclose(share[turns > 32 * step], 1.0, atol=1e-12)
+    assert np.allclose(share[turns < 1 / step], 0.0, atol=1e-12)
+    mixed = (turns < 30) & (turns > 1.1)
+    assert ((share[mixed] > 0) & (share[mixed] < 1)).all() and (np.diff(share) <= 1e-15).all()
+
+
+def test_factors_divide_and_zero_leaves(plib):
+    fac = np.linspace(1, 8, 32, dtype=np.float32)
+    fac[5] = 0
+    plain = frequencies(plib, 64)[1]
+    rc, got, _ = frequencies(plib, 64, factors=fac)
+    assert rc == 0
+    np.testing.assert_allclose(got, plain / np.where(fac == 0, 1, fac), rtol=1e-14)
+
+
+@pytest.mark.parametrize("bad", [dict(n_rot=0), dict(n_rot=3), dict(n_rot=1026), dict(n_rot=-2), dict(base=0.0),
+                                 dict(base=-1.0), dict(base=math.nan), dict(base=math.inf), dict(scaling=4),
+                                 dict(scaling=-1), dict(scaling=1, factor=0.0), dict(scaling=3, factor=math.nan),
+                                 dict(scaling=3, factor=2.0, trained=0), dict(scaling=3, factor=2.0, base=1.0),
+                                 dict(scaling=3, factor=2.0, fast=0.0), dict(scaling=3, factor=2.0, slow=-1.0),
+                                 dict(scaling=2, factor=2.0, n_rot=2)])
+def test_frequencies_refuse(plib, bad):
+    rc, got, mag = frequencies(plib, **{"n_rot": 64, **bad})
+    assert rc == -1 and (got == -7.0).all() and mag == -7.0
+    refused(plib, "n_rot is even")
+
+
+def test_frequencies_without_output(plib):
+    assert plib.gncx_hip_rope_frequencies(64, 1e4, 0, 1.0, 0, 0.0, 0.0, None, None, None) == -1
+    refused(plib, "no output")
+    out = np.zeros(32)
+    assert plib.gncx_hip_rope_frequencies(64, 1e4, 3, 2.0, 4096, 32.0, 1.0, None, out.ctypes.data, None) == -1
+    refused(plib, "no output")
+    assert plib.gncx_hip_rope_frequencies(64, 1e4, 0, 1.0, 0, 0.0, 0.0, None, out.ctypes.data, None) == 0
+    assert out[0] == 1.0
+
+
+# ---- refusals -------------------------------------------------------------------------------
+def cache(**over):
+    f = dict(k_pages=None, v_pages=None, scales=None, n_pages=4, page_tokens=32, n_kv_heads=2, head_dim=64)
+    return gncx.PagedCache(**{**f, **over})
+
+
+def batch(**over):
+    f = dict(n_seqs=2, n_rows=3, max_pages=4, row_start=None, lengths=None, pages=None)
+    return gncx.PagedBatch(**{**f, **over})
+
+
+def attend(lib, c, b, heads=4):
+    out = np.full(8, 7.0, np.float32)
+    lib.gncx_hip_last_status()
+    lib.gncx_hip_attention_paged(None if c is None else C.byref(c), None if b is None else C.byref(b), None, heads, 1.0,
+                                 0, out.ctypes.data)
+    assert (out == 7.0).all()
+
+
+def append(lib, c, b, heads=4, weight=-1):
+    out = np.full(8, 7.0, np.float32)
+    lib.gncx_hip_last_status()
+    lib.gncx_hip_kv_append_paged(None if c is None else C.byref(c), None if b is None else C.byref(b), None, None, None,
+                                 heads, None, 0, 0, weight, 1e-6, None, out.ctypes.data)
+    assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("call", [attend, append])
+def test_paged_refuses_geometry(plib, call):
+    for c in (cache(head_dim=96), cache(head_dim=0), cache(n_kv_heads=0), cache(n_kv_heads=3), cache(n_pages=0),
+              cache(page_tokens=8), cache(page_tokens=48), cache(page_tokens=512), cache(page_tokens=0),
+              cache(n_kv_heads=65536)):
+        call(plib, c, batch())
+        refused(plib, "invalid cache geometry")
+    for heads in (0, 3, -4, 65536):
+        call(plib, cache(), batch(), heads)
+        refused(plib, "invalid cache geometry")
+    for b in (batch(n_seqs=0), batch(n_seqs=65537), batch(n_rows=-1), batch(max_pages=0), batch(max_pages=2 ** 25 + 1),
+              batch(n_rows=2 ** 29)):
+        call(plib, cache(), b)
+        refused(plib, "invalid batch")
+    call(plib, None, batch())
+    refused(plib, "no cache or batch")
+    call(plib, cache(), None)
+    refused(plib, "no cache or batch")
+
+
+def test_append_refuses_missing_norm_weights(plib):
+    append(plib, cache(), batch(), weight=1)
+    refused(plib, "no norm weights")
+
+
+def test_rope_rows_refuses_geometry(plib):
+    out = np.full(8, 7.0, np.float32)
+    for rows, stride, heads, hd, ostride in ((-1, 64, 1, 64, 64), (1, 64, 0, 64, 64), (1, 64, 1, 63, 64),
+                                             (1, 64, 1, 0, 64), (1, 2048, 1, 1026, 2048), (1, 127, 2, 64, 128),
+                                             (1, 128, 2, 64, 127), (1, -128, 1, 64, 128), (1, 2 ** 30, 65536, 2, 2 ** 30)):
+        plib.gncx_hip_last_status()
+        plib.gncx_hip_rope_rows(None, rows, stride, heads, hd, None, None, ostride, out.ctypes.data)
+        refused(plib, "head_dim is even")
+    assert (out == 7.0).all()
+
+
+def test_logprobs_refuse_sizes_and_lone_outputs(plib):
+    out = np.full(8, 7.0, np.float32)
+    o = out.ctypes.data
+    for rows, vocab, top in ((-1, 10, 0), (1, 0, 0), (1, 2 ** 22 + 1, 0), (1, 10, -1), (1, 10, 65)):
+        plib.gncx_hip_last_status()
+        plib.gncx_hip_token_logprobs(None, rows, vocab, None, top, None, o, o, o)
+        refused(plib, "0 to 64 alternatives")
+    for tokens, logp, top, words, best in ((None, o, 0, None, None), (o, None, 0, None, None), (None, None, 1, None, o),
+                                           (None, None, 1, o, None)):
+        plib.gncx_hip_last_status()
+        plib.gncx_hip_token_logprobs(None, 1, 10, tokens, top, logp, None, words, best)
+        refused(plib, "come with")
+    assert (out == 7.0).all()
+
+
+def test_no_rows_are_no_error(plib):
+    plib.gncx_hip_last_status()
+    attend(plib, cache(), batch(n_rows=0))
+    append(plib, cache(), batch(n_rows=0))
+    plib.gncx_hip_rope_rows(None, 0, 0, 0, 0, None, None, 0, None)
+    plib.gncx_hip_token_logprobs(None, 0, 0, None, 0, None, None, None, None)
+    assert plib.gncx_hip_last_status() == 0
+
+
+def test_structs_match_header(tmp_path):
+    """The ctypes mirrors have the layout that the header declares."""
+    py = {"GNCXPagedCache": gncx.PagedCache, "GNCXPagedBatch": gncx.PagedBatch, "GNCXRotation": gncx.Rotation}
+    lines = ["#include <stdio.h>", "#include <stddef.h>", '#include "gncx_llm_core.h"', "int main(void) {"]
+    for s, t in py.items():
+        lines.append(f'printf("{s} sizeof %zu\\n", sizeof({s}));')
+        lines += [f'printf("{s} {f} %zu\\n", offsetof({s}, {f}));' for f, _ in t._fields_]
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-std=c11", "-I", str(ROOT / "include"), str(src), "-o", str(exe)], check=True)
+    for ln in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        s, f, v = ln.split()
+        assert (C.sizeof(py[s]) if f == "sizeof" else getattr(py[s], f).offset) == int(v), (s, f)
