@@ -229,7 +229,7 @@ struct PagedArgs {
     uint8_t* k_pages;
     uint8_t* v_pages;
     float* scales;
-    int32_t n_pages, page_tokens, n_kv, head_dim;
+    int32_t n_pages, page_bits, n_kv, head_dim;  // pages of 2^page_bits tokens
     int32_t n_seqs, n_rows, max_pages;
     const int32_t* row_start;
     const int32_t* lengths;

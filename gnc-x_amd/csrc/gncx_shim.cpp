@@ -3342,7 +3342,9 @@ bool paged_geometry(const GNCXPagedCache* c, const GNCXPagedBatch* b, int32_t n_
         set_error(where, "invalid batch (1 to 65536 sequences, up to 2^30 positions, n_rows * n_heads below 2^31)", -1);
         return false;
     }
-    a = PagedArgs{c->k_pages, c->v_pages, c->scales, c->n_pages, pt,        c->n_kv_heads, c->head_dim,
+    int32_t bits = 4;
+    while (1 << bits < pt) ++bits;
+    a = PagedArgs{c->k_pages, c->v_pages, c->scales,    c->n_pages,   bits,       c->n_kv_heads, c->head_dim,
                   b->n_seqs,  b->n_rows,  b->max_pages, b->row_start, b->lengths, b->pages};
     const size_t blocks = static_cast<size_t>(c->n_pages) * c->n_kv_heads * (pt / kKvBlock);
     z.codes = blocks * kKvBlock * c->head_dim;

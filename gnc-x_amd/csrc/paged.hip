@@ -159,7 +159,7 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedArgs& c, int s) {
     SeqRows r;
     r.row0 = clamp_row(c, c.row_start[s]);
     r.len = c.lengths[s];
-    const int32_t room = c.max_pages * c.page_tokens;
+    const int32_t room = c.max_pages << c.page_bits;
     r.count = r.len < 0 || r.len > room ? 0 : min(max(clamp_row(c, c.row_start[s + 1]) - r.row0, 0), room - r.len);
     return r;
 }
@@ -177,12 +177,21 @@ __device__ __forceinline__ int find_seq(int n_seqs, int64_t at, F&& first) {
     }
     return found - 1;
 }
+// Where a key's page stands in the table (the last one's place for keys past it, which are
+// hidden), and its block in the pool, -1 if the page is not there.
+__device__ __forceinline__ int32_t page_at(const PagedArgs& c, const int32_t* table, int32_t key) {
+    return table[min(key >> c.page_bits, c.max_pages - 1)];
+}
+__device__ __forceinline__ int64_t block_in(const PagedArgs& c, int32_t page, int head, int32_t key) {
+    const int64_t b = ((static_cast<int64_t>(page) * c.n_kv + head) << (c.page_bits - 4)) +
+                      ((key >> 4) & ((1 << (c.page_bits - 4)) - 1));
+    return static_cast<uint32_t>(page) < static_cast<uint32_t>(c.n_pages) ? b : -1;
+}
+
 // The block of a position below max_pages * page_tokens: its number in the pool's
 // [page][head] order, -1 if its page is not there.
 __device__ __forceinline__ int64_t block_of(const PagedArgs& c, int s, int head, int32_t pos) {
-    const int32_t page = c.pages[static_cast<size_t>(s) * c.max_pages + pos / c.page_tokens];
-    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.n_pages)) return -1;
-    return (static_cast<int64_t>(page) * c.n_kv + head) * (c.page_tokens / kKvBlock) + pos % c.page_tokens / kKvBlock;
+    return block_in(c, page_at(c, c.pages + static_cast<size_t>(s) * c.max_pages, pos), head, pos);
 }
 
 // ---- appending ----------------------------------------------------------------------
@@ -405,56 +414,24 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
 // 2^14), weights as three bfloat16 (24 bits, and the range of a float, so that the
 // values' scales need no care).  Scores, sums and outputs are held in 32 bits.
 constexpr int kAttnThreads = 256, kAttnWaves = 4;
-constexpr int kMaxParts = 128;
+constexpr float kInf = __builtin_inff();
 
-struct PagedParams {
-    PagedArgs c;
-    const float* q;
-    float* out;
-    float2* part_ml;  // [slot][KV head][part][row] maximum, sum
-    float* part_o;    // [slot][KV head][part][row][HD], divided by the sum
-    int32_t n_heads, group, sw, parts, least;  // least: steps of a part at least
-    float scale;      // attn_scale log2(e)
-    int64_t slots;
-};
-
-// The rows, keys and parts of a work-group.  Rows of a sequence and KV head are
-// numbered token by token, `group` heads each; tile t takes rows [R t, R t + R), and
-// sequence s has the slots from row_start[s] group / R + s on.
-struct Tile {
-    int seq, row_lo, rows, n_parts, step0, step1, per;  // steps of 64 keys; per: of a part
-    int32_t lo, hi;                                     // keys that some row may see
-    SeqRows r;
-};
-template <int R>
-__device__ __forceinline__ bool find_tile(const PagedParams& p, int64_t slot, Tile& t) {
-    const PagedArgs& c = p.c;
-    auto first = [&](int i) { return static_cast<int64_t>(clamp_row(c, c.row_start[i])) * p.group / R + i; };
-    t.seq = find_seq(c.n_seqs, slot, first);
-    if (t.seq < 0) return false;
-    t.r = seq_rows(c, t.seq);
-    const int64_t nth = slot - first(t.seq);
-    t.rows = t.r.count * p.group;
-    if (nth * R >= t.rows) return false;
-    t.row_lo = static_cast<int>(nth) * R;
-    const int32_t t0 = t.row_lo / p.group, t1 = (min(t.row_lo + R, t.rows) - 1) / p.group;
-    t.hi = t.r.len + t1 + 1;
-    t.lo = p.sw > 0 ? max(t.r.len + t0 - p.sw + 1, 0) : 0;
-    t.step0 = t.lo / 64;
-    t.step1 = (t.hi + 63) / 64;
-    const int n = t.step1 - t.step0;
-    t.per = max((n + p.parts - 1) / p.parts, p.least);
-    t.n_parts = (n + t.per - 1) / t.per;
-    return true;
+__device__ __forceinline__ uint32_t as_bits(float x) { return __builtin_bit_cast(uint32_t, x); }
+__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
+// Over the four lanes of a column: lanes 16 apart, then 32 apart.  The swap of two copies
+// leaves one of each pair in the first, the other in the second.
+template <class F>
+__device__ __forceinline__ float over_column(float v, F&& f) {
+    const auto a = __builtin_amdgcn_permlane16_swap(as_bits(v), as_bits(v), false, false);
+    v = f(as_float(a[0]), as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(as_bits(v), as_bits(v), false, false);
+    return f(as_float(b[0]), as_float(b[1]));
 }
-
 __device__ __forceinline__ float xor_max(float v) {
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
+    return over_column(v, [](float a, float b) { return fmaxf(a, b); });
 }
 __device__ __forceinline__ float xor_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
+    return over_column(v, [](float a, float b) { return a + b; });
 }
 __device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {  // of a, then b
     return __builtin_amdgcn_perm(b, a, 0x07060302u);
@@ -476,85 +453,416 @@ __device__ __forceinline__ bf16x8 codes_bf16(uint32_t w0, uint32_t w1, float sca
 // 0x80 in every byte of w that is a NaN
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// KEYS: the four waves share 16 RT rows and take every fourth step each (few rows: a
-// decode step); otherwise each has 16 RT rows of its own.
-template <int HD, int RT, bool KEYS>
-__global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(PagedParams p) {
-    constexpr int R = KEYS ? 16 * RT : 16 * RT * kAttnWaves;
-    constexpr int kSlices = HD / 64, kDims = HD / 16;
-    constexpr float kInf = __builtin_inff();
-    const PagedArgs& c = p.c;
-    const int tid = threadIdx.x, wv = tid >> 6, lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % c.n_kv;
-    const int part = static_cast<int>(blockIdx.x / c.n_kv) % p.parts;
-    const int64_t slot = blockIdx.x / c.n_kv / p.parts;
-    Tile t;
-    if (!find_tile<R>(p, slot, t) || part >= t.n_parts) return;
-    // this wave's rows, and the steps that they see
-    const int row_w = t.row_lo + (KEYS ? 0 : 16 * RT * wv);
-    if (!KEYS && row_w >= t.rows) return;
-    const int last_w = min(row_w + 16 * RT, t.rows) - 1;
-    const int32_t pos_first = t.r.len + row_w / p.group, pos_last = t.r.len + last_w / p.group;
-    const int32_t lo_w = p.sw > 0 ? max(pos_first - p.sw + 1, 0) : 0;
-    const int32_t low_most = p.sw > 0 ? max(pos_last - p.sw + 1, 0) : 0;
-    int step = t.step0 + part * t.per, step_end = min(step + t.per, t.step1);
-    if (!KEYS) {
-        step = max(step, lo_w / 64);
-        step_end = min(step_end, (pos_last + 64) / 64);
+struct PagedParams {
+    PagedArgs c;
+    const float* q;
+    float* out;
+    float2* part_ml;  // [part][row] maximum, sum
+    float* part_o;    // [part][row][HD], divided by the sum
+    int32_t n_heads, group, sw;
+    int32_t target;   // work-groups that a split aims at
+    bool split;       // whether keys are split
+    float scale;      // attn_scale log2(e)
+};
+constexpr int kTarget = 1024;    // work-groups that a split of keys aims at (64 sequences of 100 to 8000
+                                 // tokens, 8 KV heads: 512 117.5 us, 1024 and 2048 110; 60001 tokens 19.9, 19.8, 21.0)
+constexpr int kMostParts = 128;  // of a row
+constexpr int kLeastSteps = 4;   // of a part
+
+// The work of a call.  Rows of a sequence and KV head are numbered token by token,
+// `group` heads each, and cut into tiles of R; a tile's steps of 64 keys are cut into
+// parts of `per`, so many that the whole call's are about p.target work-groups'
+// (whatever the lengths are: they are read here).  Units, a tile's part each, are numbered
+// sequence by sequence.
+struct Unit {
+    int seq, tile, part, n_parts, per, first;  // first: number of the tile's first unit
+    SeqRows r;
+};
+struct SeqWork {
+    int tiles, steps;
+    SeqRows r;
+};
+template <int R>
+__device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int s) {
+    SeqWork w{0, 0, {0, 0, 0}};
+    if (s >= p.c.n_seqs) return w;
+    w.r = seq_rows(p.c, s);
+    w.tiles = (w.r.count * p.group + R - 1) / R;
+    const int lo = p.sw > 0 ? max(w.r.len - p.sw + 1, 0) / 64 : 0;
+    w.steps = w.tiles ? (w.r.len + w.r.count + 63) / 64 - lo : 0;
+    return w;
+}
+// Sum over the lanes up to this one: row_shr by 1, 2, 4 and 8 within rows of 16, then the
+// rows' totals carried up, as in wave_sum_lane63.
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ int dpp_add_int(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+}
+__device__ __forceinline__ int wave_prefix(int v) {
+    v = dpp_add_int<0x111>(v);
+    v = dpp_add_int<0x112>(v);
+    v = dpp_add_int<0x114>(v);
+    v = dpp_add_int<0x118>(v);
+    v = dpp_add_int<0x142, 0xa>(v);
+    return dpp_add_int<0x143, 0xc>(v);
+}
+// Unit `index` of the call (or, by_tile, the first unit of tile `index`), by a wave; false
+// if there is none.
+template <int R, bool BY_TILE>
+__device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit& u) {
+    const int lane = threadIdx.x & 63;
+    SeqWork w = seq_work<R>(p, lane);
+    int per = 1 << 26;  // (more steps than there can be)
+    if (p.split) {
+        float total = 0.0f;  // (of 24 bits: it only sets the split)
+        int most = 0;
+        for (int s0 = 0;;) {
+            total += static_cast<float>(w.tiles) * static_cast<float>(w.steps);
+            most = max(most, w.steps);
+            s0 += 64;
+            if (s0 >= p.c.n_seqs) break;
+            w = seq_work<R>(p, s0 + lane);
+        }
+        total = wave_sum(total);
+        most = static_cast<int>(wave_max(static_cast<float>(most)));  // (2^24 at most)
+        per = max(max(kLeastSteps, (most + kMostParts - 1) / kMostParts),
+                  static_cast<int>(ceilf(total * static_cast<float>(p.c.n_kv) / static_cast<float>(p.target))));
+        if (p.c.n_seqs > 64) w = seq_work<R>(p, lane);
     }
-    // queries: lane (n, g) has floats 64 i + 16 g + 0 .. 15 of row n, as the keys' lanes do
-    f16x8 qh[RT][2 * kSlices], ql[RT][2 * kSlices];
-    float fac[RT], m[RT], l[RT];
-    int32_t pos[RT];
-    f32x4 o[RT][kDims];
+    int units = 0, tiles = 0;  // of the sequences before
+    for (int s0 = 0; s0 < p.c.n_seqs; s0 += 64) {
+        if (s0) w = seq_work<R>(p, s0 + lane);
+        const int parts = w.steps ? (w.steps - 1) / per + 1 : 0;
+        const int to_unit = units + wave_prefix(w.tiles * parts);
+        const int to_tile = BY_TILE ? tiles + wave_prefix(w.tiles) : 0;
+        const uint64_t past = __ballot((BY_TILE ? to_tile : to_unit) > index);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            u.seq = s0 + l;
+            u.n_parts = of(parts);
+            u.per = per;
+            u.r = SeqRows{of(w.r.row0), of(w.r.count), of(w.r.len)};
+            const int before = of(to_unit - w.tiles * parts);
+            if constexpr (BY_TILE) {
+                u.tile = index - of(to_tile - w.tiles);
+                u.part = 0;
+            } else {
+                u.tile = (index - before) / u.n_parts;
+                u.part = index - before - u.tile * u.n_parts;
+            }
+            u.first = before + u.tile * u.n_parts;
+            return true;
+        }
+        units = __builtin_amdgcn_readlane(to_unit, 63);
+        if constexpr (BY_TILE) tiles = __builtin_amdgcn_readlane(to_tile, 63);
+    }
+    return false;
+}
+
+// Rows of queries as the products take them: lane (n, g) has floats 64 i + 16 g + 0 .. 15
+// of row n, as the keys' lanes do.
+template <int HD>
+__device__ __forceinline__ void split_queries(const float* q, int g, float scale, f16x8 (&qh)[HD / 32],
+                                              f16x8 (&ql)[HD / 32], float& fac) {
+    f32x4 v[HD / 64][4];
+    float most = 0.0f;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int row = min(row_w + 16 * rt + n, t.rows - 1);
-        pos[rt] = t.r.len + row / p.group;
-        const float* q = p.q + ((static_cast<size_t>(t.r.row0) + row / p.group) * p.n_heads + hk * p.group + row % p.group) * HD;
-        f32x4 v[kSlices][4];
-        float most = 0.0f;
+    for (int i = 0; i < HD / 64; ++i)
 #pragma unroll
-        for (int i = 0; i < kSlices; ++i)
+        for (int j = 0; j < 4; ++j) {
+            v[i][j] = *reinterpret_cast<const f32x4*>(q + 64 * i + 16 * g + 4 * j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(v[i][j][k]));
+        }
+    most = xor_max(most);
+    int e = 0;
+    (void)frexpf(most, &e);
+    e = most > 0.0f && most < kInf ? e - 14 : 0;
+    fac = ldexpf(scale, e);
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            const float x = ldexpf(v[i][j / 4][j % 4], -e);
+            const _Float16 h = static_cast<_Float16>(x);
+            qh[2 * i + j / 8][j % 8] = h;
+            ql[2 * i + j / 8][j % 8] = static_cast<_Float16>(x - static_cast<float>(h));
+        }
+}
+
+// A row's running maximum, sum (of this lane's keys) and output.
+template <int HD>
+struct RowState {
+    float m = -kInf, l = 0.0f;
+    f32x4 o[HD / 16];
+    __device__ RowState() {
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // Scores (of this lane's 16 keys, those in `seen` seen) to weights, as the products
+    // take them: e = three numbers of 8 bits, cut off one after the other, nothing lost.
+    __device__ __forceinline__ void weigh(const f32x4 (&s)[4], float f, uint32_t seen, bool full, bf16x8 (&w)[2][3]) {
+        float x[16], most = -kInf;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[j] = s[j / 4][j % 4] * f;
+        if (!full)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) x[j] = seen >> j & 1u ? x[j] : -kInf;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
+        const float mx = fmaxf(m, xor_max(most)), use = mx == -kInf ? 0.0f : mx;
+        const float alpha = __builtin_amdgcn_exp2f(m - use);
+        m = mx;
+        float sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            uint32_t a[4], b[4], c[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[i][j] = *reinterpret_cast<const f32x4*>(q + 64 * i + 16 * g + 4 * j);
+                uint32_t h[2], md[2], lw[2];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(v[i][j][k]));
+                for (int i = 0; i < 2; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(x[8 * k + 2 * j + i] - use);
+                    sum += e;
+                    h[i] = __builtin_bit_cast(uint32_t, e) & 0xffff0000u;
+                    const float r1 = e - __builtin_bit_cast(float, h[i]);
+                    md[i] = __builtin_bit_cast(uint32_t, r1) & 0xffff0000u;
+                    lw[i] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, md[i]));
+                }
+                a[j] = high_halves(h[0], h[1]);
+                b[j] = high_halves(md[0], md[1]);
+                c[j] = high_halves(lw[0], lw[1]);
             }
-        most = xor_max(most);
-        int e = 0;
-        (void)frexpf(most, &e);
-        e = most > 0.0f && most < kInf ? e - 14 : 0;
-        fac[rt] = ldexpf(p.scale, e);
+            w[k][0] = __builtin_bit_cast(bf16x8, make_uint4(a[0], a[1], a[2], a[3]));
+            w[k][1] = __builtin_bit_cast(bf16x8, make_uint4(b[0], b[1], b[2], b[3]));
+            w[k][2] = __builtin_bit_cast(bf16x8, make_uint4(c[0], c[1], c[2], c[3]));
+        }
+        l = l * alpha + sum;
+        // (most steps leave every row's maximum as it is)
+        if (__any(alpha != 1.0f))
 #pragma unroll
-        for (int i = 0; i < kSlices; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float x = ldexpf(v[i][j / 4][j % 4], -e);
-                const _Float16 h = static_cast<_Float16>(x);
-                qh[rt][2 * i + j / 8][j % 8] = h;
-                ql[rt][2 * i + j / 8][j % 8] = static_cast<_Float16>(x - static_cast<float>(h));
-            }
-        m[rt] = -kInf;
-        l[rt] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) o[rt][d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
     }
-    const int32_t room = c.max_pages * c.page_tokens;
-    for (step += KEYS ? wv : 0; step < step_end; step += KEYS ? kAttnWaves : 1) {
-        const int32_t k0 = 64 * step;
-        // the lane's block of K (rows of the product), and of V, scores and scales
-        const int32_t at_k = k0 + 16 * (n >> 2), at_v = k0 + 16 * g;
-        const int64_t bk = at_k < room ? block_of(c, t.seq, hk, at_k) : -1;
-        const int64_t bv = at_v < room ? block_of(c, t.seq, hk, at_v) : -1;
-        // (a block that is not there: the first one is read, and hidden)
+    __device__ __forceinline__ void add(int d, bf16x8 a, bf16x8 b, const bf16x8 (&w)[2][3]) {
+#pragma unroll
+        for (int k = 2; k >= 0; --k) {
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[0][k], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, w[1][k], o[d], 0, 0, 0);
+        }
+    }
+    // The same without the NaN codes among a's and b's sources, then NaN where this row
+    // sees one of them (na, nb: one for each): a step that is not seen whole.
+    __device__ __forceinline__ void add_nan(int d, bf16x8 na, bf16x8 nb, uint32_t seen) {
+        auto ones = [&](int j) {
+            return ((seen >> j & 1u) ? 0x3f80u : 0u) | ((seen >> (j + 1) & 1u) ? 0x3f800000u : 0u);
+        };
+        f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
+        count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            na, __builtin_bit_cast(bf16x8, make_uint4(ones(0), ones(2), ones(4), ones(6))), count, 0, 0, 0);
+        count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            nb, __builtin_bit_cast(bf16x8, make_uint4(ones(8), ones(10), ones(12), ones(14))), count, 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (count[r] > 0.0f) o[d][r] = __builtin_nanf("");
+    }
+};
+// Keys at .. at + 15 that the row at pos sees, one bit each
+__device__ __forceinline__ uint32_t seen_bits(int32_t at, int32_t pos, int32_t sw) {
+    auto below = [&](int32_t n) {  // keys below n
+        const int32_t k = min(max(n - at, 0), 16);
+        return (1u << k) - 1u;
+    };
+    const uint32_t in = below(pos + 1);
+    return sw > 0 ? in & ~below(max(pos - sw + 1, 0)) : in;
+}
+__device__ __forceinline__ float* row_of(float* base, const PagedParams& p, const SeqRows& r, int hk, int row, int hd) {
+    return base + ((static_cast<size_t>(r.row0) + row / p.group) * p.n_heads + hk * p.group + row % p.group) * hd;
+}
+
+// Few rows a sequence (a decode step): a work-group has 16 rows, and its four waves take
+// every fourth step each.
+template <int HD>
+__global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_kernel(PagedParams p) {
+    constexpr int R = 16, kSlices = HD / 64, kDims = HD / 16;
+    // the waves' parts of a row (a row of HD + 4 floats: no two rows on the same banks)
+    __shared__ __align__(16) float os[kAttnWaves][R][HD + 4];
+    __shared__ float2 mls[kAttnWaves][R];
+    const PagedArgs& c = p.c;
+    const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x % c.n_kv, unit = blockIdx.x / c.n_kv;
+    Unit u;
+    if (!find_unit<R, false>(p, unit, u)) return;
+    const int rows = u.r.count * p.group, row_lo = u.tile * R, row_hi = min(row_lo + R, rows);
+    const int32_t pos_first = u.r.len + row_lo / p.group, pos_last = u.r.len + (row_hi - 1) / p.group;
+    const int32_t low_first = p.sw > 0 ? max(pos_first - p.sw + 1, 0) : 0;
+    const int32_t low_last = p.sw > 0 ? max(pos_last - p.sw + 1, 0) : 0;
+    const int step0 = (p.sw > 0 ? max(u.r.len - p.sw + 1, 0) / 64 : 0) + u.part * u.per;
+    const int step1 = min(step0 + u.per, pos_last / 64 + 1);
+    const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
+    int step = step0 + wv;
+    // keys of a step that this lane's blocks begin at: of K, whose rows it loads, and of V
+    const int at_k = 16 * (n >> 2), at_v = 16 * g;
+    int32_t page_k = page_at(c, table, 64 * step + at_k), page_v = page_at(c, table, 64 * step + at_v);
+    const int row = min(row_lo + n, rows - 1);
+    const int32_t pos = u.r.len + row / p.group;
+    f16x8 qh[HD / 32], ql[HD / 32];
+    float fac;
+    split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, qh, ql, fac);
+    RowState<HD> st;
+    // (a block that is not there: the first one is read, and hidden)
+    uint4 kw[4][kSlices], vw[kDims];
+    auto load_k = [&](int64_t b) {
+        const uint8_t* from = c.k_pages + max(b, int64_t{0}) * (kKvBlock * HD) + (n & 3) * HD + 16 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i) kw[j][i] = *reinterpret_cast<const uint4*>(from + 4 * j * HD + 64 * i);
+    };
+    float2 scale;
+    auto in_order = [] { asm volatile("" ::: "memory"); };
+    auto load_v = [&](int64_t b) {
+        scale = *reinterpret_cast<const float2*>(c.scales + 2 * max(b, int64_t{0}));
+        in_order();
+        const uint8_t* from = c.v_pages + max(b, int64_t{0}) * (kKvBlock * HD) + 16 * n;
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) vw[d] = *reinterpret_cast<const uint4*>(from + 256 * d);
+    };
+    // Loads return in the order of their issue, so that what is waited for first goes out
+    // first: the pages of the step after next, the next step's keys while this one's scores
+    // are weighed, its values when this one's are used up.  Behind the last step the
+    // first block is read, from the caches.
+    int64_t bv = block_in(c, page_v, hk, 64 * step + at_v);
+    load_k(block_in(c, page_k, hk, 64 * step + at_k));
+    page_k = page_at(c, table, 64 * (step + kAttnWaves) + at_k);
+    page_v = page_at(c, table, 64 * (step + kAttnWaves) + at_v);
+    in_order();
+    load_v(bv);
+    for (; step < step1; step += kAttnWaves) {
+        const int32_t k0 = 64 * step, next = step + kAttnWaves;
+        f32x4 s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i) {
+                const f16x8 a = codes_f16(kw[j][i].x, kw[j][i].y), b = codes_f16(kw[j][i].z, kw[j][i].w);
+                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[2 * i], s[j], 0, 0, 0);
+                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[2 * i + 1], s[j], 0, 0, 0);
+                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[2 * i], s[j], 0, 0, 0);
+                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[2 * i + 1], s[j], 0, 0, 0);
+            }
+        }
+        const bool there = bv >= 0 && k0 + at_v <= pos_last && k0 + at_v + 16 > low_first;
+        const bool full = k0 + 63 <= pos_first && k0 >= low_last && __ballot(there) == ~uint64_t{0};
+        const uint32_t seen = there ? seen_bits(k0 + at_v, pos, p.sw) : 0u;
+        const bool more = next < step1;
+        const int64_t next_k = more ? block_in(c, page_k, hk, 64 * next + at_k) : 0;
+        bv = more ? block_in(c, page_v, hk, 64 * next + at_v) : 0;
+        page_k = page_at(c, table, 64 * (next + kAttnWaves) + at_k);
+        page_v = page_at(c, table, 64 * (next + kAttnWaves) + at_v);
+        load_k(next_k);
+        const float2 sc = there ? scale : make_float2(1.0f, 1.0f);
+        bf16x8 w[2][3];
+        st.weigh(s, fac * sc.x, seen, full, w);
+        // NaN codes of V, which rows that do not see them must not meet (0 NaN is NaN), are
+        // taken out of a step that is not seen whole, and met by a product of their own
+        uint32_t bad = 0;
+        if (!full)
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+                bad |= nan_bytes(vw[d].x) | nan_bytes(vw[d].y) | nan_bytes(vw[d].z) | nan_bytes(vw[d].w);
+        if (!__any(bad != 0)) {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d)
+                st.add(d, codes_bf16(vw[d].x, vw[d].y, sc.y), codes_bf16(vw[d].z, vw[d].w, sc.y), w);
+        } else {
+#pragma unroll
+            for (int d = 0; d < kDims; ++d) {
+                const uint32_t z[4] = {nan_bytes(vw[d].x) >> 7, nan_bytes(vw[d].y) >> 7, nan_bytes(vw[d].z) >> 7,
+                                       nan_bytes(vw[d].w) >> 7};
+                st.add(d, codes_bf16(vw[d].x & ~(z[0] * 0xffu), vw[d].y & ~(z[1] * 0xffu), sc.y),
+                       codes_bf16(vw[d].z & ~(z[2] * 0xffu), vw[d].w & ~(z[3] * 0xffu), sc.y), w);
+                // (0x38: one)
+                st.add_nan(d, codes_bf16(z[0] * 0x38u, z[1] * 0x38u, 1.0f), codes_bf16(z[2] * 0x38u, z[3] * 0x38u, 1.0f),
+                           seen);
+            }
+        }
+        load_v(bv);
+        // (otherwise the compiler joins these loads with those before the loop, at its top)
+        asm volatile("; the next step's values are on their way" ::: "memory");
+    }
+    const float l = xor_sum(st.l);
+    // divided by the sum here, before the parts' weights meet the values
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    if (g == 0) mls[wv][n] = make_float2(st.m, l);
+#pragma unroll
+    for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(&os[wv][n][16 * d + 4 * g]) = st.o[d] * inv;
+    __syncthreads();
+    // (a unit's parts: [unit][KV head][row])
+    const size_t part_row = (static_cast<size_t>(unit) * c.n_kv + hk) * R;
+    for (int i = tid; i < (row_hi - row_lo) * (HD / 4); i += kAttnThreads) {
+        const int r = i / (HD / 4), d = i % (HD / 4);
+        float M = -kInf, L = 0.0f, wt[kAttnWaves];
+#pragma unroll
+        for (int k = 0; k < kAttnWaves; ++k) M = fmaxf(M, mls[k][r].x);
+        const float use = M == -kInf ? 0.0f : M;
+#pragma unroll
+        for (int k = 0; k < kAttnWaves; ++k) {
+            wt[k] = mls[k][r].y * __builtin_amdgcn_exp2f(mls[k][r].x - use);
+            L += wt[k];
+        }
+        const float share = L != 0.0f ? 1.0f / L : 0.0f;
+        f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < kAttnWaves; ++k)
+            if (wt[k] != 0.0f) x += (wt[k] * share) * *reinterpret_cast<const f32x4*>(&os[k][r][4 * d]);
+        float* to = row_of(p.out, p, u.r, hk, row_lo + r, HD);
+        if (u.n_parts > 1) {
+            if (d == 0) p.part_ml[part_row + r] = make_float2(M, L);
+            to = p.part_o + (part_row + r) * HD;
+        }
+        *reinterpret_cast<f32x4*>(to + 4 * d) = x;
+    }
+}
+
+// Many rows (prompts): a wave has 16 RT rows of its own, a work-group four times as many.
+template <int HD, int RT>
+__global__ __launch_bounds__(kAttnThreads) void paged_rows_kernel(PagedParams p) {
+    constexpr int R = 16 * RT * kAttnWaves, kSlices = HD / 64, kDims = HD / 16;
+    const PagedArgs& c = p.c;
+    const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x % c.n_kv, unit = blockIdx.x / c.n_kv;
+    Unit u;
+    if (!find_unit<R, false>(p, unit, u)) return;
+    const int rows = u.r.count * p.group, row_lo = u.tile * R + 16 * RT * wv, row_hi = min(row_lo + 16 * RT, rows);
+    if (row_lo >= rows) return;
+    const int32_t pos_first = u.r.len + row_lo / p.group, pos_last = u.r.len + (row_hi - 1) / p.group;
+    const int32_t low_first = p.sw > 0 ? max(pos_first - p.sw + 1, 0) : 0;
+    const int32_t low_last = p.sw > 0 ? max(pos_last - p.sw + 1, 0) : 0;
+    const int step0 = (p.sw > 0 ? max(u.r.len - p.sw + 1, 0) / 64 : 0) + u.part * u.per;
+    const int step1 = min(step0 + u.per, pos_last / 64 + 1);
+    const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
+    f16x8 qh[RT][HD / 32], ql[RT][HD / 32];
+    float fac[RT];
+    int32_t pos[RT];
+    RowState<HD> st[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const int row = min(row_lo + 16 * rt + n, rows - 1);
+        pos[rt] = u.r.len + row / p.group;
+        split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, qh[rt], ql[rt], fac[rt]);
+    }
+    for (int step = max(step0, low_first / 64); step < step1; ++step) {
+        const int32_t k0 = 64 * step, at_k = k0 + 16 * (n >> 2), at_v = k0 + 16 * g;
+        const int64_t bk = block_in(c, page_at(c, table, at_k), hk, at_k);
+        const int64_t bv = block_in(c, page_at(c, table, at_v), hk, at_v);
         const uint8_t* kp = c.k_pages + (bk < 0 ? 0 : bk) * (kKvBlock * HD) + (n & 3) * HD + 16 * g;
         const uint8_t* vp = c.v_pages + (bv < 0 ? 0 : bv) * (kKvBlock * HD) + 16 * n;
-        float2 scale = *reinterpret_cast<const float2*>(c.scales + 2 * (bv < 0 ? 0 : bv));
-        const bool there = bv >= 0 && at_v < t.hi && at_v + 16 > t.lo;
-        if (!there) scale = make_float2(1.0f, 1.0f);
-        const bool full = k0 + 63 <= pos_first && k0 >= low_most && __ballot(there) == ~uint64_t{0};
+        float2 sc = *reinterpret_cast<const float2*>(c.scales + 2 * (bv < 0 ? 0 : bv));
+        const bool there = bv >= 0 && at_v <= pos_last && at_v + 16 > low_first;
+        if (!there) sc = make_float2(1.0f, 1.0f);
+        const bool full = k0 + 63 <= pos_first && k0 >= low_last && __ballot(there) == ~uint64_t{0};
         uint4 kw[4][kSlices], vw[kDims];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -579,240 +887,178 @@ __global__ __launch_bounds__(kAttnThreads) void paged_attn_kernel(PagedParams p)
                 }
             }
         }
-        // NaN codes of V, which rows that do not see them must not meet (0 NaN is NaN), are
-        // taken out of a step that is not seen whole, and met by a product of their own
-        uint32_t bad = 0;
+        uint32_t bad = 0, seen[RT];
         if (!full)
 #pragma unroll
             for (int d = 0; d < kDims; ++d)
                 bad |= nan_bytes(vw[d].x) | nan_bytes(vw[d].y) | nan_bytes(vw[d].z) | nan_bytes(vw[d].w);
-        const bool clean = !__any(bad != 0);
-        bf16x8 w[RT][2][3], sees[RT][2];
+        bf16x8 w[RT][2][3];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-            const float f = fac[rt] * scale.x;
-            float x[16], most = -kInf;
-            uint32_t seen = 0xffffu;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = s[rt][j / 4][j % 4] * f;
-            if (!full) {
-                const int32_t low = p.sw > 0 ? pos[rt] - p.sw + 1 : 0;
-                seen = 0;
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const bool in = there && at_v + j <= pos[rt] && at_v + j >= low;
-                    x[j] = in ? x[j] : -kInf;
-                    seen |= in ? 1u << j : 0u;
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
-            const float mx = fmaxf(m[rt], xor_max(most)), use = mx == -kInf ? 0.0f : mx;
-            const float alpha = __builtin_amdgcn_exp2f(m[rt] - use);
-            m[rt] = mx;
-            float sum = 0.0f;
-            uint32_t h[16], md[16], lw[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const float e = __builtin_amdgcn_exp2f(x[j] - use);
-                sum += e;
-                // e = three numbers of 8 bits, cut off one after the other: nothing is lost
-                h[j] = __builtin_bit_cast(uint32_t, e) & 0xffff0000u;
-                const float r1 = e - __builtin_bit_cast(float, h[j]);
-                md[j] = __builtin_bit_cast(uint32_t, r1) & 0xffff0000u;
-                lw[j] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, md[j]));
-            }
-            l[rt] = l[rt] * alpha + sum;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                uint4 a, b, cc, dd;
-                a = make_uint4(high_halves(h[8 * k], h[8 * k + 1]), high_halves(h[8 * k + 2], h[8 * k + 3]),
-                               high_halves(h[8 * k + 4], h[8 * k + 5]), high_halves(h[8 * k + 6], h[8 * k + 7]));
-                b = make_uint4(high_halves(md[8 * k], md[8 * k + 1]), high_halves(md[8 * k + 2], md[8 * k + 3]),
-                               high_halves(md[8 * k + 4], md[8 * k + 5]), high_halves(md[8 * k + 6], md[8 * k + 7]));
-                cc = make_uint4(high_halves(lw[8 * k], lw[8 * k + 1]), high_halves(lw[8 * k + 2], lw[8 * k + 3]),
-                                high_halves(lw[8 * k + 4], lw[8 * k + 5]), high_halves(lw[8 * k + 6], lw[8 * k + 7]));
-                w[rt][k][0] = __builtin_bit_cast(bf16x8, a);
-                w[rt][k][1] = __builtin_bit_cast(bf16x8, b);
-                w[rt][k][2] = __builtin_bit_cast(bf16x8, cc);
-                auto one = [&](int j) {
-                    return ((seen >> j & 1u) ? 0x3f80u : 0u) | ((seen >> (j + 1) & 1u) ? 0x3f800000u : 0u);
-                };
-                dd = make_uint4(one(8 * k), one(8 * k + 2), one(8 * k + 4), one(8 * k + 6));
-                sees[rt][k] = __builtin_bit_cast(bf16x8, dd);
-            }
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) o[rt][d] *= alpha;
+            seen[rt] = there ? seen_bits(at_v, pos[rt], p.sw) : 0u;
+            st[rt].weigh(s[rt], fac[rt] * sc.x, seen[rt], full, w[rt]);
         }
-        if (clean) {
+        if (!__any(bad != 0)) {
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
-                const bf16x8 a = codes_bf16(vw[d].x, vw[d].y, scale.y), b = codes_bf16(vw[d].z, vw[d].w, scale.y);
+                const bf16x8 a = codes_bf16(vw[d].x, vw[d].y, sc.y), b = codes_bf16(vw[d].z, vw[d].w, sc.y);
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                    for (int k = 2; k >= 0; --k) {
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[rt][0][k], o[rt][d], 0, 0, 0);
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, w[rt][1][k], o[rt][d], 0, 0, 0);
-                    }
+                for (int rt = 0; rt < RT; ++rt) st[rt].add(d, a, b, w[rt]);
             }
         } else {
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
                 const uint32_t z[4] = {nan_bytes(vw[d].x) >> 7, nan_bytes(vw[d].y) >> 7, nan_bytes(vw[d].z) >> 7,
                                        nan_bytes(vw[d].w) >> 7};
-                const bf16x8 a = codes_bf16(vw[d].x & ~(z[0] * 0xffu), vw[d].y & ~(z[1] * 0xffu), scale.y);
-                const bf16x8 b = codes_bf16(vw[d].z & ~(z[2] * 0xffu), vw[d].w & ~(z[3] * 0xffu), scale.y);
+                const bf16x8 a = codes_bf16(vw[d].x & ~(z[0] * 0xffu), vw[d].y & ~(z[1] * 0xffu), sc.y);
+                const bf16x8 b = codes_bf16(vw[d].z & ~(z[2] * 0xffu), vw[d].w & ~(z[3] * 0xffu), sc.y);
                 const bf16x8 na = codes_bf16(z[0] * 0x38u, z[1] * 0x38u, 1.0f);  // (0x38: one)
                 const bf16x8 nb = codes_bf16(z[2] * 0x38u, z[3] * 0x38u, 1.0f);
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
-#pragma unroll
-                    for (int k = 2; k >= 0; --k) {
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[rt][0][k], o[rt][d], 0, 0, 0);
-                        o[rt][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, w[rt][1][k], o[rt][d], 0, 0, 0);
-                    }
-                    f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
-                    count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(na, sees[rt][0], count, 0, 0, 0);
-                    count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(nb, sees[rt][1], count, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (count[r] > 0.0f) o[rt][d][r] = __builtin_nanf("");
+                    st[rt].add(d, a, b, w[rt]);
+                    st[rt].add_nan(d, na, nb, seen[rt]);
                 }
             }
         }
     }
-    // out: floats 16 d + 4 g .. + 3 of row n
-    const size_t part_row = ((static_cast<size_t>(slot) * c.n_kv + hk) * p.parts + part) * R;
-    auto out_of = [&](int row) {  // row of the sequence
-        return p.out + ((static_cast<size_t>(t.r.row0) + row / p.group) * p.n_heads + hk * p.group + row % p.group) * HD;
-    };
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        l[rt] = xor_sum(l[rt]);
-        // divided by the sum here, before the parts' weights meet the values
-        const float inv = l[rt] != 0.0f ? 1.0f / l[rt] : 0.0f;
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) o[rt][d] *= inv;
-    }
-    if constexpr (!KEYS) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int row = row_w + 16 * rt + n;
-            if (row >= t.rows) continue;
-            float* to = out_of(row);
-            if (t.n_parts > 1) {
-                const size_t i = part_row + row - t.row_lo;
-                if (g == 0) p.part_ml[i] = make_float2(m[rt], l[rt]);
-                to = p.part_o + i * HD;
-            }
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(to + 16 * d + 4 * g) = o[rt][d];
+        const float l = xor_sum(st[rt].l), inv = l != 0.0f ? 1.0f / l : 0.0f;
+        const int row = row_lo + 16 * rt + n;
+        if (row >= rows) continue;
+        float* to = row_of(p.out, p, u.r, hk, row, HD);
+        if (u.n_parts > 1) {
+            const size_t i = (static_cast<size_t>(unit) * c.n_kv + hk) * R + row - u.tile * R;
+            if (g == 0) p.part_ml[i] = make_float2(st[rt].m, l);
+            to = p.part_o + i * HD;
         }
-    } else {
-        // the waves' parts of a row meet in LDS (a row of HD + 4 floats: no two rows on the same banks)
-        __shared__ __align__(16) float os[kAttnWaves][R][HD + 4];
-        __shared__ float2 mls[kAttnWaves][R];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (g == 0) mls[wv][16 * rt + n] = make_float2(m[rt], l[rt]);
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(&os[wv][16 * rt + n][16 * d + 4 * g]) = o[rt][d];
-        }
-        __syncthreads();
-        const int rows = min(R, t.rows - t.row_lo);
-        for (int i = tid; i < rows * (HD / 4); i += kAttnThreads) {
-            const int row = i / (HD / 4), d = i % (HD / 4);
-            float M = -kInf, L = 0.0f, wt[kAttnWaves];
-#pragma unroll
-            for (int k = 0; k < kAttnWaves; ++k) M = fmaxf(M, mls[k][row].x);
-            const float use = M == -kInf ? 0.0f : M;
-#pragma unroll
-            for (int k = 0; k < kAttnWaves; ++k) {
-                wt[k] = mls[k][row].y * __builtin_amdgcn_exp2f(mls[k][row].x - use);
-                L += wt[k];
-            }
-            const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < kAttnWaves; ++k)
-                if (wt[k] != 0.0f) x += (wt[k] * inv) * *reinterpret_cast<const f32x4*>(&os[k][row][4 * d]);
-            float* to = out_of(t.row_lo + row);
-            if (t.n_parts > 1) {
-                if (d == 0) p.part_ml[part_row + row] = make_float2(M, L);
-                to = p.part_o + (part_row + row) * HD;
-            }
-            *reinterpret_cast<f32x4*>(to + 4 * d) = x;
-        }
+        for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(to + 16 * d + 4 * g) = st[rt].o[d] * inv;
     }
 }
 
-// out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the parts c.
+// out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the parts c.  HD / 4
+// threads have a row's floats; up to kAtOnce parts they have the row to themselves, more
+// parts are shared by the work-group, whose sums then meet in LDS.
 template <int HD, int R>
 __global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedParams p) {
+    constexpr int kCols = HD / 4, kWide = kAttnThreads / kCols, kAtOnce = 8;
+    __shared__ __align__(16) f32x4 sums[kWide][kCols];
+    __shared__ float2 mls[kWide];
     const PagedArgs& c = p.c;
-    const int hk = blockIdx.x % c.n_kv;
-    const int64_t slot = blockIdx.x / c.n_kv;
-    Tile t;
-    if (!find_tile<R>(p, slot, t) || t.n_parts == 1) return;
-    const size_t base = (static_cast<size_t>(slot) * c.n_kv + hk) * p.parts * R;
-    const int rows = min(R, t.rows - t.row_lo);
-    for (int i = threadIdx.x; i < rows * (HD / 4); i += kAttnThreads) {
-        const int row = i / (HD / 4), d = i % (HD / 4);
-        float M = -__builtin_inff(), L = 0.0f;
-        for (int k = 0; k < t.n_parts; ++k) M = fmaxf(M, p.part_ml[base + static_cast<size_t>(k) * R + row].x);
-        const float use = M == -__builtin_inff() ? 0.0f : M;
-        for (int k = 0; k < t.n_parts; ++k) {
-            const float2 ml = p.part_ml[base + static_cast<size_t>(k) * R + row];
-            L += ml.y * __builtin_amdgcn_exp2f(ml.x - use);
-        }
-        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+    const int hk = blockIdx.x % c.n_kv, tile = blockIdx.x / c.n_kv;
+    Unit u;
+    if (!find_unit<R, true>(p, tile, u) || u.n_parts == 1) return;
+    const int col = threadIdx.x % kCols, k0 = threadIdx.x / kCols;
+    const int rows = min(u.r.count * p.group - u.tile * R, R);
+    const size_t stride = static_cast<size_t>(c.n_kv) * R;
+    // a row's parts first, first + every, ..: M, L and x, their mean
+    struct Mean {
+        float M = -kInf, L = 0.0f;
         f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = 0; k < t.n_parts; ++k) {
-            const size_t at = base + static_cast<size_t>(k) * R + row;
-            const float2 ml = p.part_ml[at];
-            const float w = ml.y * __builtin_amdgcn_exp2f(ml.x - use);
-            if (w != 0.0f) x += (w * inv) * *reinterpret_cast<const f32x4*>(p.part_o + at * HD + 4 * d);
+    };
+    auto parts_of = [&](int r, int first, int every) {
+        const size_t base = (static_cast<size_t>(u.first) * c.n_kv + hk) * R + r;
+        Mean s;
+        for (int k1 = first; k1 < u.n_parts; k1 += every * kAtOnce) {
+            float2 ml[kAtOnce];
+            f32x4 v[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                const size_t at = base + static_cast<size_t>(min(k1 + i * every, u.n_parts - 1)) * stride;
+                ml[i] = p.part_ml[at];
+                v[i] = *reinterpret_cast<const f32x4*>(p.part_o + at * HD + 4 * col);
+            }
+            float mx = s.M;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) mx = fmaxf(mx, ml[i].x);
+            const float use = mx == -kInf ? 0.0f : mx, old = s.L * __builtin_amdgcn_exp2f(s.M - use);
+            float w[kAtOnce], sum = old;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                w[i] = k1 + i * every < u.n_parts ? ml[i].y * __builtin_amdgcn_exp2f(ml[i].x - use) : 0.0f;
+                sum += w[i];
+            }
+            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+            s.x *= old * inv;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (w[i] != 0.0f) s.x += (w[i] * inv) * v[i];
+            s.L = sum;
+            s.M = mx;
         }
-        const int r = t.row_lo + row;
-        *reinterpret_cast<f32x4*>(p.out + ((static_cast<size_t>(t.r.row0) + r / p.group) * p.n_heads + hk * p.group +
-                                           r % p.group) * HD + 4 * d) = x;
+        return s;
+    };
+    auto store = [&](int r, const f32x4& x) {
+        *reinterpret_cast<f32x4*>(row_of(p.out, p, u.r, hk, u.tile * R + r, HD) + 4 * col) = x;
+    };
+    if (u.n_parts <= kAtOnce) {
+        for (int r = blockIdx.y * kWide + k0; r < rows; r += gridDim.y * kWide) store(r, parts_of(r, 0, 1).x);
+        return;
+    }
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        const Mean s = parts_of(r, k0, kWide);
+        sums[k0][col] = s.x;
+        if (col == 0) mls[k0] = make_float2(s.M, s.L);
+        __syncthreads();
+        if (k0 == 0) {
+            float M = -kInf, w[kWide], sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kWide; ++k) M = fmaxf(M, mls[k].x);
+            const float use = M == -kInf ? 0.0f : M;
+#pragma unroll
+            for (int k = 0; k < kWide; ++k) {
+                w[k] = mls[k].y * __builtin_amdgcn_exp2f(mls[k].x - use);
+                sum += w[k];
+            }
+            const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+            f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < kWide; ++k)
+                if (w[k] != 0.0f) x += (w[k] * inv) * sums[k][col];
+            store(r, x);
+        }
+        __syncthreads();
     }
 }
 
 // The split of a call, from what the host knows of it: few rows a sequence share
-// their keys over the waves, many have waves of their own; keys are cut into parts
-// until there are work-groups for the chip.
+// their keys over the waves, many have waves of their own.
 struct PagedPlan {
-    bool keys;
-    int32_t rows, parts, least;
-    int64_t slots;
+    bool keys, split;
+    int32_t rows, target;
+    int64_t tiles, units;  // at most
 };
 PagedPlan paged_plan(const PagedAttnArgs& a) {
     PagedPlan pl;
     const int64_t group = a.n_heads / a.c.n_kv, rows = group * a.c.n_rows;
     pl.keys = rows <= 32 * static_cast<int64_t>(a.c.n_seqs);
     pl.rows = pl.keys ? 16 : a.c.head_dim == 256 ? 64 : 128;
-    pl.least = pl.keys ? 4 : 8;
-    pl.slots = rows / pl.rows + a.c.n_seqs;
-    const int64_t groups = (pl.keys ? std::max<int64_t>(rows / pl.rows, a.c.n_seqs) : pl.slots) * a.c.n_kv;
-    const int64_t steps = (static_cast<int64_t>(a.c.max_pages) * a.c.page_tokens + 63) / 64;
-    const int64_t want = (512 + groups - 1) / groups, most = (steps + pl.least - 1) / pl.least;
-    pl.parts = static_cast<int32_t>(std::max<int64_t>(1, std::min<int64_t>({want, most, kMaxParts})));
+    pl.tiles = rows / pl.rows + a.c.n_seqs;
+    pl.target = pl.keys ? kTarget : 512;
+    // tiles for the chip without a split: no parts, no merge
+    const int64_t steps = ((static_cast<int64_t>(a.c.max_pages) << a.c.page_bits) + 63) / 64;
+    pl.split = steps > kLeastSteps && pl.tiles * a.c.n_kv < (pl.keys ? 2 * pl.target : 512);
+    // units = sum over tiles of ceil(steps / per) <= target / n_kv + tiles (and one for the
+    // device's rounding of per, which takes less than a part in 10^6 of it)
+    pl.units = pl.tiles + (pl.split ? pl.target / a.c.n_kv + 2 : 0);
     return pl;
 }
 
 template <int HD>
 hipError_t paged_attention(PagedParams& p, const PagedPlan& pl, hipStream_t stream) {
-    const int64_t groups = pl.slots * p.c.n_kv;
-    if (groups * pl.parts > 0x7fffffff) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<uint32_t>(groups * pl.parts));
+    if (pl.units * p.c.n_kv > 0x7fffffff) return hipErrorInvalidValue;
+    const dim3 grid(static_cast<uint32_t>(pl.units * p.c.n_kv));
     constexpr int kOwn = HD == 256 ? 1 : 2;
-    if (pl.keys) hipLaunchKernelGGL((paged_attn_kernel<HD, 1, true>), grid, dim3(kAttnThreads), 0, stream, p);
-    else hipLaunchKernelGGL((paged_attn_kernel<HD, kOwn, false>), grid, dim3(kAttnThreads), 0, stream, p);
+    if (pl.keys) hipLaunchKernelGGL(paged_keys_kernel<HD>, grid, dim3(kAttnThreads), 0, stream, p);
+    else hipLaunchKernelGGL((paged_rows_kernel<HD, kOwn>), grid, dim3(kAttnThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || pl.parts == 1) return e;
-    const dim3 merge(static_cast<uint32_t>(groups));
+    if (e != hipSuccess || !pl.split) return e;
+    // a tile's rows in as many work-groups as make 512 of them
+    const int64_t rows = std::min<int64_t>(pl.rows, static_cast<int64_t>(p.c.n_rows) * p.group), tiles = pl.tiles * p.c.n_kv;
+    const dim3 merge(static_cast<uint32_t>(tiles),
+                     static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 512 / tiles))));
     if (pl.keys) hipLaunchKernelGGL((paged_merge_kernel<HD, 16>), merge, dim3(kAttnThreads), 0, stream, p);
     else hipLaunchKernelGGL((paged_merge_kernel<HD, 64 * kOwn>), merge, dim3(kAttnThreads), 0, stream, p);
     return hipGetLastError();
@@ -858,8 +1104,8 @@ hipError_t launch_kv_append_paged(const AppendArgs& a, hipStream_t stream) {
 
 size_t attention_paged_workspace_bytes(const PagedAttnArgs& a) {
     const PagedPlan pl = paged_plan(a);
-    if (pl.parts == 1) return 0;
-    return static_cast<size_t>(pl.slots) * a.c.n_kv * pl.parts * pl.rows * (sizeof(float2) + sizeof(float) * a.c.head_dim);
+    if (!pl.split) return 0;
+    return static_cast<size_t>(pl.units) * a.c.n_kv * pl.rows * (sizeof(float2) + sizeof(float) * a.c.head_dim);
 }
 
 hipError_t launch_attention_paged(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, hipStream_t stream) {
@@ -872,12 +1118,11 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, void* workspace, size_
     p.n_heads = a.n_heads;
     p.group = a.n_heads / a.c.n_kv;
     p.sw = a.sliding_window;
-    p.parts = pl.parts;
-    p.least = pl.least;
+    p.target = pl.target;
+    p.split = pl.split;
     p.scale = a.scale * 1.44269504088896341f;
-    p.slots = pl.slots;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.slots) * a.c.n_kv * pl.parts * pl.rows * a.c.head_dim);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.units) * a.c.n_kv * pl.rows * a.c.head_dim);
     if (a.c.head_dim == 64) return paged_attention<64>(p, pl, stream);
     if (a.c.head_dim == 128) return paged_attention<128>(p, pl, stream);
     if (a.c.head_dim == 256) return paged_attention<256>(p, pl, stream);
