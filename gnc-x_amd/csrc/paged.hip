@@ -20,12 +20,11 @@ namespace {
 
 using namespace dev;
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 // ---- rotation ------------------------------------------------------------------
 // cos and sin of position * freq: the angle's turns in 64 bits, as 32 keep a far
@@ -409,11 +408,13 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
 // blocks; a 16-key product takes four tokens of each, so that the lanes of group
 // lane / 16 hold the scores of all 16 tokens of one block, and read those tokens of
 // V as 16 bytes of one float's row.
-// Precision: codes are exact in fp16 and code times scale in bfloat16.  Queries go in
-// as pairs of fp16 (22 bits, behind a power of two that takes the row's largest to
-// 2^14), weights as three bfloat16 (24 bits, and the range of a float, so that the
-// values' scales need no care).  Scores, sums and outputs are held in 32 bits.
+// Precision: codes are exact in fp16.  Queries go in as pairs of fp16 (22 bits, behind a
+// power of two that takes the row's largest to 2^14), and so do weights, each times its
+// block's value scale over the largest scale so far, `unit` (powers of two).  Scores, sums
+// and outputs are held in 32 bits, maxima rounded up to whole numbers, so that rescaling is
+// exact.
 constexpr int kAttnThreads = 256, kAttnWaves = 4;
+__device__ __forceinline__ u32x4 four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return u32x4{a, b, c, d}; }
 constexpr float kInf = __builtin_inff();
 
 __device__ __forceinline__ uint32_t as_bits(float x) { return __builtin_bit_cast(uint32_t, x); }
@@ -433,9 +434,6 @@ __device__ __forceinline__ float xor_max(float v) {
 __device__ __forceinline__ float xor_sum(float v) {
     return over_column(v, [](float a, float b) { return a + b; });
 }
-__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {  // of a, then b
-    return __builtin_amdgcn_perm(b, a, 0x07060302u);
-}
 __device__ __forceinline__ f16x8 codes_f16(uint32_t w0, uint32_t w1) {
     const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, false);
     const f16x2 b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, 1.0f, true);
@@ -443,15 +441,12 @@ __device__ __forceinline__ f16x8 codes_f16(uint32_t w0, uint32_t w1) {
     const f16x2 d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, 1.0f, true);
     return f16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
 }
-__device__ __forceinline__ bf16x8 codes_bf16(uint32_t w0, uint32_t w1, float scale) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, false);
-    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, scale, true);
-    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, false);
-    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, scale, true);
-    return bf16x8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
-}
 // 0x80 in every byte of w that is a NaN
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ u32x4 without_nan(u32x4 x) {
+    auto zeros = [](uint32_t w) { return w & ~((nan_bytes(w) >> 7) * 0xffu); };
+    return four(zeros(x.x), zeros(x.y), zeros(x.z), zeros(x.w));
+}
 
 struct PagedParams {
     PagedArgs c;
@@ -466,6 +461,9 @@ struct PagedParams {
 };
 constexpr int kTarget = 1024;    // work-groups that a split of keys aims at (64 sequences of 100 to 8000
                                  // tokens, 8 KV heads: 512 117.5 us, 1024 and 2048 110; 60001 tokens 19.9, 19.8, 21.0)
+#ifndef ROWS_TARGET
+#define ROWS_TARGET 2048
+#endif
 constexpr int kMostParts = 128;  // of a row
 constexpr int kLeastSteps = 4;   // of a part
 
@@ -561,7 +559,8 @@ __device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit&
 }
 
 // Rows of queries as the products take them: lane (n, g) has floats 64 i + 16 g + 0 .. 15
-// of row n, as the keys' lanes do.
+// of row n, as the keys' lanes do.  The scale's sign goes into them, so that fac, the
+// factor of their products, is positive and keeps the scores' order.
 template <int HD>
 __device__ __forceinline__ void split_queries(const float* q, int g, float scale, f16x8 (&qh)[HD / 32],
                                               f16x8 (&ql)[HD / 32], float& fac) {
@@ -579,19 +578,20 @@ __device__ __forceinline__ void split_queries(const float* q, int g, float scale
     int e = 0;
     (void)frexpf(most, &e);
     e = most > 0.0f && most < kInf ? e - 14 : 0;
-    fac = ldexpf(scale, e);
+    fac = ldexpf(scale == 0.0f ? 1.0f : fabsf(scale), e);
+    const float sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-            const float x = ldexpf(v[i][j / 4][j % 4], -e);
+            const float x = ldexpf(sign * v[i][j / 4][j % 4], -e);
             const _Float16 h = static_cast<_Float16>(x);
             qh[2 * i + j / 8][j % 8] = h;
             ql[2 * i + j / 8][j % 8] = static_cast<_Float16>(x - static_cast<float>(h));
         }
 }
 
-// A row's running maximum, sum (of this lane's keys) and output.
+// A row's running maximum, sum (of this lane's keys) and output, in units of 2^(unit - 14).
 template <int HD>
 struct RowState {
     float m = -kInf, l = 0.0f;
@@ -600,81 +600,229 @@ struct RowState {
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // Scores (of this lane's 16 keys, those in `seen` seen) to weights, as the products
-    // take them: e = three numbers of 8 bits, cut off one after the other, nothing lost.
-    __device__ __forceinline__ void weigh(const f32x4 (&s)[4], float f, uint32_t seen, bool full, bf16x8 (&w)[2][3]) {
-        float x[16], most = -kInf;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) x[j] = s[j / 4][j % 4] * f;
+    // A step's scores, f s for the `seen` of this lane's 16 keys: the others to -inf, the
+    // maximum raised, sum and output rescaled to it (and the output by `units`).  Returns
+    // the maximum to weigh by.
+    __device__ __forceinline__ float raise(f32x4 (&s)[4], float f, uint32_t seen, bool full, float units) {
+        float most = -kInf;
         if (!full)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) x[j] = seen >> j & 1u ? x[j] : -kInf;
+            for (int j = 0; j < 16; ++j) s[j / 4][j % 4] = seen >> j & 1u ? s[j / 4][j % 4] : -kInf;
 #pragma unroll
-        for (int j = 0; j < 16; ++j) most = fmaxf(most, x[j]);
-        const float mx = fmaxf(m, xor_max(most)), use = mx == -kInf ? 0.0f : mx;
-        const float alpha = __builtin_amdgcn_exp2f(m - use);
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, s[j / 4][j % 4]);
+        const float mx = fmaxf(m, ceilf(xor_max(most * f))), use = mx == -kInf ? 0.0f : mx;
+        const float alpha = __builtin_amdgcn_exp2f(m - use), by = alpha * units;
         m = mx;
-        float sum = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            uint32_t a[4], b[4], c[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t h[2], md[2], lw[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(x[8 * k + 2 * j + i] - use);
-                    sum += e;
-                    h[i] = __builtin_bit_cast(uint32_t, e) & 0xffff0000u;
-                    const float r1 = e - __builtin_bit_cast(float, h[i]);
-                    md[i] = __builtin_bit_cast(uint32_t, r1) & 0xffff0000u;
-                    lw[i] = __builtin_bit_cast(uint32_t, r1 - __builtin_bit_cast(float, md[i]));
-                }
-                a[j] = high_halves(h[0], h[1]);
-                b[j] = high_halves(md[0], md[1]);
-                c[j] = high_halves(lw[0], lw[1]);
-            }
-            w[k][0] = __builtin_bit_cast(bf16x8, make_uint4(a[0], a[1], a[2], a[3]));
-            w[k][1] = __builtin_bit_cast(bf16x8, make_uint4(b[0], b[1], b[2], b[3]));
-            w[k][2] = __builtin_bit_cast(bf16x8, make_uint4(c[0], c[1], c[2], c[3]));
-        }
-        l = l * alpha + sum;
+        l *= alpha;
         // (most steps leave every row's maximum as it is)
-        if (__any(alpha != 1.0f))
+        if (__any(by != 1.0f))
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d) o[d] *= alpha;
-    }
-    __device__ __forceinline__ void add(int d, bf16x8 a, bf16x8 b, const bf16x8 (&w)[2][3]) {
-#pragma unroll
-        for (int k = 2; k >= 0; --k) {
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, w[0][k], o[d], 0, 0, 0);
-            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b, w[1][k], o[d], 0, 0, 0);
-        }
-    }
-    // The same without the NaN codes among a's and b's sources, then NaN where this row
-    // sees one of them (na, nb: one for each): a step that is not seen whole.
-    __device__ __forceinline__ void add_nan(int d, bf16x8 na, bf16x8 nb, uint32_t seen) {
-        auto ones = [&](int j) {
-            return ((seen >> j & 1u) ? 0x3f80u : 0u) | ((seen >> (j + 1) & 1u) ? 0x3f800000u : 0u);
-        };
-        f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
-        count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            na, __builtin_bit_cast(bf16x8, make_uint4(ones(0), ones(2), ones(4), ones(6))), count, 0, 0, 0);
-        count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            nb, __builtin_bit_cast(bf16x8, make_uint4(ones(8), ones(10), ones(12), ones(14))), count, 0, 0, 0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (count[r] > 0.0f) o[d][r] = __builtin_nanf("");
+            for (int d = 0; d < HD / 16; ++d) o[d] *= by;
+        return use;
     }
 };
+// o += the values a and b (of tokens 0 to 7 and 8 to 15 of the lane's block) by their weights
+__device__ __forceinline__ void add_values(f32x4& o, f16x8 a, f16x8 b, const f16x8 (&hi)[2], const f16x8 (&lo)[2]) {
+    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, lo[0], o, 0, 0, 0);
+    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, lo[1], o, 0, 0, 0);
+    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[0], o, 0, 0, 0);
+    o = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, hi[1], o, 0, 0, 0);
+}
+// Weights 2^(f s - use) of this lane's 16 keys as fp16 pairs; returns their sum.  Two a
+// conversion, and the rest as one mixed fma that reads its half in place (written out, as
+// the compiler converts every half back, alone).
+__device__ __forceinline__ float weigh(const f32x4 (&s)[4], float f, float use, f16x8 (&hi)[2], f16x8 (&lo)[2]) {
+    float sum = 0.0f;
+    uint32_t h[8], r[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(s[j / 2][2 * j % 4], f, -use));
+        const float y = __builtin_amdgcn_exp2f(fmaf(s[j / 2][2 * j % 4 + 1], f, -use));
+        sum += x + y;
+        h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2));
+        float a, b;
+        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[0,0,1]" : "=v"(a) : "v"(x), "v"(h[j]));
+        asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(b) : "v"(y), "v"(h[j]));
+        r[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        hi[k] = __builtin_bit_cast(f16x8, four(h[4 * k], h[4 * k + 1], h[4 * k + 2], h[4 * k + 3]));
+        lo[k] = __builtin_bit_cast(f16x8, four(r[4 * k], r[4 * k + 1], r[4 * k + 2], r[4 * k + 3]));
+    }
+    return sum;
+}
+// The largest of the four lane groups' values
+__device__ __forceinline__ int most_of_groups(int v) {
+    return max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+               max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
+constexpr int kNoUnit = -1000;
+
 // Keys at .. at + 15 that the row at pos sees, one bit each
+__device__ __forceinline__ uint32_t below_bits(int32_t at, int32_t n) {  // those below n
+    return (1u << min(max(n - at, 0), 16)) - 1u;
+}
 __device__ __forceinline__ uint32_t seen_bits(int32_t at, int32_t pos, int32_t sw) {
-    auto below = [&](int32_t n) {  // keys below n
-        const int32_t k = min(max(n - at, 0), 16);
-        return (1u << k) - 1u;
-    };
-    const uint32_t in = below(pos + 1);
-    return sw > 0 ? in & ~below(max(pos - sw + 1, 0)) : in;
+    const uint32_t in = below_bits(at, pos + 1);
+    return sw > 0 ? in & ~below_bits(at, max(pos - sw + 1, 0)) : in;
+}
+// What a wave's rows are, and where they look.
+template <int HD, int RT>
+struct WaveRows {
+    f16x8 qh[RT][HD / 32], ql[RT][HD / 32];
+    float fac[RT];
+    int32_t pos[RT];
+    int32_t pos_first, pos_last, low_first, low_last;  // of its rows; the first keys that they see
+    // the last key of a step, and its first, are seen by every row
+    __device__ __forceinline__ bool whole(int32_t k0) const { return k0 + 63 <= pos_first && k0 >= low_last; }
+    // keys at .. at + 15 may be seen by some row
+    __device__ __forceinline__ bool meets(int32_t at) const { return at <= pos_last && at + 16 > low_first; }
+    // s += the keys' floats 64 i + 16 g .. by the queries'
+    __device__ __forceinline__ void score(f32x4& s, u32x4 x, int i, int rt) const {
+        score(s, x, i, rt, ql[rt][2 * i], ql[rt][2 * i + 1]);
+    }
+    __device__ __forceinline__ void score(f32x4& s, u32x4 x, int i, int rt, f16x8 la, f16x8 lb) const {
+        const f16x8 a = codes_f16(x.x, x.y), b = codes_f16(x.z, x.w);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, la, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, lb, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[rt][2 * i], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[rt][2 * i + 1], s, 0, 0, 0);
+    }
+};
+// 0xff for the bytes of tokens that are in `seen`
+__device__ __forceinline__ uint32_t bytes_of(uint32_t seen, int t0) {
+    return ((seen >> t0 & 1u) * 0xffu) | ((seen >> (t0 + 1) & 1u) * 0xff00u) |
+           ((seen >> (t0 + 2) & 1u) * 0xff0000u) | ((seen >> (t0 + 3) & 1u) * 0xff000000u);
+}
+__device__ __forceinline__ u32x4 only_seen(u32x4 x, uint32_t seen) {
+    return four(x.x & bytes_of(seen, 0), x.y & bytes_of(seen, 4), x.z & bytes_of(seen, 8), x.w & bytes_of(seen, 12));
+}
+__device__ __forceinline__ int scale_exponent(float scale) { return static_cast<int>(as_bits(scale) >> 23 & 0xffu) - 127; }
+
+// Whether the blocks' value scales allow one unit for all: a scale of more than 16 below
+// the unit would leave bits of its weights behind in fp16.  Raises the unit; `units` is
+// what outputs are to be multiplied by.
+__device__ __forceinline__ bool one_unit(bool there, float scale, int& unit, float& units) {
+    const int own = scale_exponent(scale);
+    const int top = max(unit, most_of_groups(there ? own : kNoUnit));
+    if (-most_of_groups(there ? -own : kNoUnit) < top - 16) return false;
+    units = unit == top ? 1.0f : ldexpf(1.0f, max(unit - top, -200));
+    unit = top;
+    return true;
+}
+// A step of RT row tiles, from their products with the keys on: sc are the scales of this
+// lane's block, if it is there, and values(d) the codes of its float 16 d + n.
+template <int HD, int RT, class Values>
+__device__ __forceinline__ void take_step(RowState<HD> (&st)[RT], f32x4 (&s)[RT][4], const float (&fac)[RT], float2 sc,
+                                          bool there, bool full, const uint32_t (&seen)[RT], int unit, float units,
+                                          Values&& values) {
+    f16x8 hi[RT][2], lo[RT][2];
+    const float kf = there ? sc.x : 1.0f;
+    const int up = there ? scale_exponent(sc.y) - unit + 14 : 0;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+        const float f = fac[rt] * kf, use = st[rt].raise(s[rt], f, seen[rt], full, units);
+        __builtin_amdgcn_sched_barrier(0);
+        st[rt].l += ldexpf(weigh(s[rt], f, use - static_cast<float>(up), hi[rt], lo[rt]), -up);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int d = 0; d < HD / 16; ++d) {
+        if (RT > 1 && d % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+        const u32x4 x = values(d);
+        const f16x8 a = codes_f16(x.x, x.y), b = codes_f16(x.z, x.w);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) add_values(st[rt].o[d], a, b, hi[rt], lo[rt]);
+    }
+}
+
+// The same for every step, from `step` on, one after the other: for those whose values'
+// scales are far apart (the blocks of a range of scales at a time, in a unit of their own),
+// and those not seen whole with NaN codes among the values: rows that do not see one must
+// not meet it (0 NaN is NaN), so NaN codes are taken out and met by a product of their own.
+// (Inside the loops of the others this would cost them 60 registers.)
+template <int HD, int RT>
+__device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* table, int hk, const WaveRows<HD, RT>& w,
+                                           RowState<HD> (&st)[RT], int& unit, int step, int every, int end) {
+    const PagedArgs& c = p.c;
+    const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    for (; step < end; step += every) {
+        const int32_t k0 = 64 * step, at_k = k0 + 16 * (n >> 2), at_v = k0 + 16 * g;
+        const int64_t bk = block_in(c, page_at(c, table, at_k), hk, at_k);
+        const int64_t bv = block_in(c, page_at(c, table, at_v), hk, at_v);
+        const uint8_t* kp = c.k_pages + max(bk, int64_t{0}) * (kKvBlock * HD) + (n & 3) * HD + 16 * g;
+        const uint8_t* vp = c.v_pages + max(bv, int64_t{0}) * (kKvBlock * HD) + 16 * n;
+        const float2 sc = *reinterpret_cast<const float2*>(c.scales + 2 * max(bv, int64_t{0}));
+        const bool there = bv >= 0 && w.meets(at_v);
+        const bool full = w.whole(k0) && __ballot(there) == ~uint64_t{0};
+        const int own = scale_exponent(sc.y), top = max(unit, most_of_groups(there ? own : kNoUnit));
+        const float units = ldexpf(1.0f, max(unit - top, -200)), kf = there ? sc.x : 1.0f;
+        unit = top;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            f32x4 s[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < HD / 64; ++i)
+                    w.score(s[j], *reinterpret_cast<const u32x4*>(kp + 4 * j * HD + 64 * i), i, rt);
+            }
+            const uint32_t seen = there ? seen_bits(at_v, w.pos[rt], p.sw) : 0u;
+            const float f = w.fac[rt] * kf, use = st[rt].raise(s, f, seen, full, units);
+            bool left = there;
+            auto pass = [&](int t, auto&& add) {  // the blocks with scales within 16 below 2^t, in units of 2^(t - 14)
+                const bool now = left && own >= t - 16;
+                left = left && !now;
+                f16x8 hi[2], lo[2];
+                const int up = now ? own - t + 14 : 0;
+                st[rt].l += ldexpf(weigh(s, f, now ? use - static_cast<float>(up) : kInf, hi, lo), -up);
+#pragma unroll
+                for (int d = 0; d < HD / 16; ++d) {
+                    u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
+                    if (!full) x = without_nan(x);
+                    add(d, codes_f16(x.x, x.y), codes_f16(x.z, x.w), hi, lo);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            pass(unit, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
+                add_values(st[rt].o[d], a, b, hi, lo);
+            });
+            while (__any(left)) {
+                const int t = most_of_groups(left ? own : kNoUnit);
+                const float back = ldexpf(1.0f, max(t - unit, -200));
+                pass(t, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
+                    f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
+                    add_values(part, a, b, hi, lo);
+                    st[rt].o[d] += part * back;
+                });
+            }
+            if (full) continue;
+            auto ones = [&](int j) {
+                return ((seen >> j & 1u) ? 0x3c00u : 0u) | ((seen >> (j + 1) & 1u) ? 0x3c000000u : 0u);
+            };
+            const f16x8 first = __builtin_bit_cast(f16x8, four(ones(0), ones(2), ones(4), ones(6)));
+            const f16x8 second = __builtin_bit_cast(f16x8, four(ones(8), ones(10), ones(12), ones(14)));
+            auto marks = [](uint32_t v) { return (nan_bytes(v) >> 7) * 0x38u; };  // (0x38: one)
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d) {
+                const u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
+                f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
+                count = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(marks(x.x), marks(x.y)), first, count, 0, 0, 0);
+                count = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(marks(x.z), marks(x.w)), second, count, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (count[r] > 0.0f) st[rt].o[d][r] = __builtin_nanf("");
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+}
+// A lane's part of a row: its sum over all keys, and the factor of its output
+__device__ __forceinline__ float2 sum_and_share(float l, int unit) {
+    l = xor_sum(l);
+    return make_float2(l, l != 0.0f ? ldexpf(1.0f / l, unit == kNoUnit ? 0 : unit - 14) : 0.0f);
 }
 __device__ __forceinline__ float* row_of(float* base, const PagedParams& p, const SeqRows& r, int hk, int row, int hd) {
     return base + ((static_cast<size_t>(r.row0) + row / p.group) * p.n_heads + hk * p.group + row % p.group) * hd;
@@ -694,30 +842,31 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     Unit u;
     if (!find_unit<R, false>(p, unit, u)) return;
     const int rows = u.r.count * p.group, row_lo = u.tile * R, row_hi = min(row_lo + R, rows);
-    const int32_t pos_first = u.r.len + row_lo / p.group, pos_last = u.r.len + (row_hi - 1) / p.group;
-    const int32_t low_first = p.sw > 0 ? max(pos_first - p.sw + 1, 0) : 0;
-    const int32_t low_last = p.sw > 0 ? max(pos_last - p.sw + 1, 0) : 0;
+    WaveRows<HD, 1> w;
+    w.pos_first = u.r.len + row_lo / p.group;
+    w.pos_last = u.r.len + (row_hi - 1) / p.group;
+    w.low_first = p.sw > 0 ? max(w.pos_first - p.sw + 1, 0) : 0;
+    w.low_last = p.sw > 0 ? max(w.pos_last - p.sw + 1, 0) : 0;
     const int step0 = (p.sw > 0 ? max(u.r.len - p.sw + 1, 0) / 64 : 0) + u.part * u.per;
-    const int step1 = min(step0 + u.per, pos_last / 64 + 1);
+    const int step1 = min(step0 + u.per, w.pos_last / 64 + 1);
     const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
     int step = step0 + wv;
     // keys of a step that this lane's blocks begin at: of K, whose rows it loads, and of V
     const int at_k = 16 * (n >> 2), at_v = 16 * g;
     int32_t page_k = page_at(c, table, 64 * step + at_k), page_v = page_at(c, table, 64 * step + at_v);
     const int row = min(row_lo + n, rows - 1);
-    const int32_t pos = u.r.len + row / p.group;
-    f16x8 qh[HD / 32], ql[HD / 32];
-    float fac;
-    split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, qh, ql, fac);
-    RowState<HD> st;
+    w.pos[0] = u.r.len + row / p.group;
+    split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, w.qh[0], w.ql[0], w.fac[0]);
+    RowState<HD> st[1];
+    int unit_exp = kNoUnit;
     // (a block that is not there: the first one is read, and hidden)
-    uint4 kw[4][kSlices], vw[kDims];
+    u32x4 kw[4][kSlices], vw[kDims];
     auto load_k = [&](int64_t b) {
         const uint8_t* from = c.k_pages + max(b, int64_t{0}) * (kKvBlock * HD) + (n & 3) * HD + 16 * g;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < kSlices; ++i) kw[j][i] = *reinterpret_cast<const uint4*>(from + 4 * j * HD + 64 * i);
+            for (int i = 0; i < kSlices; ++i) kw[j][i] = *reinterpret_cast<const u32x4*>(from + 4 * j * HD + 64 * i);
     };
     float2 scale;
     auto in_order = [] { asm volatile("" ::: "memory"); };
@@ -726,7 +875,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
         in_order();
         const uint8_t* from = c.v_pages + max(b, int64_t{0}) * (kKvBlock * HD) + 16 * n;
 #pragma unroll
-        for (int d = 0; d < kDims; ++d) vw[d] = *reinterpret_cast<const uint4*>(from + 256 * d);
+        for (int d = 0; d < kDims; ++d) vw[d] = *reinterpret_cast<const u32x4*>(from + 256 * d);
     };
     // Loads return in the order of their issue, so that what is waited for first goes out
     // first: the pages of the step after next, the next step's keys while this one's scores
@@ -740,64 +889,49 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     load_v(bv);
     for (; step < step1; step += kAttnWaves) {
         const int32_t k0 = 64 * step, next = step + kAttnWaves;
-        f32x4 s[4];
+        f32x4 s[1][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            s[0][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < kSlices; ++i) {
-                const f16x8 a = codes_f16(kw[j][i].x, kw[j][i].y), b = codes_f16(kw[j][i].z, kw[j][i].w);
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[2 * i], s[j], 0, 0, 0);
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[2 * i + 1], s[j], 0, 0, 0);
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[2 * i], s[j], 0, 0, 0);
-                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[2 * i + 1], s[j], 0, 0, 0);
-            }
+            for (int i = 0; i < kSlices; ++i) w.score(s[0][j], kw[j][i], i, 0);
         }
-        const bool there = bv >= 0 && k0 + at_v <= pos_last && k0 + at_v + 16 > low_first;
-        const bool full = k0 + 63 <= pos_first && k0 >= low_last && __ballot(there) == ~uint64_t{0};
-        const uint32_t seen = there ? seen_bits(k0 + at_v, pos, p.sw) : 0u;
+        const bool there = bv >= 0 && w.meets(k0 + at_v);
+        const bool full = w.whole(k0) && __ballot(there) == ~uint64_t{0};
+        const uint32_t seen[1] = {there ? seen_bits(k0 + at_v, w.pos[0], p.sw) : 0u};
         const bool more = next < step1;
         const int64_t next_k = more ? block_in(c, page_k, hk, 64 * next + at_k) : 0;
         bv = more ? block_in(c, page_v, hk, 64 * next + at_v) : 0;
         page_k = page_at(c, table, 64 * (next + kAttnWaves) + at_k);
         page_v = page_at(c, table, 64 * (next + kAttnWaves) + at_v);
         load_k(next_k);
-        const float2 sc = there ? scale : make_float2(1.0f, 1.0f);
-        bf16x8 w[2][3];
-        st.weigh(s, fac * sc.x, seen, full, w);
-        // NaN codes of V, which rows that do not see them must not meet (0 NaN is NaN), are
-        // taken out of a step that is not seen whole, and met by a product of their own
-        uint32_t bad = 0;
-        if (!full)
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-                bad |= nan_bytes(vw[d].x) | nan_bytes(vw[d].y) | nan_bytes(vw[d].z) | nan_bytes(vw[d].w);
-        if (!__any(bad != 0)) {
-#pragma unroll
-            for (int d = 0; d < kDims; ++d)
-                st.add(d, codes_bf16(vw[d].x, vw[d].y, sc.y), codes_bf16(vw[d].z, vw[d].w, sc.y), w);
-        } else {
+        float units;
+        if (!one_unit(there, scale.y, unit_exp, units)) break;
+        // values that no row sees may hold anything
+        u32x4 seen_bytes = four(~0u, ~0u, ~0u, ~0u);
+        if (!full) {
+            const uint32_t some = there ? seen_bits(k0 + at_v, w.pos_last, 0) & ~below_bits(k0 + at_v, w.low_first) : 0u;
+            seen_bytes = only_seen(seen_bytes, some);
+            uint32_t bad = 0;
 #pragma unroll
             for (int d = 0; d < kDims; ++d) {
-                const uint32_t z[4] = {nan_bytes(vw[d].x) >> 7, nan_bytes(vw[d].y) >> 7, nan_bytes(vw[d].z) >> 7,
-                                       nan_bytes(vw[d].w) >> 7};
-                st.add(d, codes_bf16(vw[d].x & ~(z[0] * 0xffu), vw[d].y & ~(z[1] * 0xffu), sc.y),
-                       codes_bf16(vw[d].z & ~(z[2] * 0xffu), vw[d].w & ~(z[3] * 0xffu), sc.y), w);
-                // (0x38: one)
-                st.add_nan(d, codes_bf16(z[0] * 0x38u, z[1] * 0x38u, 1.0f), codes_bf16(z[2] * 0x38u, z[3] * 0x38u, 1.0f),
-                           seen);
+                const u32x4 x = vw[d] & seen_bytes;
+                bad |= nan_bytes(x.x) | nan_bytes(x.y) | nan_bytes(x.z) | nan_bytes(x.w);
             }
+            if (__any(bad != 0)) break;
         }
+        take_step<HD, 1>(st, s, w.fac, scale, there, full, seen, unit_exp, units,
+                         [&](int d) { return vw[d] & seen_bytes; });
         load_v(bv);
         // (otherwise the compiler joins these loads with those before the loop, at its top)
         asm volatile("; the next step's values are on their way" ::: "memory");
     }
-    const float l = xor_sum(st.l);
+    if (step < step1) hard_steps<HD, 1>(p, table, hk, w, st, unit_exp, step, kAttnWaves, step1);
     // divided by the sum here, before the parts' weights meet the values
-    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    if (g == 0) mls[wv][n] = make_float2(st.m, l);
+    const float2 ls = sum_and_share(st[0].l, unit_exp);
+    if (g == 0) mls[wv][n] = make_float2(st[0].m, ls.x);
 #pragma unroll
-    for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(&os[wv][n][16 * d + 4 * g]) = st.o[d] * inv;
+    for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(&os[wv][n][16 * d + 4 * g]) = st[0].o[d] * ls.y;
     __syncthreads();
     // (a unit's parts: [unit][KV head][row])
     const size_t part_row = (static_cast<size_t>(unit) * c.n_kv + hk) * R;
@@ -827,114 +961,159 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
 }
 
 // Many rows (prompts): a wave has 16 RT rows of its own, a work-group four times as many.
+// The codes of a step are staged in LDS for all of them, two steps in turn: the next one's
+// are on their way from memory during a step, and laid down at its end, so that a step
+// takes one barrier.
 template <int HD, int RT>
-__global__ __launch_bounds__(kAttnThreads) void paged_rows_kernel(PagedParams p) {
+__global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_kernel(PagedParams p) {
     constexpr int R = 16 * RT * kAttnWaves, kSlices = HD / 64, kDims = HD / 16;
+    constexpr int kChunks = HD / 16;  // 16-byte chunks of a key; of a step there are 64 times as many
+    __shared__ __align__(16) u32x4 ks[2][64 * kChunks], vs[2][64 * kChunks];
+    __shared__ __align__(16) f16x8 qlow[RT * 2 * kSlices][kAttnThreads];  // the queries' low halves: they would take the registers that a step needs
     const PagedArgs& c = p.c;
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
     const int hk = blockIdx.x % c.n_kv, unit = blockIdx.x / c.n_kv;
     Unit u;
     if (!find_unit<R, false>(p, unit, u)) return;
-    const int rows = u.r.count * p.group, row_lo = u.tile * R + 16 * RT * wv, row_hi = min(row_lo + 16 * RT, rows);
-    if (row_lo >= rows) return;
-    const int32_t pos_first = u.r.len + row_lo / p.group, pos_last = u.r.len + (row_hi - 1) / p.group;
-    const int32_t low_first = p.sw > 0 ? max(pos_first - p.sw + 1, 0) : 0;
-    const int32_t low_last = p.sw > 0 ? max(pos_last - p.sw + 1, 0) : 0;
-    const int step0 = (p.sw > 0 ? max(u.r.len - p.sw + 1, 0) / 64 : 0) + u.part * u.per;
-    const int step1 = min(step0 + u.per, pos_last / 64 + 1);
+    const int rows = u.r.count * p.group, tile_lo = u.tile * R, tile_hi = min(tile_lo + R, rows);
     const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
-    f16x8 qh[RT][HD / 32], ql[RT][HD / 32];
-    float fac[RT];
-    int32_t pos[RT];
+    const int step0 = (p.sw > 0 ? max(u.r.len - p.sw + 1, 0) / 64 : 0) + u.part * u.per;
+    const int step1 = min(step0 + u.per, (u.r.len + (tile_hi - 1) / p.group) / 64 + 1);
+    // this wave's rows (the last one again where there are fewer) and what they see
+    const int row_lo = min(tile_lo + 16 * RT * wv, rows - 1), row_hi = min(row_lo + 16 * RT, rows);
+    WaveRows<HD, RT> w;
+    w.pos_first = u.r.len + row_lo / p.group;
+    w.pos_last = u.r.len + (row_hi - 1) / p.group;
+    w.low_first = p.sw > 0 ? max(w.pos_first - p.sw + 1, 0) : 0;
+    w.low_last = p.sw > 0 ? max(w.pos_last - p.sw + 1, 0) : 0;
+    // K's chunk x of key t stands at chunk x ^ turn(t), so that the eight lanes that read at
+    // once, keys 0 to 3 of two blocks, meet eight different columns of banks
+    auto turn = [](int t) { return HD == 64 ? t & 3 : (t & 3) | (t >> 4 & 1) << 2; };
+    // Thread tid stages chunks tid + 256 k of K and of V, which lie in one block for a wave
+    u32x4 kw[kSlices], vw[kSlices];
+    auto load_step = [&](int32_t page, int step) {
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) {
+            const int at = tid + kAttnThreads * k, t = at / kChunks;
+            const int b = __builtin_amdgcn_readfirstlane(t / kKvBlock);
+            const int64_t blk = block_in(c, __builtin_amdgcn_readlane(page, 16 * b), hk, 64 * step + 16 * b);
+            const size_t from = static_cast<size_t>(max(blk, int64_t{0})) * (kKvBlock * HD);
+            kw[k] = *reinterpret_cast<const u32x4*>(c.k_pages + from + t % kKvBlock * HD + 16 * (at % kChunks ^ turn(t)));
+            vw[k] = *reinterpret_cast<const u32x4*>(c.v_pages + from + 16 * (at % (16 * kChunks)));
+        }
+    };
+    const int32_t tile_end = u.r.len + (tile_hi - 1) / p.group + 1;
+    const int32_t tile_low = p.sw > 0 ? max(u.r.len + tile_lo / p.group - p.sw + 1, 0) : 0;
+    auto store_step = [&](int buf, int step) {
+        // values that no row of the work-group sees may hold anything: zeros
+        const bool inside = 64 * step >= tile_low && 64 * step + 64 <= tile_end;
+#pragma unroll
+        for (int k = 0; k < kSlices; ++k) {
+            if (!inside) {
+                const int at = 64 * step + 16 * __builtin_amdgcn_readfirstlane((tid + kAttnThreads * k) / (16 * kChunks));
+                vw[k] = only_seen(vw[k], below_bits(at, tile_end) & ~below_bits(at, tile_low));
+            }
+            ks[buf][tid + kAttnThreads * k] = kw[k];
+            vs[buf][tid + kAttnThreads * k] = vw[k];
+        }
+    };
+    auto scale_of = [&](int64_t b) { return *reinterpret_cast<const float2*>(c.scales + 2 * max(b, int64_t{0})); };
+    auto in_order = [] { asm volatile("" ::: "memory"); };
+    if (step0 >= step1) {
+        // (a part behind its tile's last key)
+        for (int i = tid; i < tile_hi - tile_lo; i += kAttnThreads)
+            p.part_ml[(static_cast<size_t>(unit) * c.n_kv + hk) * R + i] = make_float2(-kInf, 0.0f);
+        return;
+    }
+    int32_t page = page_at(c, table, 64 * step0 + 16 * g);
+    load_step(page, step0);
+    int64_t bv = block_in(c, page, hk, 64 * step0 + 16 * g);
+    float2 scale = scale_of(bv);
+    page = page_at(c, table, 64 * (step0 + 1) + 16 * g);
     RowState<HD> st[RT];
+    int unit_exp = kNoUnit, hard = -1;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const int row = min(row_lo + 16 * rt + n, rows - 1);
-        pos[rt] = u.r.len + row / p.group;
-        split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, qh[rt], ql[rt], fac[rt]);
+        w.pos[rt] = u.r.len + row / p.group;
+        split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, w.qh[rt], w.ql[rt], w.fac[rt]);
+#pragma unroll
+        for (int k = 0; k < 2 * kSlices; ++k) qlow[2 * kSlices * rt + k][tid] = w.ql[rt][k];
     }
-    for (int step = max(step0, low_first / 64); step < step1; ++step) {
-        const int32_t k0 = 64 * step, at_k = k0 + 16 * (n >> 2), at_v = k0 + 16 * g;
-        const int64_t bk = block_in(c, page_at(c, table, at_k), hk, at_k);
-        const int64_t bv = block_in(c, page_at(c, table, at_v), hk, at_v);
-        const uint8_t* kp = c.k_pages + (bk < 0 ? 0 : bk) * (kKvBlock * HD) + (n & 3) * HD + 16 * g;
-        const uint8_t* vp = c.v_pages + (bv < 0 ? 0 : bv) * (kKvBlock * HD) + 16 * n;
-        float2 sc = *reinterpret_cast<const float2*>(c.scales + 2 * (bv < 0 ? 0 : bv));
-        const bool there = bv >= 0 && at_v <= pos_last && at_v + 16 > low_first;
-        if (!there) sc = make_float2(1.0f, 1.0f);
-        const bool full = k0 + 63 <= pos_first && k0 >= low_last && __ballot(there) == ~uint64_t{0};
-        uint4 kw[4][kSlices], vw[kDims];
+    store_step(0, step0);
+    for (int step = step0; step < step1; ++step) {
+        const int cur = (step - step0) & 1;
+        const int32_t k0 = 64 * step, at_v = k0 + 16 * g;
+        __syncthreads();
+        // (behind the last step the first block is read, from the caches)
+        const bool more = step + 1 < step1;
+        const int64_t bv_now = bv;
+        const float2 sc = scale;
+        const int32_t page_next = more ? page : -1;
+        load_step(page_next, step + 1);
+        bv = block_in(c, page_next, hk, 64 * (step + 1) + 16 * g);
+        scale = scale_of(bv);
+        page = page_at(c, table, 64 * (step + 2) + 16 * g);
+        in_order();
+        if (k0 <= w.pos_last && k0 + 63 >= w.low_first && hard < 0) {
+            const bool there = bv_now >= 0 && w.meets(at_v);
+            const bool full = w.whole(k0) && __ballot(there) == ~uint64_t{0};
+            const u32x4* values = vs[cur] + g * HD + n;  // float 16 d + n of the lane's block
+            uint32_t bad = 0;
+            if (!full)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int i = 0; i < kSlices; ++i) kw[j][i] = *reinterpret_cast<const uint4*>(kp + 4 * j * HD + 64 * i);
-#pragma unroll
-        for (int d = 0; d < kDims; ++d) vw[d] = *reinterpret_cast<const uint4*>(vp + 256 * d);
-        f32x4 s[RT][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) s[rt][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int i = 0; i < kSlices; ++i) {
-                const f16x8 a = codes_f16(kw[j][i].x, kw[j][i].y), b = codes_f16(kw[j][i].z, kw[j][i].w);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[rt][2 * i], s[rt][j], 0, 0, 0);
-                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[rt][2 * i + 1], s[rt][j], 0, 0, 0);
-                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[rt][2 * i], s[rt][j], 0, 0, 0);
-                    s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[rt][2 * i + 1], s[rt][j], 0, 0, 0);
+                for (int d = 0; d < kDims; ++d) {
+                    const u32x4 x = values[16 * d];
+                    bad |= nan_bytes(x.x) | nan_bytes(x.y) | nan_bytes(x.z) | nan_bytes(x.w);
                 }
-            }
-        }
-        uint32_t bad = 0, seen[RT];
-        if (!full)
+            float units;
+            if (__any(bad != 0) || !one_unit(there, sc.y, unit_exp, units)) {
+                hard = step;
+            } else {
+                f32x4 s[RT][4];
 #pragma unroll
-            for (int d = 0; d < kDims; ++d)
-                bad |= nan_bytes(vw[d].x) | nan_bytes(vw[d].y) | nan_bytes(vw[d].z) | nan_bytes(vw[d].w);
-        bf16x8 w[RT][2][3];
+                for (int j = 0; j < 4; ++j) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            seen[rt] = there ? seen_bits(at_v, pos[rt], p.sw) : 0u;
-            st[rt].weigh(s[rt], fac[rt] * sc.x, seen[rt], full, w[rt]);
-        }
-        if (!__any(bad != 0)) {
+                    for (int rt = 0; rt < RT; ++rt) s[rt][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                    const int t = 16 * (n >> 2) + 4 * j + (n & 3);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int d = 0; d < kDims; ++d) {
-                const bf16x8 a = codes_bf16(vw[d].x, vw[d].y, sc.y), b = codes_bf16(vw[d].z, vw[d].w, sc.y);
+                    for (int i = 0; i < kSlices; ++i) {
+                        const u32x4 x = ks[cur][t * kChunks + ((4 * i + g) ^ turn(t))];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) st[rt].add(d, a, b, w[rt]);
-            }
-        } else {
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) {
-                const uint32_t z[4] = {nan_bytes(vw[d].x) >> 7, nan_bytes(vw[d].y) >> 7, nan_bytes(vw[d].z) >> 7,
-                                       nan_bytes(vw[d].w) >> 7};
-                const bf16x8 a = codes_bf16(vw[d].x & ~(z[0] * 0xffu), vw[d].y & ~(z[1] * 0xffu), sc.y);
-                const bf16x8 b = codes_bf16(vw[d].z & ~(z[2] * 0xffu), vw[d].w & ~(z[3] * 0xffu), sc.y);
-                const bf16x8 na = codes_bf16(z[0] * 0x38u, z[1] * 0x38u, 1.0f);  // (0x38: one)
-                const bf16x8 nb = codes_bf16(z[2] * 0x38u, z[3] * 0x38u, 1.0f);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    st[rt].add(d, a, b, w[rt]);
-                    st[rt].add_nan(d, na, nb, seen[rt]);
+                        for (int rt = 0; rt < RT; ++rt)
+                            w.score(s[rt][j], x, i, rt, qlow[2 * (kSlices * rt + i)][tid], qlow[2 * (kSlices * rt + i) + 1][tid]);
+                    }
                 }
+                uint32_t seen[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) seen[rt] = there ? seen_bits(at_v, w.pos[rt], p.sw) : 0u;
+                take_step<HD, RT>(st, s, w.fac, sc, there, full, seen, unit_exp, units, [&](int d) { return values[16 * d]; });
             }
         }
+        if (more) store_step(cur ^ 1, step + 1);
     }
+    if (hard >= 0) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int k = 0; k < 2 * kSlices; ++k) w.ql[rt][k] = qlow[2 * kSlices * rt + k][tid];
+        hard_steps<HD, RT>(p, table, hk, w, st, unit_exp, hard, 1, min(step1, w.pos_last / 64 + 1));
+    }
+    const int own = tile_lo + 16 * RT * wv;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float l = xor_sum(st[rt].l), inv = l != 0.0f ? 1.0f / l : 0.0f;
-        const int row = row_lo + 16 * rt + n;
+        const float2 ls = sum_and_share(st[rt].l, unit_exp);
+        const int row = own + 16 * rt + n;
         if (row >= rows) continue;
         float* to = row_of(p.out, p, u.r, hk, row, HD);
         if (u.n_parts > 1) {
-            const size_t i = (static_cast<size_t>(unit) * c.n_kv + hk) * R + row - u.tile * R;
-            if (g == 0) p.part_ml[i] = make_float2(st[rt].m, l);
+            const size_t i = (static_cast<size_t>(unit) * c.n_kv + hk) * R + row - tile_lo;
+            if (g == 0) p.part_ml[i] = make_float2(st[rt].m, ls.x);
             to = p.part_o + i * HD;
         }
 #pragma unroll
-        for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(to + 16 * d + 4 * g) = st[rt].o[d] * inv;
+        for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(to + 16 * d + 4 * g) = st[rt].o[d] * ls.y;
     }
 }
 
@@ -1036,10 +1215,10 @@ PagedPlan paged_plan(const PagedAttnArgs& a) {
     pl.keys = rows <= 32 * static_cast<int64_t>(a.c.n_seqs);
     pl.rows = pl.keys ? 16 : a.c.head_dim == 256 ? 64 : 128;
     pl.tiles = rows / pl.rows + a.c.n_seqs;
-    pl.target = pl.keys ? kTarget : 512;
+    pl.target = pl.keys ? kTarget : ROWS_TARGET;
     // tiles for the chip without a split: no parts, no merge
     const int64_t steps = ((static_cast<int64_t>(a.c.max_pages) << a.c.page_bits) + 63) / 64;
-    pl.split = steps > kLeastSteps && pl.tiles * a.c.n_kv < (pl.keys ? 2 * pl.target : 512);
+    pl.split = steps > kLeastSteps && pl.tiles * a.c.n_kv < (pl.keys ? 2 * kTarget : 2048);
     // units = sum over tiles of ceil(steps / per) <= target / n_kv + tiles (and one for the
     // device's rounding of per, which takes less than a part in 10^6 of it)
     pl.units = pl.tiles + (pl.split ? pl.target / a.c.n_kv + 2 : 0);
@@ -1055,10 +1234,10 @@ hipError_t paged_attention(PagedParams& p, const PagedPlan& pl, hipStream_t stre
     else hipLaunchKernelGGL((paged_rows_kernel<HD, kOwn>), grid, dim3(kAttnThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !pl.split) return e;
-    // a tile's rows in as many work-groups as make 512 of them
+    // a tile's rows in as many work-groups as make 2048 of them
     const int64_t rows = std::min<int64_t>(pl.rows, static_cast<int64_t>(p.c.n_rows) * p.group), tiles = pl.tiles * p.c.n_kv;
     const dim3 merge(static_cast<uint32_t>(tiles),
-                     static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 512 / tiles))));
+                     static_cast<uint32_t>(std::max<int64_t>(1, std::min<int64_t>(rows, 2048 / tiles))));
     if (pl.keys) hipLaunchKernelGGL((paged_merge_kernel<HD, 16>), merge, dim3(kAttnThreads), 0, stream, p);
     else hipLaunchKernelGGL((paged_merge_kernel<HD, 64 * kOwn>), merge, dim3(kAttnThreads), 0, stream, p);
     return hipGetLastError();
