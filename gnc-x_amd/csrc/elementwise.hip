@@ -1201,6 +1201,12 @@ __device__ __forceinline__ void finish_top(const LogprobParams& p, size_t row, c
     p.out_top_logprobs[row * p.n_top + i] = r.logprob(e.x);
 }
 
+// e^d for d <= 0, to two steps: log2(e) in two parts, as one of 24 bits would leave d 2^-26
+// of an error.  (expf, with its range and special cases, 1999 rows of 32000: 60 us, not 51.)
+__device__ __forceinline__ float exp_of(float d) {
+    return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502f, d * 1.92596299e-8f));
+}
+
 template <int V>
 __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobParams p) {
     typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -1226,13 +1232,11 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
             for (int i = 0; i < 4; ++i) x[j][i] = at + i < p.vocab ? row[at + i] : -__builtin_inff();
         }
     }
+    // (a NaN is no maximum, and its exponential below that of -200)
 #pragma unroll
     for (int j = 0; j < V; ++j)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[j][i] = clean(x[j][i]);
-            most = fmaxf(most, x[j][i]);
-        }
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, x[j][i]);
     maxima[tid] = most;
     if (tid == 0) sh.held = 0;
     __syncthreads();
@@ -1242,15 +1246,17 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
         m = wave_max(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
     }
     double s = 0.0, t = 0.0;
+    const bool finite = fabsf(m) < __builtin_inff();
     if (m > -__builtin_inff())
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             float e[4], f[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                // (x == m: an infinite maximum; below -104 the exponential is 0)
-                const float d = x[j][i] == m ? 0.0f : fmaxf(x[j][i] - m, -200.0f);
-                e[i] = expf(d);
+                // (below -104 the exponential is 0; beside an infinite maximum all others' are)
+                float d = fmaxf(x[j][i] - m, -200.0f);
+                if (!finite) d = x[j][i] == m ? 0.0f : -200.0f;
+                e[i] = exp_of(d);
                 f[i] = e[i] * d;
             }
             s += (static_cast<double>(e[0]) + e[1]) + (static_cast<double>(e[2]) + e[3]);
@@ -1262,7 +1268,11 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
         sums[wv][0] = s;
         sums[wv][1] = t;
     }
-    if (p.n_top) gather_words(x, v0, nth_largest(maxima, p.n_top, lane), sh);
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
+    gather_words(x, v0, nth_largest(maxima, p.n_top, lane), sh);
     __syncthreads();
     const size_t part = blockIdx.x;
     const bool whole = p.n_chunks == 1;
@@ -1283,11 +1293,105 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
             p.sums[3 * part + 2] = t;
         }
     }
-    if (p.n_top == 0) return;
     rank_words(x, v0, p.n_top, whole ? tops : p.best + part * p.n_top, sh);
     if (!whole) return;
     __syncthreads();
     if (tid < p.n_top) finish_top(p, b, r, tid, tops[tid]);
+}
+
+// Without alternatives a thread runs through its words with a maximum of its own, moved
+// only where it is passed by 8 (an exponential of up to e^8 does not hurt), so that a
+// part may be a row of any length and takes few registers.
+constexpr int kStreamVectors = 8;  // float4 in flight
+__global__ __launch_bounds__(kCandThreads) void logprob_stream_kernel(LogprobParams p, int32_t words) {
+    typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int kWavesHere = kCandThreads / 64;
+    __shared__ double sums[kWavesHere][3];
+    const size_t b = blockIdx.x / p.n_chunks;
+    const int c = blockIdx.x % p.n_chunks, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+    const int64_t first = static_cast<int64_t>(c) * words, end = first + words < p.vocab ? first + words : p.vocab;
+    const float* row = p.logits + b * p.vocab;
+    float m = -__builtin_inff();
+    double s = 0.0, t = 0.0;
+    for (int64_t at0 = first + 4 * tid; at0 < end; at0 += 4 * kCandThreads * kStreamVectors) {
+        float x[kStreamVectors][4], most = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < kStreamVectors; ++j) {
+            const int64_t at = at0 + 4 * kCandThreads * j;
+            if (at + 4 <= end) {
+                const float4a4 w = *reinterpret_cast<const float4a4*>(row + at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = w[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[j][i] = at + i < end ? row[at + i] : -__builtin_inff();
+            }
+        }
+        // (a NaN is no maximum, and its exponential below that of -200)
+#pragma unroll
+        for (int j = 0; j < kStreamVectors; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) most = fmaxf(most, x[j][i]);
+        if (most > m + 8.0f) {
+            if (s > 0.0) {
+                const double d = static_cast<double>(m) - static_cast<double>(most), f = exp(d);
+                t = f > 0.0 ? f * (t + d * s) : 0.0;
+                s *= f;
+            }
+            m = most;
+        }
+        const bool finite = fabsf(m) < __builtin_inff();
+#pragma unroll
+        for (int j = 0; j < kStreamVectors; ++j) {
+            float e[4], f[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // (below -104 the exponential is 0; beside an infinite maximum all others' are)
+                float d = fmaxf(x[j][i] - m, -200.0f);
+                if (!finite) d = x[j][i] == m && m > 0.0f ? 0.0f : -200.0f;
+                e[i] = exp_of(d);
+                f[i] = e[i] * d;
+            }
+            s += (static_cast<double>(e[0]) + e[1]) + (static_cast<double>(e[2]) + e[3]);
+            t += (static_cast<double>(f[0]) + f[1]) + (static_cast<double>(f[2]) + f[3]);
+        }
+    }
+    // the threads' sums to the wave's maximum, the waves' to the work-group's
+    auto moved = [](double& s, double& t, float from, float to) {
+        const double d = from == to ? 0.0 : static_cast<double>(from) - static_cast<double>(to), f = exp(d);
+        t = f > 0.0 && s > 0.0 ? f * (t + d * s) : 0.0;
+        s = s > 0.0 ? f * s : 0.0;
+    };
+    const float mw = wave_max(m);
+    moved(s, t, m, mw);
+    s = wave_sum_f64(s);
+    t = wave_sum_f64(t);
+    if (lane == 0) {
+        sums[wv][0] = mw;
+        sums[wv][1] = s;
+        sums[wv][2] = t;
+    }
+    __syncthreads();
+    if (tid) return;
+    float M = mw;
+#pragma unroll
+    for (int w = 1; w < kWavesHere; ++w) M = fmaxf(M, static_cast<float>(sums[w][0]));
+    s = t = 0.0;
+#pragma unroll
+    for (int w = 0; w < kWavesHere; ++w) {
+        double ws = sums[w][1], wt = sums[w][2];
+        moved(ws, wt, static_cast<float>(sums[w][0]), M);
+        s += ws;
+        t += wt;
+    }
+    if (p.n_chunks == 1) {
+        finish_row(p, b, RowSums{M, log(s)}, s, t);
+    } else {
+        double* to = p.sums + 3 * static_cast<size_t>(blockIdx.x);
+        to[0] = M;
+        to[1] = s;
+        to[2] = t;
+    }
 }
 
 __global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParams p) {
@@ -1377,11 +1481,14 @@ __global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParam
     }
 }
 
-// float4 of a thread: the fewest that leave 512 parts over all rows
-int32_t logprob_vectors(int32_t n_rows, int32_t vocab) {
-    int32_t v = 2;
-    while (v < 16 && static_cast<int64_t>(n_rows) * ((vocab + 1024 * v - 1) / (1024 * v)) > 512) v *= 2;
-    return v;
+// Words of a part: the most that leave 1024 parts over all rows, up to a row without
+// alternatives, else what registers hold (64 x 151936, 20 alternatives: 8192 words 22.8 us,
+// 16384 25.4).
+int32_t logprob_words(int32_t n_rows, int32_t vocab, int32_t n_top) {
+    const int32_t most = n_top ? 16384 : kMaxBeamVocab;
+    int32_t w = 2048;
+    while (w < most && w < vocab && static_cast<int64_t>(n_rows) * ((vocab + 2 * w - 1) / (2 * w)) >= 1024) w *= 2;
+    return w;
 }
 
 template <class F>
@@ -1497,7 +1604,7 @@ hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t voca
 }
 
 size_t token_logprobs_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t n_top) {
-    const int32_t words = 1024 * logprob_vectors(n_rows, vocab), chunks = (vocab + words - 1) / words;
+    const int32_t words = logprob_words(n_rows, vocab, n_top), chunks = (vocab + words - 1) / words;
     return chunks == 1 ? 0 : static_cast<size_t>(n_rows) * chunks * (3 * sizeof(double) + sizeof(float2) * n_top);
 }
 
@@ -1507,13 +1614,13 @@ hipError_t launch_token_logprobs(const float* logits, int32_t n_rows, int32_t vo
     if (n_rows < 1 || vocab < 1 || vocab > kMaxBeamVocab || n_top < 0 || n_top > kMaxTopWords ||
         workspace_bytes < token_logprobs_workspace_bytes(n_rows, vocab, n_top))
         return hipErrorInvalidValue;
-    const int32_t v = logprob_vectors(n_rows, vocab);
+    const int32_t words = logprob_words(n_rows, vocab, n_top);
     LogprobParams p{};
     p.logits = logits;
     p.tokens = tokens;
     p.vocab = vocab;
     p.n_top = n_top;
-    p.n_chunks = (vocab + 1024 * v - 1) / (1024 * v);
+    p.n_chunks = (vocab + words - 1) / words;
     const int64_t parts = static_cast<int64_t>(n_rows) * p.n_chunks;
     if (parts > 0x7fffffff) return hipErrorInvalidValue;
     p.sums = static_cast<double*>(workspace);
@@ -1523,10 +1630,12 @@ hipError_t launch_token_logprobs(const float* logits, int32_t n_rows, int32_t vo
     p.out_top_tokens = out_top_tokens;
     p.out_top_logprobs = out_top_logprobs;
     const dim3 grid(static_cast<uint32_t>(parts));
-    if (v == 2) hipLaunchKernelGGL(logprob_parts_kernel<2>, grid, dim3(kCandThreads), 0, stream, p);
-    else if (v == 4) hipLaunchKernelGGL(logprob_parts_kernel<4>, grid, dim3(kCandThreads), 0, stream, p);
-    else if (v == 8) hipLaunchKernelGGL(logprob_parts_kernel<8>, grid, dim3(kCandThreads), 0, stream, p);
-    else hipLaunchKernelGGL(logprob_parts_kernel<16>, grid, dim3(kCandThreads), 0, stream, p);
+    const dim3 block(kCandThreads);
+    if (n_top == 0) hipLaunchKernelGGL(logprob_stream_kernel, grid, block, 0, stream, p, words);
+    else if (words == 2048) hipLaunchKernelGGL(logprob_parts_kernel<2>, grid, block, 0, stream, p);
+    else if (words == 4096) hipLaunchKernelGGL(logprob_parts_kernel<4>, grid, block, 0, stream, p);
+    else if (words == 8192) hipLaunchKernelGGL(logprob_parts_kernel<8>, grid, block, 0, stream, p);
+    else hipLaunchKernelGGL(logprob_parts_kernel<16>, grid, block, 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.n_chunks == 1) return e;
     hipLaunchKernelGGL(logprob_join_kernel, dim3(n_rows), dim3(kCandThreads), 0, stream, p);
