@@ -840,6 +840,17 @@ __device__ __forceinline__ float nth_largest(const float* maxima, int n, int lan
     return least > 0x007fffffu ? unordered(least) : -__builtin_inff();  // (0x007fffff: -inf itself)
 }
 
+// The same of 64 floats, one a lane: a quarter of the counting, for few of them.
+__device__ __forceinline__ float nth_of_wave(float v, int n) {
+    const uint32_t o = ordered(v);
+    uint32_t least = 0;
+    for (int bit = 31; bit >= 14; --bit) {
+        const uint32_t t = least | 1u << bit;
+        if (__builtin_popcountll(__ballot(o >= t)) >= n) least = t;
+    }
+    return least > 0x007fffffu ? unordered(least) : -__builtin_inff();
+}
+
 // v and another lane's, through DPP (no LDS round trip, unlike a shuffle)
 template <int CTRL, int ROW_MASK = 0xf>
 __device__ __forceinline__ double dpp_add_f64(double v) {
@@ -874,7 +885,7 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 // The n_out best of the words that a work-group holds (thread tid's words: v0 + 1024 j +
 // i), in two steps with a barrier between them: those that reach `least`
 // (nth_largest's of the threads' maxima) go to LDS, held being 0 before a barrier, then
-// the best go to `best` in falling order, -inf behind the last.
+// the best go to `best` in falling order, -inf behind the last.  A NaN is no word, -0 is 0.
 struct PartWords {
     uint64_t keys[kMostRanked];
     uint64_t redk[kCandThreads / 64];
@@ -894,7 +905,7 @@ __device__ __forceinline__ void gather_words(const float (&x)[V][4], int v0, flo
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (x[j][i] >= least && x[j][i] > -__builtin_inff()) {
-                    if (at < kMostRanked) sh.keys[at] = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
+                    if (at < kMostRanked) sh.keys[at] = key_of(x[j][i] + 0.0f, static_cast<uint32_t>(v0 + 1024 * j + i));
                     ++at;
                 }
     }
@@ -924,7 +935,7 @@ __device__ __forceinline__ void rank_words(const float (&x)[V][4], int v0, int n
         for (int j = 0; j < V; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint64_t o = key_of(x[j][i], static_cast<uint32_t>(v0 + 1024 * j + i));
+                const uint64_t o = key_of(x[j][i] + 0.0f, static_cast<uint32_t>(v0 + 1024 * j + i));
                 if (x[j][i] > -__builtin_inff() && o < last && o > k) k = o;
             }
         k = wave_max_u64(k);
@@ -1186,13 +1197,14 @@ struct RowSums {
         return static_cast<float>((x == m ? 0.0 : static_cast<double>(x) - static_cast<double>(m)) - log_s);
     }
 };
-__device__ __forceinline__ void finish_row(const LogprobParams& p, size_t row, const RowSums& r, double s, double t) {
-    if (p.tokens) {
-        const int32_t w = p.tokens[row];
-        const bool in = w >= 0 && w < p.vocab;
-        const float x = in ? clean(p.logits[row * p.vocab + w]) : -__builtin_inff();
-        p.out_logprobs[row] = r.logprob(x);
-    }
+// -inf without a token within the vocabulary
+__device__ __forceinline__ float logit_of_token(const LogprobParams& p, size_t row) {
+    const int32_t w = p.tokens ? p.tokens[row] : -1;
+    return w >= 0 && w < p.vocab ? clean(p.logits[row * p.vocab + w]) : -__builtin_inff();
+}
+__device__ __forceinline__ void finish_row(const LogprobParams& p, size_t row, const RowSums& r, double s, double t,
+                                           float token_logit) {
+    if (p.tokens) p.out_logprobs[row] = r.logprob(token_logit);
     if (p.out_entropy) p.out_entropy[row] = s > 0.0 ? static_cast<float>(r.log_s - t / s) : 0.0f;
 }
 __device__ __forceinline__ void finish_top(const LogprobParams& p, size_t row, const RowSums& r, int i, float2 e) {
@@ -1268,11 +1280,15 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
         sums[wv][0] = s;
         sums[wv][1] = t;
     }
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[j][i] = clean(x[j][i]);
-    gather_words(x, v0, nth_largest(maxima, p.n_top, lane), sh);
+    // (up to 32 of 64 groups of threads: 64 rows of 151936, 20 best, 22.8 -> 21.6 us)
+    float least;
+    if (p.n_top > 32) {
+        least = nth_largest(maxima, p.n_top, lane);
+    } else {
+        const float4 w = reinterpret_cast<const float4*>(maxima)[lane];
+        least = nth_of_wave(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), p.n_top);
+    }
+    gather_words(x, v0, least, sh);
     __syncthreads();
     const size_t part = blockIdx.x;
     const bool whole = p.n_chunks == 1;
@@ -1286,7 +1302,7 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
     const RowSums r{m, log(s)};
     if (tid == 0) {
         if (whole) {
-            finish_row(p, b, r, s, t);
+            finish_row(p, b, r, s, t, logit_of_token(p, b));
         } else {
             p.sums[3 * part] = m;
             p.sums[3 * part + 1] = s;
@@ -1385,7 +1401,7 @@ __global__ __launch_bounds__(kCandThreads) void logprob_stream_kernel(LogprobPar
         t += wt;
     }
     if (p.n_chunks == 1) {
-        finish_row(p, b, RowSums{M, log(s)}, s, t);
+        finish_row(p, b, RowSums{M, log(s)}, s, t, logit_of_token(p, b));
     } else {
         double* to = p.sums + 3 * static_cast<size_t>(blockIdx.x);
         to[0] = M;
@@ -1401,6 +1417,14 @@ __global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParam
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, parts = p.n_chunks;
     const double* sums = p.sums + 3 * row * parts;
     const float2* best = p.best + row * parts * p.n_top;
+    // (read ahead of what needs the sums: the first entries of the parts' lists, and the token's logit)
+    int shift = 0;
+    while (parts << shift < kGroups && 1 << shift < p.n_top) ++shift;
+    const int first = 1 << shift;
+    float most = -__builtin_inff();
+    for (int j = tid; j < parts << shift; j += kGroups)
+        if ((j & (first - 1)) < p.n_top) most = fmaxf(most, best[static_cast<size_t>(j >> shift) * p.n_top + (j & (first - 1))].x);
+    const float token_logit = logit_of_token(p, row);
     // every wave: the parts' maxima and sums
     float m = -__builtin_inff();
     for (int c = lane; c < parts; c += 64) m = fmaxf(m, static_cast<float>(sums[3 * c]));
@@ -1418,18 +1442,12 @@ __global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParam
     t = wave_sum_f64(t);
     const RowSums r{m, log(s)};
     if (tid == 0) {
-        finish_row(p, row, r, s, t);
+        finish_row(p, row, r, s, t, token_logit);
         sh.held = 0;
     }
     if (p.n_top == 0) return;
     // The parts' lists fall: a threshold from their first 2^shift entries, and a list
     // is read on only while it stays above.
-    int shift = 0;
-    while (parts << shift < kGroups && 1 << shift < p.n_top) ++shift;
-    const int first = 1 << shift;
-    float most = -__builtin_inff();
-    for (int j = tid; j < parts << shift; j += kGroups)
-        if ((j & (first - 1)) < p.n_top) most = fmaxf(most, best[static_cast<size_t>(j >> shift) * p.n_top + (j & (first - 1))].x);
     maxima[tid] = most;
     __syncthreads();
     const float least = nth_largest(maxima, p.n_top, lane);
