@@ -163,7 +163,7 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedArgs& c, int s) {
     return r;
 }
 // The last sequence s with first(s) <= at, by a wave; -1 before the first.  first
-// ascends (where row_start does; otherwise some sequence or none is found).
+// ascends (where row_start does; otherwise any sequence, or none, is found).
 template <class F>
 __device__ __forceinline__ int find_seq(int n_seqs, int64_t at, F&& first) {
     const int lane = threadIdx.x & 63;
@@ -276,7 +276,7 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
         const int s = find_seq(c.n_seqs, row, [&](int i) { return clamp_row(c, c.row_start[i]); });
         if (s < 0) return;
         const SeqRows r = seq_rows(c, s);
-        if (row - r.row0 >= r.count) return;
+        if (row < r.row0 || row - r.row0 >= r.count) return;
         if (tid < half) turn_of(r.len + row - r.row0, a.rot.freqs[tid], a.rot.magnitude, cs[tid], sn[tid]);
         __syncthreads();
         if (h >= a.n_heads) return;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
     if (s < 0) return;
     const SeqRows r = seq_rows(c, s);
     const int64_t nth = slot - first_slot(s);
-    if (r.count == 0 || nth > (r.len + r.count - 1) / kKvBlock - r.len / kKvBlock) return;
+    if (r.count == 0 || nth < 0 || nth > (r.len + r.count - 1) / kKvBlock - r.len / kKvBlock) return;
     const int32_t base = (r.len / kKvBlock + static_cast<int32_t>(nth)) * kKvBlock;  // the block's first position
     const int64_t block = block_of(c, s, hk, base);
     if (block < 0) return;
@@ -457,13 +457,15 @@ struct PagedParams {
     int32_t n_heads, group, sw;
     int32_t target;   // work-groups that a split aims at
     bool split;       // whether keys are split
+    int32_t units;    // that there is place for
     float scale;      // attn_scale log2(e)
 };
-constexpr int kTarget = 1024;    // work-groups that a split of keys aims at (64 sequences of 100 to 8000
-                                 // tokens, 8 KV heads: 512 117.5 us, 1024 and 2048 110; 60001 tokens 19.9, 19.8, 21.0)
-#ifndef ROWS_TARGET
-#define ROWS_TARGET 2048
-#endif
+// Work-groups that a split of keys aims at, for few rows a sequence and for many
+// (64 sequences of 100 to 8000 tokens, 8 KV heads: 512 117.5 us, 1024 and 2048 110; 60001
+// tokens 19.9, 19.8, 21.0.  Prompts of 1, 333 and 1666 tokens behind 2000, 700 and 0, 32
+// heads on 8: 512 619 us, 1024 316, 2048 271, 4096 395.  Equal shares of steps for as many
+// work-groups as the chip holds, whatever tiles they end in: 113, 26.5 and 283.)
+constexpr int kKeysTarget = 1024, kRowsTarget = 2048;
 constexpr int kMostParts = 128;  // of a row
 constexpr int kLeastSteps = 4;   // of a part
 
@@ -473,9 +475,16 @@ constexpr int kLeastSteps = 4;   // of a part
 // (whatever the lengths are: they are read here).  Units, a tile's part each, are numbered
 // sequence by sequence.
 struct Unit {
-    int seq, tile, part, n_parts, per, first;  // first: number of the tile's first unit
+    int seq, tile, part, n_parts, per;
+    int64_t first;  // number of the tile's first unit
     SeqRows r;
 };
+// The first key that a row at pos sees
+__device__ __forceinline__ int32_t low_of(const PagedParams& p, int32_t pos) {
+    return p.sw > 0 ? max(pos - p.sw + 1, 0) : 0;
+}
+// A sequence's tiles, and the steps of 64 keys that a tile may meet: up to the sequence's
+// last key, and with a window no more than its tokens' windows can lie in.
 struct SeqWork {
     int tiles, steps;
     SeqRows r;
@@ -486,15 +495,18 @@ __device__ __forceinline__ SeqWork seq_work(const PagedParams& p, int s) {
     if (s >= p.c.n_seqs) return w;
     w.r = seq_rows(p.c, s);
     w.tiles = (w.r.count * p.group + R - 1) / R;
-    const int lo = p.sw > 0 ? max(w.r.len - p.sw + 1, 0) / 64 : 0;
-    w.steps = w.tiles ? (w.r.len + w.r.count + 63) / 64 - lo : 0;
+    if (w.tiles == 0) return w;
+    w.steps = (w.r.len + w.r.count + 63) / 64 - low_of(p, w.r.len) / 64;
+    if (p.sw > 0) w.steps = min(w.steps, (min(p.sw, 1 << 30) + R / p.group + 63) / 64 + 1);
     return w;
 }
 // Sum over the lanes up to this one: row_shr by 1, 2, 4 and 8 within rows of 16, then the
-// rows' totals carried up, as in wave_sum_lane63.
+// rows' totals carried up, as in wave_sum_lane63.  Sums stop at INT_MAX (a row_start that
+// does not ascend may count any number).
+__device__ __forceinline__ int add_up(int a, int b) { return __builtin_elementwise_add_sat(a, b); }
 template <int CTRL, int ROW_MASK = 0xf>
 __device__ __forceinline__ int dpp_add_int(int v) {
-    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+    return add_up(v, __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false));
 }
 __device__ __forceinline__ int wave_prefix(int v) {
     v = dpp_add_int<0x111>(v);
@@ -524,32 +536,34 @@ __device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit&
         total = wave_sum(total);
         most = static_cast<int>(wave_max(static_cast<float>(most)));  // (2^24 at most)
         per = max(max(kLeastSteps, (most + kMostParts - 1) / kMostParts),
-                  static_cast<int>(ceilf(total * static_cast<float>(p.c.n_kv) / static_cast<float>(p.target))));
+                  static_cast<int>(ceilf(fminf(total * static_cast<float>(p.c.n_kv) / static_cast<float>(p.target), 1 << 26))));
         if (p.c.n_seqs > 64) w = seq_work<R>(p, lane);
     }
     int units = 0, tiles = 0;  // of the sequences before
     for (int s0 = 0; s0 < p.c.n_seqs; s0 += 64) {
         if (s0) w = seq_work<R>(p, s0 + lane);
         const int parts = w.steps ? (w.steps - 1) / per + 1 : 0;
-        const int to_unit = units + wave_prefix(w.tiles * parts);
-        const int to_tile = BY_TILE ? tiles + wave_prefix(w.tiles) : 0;
+        const int64_t own = static_cast<int64_t>(w.tiles) * parts;
+        const int to_unit = add_up(units, wave_prefix(static_cast<int>(min(own, int64_t{0x7fffffff}))));
+        const int to_tile = BY_TILE ? add_up(tiles, wave_prefix(w.tiles)) : 0;
         const uint64_t past = __ballot((BY_TILE ? to_tile : to_unit) > index);
         if (past) {
             const int l = __builtin_ctzll(past);
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            auto before = [&](int v, int none) { return l ? __builtin_amdgcn_readlane(v, l - 1) : none; };
             u.seq = s0 + l;
             u.n_parts = of(parts);
             u.per = per;
             u.r = SeqRows{of(w.r.row0), of(w.r.count), of(w.r.len)};
-            const int before = of(to_unit - w.tiles * parts);
+            const int first = before(to_unit, units);
             if constexpr (BY_TILE) {
-                u.tile = index - of(to_tile - w.tiles);
+                u.tile = index - before(to_tile, tiles);
                 u.part = 0;
             } else {
-                u.tile = (index - before) / u.n_parts;
-                u.part = index - before - u.tile * u.n_parts;
+                u.tile = (index - first) / u.n_parts;
+                u.part = index - first - u.tile * u.n_parts;
             }
-            u.first = before + u.tile * u.n_parts;
+            u.first = first + static_cast<int64_t>(u.tile) * u.n_parts;
             return true;
         }
         units = __builtin_amdgcn_readlane(to_unit, 63);
@@ -674,18 +688,21 @@ struct WaveRows {
     float fac[RT];
     int32_t pos[RT];
     int32_t pos_first, pos_last, low_first, low_last;  // of its rows; the first keys that they see
+    __device__ __forceinline__ void look(const PagedParams& p, const SeqRows& r, int row_lo, int row_hi) {
+        pos_first = r.len + row_lo / p.group;
+        pos_last = r.len + (row_hi - 1) / p.group;
+        low_first = low_of(p, pos_first);
+        low_last = low_of(p, pos_last);
+    }
     // the last key of a step, and its first, are seen by every row
     __device__ __forceinline__ bool whole(int32_t k0) const { return k0 + 63 <= pos_first && k0 >= low_last; }
     // keys at .. at + 15 may be seen by some row
     __device__ __forceinline__ bool meets(int32_t at) const { return at <= pos_last && at + 16 > low_first; }
     // s += the keys' floats 64 i + 16 g .. by the queries'
     __device__ __forceinline__ void score(f32x4& s, u32x4 x, int i, int rt) const {
-        score(s, x, i, rt, ql[rt][2 * i], ql[rt][2 * i + 1]);
-    }
-    __device__ __forceinline__ void score(f32x4& s, u32x4 x, int i, int rt, f16x8 la, f16x8 lb) const {
         const f16x8 a = codes_f16(x.x, x.y), b = codes_f16(x.z, x.w);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, la, s, 0, 0, 0);
-        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, lb, s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[rt][2 * i], s, 0, 0, 0);
+        s = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, ql[rt][2 * i + 1], s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[rt][2 * i], s, 0, 0, 0);
         s = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, qh[rt][2 * i + 1], s, 0, 0, 0);
     }
@@ -727,13 +744,18 @@ __device__ __forceinline__ void take_step(RowState<HD> (&st)[RT], f32x4 (&s)[RT]
         st[rt].l += ldexpf(weigh(s[rt], f, use - static_cast<float>(up), hi[rt], lo[rt]), -up);
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (RT > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) {
         if (RT > 1 && d % 2 == 0) __builtin_amdgcn_sched_barrier(0);
         const u32x4 x = values(d);
         const f16x8 a = codes_f16(x.x, x.y), b = codes_f16(x.z, x.w);
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) add_values(st[rt].o[d], a, b, hi[rt], lo[rt]);
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+                st[rt].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h & 1 ? b : a, h < 2 ? lo[rt][h] : hi[rt][h - 2],
+                                                                     st[rt].o[d], 0, 0, 0);
     }
 }
 
@@ -843,11 +865,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     if (!find_unit<R, false>(p, unit, u)) return;
     const int rows = u.r.count * p.group, row_lo = u.tile * R, row_hi = min(row_lo + R, rows);
     WaveRows<HD, 1> w;
-    w.pos_first = u.r.len + row_lo / p.group;
-    w.pos_last = u.r.len + (row_hi - 1) / p.group;
-    w.low_first = p.sw > 0 ? max(w.pos_first - p.sw + 1, 0) : 0;
-    w.low_last = p.sw > 0 ? max(w.pos_last - p.sw + 1, 0) : 0;
-    const int step0 = (p.sw > 0 ? max(u.r.len - p.sw + 1, 0) / 64 : 0) + u.part * u.per;
+    w.look(p, u.r, row_lo, row_hi);
+    const int step0 = w.low_first / 64 + u.part * u.per;
     const int step1 = min(step0 + u.per, w.pos_last / 64 + 1);
     const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
     int step = step0 + wv;
@@ -977,15 +996,13 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
     if (!find_unit<R, false>(p, unit, u)) return;
     const int rows = u.r.count * p.group, tile_lo = u.tile * R, tile_hi = min(tile_lo + R, rows);
     const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
-    const int step0 = (p.sw > 0 ? max(u.r.len - p.sw + 1, 0) / 64 : 0) + u.part * u.per;
+    const int32_t tile_low = low_of(p, u.r.len + tile_lo / p.group);
+    const int step0 = tile_low / 64 + u.part * u.per;
     const int step1 = min(step0 + u.per, (u.r.len + (tile_hi - 1) / p.group) / 64 + 1);
     // this wave's rows (the last one again where there are fewer) and what they see
     const int row_lo = min(tile_lo + 16 * RT * wv, rows - 1), row_hi = min(row_lo + 16 * RT, rows);
     WaveRows<HD, RT> w;
-    w.pos_first = u.r.len + row_lo / p.group;
-    w.pos_last = u.r.len + (row_hi - 1) / p.group;
-    w.low_first = p.sw > 0 ? max(w.pos_first - p.sw + 1, 0) : 0;
-    w.low_last = p.sw > 0 ? max(w.pos_last - p.sw + 1, 0) : 0;
+    w.look(p, u.r, row_lo, row_hi);
     // K's chunk x of key t stands at chunk x ^ turn(t), so that the eight lanes that read at
     // once, keys 0 to 3 of two blocks, meet eight different columns of banks
     auto turn = [](int t) { return HD == 64 ? t & 3 : (t & 3) | (t >> 4 & 1) << 2; };
@@ -1003,7 +1020,6 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
         }
     };
     const int32_t tile_end = u.r.len + (tile_hi - 1) / p.group + 1;
-    const int32_t tile_low = p.sw > 0 ? max(u.r.len + tile_lo / p.group - p.sw + 1, 0) : 0;
     auto store_step = [&](int buf, int step) {
         // values that no row of the work-group sees may hold anything: zeros
         const bool inside = 64 * step >= tile_low && 64 * step + 64 <= tile_end;
@@ -1070,6 +1086,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
             if (__any(bad != 0) || !one_unit(there, sc.y, unit_exp, units)) {
                 hard = step;
             } else {
+                __builtin_amdgcn_s_setprio(1);  // (a wave with products to issue goes first: 268 -> 262 us)
                 f32x4 s[RT][4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -1080,17 +1097,25 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
 #pragma unroll
                     for (int i = 0; i < kSlices; ++i) {
                         const u32x4 x = ks[cur][t * kChunks + ((4 * i + g) ^ turn(t))];
+                        const f16x8 k[2] = {codes_f16(x.x, x.y), codes_f16(x.z, x.w)};
+                        // (the row tiles in turn: a product waits for the one before it on its sums)
 #pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            w.score(s[rt][j], x, i, rt, qlow[2 * (kSlices * rt + i)][tid], qlow[2 * (kSlices * rt + i) + 1][tid]);
+                        for (int h = 0; h < 4; ++h)
+#pragma unroll
+                            for (int rt = 0; rt < RT; ++rt)
+                                s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    k[h & 1], h < 2 ? qlow[2 * (kSlices * rt + i) + h][tid] : w.qh[rt][2 * i + h - 2], s[rt][j],
+                                    0, 0, 0);
                     }
                 }
+                __builtin_amdgcn_s_setprio(0);
                 uint32_t seen[RT];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) seen[rt] = there ? seen_bits(at_v, w.pos[rt], p.sw) : 0u;
                 take_step<HD, RT>(st, s, w.fac, sc, there, full, seen, unit_exp, units, [&](int d) { return values[16 * d]; });
             }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (more) store_step(cur ^ 1, step + 1);
     }
     if (hard >= 0) {
@@ -1128,7 +1153,7 @@ __global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedParams p
     const PagedArgs& c = p.c;
     const int hk = blockIdx.x % c.n_kv, tile = blockIdx.x / c.n_kv;
     Unit u;
-    if (!find_unit<R, true>(p, tile, u) || u.n_parts == 1) return;
+    if (!find_unit<R, true>(p, tile, u) || u.n_parts == 1 || u.first + u.n_parts > p.units) return;
     const int col = threadIdx.x % kCols, k0 = threadIdx.x / kCols;
     const int rows = min(u.r.count * p.group - u.tile * R, R);
     const size_t stride = static_cast<size_t>(c.n_kv) * R;
@@ -1215,10 +1240,10 @@ PagedPlan paged_plan(const PagedAttnArgs& a) {
     pl.keys = rows <= 32 * static_cast<int64_t>(a.c.n_seqs);
     pl.rows = pl.keys ? 16 : a.c.head_dim == 256 ? 64 : 128;
     pl.tiles = rows / pl.rows + a.c.n_seqs;
-    pl.target = pl.keys ? kTarget : ROWS_TARGET;
+    pl.target = pl.keys ? kKeysTarget : kRowsTarget;
     // tiles for the chip without a split: no parts, no merge
     const int64_t steps = ((static_cast<int64_t>(a.c.max_pages) << a.c.page_bits) + 63) / 64;
-    pl.split = steps > kLeastSteps && pl.tiles * a.c.n_kv < (pl.keys ? 2 * kTarget : 2048);
+    pl.split = steps > kLeastSteps && pl.tiles * a.c.n_kv < 2048;
     // units = sum over tiles of ceil(steps / per) <= target / n_kv + tiles (and one for the
     // device's rounding of per, which takes less than a part in 10^6 of it)
     pl.units = pl.tiles + (pl.split ? pl.target / a.c.n_kv + 2 : 0);
@@ -1299,6 +1324,7 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, void* workspace, size_
     p.sw = a.sliding_window;
     p.target = pl.target;
     p.split = pl.split;
+    p.units = static_cast<int32_t>(std::min<int64_t>(pl.units, INT32_MAX));
     p.scale = a.scale * 1.44269504088896341f;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.units) * a.c.n_kv * pl.rows * a.c.head_dim);

@@ -259,8 +259,8 @@ class Paged:
                 seen = see.any(0)[:, None]
                 kh, vh = torch.where(seen, kh, 0.0), torch.where(seen, vh, 0.0)
                 sc = torch.where(see, qh @ kh.t().contiguous() * self.scale, -math.inf)
-                size = torch.where(see, qh.abs() @ kh.abs().t().contiguous(), 0.0).amax(1, keepdim=True) * self.scale
-                far = torch.where(see, kh.abs().sum(1)[None, :], 0.0).amax(1, keepdim=True) * self.scale
+                size = torch.where(see, qh.abs() @ kh.abs().t().contiguous(), 0.0).amax(1, keepdim=True) * abs(self.scale)
+                far = torch.where(see, kh.abs().sum(1)[None, :], 0.0).amax(1, keepdim=True) * abs(self.scale)
                 w = torch.exp(sc - sc.amax(1, keepdim=True).clamp(min=-1e300))
                 l = w.sum(1, keepdim=True).clamp(min=1e-300)
                 want = w @ vh / l
@@ -786,6 +786,63 @@ def test_calls_on_another_stream(lib, torch_mod):
             assert torch.equal(p.out, want)
     finally:
         lib.gncx_hip_set_stream(None)
+
+
+@pytest.mark.parametrize("seqs,most", [(65, 90), (300, 40), (2100, 0)])
+@pytest.mark.parametrize("new", [1, 3])
+def test_many_sequences(lib, torch_mod, seqs, most, new):
+    """More sequences than a wave has lanes, some without rows; 2100 without a split."""
+    rng = np.random.default_rng(seqs)
+    held = rng.integers(0, most + 1, seqs).tolist()
+    p = Paged(torch_mod, held, [0 if i % 7 == 3 else new for i in range(seqs)], H=2, KV=1, hd=64, page=16, seed=30)
+    p.append(lib)
+    p.attend(lib)
+    p.check_attention()
+
+
+@pytest.mark.parametrize("sw", [1, 70, 300, 2 ** 31 - 1])
+@pytest.mark.parametrize("H,KV,hd", [(8, 2, 128), (3, 1, 64), (6, 2, 256)])
+def test_windows_of_long_prompts(lib, torch_mod, sw, H, KV, hd):
+    p = Paged(torch_mod, [2000, 0], [600, 130], H=H, KV=KV, hd=hd, seed=31)
+    p.append(lib)
+    p.attend(lib, sw)
+    p.check_attention(sw=sw)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, 3.0])
+@pytest.mark.parametrize("new", [1, 50])
+def test_scales_of_the_scores(lib, torch_mod, scale, new):
+    p = Paged(torch_mod, [300], [new], H=4, KV=2, hd=64, seed=32)
+    p.scale = scale
+    p.append(lib)
+    p.attend(lib)
+    p.check_attention()
+
+
+@pytest.mark.parametrize("starts", [[0, 60, 20, 90], [90, 60, 30, 0], [-5, 1000000, -7, 90], [0, 90, 0, 90]])
+@pytest.mark.parametrize("held", [[10, 700, 3], [2000, 2000, 2000]])
+def test_row_starts_that_do_not_ascend(lib, torch_mod, starts, held):
+    """What such rows receive is open; rows that are not the call's, and pages that no table
+    names, stay as they are, and the next call is answered."""
+    torch = torch_mod
+    p = Paged(torch, held, [30, 30, 30], H=8, KV=2, hd=64, seed=33, room=3)
+    free = sorted(set(range(p.n_pages)) - set(p.table.ravel().tolist()))
+    p.starts = np.array(starts, np.int32)
+    p.upload()
+    behind = torch.full((40, 8 * 64), 7.0, device="cuda")
+    buffers = [torch.cat([x, behind]) for x in (p.q, p.out)]
+    p.batch.n_rows = 90
+    before = state(p)
+    p.append(lib, Turn(torch, 64), 1, out=buffers[0][:90])
+    p.attend(lib, out=buffers[1][:90])
+    torch.cuda.synchronize()
+    assert torch.equal(buffers[0][90:], behind) and torch.equal(buffers[1][90:], behind)
+    for now, was in zip(state(p), before):
+        assert torch.equal(now[free].float().nan_to_num(nan=-1), was[free].float().nan_to_num(nan=-1))
+    other = Paged(torch, [100], [1], seed=34)
+    other.append(lib)
+    other.attend(lib)
+    other.check_attention()
 
 
 # ---- log probabilities ------------------------------------------------------------------
