@@ -461,10 +461,12 @@ struct PagedParams {
     float scale;      // attn_scale log2(e)
 };
 // Work-groups that a split of keys aims at, for few rows a sequence and for many
-// (64 sequences of 100 to 8000 tokens, 8 KV heads: 512 117.5 us, 1024 and 2048 110; 60001
-// tokens 19.9, 19.8, 21.0.  Prompts of 1, 333 and 1666 tokens behind 2000, 700 and 0, 32
-// heads on 8: 512 619 us, 1024 316, 2048 271, 4096 395.  Equal shares of steps for as many
-// work-groups as the chip holds, whatever tiles they end in: 113, 26.5 and 283.)
+// (64 sequences of 100 to 8000 tokens, 8 KV heads of 128: 512 117.5 us, 1024 and 2048 110; one
+// of 60001 tokens, 4 KV heads: 19.9, 19.8, 21.0.  Four prompts of 300 to 700 tokens behind
+// 1152 to 3799, 32 heads on 8: 1024 316 us, 1536 283, 2048 254, 4096 395: a part costs 8 us
+// beside its steps' 4 us each, long parts end unevenly.  Equal shares of steps for as many
+// work-groups as the chip holds, whatever tiles they end in, were slower in all three: 113,
+// 26.5 and 283.)
 constexpr int kKeysTarget = 1024, kRowsTarget = 2048;
 constexpr int kMostParts = 128;  // of a row
 constexpr int kLeastSteps = 4;   // of a part
@@ -1086,16 +1088,18 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
             if (__any(bad != 0) || !one_unit(there, sc.y, unit_exp, units)) {
                 hard = step;
             } else {
-                __builtin_amdgcn_s_setprio(1);  // (a wave with products to issue goes first: 268 -> 262 us)
+                __builtin_amdgcn_s_setprio(1);  // (a wave with products to issue goes first: 260 -> 255 us)
                 f32x4 s[RT][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int i = 0; i < kSlices; ++i) {
+                    f16x8 low[RT][2];
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) s[rt][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                    const int t = 16 * (n >> 2) + 4 * j + (n & 3);
-                    __builtin_amdgcn_sched_barrier(0);
+                    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-                    for (int i = 0; i < kSlices; ++i) {
+                        for (int h = 0; h < 2; ++h) low[rt][h] = qlow[2 * (kSlices * rt + i) + h][tid];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int t = 16 * (n >> 2) + 4 * j + (n & 3);
                         const u32x4 x = ks[cur][t * kChunks + ((4 * i + g) ^ turn(t))];
                         const f16x8 k[2] = {codes_f16(x.x, x.y), codes_f16(x.z, x.w)};
                         // (the row tiles in turn: a product waits for the one before it on its sums)
@@ -1104,8 +1108,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
 #pragma unroll
                             for (int rt = 0; rt < RT; ++rt)
                                 s[rt][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    k[h & 1], h < 2 ? qlow[2 * (kSlices * rt + i) + h][tid] : w.qh[rt][2 * i + h - 2], s[rt][j],
-                                    0, 0, 0);
+                                    k[h & 1], h < 2 ? low[rt][h] : w.qh[rt][2 * i + h - 2],
+                                    i == 0 && h == 0 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : s[rt][j], 0, 0, 0);
                     }
                 }
                 __builtin_amdgcn_s_setprio(0);
