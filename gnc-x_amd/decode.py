@@ -45,7 +45,13 @@ differences are where the streamer works on host memory:
   gncx_hip_attention_tree) and keeps the accepted path's cache rows
   (gncx_hip_kv_keep_rows); beam_search() decodes beams side by side, chosen by
   gncx_hip_beam_select and followed by the caches through
-  gncx_hip_kv_reorder.
+  gncx_hip_kv_reorder;
+* generate_batch() decodes many sequences at once over paged caches of 8-bit
+  blocks (PagedSequences: gncx_hip_kv_append_paged and
+  gncx_hip_attention_paged in the place of the prologue + attention calls),
+  its tokens and their log probabilities from gncx_hip_token_logprobs, with a
+  rotation for longer contexts if asked (gncx_hip_rope_frequencies); score()
+  gives the log probabilities of a text.
 
 Weights are random-init with the block statistics of the synthetic
 benchmark inputs: fp16 scales |N(0, 0.02)|, uniform random code bytes,
@@ -56,7 +62,8 @@ from __future__ import annotations
 import ctypes as C
 from dataclasses import dataclass, field
 
-from . import Q4_K, Q6_K, DecodeLayer, DecodeModel, DecodeState, DecodeTensor, check, row_bytes
+from . import (Q4_K, Q6_K, ROPE_PLAIN, DecodeLayer, DecodeModel, DecodeState, DecodeTensor, PagedBatch, PagedCache,
+               Rotation, check, row_bytes)
 
 _ALIGN = 32  # GGUF default data alignment
 
@@ -271,6 +278,70 @@ def lookup_draft(ids, depth: int = 8, width: int = 4):
                 parents.append(node)
             node = at[node, t]
     return tokens, parents
+
+
+class PagedSequences:
+    """The caches of several sequences, of 8-bit blocks in pages: sequence i has
+    room for room[i] positions, in pages that are its own and the same in every
+    layer's pool.  scaling: the arguments of gncx_hip_rope_frequencies behind the
+    base by name, for contexts longer than the trained one."""
+
+    def __init__(self, lib, torch, model: Model, room, page: int = 64, scaling: dict | None = None,
+                 device: str = "cuda"):
+        s = model.shape
+        self.lib, self.torch, self.m, self.device = lib, torch, model, device
+        need = [-(-max(int(r), 1) // page) for r in room]
+        self.n_pages, self.max_pages, self.page = sum(need), max(need), page
+        table = torch.full((len(need), self.max_pages), -1, dtype=torch.int32)
+        at = 0
+        for i, n in enumerate(need):
+            table[i, :n] = torch.arange(at, at + n, dtype=torch.int32)
+            at += n
+        self.table = table.to(device)
+        # (what no token was appended to is never seen: it may hold anything)
+        codes = (s.n_layers, self.n_pages, s.n_kv, page * s.head_dim)
+        self.k, self.v = (torch.empty(codes, dtype=torch.uint8, device=device) for _ in range(2))
+        self.scales = torch.empty(s.n_layers, self.n_pages, s.n_kv, page // 16, 2, dtype=torch.float32, device=device)
+        self.freqs = torch.empty(s.head_dim // 2, dtype=torch.float64, device=device)
+        magnitude = C.c_float()
+        given = dict(scaling=ROPE_PLAIN, factor=1.0, trained_context=0, beta_fast=32.0, beta_slow=1.0, factors=None)
+        if set(scaling or ()) - set(given):
+            raise ValueError("a scaling has " + ", ".join(given))
+        given.update(scaling or {})
+        factors = given["factors"]
+        if lib.gncx_hip_rope_frequencies(s.head_dim, s.rope_base, given["scaling"], given["factor"],
+                                         given["trained_context"], given["beta_fast"], given["beta_slow"],
+                                         None if factors is None else factors.data_ptr(), self.freqs.data_ptr(),
+                                         C.addressof(magnitude)):
+            check(lib)
+        self.rotation = Rotation(self.freqs.data_ptr(), s.head_dim, 0, magnitude.value)
+        self.lengths = [0] * len(need)
+
+    def begin(self, counts):
+        """The next pass has counts[i] further tokens of sequence i, row by row."""
+        starts = [0]
+        for n in counts:
+            starts.append(starts[-1] + int(n))
+        on = lambda a: self.torch.tensor(a, dtype=self.torch.int32).to(self.device)  # noqa: E731
+        self.counts, self._starts, self._lengths = list(counts), on(starts), on(self.lengths)
+        self.batch = PagedBatch(len(counts), starts[-1], self.max_pages, self._starts.data_ptr(),
+                                self._lengths.data_ptr(), self.table.data_ptr())
+
+    def end(self):
+        self.lengths = [a + n for a, n in zip(self.lengths, self.counts)]
+
+    def attention(self, l, q, k, v, out, scale):
+        """Layer l's prologue (per-head RMSNorm and rotation of q and k, q in its
+        place), its keys and values into the cache, and its attention."""
+        s, m, P = self.m.shape, self.m, f"blk.{l}"
+        cache = PagedCache(self.k[l].data_ptr(), self.v[l].data_ptr(), self.scales[l].data_ptr(), self.n_pages,
+                           self.page, s.n_kv, s.head_dim)
+        self.lib.gncx_hip_kv_append_paged(C.byref(cache), C.byref(self.batch), q.data_ptr(), k.data_ptr(),
+                                          v.data_ptr(), s.n_heads, m.base, m.off(f"{P}.attn_q_norm.weight"),
+                                          m.off(f"{P}.attn_k_norm.weight"), 1, s.eps, C.byref(self.rotation),
+                                          q.data_ptr())
+        self.lib.gncx_hip_attention_paged(C.byref(cache), C.byref(self.batch), q.data_ptr(), s.n_heads, scale, 0,
+                                          out.data_ptr())
 
 
 class Decoder:
@@ -649,20 +720,33 @@ class Decoder:
     def _rows_logits(self, tokens, attention):
         """Logits [len(tokens)][vocab] of one pass over the tokens, with
         attention(l, q, k, v, out) over each layer's row tensors."""
+        return self._rows_head(self._rows_normed(tokens, attention))
+
+    def _rows_normed(self, tokens, attention, keep=None):
+        """The same up to the lm_head: the normed rows, of the rows in `keep` where
+        it is given."""
         torch, s, L, m = self.torch, self.s, self.lib, self.m
         n = len(tokens)
         row = lambda d: torch.empty(n, d, dtype=torch.float32, device=self.hidden.device)  # noqa: E731
         bh, bn, bp = row(s.embed), row(s.embed), row(s.embed)
         bq, bk, bv, ba = row(s.q_dim), row(s.kv_dim), row(s.kv_dim), row(s.q_dim)
-        bg, bu, logits = row(s.ffn), row(s.ffn), row(s.vocab)
+        bg, bu = row(s.ffn), row(s.ffn)
         ids = (C.c_int32 * n)(*(int(t) for t in tokens))
         L.gncx_hip_fetch_token_embeddings(s.embd_type, m.base, m.off("token_embd.weight"), ids, n, s.vocab, s.embed,
                                           1.0, bh.data_ptr())
         self._rows_layers(n, lambda l: attention(l, bq, bk, bv, ba), bh, bq, bk, bv, ba, bp, bg, bu)
+        if keep is not None:
+            at = torch.tensor(keep, dtype=torch.long, device=bh.device)
+            bh, bp, bn, n = bh[at], bp[at], bn[at], len(keep)
         L.gncx_hip_add_rmsnorm_rows(bh.data_ptr(), bp.data_ptr(), n, m.base, m.off("output_norm.weight"), s.embed,
                                     s.eps, bn.data_ptr())
-        L.gncx_xfold_universal_matbatch(m.base, m.off("token_embd.weight"), s.embd_type, bn.data_ptr(), n, s.embed,
-                                        s.vocab, logits.data_ptr(), None)
+        return bn
+
+    def _rows_head(self, bn):
+        s, m, n = self.s, self.m, bn.shape[0]
+        logits = self.torch.empty(n, s.vocab, dtype=self.torch.float32, device=bn.device)
+        self.lib.gncx_xfold_universal_matbatch(m.base, m.off("token_embd.weight"), s.embd_type, bn.data_ptr(), n,
+                                               s.embed, s.vocab, logits.data_ptr(), None)
         return logits
 
     def verify_tree(self, tokens, parents, pos: int):
@@ -793,6 +877,108 @@ class Decoder:
             if end >= 0:
                 finished = torch.where(parents < 0, 0, finished[came] | (tokens == end).int())
         return [(t, c) for t, c in zip(chosen.tolist(), scores.tolist()) if c > float("-inf")]
+
+    # -- many sequences -------------------------------------------------------------
+    def _logprobs(self, logits, tokens=None, n_top: int = 0):
+        """(log probabilities of `tokens` and entropies, None without them;
+        alternatives and their log probabilities, [n][n_top])"""
+        torch, n, P = self.torch, logits.shape[0], lambda t: None if t is None else t.data_ptr()
+        new = lambda *d: torch.empty(n, *d, dtype=torch.float32, device=logits.device)  # noqa: E731
+        lp, ent = (None, None) if tokens is None else (new(), new())
+        top, top_lp = new(n_top).view(torch.int32), new(n_top)
+        self.lib.gncx_hip_token_logprobs(logits.data_ptr(), n, self.s.vocab, P(tokens), n_top, P(lp), P(ent),
+                                         top.data_ptr() if n_top else None, top_lp.data_ptr() if n_top else None)
+        check(self.lib)
+        return lp, ent, top, top_lp
+
+    def score(self, ids, n_top: int = 0):
+        """(log probabilities, entropies, alternatives) of ids[1:], each behind the
+        ids before it: in nats, and alternatives[i] the n_top (at most 64) most
+        probable [(token, log probability)] there."""
+        self._device_only("scoring")
+        s, m, n = self.s, self.m, len(ids) - 1
+        if n < 1 or n > self.max_seq:
+            raise ValueError("at least two ids, and the KV cache holds all but the last")
+        if not 0 <= n_top <= 64:
+            raise ValueError("0 to 64 alternatives")
+
+        def attention(l, q, k, v, out):
+            p = f"blk.{l}"
+            self.lib.gncx_hip_attention_prefill(q.data_ptr(), k.data_ptr(), v.data_ptr(), self.kc[l].data_ptr(),
+                                                self.vc[l].data_ptr(), 0, n, s.n_heads, s.n_kv, s.head_dim, self.scale,
+                                                0, m.base, m.off(f"{p}.attn_q_norm.weight"),
+                                                m.off(f"{p}.attn_k_norm.weight"), 1, s.eps, 0, 0, s.rope_base,
+                                                out.data_ptr())
+
+        bn = self._rows_normed(ids[:-1], attention)
+        tokens = self.torch.tensor([int(t) for t in ids[1:]], dtype=self.torch.int32, device=bn.device)
+        lps, ents, tops = [], [], []
+        for i in range(0, n, 1024):  # (rows of logits at once: 0.6 GB of a vocabulary of 151936)
+            lp, ent, top, top_lp = self._logprobs(self._rows_head(bn[i:i + 1024]), tokens[i:i + 1024], n_top)
+            lps += lp.tolist()
+            ents += ent.tolist()
+            tops += [list(zip(a, b)) for a, b in zip(top.tolist(), top_lp.tolist())]
+        return lps, ents, tops
+
+    def generate_batch(self, prompts, n_new: int, end: int = -1, n_top: int = 0, page: int = 64,
+                       scaling: dict | None = None, rows_at_once: int = 4096):
+        """n_new greedy tokens of each prompt, all decoded together over paged 8-bit
+        caches of the call's own: [(token ids, their log probabilities,
+        alternatives)], alternatives[i] the n_top (at most 64) most probable
+        [(token, log probability)] where token i was chosen.  A sequence ends behind
+        the token `end` (if not negative).  Prompts go in with up to rows_at_once
+        tokens a pass; `scaling` as in PagedSequences."""
+        self._device_only("a batch")
+        prompts = [[int(t) for t in p] for p in prompts]
+        if not prompts or not all(prompts) or n_new < 1 or rows_at_once < 1:
+            raise ValueError("prompts of at least one token, and at least one new one")
+        if page not in (16, 32, 64, 128, 256) or not 0 <= n_top <= 64:
+            raise ValueError("pages of 16, 32, 64, 128 or 256 positions, 0 to 64 alternatives")
+        if any(not 0 <= t < self.s.vocab for p in prompts for t in p):
+            raise ValueError("a prompt's token is outside the vocabulary")
+        torch, n = self.torch, len(prompts)
+        seqs = PagedSequences(self.lib, torch, self.m, [len(p) + n_new - 1 for p in prompts], page, scaling,
+                              self.hidden.device)
+
+        def normed(tokens, counts, keep=None):
+            seqs.begin(counts)
+            rows = self._rows_normed(tokens, lambda l, q, k, v, out: seqs.attention(l, q, k, v, out, self.scale), keep)
+            check(self.lib)
+            seqs.end()
+            return rows
+
+        last = torch.empty(n, self.s.embed, dtype=torch.float32, device=self.hidden.device)
+        first = 0
+        while first < n:  # (sequences before `first` have their prompts' tokens in)
+            counts, tokens, keep, ended = [0] * n, [], [], []
+            for i in range(first, n):
+                at = seqs.lengths[i]
+                counts[i] = min(len(prompts[i]) - at, rows_at_once - len(tokens))
+                tokens += prompts[i][at:at + counts[i]]
+                if at + counts[i] < len(prompts[i]):
+                    break
+                keep.append(len(tokens) - 1)
+                ended.append(i)
+            rows = normed(tokens, counts, keep or [0])
+            if ended:
+                last[ended] = rows
+                first = ended[-1] + 1
+        out = [([], [], []) for _ in prompts]
+        live = list(range(n))
+        while True:
+            _, _, top, top_lp = self._logprobs(self._rows_head(last), n_top=max(n_top, 1))
+            going = []
+            for i, words, lps in zip(live, top.tolist(), top_lp.tolist()):
+                ids, chosen, others = out[i]
+                ids.append(max(words[0], 0))  # (-1: no logit above -inf)
+                chosen.append(lps[0])
+                others.append(list(zip(words, lps))[:n_top])
+                if len(ids) < n_new and ids[-1] != end:
+                    going.append(i)
+            live = going
+            if not live:
+                return out
+            last = normed([out[i][0][-1] for i in live], [int(i in live) for i in range(n)])
 
     def _matbatch_multi_addnorm(self, p, names, norm, hidden, delta, b, out_dims, outs):
         """gncx_hip_matbatch_multi_addnorm: hidden += delta (None: no add), then

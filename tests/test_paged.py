@@ -203,3 +203,90 @@ def test_structs_match_header(tmp_path):
     for ln in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
         s, f, v = ln.split()
         assert (C.sizeof(py[s]) if f == "sizeof" else getattr(py[s], f).offset) == int(v), (s, f)
+
+
+# ---- the decode driver -----------------------------------------------------------------
+class Stand:
+    """A stand-in model whose next id is 3 t + 1 (and 0 the second choice), over sequences
+    that only count; the passes' rows."""
+
+    def __init__(self, dec, monkeypatch, vocab=50):
+        import types
+        import torch
+        self.torch, self.scale, self.hidden, self.lib, self.m = torch, 1.0, torch.zeros(vocab), None, None
+        self.s = types.SimpleNamespace(vocab=vocab, embed=vocab)
+        self.passes, stand = [], self
+
+        class Counts:
+            def __init__(self, lib, torch, model, room, *_):
+                self.room, self.lengths = room, [0] * len(room)
+
+            def begin(self, counts):
+                stand.passes.append(counts)
+                self.counts = counts
+
+            def end(self):
+                self.lengths = [a + n for a, n in zip(self.lengths, self.counts)]
+                assert all(a <= r for a, r in zip(self.lengths, self.room))
+
+        monkeypatch.setattr(dec, "PagedSequences", Counts)
+        monkeypatch.setattr(dec, "check", lambda lib: None)
+
+    def _device_only(self, what):
+        pass
+
+    def _rows_normed(self, tokens, attention, keep=None):
+        assert len(tokens) == sum(self.passes[-1])
+        return self.torch.nn.functional.one_hot(self.torch.tensor(tokens), self.s.vocab).float()[
+            range(len(tokens)) if keep is None else keep]
+
+    def _rows_head(self, rows):
+        t = rows.argmax(1)
+        return self.torch.nn.functional.one_hot((3 * t + 1) % self.s.vocab, self.s.vocab).float()
+
+    def _logprobs(self, logits, tokens=None, n_top=0):
+        top = self.torch.topk(logits.log_softmax(1), n_top)
+        return None, None, top.indices.int(), top.values
+
+
+@pytest.mark.parametrize("at_once", [1, 2, 3, 7, 100])
+def test_generate_batch_fills_its_passes(plib, monkeypatch, at_once):
+    import gncx_amd.decode as dec
+    d = Stand(dec, monkeypatch)
+    prompts, n_new = [[5], [1, 2, 3, 4], [9, 8], [7] * 9, [2]], 4
+    got = dec.Decoder.generate_batch(d, prompts, n_new, n_top=1, rows_at_once=at_once)
+    follow = lambda t, n: [t := (3 * t + 1) % 50 for _ in range(n)]  # noqa: E731
+    assert [ids for ids, _, _ in got] == [follow(p[-1], n_new) for p in prompts]
+    assert all(len(lps) == len(tops) == n_new and top[0] == (t, lp) and len(top) == 1
+               for ids, lps, tops in got for t, lp, top in zip(ids, lps, tops))
+    first = d.passes[:-(n_new - 1)]
+    assert [sum(c) for c in zip(*first)] == [len(p) for p in prompts]
+    assert [sum(c) for c in first] == [at_once] * (17 // at_once) + [17 % at_once] * (17 % at_once > 0)
+    assert d.passes[-(n_new - 1):] == [[1] * 5] * (n_new - 1)
+    # 16 = 3 * 5 + 1 ends the first sequence at once
+    d.passes.clear()
+    got = dec.Decoder.generate_batch(d, prompts, n_new, end=16)
+    assert got[0][0] == [16] and got[0][2] == [[]] and d.passes[1][0] == 0
+    assert all(ids == (full[:full.index(16) + 1] if 16 in full else full)
+               for (ids, _, _), full in zip(got, (follow(p[-1], n_new) for p in prompts)))
+
+
+def test_driver_refusals(plib, monkeypatch):
+    import gncx_amd.decode as dec
+    d = Stand(dec, monkeypatch)
+    for args, kw in ((([], 3), {}), (([[1], []], 3), {}), (([[1]], 0), {}), (([[1]], 1), dict(page=48)),
+                     (([[1]], 1), dict(n_top=65)), (([[1]], 1), dict(rows_at_once=0)), (([[50]], 1), {}), (([[-1]], 1), {})):
+        with pytest.raises(ValueError):
+            dec.Decoder.generate_batch(d, *args, **kw)
+    d.max_seq = 3
+    for ids, top in (([], 0), ([1], 0), ([1] * 5, 0), ([1, 2], 65), ([1, 2], -1)):
+        with pytest.raises(ValueError):
+            dec.Decoder.score(d, ids, top)
+    assert not d.passes
+    import types
+    import torch
+    host = types.SimpleNamespace(hidden=torch.zeros(1))
+    host._device_only = lambda what: dec.Decoder._device_only(host, what)
+    for call in (lambda: dec.Decoder.generate_batch(host, [[1]], 1), lambda: dec.Decoder.score(host, [1, 2])):
+        with pytest.raises(ValueError, match="device memory"):
+            call()
