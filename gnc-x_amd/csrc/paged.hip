@@ -464,7 +464,8 @@ struct PagedParams {
 // (64 sequences of 100 to 8000 tokens, 8 KV heads of 128: 512 117.5 us, 1024 and 2048 110; one
 // of 60001 tokens, 4 KV heads: 19.9, 19.8, 21.0.  Four prompts of 300 to 700 tokens behind
 // 1152 to 3799, 32 heads on 8: 1024 316 us, 1536 283, 2048 254, 4096 395: a part costs 8 us
-// beside its steps' 4 us each, long parts end unevenly.  Equal shares of steps for as many
+// beside its steps' 4 us each, long parts end unevenly.  Full parts with a short last one
+// instead of equal ones: the 64 114.4 us for 112.4, the prompts 265.8 for 257.5.  Equal shares of steps for as many
 // work-groups as the chip holds, whatever tiles they end in, were slower in all three: 113,
 // 26.5 and 283.)
 constexpr int kKeysTarget = 1024, kRowsTarget = 2048;
@@ -473,13 +474,18 @@ constexpr int kLeastSteps = 4;   // of a part
 
 // The work of a call.  Rows of a sequence and KV head are numbered token by token,
 // `group` heads each, and cut into tiles of R; a tile's steps of 64 keys are cut into
-// parts of `per`, so many that the whole call's are about p.target work-groups'
+// equal parts of at most `per`, so many that the whole call's are about p.target work-groups'
 // (whatever the lengths are: they are read here).  Units, a tile's part each, are numbered
 // sequence by sequence.
 struct Unit {
     int seq, tile, part, n_parts, per;
     int64_t first;  // number of the tile's first unit
     SeqRows r;
+    // where part k of a tile of `steps` (2^24 at most) begins; parts behind those of `per` are empty
+    __device__ __forceinline__ int begin(int k, int steps) const {
+        const uint32_t n = static_cast<uint32_t>((steps - 1) / per) + 1;  // (128 at most)
+        return static_cast<int>(min(static_cast<uint32_t>(k), n) * static_cast<uint32_t>(steps) / n);
+    }
 };
 // The first key that a row at pos sees
 __device__ __forceinline__ int32_t low_of(const PagedParams& p, int32_t pos) {
@@ -868,8 +874,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     const int rows = u.r.count * p.group, row_lo = u.tile * R, row_hi = min(row_lo + R, rows);
     WaveRows<HD, 1> w;
     w.look(p, u.r, row_lo, row_hi);
-    const int step0 = w.low_first / 64 + u.part * u.per;
-    const int step1 = min(step0 + u.per, w.pos_last / 64 + 1);
+    const int first = w.low_first / 64, steps = w.pos_last / 64 + 1 - first;
+    const int step0 = first + u.begin(u.part, steps), step1 = first + u.begin(u.part + 1, steps);
     const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
     int step = step0 + wv;
     // keys of a step that this lane's blocks begin at: of K, whose rows it loads, and of V
@@ -999,8 +1005,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
     const int rows = u.r.count * p.group, tile_lo = u.tile * R, tile_hi = min(tile_lo + R, rows);
     const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
     const int32_t tile_low = low_of(p, u.r.len + tile_lo / p.group);
-    const int step0 = tile_low / 64 + u.part * u.per;
-    const int step1 = min(step0 + u.per, (u.r.len + (tile_hi - 1) / p.group) / 64 + 1);
+    const int first = tile_low / 64, steps = (u.r.len + (tile_hi - 1) / p.group) / 64 + 1 - first;
+    const int step0 = first + u.begin(u.part, steps), step1 = first + u.begin(u.part + 1, steps);
     // this wave's rows (the last one again where there are fewer) and what they see
     const int row_lo = min(tile_lo + 16 * RT * wv, rows - 1), row_hi = min(row_lo + 16 * RT, rows);
     WaveRows<HD, RT> w;
