@@ -80,6 +80,14 @@ __device__ __forceinline__ float wave_sum(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ double dpp_add_f64(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROW_MASK, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROW_MASK, 0xf, false);
+    return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 // Sum over aligned groups of N = 4, 8 or 16 lanes (the first N / 4 + 1 steps
 // of wave_sum_lane63); every lane of a group ends with the same sum.
 template <int N>

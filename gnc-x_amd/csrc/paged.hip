@@ -27,14 +27,28 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // ---- rotation ------------------------------------------------------------------
-// cos and sin of position * freq: the angle's turns in 64 bits, as 32 keep a far
-// position's only to 2^-24 of it, then one turn at most in 32.
-__device__ __forceinline__ void turn_of(int32_t pos, double freq, float magnitude, float& c, float& s) {
+// cos and sin of position * freq, times the magnitude, in 64 bits (32 keep a far position's
+// angle only to 2^-24 of it; and the chip multiplies and adds 64 bits as fast).  The angle's
+// turns less the nearest quarter leave x in [-pi / 4, pi / 4], whose Taylor sums are off by
+// 4 10^-13 at most; the quarter swaps and negates them.
+__device__ __forceinline__ void turn_of(int32_t pos, double freq, double magnitude, double& c, double& s) {
     double t = static_cast<double>(pos) * freq * 0.15915494309189535;  // 1 / (2 pi)
     t -= rint(t);
-    sincospif(2.0f * static_cast<float>(t), &s, &c);
-    c *= magnitude;
-    s *= magnitude;
+    const double k = rint(4.0 * t), x = (t - 0.25 * k) * 6.283185307179586, z = x * x;
+    double a = fma(z, 1.0 / 6227020800.0, -1.0 / 39916800.0), b = fma(z, 1.0 / 479001600.0, -1.0 / 3628800.0);
+    a = fma(z, a, 1.0 / 362880.0);
+    b = fma(z, b, 1.0 / 40320.0);
+    a = fma(z, a, -1.0 / 5040.0);
+    b = fma(z, b, -1.0 / 720.0);
+    a = fma(z, a, 1.0 / 120.0);
+    b = fma(z, b, 1.0 / 24.0);
+    a = fma(z, a, -1.0 / 6.0);
+    b = fma(z, b, -0.5);
+    a = fma(x * z, a, x);
+    b = fma(z, b, 1.0);
+    const int q = static_cast<int>(k) & 3;
+    c = magnitude * (q & 1 ? a : b) * (q == 1 || q == 2 ? -1.0 : 1.0);
+    s = magnitude * (q & 1 ? b : a) * (q >= 2 ? -1.0 : 1.0);
 }
 
 // Floats of pair p of a head: the rotated part's pairs, then the rest's, paired alike.
@@ -84,10 +98,11 @@ struct FourPairs {
     }
 };
 
-__device__ __forceinline__ void turn_pairs(float (&a)[4], float (&b)[4], const float (&c)[4], const float (&s)[4]) {
+template <class T>
+__device__ __forceinline__ void turn_pairs(T (&a)[4], T (&b)[4], const T (&c)[4], const T (&s)[4]) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const float x = a[j] * c[j] - b[j] * s[j];
+        const T x = a[j] * c[j] - b[j] * s[j];
         b[j] = b[j] * c[j] + a[j] * s[j];
         a[j] = x;
     }
@@ -112,10 +127,10 @@ __global__ __launch_bounds__(kRopeThreads) void rope_rows_kernel(RopeRowsParams 
     const int h0 = blockIdx.y * p.heads_per_group, h1 = min(h0 + p.heads_per_group, p.n_heads);
     const int32_t pos = p.positions[row];
     for (int i = tid; i < pairs; i += kRopeThreads) {
-        float c = 1.0f, s = 0.0f;
+        double c = 1.0, s = 0.0;
         if (i < half) turn_of(pos, p.rot.freqs[i], p.rot.magnitude, c, s);
-        cs[i] = c;
-        sn[i] = s;
+        cs[i] = static_cast<float>(c);
+        sn[i] = static_cast<float>(s);
     }
     __syncthreads();
     const float* in = p.rows + static_cast<size_t>(row) * p.stride;
@@ -224,6 +239,19 @@ __device__ __forceinline__ uint32_t moved_codes(uint32_t w, float f) {
 }
 
 template <int N>
+__device__ __forceinline__ double lanes_sum(double v) {  // (the same steps)
+    v = dpp_add_f64<0xb1>(v);
+    v = dpp_add_f64<0x4e>(v);
+    v = dpp_add_f64<0x141>(v);
+    if constexpr (N >= 16) v = dpp_add_f64<0x140>(v);
+    return N == 32 ? v + __shfl_xor(v, 16, 64) : v;
+}
+__device__ __forceinline__ float root_inverse(float v) { return 1.0f / sqrtf(v); }
+__device__ __forceinline__ double root_inverse(double v) {  // one step of Newton's on 24 bits
+    const double y = __builtin_amdgcn_rsq(v), e = fma(-v * y, y, 1.0);
+    return e == e ? fma(0.5 * y, e, y) : y;  // (0 and infinity)
+}
+template <int N>
 __device__ __forceinline__ float lanes_sum(float v) {
     if constexpr (N == 32) {
         v = group_sum<16>(v);
@@ -231,6 +259,15 @@ __device__ __forceinline__ float lanes_sum(float v) {
     } else {
         return group_sum<N>(v);
     }
+}
+// v in 32 bits with the last one set where it is not exact: what is then rounded to fewer
+// is rounded as v would be.
+__device__ __forceinline__ float odd_float(double v) {
+    const float f = static_cast<float>(v);
+    const double back = static_cast<double>(f);
+    if (back == v || !(fabsf(f) < __builtin_inff())) return f;
+    const uint32_t bits = __builtin_bit_cast(uint32_t, f) - (fabs(back) > fabs(v) ? 1u : 0u);
+    return __builtin_bit_cast(float, bits | 1u);
 }
 
 struct AppendParams {
@@ -256,12 +293,12 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
     const bool inter = a.rot.interleaved != 0;
     const int half = a.rot.n_rot / 2;
     const FourPairs at(u, a.rot.n_rot, HD, inter);
-    auto normed = [&](float(&x)[4], float(&y)[4], const float* gamma) {
-        float ss = 0.0f;
+    auto normed = [&]<class T>(T(&x)[4], T(&y)[4], const float* gamma) {
+        T ss = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) ss += x[j] * x[j] + y[j] * y[j];
         ss = lanes_sum<kPer>(ss);
-        const float inv = 1.0f / sqrtf(ss / HD + a.eps);
+        const T inv = root_inverse(ss / HD + static_cast<T>(a.eps));
         float gx[4], gy[4];
         if (gamma) at.load(gamma, gx, gy);
 #pragma unroll
@@ -277,7 +314,12 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
         if (s < 0) return;
         const SeqRows r = seq_rows(c, s);
         if (row < r.row0 || row - r.row0 >= r.count) return;
-        if (tid < half) turn_of(r.len + row - r.row0, a.rot.freqs[tid], a.rot.magnitude, cs[tid], sn[tid]);
+        if (tid < half) {
+            double cc, ss;
+            turn_of(r.len + row - r.row0, a.rot.freqs[tid], a.rot.magnitude, cc, ss);
+            cs[tid] = static_cast<float>(cc);
+            sn[tid] = static_cast<float>(ss);
+        }
         __syncthreads();
         if (h >= a.n_heads) return;
         const size_t head = (static_cast<size_t>(row) * a.n_heads + h) * HD;
@@ -332,12 +374,25 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
         }
     }
     if (!which) {
-        if (a.norm) normed(x, y, a.k_gamma);
+        // K in 64 bits up to its codes, so that they are the formula's (in 32 one in a million
+        // is rounded to the other side; 1752 rows, 32 heads on 8 of 128: 27.5 us for 26.2)
+        double dx[4], dy[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            dx[j] = x[j];
+            dy[j] = y[j];
+        }
+        if (a.norm) normed(dx, dy, a.k_gamma);
         if (is_new && 4 * u < half) {
-            float cc[4], ss[4];
+            double cc[4], ss[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) turn_of(base + tok, a.rot.freqs[4 * u + j], a.rot.magnitude, cc[j], ss[j]);
-            turn_pairs(x, y, cc, ss);
+            turn_pairs(dx, dy, cc, ss);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            x[j] = odd_float(dx[j]);
+            y[j] = odd_float(dy[j]);
         }
     }
     float amax = 0.0f;

@@ -271,8 +271,14 @@ class Paged:
 
 
 def nearest_e4m3(x):
-    """How far a stored value may be from x / scale: half a step, 2^-4 of it, 2^-10 below the normal ones."""
-    return (2.0 ** -4 * x.abs()).clamp(min=2.0 ** -10)
+    """How far a stored value may be from x / scale: half a step, 2^-4 of the power of two
+    below it, 2^-10 below the normal ones."""
+    return power_below(x).clamp(min=2.0 ** -6) / 16
+
+
+def power_below(x):
+    m, e = x.abs().frexp()
+    return (0 * x + 1).ldexp(e - 1) * (m != 0)
 
 
 def check_append(p, before, turn=None, norm=-1, q=True):
@@ -283,17 +289,20 @@ def check_append(p, before, turn=None, norm=-1, q=True):
     k, v, scales = k0.clone(), v0.clone(), s0.clone()
     turn = turn or Turn(torch, 0)
 
-    def head(x, n, gamma, at):
-        """64-bit result and how far 32 bits may be off.  A norm's sum (positive terms) is off
+    def head(x, n, gamma, at, bits=32):
+        """64-bit result and how far 32 bits may be off (64: 2^-14 of that, as
+        the kernel's cosine and sine, to 2^-41 of 1, count the most).  A norm's sum (positive terms) is off
         by at most 14 of its roundings, its root by half of that; with the root, the
         division and the products, 12 u of an element, and 12 u mag (|a| + |b|) turned."""
         x = x.double().view(-1, n, p.hd)
+        less = 2.0 ** -14 if bits == 64 else 1.0
         if norm < 0:
-            return turn(x, at)
+            y, tol = turn(x, at)
+            return y, tol * less
         x = x / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS)
         x = x * gamma.double() if norm > 0 else x
         y, tol = turn(x, at)
-        return y, tol * (25 / 13) + 12 * U * x.abs()
+        return y, (tol * (25 / 13) + 12 * U * x.abs()) * less
 
     for s, (a, n) in enumerate(zip(p.held, p.new)):
         room = p.max_pages * p.page
@@ -306,7 +315,7 @@ def check_append(p, before, turn=None, norm=-1, q=True):
         if q:
             want, tol = head(p.q[rows], p.H, p.gamma[0], at)
             assert ((p.out[rows].double().view(n, p.H, p.hd) - want).abs() <= tol).all()
-        wk, tk = head(p.kr[rows], p.KV, p.gamma[1], at)
+        wk, tk = head(p.kr[rows], p.KV, p.gamma[1], at, 64)
         wv = p.vr[rows].double().view(n, p.KV, p.hd)
         pos = a
         while pos < a + n:
