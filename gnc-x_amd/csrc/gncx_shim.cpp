@@ -3385,8 +3385,17 @@ GNCX_API int gncx_hip_rope_frequencies(int32_t n_rot, double base, int32_t scali
     }
     const int32_t half = n_rot / 2;
     std::array<float, 512> fac{};
+    const bool fac_there = factors && is_device_ptr(factors), out_there = is_device_ptr(out_freqs);
+    if (fac_there || out_there) {
+        if (!ensure_runtime(where)) return -1;
+        Allocations seen;
+        if ((fac_there && !on_device(factors, sizeof(float) * half, "factors", where, seen)) ||
+            (out_there && !on_device(out_freqs, sizeof(double) * half, "out_freqs", where, seen, 8)) ||
+            !check(hipStreamSynchronize(g_rt.stream), where))
+            return -1;
+    }
     if (factors) {
-        if (is_device_ptr(factors)) {
+        if (fac_there) {
             if (!check(hipMemcpy(fac.data(), factors, sizeof(float) * half, hipMemcpyDeviceToHost), where)) return -1;
         } else {
             std::memcpy(fac.data(), factors, sizeof(float) * half);
@@ -3412,7 +3421,7 @@ GNCX_API int gncx_hip_rope_frequencies(int32_t n_rot, double base, int32_t scali
         }
         if (factors && fac[i] != 0.0f) f[i] /= fac[i];
     }
-    if (is_device_ptr(out_freqs)) {
+    if (out_there) {
         if (!check(hipMemcpy(out_freqs, f.data(), sizeof(double) * half, hipMemcpyHostToDevice), where)) return -1;
     } else {
         std::memcpy(out_freqs, f.data(), sizeof(double) * half);

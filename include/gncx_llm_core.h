@@ -532,8 +532,8 @@ typedef struct GNCXPagedCache {
     int32_t n_pages, page_tokens, n_kv_heads, head_dim;
 } GNCXPagedCache;
 /* The sequences of a call (device arrays).  Rows row_start[s] ..
- * row_start[s + 1] - 1 (ascending, up to n_rows) are the next tokens of
- * sequence s, whose pages hold lengths[s] tokens before them: row
+ * row_start[s + 1] - 1 (ascending, up to n_rows; what rows get otherwise is
+ * open) are the next tokens of sequence s, whose pages hold lengths[s] tokens before them: row
  * row_start[s] + i is at position lengths[s] + i, which lies in the page
  * pages[s * max_pages + position / page_tokens].  A sequence may have no rows.
  * Rows behind the last sequence's, rows past max_pages * page_tokens positions
@@ -568,8 +568,8 @@ typedef struct GNCXRotation {
  *                     *out_magnitude (host) is 0.1 ln(factor) + 1, otherwise 1
  * and divided by factors[i] (host or device, n_rot / 2 floats, as a GGUF's
  * rope_freqs tensor holds; NULL for none, 0 leaves a pair as it is).  Waits for
- * the device where out_freqs is device memory.  0, or -1 with
- * gncx_hip_last_error set. */
+ * the device where one of them is device memory (8-byte aligned out_freqs), and is
+ * then no call for a capture.  0, or -1 with gncx_hip_last_error set. */
 enum { GNCX_ROPE_PLAIN = 0, GNCX_ROPE_LINEAR = 1, GNCX_ROPE_BASE = 2, GNCX_ROPE_YARN = 3 };
 int gncx_hip_rope_frequencies(int32_t n_rot, double base, int32_t scaling, double factor, int32_t trained_context,
                               double beta_fast, double beta_slow, const float* factors, double* out_freqs,
@@ -592,7 +592,9 @@ void gncx_hip_rope_rows(const float* rows, int32_t n_rows, int32_t row_stride, i
  * their codes are rounded to the new one (exact but for codes that become
  * subnormal).  Infinities and NaN are stored as NaN.  Rows of one call go to
  * places of their own: no page that is appended to may stand twice in the tables.
- * No two of the arguments' arrays overlap but as said. */
+ * Codes are the nearest to the formula's value in 64 bits, queries are formed in 32.
+ * Rows and out_q are 16-byte aligned, norm weights in device memory too.  No two of
+ * the arguments' arrays overlap but as said. */
 void gncx_hip_kv_append_paged(const GNCXPagedCache* cache, const GNCXPagedBatch* batch, const float* q_rows,
                               const float* k_rows, const float* v_rows, int32_t n_heads, const uint8_t* mmap_base,
                               size_t q_norm_offset, size_t k_norm_offset, int32_t has_norm_weight, float norm_eps,

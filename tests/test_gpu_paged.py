@@ -118,6 +118,14 @@ def test_rope_frequencies_on_the_device(lib, torch_mod):
     for f, o in ((d_fac.data_ptr(), out.data_ptr()), (fac.ctypes.data, host.ctypes.data)):
         assert lib.gncx_hip_rope_frequencies(64, 1e4, gncx.ROPE_YARN, 4.0, 4096, 32.0, 1.0, f, o, C.addressof(mag)) == 0
     assert (out.cpu().numpy() == host).all() and host[0] == 1.0
+    # memory that ends before the last of them, or lies between two
+    end = torch.zeros(2 ** 22, dtype=torch.float64, device="cuda")  # (an allocation of its own)
+    for f, o, text in ((None, end.data_ptr() + 8 * (2 ** 22 - 31), "past the end"), (None, out.data_ptr() + 4, "8-byte"),
+                       (end.data_ptr() + 8 * 2 ** 22 - 4 * 31, host.ctypes.data, "past the end")):
+        lib.gncx_hip_last_status()
+        assert lib.gncx_hip_rope_frequencies(64, 1e4, gncx.ROPE_PLAIN, 1.0, 0, 0.0, 0.0, f, o, None) == -1
+        refused(lib, text)
+    assert (end == 0).all() and (out.cpu().numpy() == host).all()
 
 
 def test_rope_refusals(lib, torch_mod):
