@@ -44,6 +44,9 @@ __device__ __forceinline__ uint4 ld16_a2(const uint8_t* p) {
 
 __device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xffu; }
 
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
+
 __device__ __forceinline__ float half_bits_to_float(uint32_t h) {
     // v_cvt_f32_f16: exact IEEE conversion (subnormal halves are normal floats)
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));

@@ -1,13 +1,15 @@
-// paged.hip -- many sequences at once over a paged cache of 8-bit blocks: rotary
-// positions of rows, appending keys and values (with the per-head RMSNorm and the
-// rotation on the way), and attention over the cache.
+// paged.h -- a part of attention.hip: many sequences at once over a paged cache of
+// 8-bit blocks.  Rotary positions of rows, appending keys and values (with the
+// per-head RMSNorm and the rotation on the way), and attention over the cache.
 //
 // A block is 16 positions of one KV head, K as [16][HD] and V as [HD][16] e4m3
 // codes, each with a power of two as scale.  A power of two costs up to a bit of
 // range that e4m3 has to spare, and buys that a value's code is the same digits in
 // any scale: a block whose scale grows while tokens are appended keeps its codes
-// exactly (but for those that become subnormal), and bfloat16, which the matrix
-// instructions take, holds code times scale exactly.
+// exactly (but for those that become subnormal), and a scale is an addition to the
+// exponent of the block's scores and weights, while the matrix instructions take
+// the codes themselves, exact in fp16.
+#pragma once
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -472,8 +474,6 @@ constexpr int kAttnThreads = 256, kAttnWaves = 4;
 __device__ __forceinline__ u32x4 four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return u32x4{a, b, c, d}; }
 constexpr float kInf = __builtin_inff();
 
-__device__ __forceinline__ uint32_t as_bits(float x) { return __builtin_bit_cast(uint32_t, x); }
-__device__ __forceinline__ float as_float(uint32_t x) { return __builtin_bit_cast(float, x); }
 // Over the four lanes of a column: lanes 16 apart, then 32 apart.  The swap of two copies
 // leaves one of each pair in the first, the other in the second.
 template <class F>
@@ -517,13 +517,12 @@ struct PagedParams {
 };
 // Work-groups that a split of keys aims at, for few rows a sequence and for many
 // (64 sequences of 100 to 8000 tokens, 8 KV heads of 128: 512 117.5 us, 1024 and 2048 110; one
-// of 60001 tokens, 4 KV heads: 19.9, 19.8, 21.0.  Four prompts of 300 to 700 tokens behind
-// 1152 to 3799, 32 heads on 8: 1024 316 us, 1536 283, 2048 254, 4096 395: a part costs 8 us
-// beside its steps' 4 us each, long parts end unevenly.  Full parts with a short last one
-// instead of equal ones: the 64 114.4 us for 112.4, the prompts 265.8 for 257.5.  Equal shares of steps for as many
-// work-groups as the chip holds, whatever tiles they end in, were slower in all three: 113,
-// 26.5 and 283.)
-constexpr int kKeysTarget = 1024, kRowsTarget = 2048;
+// of 60001 tokens, 4 KV heads: 19.9, 19.8, 21.0.  Prompts, 32 heads on 8 KV heads: four of
+// 300 to 700 tokens behind 1152 to 3799, 512 246 us, 768 241, 1024 244, 2048 263; one of 600
+// behind 30000, 725, 594, 665, 642; 40 of 100 behind 500 to 3000, 314, 313, 342, 381.  Equal
+// shares of steps for as many work-groups as the chip holds, whatever tiles they end in,
+// were slower: the 64 113 us, the 60001 26.5, the four 283.)
+constexpr int kKeysTarget = 1024, kRowsTarget = 768;
 constexpr int kMostParts = 128;  // of a row
 constexpr int kLeastSteps = 4;   // of a part
 
@@ -602,9 +601,26 @@ __device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit&
                   static_cast<int>(ceilf(fminf(total * static_cast<float>(p.c.n_kv) / static_cast<float>(p.target), 1 << 26))));
         if (p.c.n_seqs > 64) w = seq_work<R>(p, lane);
     }
+    int seq = lane;
+    // Few long parts end unevenly: those of many rows are in falling order (four prompts as
+    // above 272 -> 241 us, 16 of 64 to 200 tokens behind up to 6000 250 -> 222).
+    if (R >= 64 && p.split && p.c.n_seqs > 1 && p.c.n_seqs <= 64) {
+        const int parts = w.steps ? (w.steps - 1) / per + 1 : 1, each = w.steps ? (w.steps - 1) / parts + 1 : 0;
+        int rank = 0;
+        for (int l = 0; l < p.c.n_seqs; ++l) {
+            const int o = __builtin_amdgcn_readlane(each, l);
+            rank += o > each || (o == each && l < lane);
+        }
+        seq = __builtin_amdgcn_ds_permute(4 * (lane < p.c.n_seqs ? rank : lane), lane);
+        auto moved = [&](int v) { return __shfl(v, seq, 64); };
+        w = SeqWork{moved(w.tiles), moved(w.steps), {moved(w.r.row0), moved(w.r.count), moved(w.r.len)}};
+    }
     int units = 0, tiles = 0;  // of the sequences before
     for (int s0 = 0; s0 < p.c.n_seqs; s0 += 64) {
-        if (s0) w = seq_work<R>(p, s0 + lane);
+        if (s0) {
+            seq = s0 + lane;
+            w = seq_work<R>(p, seq);
+        }
         const int parts = w.steps ? (w.steps - 1) / per + 1 : 0;
         const int64_t own = static_cast<int64_t>(w.tiles) * parts;
         const int to_unit = add_up(units, wave_prefix(static_cast<int>(min(own, int64_t{0x7fffffff}))));
@@ -614,9 +630,9 @@ __device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit&
             const int l = __builtin_ctzll(past);
             auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             auto before = [&](int v, int none) { return l ? __builtin_amdgcn_readlane(v, l - 1) : none; };
-            u.seq = s0 + l;
+            u.seq = of(seq);
             u.n_parts = of(parts);
-            u.per = per;
+            u.per = (of(w.steps) - 1) / u.n_parts + 1;
             u.r = SeqRows{of(w.r.row0), of(w.r.count), of(w.r.len)};
             const int first = before(to_unit, units);
             if constexpr (BY_TILE) {
@@ -627,6 +643,7 @@ __device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit&
                 u.part = index - first - u.tile * u.n_parts;
             }
             u.first = first + static_cast<int64_t>(u.tile) * u.n_parts;
+            if (R >= 64) u.tile = of(w.tiles) - 1 - u.tile;  // (the last tiles see the most keys)
             return true;
         }
         units = __builtin_amdgcn_readlane(to_unit, 63);
@@ -670,10 +687,10 @@ __device__ __forceinline__ void split_queries(const float* q, int g, float scale
 
 // A row's running maximum, sum (of this lane's keys) and output, in units of 2^(unit - 14).
 template <int HD>
-struct RowState {
+struct PagedRow {
     float m = -kInf, l = 0.0f;
     f32x4 o[HD / 16];
-    __device__ RowState() {
+    __device__ PagedRow() {
 #pragma unroll
         for (int d = 0; d < HD / 16; ++d) o[d] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -794,7 +811,7 @@ __device__ __forceinline__ bool one_unit(bool there, float scale, int& unit, flo
 // A step of RT row tiles, from their products with the keys on: sc are the scales of this
 // lane's block, if it is there, and values(d) the codes of its float 16 d + n.
 template <int HD, int RT, class Values>
-__device__ __forceinline__ void take_step(RowState<HD> (&st)[RT], f32x4 (&s)[RT][4], const float (&fac)[RT], float2 sc,
+__device__ __forceinline__ void take_step(PagedRow<HD> (&st)[RT], f32x4 (&s)[RT][4], const float (&fac)[RT], float2 sc,
                                           bool there, bool full, const uint32_t (&seen)[RT], int unit, float units,
                                           Values&& values) {
     f16x8 hi[RT][2], lo[RT][2];
@@ -829,7 +846,7 @@ __device__ __forceinline__ void take_step(RowState<HD> (&st)[RT], f32x4 (&s)[RT]
 // (Inside the loops of the others this would cost them 60 registers.)
 template <int HD, int RT>
 __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* table, int hk, const WaveRows<HD, RT>& w,
-                                           RowState<HD> (&st)[RT], int& unit, int step, int every, int end) {
+                                           PagedRow<HD> (&st)[RT], int& unit, int step, int every, int end) {
     const PagedArgs& c = p.c;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     for (; step < end; step += every) {
@@ -939,7 +956,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     const int row = min(row_lo + n, rows - 1);
     w.pos[0] = u.r.len + row / p.group;
     split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, w.qh[0], w.ql[0], w.fac[0]);
-    RowState<HD> st[1];
+    PagedRow<HD> st[1];
     int unit_exp = kNoUnit;
     // (a block that is not there: the first one is read, and hidden)
     u32x4 kw[4][kSlices], vw[kDims];
@@ -1109,7 +1126,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
     int64_t bv = block_in(c, page, hk, 64 * step0 + 16 * g);
     float2 scale = scale_of(bv);
     page = page_at(c, table, 64 * (step0 + 1) + 16 * g);
-    RowState<HD> st[RT];
+    PagedRow<HD> st[RT];
     int unit_exp = kNoUnit, hard = -1;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {

@@ -786,6 +786,53 @@ def test_captured_decode_steps(lib, torch_mod):
         lib.gncx_hip_set_stream(None)
 
 
+def test_two_captured_graphs_beside_one_another(lib, torch_mod):
+    """Two graphs of attention and log probabilities, replayed at once on two streams with
+    eager calls (that grow the eager workspaces) between: each has its own parts."""
+    torch = torch_mod
+    sets = []
+    for i, (held, new) in enumerate((([5000, 300], [1, 1]), ([2500], [40]))):
+        p = Paged(torch, held, new, H=32, KV=8, hd=128, seed=40 + i)
+        p.append(lib)
+        p.attend(lib)
+        x = 3 * randn(torch, 50 + i, 3, 60000 + 7000 * i)
+        sets.append((p, p.out.clone(), x, logprobs(lib, torch, x, whole(torch, [5, 6, 7]), 9)))
+    streams, graphs, outs = [torch.cuda.Stream() for _ in sets], [], []
+    torch.cuda.synchronize()
+    try:
+        for (p, _, x, _), stream in zip(sets, streams):
+            lib.gncx_hip_set_stream(stream.cuda_stream)
+            graph, tokens = torch.cuda.CUDAGraph(), whole(torch, [5, 6, 7])
+            out = [torch.empty(3, device="cuda"), torch.empty(3, device="cuda"),
+                   torch.empty(3, 9, dtype=torch.int32, device="cuda"), torch.empty(3, 9, device="cuda")]
+            torch.cuda.synchronize()
+            with torch.cuda.graph(graph, stream=stream):
+                p.attend(lib)
+                lib.gncx_hip_token_logprobs(x.data_ptr(), 3, x.shape[1], tokens.data_ptr(), 9,
+                                            *(t.data_ptr() for t in out))
+            graphs.append(graph)
+            outs.append((out, tokens))
+        lib.gncx_hip_set_stream(None)
+        for i in range(4):
+            for (p, *_), (out, _) in zip(sets, outs):
+                p.out.zero_()
+                for t in out:
+                    t.zero_()
+            torch.cuda.synchronize()
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+            other = Paged(torch, [3000] * (1 + i), [1 + 20 * i] * (1 + i), H=32, KV=8, hd=128, seed=60 + i)
+            other.append(lib)
+            other.attend(lib)
+            torch.cuda.synchronize()
+            for (p, want, _, answer), (out, _) in zip(sets, outs):
+                assert torch.equal(p.out, want) and all(torch.equal(a, b) for a, b in zip(out, answer))
+            other.check_attention()
+    finally:
+        lib.gncx_hip_set_stream(None)
+
+
 def test_calls_on_another_stream(lib, torch_mod):
     torch = torch_mod
     p = Paged(torch, [2000, 3], [1, 1], H=32, KV=8, hd=128, seed=15)
