@@ -1168,7 +1168,11 @@ int32_t select_vectors(int32_t n_beams, int32_t vocab) {
 // log p(v) = x_v - m - log S and H = log S - T / S, with S the sum of e^(x - m) and T that
 // of e^(x - m) (x - m).  As in beam search's selection, a work-group holds a part of
 // a row in registers and leaves its maximum, its two sums and its n_top best; a second
-// kernel joins the parts of a row.  A row of one part is finished by the first.
+// kernel joins the parts of a row.  A row of one part is finished by the first.  Bound by
+// reading the logits where rows are many (1999 x 32000 without alternatives 49 us, 5.2 TB/s of
+// 256 MB), by the parts' chain of maximum, sums, threshold and ranking where alternatives are
+// asked for (64 x 151936, 20 best: 15.5 and 5.6 us, 39 MB), by two launches and their
+// latencies for one row (4.4 and 5.4).
 struct LogprobParams {
     const float* logits;
     const int32_t* tokens;  // null: no out_logprobs

@@ -110,8 +110,13 @@ __device__ __forceinline__ void turn_pairs(T (&a)[4], T (&b)[4], const T (&c)[4]
     }
 }
 
-// A work-group takes a row and some of its heads; its first threads form the
-// row's cosines and sines, one pair each, for all of them.
+// (a, b) -> (a cos - b sin, b cos + a sin) over a row's pairs.  Bound by memory, 8 bytes a
+// float (2048 rows of 40 heads of 128, half of each turned: 13 to 14 us, 6 TB/s of 84 MB that
+// the caches hold in part), a single row by the launch.  A work-group takes a row and some of
+// its heads; its first threads form the row's cosines and sines, one pair each, for all of
+// them, so that 64-bit angles cost a head's share of the heads.  Heads of 8 floats and more
+// move as float4 where strides and addresses allow, others one float at a time (any even
+// size, stride and alignment).
 constexpr int kRopeThreads = 256;
 constexpr int kMaxRopeDim = 1024;
 struct RopeRowsParams {
@@ -278,7 +283,11 @@ struct AppendParams {
     int32_t head_groups;  // of a row's queries
 };
 
-// Blocks and queries in one launch.  A work-group takes the new tokens of one block
+// scale = max(old, 2^e), e the least with amax <= 448 2^e over the new values; codes are
+// x / scale rounded to e4m3, old ones times old / scale again.  Blocks and queries in one
+// launch: few rows are bound by it and by two dependent reads (one row 4.6 us, 64 rows of 64
+// sequences 8.0), many by memory and the 64-bit rotation of K (1752 rows of 32 heads on 8 of
+// 128, 106 MB: 28 us, 3.8 TB/s).  A work-group takes the new tokens of one block
 // of K or of V: 16 tokens, HD / 8 threads each.  Nobody else touches the block, so
 // its old tokens are moved to a larger scale on the way, without atomics.  Sequence
 // s has the blocks from slot row_start[s] / 16 + 2 s on: as many as it can touch.
@@ -931,7 +940,11 @@ __device__ __forceinline__ float* row_of(float* base, const PagedParams& p, cons
 }
 
 // Few rows a sequence (a decode step): a work-group has 16 rows, and its four waves take
-// every fourth step each.
+// every fourth step each, from memory straight into registers, as no wave needs another's
+// keys.  Bound by reading the cache: 64 sequences of 100 to 8000 tokens, 8 KV heads of 128,
+// 538 MB in 106 us (5.1 TB/s; the same loads alone take as long); one of 60001 tokens, 4 KV
+// heads, 62 MB in 16 us, of which 3 are the start and the last wave's end; one of 1000 tokens
+// 7.5 us of latencies: sequence, page, codes, products, parts.
 template <int HD>
 __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_kernel(PagedParams p) {
     constexpr int R = 16, kSlices = HD / 64, kDims = HD / 16;
@@ -1060,6 +1073,12 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
 }
 
 // Many rows (prompts): a wave has 16 RT rows of its own, a work-group four times as many.
+// Bound by the issue of vector and matrix instructions, which share it (584 of them and 128
+// products of two slots each a wave and step): four prompts of 300 to 700 tokens behind 1152
+// to 3799, 32 heads on 8 of 128, 2 x 101 GFLOP in 242 us; in the loop 1060 TFLOP/s, of the
+// 1315 that a large library product reaches; the rest are the parts' starts and ends.
+// (32x32x16 products, half as many instructions: heads of 128 6% slower, of 256 34%, of 64
+// 9% faster.)
 // The codes of a step are staged in LDS for all of them, two steps in turn: the next one's
 // are on their way from memory during a step, and laid down at its end, so that a step
 // takes one barrier.
@@ -1224,7 +1243,10 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
     }
 }
 
-// out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the parts c.  HD / 4
+// out = sum_c w_c o_c / sum_c w_c with w_c = l_c 2^(m_c - M) over the parts c.  Bound by
+// latency (a launch, the sequences, the parts: 2.9 to 5.4 us for decode steps) or by reading
+// the parts (the four prompts 22 us).  In the attention's own launch, by the last work-group
+// of a tile with device-scope accesses, it took 2 to 30 us longer.  HD / 4
 // threads have a row's floats; up to kAtOnce parts they have the row to themselves, more
 // parts are shared by the work-group, whose sums then meet in LDS.
 template <int HD, int R>
