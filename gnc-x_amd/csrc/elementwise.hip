@@ -851,7 +851,6 @@ __device__ __forceinline__ float nth_of_wave(float v, int n) {
     return least > 0x007fffffu ? unordered(least) : -__builtin_inff();
 }
 
-// v and another lane's, through DPP (no LDS round trip, unlike a shuffle)
 // Sum over the wave, returned in every lane: wave_sum's steps.
 __device__ __forceinline__ double wave_sum_f64(double v) {
     v = dpp_add_f64<0xb1>(v);
@@ -879,13 +878,13 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 // i), in two steps with a barrier between them: those that reach `least`
 // (nth_largest's of the threads' maxima) go to LDS, held being 0 before a barrier, then
 // the best go to `best` in falling order, -inf behind the last.  A NaN is no word, -0 is 0.
-struct PartWords {
-    uint64_t keys[kMostRanked];
-    uint64_t redk[kCandThreads / 64];
-    int held;
+struct PartWords {  // (arrays of LDS: as one object they cost beam search 0.1 us)
+    uint64_t (&keys)[kMostRanked];
+    uint64_t (&redk)[kCandThreads / 64];
+    int& held;
 };
 template <int V>
-__device__ __forceinline__ void gather_words(const float (&x)[V][4], int v0, float least, PartWords& sh) {
+__device__ __forceinline__ void gather_words(const float (&x)[V][4], int v0, float least, const PartWords& sh) {
     int mine = 0;
 #pragma unroll
     for (int j = 0; j < V; ++j)
@@ -904,7 +903,7 @@ __device__ __forceinline__ void gather_words(const float (&x)[V][4], int v0, flo
     }
 }
 template <int V>
-__device__ __forceinline__ void rank_words(const float (&x)[V][4], int v0, int n_out, float2* best, PartWords& sh) {
+__device__ __forceinline__ void rank_words(const float (&x)[V][4], int v0, int n_out, float2* best, const PartWords& sh) {
     constexpr int kWavesHere = kCandThreads / 64;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int n = sh.held;
@@ -952,7 +951,10 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
     constexpr int kWavesHere = kCandThreads / 64;
     __shared__ __align__(16) float maxima[kGroups];
     __shared__ double sums[kWavesHere];
-    __shared__ PartWords sh;
+    __shared__ uint64_t keys[kMostRanked];
+    __shared__ uint64_t redk[kCandThreads / 64];
+    __shared__ int held;
+    const PartWords sh{keys, redk, held};
     const int b = blockIdx.y, c = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     if (p.finished && p.finished[b]) return;
     const int v0 = c * 1024 * V + 4 * tid;  // this thread's words: v0 + 1024 j + i
@@ -1222,7 +1224,10 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
     constexpr int kWavesHere = kCandThreads / 64;
     __shared__ __align__(16) float maxima[kGroups];
     __shared__ double sums[kWavesHere][2];
-    __shared__ PartWords sh;
+    __shared__ uint64_t keys[kMostRanked];
+    __shared__ uint64_t redk[kCandThreads / 64];
+    __shared__ int held;
+    const PartWords sh{keys, redk, held};
     __shared__ float2 tops[kMaxTopWords];
     const size_t b = blockIdx.x / p.n_chunks;
     const int c = blockIdx.x % p.n_chunks, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -1409,7 +1414,10 @@ __global__ __launch_bounds__(kCandThreads) void logprob_stream_kernel(LogprobPar
 
 __global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParams p) {
     __shared__ __align__(16) float maxima[kGroups];
-    __shared__ PartWords sh;
+    __shared__ uint64_t keys[kMostRanked];
+    __shared__ uint64_t redk[kCandThreads / 64];
+    __shared__ int held;
+    const PartWords sh{keys, redk, held};
     const size_t row = blockIdx.x;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, parts = p.n_chunks;
     const double* sums = p.sums + 3 * row * parts;

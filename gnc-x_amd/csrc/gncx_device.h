@@ -83,6 +83,7 @@ __device__ __forceinline__ float wave_sum(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
+// v and another lane's, through DPP (no LDS round trip, unlike a shuffle)
 template <int CTRL, int ROW_MASK = 0xf>
 __device__ __forceinline__ double dpp_add_f64(double v) {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
