@@ -1657,6 +1657,8 @@ __global__ __launch_bounds__(kThreads) void tree_prologue_kernel(TreeParams p, T
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 
 // (by value: a bit cast of a vector's element in place takes the first element)
+__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
+__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
 // the float of exponent field `field` (2^(field - 127))
 __device__ __forceinline__ float pow2_field(int field) { return __builtin_bit_cast(float, field << 23); }
 // amax's exponent field, kept where 2^(+-(14 + e)) are normal floats

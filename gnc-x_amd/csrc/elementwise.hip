@@ -10,6 +10,7 @@
 #include "gncx_act.h"
 #include "gncx_device.h"
 #include "gncx_launch.h"
+#include "gncx_wave64.h"
 
 namespace gncx {
 namespace {
@@ -849,20 +850,6 @@ __device__ __forceinline__ float nth_of_wave(float v, int n) {
         if (__builtin_popcountll(__ballot(o >= t)) >= n) least = t;
     }
     return least > 0x007fffffu ? unordered(least) : -__builtin_inff();
-}
-
-// Sum over the wave, returned in every lane: wave_sum's steps.
-__device__ __forceinline__ double wave_sum_f64(double v) {
-    v = dpp_add_f64<0xb1>(v);
-    v = dpp_add_f64<0x4e>(v);
-    v = dpp_add_f64<0x141>(v);
-    v = dpp_add_f64<0x140>(v);
-    v = dpp_add_f64<0x142, 0xa>(v);
-    v = dpp_add_f64<0x143, 0xc>(v);
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), 63);
-    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), 63);
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {

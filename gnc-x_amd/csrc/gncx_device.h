@@ -44,9 +44,6 @@ __device__ __forceinline__ uint4 ld16_a2(const uint8_t* p) {
 
 __device__ __forceinline__ uint32_t byte_of(uint32_t w, int i) { return (w >> (8 * i)) & 0xffu; }
 
-__device__ __forceinline__ float as_float(uint32_t u) { return __builtin_bit_cast(float, u); }
-__device__ __forceinline__ uint32_t as_bits(float f) { return __builtin_bit_cast(uint32_t, f); }
-
 __device__ __forceinline__ float half_bits_to_float(uint32_t h) {
     // v_cvt_f32_f16: exact IEEE conversion (subnormal halves are normal floats)
     return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
@@ -81,15 +78,6 @@ __device__ __forceinline__ float wave_sum_lane63(float v) {
 __device__ __forceinline__ float wave_sum(float v) {
     v = wave_sum_lane63(v);
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
-
-// v and another lane's, through DPP (no LDS round trip, unlike a shuffle)
-template <int CTRL, int ROW_MASK = 0xf>
-__device__ __forceinline__ double dpp_add_f64(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(u), CTRL, ROW_MASK, 0xf, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(u >> 32), CTRL, ROW_MASK, 0xf, false);
-    return v + __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // Sum over aligned groups of N = 4, 8 or 16 lanes (the first N / 4 + 1 steps

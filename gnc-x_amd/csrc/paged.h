@@ -16,6 +16,7 @@
 
 #include "gncx_device.h"
 #include "gncx_launch.h"
+#include "gncx_wave64.h"
 
 namespace gncx {
 namespace {
