@@ -525,14 +525,6 @@ struct PagedParams {
     int32_t units;    // that there is place for
     float scale;      // attn_scale log2(e)
 };
-// Work-groups that a split of keys aims at, for few rows a sequence and for many
-// (64 sequences of 100 to 8000 tokens, 8 KV heads of 128: 512 117.5 us, 1024 and 2048 110; one
-// of 60001 tokens, 4 KV heads: 19.9, 19.8, 21.0.  Prompts, 32 heads on 8 KV heads: four of
-// 300 to 700 tokens behind 1152 to 3799, 512 246 us, 768 241, 1024 244, 2048 263; one of 600
-// behind 30000, 725, 594, 665, 642; 40 of 100 behind 500 to 3000, 314, 313, 342, 381.  Equal
-// shares of steps for as many work-groups as the chip holds, whatever tiles they end in,
-// were slower: the 64 113 us, the 60001 26.5, the four 283.)
-constexpr int kKeysTarget = 1024, kRowsTarget = 768;
 constexpr int kMostParts = 128;  // of a row
 constexpr int kLeastSteps = 4;   // of a part
 
@@ -1333,7 +1325,9 @@ __global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedParams p
 }
 
 // The split of a call, from what the host knows of it: few rows a sequence share
-// their keys over the waves, many have waves of their own.
+// their keys over the waves, many have waves of their own.  (Equal shares of steps for as many
+// work-groups as the chip holds, whatever tiles they end in, were slower: 64 sequences of 100
+// to 8000 113 us for 112, one of 60001 26.5 for 21.1, the four prompts below 283 for 255.)
 struct PagedPlan {
     bool keys, split;
     int32_t rows, target;
@@ -1345,10 +1339,26 @@ PagedPlan paged_plan(const PagedAttnArgs& a) {
     pl.keys = rows <= 32 * static_cast<int64_t>(a.c.n_seqs);
     pl.rows = pl.keys ? 16 : a.c.head_dim == 256 ? 64 : 128;
     pl.tiles = rows / pl.rows + a.c.n_seqs;
-    pl.target = pl.keys ? kKeysTarget : kRowsTarget;
-    // tiles for the chip without a split: no parts, no merge
-    const int64_t steps = ((static_cast<int64_t>(a.c.max_pages) << a.c.page_bits) + 63) / 64;
-    pl.split = steps > kLeastSteps && pl.tiles * a.c.n_kv < 2048;
+    // work-groups without a split, and the steps that one may then have
+    const int64_t whole = pl.tiles * a.c.n_kv;
+    int64_t steps = ((static_cast<int64_t>(a.c.max_pages) << a.c.page_bits) + 63) / 64;
+    if (a.sliding_window > 0) steps = std::min(steps, (a.sliding_window + pl.rows / group + 63) / 64 + 1);
+    if (pl.keys) {
+        // Without a split a work-group has 0.36 us a step; a split costs 9 us of parts and
+        // merge.  So few steps are left whole, and more where others read meanwhile (8 KV
+        // heads of 128; split, whole; 1 sequence of 400 10.9, 8.4 us, of 1000 10.8, 11.2; 64
+        // of 1000 38, 29, of 100 to 8000 112, 124; 16 of 100 to 8000 39, 61; 200 of 100 to
+        // 2000 115, 96).  Targets of 512 and 1024: 16 of 100 to 8000 38.9, 40.8, 8 of 4000
+        // 19.4, 24.5, 64 of 100 to 8000 120, 112.
+        pl.split = steps > 10 + whole / 16 && whole < 2048;
+        pl.target = whole < 512 ? 512 : 1024;
+    } else {
+        // Prompts, 32 heads on 8 KV heads, targets of 512, 768, 1024 and 2048: four of 306 to
+        // 674 tokens behind 1152 to 3799 246, 241, 244, 263 us; one of 600 behind 30000 725,
+        // 594, 665, 642; 40 of 100 behind 500 to 3000 314, 313, 342, 381.
+        pl.split = steps > kLeastSteps && whole < 2048;
+        pl.target = 768;
+    }
     // units = sum over tiles of ceil(steps / per) <= target / n_kv + tiles (and one for the
     // device's rounding of per, which takes less than a part in 10^6 of it)
     pl.units = pl.tiles + (pl.split ? pl.target / a.c.n_kv + 2 : 0);
