@@ -1492,10 +1492,11 @@ __global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParam
 }
 
 // Words of a part: the most that leave 1024 parts over all rows, up to a row without
-// alternatives, else what registers hold (64 x 151936, 20 alternatives: 8192 words 22.8 us,
-// 16384 25.4).
+// alternatives, else what leaves four work-groups a CU their registers (20 alternatives, 4096,
+// 8192 and 16384 words: 64 x 151936 22.1, 21.5, 25.4 us; 128 x 151936 32.0, 29.8, 37.9; 2000 x
+// 32000 84, 75, 95).
 int32_t logprob_words(int32_t n_rows, int32_t vocab, int32_t n_top) {
-    const int32_t most = n_top ? 16384 : kMaxBeamVocab;
+    const int32_t most = n_top ? 8192 : kMaxBeamVocab;
     int32_t w = 2048;
     while (w < most && w < vocab && static_cast<int64_t>(n_rows) * ((vocab + 2 * w - 1) / (2 * w)) >= 1024) w *= 2;
     return w;
@@ -1644,8 +1645,7 @@ hipError_t launch_token_logprobs(const float* logits, int32_t n_rows, int32_t vo
     if (n_top == 0) hipLaunchKernelGGL(logprob_stream_kernel, grid, block, 0, stream, p, words);
     else if (words == 2048) hipLaunchKernelGGL(logprob_parts_kernel<2>, grid, block, 0, stream, p);
     else if (words == 4096) hipLaunchKernelGGL(logprob_parts_kernel<4>, grid, block, 0, stream, p);
-    else if (words == 8192) hipLaunchKernelGGL(logprob_parts_kernel<8>, grid, block, 0, stream, p);
-    else hipLaunchKernelGGL(logprob_parts_kernel<16>, grid, block, 0, stream, p);
+    else hipLaunchKernelGGL(logprob_parts_kernel<8>, grid, block, 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.n_chunks == 1) return e;
     hipLaunchKernelGGL(logprob_join_kernel, dim3(n_rows), dim3(kCandThreads), 0, stream, p);
