@@ -861,16 +861,16 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
     return v;
 }
 
-// The n_out best of the words that a work-group holds (thread tid's words: v0 + 1024 j +
-// i), in two steps with a barrier between them: those that reach `least`
+// The n_out best of the words that a work-group of T threads holds (thread tid's words: v0 +
+// 4 T j + i), in two steps with a barrier between them: those that reach `least`
 // (nth_largest's of the threads' maxima) go to LDS, held being 0 before a barrier, then
 // the best go to `best` in falling order, -inf behind the last.  A NaN is no word, -0 is 0.
 struct PartWords {  // (arrays of LDS: as one object they cost beam search 0.1 us)
     uint64_t (&keys)[kMostRanked];
-    uint64_t (&redk)[kCandThreads / 64];
+    uint64_t* redk;  // a wave's
     int& held;
 };
-template <int V>
+template <int V, int T>
 __device__ __forceinline__ void gather_words(const float (&x)[V][4], int v0, float least, const PartWords& sh) {
     int mine = 0;
 #pragma unroll
@@ -884,18 +884,18 @@ __device__ __forceinline__ void gather_words(const float (&x)[V][4], int v0, flo
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (x[j][i] >= least && x[j][i] > -__builtin_inff()) {
-                    if (at < kMostRanked) sh.keys[at] = key_of(x[j][i] + 0.0f, static_cast<uint32_t>(v0 + 1024 * j + i));
+                    if (at < kMostRanked) sh.keys[at] = key_of(x[j][i] + 0.0f, static_cast<uint32_t>(v0 + 4 * T * j + i));
                     ++at;
                 }
     }
 }
-template <int V>
+template <int V, int T>
 __device__ __forceinline__ void rank_words(const float (&x)[V][4], int v0, int n_out, float2* best, const PartWords& sh) {
-    constexpr int kWavesHere = kCandThreads / 64;
+    constexpr int kWavesHere = T / 64;
     const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
     const int n = sh.held;
     if (n <= kMostRanked) {
-        for (int i = tid; i < n; i += kCandThreads) {
+        for (int i = tid; i < n; i += T) {
             const uint64_t k = sh.keys[i];
             int rank = 0;
 #pragma unroll 8
@@ -904,7 +904,7 @@ __device__ __forceinline__ void rank_words(const float (&x)[V][4], int v0, int n
                 best[rank] = make_float2(unordered(static_cast<uint32_t>(k >> 32)),
                                          __builtin_bit_cast(float, ~static_cast<uint32_t>(k)));
         }
-        for (int i = n + tid; i < n_out; i += kCandThreads) best[i] = make_float2(-__builtin_inff(), 0.0f);
+        for (int i = n + tid; i < n_out; i += T) best[i] = make_float2(-__builtin_inff(), 0.0f);
         return;
     }
     uint64_t last = ~uint64_t{0};
@@ -914,7 +914,7 @@ __device__ __forceinline__ void rank_words(const float (&x)[V][4], int v0, int n
         for (int j = 0; j < V; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint64_t o = key_of(x[j][i] + 0.0f, static_cast<uint32_t>(v0 + 1024 * j + i));
+                const uint64_t o = key_of(x[j][i] + 0.0f, static_cast<uint32_t>(v0 + 4 * T * j + i));
                 if (x[j][i] > -__builtin_inff() && o < last && o > k) k = o;
             }
         k = wave_max_u64(k);
@@ -989,7 +989,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
     l = wave_sum_f64(l);
     if (lane == 0) sums[wv] = l;
     const float least = nth_largest(maxima, p.n_out, lane);
-    gather_words(x, v0, least, sh);
+    gather_words<V, kCandThreads>(x, v0, least, sh);
     __syncthreads();
     const size_t part = static_cast<size_t>(b) * p.n_chunks + c;
     float2* best = p.best + part * p.n_out;
@@ -999,7 +999,7 @@ __global__ __launch_bounds__(kCandThreads) void select_parts_kernel(SelectParams
         for (int w = 1; w < kWavesHere; ++w) s += sums[w];
         p.ml[part] = make_double2(m, s);
     }
-    rank_words(x, v0, p.n_out, best, sh);
+    rank_words<V, kCandThreads>(x, v0, p.n_out, best, sh);
 }
 
 // The order of equal scores: the lower beam, then the larger logit (64 bits may not
@@ -1205,25 +1205,25 @@ __device__ __forceinline__ float exp_of(float d) {
     return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502f, d * 1.92596299e-8f));
 }
 
-template <int V>
-__global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobParams p) {
+template <int V, int T>
+__global__ __launch_bounds__(T) void logprob_parts_kernel(LogprobParams p) {
     typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));
-    constexpr int kWavesHere = kCandThreads / 64;
-    __shared__ __align__(16) float maxima[kGroups];
+    constexpr int kWavesHere = T / 64;
+    __shared__ __align__(16) float maxima[T];
     __shared__ double sums[kWavesHere][2];
     __shared__ uint64_t keys[kMostRanked];
-    __shared__ uint64_t redk[kCandThreads / 64];
+    __shared__ uint64_t redk[kWavesHere];
     __shared__ int held;
     const PartWords sh{keys, redk, held};
     __shared__ float2 tops[kMaxTopWords];
     const size_t b = blockIdx.x / p.n_chunks;
     const int c = blockIdx.x % p.n_chunks, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-    const int v0 = c * 1024 * V + 4 * tid;  // this thread's words: v0 + 1024 j + i
+    const int v0 = c * 4 * T * V + 4 * tid;  // this thread's words: v0 + 4 T j + i
     const float* row = p.logits + b * p.vocab;
     float x[V][4], most = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-        const int at = v0 + 1024 * j;
+        const int at = v0 + 4 * T * j;
         if (at + 4 <= p.vocab) {
             const float4a4 w = *reinterpret_cast<const float4a4*>(row + at);
 #pragma unroll
@@ -1242,7 +1242,9 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
     if (tid == 0) sh.held = 0;
     __syncthreads();
     float m;
-    {
+    if constexpr (T == 64) {
+        m = wave_max(most);
+    } else {
         const float4 w = reinterpret_cast<const float4*>(maxima)[lane];
         m = wave_max(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)));
     }
@@ -1271,13 +1273,15 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
     }
     // (up to 32 of 64 groups of threads: 64 rows of 151936, 20 best, 22.8 -> 21.6 us)
     float least;
-    if (p.n_top > 32) {
+    if constexpr (T == 64) {
+        least = nth_of_wave(most, p.n_top);
+    } else if (p.n_top > 32) {
         least = nth_largest(maxima, p.n_top, lane);
     } else {
         const float4 w = reinterpret_cast<const float4*>(maxima)[lane];
         least = nth_of_wave(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), p.n_top);
     }
-    gather_words(x, v0, least, sh);
+    gather_words<V, T>(x, v0, least, sh);
     __syncthreads();
     const size_t part = blockIdx.x;
     const bool whole = p.n_chunks == 1;
@@ -1298,7 +1302,7 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
             p.sums[3 * part + 2] = t;
         }
     }
-    rank_words(x, v0, p.n_top, whole ? tops : p.best + part * p.n_top, sh);
+    rank_words<V, T>(x, v0, p.n_top, whole ? tops : p.best + part * p.n_top, sh);
     if (!whole) return;
     __syncthreads();
     if (tid < p.n_top) finish_top(p, b, r, tid, tops[tid]);
@@ -1308,9 +1312,10 @@ __global__ __launch_bounds__(kCandThreads) void logprob_parts_kernel(LogprobPara
 // only where it is passed by 8 (an exponential of up to e^8 does not hurt), so that a
 // part may be a row of any length and takes few registers.
 constexpr int kStreamVectors = 8;  // float4 in flight
-__global__ __launch_bounds__(kCandThreads) void logprob_stream_kernel(LogprobParams p, int32_t words) {
+template <int T>
+__global__ __launch_bounds__(T) void logprob_stream_kernel(LogprobParams p, int32_t words) {
     typedef float float4a4 __attribute__((ext_vector_type(4), aligned(4)));
-    constexpr int kWavesHere = kCandThreads / 64;
+    constexpr int kWavesHere = T / 64;
     __shared__ double sums[kWavesHere][3];
     const size_t b = blockIdx.x / p.n_chunks;
     const int c = blockIdx.x % p.n_chunks, tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
@@ -1318,11 +1323,11 @@ __global__ __launch_bounds__(kCandThreads) void logprob_stream_kernel(LogprobPar
     const float* row = p.logits + b * p.vocab;
     float m = -__builtin_inff();
     double s = 0.0, t = 0.0;
-    for (int64_t at0 = first + 4 * tid; at0 < end; at0 += 4 * kCandThreads * kStreamVectors) {
+    for (int64_t at0 = first + 4 * tid; at0 < end; at0 += 4 * T * kStreamVectors) {
         float x[kStreamVectors][4], most = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < kStreamVectors; ++j) {
-            const int64_t at = at0 + 4 * kCandThreads * j;
+            const int64_t at = at0 + 4 * T * j;
             if (at + 4 <= end) {
                 const float4a4 w = *reinterpret_cast<const float4a4*>(row + at);
 #pragma unroll
@@ -1371,23 +1376,25 @@ __global__ __launch_bounds__(kCandThreads) void logprob_stream_kernel(LogprobPar
     moved(s, t, m, mw);
     s = wave_sum_f64(s);
     t = wave_sum_f64(t);
-    if (lane == 0) {
+    if (lane == 0 && T > 64) {
         sums[wv][0] = mw;
         sums[wv][1] = s;
         sums[wv][2] = t;
     }
-    __syncthreads();
+    if (T > 64) __syncthreads();
     if (tid) return;
     float M = mw;
 #pragma unroll
     for (int w = 1; w < kWavesHere; ++w) M = fmaxf(M, static_cast<float>(sums[w][0]));
-    s = t = 0.0;
+    if (T > 64) {
+        s = t = 0.0;
 #pragma unroll
-    for (int w = 0; w < kWavesHere; ++w) {
-        double ws = sums[w][1], wt = sums[w][2];
-        moved(ws, wt, static_cast<float>(sums[w][0]), M);
-        s += ws;
-        t += wt;
+        for (int w = 0; w < kWavesHere; ++w) {
+            double ws = sums[w][1], wt = sums[w][2];
+            moved(ws, wt, static_cast<float>(sums[w][0]), M);
+            s += ws;
+            t += wt;
+        }
     }
     if (p.n_chunks == 1) {
         finish_row(p, b, RowSums{M, log(s)}, s, t, logit_of_token(p, b));
@@ -1491,6 +1498,10 @@ __global__ __launch_bounds__(kCandThreads) void logprob_join_kernel(LogprobParam
     }
 }
 
+// Rows of so few words are a wave's (20000 x 300 72 -> 28 us, with 3 alternatives 55 -> 28;
+// 4000 x 1000 22.1 -> 9.3, with 20 16.7 -> 11.0), unless more than 32 of 64 lanes' maxima would
+// make their threshold (64 x 1000, 64 alternatives: 61 us, not 7.7)
+constexpr int32_t kWaveWords = 1024;
 // Words of a part: the most that leave 1024 parts over all rows, up to a row without
 // alternatives, else what leaves four work-groups a CU their registers (20 alternatives, 4096,
 // 8192 and 16384 words: 64 x 151936 22.1, 21.5, 25.4 us; 128 x 151936 32.0, 29.8, 37.9; 2000 x
@@ -1641,11 +1652,13 @@ hipError_t launch_token_logprobs(const float* logits, int32_t n_rows, int32_t vo
     p.out_top_tokens = out_top_tokens;
     p.out_top_logprobs = out_top_logprobs;
     const dim3 grid(static_cast<uint32_t>(parts));
-    const dim3 block(kCandThreads);
-    if (n_top == 0) hipLaunchKernelGGL(logprob_stream_kernel, grid, block, 0, stream, p, words);
-    else if (words == 2048) hipLaunchKernelGGL(logprob_parts_kernel<2>, grid, block, 0, stream, p);
-    else if (words == 4096) hipLaunchKernelGGL(logprob_parts_kernel<4>, grid, block, 0, stream, p);
-    else hipLaunchKernelGGL(logprob_parts_kernel<8>, grid, block, 0, stream, p);
+    const dim3 block(kCandThreads), wave(64);
+    if (n_top == 0 && vocab <= kWaveWords) hipLaunchKernelGGL(logprob_stream_kernel<64>, grid, wave, 0, stream, p, words);
+    else if (n_top == 0) hipLaunchKernelGGL(logprob_stream_kernel<kCandThreads>, grid, block, 0, stream, p, words);
+    else if (vocab <= kWaveWords && n_top <= 32) hipLaunchKernelGGL((logprob_parts_kernel<kWaveWords / 256, 64>), grid, wave, 0, stream, p);
+    else if (words == 2048) hipLaunchKernelGGL((logprob_parts_kernel<2, kCandThreads>), grid, block, 0, stream, p);
+    else if (words == 4096) hipLaunchKernelGGL((logprob_parts_kernel<4, kCandThreads>), grid, block, 0, stream, p);
+    else hipLaunchKernelGGL((logprob_parts_kernel<8, kCandThreads>), grid, block, 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || p.n_chunks == 1) return e;
     hipLaunchKernelGGL(logprob_join_kernel, dim3(n_rows), dim3(kCandThreads), 0, stream, p);

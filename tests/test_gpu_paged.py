@@ -962,7 +962,7 @@ def check_logprobs(torch, x, tokens, n_top, got):
         assert (words[:, k:] == -1).all() and (best[:, k:] == -math.inf).all()
 
 
-@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 5), (2, 300), (1, 2047), (1, 2048), (1, 2049), (5, 4097),
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 2), (3, 5), (2, 300), (3, 1023), (2, 1024), (2, 1025), (5000, 700), (1, 2047), (1, 2048), (1, 2049), (5, 4097),
                                          (1, 50257), (64, 32000), (300, 1000), (700, 16385), (1, 151936), (9, 151936),
                                          (1, 2 ** 22)])
 @pytest.mark.parametrize("n_top", [0, 1, 20, 64])
@@ -974,7 +974,7 @@ def test_logprobs(lib, torch_mod, rows, vocab, n_top):
     check_logprobs(torch, x, tokens, n_top, logprobs(lib, torch, x, tokens, n_top))
 
 
-@pytest.mark.parametrize("rows,vocab", [(1, 7), (4, 3000), (2, 60000), (700, 20000)])
+@pytest.mark.parametrize("rows,vocab", [(1, 7), (3, 900), (4, 3000), (2, 60000), (700, 20000)])
 @pytest.mark.parametrize("kind", ["equal", "masked", "none", "nan", "inf", "steep", "flat", "ties", "lowest"])
 def test_logprobs_of_odd_rows(lib, torch_mod, rows, vocab, kind):
     torch = torch_mod
