@@ -186,18 +186,21 @@ __device__ __forceinline__ SeqRows seq_rows(const PagedArgs& c, int s) {
     return r;
 }
 // The last sequence s with first(s) <= at, by a wave; -1 before the first.  first
-// ascends (where row_start does; otherwise any sequence, or none, is found).
+// ascends (where row_start does; otherwise any sequence, or none, is found).  Sixty-four
+// sequences are looked at at once, then those between two of them (one after the other,
+// 1000 sequences of one row cost the append 101 us).
 template <class F>
 __device__ __forceinline__ int find_seq(int n_seqs, int64_t at, F&& first) {
     const int lane = threadIdx.x & 63;
-    int found = 0;
-    for (int s0 = 0; s0 < n_seqs; s0 += 64) {
-        const int s = s0 + lane;
-        const uint64_t in = __ballot(s < n_seqs && first(min(s, n_seqs - 1)) <= at);
-        found += __builtin_popcountll(in);
-        if (~in) break;
+    int lo = 0;
+    for (int span = n_seqs;;) {
+        const int every = (span + 63) / 64, k = lane * every;
+        const int found = __builtin_popcountll(__ballot(k < span && first(lo + min(k, span - 1)) <= at));
+        if (found == 0) return -1;
+        lo += (found - 1) * every;
+        span = min(every, span - (found - 1) * every);
+        if (every == 1) return lo;
     }
-    return found - 1;
 }
 // Where a key's page stands in the table (the last one's place for keys past it, which are
 // hidden), and its block in the pool, -1 if the page is not there.
@@ -281,6 +284,7 @@ __device__ __forceinline__ float odd_float(double v) {
 struct AppendParams {
     AppendArgs a;
     int64_t kv_groups;    // work-groups of the cache's blocks
+    bool by_rows;         // a slot a row
     int32_t head_groups;  // of a row's queries
 };
 
@@ -291,7 +295,8 @@ struct AppendParams {
 // 128, 106 MB: 28 us, 3.8 TB/s).  A work-group takes the new tokens of one block
 // of K or of V: 16 tokens, HD / 8 threads each.  Nobody else touches the block, so
 // its old tokens are moved to a larger scale on the way, without atomics.  Sequence
-// s has the blocks from slot row_start[s] / 16 + 2 s on: as many as it can touch.
+// s has the blocks from slot row_start[s] / 16 + 2 s on, or from row_start[s] on where those are
+// fewer in all (decode steps): as many as it can touch.
 // The other work-groups take 16 heads of a query row each.
 template <int HD>
 __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
@@ -349,7 +354,10 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
     }
     const int which = blockIdx.x & 1, hk = (blockIdx.x >> 1) % c.n_kv;
     const int64_t slot = (blockIdx.x >> 1) / c.n_kv;
-    auto first_slot = [&](int i) { return static_cast<int64_t>(clamp_row(c, c.row_start[i]) >> 4) + 2 * i; };
+    auto first_slot = [&](int i) {
+        const int32_t r = clamp_row(c, c.row_start[i]);
+        return p.by_rows ? static_cast<int64_t>(r) : static_cast<int64_t>(r >> 4) + 2 * i;
+    };
     const int s = find_seq(c.n_seqs, slot, first_slot);
     if (s < 0) return;
     const SeqRows r = seq_rows(c, s);
@@ -585,8 +593,26 @@ __device__ __forceinline__ int wave_prefix(int v) {
 template <int R, bool BY_TILE>
 __device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit& u) {
     const int lane = threadIdx.x & 63;
+    constexpr int kAll = 1 << 26;  // (more steps than there can be)
+    if (!BY_TILE && !p.split && p.c.n_seqs > 64) {
+        // tiles have places from row_start[s] group / R + s on: as many as there can be
+        auto first = [&](int s) { return static_cast<int64_t>(clamp_row(p.c, p.c.row_start[s])) * p.group / R + s; };
+        const int s = find_seq(p.c.n_seqs, index, first);
+        if (s < 0) return false;
+        const SeqWork w = seq_work<R>(p, s);
+        const int64_t tile = index - first(s);
+        if (tile < 0 || tile >= w.tiles) return false;
+        u.seq = s;
+        u.tile = static_cast<int>(tile);
+        u.part = 0;
+        u.n_parts = 1;
+        u.per = kAll;
+        u.first = index;
+        u.r = w.r;
+        return true;
+    }
     SeqWork w = seq_work<R>(p, lane);
-    int per = 1 << 26;  // (more steps than there can be)
+    int per = kAll;
     if (p.split) {
         float total = 0.0f;  // (of 24 bits: it only sets the split)
         int most = 0;
@@ -1409,8 +1435,10 @@ hipError_t launch_rope_rows(const float* rows, int32_t n_rows, int32_t row_strid
 }
 
 hipError_t launch_kv_append_paged(const AppendArgs& a, hipStream_t stream) {
-    AppendParams p{a, 0, (a.n_heads + 15) / 16};
-    p.kv_groups = (static_cast<int64_t>(a.c.n_rows / kKvBlock) + 2 * a.c.n_seqs) * a.c.n_kv * 2;
+    AppendParams p{a, 0, false, (a.n_heads + 15) / 16};
+    const int64_t by_blocks = static_cast<int64_t>(a.c.n_rows / kKvBlock) + 2 * a.c.n_seqs;
+    p.by_rows = a.c.n_rows < by_blocks;
+    p.kv_groups = std::min<int64_t>(a.c.n_rows, by_blocks) * a.c.n_kv * 2;
     const int64_t groups = p.kv_groups + (a.q ? static_cast<int64_t>(a.c.n_rows) * p.head_groups : 0);
     if (groups > 0x7fffffff) return hipErrorInvalidValue;
     const dim3 grid(static_cast<uint32_t>(groups));

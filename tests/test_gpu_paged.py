@@ -852,7 +852,7 @@ def test_calls_on_another_stream(lib, torch_mod):
         lib.gncx_hip_set_stream(None)
 
 
-@pytest.mark.parametrize("seqs,most", [(65, 90), (300, 40), (2100, 0)])
+@pytest.mark.parametrize("seqs,most", [(65, 90), (300, 40), (2100, 0), (4200, 0)])
 @pytest.mark.parametrize("new", [1, 3])
 def test_many_sequences(lib, torch_mod, seqs, most, new):
     """More sequences than a wave has lanes, some without rows; 2100 without a split."""
