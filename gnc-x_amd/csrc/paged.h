@@ -964,15 +964,18 @@ __device__ __forceinline__ float* row_of(float* base, const PagedParams& p, cons
 // 538 MB in 106 us (5.1 TB/s; the same loads alone take as long); one of 60001 tokens, 4 KV
 // heads, 62 MB in 16 us, of which 3 are the start and the last wave's end; one of 1000 tokens
 // 7.5 us of latencies: sequence, page, codes, products, parts.
-template <int HD>
+// With ALONE, where they are many and short (nothing is split), each wave has 16 rows of its
+// own, all steps of them: no wave is without keys.
+template <int HD, bool ALONE>
 __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_kernel(PagedParams p) {
-    constexpr int R = 16, kSlices = HD / 64, kDims = HD / 16;
+    constexpr int R = 16, kSlices = HD / 64, kDims = HD / 16, kEvery = ALONE ? 1 : kAttnWaves;
     // the waves' parts of a row (a row of HD + 4 floats: no two rows on the same banks)
-    __shared__ __align__(16) float os[kAttnWaves][R][HD + 4];
-    __shared__ float2 mls[kAttnWaves][R];
+    __shared__ __align__(16) float os[ALONE ? 1 : kAttnWaves][R][HD + 4];
+    __shared__ float2 mls[ALONE ? 1 : kAttnWaves][R];
     const PagedArgs& c = p.c;
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % c.n_kv, unit = blockIdx.x / c.n_kv;
+    const uint32_t place = ALONE ? kAttnWaves * blockIdx.x + wv : blockIdx.x;
+    const int hk = place % c.n_kv, unit = place / c.n_kv;
     Unit u;
     if (!find_unit<R, false>(p, unit, u)) return;
     const int rows = u.r.count * p.group, row_lo = u.tile * R, row_hi = min(row_lo + R, rows);
@@ -981,7 +984,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     const int first = w.low_first / 64, steps = w.pos_last / 64 + 1 - first;
     const int step0 = first + u.begin(u.part, steps), step1 = first + u.begin(u.part + 1, steps);
     const int32_t* table = c.pages + static_cast<size_t>(u.seq) * c.max_pages;
-    int step = step0 + wv;
+    int step = ALONE ? step0 : step0 + wv;
     // keys of a step that this lane's blocks begin at: of K, whose rows it loads, and of V
     const int at_k = 16 * (n >> 2), at_v = 16 * g;
     int32_t page_k = page_at(c, table, 64 * step + at_k), page_v = page_at(c, table, 64 * step + at_v);
@@ -1014,12 +1017,12 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     // first block is read, from the caches.
     int64_t bv = block_in(c, page_v, hk, 64 * step + at_v);
     load_k(block_in(c, page_k, hk, 64 * step + at_k));
-    page_k = page_at(c, table, 64 * (step + kAttnWaves) + at_k);
-    page_v = page_at(c, table, 64 * (step + kAttnWaves) + at_v);
+    page_k = page_at(c, table, 64 * (step + kEvery) + at_k);
+    page_v = page_at(c, table, 64 * (step + kEvery) + at_v);
     in_order();
     load_v(bv);
-    for (; step < step1; step += kAttnWaves) {
-        const int32_t k0 = 64 * step, next = step + kAttnWaves;
+    for (; step < step1; step += kEvery) {
+        const int32_t k0 = 64 * step, next = step + kEvery;
         f32x4 s[1][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -1033,8 +1036,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
         const bool more = next < step1;
         const int64_t next_k = more ? block_in(c, page_k, hk, 64 * next + at_k) : 0;
         bv = more ? block_in(c, page_v, hk, 64 * next + at_v) : 0;
-        page_k = page_at(c, table, 64 * (next + kAttnWaves) + at_k);
-        page_v = page_at(c, table, 64 * (next + kAttnWaves) + at_v);
+        page_k = page_at(c, table, 64 * (next + kEvery) + at_k);
+        page_v = page_at(c, table, 64 * (next + kEvery) + at_v);
         load_k(next_k);
         float units;
         if (!one_unit(there, scale.y, unit_exp, units)) break;
@@ -1057,9 +1060,16 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
         // (otherwise the compiler joins these loads with those before the loop, at its top)
         asm volatile("; the next step's values are on their way" ::: "memory");
     }
-    if (step < step1) hard_steps<HD, 1>(p, table, hk, w, st, unit_exp, step, kAttnWaves, step1);
+    if (step < step1) hard_steps<HD, 1>(p, table, hk, w, st, unit_exp, step, kEvery, step1);
     // divided by the sum here, before the parts' weights meet the values
     const float2 ls = sum_and_share(st[0].l, unit_exp);
+    if constexpr (ALONE) {
+        if (row_lo + n >= row_hi) return;
+        float* to = row_of(p.out, p, u.r, hk, row_lo + n, HD);
+#pragma unroll
+        for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(to + 16 * d + 4 * g) = st[0].o[d] * ls.y;
+        return;
+    }
     if (g == 0) mls[wv][n] = make_float2(st[0].m, ls.x);
 #pragma unroll
     for (int d = 0; d < kDims; ++d) *reinterpret_cast<f32x4*>(&os[wv][n][16 * d + 4 * g]) = st[0].o[d] * ls.y;
@@ -1355,7 +1365,7 @@ __global__ __launch_bounds__(kAttnThreads) void paged_merge_kernel(PagedParams p
 // work-groups as the chip holds, whatever tiles they end in, were slower: 64 sequences of 100
 // to 8000 113 us for 112, one of 60001 26.5 for 21.1, the four prompts below 283 for 255.)
 struct PagedPlan {
-    bool keys, split;
+    bool keys, split, alone;
     int32_t rows, target;
     int64_t tiles, units;  // at most
 };
@@ -1385,6 +1395,9 @@ PagedPlan paged_plan(const PagedAttnArgs& a) {
         pl.split = steps > kLeastSteps && whole < 2048;
         pl.target = 768;
     }
+    // (8 KV heads of 128, by four waves and alone: 1000 sequences of 20 to 100 tokens 126, 55 us,
+    // 300 of 500 73, 74, of 2000 226, 265)
+    pl.alone = pl.keys && whole >= 2048 && steps <= 8;
     // units = sum over tiles of ceil(steps / per) <= target / n_kv + tiles (and one for the
     // device's rounding of per, which takes less than a part in 10^6 of it)
     pl.units = pl.tiles + (pl.split ? pl.target / a.c.n_kv + 2 : 0);
@@ -1396,7 +1409,9 @@ hipError_t paged_attention(PagedParams& p, const PagedPlan& pl, hipStream_t stre
     if (pl.units * p.c.n_kv > 0x7fffffff) return hipErrorInvalidValue;
     const dim3 grid(static_cast<uint32_t>(pl.units * p.c.n_kv));
     constexpr int kOwn = HD == 256 ? 1 : 2;
-    if (pl.keys) hipLaunchKernelGGL(paged_keys_kernel<HD>, grid, dim3(kAttnThreads), 0, stream, p);
+    const dim3 fourth((grid.x + kAttnWaves - 1) / kAttnWaves);
+    if (pl.alone) hipLaunchKernelGGL((paged_keys_kernel<HD, true>), fourth, dim3(kAttnThreads), 0, stream, p);
+    else if (pl.keys) hipLaunchKernelGGL((paged_keys_kernel<HD, false>), grid, dim3(kAttnThreads), 0, stream, p);
     else hipLaunchKernelGGL((paged_rows_kernel<HD, kOwn>), grid, dim3(kAttnThreads), 0, stream, p);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !pl.split) return e;

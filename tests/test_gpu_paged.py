@@ -864,6 +864,37 @@ def test_many_sequences(lib, torch_mod, seqs, most, new):
     p.check_attention()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new,sw,bad", [(1, 0, False), (3, 40, False), (2, 0, True)])
+def test_many_short_sequences(lib, torch_mod, hd, new, sw, bad):
+    """More than 2048 (sequence, KV head) pairs of few steps: a wave each; with NaN codes in
+    held tokens of some sequences, which only those meet."""
+    torch = torch_mod
+    rng = np.random.default_rng(hd)
+    held = rng.integers(0, 400, 300).tolist()
+    p = Paged(torch, held, [0 if i % 9 == 4 else new for i in range(300)], H=16, KV=8, hd=hd, page=32, seed=35)
+    p.append(lib)
+    if bad:
+        for s in range(0, 300, 50):
+            if held[s]:
+                p.v[int(p.table[s, 0]), 3, 0, 5, 0] = 0x7f
+    p.attend(lib, sw)
+    if bad:
+        seen = torch.zeros_like(p.out, dtype=torch.bool).view(-1, 16, hd)
+        for s in range(0, 300, 50):
+            if held[s]:
+                seen[int(p.starts[s]):int(p.starts[s + 1]), 6:8, 5] = True
+        rows = int(p.starts[-1])
+        assert torch.equal(p.out.view(-1, 16, hd)[:rows].isnan(), seen[:rows])
+        p.out.nan_to_num_(nan=0.0)
+        for s in range(0, 300, 50):
+            if held[s]:
+                p.v[int(p.table[s, 0]), 3, 0, 5, 0] = 0
+                p.out.view(-1, 16, hd)[int(p.starts[s]):int(p.starts[s + 1]), 6:8, 5] = math.nan
+        p.held = [-1 if s % 50 == 0 else a for s, a in enumerate(held)]  # (checked above)
+    p.check_attention(sw=sw)
+
+
 @pytest.mark.parametrize("sw", [1, 70, 300, 2 ** 31 - 1])
 @pytest.mark.parametrize("H,KV,hd", [(8, 2, 128), (3, 1, 64), (6, 2, 256)])
 def test_windows_of_long_prompts(lib, torch_mod, sw, H, KV, hd):
