@@ -374,16 +374,9 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
     const int row = r.row0 + base - r.len + tok;
     const size_t head = (static_cast<size_t>(row) * c.n_kv + hk) * HD;
     uint8_t* codes = (which ? c.v_pages : c.k_pages) + static_cast<size_t>(block) * (kKvBlock * HD);
-    // old codes: of K the thread's own eight, of V eight tokens of a float
-    uint32_t old0 = 0, old1 = 0;
-    if (which) {
-        const uint2 w = reinterpret_cast<const uint2*>(codes)[tid];
-        old0 = w.x;
-        old1 = w.y;
-    } else if (tok < held) {
-        old0 = *reinterpret_cast<const uint32_t*>(codes + tok * HD + at.off_a);
-        old1 = *reinterpret_cast<const uint32_t*>(codes + tok * HD + at.off_b);
-    }
+    // old codes of V: eight tokens of a float (those of K are read where they move)
+    uint2 old = make_uint2(0, 0);
+    if (which) old = reinterpret_cast<const uint2*>(codes)[tid];
     float x[4] = {}, y[4] = {};
     if (is_new) {
         if (which) {
@@ -445,8 +438,8 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
             w1 = inter ? four_codes(x[2], y[2], x[3], y[3]) : four_codes(y[0], y[1], y[2], y[3]);
         } else {
             if (!moves || tok >= held) return;
-            w0 = moved_codes(old0, f);
-            w1 = moved_codes(old1, f);
+            w0 = moved_codes(*reinterpret_cast<const uint32_t*>(codes + tok * HD + at.off_a), f);
+            w1 = moved_codes(*reinterpret_cast<const uint32_t*>(codes + tok * HD + at.off_b), f);
         }
         *reinterpret_cast<uint32_t*>(codes + tok * HD + at.off_a) = w0;
         *reinterpret_cast<uint32_t*>(codes + tok * HD + at.off_b) = w1;
@@ -463,18 +456,18 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
     __syncthreads();
     const uint2 fresh = reinterpret_cast<const uint2*>(vt)[tid];
     // of bytes t0 .. t0 + 3: those below `held` moved, those in [held, end) new, the others as they are
-    auto mixed = [&](uint32_t old, uint32_t now, int t0) {
+    auto mixed = [&](uint32_t was_w, uint32_t now, int t0) {
         auto below = [&](int n) {  // bytes of tokens below n
             const int k = min(max(n - t0, 0), 4);
             return k == 4 ? 0xffffffffu : (1u << 8 * k) - 1u;
         };
         const uint32_t kept = below(held), all = below(end);
-        const uint32_t m = moves ? moved_codes(old, f) : old;
-        return (m & kept) | (now & all & ~kept) | (old & ~all);
+        const uint32_t m = moves ? moved_codes(was_w, f) : was_w;
+        return (m & kept) | (now & all & ~kept) | (was_w & ~all);
     };
     const int t0 = tid % 2 * 8;
     if (t0 < end && (moves || t0 + 8 > held))
-        reinterpret_cast<uint2*>(codes)[tid] = make_uint2(mixed(old0, fresh.x, t0), mixed(old1, fresh.y, t0 + 4));
+        reinterpret_cast<uint2*>(codes)[tid] = make_uint2(mixed(old.x, fresh.x, t0), mixed(old.y, fresh.y, t0 + 4));
 }
 
 // ---- attention ----------------------------------------------------------------------
