@@ -291,7 +291,7 @@ struct AppendParams {
 // scale = max(old, 2^e), e the least with amax <= 448 2^e over the new values; codes are
 // x / scale rounded to e4m3, old ones times old / scale again.  Blocks and queries in one
 // launch: few rows are bound by it and by two dependent reads (one row 4.6 us, 64 rows of 64
-// sequences 8.0), many by memory and the 64-bit rotation of K (1752 rows of 32 heads on 8 of
+// sequences 8.0), many by memory and the 64-bit rotation of K (2462 rows of 32 heads on 8 of
 // 128, 106 MB: 28 us, 3.8 TB/s).  A work-group takes the new tokens of one block
 // of K or of V: 16 tokens, HD / 8 threads each.  Nobody else touches the block, so
 // its old tokens are moved to a larger scale on the way, without atomics.  Sequence
@@ -388,7 +388,7 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
     }
     if (!which) {
         // K in 64 bits up to its codes, so that they are the formula's (in 32 one in a million
-        // is rounded to the other side; 1752 rows, 32 heads on 8 of 128: 27.5 us for 26.2)
+        // is rounded to the other side; 2462 rows, 32 heads on 8 of 128: 27.5 us for 26.2)
         double dx[4], dy[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
