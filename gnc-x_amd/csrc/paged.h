@@ -1032,8 +1032,6 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
         page_k = page_at(c, table, 64 * (next + kEvery) + at_k);
         page_v = page_at(c, table, 64 * (next + kEvery) + at_v);
         load_k(next_k);
-        float units;
-        if (!one_unit(there, scale.y, unit_exp, units)) break;
         // values that no row sees may hold anything
         u32x4 seen_bytes = four(~0u, ~0u, ~0u, ~0u);
         if (!full) {
@@ -1047,6 +1045,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
             }
             if (__any(bad != 0)) break;
         }
+        float units;  // (raised last: the outputs follow in this step, or not at all)
+        if (!one_unit(there, scale.y, unit_exp, units)) break;
         take_step<HD, 1>(st, s, w.fac, scale, there, full, seen, unit_exp, units,
                          [&](int d) { return vw[d] & seen_bytes; });
         load_v(bv);
