@@ -13,6 +13,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "gncx_device.h"
 #include "gncx_launch.h"
@@ -524,7 +525,8 @@ struct PagedParams {
     int32_t target;   // work-groups that a split aims at
     bool split;       // whether keys are split
     int32_t units;    // that there is place for
-    float scale;      // attn_scale log2(e)
+    float scale;      // |attn_scale| log2(e), 1 for 0
+    float sign;       // attn_scale's, 0 for 0
 };
 constexpr int kMostParts = 128;  // of a row
 constexpr int kLeastSteps = 4;   // of a part
@@ -674,11 +676,11 @@ __device__ __forceinline__ bool find_unit(const PagedParams& p, int index, Unit&
 }
 
 // Rows of queries as the products take them: lane (n, g) has floats 64 i + 16 g + 0 .. 15
-// of row n, as the keys' lanes do.  The scale's sign goes into them, so that fac, the
-// factor of their products, is positive and keeps the scores' order.
+// of row n, as the keys' lanes do, in units of 2^exp.  The scale's sign goes into them, so
+// that the factor of their products is positive and keeps the scores' order.
 template <int HD>
-__device__ __forceinline__ void split_queries(const float* q, int g, float scale, f16x8 (&qh)[HD / 32],
-                                              f16x8 (&ql)[HD / 32], float& fac) {
+__device__ __forceinline__ void split_queries(const float* q, int g, float sign, f16x8 (&qh)[HD / 32],
+                                              f16x8 (&ql)[HD / 32], int& exp) {
     f32x4 v[HD / 64][4];
     float most = 0.0f;
 #pragma unroll
@@ -693,8 +695,7 @@ __device__ __forceinline__ void split_queries(const float* q, int g, float scale
     int e = 0;
     (void)frexpf(most, &e);
     e = most > 0.0f && most < kInf ? e - 14 : 0;
-    fac = ldexpf(scale == 0.0f ? 1.0f : fabsf(scale), e);
-    const float sign = scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
+    exp = e;
 #pragma unroll
     for (int i = 0; i < HD / 64; ++i)
 #pragma unroll
@@ -786,7 +787,7 @@ __device__ __forceinline__ uint32_t seen_bits(int32_t at, int32_t pos, int32_t s
 template <int HD, int RT>
 struct WaveRows {
     f16x8 qh[RT][HD / 32], ql[RT][HD / 32];
-    float fac[RT];
+    int exp[RT];  // of its queries' units
     int32_t pos[RT];
     int32_t pos_first, pos_last, low_first, low_last;  // of its rows; the first keys that they see
     __device__ __forceinline__ void look(const PagedParams& p, const SeqRows& r, int row_lo, int row_hi) {
@@ -817,6 +818,14 @@ __device__ __forceinline__ u32x4 only_seen(u32x4 x, uint32_t seen) {
     return four(x.x & bytes_of(seen, 0), x.y & bytes_of(seen, 4), x.z & bytes_of(seen, 8), x.w & bytes_of(seen, 12));
 }
 __device__ __forceinline__ int scale_exponent(float scale) { return static_cast<int>(as_bits(scale) >> 23 & 0xffu) - 127; }
+// What a product of a row in units of 2^row_exp and a block of keys counts as a score.  From
+// the exponents' sum, as either's float alone may be subnormal where both make an ordinary
+// number; and never 0, by which a hidden key's -inf would be NaN, or infinite, by which a
+// product of 0 would.
+__device__ __forceinline__ float score_factor(float scale, int row_exp, bool there, float key_scale) {
+    const float f = ldexpf(scale, row_exp + (there ? scale_exponent(key_scale) : 0));
+    return fminf(fmaxf(f, 0x1p-126f), 0x1.fffffep127f);
+}
 
 // Whether the blocks' value scales allow one unit for all: a scale of more than 16 below
 // the unit would leave bits of its weights behind in fp16.  Raises the unit; `units` is
@@ -832,15 +841,14 @@ __device__ __forceinline__ bool one_unit(bool there, float scale, int& unit, flo
 // A step of RT row tiles, from their products with the keys on: sc are the scales of this
 // lane's block, if it is there, and values(d) the codes of its float 16 d + n.
 template <int HD, int RT, class Values>
-__device__ __forceinline__ void take_step(PagedRow<HD> (&st)[RT], f32x4 (&s)[RT][4], const float (&fac)[RT], float2 sc,
-                                          bool there, bool full, const uint32_t (&seen)[RT], int unit, float units,
-                                          Values&& values) {
+__device__ __forceinline__ void take_step(PagedRow<HD> (&st)[RT], f32x4 (&s)[RT][4], float scale, const int (&exp)[RT],
+                                          float2 sc, bool there, bool full, const uint32_t (&seen)[RT], int unit,
+                                          float units, Values&& values) {
     f16x8 hi[RT][2], lo[RT][2];
-    const float kf = there ? sc.x : 1.0f;
     const int up = there ? scale_exponent(sc.y) - unit + 14 : 0;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float f = fac[rt] * kf, use = st[rt].raise(s[rt], f, seen[rt], full, units);
+        const float f = score_factor(scale, exp[rt], there, sc.x), use = st[rt].raise(s[rt], f, seen[rt], full, units);
         __builtin_amdgcn_sched_barrier(0);
         st[rt].l += ldexpf(weigh(s[rt], f, use - static_cast<float>(up), hi[rt], lo[rt]), -up);
         __builtin_amdgcn_sched_barrier(0);
@@ -880,7 +888,7 @@ __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* 
         const bool there = bv >= 0 && w.meets(at_v);
         const bool full = w.whole(k0) && __ballot(there) == ~uint64_t{0};
         const int own = scale_exponent(sc.y), top = max(unit, most_of_groups(there ? own : kNoUnit));
-        const float units = ldexpf(1.0f, max(unit - top, -200)), kf = there ? sc.x : 1.0f;
+        const float units = ldexpf(1.0f, max(unit - top, -200));
         unit = top;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -893,7 +901,7 @@ __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* 
                     w.score(s[j], *reinterpret_cast<const u32x4*>(kp + 4 * j * HD + 64 * i), i, rt);
             }
             const uint32_t seen = there ? seen_bits(at_v, w.pos[rt], p.sw) : 0u;
-            const float f = w.fac[rt] * kf, use = st[rt].raise(s, f, seen, full, units);
+            const float f = score_factor(p.scale, w.exp[rt], there, sc.x), use = st[rt].raise(s, f, seen, full, units);
             bool left = there;
             auto pass = [&](int t, auto&& add) {  // the blocks with scales within 16 below 2^t, in units of 2^(t - 14)
                 const bool now = left && own >= t - 16;
@@ -983,7 +991,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     int32_t page_k = page_at(c, table, 64 * step + at_k), page_v = page_at(c, table, 64 * step + at_v);
     const int row = min(row_lo + n, rows - 1);
     w.pos[0] = u.r.len + row / p.group;
-    split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, w.qh[0], w.ql[0], w.fac[0]);
+    split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.sign, w.qh[0], w.ql[0], w.exp[0]);
     PagedRow<HD> st[1];
     int unit_exp = kNoUnit;
     // (a block that is not there: the first one is read, and hidden)
@@ -1047,7 +1055,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
         }
         float units;  // (raised last: the outputs follow in this step, or not at all)
         if (!one_unit(there, scale.y, unit_exp, units)) break;
-        take_step<HD, 1>(st, s, w.fac, scale, there, full, seen, unit_exp, units,
+        take_step<HD, 1>(st, s, p.scale, w.exp, scale, there, full, seen, unit_exp, units,
                          [&](int d) { return vw[d] & seen_bytes; });
         load_v(bv);
         // (otherwise the compiler joins these loads with those before the loop, at its top)
@@ -1173,7 +1181,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
     for (int rt = 0; rt < RT; ++rt) {
         const int row = min(row_lo + 16 * rt + n, rows - 1);
         w.pos[rt] = u.r.len + row / p.group;
-        split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.scale, w.qh[rt], w.ql[rt], w.fac[rt]);
+        split_queries<HD>(row_of(const_cast<float*>(p.q), p, u.r, hk, row, HD), g, p.sign, w.qh[rt], w.ql[rt], w.exp[rt]);
 #pragma unroll
         for (int k = 0; k < 2 * kSlices; ++k) qlow[2 * kSlices * rt + k][tid] = w.ql[rt][k];
     }
@@ -1235,7 +1243,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
                 uint32_t seen[RT];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) seen[rt] = there ? seen_bits(at_v, w.pos[rt], p.sw) : 0u;
-                take_step<HD, RT>(st, s, w.fac, sc, there, full, seen, unit_exp, units, [&](int d) { return values[16 * d]; });
+                take_step<HD, RT>(st, s, p.scale, w.exp, sc, there, full, seen, unit_exp, units,
+                                  [&](int d) { return values[16 * d]; });
             }
         }
         __builtin_amdgcn_s_setprio(0);
@@ -1476,7 +1485,8 @@ hipError_t launch_attention_paged(const PagedAttnArgs& a, void* workspace, size_
     p.target = pl.target;
     p.split = pl.split;
     p.units = static_cast<int32_t>(std::min<int64_t>(pl.units, INT32_MAX));
-    p.scale = a.scale * 1.44269504088896341f;
+    p.scale = a.scale == 0.0f ? 1.0f : std::fabs(a.scale) * 1.44269504088896341f;
+    p.sign = a.scale < 0.0f ? -1.0f : a.scale == 0.0f ? 0.0f : 1.0f;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + static_cast<size_t>(pl.units) * a.c.n_kv * pl.rows * a.c.head_dim);
     if (a.c.head_dim == 64) return paged_attention<64>(p, pl, stream);
