@@ -744,16 +744,16 @@ __device__ __forceinline__ void add_values(f32x4& o, f16x8 a, f16x8 b, const f16
     o = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, hi[0], o, 0, 0, 0);
     o = __builtin_amdgcn_mfma_f32_16x16x32_f16(b, hi[1], o, 0, 0, 0);
 }
-// Weights 2^(f s - use) of this lane's 16 keys as fp16 pairs; returns their sum.  Two a
+// Weights w(product) of this lane's 16 keys as fp16 pairs; returns their sum.  Two a
 // conversion, and the rest as one mixed fma that reads its half in place (written out, as
 // the compiler converts every half back, alone).
-__device__ __forceinline__ float weigh(const f32x4 (&s)[4], float f, float use, f16x8 (&hi)[2], f16x8 (&lo)[2]) {
+template <class Weight>
+__device__ __forceinline__ float weigh(const f32x4 (&s)[4], f16x8 (&hi)[2], f16x8 (&lo)[2], Weight&& w) {
     float sum = 0.0f;
     uint32_t h[8], r[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(s[j / 2][2 * j % 4], f, -use));
-        const float y = __builtin_amdgcn_exp2f(fmaf(s[j / 2][2 * j % 4 + 1], f, -use));
+        const float x = w(s[j / 2][2 * j % 4]), y = w(s[j / 2][2 * j % 4 + 1]);
         sum += x + y;
         h[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{x, y}, f16x2));
         float a, b;
@@ -838,21 +838,35 @@ __device__ __forceinline__ bool one_unit(bool there, float scale, int& unit, flo
     unit = top;
     return true;
 }
+// Maxima up to which a weight is 2^(f s - (use - up)) in one fma: use - up is exact, and f s,
+// not rounded there, at most 1/4 above use, which is.  (From 2^24 on use - up would be rounded
+// by 1 and more, and equal scores of two blocks weigh differently; from 2^25 on f s may lie so
+// far above use that a weight is infinite in fp16, and later so far below that all are 0.)
+constexpr float kMostOneFma = 0x1p22f;
 // A step of RT row tiles, from their products with the keys on: sc are the scales of this
-// lane's block, if it is there, and values(d) the codes of its float 16 d + n.
+// lane's block, if it is there, and values(d) the codes of its float 16 d + n.  False if a
+// maximum is larger than that: then nothing but maxima, sums and outputs in their units is
+// changed, so that the step can be taken again.
 template <int HD, int RT, class Values>
-__device__ __forceinline__ void take_step(PagedRow<HD> (&st)[RT], f32x4 (&s)[RT][4], float scale, const int (&exp)[RT],
+__device__ __forceinline__ bool take_step(PagedRow<HD> (&st)[RT], f32x4 (&s)[RT][4], float scale, const int (&exp)[RT],
                                           float2 sc, bool there, bool full, const uint32_t (&seen)[RT], int unit,
                                           float units, Values&& values) {
     f16x8 hi[RT][2], lo[RT][2];
     const int up = there ? scale_exponent(sc.y) - unit + 14 : 0;
+    float sum[RT];
+    bool large = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float f = score_factor(scale, exp[rt], there, sc.x), use = st[rt].raise(s[rt], f, seen[rt], full, units);
         __builtin_amdgcn_sched_barrier(0);
-        st[rt].l += ldexpf(weigh(s[rt], f, use - static_cast<float>(up), hi[rt], lo[rt]), -up);
+        large = large || fabsf(use) > kMostOneFma;
+        const float base = use - static_cast<float>(up);
+        sum[rt] = weigh(s[rt], hi[rt], lo[rt], [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, f, -base)); });
         __builtin_amdgcn_sched_barrier(0);
     }
+    if (__any(large)) return false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) st[rt].l += ldexpf(sum[rt], -up);
     if (RT > 1) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
     for (int d = 0; d < HD / 16; ++d) {
@@ -866,16 +880,24 @@ __device__ __forceinline__ void take_step(PagedRow<HD> (&st)[RT], f32x4 (&s)[RT]
                 st[rt].o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h & 1 ? b : a, h < 2 ? lo[rt][h] : hi[rt][h - 2],
                                                                      st[rt].o[d], 0, 0, 0);
     }
+    return true;
 }
-
-// The same for every step, from `step` on, one after the other: for those whose values'
-// scales are far apart (the blocks of a range of scales at a time, in a unit of their own),
-// and those not seen whole with NaN codes among the values: rows that do not see one must
-// not meet it (0 NaN is NaN), so NaN codes are taken out and met by a product of their own.
-// (Inside the loops of the others this would cost them 60 registers.)
-template <int HD, int RT>
-__device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* table, int hk, const WaveRows<HD, RT>& w,
-                                           PagedRow<HD> (&st)[RT], int& unit, int step, int every, int end) {
+// The distance of a score of any size to its row's maximum: f s is rounded before that is
+// taken off, so that the largest's is 0 and equal scores' are equal
+__device__ __forceinline__ float below_most(float s, float f, float use) {
+#pragma clang fp contract(off)
+    const float score = s * f;
+    return score - use;
+}
+// The same of one row tile for every step, from `step` on, one after the other: for those with
+// large scores, those whose values' scales are far apart (the blocks of a range of scales at a
+// time, in a unit of their own), and those not seen whole with NaN codes among the values: rows
+// that do not see one must not meet it (0 NaN is NaN), so NaN codes are taken out and met by a
+// product of their own.  (Inside the loops of the others this would cost them 60 registers, and
+// here two row tiles at once spilled: four prompts 248 us, not 236.)
+template <int HD>
+__device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* table, int hk, const WaveRows<HD, 1>& w,
+                                           PagedRow<HD>& st, int& unit, int step, int every, int end) {
     const PagedArgs& c = p.c;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
     for (; step < end; step += every) {
@@ -890,63 +912,64 @@ __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* 
         const int own = scale_exponent(sc.y), top = max(unit, most_of_groups(there ? own : kNoUnit));
         const float units = ldexpf(1.0f, max(unit - top, -200));
         unit = top;
+        f32x4 s[4];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            f32x4 s[4];
+        for (int j = 0; j < 4; ++j) {
+            s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int i = 0; i < HD / 64; ++i)
-                    w.score(s[j], *reinterpret_cast<const u32x4*>(kp + 4 * j * HD + 64 * i), i, rt);
-            }
-            const uint32_t seen = there ? seen_bits(at_v, w.pos[rt], p.sw) : 0u;
-            const float f = score_factor(p.scale, w.exp[rt], there, sc.x), use = st[rt].raise(s, f, seen, full, units);
-            bool left = there;
-            auto pass = [&](int t, auto&& add) {  // the blocks with scales within 16 below 2^t, in units of 2^(t - 14)
-                const bool now = left && own >= t - 16;
-                left = left && !now;
-                f16x8 hi[2], lo[2];
-                const int up = now ? own - t + 14 : 0;
-                st[rt].l += ldexpf(weigh(s, f, now ? use - static_cast<float>(up) : kInf, hi, lo), -up);
-#pragma unroll
-                for (int d = 0; d < HD / 16; ++d) {
-                    u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
-                    if (!full) x = without_nan(x);
-                    add(d, codes_f16(x.x, x.y), codes_f16(x.z, x.w), hi, lo);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
-            };
-            pass(unit, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
-                add_values(st[rt].o[d], a, b, hi, lo);
-            });
-            while (__any(left)) {
-                const int t = most_of_groups(left ? own : kNoUnit);
-                const float back = ldexpf(1.0f, max(t - unit, -200));
-                pass(t, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
-                    f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
-                    add_values(part, a, b, hi, lo);
-                    st[rt].o[d] += part * back;
-                });
-            }
-            if (full) continue;
-            auto ones = [&](int j) {
-                return ((seen >> j & 1u) ? 0x3c00u : 0u) | ((seen >> (j + 1) & 1u) ? 0x3c000000u : 0u);
-            };
-            const f16x8 first = __builtin_bit_cast(f16x8, four(ones(0), ones(2), ones(4), ones(6)));
-            const f16x8 second = __builtin_bit_cast(f16x8, four(ones(8), ones(10), ones(12), ones(14)));
-            auto marks = [](uint32_t v) { return (nan_bytes(v) >> 7) * 0x38u; };  // (0x38: one)
+            for (int i = 0; i < HD / 64; ++i)
+                w.score(s[j], *reinterpret_cast<const u32x4*>(kp + 4 * j * HD + 64 * i), i, 0);
+        }
+        const uint32_t seen = there ? seen_bits(at_v, w.pos[0], p.sw) : 0u;
+        const float f = score_factor(p.scale, w.exp[0], there, sc.x), use = st.raise(s, f, seen, full, units);
+        bool left = there;
+        auto pass = [&](int t, auto&& add) {  // the blocks with scales within 16 below 2^t, in units of 2^(t - 14)
+            const bool now = left && own >= t - 16;
+            left = left && !now;
+            f16x8 hi[2], lo[2];
+            const int up = now ? own - t + 14 : 0;
+            const float base = now ? use - static_cast<float>(up) : kInf, off = now ? static_cast<float>(up) : -kInf;
+            const float sum = __any(fabsf(use) > kMostOneFma)
+                                  ? weigh(s, hi, lo, [&](float x) { return __builtin_amdgcn_exp2f(below_most(x, f, use) + off); })
+                                  : weigh(s, hi, lo, [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, f, -base)); });
+            st.l += ldexpf(sum, -up);
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) {
-                const u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
-                f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
-                count = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(marks(x.x), marks(x.y)), first, count, 0, 0, 0);
-                count = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(marks(x.z), marks(x.w)), second, count, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (count[r] > 0.0f) st[rt].o[d][r] = __builtin_nanf("");
+                u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
+                if (!full) x = without_nan(x);
+                add(d, codes_f16(x.x, x.y), codes_f16(x.z, x.w), hi, lo);
                 __builtin_amdgcn_sched_barrier(0);
             }
+        };
+        pass(unit, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
+            add_values(st.o[d], a, b, hi, lo);
+        });
+        while (__any(left)) {
+            const int t = most_of_groups(left ? own : kNoUnit);
+            const float back = ldexpf(1.0f, max(t - unit, -200));
+            pass(t, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
+                f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
+                add_values(part, a, b, hi, lo);
+                st.o[d] += part * back;
+            });
+        }
+        if (full) continue;
+        auto ones = [&](int j) {
+            return ((seen >> j & 1u) ? 0x3c00u : 0u) | ((seen >> (j + 1) & 1u) ? 0x3c000000u : 0u);
+        };
+        const f16x8 first = __builtin_bit_cast(f16x8, four(ones(0), ones(2), ones(4), ones(6)));
+        const f16x8 second = __builtin_bit_cast(f16x8, four(ones(8), ones(10), ones(12), ones(14)));
+        auto marks = [](uint32_t v) { return (nan_bytes(v) >> 7) * 0x38u; };  // (0x38: one)
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+            const u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
+            f32x4 count = {0.0f, 0.0f, 0.0f, 0.0f};
+            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(marks(x.x), marks(x.y)), first, count, 0, 0, 0);
+            count = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes_f16(marks(x.z), marks(x.w)), second, count, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (count[r] > 0.0f) st.o[d][r] = __builtin_nanf("");
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 }
@@ -1055,13 +1078,14 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
         }
         float units;  // (raised last: the outputs follow in this step, or not at all)
         if (!one_unit(there, scale.y, unit_exp, units)) break;
-        take_step<HD, 1>(st, s, p.scale, w.exp, scale, there, full, seen, unit_exp, units,
-                         [&](int d) { return vw[d] & seen_bytes; });
+        if (!take_step<HD, 1>(st, s, p.scale, w.exp, scale, there, full, seen, unit_exp, units,
+                              [&](int d) { return vw[d] & seen_bytes; }))
+            break;
         load_v(bv);
         // (otherwise the compiler joins these loads with those before the loop, at its top)
         asm volatile("; the next step's values are on their way" ::: "memory");
     }
-    if (step < step1) hard_steps<HD, 1>(p, table, hk, w, st, unit_exp, step, kEvery, step1);
+    if (step < step1) hard_steps<HD>(p, table, hk, w, st[0], unit_exp, step, kEvery, step1);
     // divided by the sum here, before the parts' weights meet the values
     const float2 ls = sum_and_share(st[0].l, unit_exp);
     if constexpr (ALONE) {
@@ -1243,24 +1267,35 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
                 uint32_t seen[RT];
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) seen[rt] = there ? seen_bits(at_v, w.pos[rt], p.sw) : 0u;
-                take_step<HD, RT>(st, s, p.scale, w.exp, sc, there, full, seen, unit_exp, units,
-                                  [&](int d) { return values[16 * d]; });
+                if (!take_step<HD, RT>(st, s, p.scale, w.exp, sc, there, full, seen, unit_exp, units,
+                                       [&](int d) { return values[16 * d]; }))
+                    hard = step;
             }
         }
         __builtin_amdgcn_s_setprio(0);
         if (more) store_step(cur ^ 1, step + 1);
     }
-    if (hard >= 0) {
+    int unit_of[RT];
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+    for (int rt = 0; rt < RT; ++rt) unit_of[rt] = unit_exp;
+    if (hard >= 0)
 #pragma unroll
-            for (int k = 0; k < 2 * kSlices; ++k) w.ql[rt][k] = qlow[2 * kSlices * rt + k][tid];
-        hard_steps<HD, RT>(p, table, hk, w, st, unit_exp, hard, 1, min(step1, w.pos_last / 64 + 1));
-    }
+        for (int rt = 0; rt < RT; ++rt) {
+            WaveRows<HD, 1> one;
+#pragma unroll
+            for (int k = 0; k < 2 * kSlices; ++k) {
+                one.qh[0][k] = w.qh[rt][k];
+                one.ql[0][k] = qlow[2 * kSlices * rt + k][tid];
+            }
+            one.exp[0] = w.exp[rt];
+            one.pos[0] = w.pos[rt];
+            one.look(p, u.r, row_lo, row_hi);
+            hard_steps<HD>(p, table, hk, one, st[rt], unit_of[rt], hard, 1, min(step1, w.pos_last / 64 + 1));
+        }
     const int own = tile_lo + 16 * RT * wv;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float2 ls = sum_and_share(st[rt].l, unit_exp);
+        const float2 ls = sum_and_share(st[rt].l, unit_of[rt]);
         const int row = own + 16 * rt + n;
         if (row >= rows) continue;
         float* to = row_of(p.out, p, u.r, hk, row, HD);
