@@ -828,13 +828,14 @@ __device__ __forceinline__ float score_factor(float scale, int row_exp, bool the
 }
 
 // Whether the blocks' value scales allow one unit for all: a scale of more than 16 below
-// the unit would leave bits of its weights behind in fp16.  Raises the unit; `units` is
-// what outputs are to be multiplied by.
+// the unit would leave bits of its weights behind in fp16, and one of more than 16 above it
+// those of weights that are small by now.  Raises the unit; `units` is what outputs are to
+// be multiplied by.
 __device__ __forceinline__ bool one_unit(bool there, float scale, int& unit, float& units) {
     const int own = scale_exponent(scale);
     const int top = max(unit, most_of_groups(there ? own : kNoUnit));
-    if (-most_of_groups(there ? -own : kNoUnit) < top - 16) return false;
-    units = unit == top ? 1.0f : ldexpf(1.0f, max(unit - top, -200));
+    if (-most_of_groups(there ? -own : kNoUnit) < top - 16 || (unit != kNoUnit && top > unit + 16)) return false;
+    units = ldexpf(1.0f, max(unit - top, -200));
     unit = top;
     return true;
 }
@@ -890,16 +891,22 @@ __device__ __forceinline__ float below_most(float s, float f, float use) {
     return score - use;
 }
 // The same of one row tile for every step, from `step` on, one after the other: for those with
-// large scores, those whose values' scales are far apart (the blocks of a range of scales at a
-// time, in a unit of their own), and those not seen whole with NaN codes among the values: rows
-// that do not see one must not meet it (0 NaN is NaN), so NaN codes are taken out and met by a
-// product of their own.  (Inside the loops of the others this would cost them 60 registers, and
-// here two row tiles at once spilled: four prompts 248 us, not 236.)
+// large scores, those not seen whole with NaN codes among the values, and those whose values'
+// scales are far apart.  Rows that do not see a NaN code must not meet it (0 NaN is NaN), so
+// these are taken out and met by a product of their own.  From the first step with scales far
+// apart on, outputs are in one unit that holds a sum of the largest values as of the smallest,
+// and blocks are taken by their scales, 2^16 at a time, with weights by the row's maximum
+// among them: what a block adds has its own 22 bits, whatever others hold and weigh.
+// (Inside the loops of the others this would cost them 60 registers, and here two row tiles
+// at once spilled: four prompts 248 us, not 236.)
 template <int HD>
 __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* table, int hk, const WaveRows<HD, 1>& w,
                                            PagedRow<HD>& st, int& unit, int step, int every, int end) {
     const PagedArgs& c = p.c;
     const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+    // 448 2^120 of every key, by 2^(far - 14), is below 2^127
+    const int far = 48 - __builtin_clz(w.pos_last + 1);
+    bool wide = false;
     for (; step < end; step += every) {
         const int32_t k0 = 64 * step, at_k = k0 + 16 * (n >> 2), at_v = k0 + 16 * g;
         const int64_t bk = block_in(c, page_at(c, table, at_k), hk, at_k);
@@ -909,9 +916,13 @@ __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* 
         const float2 sc = *reinterpret_cast<const float2*>(c.scales + 2 * max(bv, int64_t{0}));
         const bool there = bv >= 0 && w.meets(at_v);
         const bool full = w.whole(k0) && __ballot(there) == ~uint64_t{0};
-        const int own = scale_exponent(sc.y), top = max(unit, most_of_groups(there ? own : kNoUnit));
-        const float units = ldexpf(1.0f, max(unit - top, -200));
-        unit = top;
+        const int own = scale_exponent(sc.y);
+        float units = 1.0f;
+        if (!wide && !one_unit(there, sc.y, unit, units)) {
+            wide = true;
+            if (unit != kNoUnit) units = ldexpf(1.0f, unit - far);
+            unit = far;
+        }
         f32x4 s[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -922,36 +933,45 @@ __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* 
         }
         const uint32_t seen = there ? seen_bits(at_v, w.pos[0], p.sw) : 0u;
         const float f = score_factor(p.scale, w.exp[0], there, sc.x), use = st.raise(s, f, seen, full, units);
-        bool left = there;
-        auto pass = [&](int t, auto&& add) {  // the blocks with scales within 16 below 2^t, in units of 2^(t - 14)
-            const bool now = left && own >= t - 16;
-            left = left && !now;
-            f16x8 hi[2], lo[2];
-            const int up = now ? own - t + 14 : 0;
-            const float base = now ? use - static_cast<float>(up) : kInf, off = now ? static_cast<float>(up) : -kInf;
+        f16x8 hi[2], lo[2];
+        auto values = [&](int d, auto&& add) {
+            u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
+            if (!full) x = without_nan(x);
+            add(codes_f16(x.x, x.y), codes_f16(x.z, x.w));
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        if (!wide) {
+            const int up = there ? own - unit + 14 : 0;
+            const float off = static_cast<float>(up), base = use - off;
             const float sum = __any(fabsf(use) > kMostOneFma)
                                   ? weigh(s, hi, lo, [&](float x) { return __builtin_amdgcn_exp2f(below_most(x, f, use) + off); })
                                   : weigh(s, hi, lo, [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, f, -base)); });
             st.l += ldexpf(sum, -up);
 #pragma unroll
-            for (int d = 0; d < HD / 16; ++d) {
-                u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
-                if (!full) x = without_nan(x);
-                add(d, codes_f16(x.x, x.y), codes_f16(x.z, x.w), hi, lo);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        pass(unit, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
-            add_values(st.o[d], a, b, hi, lo);
-        });
-        while (__any(left)) {
+            for (int d = 0; d < HD / 16; ++d)
+                values(d, [&](f16x8 a, f16x8 b) { add_values(st.o[d], a, b, hi, lo); });
+        }
+        for (bool left = wide && there; __any(left);) {
             const int t = most_of_groups(left ? own : kNoUnit);
-            const float back = ldexpf(1.0f, max(t - unit, -200));
-            pass(t, [&](int d, f16x8 a, f16x8 b, const f16x8(&hi)[2], const f16x8(&lo)[2]) {
-                f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
-                add_values(part, a, b, hi, lo);
-                st.o[d] += part * back;
-            });
+            const bool now = left && own >= t - 16;
+            left = left && !now;
+            float most = -kInf;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) most = fmaxf(most, s[j / 4][j % 4]);
+            most = ceilf(xor_max(now ? most * f : -kInf));
+            // (a row that sees none of these blocks: nothing is added)
+            const float base = most == -kInf ? 0.0f : most, off = now ? static_cast<float>(own - t + 14) : -kInf;
+            const int down = static_cast<int>(fmaxf(most - use, -1000.0f));
+            const float sum = weigh(s, hi, lo, [&](float x) { return __builtin_amdgcn_exp2f(below_most(x, f, base) + off); });
+            st.l += ldexpf(sum, down + (now ? t - own - 14 : 0));
+#pragma unroll
+            for (int d = 0; d < HD / 16; ++d)
+                values(d, [&](f16x8 a, f16x8 b) {
+                    f32x4 part = {0.0f, 0.0f, 0.0f, 0.0f};
+                    add_values(part, a, b, hi, lo);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) st.o[d][r] += ldexpf(part[r], down + t - far);
+                });
         }
         if (full) continue;
         auto ones = [&](int j) {

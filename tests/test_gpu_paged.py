@@ -1266,6 +1266,239 @@ def test_equal_large_scores_weigh_the_same(lib, torch_mod, e, new):
     assert ((p.out.view(new, 2, 64).double() - want).abs() <= 2.0 ** -20 * size).all()
 
 
+def check_around_nan(lib, p, places, sw=0):
+    """Attention with NaN codes at places (sequence, position, KV head, float) among the
+    values: NaN in that float of the rows that see it, everything else against 64 bits."""
+    torch, G = p.torch, p.H // p.KV
+    bad = torch.zeros(p.out.shape[0], p.H, p.hd, dtype=torch.bool, device="cuda")
+    codes = []
+    for s, t, b, d in places:
+        codes.append((int(p.table[s, t // p.page]), b, t % p.page // BLOCK, d, t % BLOCK))
+        r0, a = int(p.starts[s]), p.held[s]
+        last = min(p.new[s], t + sw - a) if sw else p.new[s]
+        bad[r0 + max(t - a, 0):r0 + last, b * G:(b + 1) * G, d] = True
+    for at in codes:
+        p.v[at] = 0x7f
+    p.attend(lib, sw)
+    got = p.out.clone()
+    assert torch.equal(got.isnan().view(bad.shape), bad)
+    for at in codes:
+        p.v[at] = 0
+    p.attend(lib, sw)
+    p.check_attention(out=torch.where(bad.view(got.shape), p.out, got), sw=sw)
+
+
+def grow_values(p, s, t, e):
+    """The values of the block of sequence s's position t times 2^e."""
+    p.scales[int(p.table[s, t // p.page]), :, t % p.page // BLOCK, 1] *= 2.0 ** e
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("held,new,sw", [([600, 30], [1, 1], 0), ([600, 620], [3, 3], 0), ([610], [3], 500),
+                                         ([1000, 20], [90, 70], 0)])
+def test_nan_values_in_a_step_whose_scale_grows(lib, torch_mod, hd, held, new, sw):
+    """A NaN code among the values of the last, partial step, whose scale is above those of
+    the wave's steps before: other floats, and rows that do not see it, are as without it."""
+    p = Paged(torch_mod, held, new, H=4, KV=2, hd=hd, page=32, seed=70)
+    p.append(lib)
+    ends = [a + n - 1 for a, n in zip(held, new)]
+    for s, t in enumerate(ends):
+        grow_values(p, s, t, 3)
+    check_around_nan(lib, p, [(s, t, 1, 5 + s) for s, t in enumerate(ends)], sw)
+
+
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 3])
+def test_nan_values_of_many_short_sequences_whose_scales_grow(lib, torch_mod, hd, new):
+    """The same where each sequence and KV head is a wave's."""
+    held = np.random.default_rng(hd).integers(100, 400, 300).tolist()
+    p = Paged(torch_mod, held, [new] * 300, H=16, KV=8, hd=hd, page=32, seed=71)
+    p.append(lib)
+    places = [(s, held[s] + new - 1, s % 8, s % hd) for s in range(0, 300, 7)]
+    for s, t, _, _ in places:
+        grow_values(p, s, t, 3)
+    check_around_nan(lib, p, places)
+
+
+# held, new, H, KV: decode rows, prompts, and a wave for each sequence and KV head
+FORMS = [([100, 700], [1, 1], 4, 2), ([600], [70], 4, 2), ([70 + 2 * i for i in range(130)], [1] * 130, 16, 16)]
+
+
+@pytest.mark.parametrize("held,new,H,KV", FORMS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_of_very_small_and_very_large_factors(lib, torch_mod, held, new, H, KV, hd):
+    """Queries near the least float, beside keys of zeros, of ordinary size and near the
+    largest; a tiny scale of the scores."""
+    torch = torch_mod
+    p = Paged(torch, held, new, H=H, KV=KV, hd=hd, page=16, seed=74)
+    p.append(lib)
+    q, scales = p.q.clone(), p.scales.clone()
+    for big in (1.0, 1e-10, 1e-20, 1e-38):
+        p.q = big * q
+        p.attend(lib)
+        p.check_attention()
+    # products that are ordinary numbers: 2^-125 2^125
+    p.q = q * 2.0 ** -125
+    p.scales[..., 0] *= 2.0 ** 125
+    p.attend(lib)
+    p.check_attention()
+    p.scales.copy_(scales)
+    # keys of zeros: the first two blocks' and every third one's
+    for s, (a, n) in enumerate(zip(held, new)):
+        for t in range(0, a + n, BLOCK):
+            if t < 2 * BLOCK or t // BLOCK % 3 == 0:
+                p.k[int(p.table[s, t // 16])] = 0
+                p.scales[int(p.table[s, t // 16]), ..., 0] = 2.0 ** -100
+    for big in (1.0, 1e-10, 1e-20, 1e-38):
+        p.q = big * q
+        p.attend(lib)
+        p.check_attention()
+    p.q, p.scale = q, 1e-30
+    p.attend(lib)
+    p.check_attention()
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_attention_of_large_queries_and_keys_that_do_not_meet(lib, torch_mod, new):
+    """Queries with one large float, keys that are zero there and large elsewhere: every
+    score is zero, and the output the mean of the values."""
+    torch = torch_mod
+    p = Paged(torch, [200], [new], H=4, KV=2, hd=64, page=16, seed=75)
+    p.append(lib)
+    p.k[..., 7] = 0
+    p.scales[..., 0] *= 2.0 ** 90
+    p.q.zero_().view(new, 4, 64)[..., 7] = 2.0 ** 100
+    p.attend(lib)
+    _, v, _ = p.tokens(0, 200 + new)
+    v = v.repeat_interleave(2, 1)
+    for i in range(new):
+        x = v[:201 + i]
+        assert ((p.out.view(new, 4, 64)[i] - x.mean(0)).abs() <= 2.0 ** -20 * x.abs().mean(0)).all()
+
+
+@pytest.mark.parametrize("e", [22, 24, 25, 27, 31, 60])
+@pytest.mark.parametrize("held,new,H,KV", FORMS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_attention_of_large_scores(lib, torch_mod, e, held, new, H, KV, hd):
+    """Queries of 2^e: where one key's score is above all others by more than both may be off
+    (check_attention's ds) and 30, it has all the weight, and the output is its value."""
+    torch = torch_mod
+    p = Paged(torch, held, new, H=H, KV=KV, hd=hd, seed=72)
+    p.append(lib)
+    p.q *= 2.0 ** e
+    p.attend(lib)
+    assert p.out.isfinite().all()
+    rows = clear = 0
+    for s in range(0, len(held), 1 + len(held) // 40):
+        a, n, r0 = held[s], new[s], int(p.starts[s])
+        k, v, _ = p.tokens(s, a + n)
+        hidden = torch.arange(a + n, device="cuda")[None, :] > torch.arange(a, a + n, device="cuda")[:, None]
+        for h in range(H):
+            q = p.q[r0:r0 + n].view(n, H, hd)[:, h].double().contiguous()
+            kh, vh = k[:, h // (H // KV)].contiguous(), v[:, h // (H // KV)].contiguous()
+            sc = (q @ kh.t().contiguous() * p.scale).masked_fill(hidden, -math.inf)
+            size = (q.abs() @ kh.abs().t().contiguous() * p.scale).amax(1)
+            far = kh.abs().sum(1).amax() * p.scale
+            ds = (2.0 ** -21 + 8 * math.sqrt(hd) * U) * size + 2.0 ** -36 * q.abs().amax(1) * far
+            top = sc.topk(2, dim=1)
+            lead = top.values[:, 0] - top.values[:, 1] > 2 * ds + 30
+            want = vh[top.indices[:, 0]]
+            off = (p.out[r0:r0 + n].view(n, H, hd)[:, h].double() - want).abs()
+            assert (off <= 2.0 ** -20 * want.abs())[lead].all()
+            rows, clear = rows + n, clear + int(lead.sum())
+    assert 2 * clear > rows
+
+
+@pytest.mark.parametrize("e", range(18, 32))
+@pytest.mark.parametrize("new", [1, 70])
+def test_equal_large_scores_weigh_the_same(lib, torch_mod, e, new):
+    """Two blocks of the same keys whose values' scales differ by odd powers of two: the
+    query's best keys, one of each, have half the weight each."""
+    torch = torch_mod
+    p = Paged(torch, [200], [new], H=2, KV=2, hd=64, page=16, seed=73)
+    p.append(lib)
+    one, two = int(p.table[0, 3]), int(p.table[0, 8])
+    p.k[two], p.scales[two, ..., 0] = p.k[one], p.scales[one, ..., 0]
+    grow_values(p, 0, 8 * 16, -3)
+    k, v, _ = p.tokens(0, 200)
+    p.q.view(new, 2, 64).copy_(2.0 ** e * k[3 * 16 + 5])  # (its score is |k|^2 2^e / 8, 2^(e + 3), far above the others)
+    p.attend(lib)
+    want = (v[3 * 16 + 5] + v[8 * 16 + 5]) / 2
+    size = (v[3 * 16 + 5].abs() + v[8 * 16 + 5].abs()) / 2
+    assert ((p.out.view(new, 2, 64).double() - want).abs() <= 2.0 ** -20 * size).all()
+
+
+def grow_all_values(p, exponents):
+    """Every held or new block's values times 2^e, e = exponents(sequence, block)."""
+    for s, (a, n) in enumerate(zip(p.held, p.new)):
+        for t in range(0, a + n, BLOCK):
+            grow_values(p, s, t, exponents(s, t // BLOCK))
+
+
+@pytest.mark.parametrize("held,new,H,KV", FORMS)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("sw", [0, 90])
+def test_values_of_scales_far_apart(lib, torch_mod, held, new, H, KV, hd, sw):
+    """Blocks of values more than 2^16 apart, near and far, in any order; blocks of zeros."""
+    torch = torch_mod
+    p = Paged(torch, held, new, H=H, KV=KV, hd=hd, page=16, seed=76)
+    p.append(lib)
+    kept = p.scales.clone()
+    rng = np.random.default_rng(hd)
+    for span in (17, 40, 110):
+        p.scales.copy_(kept)
+        grow_all_values(p, lambda s, b: int(rng.integers(-min(span, 90), span)))
+        p.attend(lib, sw)
+        p.check_attention(sw=sw)
+    for first in (True, False):  # (rising and falling through the sequence)
+        p.scales.copy_(kept)
+        grow_all_values(p, lambda s, b: min(6 * b - 90, 110) if first else max(110 - 6 * b, -90))
+        p.attend(lib, sw)
+        p.check_attention(sw=sw)
+    p.scales.copy_(kept)
+    for s, (a, n) in enumerate(zip(held, new)):
+        for t in range(16 * (s % 3), a + n, 48):
+            p.v[int(p.table[s, t // 16])] = 0
+            p.scales[int(p.table[s, t // 16]), ..., 1] = 2.0 ** -100
+    p.attend(lib, sw)
+    p.check_attention(sw=sw)
+
+
+@pytest.mark.parametrize("held,new,H,KV", FORMS)
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("low", [-30.0, -45.0, -300.0])
+def test_large_values_of_little_weight(lib, torch_mod, held, new, H, KV, hd, low):
+    """Blocks of values of 2^110 whose keys have weights of about e^low, beside blocks of small
+    values: what the large ones leave of the sum, nothing for e^-300, is what counts."""
+    torch = torch_mod
+    p = Paged(torch, held, new, H=H, KV=KV, hd=hd, page=16, seed=77)
+    p.append(lib)
+    p.q.view(-1, H, hd)[..., 3] = 128.0 * math.sqrt(hd)  # (scores are 128 k_3 and an ordinary rest)
+    big, small = {-30.0: (50, 0), -45.0: (80, 0), -300.0: (110, -80)}[low]
+    grow_all_values(p, lambda s, b: big if b % 5 == 2 else small)
+    f8 = torch.float8_e4m3fn
+    k = p.k.view(f8).float()
+    k[..., 3] = 0
+    for s, (a, n) in enumerate(zip(held, new)):
+        for t in range(2 * BLOCK, a + n, 5 * BLOCK):
+            name = int(p.table[s, t // 16])
+            k[name, ..., 3] = low / 128.0 / p.scales[name, :, 0, 0][:, None, None]
+    assert (k[..., 3].nan_to_num() >= -448).all()
+    p.k.copy_(k.to(f8).view(torch.uint8))
+    p.attend(lib)
+    p.check_attention()
+
+
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("held,new", [([600, 620], [3, 3]), ([1000, 20], [90, 70])])
+def test_nan_values_among_scales_far_apart(lib, torch_mod, hd, held, new):
+    p = Paged(torch_mod, held, new, H=4, KV=2, hd=hd, page=16, seed=78)
+    p.append(lib)
+    grow_all_values(p, lambda s, b: (0, 30, -40, 3, 60)[b % 5])
+    places = [(s, a + n - 1, 1, 5) for s, (a, n) in enumerate(zip(held, new))]
+    check_around_nan(lib, p, places + [(0, held[0], 0, 9), (1, held[1] + 1, 0, 40)])
+
+
 # ---- log probabilities ------------------------------------------------------------------
 def logprobs(lib, torch, x, tokens, n_top, entropy=True):
     rows, vocab = x.shape
