@@ -707,6 +707,12 @@ __device__ __forceinline__ void split_queries(const float* q, int g, float sign,
         }
 }
 
+// Maxima up to which a weight is 2^(f s - (use - up)) in one fma: use - up is exact, and f s,
+// not rounded there, at most 1/4 above use, which is.  (From 2^24 on use - up would be rounded
+// by 1 and more, and equal scores of two blocks weigh differently; from 2^25 on f s may lie so
+// far above use that a weight is infinite in fp16, and later so far below that all are 0.)
+constexpr float kMostOneFma = 0x1p22f;
+
 // A row's running maximum, sum (of this lane's keys) and output, in units of 2^(unit - 14).
 template <int HD>
 struct PagedRow {
@@ -718,8 +724,8 @@ struct PagedRow {
     }
     // A step's scores, f s for the `seen` of this lane's 16 keys: the others to -inf, the
     // maximum raised, sum and output rescaled to it (and the output by `units`).  Returns
-    // the maximum to weigh by.
-    __device__ __forceinline__ float raise(f32x4 (&s)[4], float f, uint32_t seen, bool full, float units) {
+    // the maximum to weigh by, and in `large` whether one was raised past kMostOneFma.
+    __device__ __forceinline__ float raise(f32x4 (&s)[4], float f, uint32_t seen, bool full, float units, bool& large) {
         float most = -kInf;
         if (!full)
 #pragma unroll
@@ -731,9 +737,11 @@ struct PagedRow {
         m = mx;
         l *= alpha;
         // (most steps leave every row's maximum as it is)
-        if (__any(by != 1.0f))
+        if (__any(by != 1.0f)) {
 #pragma unroll
             for (int d = 0; d < HD / 16; ++d) o[d] *= by;
+            large = large || __any(fabsf(use) > kMostOneFma);
+        }
         return use;
     }
 };
@@ -839,11 +847,6 @@ __device__ __forceinline__ bool one_unit(bool there, float scale, int& unit, flo
     unit = top;
     return true;
 }
-// Maxima up to which a weight is 2^(f s - (use - up)) in one fma: use - up is exact, and f s,
-// not rounded there, at most 1/4 above use, which is.  (From 2^24 on use - up would be rounded
-// by 1 and more, and equal scores of two blocks weigh differently; from 2^25 on f s may lie so
-// far above use that a weight is infinite in fp16, and later so far below that all are 0.)
-constexpr float kMostOneFma = 0x1p22f;
 // A step of RT row tiles, from their products with the keys on: sc are the scales of this
 // lane's block, if it is there, and values(d) the codes of its float 16 d + n.  False if a
 // maximum is larger than that: then nothing but maxima, sums and outputs in their units is
@@ -858,14 +861,13 @@ __device__ __forceinline__ bool take_step(PagedRow<HD> (&st)[RT], f32x4 (&s)[RT]
     bool large = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const float f = score_factor(scale, exp[rt], there, sc.x), use = st[rt].raise(s[rt], f, seen[rt], full, units);
+        const float f = score_factor(scale, exp[rt], there, sc.x), use = st[rt].raise(s[rt], f, seen[rt], full, units, large);
         __builtin_amdgcn_sched_barrier(0);
-        large = large || fabsf(use) > kMostOneFma;
         const float base = use - static_cast<float>(up);
         sum[rt] = weigh(s[rt], hi[rt], lo[rt], [&](float x) { return __builtin_amdgcn_exp2f(fmaf(x, f, -base)); });
         __builtin_amdgcn_sched_barrier(0);
     }
-    if (__any(large)) return false;
+    if (large) return false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) st[rt].l += ldexpf(sum[rt], -up);
     if (RT > 1) __builtin_amdgcn_s_setprio(1);
@@ -932,7 +934,8 @@ __device__ __forceinline__ void hard_steps(const PagedParams& p, const int32_t* 
                 w.score(s[j], *reinterpret_cast<const u32x4*>(kp + 4 * j * HD + 64 * i), i, 0);
         }
         const uint32_t seen = there ? seen_bits(at_v, w.pos[0], p.sw) : 0u;
-        const float f = score_factor(p.scale, w.exp[0], there, sc.x), use = st.raise(s, f, seen, full, units);
+        bool large = false;
+        const float f = score_factor(p.scale, w.exp[0], there, sc.x), use = st.raise(s, f, seen, full, units, large);
         f16x8 hi[2], lo[2];
         auto values = [&](int d, auto&& add) {
             u32x4 x = *reinterpret_cast<const u32x4*>(vp + 256 * d);
