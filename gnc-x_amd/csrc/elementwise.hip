@@ -1637,32 +1637,43 @@ hipError_t launch_token_logprobs(const float* logits, int32_t n_rows, int32_t vo
         workspace_bytes < token_logprobs_workspace_bytes(n_rows, vocab, n_top))
         return hipErrorInvalidValue;
     const int32_t words = logprob_words(n_rows, vocab, n_top);
-    LogprobParams p{};
-    p.logits = logits;
-    p.tokens = tokens;
-    p.vocab = vocab;
-    p.n_top = n_top;
-    p.n_chunks = (vocab + words - 1) / words;
-    const int64_t parts = static_cast<int64_t>(n_rows) * p.n_chunks;
+    const int32_t n_chunks = (vocab + words - 1) / words;
+    const int64_t parts = static_cast<int64_t>(n_rows) * n_chunks;
     if (parts > 0x7fffffff) return hipErrorInvalidValue;
-    p.sums = static_cast<double*>(workspace);
-    p.best = reinterpret_cast<float2*>(p.sums + 3 * parts);
-    p.out_logprobs = out_logprobs;
-    p.out_entropy = out_entropy;
-    p.out_top_tokens = out_top_tokens;
-    p.out_top_logprobs = out_top_logprobs;
-    const dim3 grid(static_cast<uint32_t>(parts));
-    const dim3 block(kCandThreads), wave(64);
-    if (n_top == 0 && vocab <= kWaveWords) hipLaunchKernelGGL(logprob_stream_kernel<64>, grid, wave, 0, stream, p, words);
-    else if (n_top == 0) hipLaunchKernelGGL(logprob_stream_kernel<kCandThreads>, grid, block, 0, stream, p, words);
-    else if (vocab <= kWaveWords && n_top <= 32) hipLaunchKernelGGL((logprob_parts_kernel<kWaveWords / 256, 64>), grid, wave, 0, stream, p);
-    else if (words == 2048) hipLaunchKernelGGL((logprob_parts_kernel<2, kCandThreads>), grid, block, 0, stream, p);
-    else if (words == 4096) hipLaunchKernelGGL((logprob_parts_kernel<4, kCandThreads>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((logprob_parts_kernel<8, kCandThreads>), grid, block, 0, stream, p);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || p.n_chunks == 1) return e;
-    hipLaunchKernelGGL(logprob_join_kernel, dim3(n_rows), dim3(kCandThreads), 0, stream, p);
-    return hipGetLastError();
+    double* const sums = static_cast<double*>(workspace);
+    float2* const best = reinterpret_cast<float2*>(sums + 3 * parts);
+    // (rows whose parts are one launch's work-groups)
+    const int32_t at_once = std::max(1, (1 << 22) / n_chunks);
+    for (int64_t r0 = 0; r0 < n_rows; r0 += at_once) {
+        const int32_t rows = static_cast<int32_t>(std::min<int64_t>(at_once, n_rows - r0));
+        LogprobParams p{};
+        p.logits = logits + r0 * vocab;
+        p.tokens = tokens ? tokens + r0 : nullptr;
+        p.vocab = vocab;
+        p.n_top = n_top;
+        p.n_chunks = n_chunks;
+        p.sums = sums + 3 * r0 * n_chunks;
+        p.best = best + r0 * n_chunks * n_top;
+        p.out_logprobs = out_logprobs ? out_logprobs + r0 : nullptr;
+        p.out_entropy = out_entropy ? out_entropy + r0 : nullptr;
+        p.out_top_tokens = out_top_tokens ? out_top_tokens + r0 * n_top : nullptr;
+        p.out_top_logprobs = out_top_logprobs ? out_top_logprobs + r0 * n_top : nullptr;
+        const dim3 grid(static_cast<uint32_t>(rows) * n_chunks);
+        const dim3 block(kCandThreads), wave(64);
+        if (n_top == 0 && vocab <= kWaveWords) hipLaunchKernelGGL(logprob_stream_kernel<64>, grid, wave, 0, stream, p, words);
+        else if (n_top == 0) hipLaunchKernelGGL(logprob_stream_kernel<kCandThreads>, grid, block, 0, stream, p, words);
+        else if (vocab <= kWaveWords && n_top <= 32) hipLaunchKernelGGL((logprob_parts_kernel<kWaveWords / 256, 64>), grid, wave, 0, stream, p);
+        else if (words == 2048) hipLaunchKernelGGL((logprob_parts_kernel<2, kCandThreads>), grid, block, 0, stream, p);
+        else if (words == 4096) hipLaunchKernelGGL((logprob_parts_kernel<4, kCandThreads>), grid, block, 0, stream, p);
+        else hipLaunchKernelGGL((logprob_parts_kernel<8, kCandThreads>), grid, block, 0, stream, p);
+        hipError_t e = hipGetLastError();
+        if (e == hipSuccess && n_chunks > 1) {
+            hipLaunchKernelGGL(logprob_join_kernel, dim3(rows), dim3(kCandThreads), 0, stream, p);
+            e = hipGetLastError();
+        }
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace gncx

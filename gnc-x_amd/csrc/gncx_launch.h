@@ -7,6 +7,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstddef>
 #include <cstdint>
 #include <vector>
@@ -211,6 +212,18 @@ hipError_t launch_beam_select(const float* logits, int32_t n_beams, int32_t voca
                               int32_t* out_tokens, float* out_scores, void* workspace, size_t workspace_bytes,
                               hipStream_t stream);
 
+// A launch has fewer than 2^32 threads in x: work-groups of up to 512 in as many launches as
+// it takes, launch(first, grid) each.
+template <class Launch>
+hipError_t by_groups(int64_t groups, Launch&& launch) {
+    constexpr int64_t kAtOnce = int64_t{1} << 22;
+    for (int64_t first = 0; first < groups; first += kAtOnce) {
+        launch(static_cast<uint32_t>(first), dim3(static_cast<uint32_t>(std::min(kAtOnce, groups - first))));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
 // Rotary positions of rows (n_rot even, up to head_dim): see GNCXRotation.
 struct RotationArgs {
     const double* freqs;  // device [n_rot / 2]

@@ -287,6 +287,7 @@ struct AppendParams {
     int64_t kv_groups;    // work-groups of the cache's blocks
     bool by_rows;         // a slot a row
     int32_t head_groups;  // of a row's queries
+    uint32_t first;       // work-group of the launch
 };
 
 // scale = max(old, 2^e), e the least with amax <= 448 2^e over the new values; codes are
@@ -325,8 +326,9 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
             y[j] = gamma ? y[j] * inv * gy[j] : y[j] * inv;
         }
     };
-    if (blockIdx.x >= p.kv_groups) {
-        const int64_t b = blockIdx.x - p.kv_groups;
+    const uint32_t group = p.first + blockIdx.x;
+    if (group >= p.kv_groups) {
+        const int64_t b = group - p.kv_groups;
         const int row = static_cast<int>(b / p.head_groups), h = static_cast<int>(b % p.head_groups) * 16 + tid / kPer;
         const int s = find_seq(c.n_seqs, row, [&](int i) { return clamp_row(c, c.row_start[i]); });
         if (s < 0) return;
@@ -353,8 +355,8 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
         at.store(a.out_q + head, x, y);
         return;
     }
-    const int which = blockIdx.x & 1, hk = (blockIdx.x >> 1) % c.n_kv;
-    const int64_t slot = (blockIdx.x >> 1) / c.n_kv;
+    const int which = group & 1, hk = (group >> 1) % c.n_kv;
+    const int64_t slot = (group >> 1) / c.n_kv;
     auto first_slot = [&](int i) {
         const int32_t r = clamp_row(c, c.row_start[i]);
         return p.by_rows ? static_cast<int64_t>(r) : static_cast<int64_t>(r >> 4) + 2 * i;
@@ -525,6 +527,7 @@ struct PagedParams {
     int32_t target;   // work-groups that a split aims at
     bool split;       // whether keys are split
     int32_t units;    // that there is place for
+    uint32_t first;   // work-group of the launch
     float scale;      // |attn_scale| log2(e), 1 for 0
     float sign;       // attn_scale's, 0 for 0
 };
@@ -1021,7 +1024,7 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
     __shared__ float2 mls[ALONE ? 1 : kAttnWaves][R];
     const PagedArgs& c = p.c;
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const uint32_t place = ALONE ? kAttnWaves * blockIdx.x + wv : blockIdx.x;
+    const uint32_t group = p.first + blockIdx.x, place = ALONE ? kAttnWaves * group + wv : group;
     const int hk = place % c.n_kv, unit = place / c.n_kv;
     Unit u;
     if (!find_unit<R, false>(p, unit, u)) return;
@@ -1167,7 +1170,8 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_rows_ke
     __shared__ __align__(16) f16x8 qlow[RT * 2 * kSlices][kAttnThreads];  // the queries' low halves: they would take the registers that a step needs
     const PagedArgs& c = p.c;
     const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, n = lane & 15, g = lane >> 4;
-    const int hk = blockIdx.x % c.n_kv, unit = blockIdx.x / c.n_kv;
+    const uint32_t place = p.first + blockIdx.x;
+    const int hk = place % c.n_kv, unit = place / c.n_kv;
     Unit u;
     if (!find_unit<R, false>(p, unit, u)) return;
     const int rows = u.r.count * p.group, tile_lo = u.tile * R, tile_hi = min(tile_lo + R, rows);
@@ -1467,13 +1471,14 @@ PagedPlan paged_plan(const PagedAttnArgs& a) {
 template <int HD>
 hipError_t paged_attention(PagedParams& p, const PagedPlan& pl, hipStream_t stream) {
     if (pl.units * p.c.n_kv > 0x7fffffff) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<uint32_t>(pl.units * p.c.n_kv));
     constexpr int kOwn = HD == 256 ? 1 : 2;
-    const dim3 fourth((grid.x + kAttnWaves - 1) / kAttnWaves);
-    if (pl.alone) hipLaunchKernelGGL((paged_keys_kernel<HD, true>), fourth, dim3(kAttnThreads), 0, stream, p);
-    else if (pl.keys) hipLaunchKernelGGL((paged_keys_kernel<HD, false>), grid, dim3(kAttnThreads), 0, stream, p);
-    else hipLaunchKernelGGL((paged_rows_kernel<HD, kOwn>), grid, dim3(kAttnThreads), 0, stream, p);
-    const hipError_t e = hipGetLastError();
+    const int64_t groups = pl.units * p.c.n_kv;
+    const hipError_t e = by_groups(pl.alone ? (groups + kAttnWaves - 1) / kAttnWaves : groups, [&](uint32_t first, dim3 grid) {
+        p.first = first;
+        if (pl.alone) hipLaunchKernelGGL((paged_keys_kernel<HD, true>), grid, dim3(kAttnThreads), 0, stream, p);
+        else if (pl.keys) hipLaunchKernelGGL((paged_keys_kernel<HD, false>), grid, dim3(kAttnThreads), 0, stream, p);
+        else hipLaunchKernelGGL((paged_rows_kernel<HD, kOwn>), grid, dim3(kAttnThreads), 0, stream, p);
+    });
     if (e != hipSuccess || !pl.split) return e;
     // a tile's rows in as many work-groups as make 2048 of them
     const int64_t rows = std::min<int64_t>(pl.rows, static_cast<int64_t>(p.c.n_rows) * p.group), tiles = pl.tiles * p.c.n_kv;
@@ -1502,26 +1507,32 @@ hipError_t launch_rope_rows(const float* rows, int32_t n_rows, int32_t row_strid
     const int32_t most = (n_heads + at_once - 1) / at_once;
     const int32_t groups = std::min(most, std::max(1, (1024 + n_rows - 1) / n_rows));
     p.heads_per_group = (n_heads + groups - 1) / groups;
-    const dim3 grid(n_rows, (n_heads + p.heads_per_group - 1) / p.heads_per_group);
-    if (grid.y > 65535) return hipErrorInvalidValue;
-    if (vec) hipLaunchKernelGGL(rope_rows_kernel<true>, grid, dim3(kRopeThreads), 0, stream, p);
-    else hipLaunchKernelGGL(rope_rows_kernel<false>, grid, dim3(kRopeThreads), 0, stream, p);
-    return hipGetLastError();
+    const uint32_t per_row = (n_heads + p.heads_per_group - 1) / p.heads_per_group;
+    if (per_row > 65535) return hipErrorInvalidValue;
+    return by_groups(n_rows, [&](uint32_t first, dim3 grid) {
+        grid.y = per_row;
+        p.rows = rows + static_cast<size_t>(first) * row_stride;
+        p.out = out + static_cast<size_t>(first) * out_stride;
+        p.positions = positions + first;
+        if (vec) hipLaunchKernelGGL(rope_rows_kernel<true>, grid, dim3(kRopeThreads), 0, stream, p);
+        else hipLaunchKernelGGL(rope_rows_kernel<false>, grid, dim3(kRopeThreads), 0, stream, p);
+    });
 }
 
 hipError_t launch_kv_append_paged(const AppendArgs& a, hipStream_t stream) {
-    AppendParams p{a, 0, false, (a.n_heads + 15) / 16};
+    AppendParams p{a, 0, false, (a.n_heads + 15) / 16, 0};
     const int64_t by_blocks = static_cast<int64_t>(a.c.n_rows / kKvBlock) + 2 * a.c.n_seqs;
     p.by_rows = a.c.n_rows < by_blocks;
     p.kv_groups = std::min<int64_t>(a.c.n_rows, by_blocks) * a.c.n_kv * 2;
     const int64_t groups = p.kv_groups + (a.q ? static_cast<int64_t>(a.c.n_rows) * p.head_groups : 0);
     if (groups > 0x7fffffff) return hipErrorInvalidValue;
-    const dim3 grid(static_cast<uint32_t>(groups));
-    if (a.c.head_dim == 64) hipLaunchKernelGGL(append_kernel<64>, grid, dim3(128), 0, stream, p);
-    else if (a.c.head_dim == 128) hipLaunchKernelGGL(append_kernel<128>, grid, dim3(256), 0, stream, p);
-    else if (a.c.head_dim == 256) hipLaunchKernelGGL(append_kernel<256>, grid, dim3(512), 0, stream, p);
-    else return hipErrorInvalidValue;
-    return hipGetLastError();
+    if (a.c.head_dim != 64 && a.c.head_dim != 128 && a.c.head_dim != 256) return hipErrorInvalidValue;
+    return by_groups(groups, [&](uint32_t first, dim3 grid) {
+        p.first = first;
+        if (a.c.head_dim == 64) hipLaunchKernelGGL(append_kernel<64>, grid, dim3(128), 0, stream, p);
+        else if (a.c.head_dim == 128) hipLaunchKernelGGL(append_kernel<128>, grid, dim3(256), 0, stream, p);
+        else hipLaunchKernelGGL(append_kernel<256>, grid, dim3(512), 0, stream, p);
+    });
 }
 
 size_t attention_paged_workspace_bytes(const PagedAttnArgs& a) {

@@ -1657,6 +1657,90 @@ def test_logprobs_captured(lib, torch_mod):
         lib.gncx_hip_set_stream(None)
 
 
+# ---- more work-groups than a launch has place for (2^32 threads) ---------------------------
+def test_rope_of_2_24_rows(lib, torch_mod):
+    torch, t, rows = torch_mod, Turn(torch_mod, 2), 2 ** 24 + 3
+    x = randn(torch, 1, rows, 2)
+    at = torch.arange(rows, dtype=torch.int32, device="cuda") % 4096
+    out = torch.full_like(x, math.nan)
+    lib.gncx_hip_rope_rows(x.data_ptr(), rows, 2, 1, 2, at.data_ptr(), t.ref(), 2, out.data_ptr())
+    gncx.check(lib)
+    want, tol = t(x.double().view(rows, 1, 2), at)
+    assert ((out.double().view(rows, 1, 2) - want).abs() <= tol).all()
+
+
+def test_append_of_2_25_rows(lib, torch_mod):
+    """One sequence's rows in one call, and in two."""
+    torch, rows, page = torch_mod, 2 ** 25 + 40, 256
+    n_pages = -(-rows // page)
+    q, k, v = (randn(torch, i, rows, 64) for i in range(3))
+    table = torch.arange(n_pages, dtype=torch.int32, device="cuda")
+    turn = Turn(torch, 64)
+
+    def append(parts):
+        codes = [torch.zeros(n_pages * page * 64, dtype=torch.uint8, device="cuda") for _ in range(2)]
+        scales, out = torch.zeros(n_pages * page // 8, device="cuda"), torch.zeros_like(q)
+        cache = gncx.PagedCache(codes[0].data_ptr(), codes[1].data_ptr(), scales.data_ptr(), n_pages, page, 1, 64)
+        first = 0
+        for n in parts:
+            starts, length = whole(torch, [0, n]), whole(torch, [first])
+            batch = gncx.PagedBatch(1, n, n_pages, starts.data_ptr(), length.data_ptr(), table.data_ptr())
+            a = 256 * first
+            lib.gncx_hip_kv_append_paged(C.byref(cache), C.byref(batch), q.data_ptr() + a, k.data_ptr() + a,
+                                         v.data_ptr() + a, 1, None, 0, 0, 0, EPS, turn.ref(), out.data_ptr() + a)
+            gncx.check(lib)
+            first += n
+        torch.cuda.synchronize()
+        return *codes, scales, out
+
+    one, two = append([rows]), append([rows // 3, rows - rows // 3])
+    for a, b in zip(one, two):
+        assert torch.equal(a, b)
+    assert one[3].any(1).all()
+
+
+@pytest.mark.parametrize("max_pages", [1, 40])
+def test_attention_of_2_24_sequences_and_heads(lib, torch_mod, max_pages):
+    """A wave, and a work-group, for each sequence and KV head: both more than 2^24."""
+    torch, S, H, hd = torch_mod, 16500, 1024, 64
+    if max_pages == 1:
+        S = 65536
+    p = Paged(torch, [15], [1], H=H, KV=H, hd=hd, page=16, seed=79)
+    p.append(lib)
+    table = torch.full((S, max_pages), int(p.table[0, 0]), dtype=torch.int32, device="cuda")
+    lengths = torch.arange(S, dtype=torch.int32, device="cuda") % 16
+    starts = torch.arange(S + 1, dtype=torch.int32, device="cuda")
+    q = randn(torch, 80, S, H * hd)
+
+    def attend(parts):
+        out = torch.full((S, H * hd), math.nan, device="cuda")
+        for lo, hi in parts:
+            batch = gncx.PagedBatch(hi - lo, hi - lo, max_pages, starts.data_ptr(), lengths[lo:hi].data_ptr(),
+                                    table.data_ptr())
+            lib.gncx_hip_attention_paged(C.byref(p.cache), C.byref(batch), q[lo:hi].data_ptr(), H, p.scale, 0,
+                                         out[lo:hi].data_ptr())
+            gncx.check(lib)
+        return out
+
+    out = attend([(0, S)])
+    assert out.isfinite().all()
+    assert torch.equal(out, attend([(i, min(i + 7000, S)) for i in range(0, S, 7000)]))
+    # the last sequence
+    p.held, p.new, p.starts = [int(lengths[-1])], [1], np.arange(2, dtype=np.int32)
+    p.check_attention(q=q[-1:], out=out[-1:])
+
+
+@pytest.mark.parametrize("rows,n_top", [(2 ** 26 + 5, 0), (2 ** 26 + 5, 1), (2 ** 24 + 5, 33)])
+def test_logprobs_of_2_26_rows(lib, torch_mod, rows, n_top):
+    torch = torch_mod
+    x = randn(torch, 81, rows, 2)
+    tokens = torch.arange(rows, dtype=torch.int32, device="cuda") % 2
+    got = logprobs(lib, torch, x, tokens, n_top)
+    for i in list(range(0, rows - 2 ** 22, 2 ** 23)) + [rows - 2 ** 22]:
+        n = slice(i, i + 2 ** 22)
+        check_logprobs(torch, x[n], tokens[n], n_top, tuple(t[n] for t in got))
+
+
 # ---- a run of them together: the decode driver --------------------------------------------
 LOGITS = 1e-3  # the bar of this driver's logits between its batched and its one-token calls (relative L2)
 
