@@ -284,7 +284,7 @@ class PagedSequences:
     """The caches of several sequences, of 8-bit blocks in pages: sequence i has
     room for room[i] positions, in pages that are its own and the same in every
     layer's pool.  scaling: the arguments of gncx_hip_rope_frequencies behind the
-    base by name, for contexts longer than the trained one."""
+    base by name, for contexts longer than the trained one (factors: a tensor)."""
 
     def __init__(self, lib, torch, model: Model, room, page: int = 64, scaling: dict | None = None,
                  device: str = "cuda"):
@@ -309,6 +309,9 @@ class PagedSequences:
             raise ValueError("a scaling has " + ", ".join(given))
         given.update(scaling or {})
         factors = given["factors"]
+        if factors is not None and not (factors.dtype == torch.float32 and factors.is_contiguous() and
+                                        factors.numel() == s.head_dim // 2):
+            raise ValueError("factors are head_dim / 2 contiguous 32-bit floats")
         if lib.gncx_hip_rope_frequencies(s.head_dim, s.rope_base, given["scaling"], given["factor"],
                                          given["trained_context"], given["beta_fast"], given["beta_slow"],
                                          None if factors is None else factors.data_ptr(), self.freqs.data_ptr(),

@@ -290,3 +290,18 @@ def test_driver_refusals(plib, monkeypatch):
     for call in (lambda: dec.Decoder.generate_batch(host, [[1]], 1), lambda: dec.Decoder.score(host, [1, 2])):
         with pytest.raises(ValueError, match="device memory"):
             call()
+
+
+def test_sequences_refuse_factors_that_are_not_the_models(plib):
+    """The library reads head_dim / 2 floats where the tensor's memory begins."""
+    import types
+    import torch
+    import gncx_amd.decode as dec
+    model = types.SimpleNamespace(shape=types.SimpleNamespace(n_layers=1, n_kv=1, head_dim=64, rope_base=1e4))
+    make = lambda f: dec.PagedSequences(plib, torch, model, [5], 16, dict(factors=f), "cpu")  # noqa: E731
+    plain = make(None).freqs
+    assert torch.equal(make(torch.full((32,), 2.0)).freqs, plain / 2)
+    for f in (torch.ones(31), torch.ones(64), torch.ones(32, dtype=torch.float64), torch.ones(64)[::2],
+              torch.ones(32, dtype=torch.float16)):
+        with pytest.raises(ValueError, match="factors"):
+            make(f)
