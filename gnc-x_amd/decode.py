@@ -897,11 +897,14 @@ class Decoder:
     def score(self, ids, n_top: int = 0):
         """(log probabilities, entropies, alternatives) of ids[1:], each behind the
         ids before it: in nats, and alternatives[i] the n_top (at most 64) most
-        probable [(token, log probability)] there."""
+        probable [(token, log probability)] there.  One pass of up to 65535 rows,
+        whose keys and values take the KV cache's rows from 0 on."""
         self._device_only("scoring")
         s, m, n = self.s, self.m, len(ids) - 1
-        if n < 1 or n > self.max_seq:
-            raise ValueError("at least two ids, and the KV cache holds all but the last")
+        if not 1 <= n <= min(self.max_seq, 65535):
+            raise ValueError("two to 65536 ids, and the KV cache holds all but the last")
+        if any(not 0 <= int(t) < s.vocab for t in ids):
+            raise ValueError("an id is outside the vocabulary")
         if not 0 <= n_top <= 64:
             raise ValueError("0 to 64 alternatives")
 
@@ -929,12 +932,12 @@ class Decoder:
         caches of the call's own: [(token ids, their log probabilities,
         alternatives)], alternatives[i] the n_top (at most 64) most probable
         [(token, log probability)] where token i was chosen.  A sequence ends behind
-        the token `end` (if not negative).  Prompts go in with up to rows_at_once
-        tokens a pass; `scaling` as in PagedSequences."""
+        the token `end` (if not negative).  Prompts (up to 65535) go in with up to
+        rows_at_once (65535) tokens a pass; `scaling` as in PagedSequences."""
         self._device_only("a batch")
         prompts = [[int(t) for t in p] for p in prompts]
-        if not prompts or not all(prompts) or n_new < 1 or rows_at_once < 1:
-            raise ValueError("prompts of at least one token, and at least one new one")
+        if not 1 <= len(prompts) <= 65535 or not all(prompts) or n_new < 1 or not 1 <= rows_at_once <= 65535:
+            raise ValueError("up to 65535 prompts of at least one token, one new one and up to 65535 rows at once")
         if page not in (16, 32, 64, 128, 256) or not 0 <= n_top <= 64:
             raise ValueError("pages of 16, 32, 64, 128 or 256 positions, 0 to 64 alternatives")
         if any(not 0 <= t < self.s.vocab for p in prompts for t in p):

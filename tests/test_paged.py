@@ -305,3 +305,18 @@ def test_sequences_refuse_factors_that_are_not_the_models(plib):
               torch.ones(32, dtype=torch.float16)):
         with pytest.raises(ValueError, match="factors"):
             make(f)
+
+
+def test_driver_refuses_ids_and_sizes_before_a_pass(plib, monkeypatch):
+    """Ids outside the vocabulary (a pass would leave the decoder's caches without them, and a
+    last one gets -inf), and more rows than the embedding rows' call takes."""
+    import gncx_amd.decode as dec
+    d = Stand(dec, monkeypatch)
+    d.max_seq = 10 ** 6
+    for ids in ([50, 1], [1, 50], [1, -1, 2], [1] * 65537):
+        with pytest.raises(ValueError):
+            dec.Decoder.score(d, ids)
+    for prompts, kw in (([[1]] * 65536, {}), ([[1]], dict(rows_at_once=65536))):
+        with pytest.raises(ValueError):
+            dec.Decoder.generate_batch(d, prompts, 1, **kw)
+    assert not d.passes
