@@ -590,8 +590,9 @@ void gncx_hip_rope_rows(const float* rows, int32_t n_rows, int32_t row_stride, i
  * A block's scale is the least power of two that 448 times reaches every finite
  * value stored to it; where it holds earlier tokens and their scale is smaller,
  * their codes are rounded to the new one (exact but for codes that become
- * subnormal).  Infinities and NaN are stored as NaN.  Rows of one call go to
- * places of their own: no page that is appended to may stand twice in the tables.
+ * subnormal).  Infinities, NaN, and keys that norm or rotation take past the
+ * floats' range are stored as NaN.  Rows of one call go to places of their own:
+ * no page that is appended to may stand twice in the tables.
  * Codes are the nearest to the formula's value in 64 bits, queries are formed in 32.
  * Rows and out_q are 16-byte aligned, norm weights in device memory too.  No two of
  * the arguments' arrays overlap but as said. */
@@ -603,8 +604,8 @@ void gncx_hip_kv_append_paged(const GNCXPagedCache* cache, const GNCXPagedBatch*
  * cache: a row sees its sequence's positions up to its own, which the cache holds
  * already (gncx_hip_kv_append_paged), with sliding_window > 0 the last so many of
  * them; what it does not see has no part in its output, whatever it holds.  A row
- * that sees nothing (its pages are not there) gives zeros.  16-byte aligned;
- * out_rows overlaps nothing. */
+ * that sees nothing (its pages are not there) gives zeros, one with a score above
+ * the floats' range NaN.  16-byte aligned; out_rows overlaps nothing. */
 void gncx_hip_attention_paged(const GNCXPagedCache* cache, const GNCXPagedBatch* batch, const float* q_rows,
                               int32_t n_heads, float attn_scale, int32_t sliding_window, float* out_rows);
 /* For each of n_rows rows of logits [vocab] (1 to 4194304 words):

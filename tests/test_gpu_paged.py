@@ -454,6 +454,22 @@ def test_append_at_the_border_of_a_scale(lib, torch_mod):
         assert (p.scales[int(p.table[s, 0]), :, 0] == want).all()
 
 
+def test_append_of_keys_past_the_floats(lib, torch_mod):
+    """A rotated key above the largest float is stored as NaN, as an infinite one is."""
+    torch = torch_mod
+    p = Paged(torch, [0, 5], [4, 9], H=2, KV=2, hd=64)
+    turn = Turn(torch, 64)
+    p.kr[2, 3] = p.kr[2, 35] = 3e38  # (pair 3 at position 2: (cos - sin, cos + sin) of 0.84)
+    before = state(p)
+    p.append(lib, turn)
+    codes = p.k[int(p.table[0, 0]), 0, 0, 2].view(torch.float8_e4m3fn).float()
+    assert codes.isnan().nonzero().view(-1).tolist() == [35]
+    p.held, p.new, p.starts = [-1, 5], [4, 9], p.starts  # (the other sequence, as ever)
+    p.k[int(p.table[0, 0])], p.v[int(p.table[0, 0])] = before[0][int(p.table[0, 0])], before[1][int(p.table[0, 0])]
+    p.scales[int(p.table[0, 0])] = before[2][int(p.table[0, 0])]
+    check_append(p, before, turn, q=False)
+
+
 def test_append_leaves_rows_and_pages_that_are_not_there(lib, torch_mod):
     """Lengths outside the table, rows past its end, pages outside the pool, rows behind the
     last sequence: nothing of them is touched."""
@@ -1497,6 +1513,26 @@ def test_nan_values_among_scales_far_apart(lib, torch_mod, hd, held, new):
     grow_all_values(p, lambda s, b: (0, 30, -40, 3, 60)[b % 5])
     places = [(s, a + n - 1, 1, 5) for s, (a, n) in enumerate(zip(held, new))]
     check_around_nan(lib, p, places + [(0, held[0], 0, 9), (1, held[1] + 1, 0, 40)])
+
+
+def test_scores_past_the_floats(lib, torch_mod):
+    """A row with a score above the largest float is NaN, others are as ever."""
+    torch = torch_mod
+    p = Paged(torch, [100, 30], [1, 40], H=4, KV=2, hd=64, seed=83)
+    p.append(lib)
+    p.q *= 2.0 ** -20
+    p.scale *= 2.0 ** 20
+    p.attend(lib)
+    want = p.out.clone()
+    p.check_attention()
+    k, _, _ = p.tokens(0, 101)
+    p.q.view(41, 4, 64)[0, 1] = (k[50, 0] * 2.0 ** 120).float()  # (a score of |k|^2 2^137)
+    p.attend(lib)
+    bad = torch.zeros(41, 4, 64, dtype=torch.bool, device="cuda")
+    bad[0, 1] = True
+    bad = bad.view(want.shape)
+    assert torch.equal(p.out.isnan(), bad)
+    assert (p.out - want)[~bad].abs().max() <= 2.0 ** -19 * want[~bad].abs().max()
 
 
 # ---- log probabilities ------------------------------------------------------------------
