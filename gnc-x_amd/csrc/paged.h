@@ -292,8 +292,8 @@ struct AppendParams {
 
 // scale = max(old, 2^e), e the least with amax <= 448 2^e over the new values; codes are
 // x / scale rounded to e4m3, old ones times old / scale again.  Blocks and queries in one
-// launch: few rows are bound by it and by two dependent reads (one row 4.6 us, 64 rows of 64
-// sequences 8.0), many by memory and the 64-bit rotation of K (2462 rows of 32 heads on 8 of
+// launch: few rows are bound by it and by two dependent reads (one row 4.8 us, 64 rows of 64
+// sequences 7.2), many by memory and the 64-bit rotation of K (2462 rows of 32 heads on 8 of
 // 128, 106 MB: 28 us, 3.8 TB/s).  A work-group takes the new tokens of one block
 // of K or of V: 16 tokens, HD / 8 threads each.  Nobody else touches the block, so
 // its old tokens are moved to a larger scale on the way, without atomics.  Sequence
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
 // power of two that takes the row's largest to 2^14), and so do weights, each times its
 // block's value scale over the largest scale so far, `unit` (powers of two).  Scores, sums
 // and outputs are held in 32 bits, maxima rounded up to whole numbers, so that rescaling is
-// exact.
+// exact.  Where that leaves too few bits, or none, hard_steps goes on.
 constexpr int kAttnThreads = 256, kAttnWaves = 4;
 __device__ __forceinline__ u32x4 four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return u32x4{a, b, c, d}; }
 constexpr float kInf = __builtin_inff();
@@ -1157,9 +1157,9 @@ __global__ __launch_bounds__(kAttnThreads, HD == 256 ? 1 : 2) void paged_keys_ke
 }
 
 // Many rows (prompts): a wave has 16 RT rows of its own, a work-group four times as many.
-// Bound by the issue of vector and matrix instructions, which share it (584 of them and 128
+// Bound by the issue of vector and matrix instructions, which share it (586 of them and 128
 // products of two slots each a wave and step): four prompts of 300 to 700 tokens behind 1152
-// to 3799, 32 heads on 8 of 128, 2 x 101 GFLOP in 242 us; in the loop 1060 TFLOP/s, of the
+// to 3799, 32 heads on 8 of 128, 2 x 101 GFLOP in 245 us; in the loop 1050 TFLOP/s, of the
 // 1315 that a large library product reaches; the rest are the parts' starts and ends.
 // (32x32x16 products, half as many instructions: heads of 128 6% slower, of 256 34%, of 64
 // 9% faster.)
@@ -1448,12 +1448,14 @@ PagedPlan paged_plan(const PagedAttnArgs& a) {
     int64_t steps = ((static_cast<int64_t>(a.c.max_pages) << a.c.page_bits) + 63) / 64;
     if (a.sliding_window > 0) steps = std::min(steps, (a.sliding_window + pl.rows / group + 63) / 64 + 1);
     if (pl.keys) {
-        // Without a split a work-group has 0.36 us a step; a split costs 9 us of parts and
-        // merge.  So few steps are left whole, and more where others read meanwhile (8 KV
-        // heads of 128; split, whole; 1 sequence of 400 10.9, 8.4 us, of 1000 10.8, 11.2; 64
-        // of 1000 38, 29, of 100 to 8000 112, 124; 16 of 100 to 8000 39, 61; 200 of 100 to
-        // 2000 115, 96).  Targets of 512 and 1024: 16 of 100 to 8000 38.9, 40.8, 8 of 4000
-        // 19.4, 24.5, 64 of 100 to 8000 120, 112.
+        // A work-group of its own has 0.36 us for a step; parts and their merge take 10.6 for
+        // one sequence.  So few steps are left whole, and more where others read meanwhile (8 KV
+        // heads of 128; split, whole; 1 sequence of 400 10.9, 8.4 us, of 640 10.6, 9.9, of 800
+        // 10.6, 11.3; 64 of 1000 38, 29, of 100 to 8000 112, 124; 16 of 100 to 8000 39, 61; 200
+        // of 100 to 2000 115, 96).  All by the table's width, as the lengths are the device's:
+        // with a table for 8192 tokens one sequence of 400 takes 10.8 and 64 of 1000 38.
+        // Targets of 512 and 1024: 16 of 100 to 8000 38.9, 40.8, 8 of 4000 19.4, 24.5, 64 of 100
+        // to 8000 120, 112.
         pl.split = steps > 10 + whole / 16 && whole < 2048;
         pl.target = whole < 512 ? 512 : 1024;
     } else {
@@ -1464,7 +1466,7 @@ PagedPlan paged_plan(const PagedAttnArgs& a) {
         pl.target = 768;
     }
     // (8 KV heads of 128, by four waves and alone: 1000 sequences of 20 to 100 tokens 126, 55 us,
-    // 300 of 500 73, 74, of 2000 226, 265)
+    // 300 of 500 73, 74, of 2000 226, 265; in tables of more than 512 tokens always the former)
     pl.alone = pl.keys && whole >= 2048 && steps <= 8;
     // units = sum over tiles of ceil(steps / per) <= target / n_kv + tiles (and one for the
     // device's rounding of per, which takes less than a part in 10^6 of it)
