@@ -483,7 +483,9 @@ __global__ __launch_bounds__(2 * HD) void append_kernel(AppendParams p) {
 // power of two that takes the row's largest to 2^14), and so do weights, each times its
 // block's value scale over the largest scale so far, `unit` (powers of two).  Scores, sums
 // and outputs are held in 32 bits, maxima rounded up to whole numbers, so that rescaling is
-// exact.  Where that leaves too few bits, or none, hard_steps goes on.
+// exact.  (A pair's last bit is 2^-24: a weight is kept to 2^-38 of the row's largest, or to
+// 2^-22 where its block's scale is 2^16 below the unit.)  Where the scales are farther apart,
+// and where sizes leave no bits, hard_steps goes on.
 constexpr int kAttnThreads = 256, kAttnWaves = 4;
 __device__ __forceinline__ u32x4 four(uint32_t a, uint32_t b, uint32_t c, uint32_t d) { return u32x4{a, b, c, d}; }
 constexpr float kInf = __builtin_inff();

@@ -605,7 +605,10 @@ void gncx_hip_kv_append_paged(const GNCXPagedCache* cache, const GNCXPagedBatch*
  * already (gncx_hip_kv_append_paged), with sliding_window > 0 the last so many of
  * them; what it does not see has no part in its output, whatever it holds.  A row
  * that sees nothing (its pages are not there) gives zeros, one with a score above
- * the floats' range NaN.  16-byte aligned; out_rows overlaps nothing. */
+ * the floats' range NaN.  Weights are kept to 22 bits and to 2^-38 of the row's
+ * largest (to 2^-22 of it for values whose block's scale is 2^16 below another's,
+ * in proportion between), smaller ones are 0.  16-byte aligned; out_rows overlaps
+ * nothing. */
 void gncx_hip_attention_paged(const GNCXPagedCache* cache, const GNCXPagedBatch* batch, const float* q_rows,
                               int32_t n_heads, float attn_scale, int32_t sliding_window, float* out_rows);
 /* For each of n_rows rows of logits [vocab] (1 to 4194304 words):
